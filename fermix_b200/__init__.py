@@ -3,7 +3,9 @@ complex128) on NVIDIA B200, with singular-safe gradients -- a drop-in for the pu
 of ChenAo-Phys/fermix (src/fermix/__init__.py:1-10) on torch CUDA tensors, computed by
 hand-written sm_100a kernels behind a C ABI (include/fermix_b200.h).
 
-Public functions: :func:`slogdet`, :func:`slogpf`, :func:`det`, :func:`pf`.
+Public functions: :func:`slogdet`, :func:`slogpf`, :func:`det`, :func:`pf`; and, for the
+network whose orbitals they take, :func:`biased_attention`, :func:`position_bias` and
+:func:`residual_norm`.
 """
 
 from .api import (
@@ -28,6 +30,7 @@ from .api import (
     det_planar,
     pf_planar,
 )
+from .block import biased_attention, position_bias, residual_norm
 
 __version__ = "0.1.0"
 __all__ = [
@@ -50,6 +53,9 @@ __all__ = [
     "slogpf_planar",
     "det_planar",
     "pf_planar",
+    "biased_attention",
+    "position_bias",
+    "residual_norm",
     "FermixFallbackWarning",
     "__version__",
 ]

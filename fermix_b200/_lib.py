@@ -12,11 +12,12 @@ import threading
 LIB_DIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libfermix_b200.so")
 
-FX_F32, FX_F64, FX_C64, FX_C128 = 0, 1, 2, 3
+FX_F32, FX_F64, FX_C64, FX_C128, FX_BF16 = 0, 1, 2, 3, 4
 FX_PREC_DEFAULT, FX_PREC_TF32X3, FX_PREC_IEEE = 0, 1, 2
 FX_OP_SLOGDET, FX_OP_SLOGPF = 0, 1
 FX_ERR_TIMEOUT = 8
 FX_WAIT_POLLS_DEFAULT = 1 << 26
+FX_NORM_MAX_WIDTH, FX_ATTN_MAX_DIM, FX_BUCKET_MAX, FX_BUCKET_MAX_EDGE = 8192, 128, 256, 2048
 
 # every symbol include/fermix_b200.h declares, with its ctypes signature
 _vp, _i, _i64, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
@@ -53,10 +54,63 @@ SIGNATURES = {
     "fermix_slogpf_grad_planar": (
         _i, [_vp, _i, _i, _i64, _i64, _i, _vp, _vp, _vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz]),
     "fermix_workspace_bytes_planar": (_sz, [_i, _i, _i64, _i64, _i]),
+    # include/fermix_b200_block.h
+    "fermix_residual_norm": (_i, [_vp, _vp]),
+    "fermix_residual_norm_grad": (_i, [_vp, _vp, _vp, _sz]),
+    "fermix_residual_norm_grad_workspace_bytes": (_sz, [_vp]),
+    "fermix_position_bias": (_i, [_vp, _vp]),
+    "fermix_position_bias_grad": (_i, [_vp, _vp, _vp, _sz]),
+    "fermix_position_bias_grad_workspace_bytes": (_sz, [_vp]),
+    "fermix_biased_attention": (_i, [_vp, _vp, _vp, _sz]),
+    "fermix_biased_attention_workspace_bytes": (_sz, [_vp]),
+    "fermix_biased_attention_grad": (_i, [_vp, _vp, _vp, _sz]),
+    "fermix_biased_attention_grad_workspace_bytes": (_sz, [_vp]),
     # include/fermix_b200_xla.h
     "fermix_xla_custom_call": (None, [_vp, _vp, ctypes.c_char_p, _sz]),
     "fermix_xla_last_error": (_i, [_i]),
 }
+
+
+
+def _fields(kind, names):
+    return [(n, kind) for n in names.split()]
+
+
+_i32, _f32, _i64x3 = ctypes.c_int32, ctypes.c_float, ctypes.c_int64 * 3
+
+
+class NormArgs(ctypes.Structure):
+    """fx_norm_args (include/fermix_b200_block.h)."""
+
+    _fields_ = (_fields(_i32, "dtype kind gate_mode dgate_f32") + _fields(_f32, "eps") + _fields(_i32, "reserved") + _fields(_i64, "groups rows width") +
+                _fields(_vp, "x f gate scale post_weight post_bias pre_weight pre_bias r z grad_r grad_z dx df dgate "
+                        "dscale dpost_weight dpost_bias dpre_weight dpre_bias"))
+
+
+class Buckets(ctypes.Structure):
+    """fx_buckets."""
+
+    _fields_ = (_fields(_i32, "num_buckets two_sided num_edges reserved") + _fields(_vp, "edges q_pos k_pos") +
+                _fields(_i64, "q_pos_stride k_pos_stride"))
+
+
+class BiasArgs(ctypes.Structure):
+    """fx_bias_args."""
+
+    _fields_ = (_fields(_i32, "dtype reserved") + _fields(_i64, "batch heads q_len k_len") + [("buckets", Buckets)] +
+                _fields(_vp, "table out grad dtable"))
+
+
+class AttnArgs(ctypes.Structure):
+    """fx_attn_args."""
+
+    _fields_ = (_fields(_i32, "dtype causal") + _fields(_i64, "batch heads kv_heads q_len k_len dim") +
+                _fields(_f32, "scale") + _fields(_i32, "reserved") + [("buckets", Buckets)] +
+                _fields(_vp, "q k v table") + _fields(_i64x3, "q_stride k_stride v_stride") +
+                _fields(_vp, "key_mask") + _fields(_i64, "mask_stride") + _fields(_vp, "out") +
+                _fields(_i64x3, "out_stride") + _fields(_vp, "lse dout") + _fields(_i64x3, "dout_stride") +
+                _fields(_vp, "dq dk dv dtable") + _fields(_i64x3, "dq_stride dk_stride dv_stride"))
+
 
 _lib = None
 _lock = threading.Lock()

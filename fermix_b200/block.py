@@ -1,0 +1,407 @@
+"""The attention block of a neural wave function, on torch CUDA tensors: the network in front of
+the determinants turns the tokens of the occupied sites into the orbitals that ``slogdet`` /
+``slogpf`` take.
+
+* :func:`biased_attention` -- softmax attention whose scores carry a learned bias of the
+  distance between the tokens' positions, forward, gradient, and for a single new token;
+* :func:`position_bias` -- that bias as an array, and its gradient;
+* :func:`residual_norm` -- the residual between two blocks with its gate, its scale and the
+  norms on both sides.
+
+float32 and bfloat16; statistics, sums and softmax are float32, and every result is rounded
+once. Gradients go through torch autograd and are summed in a fixed order (two runs give the
+same bits). There is no CPU path and, as in the rest of the package, no fallback. None of this
+has a counterpart in the reference, whose caller brings the network.
+"""
+
+import ctypes
+import functools
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .api import _ptr, _stream_ptr
+
+_KIND = {torch.float32: _lib.FX_F32, torch.bfloat16: _lib.FX_BF16}
+_INTS = (torch.int32, torch.int64, torch.int16, torch.uint8)
+_GATE_NONE, _GATE_FULL, _GATE_ROW, _GATE_GROUP = range(4)
+
+
+# ------------------------------------------------------------------ checks
+def _tensor(t, name, like=None):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
+    if like is None:
+        if t.dtype not in _KIND:
+            raise TypeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
+        if t.device.type != "cuda":
+            raise RuntimeError(
+                f"fermix_b200 runs on CUDA devices only (got a tensor on {t.device}); "
+                "move it with .cuda() -- there is no CPU fallback"
+            )
+    else:
+        if t.dtype != like.dtype:
+            raise TypeError(f"{name} must have dtype {like.dtype}, got {t.dtype}")
+        if t.device != like.device:
+            raise ValueError(f"{name} must be on {like.device}, got {t.device}")
+    return t
+
+
+@functools.lru_cache(maxsize=64, typed=True)
+def _edges(num_buckets, max_distance, bidirectional):
+    """The least distance of each bucket after the first, of one side: a bucket for each
+    distance below half of the side's buckets, then evenly spaced in the logarithm up to
+    ``max_distance`` -- bucket ``exact + j`` starts where
+    log(d / exact) / log(max_distance / exact) >= j / (n - exact), in whole numbers."""
+    if not isinstance(num_buckets, int) or not 1 <= num_buckets <= _lib.FX_BUCKET_MAX:
+        raise ValueError(f"the table must have 1 to {_lib.FX_BUCKET_MAX} buckets, got {num_buckets}")
+    if bidirectional and num_buckets % 2:
+        raise ValueError(f"a bidirectional table must have an even number of buckets, got {num_buckets}")
+    n = num_buckets // 2 if bidirectional else num_buckets
+    exact = n // 2
+    if not isinstance(max_distance, int) or not exact < max_distance <= _lib.FX_BUCKET_MAX_EDGE:
+        raise ValueError(
+            f"max_distance must be a whole number above {exact} (the distances with a bucket of their own) and at "
+            f"most {_lib.FX_BUCKET_MAX_EDGE}, got {max_distance!r}")
+    edges, d, m = list(range(1, exact + 1)), exact, n - exact
+    for j in range(1, m if exact else 1):
+        while d**m * exact**j < max_distance**j * exact**m:
+            d += 1
+        edges.append(d)
+    return (ctypes.c_int32 * max(1, len(edges)))(*edges), len(edges)
+
+
+def _positions(pos, length, batch, device, name):
+    """An int32 (length) or (batch, length) tensor with contiguous rows, and its batch stride."""
+    if not isinstance(pos, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor, got {type(pos).__name__}")
+    if pos.dtype not in _INTS:
+        raise TypeError(f"{name} must be an integer tensor, got {pos.dtype}")
+    if pos.device != device:
+        raise ValueError(f"{name} must be on {device}, got {pos.device}")
+    if tuple(pos.shape) not in ((length,), (batch, length)):
+        raise ValueError(f"{name} must have shape ({length},) or ({batch}, {length}), got {tuple(pos.shape)}")
+    if pos.dtype != torch.int32:
+        pos = pos.to(torch.int32)
+    if pos.shape[-1] > 1 and pos.stride(-1) != 1:
+        pos = pos.contiguous()
+    return pos, pos.stride(0) if pos.dim() == 2 else 0
+
+
+def _buckets(num_buckets, max_distance, bidirectional, q_pos, k_pos, q_stride, k_stride):
+    edges, count = _edges(num_buckets, max_distance, bool(bidirectional))
+    return _lib.Buckets(num_buckets, int(bool(bidirectional)), count, 0, ctypes.addressof(edges), _ptr(q_pos),
+                        _ptr(k_pos), q_stride, k_stride)
+
+
+def _workspace(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+# ------------------------------------------------------------------ residual with its norms
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, f, post_weight, pre_weight, post_bias, pre_bias, gate, scale, form, kind, eps):
+        gate_shape, shape, gate_mode = form
+        given = None if gate is None else gate.shape
+        if gate is not None:
+            gate = gate.expand(gate_shape).contiguous()
+        r, z = torch.empty_like(x), torch.empty_like(x)
+        a = _norm_args(x, f, post_weight, pre_weight, post_bias, pre_bias, gate, scale, shape, kind, gate_mode, eps)
+        a.r, a.z = _ptr(r), _ptr(z)
+        with torch.cuda.device(x.device):
+            _lib.check(_lib.lib().fermix_residual_norm(_stream_ptr(x.device), ctypes.byref(a)))
+        ctx.save_for_backward(x, f, post_weight, pre_weight, post_bias, pre_bias, gate, scale)
+        ctx.rest, ctx.given = (shape, kind, gate_mode, eps), given
+        ctx.set_materialize_grads(False)
+        return r, z
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_r, grad_z):
+        saved = ctx.saved_tensors
+        if grad_r is None and grad_z is None:
+            return (None,) * 11
+        x = saved[0]
+        a = _norm_args(*saved, *ctx.rest)
+        grads = [None if t is None else torch.empty_like(t) for t in saved]
+        shared = ctx.given is not None and ctx.given != saved[6].shape
+        if shared:  # a gate expanded for the kernel: its gradient is summed in float32, rounded once
+            a.dgate_f32 = 1
+            grads[6] = torch.empty_like(saved[6], dtype=torch.float32)
+        # every pointer's tensor stays referenced here until the launches are queued
+        grad_r, grad_z = (None if g is None else g.contiguous() for g in (grad_r, grad_z))
+        a.grad_r, a.grad_z = _ptr(grad_r), _ptr(grad_z)
+        (a.dx, a.df, a.dpost_weight, a.dpre_weight, a.dpost_bias, a.dpre_bias, a.dgate,
+         a.dscale) = (_ptr(g) for g in grads)
+        L = _lib.lib()
+        with torch.cuda.device(x.device):
+            nb = L.fermix_residual_norm_grad_workspace_bytes(ctypes.byref(a))
+            ws = _workspace(nb, x.device)
+            _lib.check(L.fermix_residual_norm_grad(_stream_ptr(x.device), ctypes.byref(a), _ptr(ws), nb))
+        if shared:
+            grads[6] = grads[6].sum_to_size(ctx.given).to(x.dtype)
+        return (*grads, None, None, None)
+
+
+def _norm_args(x, f, post_weight, pre_weight, post_bias, pre_bias, gate, scale, shape, kind, gate_mode, eps):
+    a = _lib.NormArgs()
+    a.dtype, a.kind, a.gate_mode, a.eps = _KIND[x.dtype], kind, gate_mode, eps
+    a.groups, a.rows, a.width = shape
+    a.x, a.f, a.gate, a.scale = _ptr(x), _ptr(f), _ptr(gate), _ptr(scale)
+    a.post_weight, a.post_bias, a.pre_weight, a.pre_bias = (_ptr(t) for t in
+                                                            (post_weight, post_bias, pre_weight, pre_bias))
+    return a
+
+
+def _gate_form(gate, x):
+    """(shape the kernel takes the gate in, (groups, rows, width), mode): which entries of x an entry
+    of the gate is shared by. Shapes other than the kernel's four expand to the nearest one."""
+    width, lead = x.shape[-1], tuple(x.shape[:-1])
+    total = math.prod(lead)
+    if gate is None:
+        return None, (1, total, width), _GATE_NONE
+    shape = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape)
+    if gate.dim() > x.dim() or any(n not in (1, m) for n, m in zip(shape, x.shape)):
+        raise ValueError(f"gate must broadcast to {tuple(x.shape)}, got {tuple(gate.shape)}")
+    if shape == tuple(x.shape):
+        return gate.shape, (1, total, width), _GATE_FULL
+    if shape[:-1] == lead:
+        return gate.shape, (1, total, width), _GATE_ROW
+    # the leading dimensions it has in full, then those it is shared along
+    k = 0
+    while shape[k] == lead[k]:
+        k += 1
+    if all(n == 1 for n in shape[k:-1]):
+        groups = math.prod(lead[:k])
+        return (gate.shape if shape[-1] == width else shape[:-1] + (width,)), (
+            groups, total // groups if groups else 0, width), _GATE_GROUP
+    return x.shape, (1, total, width), _GATE_FULL
+
+
+def residual_norm(x, f, post_weight, pre_weight, *, post_bias=None, pre_bias=None, gate=None, scale=None, kind="rms",
+                  eps=1e-6):
+    """The residual between two blocks of a network with the norms on both sides of it:
+    ``u = norm(f)``, ``r = x + scale * gate * u``, ``z = norm(r)``; returns ``(r, z)``.
+
+    ``x`` is the residual stream and ``f`` the output of the block just run, (..., width), float32
+    or bfloat16, width <= 8192; ``post_*`` (width,) belong to the norm of ``f``, ``pre_*`` to that
+    of ``r`` (the input of the next block). ``kind="rms"`` divides by sqrt(mean square + eps);
+    ``"layer"`` takes the mean off first. ``scale`` (width,) and ``gate`` (anything that broadcasts
+    to ``x``: an entry each, one per row (..., 1), a vector per sample (batch, 1, width)) multiply
+    the normed branch. All of one dtype; differentiable in every tensor. z is formed from the
+    unrounded r."""
+    x = _tensor(x, "x")
+    if kind not in ("rms", "layer"):
+        raise ValueError(f"kind must be 'rms' or 'layer', got {kind!r}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= _lib.FX_NORM_MAX_WIDTH:
+        raise ValueError(f"expected (..., width) with 1 <= width <= {_lib.FX_NORM_MAX_WIDTH}, got {tuple(x.shape)}")
+    if _tensor(f, "f", x).shape != x.shape:
+        raise ValueError(f"f must have the shape of x {tuple(x.shape)}, got {tuple(f.shape)}")
+    width = x.shape[-1]
+    params = []
+    for name, t in (("post_weight", post_weight), ("pre_weight", pre_weight), ("post_bias", post_bias),
+                    ("pre_bias", pre_bias), ("scale", scale)):
+        if t is None and name not in ("post_weight", "pre_weight"):
+            params.append(None)
+            continue
+        if tuple(_tensor(t, name, x).shape) != (width,):
+            raise ValueError(f"{name} must have shape ({width},), got {tuple(t.shape)}")
+        params.append(t.contiguous())
+    if gate is not None:
+        _tensor(gate, "gate", x)
+    form = _gate_form(gate, x)
+    post_weight, pre_weight, post_bias, pre_bias, scale = params
+    return _ResidualNorm.apply(x.contiguous(), f.contiguous(), post_weight, pre_weight, post_bias, pre_bias, gate,
+                               scale, form, int(kind == "layer"), float(eps))
+
+
+# ------------------------------------------------------------------ position bias
+class _PositionBias(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, q_pos, k_pos, q_stride, k_stride, batch, q_len, k_len, max_distance, bidirectional):
+        a = _lib.BiasArgs()
+        a.dtype = _KIND[table.dtype]
+        a.batch, a.heads, a.q_len, a.k_len = batch, table.shape[0], q_len, k_len
+        a.buckets = _buckets(table.shape[1], max_distance, bidirectional, q_pos, k_pos, q_stride, k_stride)
+        out = torch.empty((batch, table.shape[0], q_len, k_len), dtype=table.dtype, device=table.device)
+        a.table, a.out = _ptr(table), _ptr(out)
+        with torch.cuda.device(table.device):
+            _lib.check(_lib.lib().fermix_position_bias(_stream_ptr(table.device), ctypes.byref(a)))
+        ctx.save_for_backward(q_pos, k_pos)
+        ctx.args, ctx.table = a, (table.shape, table.dtype)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        a = ctx.args
+        q_pos, k_pos = ctx.saved_tensors
+        grad = grad.contiguous()
+        dtable = torch.empty(ctx.table[0], dtype=ctx.table[1], device=grad.device)
+        a.grad, a.dtable = _ptr(grad), _ptr(dtable)
+        a.buckets.q_pos, a.buckets.k_pos = _ptr(q_pos), _ptr(k_pos)
+        L = _lib.lib()
+        with torch.cuda.device(grad.device):
+            nb = L.fermix_position_bias_grad_workspace_bytes(ctypes.byref(a))
+            ws = _workspace(nb, grad.device)
+            _lib.check(L.fermix_position_bias_grad(_stream_ptr(grad.device), ctypes.byref(a), _ptr(ws), nb))
+        return dtable, None, None, None, None, None, None, None, None, None
+
+
+def position_bias(table, q_pos, k_pos=None, *, max_distance=128, bidirectional=True):
+    """The learned bias of each pair of positions, ``table[h, bucket(k_pos - q_pos)]``: (heads,
+    q_len, k_len), or (batch, heads, q_len, k_len) where a position tensor is (batch, length).
+
+    ``table`` is (heads, num_buckets), float32 or bfloat16. A side has a bucket for each distance
+    below half of its buckets, and the rest evenly spaced in the logarithm up to ``max_distance``
+    (<= 2048; all longer distances share the last one); ``bidirectional`` gives half of the table to
+    each sign, otherwise keys after the query share bucket 0. ``q_pos`` and ``k_pos`` (default:
+    q_pos) are integer tensors within +-2**30, in any order. Differentiable in ``table``."""
+    table = _tensor(table, "table")
+    if table.dim() != 2:
+        raise ValueError(f"table must have shape (heads, num_buckets), got {tuple(table.shape)}")
+    if k_pos is None:
+        k_pos = q_pos
+    batch = 1
+    for name, p in (("q_pos", q_pos), ("k_pos", k_pos)):
+        if not isinstance(p, torch.Tensor):
+            raise TypeError(f"{name} must be a torch tensor, got {type(p).__name__}")
+        if p.dim() not in (1, 2):
+            raise ValueError(f"{name} must have shape (length,) or (batch, length), got {tuple(p.shape)}")
+        if p.dim() == 2:
+            batch = p.shape[0]
+    q, qs = _positions(q_pos, q_pos.shape[-1], batch, table.device, "q_pos")
+    k, ks = _positions(k_pos, k_pos.shape[-1], batch, table.device, "k_pos")
+    out = _PositionBias.apply(table.contiguous(), q, k, qs, ks, batch, q.shape[-1], k.shape[-1], max_distance,
+                              bool(bidirectional))
+    return out if q.dim() == 2 or k.dim() == 2 else out[0]
+
+
+# ------------------------------------------------------------------ attention
+def _strides(t):
+    return t.stride()[:3]
+
+
+def _attn_args(q, k, v, table, q_pos, k_pos, key_mask, out, lse, causal, scale, max_distance, bidirectional):
+    a = _lib.AttnArgs()
+    a.dtype, a.causal = _KIND[q.dtype], int(causal)
+    a.batch, a.heads, a.q_len, a.dim = q.shape
+    a.kv_heads, a.k_len = k.shape[1], k.shape[2]
+    a.scale = scale
+    qs = q_pos.stride(0) if q_pos is not None and q_pos.dim() == 2 else 0
+    ks = k_pos.stride(0) if k_pos is not None and k_pos.dim() == 2 else 0
+    if table is not None:
+        a.buckets = _buckets(table.shape[1], max_distance, bidirectional, q_pos, k_pos, qs, ks)
+    else:
+        a.buckets.q_pos, a.buckets.k_pos, a.buckets.q_pos_stride, a.buckets.k_pos_stride = _ptr(q_pos), _ptr(
+            k_pos), qs, ks
+    a.q, a.k, a.v, a.table = _ptr(q), _ptr(k), _ptr(v), _ptr(table)
+    a.q_stride[:], a.k_stride[:], a.v_stride[:] = _strides(q), _strides(k), _strides(v)
+    if key_mask is not None:
+        a.key_mask, a.mask_stride = _ptr(key_mask), key_mask.stride(0)
+    a.out, a.lse = _ptr(out), _ptr(lse)
+    a.out_stride[:] = _strides(out)
+    return a
+
+
+def _attn_forward(q, k, v, table, q_pos, k_pos, key_mask, with_lse, causal, scale, max_distance, bidirectional):
+    out = torch.empty_like(q)
+    if out.stride(-1) != 1:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if with_lse else None
+    a = _attn_args(q, k, v, table, q_pos, k_pos, key_mask, out, lse, causal, scale, max_distance, bidirectional)
+    L = _lib.lib()
+    with torch.cuda.device(q.device):
+        nb = L.fermix_biased_attention_workspace_bytes(ctypes.byref(a))
+        ws = _workspace(nb, q.device)
+        _lib.check(L.fermix_biased_attention(_stream_ptr(q.device), ctypes.byref(a), _ptr(ws), nb))
+    return out, lse
+
+
+class _BiasedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, q_pos, k_pos, key_mask, *rest):
+        out, lse = _attn_forward(q, k, v, table, q_pos, k_pos, key_mask, True, *rest)
+        ctx.save_for_backward(q, k, v, table, q_pos, k_pos, key_mask, out, lse)
+        ctx.rest = rest
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, table, q_pos, k_pos, key_mask, out, lse = ctx.saved_tensors
+        dout = _rows(dout)
+        a = _attn_args(q, k, v, table, q_pos, k_pos, key_mask, out, lse, *ctx.rest)
+        dq, dk, dv = (_rows(torch.empty_like(t)) for t in (q, k, v))
+        dtable = None if table is None else torch.empty_like(table)
+        a.dout, a.dq, a.dk, a.dv, a.dtable = _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable)
+        a.dout_stride[:], a.dq_stride[:] = _strides(dout), _strides(dq)
+        a.dk_stride[:], a.dv_stride[:] = _strides(dk), _strides(dv)
+        L = _lib.lib()
+        with torch.cuda.device(q.device):
+            nb = L.fermix_biased_attention_grad_workspace_bytes(ctypes.byref(a))
+            ws = _workspace(nb, q.device)
+            _lib.check(L.fermix_biased_attention_grad(_stream_ptr(q.device), ctypes.byref(a), _ptr(ws), nb))
+        return (dq, dk, dv, dtable) + (None,) * 8
+
+
+def _rows(t):
+    """t with the entries of a token next to each other."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 and t.is_contiguous() else t.contiguous()
+
+
+def biased_attention(q, k, v, table=None, *, q_pos=None, k_pos=None, key_mask=None, causal=False, scale=None,
+                     max_distance=128, bidirectional=True):
+    """Attention with a learned bias of the positions' distance in its scores:
+    ``softmax(scale * q k^T + table[h, bucket(k_pos - q_pos)]) v``, without the array of scores.
+
+    ``q`` is (batch, heads, q_len, dim), ``k`` and ``v`` (batch, kv_heads, k_len, dim) with heads a
+    multiple of kv_heads (head h reads key head h // (heads // kv_heads)) and dim <= 128, float32 or
+    bfloat16, any strides (the head-major view of token-major storage is read in place). ``table``
+    (heads, num_buckets), of the same dtype, ``max_distance`` and ``bidirectional`` are those of
+    :func:`position_bias`; None: no bias. ``k_pos`` defaults to 0, 1, ..., and ``q_pos`` to the last
+    q_len of them (a new token attends from the end of the cache); integer tensors (length,) or
+    (batch, length), within +-2**30. ``key_mask`` (batch, k_len) bool: False leaves a key out,
+    whatever its k and v hold. ``causal`` leaves out keys with k_pos > q_pos. A query without any
+    key gives 0 and has no gradient. ``scale`` defaults to dim ** -0.5.
+
+    Differentiable in q, k, v and table; under ``torch.no_grad()`` nothing is kept. Few queries
+    (one new token) split the keys over the device and join the parts."""
+    q = _tensor(q, "q")
+    for name, t in (("k", k), ("v", v)):
+        _tensor(t, name, q)
+    if q.dim() != 4 or k.dim() != 4 or not 1 <= q.shape[3] <= _lib.FX_ATTN_MAX_DIM:
+        raise ValueError(f"q, k and v must have shape (batch, heads, length, dim) with 1 <= dim <= "
+                         f"{_lib.FX_ATTN_MAX_DIM}, got {tuple(q.shape)}, {tuple(k.shape)}")
+    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"k and v must both have shape ({q.shape[0]}, kv_heads, k_len, {q.shape[3]}), got "
+                         f"{tuple(k.shape)} and {tuple(v.shape)}")
+    batch, heads, q_len, dim = q.shape
+    k_len = k.shape[2]
+    if heads and (k.shape[1] == 0 or heads % k.shape[1]):
+        raise ValueError(f"the {heads} heads must be a multiple of the {k.shape[1]} key heads")
+    if table is not None:
+        if _tensor(table, "table", q).dim() != 2 or table.shape[0] != heads:
+            raise ValueError(f"table must have shape ({heads}, num_buckets), got {tuple(table.shape)}")
+        table = table.contiguous()
+    if q_pos is not None:
+        q_pos, _ = _positions(q_pos, q_len, batch, q.device, "q_pos")
+    if k_pos is not None:
+        k_pos, _ = _positions(k_pos, k_len, batch, q.device, "k_pos")
+    if key_mask is not None:
+        if not isinstance(key_mask, torch.Tensor) or key_mask.dtype != torch.bool:
+            raise TypeError("key_mask must be a bool tensor (True: the key takes part)")
+        if tuple(key_mask.shape) != (batch, k_len) or key_mask.device != q.device:
+            raise ValueError(f"key_mask must have shape ({batch}, {k_len}) on {q.device}, got "
+                             f"{tuple(key_mask.shape)} on {key_mask.device}")
+        if k_len > 1 and key_mask.stride(1) != 1:
+            key_mask = key_mask.contiguous()
+    rest = (bool(causal), float(dim**-0.5 if scale is None else scale), max_distance, bool(bidirectional))
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                    (table is not None and table.requires_grad)):
+        return _BiasedAttention.apply(q, k, v, table, q_pos, k_pos, key_mask, *rest)
+    return _attn_forward(q, k, v, table, q_pos, k_pos, key_mask, False, *rest)[0]

@@ -1,0 +1,244 @@
+// Attention with the position bias: checks, choice of kernel, launch shapes, workspace.
+#include "attn_rows.cuh"
+#include "attn_rows_grad.cuh"
+#include "block_host.cuh"
+#include "position_bias.cuh"
+
+namespace {
+
+using namespace fxh;
+
+constexpr int kRC = 4;          // query rows of a block (attn_rows.cuh)
+constexpr int kMinSplit = 128;  // keys of a part, at least
+
+int check(const fx_attn_args* a) {
+  if (!a) return FX_ERR_NULL;
+  if (a->dtype != FX_F32 && a->dtype != FX_BF16) return FX_ERR_DTYPE;
+  if (a->batch < 0 || a->heads < 0 || a->kv_heads < 0 || a->q_len < 0 || a->k_len < 0 || a->dim < 1 ||
+      a->dim > FX_ATTN_MAX_DIM)
+    return FX_ERR_SHAPE;
+  if (a->batch > (1 << 30) || a->heads > 65535 || a->q_len > (1 << 30) || a->k_len > (1 << 30)) return FX_ERR_SHAPE;
+  if (a->heads > 0 && (a->kv_heads == 0 || a->heads % a->kv_heads)) return FX_ERR_SHAPE;
+  if (a->batch * a->kv_heads > 65535 || a->q_len * a->heads > (int64_t{65535} * kRC)) return FX_ERR_SHAPE;
+  return a->table ? check_buckets(a->buckets) : FX_OK;
+}
+
+bool no_rows(const fx_attn_args* a) { return a->batch == 0 || a->heads == 0 || a->q_len == 0; }
+
+void copy3(int64_t* d, const int64_t* s) {
+  for (int i = 0; i < 3; ++i) d[i] = s[i];
+}
+
+AttnArgs make(const fx_attn_args* a) {
+  AttnArgs A{};
+  A.q = a->q;
+  A.k = a->k;
+  A.v = a->v;
+  A.table = a->table;
+  copy3(A.qs, a->q_stride);
+  copy3(A.ks, a->k_stride);
+  copy3(A.vs, a->v_stride);
+  copy3(A.os, a->out_stride);
+  copy3(A.dos, a->dout_stride);
+  copy3(A.dqs, a->dq_stride);
+  copy3(A.dks, a->dk_stride);
+  copy3(A.dvs, a->dv_stride);
+  A.mask = a->key_mask;
+  A.mask_stride = a->mask_stride;
+  A.q_pos = a->buckets.q_pos;
+  A.k_pos = a->buckets.k_pos;
+  A.q_pos_stride = a->buckets.q_pos_stride;
+  A.k_pos_stride = a->buckets.k_pos_stride;
+  A.out = a->out;
+  A.lse = a->lse;
+  A.dout = a->dout;
+  A.dq = a->dq;
+  A.dk = a->dk;
+  A.dv = a->dv;
+  A.Lq = a->q_len;
+  A.Lk = a->k_len;
+  A.B = (int)a->batch;
+  A.H = (int)a->heads;
+  A.Hk = (int)a->kv_heads;
+  A.D = (int)a->dim;
+  A.causal = a->causal != 0;
+  A.scale = a->scale;
+  A.scale2 = a->scale * kLog2e;
+  if (a->table) A.buckets = make_buckets(a->buckets);
+  return A;
+}
+
+// Whether every token of these tensors starts on a 16-byte boundary and is whole vectors.
+bool aligned(const fx_attn_args* a, bool grad) {
+  const int size = a->dtype == FX_F32 ? 4 : 2;
+  uintptr_t m = (uintptr_t)a->dim * size;
+  auto add = [&](const void* p, const int64_t* s) {
+    m |= reinterpret_cast<uintptr_t>(p);
+    for (int i = 0; i < 3; ++i) m |= (uintptr_t)(s[i] * size);
+  };
+  add(a->q, a->q_stride);
+  add(a->k, a->k_stride);
+  add(a->v, a->v_stride);
+  if (grad) add(a->dout, a->dout_stride);
+  return m % 16 == 0;
+}
+
+// Lanes of a key: 16 bytes each, a power of two, eight at least.
+int lanes_of(const fx_attn_args* a) {
+  const int need = (int)((a->dim * (a->dtype == FX_F32 ? 4 : 2) + 15) / 16);
+  return need <= 8 ? 8 : need <= 16 ? 16 : 32;
+}
+
+void split_keys(const fx_attn_args* a, int sms, AttnArgs& A) {
+  const int64_t rows = a->heads / a->kv_heads * a->q_len;
+  const int64_t blocks = (rows + kRC - 1) / kRC * a->batch * a->kv_heads;
+  int64_t splits = (int64_t{8} * sms + blocks - 1) / blocks;
+  const int64_t most = (a->k_len + kMinSplit - 1) / kMinSplit;
+  splits = splits < most ? splits : most;
+  if (splits < 1) splits = 1;
+  A.split_keys = ((a->k_len + splits - 1) / splits + 31) / 32 * 32;
+  A.splits = A.split_keys ? (int)((a->k_len + A.split_keys - 1) / A.split_keys) : 1;
+  if (A.splits < 1) A.splits = 1;
+}
+
+size_t part_bytes(const fx_attn_args* a, const AttnArgs& A) {
+  return A.splits > 1 ? (size_t)(a->batch * a->heads * a->q_len) * A.splits * (a->dim + 2) * sizeof(float) + 256 : 0;
+}
+
+template <typename K>
+int raise_smem(K kern, size_t smem) {
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return FX_ERR_CUDA;
+  return FX_OK;
+}
+
+template <typename T, int LPK, bool VL>
+int launch_fwd(cudaStream_t s, const AttnArgs& A) {
+  constexpr int NE = 16 / sizeof(T), GROUPS = kRowsThreads / LPK;
+  const size_t lut = A.table ? (size_t)kRC * (2 * A.buckets.reach + 1) * 4 : 0;
+  const size_t join = (size_t)GROUPS * kRC * (2 + LPK * NE) * 4;
+  const size_t smem = lut > join ? lut : join;
+  auto kern = attn_rows_kernel<T, LPK, VL, kRC>;
+  if (raise_smem(kern, smem)) return FX_ERR_CUDA;
+  const int64_t rows = (int64_t)(A.H / A.Hk) * A.Lq;
+  kern<<<dim3(A.splits, (unsigned)((rows + kRC - 1) / kRC), A.B * A.Hk), kRowsThreads, smem, s>>>(A);
+  if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
+  if (A.splits > 1) {
+    attn_join_kernel<T><<<(unsigned)(((int64_t)A.B * A.H * A.Lq + 3) / 4), kRowsThreads, 0, s>>>(A);
+    if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
+  }
+  return FX_OK;
+}
+
+template <typename T, int LPK, bool VL>
+int launch_bwd(cudaStream_t s, const AttnArgs& A) {
+  constexpr int NE = 16 / sizeof(T), GROUPS = kRowsThreads / LPK;
+  const size_t join = (size_t)GROUPS * kRC * LPK * NE * 4;
+  const size_t hist = A.table ? (size_t)GROUPS * kRC * A.buckets.num_buckets * 8 : 0;
+  const size_t smem = hist > join ? hist : join;
+  const int64_t qrows = (int64_t)(A.H / A.Hk) * A.Lq;
+  auto kq = attn_rows_grad_kernel<T, LPK, VL, kRC, false>;
+  auto kk = attn_rows_grad_kernel<T, LPK, VL, kRC, true>;
+  if (raise_smem(kq, smem) || raise_smem(kk, join)) return FX_ERR_CUDA;
+  if (A.Lq > 0) {
+    attn_delta_kernel<T><<<(unsigned)(((int64_t)A.B * A.H * A.Lq + 3) / 4), kRowsThreads, 0, s>>>(A);
+    kq<<<dim3((unsigned)((qrows + kRC - 1) / kRC), 1, A.B * A.Hk), kRowsThreads, smem, s>>>(A);
+  }
+  if (A.Lk > 0) kk<<<dim3((unsigned)((A.Lk + kRC - 1) / kRC), 1, A.B * A.Hk), kRowsThreads, join, s>>>(A);
+  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+}
+
+template <typename T>
+int fwd(cudaStream_t s, const AttnArgs& A, int lanes, bool vec) {
+  if (lanes == 8) return vec ? launch_fwd<T, 8, true>(s, A) : launch_fwd<T, 8, false>(s, A);
+  if (lanes == 16) return vec ? launch_fwd<T, 16, true>(s, A) : launch_fwd<T, 16, false>(s, A);
+  if constexpr (sizeof(T) == 4) return vec ? launch_fwd<T, 32, true>(s, A) : launch_fwd<T, 32, false>(s, A);
+  return FX_ERR_SHAPE;
+}
+
+template <typename T>
+int bwd(cudaStream_t s, const AttnArgs& A, int lanes, bool vec) {
+  if (lanes == 8) return vec ? launch_bwd<T, 8, true>(s, A) : launch_bwd<T, 8, false>(s, A);
+  if (lanes == 16) return vec ? launch_bwd<T, 16, true>(s, A) : launch_bwd<T, 16, false>(s, A);
+  if constexpr (sizeof(T) == 4) return vec ? launch_bwd<T, 32, true>(s, A) : launch_bwd<T, 32, false>(s, A);
+  return FX_ERR_SHAPE;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fermix_biased_attention_workspace_bytes(const fx_attn_args* a) {
+  const DevInfo* D = dev_info();
+  if (check(a) || !D || no_rows(a)) return 0;
+  AttnArgs A{};
+  split_keys(a, D->sms, A);
+  return part_bytes(a, A);
+}
+
+int fermix_biased_attention(void* stream, const fx_attn_args* a, void* ws, size_t wsb) {
+  const int e = check(a);
+  if (e) return e;
+  if (no_rows(a)) return FX_OK;
+  if (!a->q || !a->out || (a->k_len > 0 && (!a->k || !a->v))) return FX_ERR_NULL;
+  const DevInfo* D = dev_info();
+  if (!D) return FX_ERR_DEVICE;
+  AttnArgs A = make(a);
+  split_keys(a, D->sms, A);
+  const size_t need = part_bytes(a, A);
+  if (need) {
+    if (!ws || wsb < need) return FX_ERR_WORKSPACE;
+    A.part = reinterpret_cast<float*>(align256(reinterpret_cast<uintptr_t>(ws)));
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool vec = aligned(a, false);
+  return a->dtype == FX_F32 ? fwd<float>(s, A, lanes_of(a), vec) : fwd<bf16>(s, A, lanes_of(a), vec);
+}
+
+size_t fermix_biased_attention_grad_workspace_bytes(const fx_attn_args* a) {
+  if (check(a) || no_rows(a)) return 0;
+  const size_t rows = (size_t)(a->batch * a->heads * a->q_len);
+  return align256(rows * 4) + (a->table ? align256(rows * a->buckets.num_buckets * 4) : 0) + 256;
+}
+
+int fermix_biased_attention_grad(void* stream, const fx_attn_args* a, void* ws, size_t wsb) {
+  const int e = check(a);
+  if (e) return e;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a->batch == 0 || a->heads == 0) {
+    if (a->table && a->heads > 0) {
+      if (!a->dtable) return FX_ERR_NULL;
+      if (cudaMemsetAsync(a->dtable, 0, (size_t)a->heads * a->buckets.num_buckets * (a->dtype == FX_F32 ? 4 : 2),
+                          s) != cudaSuccess)
+        return FX_ERR_CUDA;
+    }
+    return FX_OK;
+  }
+  if ((a->q_len > 0 && (!a->q || !a->dout || !a->out || !a->lse || !a->dq)) ||
+      (a->k_len > 0 && (!a->k || !a->v || !a->dk || !a->dv)) || (a->table && !a->dtable))
+    return FX_ERR_NULL;
+  const DevInfo* D = dev_info();
+  if (!D) return FX_ERR_DEVICE;
+  AttnArgs A = make(a);
+  const size_t rows = (size_t)(a->batch * a->heads * a->q_len);
+  const size_t need = fermix_biased_attention_grad_workspace_bytes(a);
+  if (need && (!ws || wsb < need)) return FX_ERR_WORKSPACE;
+  unsigned char* p = reinterpret_cast<unsigned char*>(align256(reinterpret_cast<uintptr_t>(ws)));
+  A.delta = reinterpret_cast<float*>(p);
+  A.dpart = reinterpret_cast<float*>(p + align256(rows * 4));
+  const bool vec = aligned(a, true);
+  const int st =
+      a->dtype == FX_F32 ? bwd<float>(s, A, lanes_of(a), vec) : bwd<bf16>(s, A, lanes_of(a), vec);
+  if (st || !a->table) return st;
+  const int nb = a->buckets.num_buckets;
+  const dim3 grid((nb + 31) / 32, A.H);
+  const int64_t parts = a->batch * a->q_len;
+  if (a->dtype == FX_F32)
+    bias_finish_kernel<float><<<grid, 1024, 0, s>>>(A.dpart, static_cast<float*>(a->dtable), parts, nb);
+  else
+    bias_finish_kernel<bf16><<<grid, 1024, 0, s>>>(A.dpart, static_cast<bf16*>(a->dtable), parts, nb);
+  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+}
+
+}  // extern "C"
