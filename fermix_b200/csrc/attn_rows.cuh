@@ -35,6 +35,7 @@ struct AttnArgs {
   int64_t Lq, Lk;
   int64_t split_keys;
   int B, H, Hk, D, causal, splits;
+  uint32_t polls;  // of each bounded wait
   float scale2;  // scale log2 e
   float scale;
   BucketArgs buckets;
@@ -70,14 +71,16 @@ __device__ __forceinline__ int attn_k_pos(const AttnArgs& A, int b, int64_t j) {
   return A.k_pos ? A.k_pos[b * A.k_pos_stride + j] : (int)j;
 }
 
-// blockIdx.x: part of the keys, .y: rows chunk of a key head, .z: batch x key head
+// Blocks: parts of the keys, then chunks of the rows of a key head, then key heads, batches.
 template <typename T, int LPK, bool VECLOAD, int RC>
 __global__ void __launch_bounds__(kRowsThreads) attn_rows_kernel(const __grid_constant__ AttnArgs A) {
   constexpr int NE = 16 / sizeof(T), U = 4, GROUPS = kRowsThreads / LPK;
   extern __shared__ float lut[];  // RC x (2 reach + 1), then the joins
   const int G = A.H / A.Hk, reach = A.buckets.reach, span = 2 * reach + 1;
-  const int b = blockIdx.z / A.Hk, hk = blockIdx.z % A.Hk;
-  const int64_t rows = (int64_t)G * A.Lq, r0 = (int64_t)blockIdx.y * RC;
+  const int64_t rows = (int64_t)G * A.Lq, chunks = (rows + RC - 1) / RC;
+  const int part = blockIdx.x % A.splits;
+  const int64_t r0 = blockIdx.x / A.splits % chunks * RC, z = blockIdx.x / A.splits / chunks;
+  const int b = (int)(z / A.Hk), hk = (int)(z % A.Hk);
   const int group = threadIdx.x / LPK, gl = threadIdx.x % LPK, c0 = gl * NE;
 
   int qp[RC];
@@ -106,7 +109,7 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_kernel(const __grid_co
     }
   }
   __syncthreads();
-  const int64_t j0 = blockIdx.x * A.split_keys;
+  const int64_t j0 = part * A.split_keys;
   const int64_t j1 = j0 + A.split_keys < A.Lk ? j0 + A.split_keys : A.Lk;
   const T* K = static_cast<const T*>(A.k) + b * A.ks[0] + hk * A.ks[1];
   const T* V = static_cast<const T*>(A.v) + b * A.vs[0] + hk * A.vs[1];
@@ -184,7 +187,7 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_kernel(const __grid_co
       acc = fmaf(so[(g * RC + r) * LPK * NE + c], f, acc);
     }
     if (A.splits > 1) {
-      float* p = A.part + (((int64_t)blockIdx.z * rows + row) * A.splits + blockIdx.x) * (A.D + 2);
+      float* p = A.part + ((z * rows + row) * A.splits + part) * (A.D + 2);
       p[2 + c] = acc;
       if (c == 0) {
         p[0] = top;

@@ -36,9 +36,9 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_grad_kernel(const __gr
   constexpr int NE = 16 / sizeof(T), GROUPS = kRowsThreads / LPK;
   extern __shared__ float sm[];
   const int G = A.H / A.Hk, nb = A.buckets.num_buckets;
-  const int b = blockIdx.z / A.Hk, hk = blockIdx.z % A.Hk;
   const int64_t qrows = (int64_t)G * A.Lq, own = KEYS ? A.Lk : qrows, other = KEYS ? qrows : A.Lk;
-  const int64_t r0 = (int64_t)blockIdx.x * RC;
+  const int64_t chunks = (own + RC - 1) / RC, r0 = blockIdx.x % chunks * RC, z = blockIdx.x / chunks;
+  const int b = (int)(z / A.Hk), hk = (int)(z % A.Hk);
   const int group = threadIdx.x / LPK, gl = threadIdx.x % LPK, c0 = gl * NE;
   float* hist = sm;  // GROUPS x RC x nb x (a, b)
   if (!KEYS && A.table)

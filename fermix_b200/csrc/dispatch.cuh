@@ -43,10 +43,11 @@ int validate(int dtype, int prec, int64_t batch, int64_t n);
 uint32_t wait_polls();
 
 // Status word of one translation unit's kernels on the current device (0 or an FX_ERR_*
-// code), reset to 0 when clear; -1 if it cannot be read. Defined in launch_tc.cu and
-// launch_update.cu, the files whose kernels have bounded waits.
+// code), reset to 0 when clear; -1 if it cannot be read. Defined in launch_tc.cu,
+// launch_update.cu and launch_attn_tc.cu, the files whose kernels have bounded waits.
 int tc_status(int clear);
 int update_status(int clear);
+int attn_tc_status(int clear);
 
 inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 

@@ -1,7 +1,6 @@
 // Attention with the position bias: checks, choice of kernel, launch shapes, workspace.
-#include "attn_rows.cuh"
+#include "attn_host.cuh"
 #include "attn_rows_grad.cuh"
-#include "block_host.cuh"
 #include "position_bias.cuh"
 
 namespace {
@@ -19,7 +18,6 @@ int check(const fx_attn_args* a) {
     return FX_ERR_SHAPE;
   if (a->batch > (1 << 30) || a->heads > 65535 || a->q_len > (1 << 30) || a->k_len > (1 << 30)) return FX_ERR_SHAPE;
   if (a->heads > 0 && (a->kv_heads == 0 || a->heads % a->kv_heads)) return FX_ERR_SHAPE;
-  if (a->batch * a->kv_heads > 65535 || a->q_len * a->heads > (int64_t{65535} * kRC)) return FX_ERR_SHAPE;
   return a->table ? check_buckets(a->buckets) : FX_OK;
 }
 
@@ -64,6 +62,7 @@ AttnArgs make(const fx_attn_args* a) {
   A.causal = a->causal != 0;
   A.scale = a->scale;
   A.scale2 = a->scale * kLog2e;
+  A.polls = wait_polls();
   if (a->table) A.buckets = make_buckets(a->buckets);
   return A;
 }
@@ -82,6 +81,12 @@ bool aligned(const fx_attn_args* a, bool grad) {
   if (grad) add(a->dout, a->dout_stride);
   return m % 16 == 0;
 }
+
+// Rows of a key head (query heads that share it x queries) from which the tensor-core kernel
+// runs; below, the rows kernel splits the keys.
+constexpr int64_t kTcRows = 17;
+
+bool use_tc(const fx_attn_args* a) { return a->heads / a->kv_heads * a->q_len >= kTcRows; }
 
 // Lanes of a key: 16 bytes each, a power of two, eight at least.
 int lanes_of(const fx_attn_args* a) {
@@ -105,14 +110,6 @@ size_t part_bytes(const fx_attn_args* a, const AttnArgs& A) {
   return A.splits > 1 ? (size_t)(a->batch * a->heads * a->q_len) * A.splits * (a->dim + 2) * sizeof(float) + 256 : 0;
 }
 
-template <typename K>
-int raise_smem(K kern, size_t smem) {
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return FX_ERR_CUDA;
-  return FX_OK;
-}
-
 template <typename T, int LPK, bool VL>
 int launch_fwd(cudaStream_t s, const AttnArgs& A) {
   constexpr int NE = 16 / sizeof(T), GROUPS = kRowsThreads / LPK;
@@ -122,7 +119,9 @@ int launch_fwd(cudaStream_t s, const AttnArgs& A) {
   auto kern = attn_rows_kernel<T, LPK, VL, kRC>;
   if (raise_smem(kern, smem)) return FX_ERR_CUDA;
   const int64_t rows = (int64_t)(A.H / A.Hk) * A.Lq;
-  kern<<<dim3(A.splits, (unsigned)((rows + kRC - 1) / kRC), A.B * A.Hk), kRowsThreads, smem, s>>>(A);
+  const int64_t blocks = (rows + kRC - 1) / kRC * A.B * A.Hk * A.splits;
+  if (blocks > kMaxGrid) return FX_ERR_SHAPE;
+  kern<<<(unsigned)blocks, kRowsThreads, smem, s>>>(A);
   if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
   if (A.splits > 1) {
     attn_join_kernel<T><<<(unsigned)(((int64_t)A.B * A.H * A.Lq + 3) / 4), kRowsThreads, 0, s>>>(A);
@@ -141,11 +140,13 @@ int launch_bwd(cudaStream_t s, const AttnArgs& A) {
   auto kq = attn_rows_grad_kernel<T, LPK, VL, kRC, false>;
   auto kk = attn_rows_grad_kernel<T, LPK, VL, kRC, true>;
   if (raise_smem(kq, smem) || raise_smem(kk, join)) return FX_ERR_CUDA;
+  const int64_t qblocks = (qrows + kRC - 1) / kRC * A.B * A.Hk, kblocks = (A.Lk + kRC - 1) / kRC * A.B * A.Hk;
+  if (qblocks > kMaxGrid || kblocks > kMaxGrid || (int64_t)A.B * A.H * A.Lq > kMaxGrid) return FX_ERR_SHAPE;
   if (A.Lq > 0) {
     attn_delta_kernel<T><<<(unsigned)(((int64_t)A.B * A.H * A.Lq + 3) / 4), kRowsThreads, 0, s>>>(A);
-    kq<<<dim3((unsigned)((qrows + kRC - 1) / kRC), 1, A.B * A.Hk), kRowsThreads, smem, s>>>(A);
+    kq<<<(unsigned)qblocks, kRowsThreads, smem, s>>>(A);
   }
-  if (A.Lk > 0) kk<<<dim3((unsigned)((A.Lk + kRC - 1) / kRC), 1, A.B * A.Hk), kRowsThreads, join, s>>>(A);
+  if (A.Lk > 0) kk<<<(unsigned)kblocks, kRowsThreads, join, s>>>(A);
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
@@ -171,7 +172,7 @@ extern "C" {
 
 size_t fermix_biased_attention_workspace_bytes(const fx_attn_args* a) {
   const DevInfo* D = dev_info();
-  if (check(a) || !D || no_rows(a)) return 0;
+  if (check(a) || !D || no_rows(a) || use_tc(a)) return 0;
   AttnArgs A{};
   split_keys(a, D->sms, A);
   return part_bytes(a, A);
@@ -185,14 +186,15 @@ int fermix_biased_attention(void* stream, const fx_attn_args* a, void* ws, size_
   const DevInfo* D = dev_info();
   if (!D) return FX_ERR_DEVICE;
   AttnArgs A = make(a);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool vec = aligned(a, false);
+  if (use_tc(a)) return launch_attn_tc_fwd(s, A, a->dtype == FX_F32, vec);
   split_keys(a, D->sms, A);
   const size_t need = part_bytes(a, A);
   if (need) {
     if (!ws || wsb < need) return FX_ERR_WORKSPACE;
     A.part = reinterpret_cast<float*>(align256(reinterpret_cast<uintptr_t>(ws)));
   }
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool vec = aligned(a, false);
   return a->dtype == FX_F32 ? fwd<float>(s, A, lanes_of(a), vec) : fwd<bf16>(s, A, lanes_of(a), vec);
 }
 
