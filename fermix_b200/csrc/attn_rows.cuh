@@ -30,7 +30,8 @@ struct AttnArgs {
   void *dq, *dk, *dv;
   int64_t dqs[3], dks[3], dvs[3];
   float* delta;   // (batch, heads, q_len)
-  float* dpart;   // partial table gradients
+  float* dpart;   // partial table gradients (heads, parts, num_buckets)
+  float* lut;     // table by distance, base 2 (heads, 2 reach + 1)
   float* part;    // split parts: (rows, splits, dim + 2)
   int64_t Lq, Lk;
   int64_t split_keys;

@@ -228,9 +228,9 @@ struct alignas(16) TileInfo {  // positions are read four at a time
   uint32_t live[R / kSub];
 };
 
-// Entries [sub * 32, sub * 32 + 32) of the tile at index j0, by one warp.
+// Entries [sub * 32, sub * 32 + 32) of the tile, by one warp; returns the live ones' bits.
 template <int R, typename Live, typename Pos>
-__device__ __forceinline__ void fill_info(TileInfo<R>& I, int sub, Live live, Pos pos) {
+__device__ __forceinline__ uint32_t fill_info(TileInfo<R>& I, int sub, Live live, Pos pos) {
   const int lane = threadIdx.x & 31, e = sub * kSub + lane;
   const bool ok = live(e);
   const int x = ok ? pos(e) : 0;
@@ -243,6 +243,7 @@ __device__ __forceinline__ void fill_info(TileInfo<R>& I, int sub, Live live, Po
     I.hi[sub] = hi;
     I.live[sub] = bits;
   }
+  return bits;
 }
 
 // ---------------------------------------------------------------- forward

@@ -1,0 +1,600 @@
+// Gradient of the biased attention on the tensor cores, in three launches: the rows' products
+// delta = o . do and the table by distance (attn_prep_kernel), then dk and dv by blocks of keys
+// (attn_dkv_kernel) and dq and the table's gradient by blocks of queries (attn_dq_kernel). Each block
+// owns what it writes, so nothing is added atomically; the scores are formed twice for that
+// (seven products instead of five).
+//
+//   p = 2^(scale2 q.k + bias2 - lse),  ds = p (do.v - delta)
+//   dv = p^T do, dk = scale ds^T q, dq = scale ds k
+//
+// In both, a thread holds one row of the 128-row block (TMEM lane), p and ds go back to TMEM as
+// the A operand of the second products, and the 64-row tiles of the other side stream through
+// shared memory, each read K-major for the scores and MN-major for the second product.
+#pragma once
+#include "attn_tc.cuh"
+
+namespace fx {
+namespace tc {
+
+constexpr int kGradN = 64;  // rows of a streamed tile
+
+// delta of every query row (LPR lanes a row), and the blocks past them: the table by distance
+// in base 2, lut[h, d + reach].
+template <typename T, int LPR, bool VEC>
+__global__ void __launch_bounds__(256) attn_prep_kernel(const __grid_constant__ AttnArgs A, int64_t row_blocks) {
+  constexpr int NE = 16 / sizeof(T);
+  if ((int64_t)blockIdx.x >= row_blocks) {
+    const int span = 2 * A.buckets.reach + 1, nb = A.buckets.num_buckets;
+    const int64_t i = ((int64_t)blockIdx.x - row_blocks) * 256 + threadIdx.x;
+    if (i < (int64_t)A.H * span)
+      A.lut[i] =
+          bias2(to_f(static_cast<const T*>(A.table)[i / span * nb + bucket_of(A.buckets, (int)(i % span) - A.buckets.reach)]));
+    return;
+  }
+  const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const bool there = row < (int64_t)A.B * A.H * A.Lq;
+  float s = 0.f;
+  if (there) {
+    const int64_t i = row % A.Lq, bh = row / A.Lq, h = bh % A.H, b = bh / A.H;
+    float x[NE], y[NE];
+    load_entries<T, NE, VEC>(static_cast<const T*>(A.out) + b * A.os[0] + h * A.os[1] + i * A.os[2],
+                             threadIdx.x % LPR * NE, A.D, x);
+    load_entries<T, NE, VEC>(static_cast<const T*>(A.dout) + b * A.dos[0] + h * A.dos[1] + i * A.dos[2],
+                             threadIdx.x % LPR * NE, A.D, y);
+#pragma unroll
+    for (int e = 0; e < NE; ++e) s = fmaf(x[e], y[e], s);
+  }
+  s = lanes_sum(s, LPR);
+  if (there && threadIdx.x % LPR == 0) A.delta[row] = s;
+}
+
+// Row r of the block from TMEM (columns col ..), times f, to p (zero: 0).
+template <typename T, int DC>
+__device__ __forceinline__ void store_row(uint32_t taddr, T* p, int64_t step, int dim, float f, bool zero, bool valid) {
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = dim % V == 0 && ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(step * sizeof(T))) & 15) == 0;
+#pragma unroll
+  for (int c = 0; c < 64 * DC; c += 16) {
+    if (c < dim) {
+      uint32_t o[16];
+      ld16(taddr + c, o);
+      tmem_wait_ld();
+      alignas(16) T r[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) r[e] = from_f<T>(zero ? 0.f : __uint_as_float(o[e]) * f);
+      if (valid) {
+        if (vec) {
+#pragma unroll
+          for (int e = 0; e < 16; e += V)
+            if (c + e < dim) *reinterpret_cast<Pack<T, V>*>(p + c + e) = *reinterpret_cast<Pack<T, V>*>(r + e);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (c + e < dim) p[c + e] = r[e];
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- dk, dv
+template <int NS, int DC, int ST>
+struct DkvShape {
+  static constexpr int kThreads = 384;  // 8 warps on the scores, one issuing, three loading
+  static constexpr uint32_t kOwn = NS * DC * 16384u, kTile = NS * DC * kGradN * 128u;
+  static constexpr uint32_t kTileBytes = 2 * kOwn + 2 * ST * kTile;
+  // TMEM: scores, do.v, [p, ds: NS parts of 32 columns], dv, dk. With one part p and ds take the
+  // place of the scores: each half of the columns in the place of its own half.
+  static constexpr int kDp = kGradN, kP = NS == 1 ? 0 : 2 * kGradN, kDs = NS == 1 ? kGradN : kP + NS * 32;
+  static constexpr int kDv = NS == 1 ? 2 * kGradN : kDs + NS * 32, kDk = kDv + 64 * DC;
+  static constexpr int kCols = kDk + 64 * DC, kAlloc = kCols <= 256 ? 256 : 512;
+  static constexpr int kInfo = ST + 1;
+};
+
+struct alignas(16) QueryInfo {
+  TileInfo<kGradN> t;
+  float lse[kGradN], delta[kGradN];  // lse +inf: a row without keys, or past the end
+};
+
+template <typename T, int NS, int DC, int ST, bool VEC>
+__global__ void __launch_bounds__(DkvShape<NS, DC, ST>::kThreads, NS == 1 && DC == 1 ? 2 : 1)
+    attn_dkv_kernel(const __grid_constant__ AttnArgs A) {
+  using S = DkvShape<NS, DC, ST>;
+  constexpr bool ASYNC = NS == 1 && VEC && sizeof(T) == 2;
+  static_assert(!ASYNC || ST >= 2, "a tile's arrival is told after the next one's issue");
+  extern __shared__ unsigned char raw[];
+  unsigned char* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  unsigned char *sK = sm, *sV = sm + S::kOwn, *sQ = sV + S::kOwn, *sO = sQ + ST * S::kTile;
+  float* lut = reinterpret_cast<float*>(sm + S::kTileBytes);
+  __shared__ QueryInfo info[S::kInfo];
+  __shared__ uint64_t full[ST], empty[ST], sfull, pfull, done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = A.H / A.Hk;
+
+  // key blocks slow, longest first under a causal order
+  const int64_t heads = (int64_t)A.B * A.Hk, nk = (A.Lk + 127) / 128;
+  const bool ordered = A.causal && !A.q_pos && !A.k_pos;
+  const int64_t kb = ordered ? blockIdx.x / heads : blockIdx.x % nk;
+  const int64_t bh = ordered ? blockIdx.x % heads : blockIdx.x / nk;
+  const int b = (int)(bh / A.Hk), hk = (int)(bh % A.Hk);
+  const int64_t j0 = kb * 128;
+  const uint8_t* mask = A.mask ? A.mask + b * A.mask_stride : nullptr;
+  const int reach = A.buckets.reach, span = 2 * reach + 1;
+
+  if (tid == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&full[i], 96);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(&sfull, 1);
+    mbar_init(&pfull, 256);
+    mbar_init(&done, 1);
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&tmem_slot, S::kAlloc);
+    tmem_relinquish();
+  }
+  const T* K = static_cast<const T*>(A.k) + b * A.ks[0] + hk * A.ks[1] + j0 * A.ks[2];
+  const T* V = static_cast<const T*>(A.v) + b * A.vs[0] + hk * A.vs[1] + j0 * A.vs[2];
+  const auto key_live = [&](int r) { return j0 + r < A.Lk && (!mask || mask[j0 + r]); };
+  load_tile<T, NS, VEC, 128>(sK, K, A.ks[2], A.D, DC, tid, S::kThreads, key_live);
+  load_tile<T, NS, VEC, 128>(sV, V, A.vs[2], A.D, DC, tid, S::kThreads, key_live);
+  cp_commit();
+  cp_wait<0>();
+  fence_proxy_async_smem();
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = tmem_slot, polls = A.polls;
+  const int64_t nq = (A.Lq + kGradN - 1) / kGradN;
+  int64_t q0 = 0;  // the first query tile that sees a key of this block
+  if (ordered) {
+    const int64_t i = j0 - (A.Lk - A.Lq);
+    q0 = i > 0 ? i / kGradN : 0;
+    if (q0 > nq) q0 = nq;
+  }
+  const int64_t per = nq - q0, tiles = per * G;
+
+  if (warp < 8) {
+    const int wg = warp >> 2, r = tid & 127;
+    const int64_t j = j0 + r;
+    const bool live = key_live(r);
+    const int kp = live ? attn_k_pos(A, b, j) : 0;
+    const int klo = __reduce_min_sync(0xffffffffu, live ? kp : INT32_MAX);
+    const int khi = __reduce_max_sync(0xffffffffu, live ? kp : INT32_MIN);
+    const uint32_t base = tmem + ((uint32_t)(warp & 3) << 21);
+    for (int64_t it = 0; it < tiles; ++it) {
+      if (A.table && it % per == 0) {  // the next head's table
+        named_barrier(2, 256);
+        const float* src = A.lut + (int64_t)(hk * G + it / per) * span;
+        for (int d = tid; d < span; d += 256) lut[d] = src[d];
+        named_barrier(2, 256);
+      }
+      const QueryInfo& I = info[it % S::kInfo];
+      wait(&sfull, it & 1, &abort_flag, polls);
+      fence_after_sync();
+      const int qlo = I.t.lo[wg], qhi = I.t.hi[wg];
+      const bool some = I.t.live[wg] != 0 && klo <= khi;
+      const bool above = (int64_t)klo - qhi >= reach, below = (int64_t)khi - qlo <= -reach;
+      const bool each = some && ((A.table && !above && !below) || (A.causal && khi > qlo));
+      const float flat = A.table && some && !each ? lut[above ? 2 * reach : 0] : 0.f;
+#pragma unroll
+      for (int c = 0; c < 32; c += 16) {
+        const int col = wg * 32 + c;
+        uint32_t s[16], dp[16];
+        ld16(base + col, s);
+        ld16(base + S::kDp + col, dp);
+        tmem_wait_ld();
+        uint32_t wp[NS][8], wd[NS][8];
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const float4 ls = *reinterpret_cast<const float4*>(&I.lse[col + e]);
+          const float4 de = *reinterpret_cast<const float4*>(&I.delta[col + e]);
+          const float l4[4] = {ls.x, ls.y, ls.z, ls.w}, d4[4] = {de.x, de.y, de.z, de.w};
+          float p[4], ds[4];
+          if (each) {
+            const int4 qp = *reinterpret_cast<const int4*>(&I.t.pos[col + e]);
+            const int q4[4] = {qp.x, qp.y, qp.z, qp.w};
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+              const int d = kp - q4[f];
+              const float bias = A.table ? lut[clamp_reach(d, reach) + reach] : 0.f;
+              p[f] = ex2(fmaf(__uint_as_float(s[e + f]), A.scale2, bias - l4[f]));
+              if (A.causal && d > 0) p[f] = 0.f;
+            }
+          } else {
+#pragma unroll
+            for (int f = 0; f < 4; ++f) p[f] = ex2(fmaf(__uint_as_float(s[e + f]), A.scale2, flat - l4[f]));
+          }
+#pragma unroll
+          for (int f = 0; f < 4; ++f) ds[f] = p[f] * (__uint_as_float(dp[e + f]) - d4[f]);
+#pragma unroll
+          for (int f = 0; f < 4; f += 2) {
+            uint32_t o[NS];
+            split2<NS>(p[f], p[f + 1], o);
+#pragma unroll
+            for (int i = 0; i < NS; ++i) wp[i][(e + f) / 2] = o[i];
+            split2<NS>(ds[f], ds[f + 1], o);
+#pragma unroll
+            for (int i = 0; i < NS; ++i) wd[i][(e + f) / 2] = o[i];
+          }
+        }
+        const uint32_t at = NS == 1 ? col - c + c / 2 : col / 2;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          st8(base + S::kP + i * 32 + at, wp[i]);
+          st8(base + S::kDs + i * 32 + at, wd[i]);
+        }
+      }
+      tmem_wait_st();
+      fence_before_sync();
+      arrive(&pfull);
+    }
+    if (tiles > 0) {
+      wait(&sfull, tiles & 1, &abort_flag, polls);
+      fence_after_sync();
+    }
+    const bool zero = !live || tiles == 0, valid = j < A.Lk;
+    const float f = abort_flag ? NAN : 1.f;
+    if (wg == 0)
+      store_row<T, DC>(base + S::kDv, static_cast<T*>(A.dv) + b * A.dvs[0] + hk * A.dvs[1] + j * A.dvs[2], A.dvs[2], A.D,
+                       f, zero, valid);
+    else
+      store_row<T, DC>(base + S::kDk, static_cast<T*>(A.dk) + b * A.dks[0] + hk * A.dks[1] + j * A.dks[2], A.dks[2], A.D,
+                       f * A.scale, zero, valid);
+  } else if (warp == 8) {
+    if (lane == 0 && tiles > 0) {
+      const uint32_t id_s = idesc_bf16(128, kGradN, false), id_o = idesc_bf16(128, (A.D + 15) / 16 * 16, true);
+      const uint32_t aK = smem_u32(sK), aV = smem_u32(sV);
+      const auto acol = [](int k) { return NS == 1 ? (k >> 1) * 32 + (k & 1) * 8 : k * 8; };
+      for (int64_t it = 0; it < tiles; ++it) {
+        const int st = (int)(it % ST);
+        const uint32_t aQ = smem_u32(sQ) + st * S::kTile, aO = smem_u32(sO) + st * S::kTile;
+        wait(&full[st], (it / ST) & 1, &abort_flag, polls);
+        scores<NS, 128, kGradN>(tmem, aK, aQ, A.D, DC, id_s);
+        scores<NS, 128, kGradN>(tmem + S::kDp, aV, aO, A.D, DC, id_s);
+        mma_commit(&sfull);
+        wait(&pfull, it & 1, &abort_flag, polls);
+        fence_after_sync();
+        values<NS, kGradN>(tmem + S::kDv, tmem + S::kP, 32, aO, DC, id_o, it > 0, acol);
+        values<NS, kGradN>(tmem + S::kDk, tmem + S::kDs, 32, aQ, DC, id_o, it > 0, acol);
+        mma_commit(&empty[st]);
+      }
+      mma_commit(&sfull);
+      if (abort_flag) {  // nothing may be in flight when the TMEM is freed
+        mma_commit(&done);
+        mbar_wait(&done, 0, polls);
+      }
+    }
+  } else {
+    const int t = tid - 288, w = t >> 5;
+    for (int64_t it = 0; it < tiles; ++it) {
+      const int st = (int)(it % ST), h = (int)(hk * G + it / per);
+      const int64_t i0 = (q0 + it % per) * kGradN;
+      QueryInfo& I = info[it % S::kInfo];
+      if (it >= ST) wait(&empty[st], (it / ST - 1) & 1, &abort_flag, polls);
+      const float* lse = A.lse + ((int64_t)b * A.H + h) * A.Lq;
+      const float* delta = A.delta + ((int64_t)b * A.H + h) * A.Lq;
+      if (w < kGradN / kSub) {
+        const uint32_t bits = fill_info<kGradN>(
+            I.t, w, [&](int e) { return i0 + e < A.Lq && lse[i0 + e] != -INFINITY; },
+            [&](int e) { return attn_q_pos(A, b, i0 + e); });
+        const int e = w * kSub + lane;
+        const bool ok = (bits >> lane) & 1u;
+        I.lse[e] = ok ? lse[i0 + e] : INFINITY;
+        I.delta[e] = ok ? delta[i0 + e] : 0.f;
+      }
+      named_barrier(1, 96);
+      const auto row_live = [&](int r) { return (I.t.live[r >> 5] >> (r & 31)) & 1u; };
+      load_tile<T, NS, VEC, kGradN>(
+          sQ + st * S::kTile, static_cast<const T*>(A.q) + b * A.qs[0] + h * A.qs[1] + i0 * A.qs[2], A.qs[2], A.D, DC, t,
+          96, row_live);
+      load_tile<T, NS, VEC, kGradN>(
+          sO + st * S::kTile, static_cast<const T*>(A.dout) + b * A.dos[0] + h * A.dos[1] + i0 * A.dos[2], A.dos[2], A.D,
+          DC, t, 96, row_live);
+      if constexpr (ASYNC) {
+        cp_commit();
+        if (it > 0) {
+          cp_wait<1>();
+          fence_proxy_async_smem();
+          arrive(&full[(it - 1) % ST]);
+        }
+        if (it + 1 < tiles) continue;
+        cp_wait<0>();
+      }
+      fence_proxy_async_smem();
+      arrive(&full[st]);
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  if (warp == 0) tmem_dealloc(tmem, S::kAlloc);
+}
+
+// ---------------------------------------------------------------- dq, dtable
+template <int NS, int DC, int ST>
+struct DqShape {
+  static constexpr int kThreads = 256;  // 4 warps on the scores, one issuing, three loading
+  static constexpr uint32_t kOwn = NS * DC * 16384u, kTile = NS * DC * kGradN * 128u;
+  static constexpr uint32_t kTileBytes = 2 * kOwn + 2 * ST * kTile;
+  // TMEM: scores, do.v, [ds: NS parts], dq. With one part ds follows the reads over the scores.
+  static constexpr int kDp = kGradN, kDs = NS == 1 ? 0 : 2 * kGradN, kDq = NS == 1 ? 2 * kGradN : kDs + NS * 32;
+  static constexpr int kCols = kDq + 64 * DC, kAlloc = kCols <= 256 ? 256 : 512;
+  static constexpr int kInfo = ST + 1;
+};
+
+// The table's gradient: a row's ds sum to 0, and a bucket that holds all of a row's keys gets
+// nothing from it. delta from the rounded output would leave its rounding there. So each
+// thread keeps a = sum p (do.v) and b = sum p of its row by bucket, in columns of its own in
+// shared memory (beyond the reach in registers), and the row gives a - b (sum a / sum b). Tables
+// of more than kWindow buckets take a launch for every kWindow of them.
+constexpr int kWindow = 64;
+
+template <typename T, int NS, int DC, int ST, bool VEC>
+__global__ void __launch_bounds__(DqShape<NS, DC, ST>::kThreads, NS == 1 && DC == 1 ? 2 : 1)
+    attn_dq_kernel(const __grid_constant__ AttnArgs A, int w0, int wn) {
+  using S = DqShape<NS, DC, ST>;
+  constexpr bool ASYNC = NS == 1 && VEC && sizeof(T) == 2;
+  static_assert(!ASYNC || ST >= 2, "a tile's arrival is told after the next one's issue");
+  extern __shared__ unsigned char raw[];
+  unsigned char* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  unsigned char *sQ = sm, *sO = sm + S::kOwn, *sK = sO + S::kOwn, *sV = sK + ST * S::kTile;
+  float2* hist = reinterpret_cast<float2*>(sm + S::kTileBytes);  // wn x 128 (a, b)
+  int2* lut = reinterpret_cast<int2*>(hist + wn * 128);           // (bias, column of its bucket or -1)
+  __shared__ TileInfo<kGradN> info[S::kInfo];
+  __shared__ uint64_t full[ST], empty[ST], sfull, pfull, done;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  __shared__ int last_live;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  const int64_t heads = (int64_t)A.B * A.H, nq = (A.Lq + 127) / 128;
+  const bool ordered = A.causal && !A.q_pos && !A.k_pos;
+  const int64_t qb = ordered ? nq - 1 - blockIdx.x / heads : blockIdx.x % nq;
+  const int64_t bh = ordered ? blockIdx.x % heads : blockIdx.x / nq;
+  const int b = (int)(bh / A.H), h = (int)(bh % A.H), hk = h / (A.H / A.Hk);
+  const int64_t i0 = qb * 128;
+  const uint8_t* mask = A.mask ? A.mask + b * A.mask_stride : nullptr;
+  const int reach = A.buckets.reach, span = 2 * reach + 1;
+  const float* lse = A.lse + bh * A.Lq;
+
+  if (tid == 0) {
+    abort_flag = 0;
+    last_live = mask ? 0 : (int)A.Lk;
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&full[i], 96);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(&sfull, 1);
+    mbar_init(&pfull, 128);
+    mbar_init(&done, 1);
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&tmem_slot, S::kAlloc);
+    tmem_relinquish();
+  }
+  const auto row_live = [&](int r) { return i0 + r < A.Lq && lse[i0 + r] != -INFINITY; };
+  load_tile<T, NS, VEC, 128>(sQ, static_cast<const T*>(A.q) + b * A.qs[0] + h * A.qs[1] + i0 * A.qs[2], A.qs[2], A.D, DC,
+                             tid, S::kThreads, row_live);
+  load_tile<T, NS, VEC, 128>(sO, static_cast<const T*>(A.dout) + b * A.dos[0] + h * A.dos[1] + i0 * A.dos[2], A.dos[2],
+                             A.D, DC, tid, S::kThreads, row_live);
+  if (A.table) {
+    for (int d = tid; d < span; d += S::kThreads) {
+      const int c = bucket_of(A.buckets, d - reach) - w0;
+      lut[d] = make_int2(__float_as_int(A.lut[(int64_t)h * span + d]), c >= 0 && c < wn ? c * 128 : -1);
+    }
+    for (int i = tid; i < wn * 128; i += S::kThreads) hist[i] = make_float2(0.f, 0.f);
+  }
+  cp_commit();
+  cp_wait<0>();
+  fence_proxy_async_smem();
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  if (mask) {  // the keys after the last live one are not visited
+    int last = 0;
+    for (int j = tid; j < (int)A.Lk; j += S::kThreads)
+      if (mask[j]) last = j + 1;
+    if (last) atomicMax(&last_live, last);
+    __syncthreads();
+  }
+  int64_t keys = last_live;
+  if (ordered) {
+    const int64_t end = i0 + 128 < A.Lq ? i0 + 128 : A.Lq, seen = A.Lk - A.Lq + end;
+    keys = seen < keys ? (seen > 0 ? seen : 0) : keys;
+  }
+  const int tiles = (int)((keys + kGradN - 1) / kGradN);
+  const uint32_t tmem = tmem_slot, polls = A.polls;
+
+  if (warp < 4) {
+    const int64_t i = i0 + tid;
+    const bool valid = i < A.Lq, live = row_live(tid);
+    const int qp = live ? attn_q_pos(A, b, i) : 0;
+    const float L = live ? lse[i] : INFINITY, delta = live ? A.delta[bh * A.Lq + i] : 0.f;
+    const int qlo = __reduce_min_sync(0xffffffffu, live ? qp : INT32_MAX);
+    const int qhi = __reduce_max_sync(0xffffffffu, live ? qp : INT32_MIN);
+    const uint32_t base = tmem + ((uint32_t)(warp & 3) << 21);
+    float2* mine = hist + tid;
+    float ta = 0.f, tb = 0.f;                      // all of the row
+    float ha = 0.f, hb = 0.f, la = 0.f, lb = 0.f;  // beyond the reach, above and below
+    const bool windows = A.table && wn < A.buckets.num_buckets;
+    for (int j = 0; j < tiles; ++j) {
+      const TileInfo<kGradN>& I = info[j % S::kInfo];
+      wait(&sfull, j & 1, &abort_flag, polls);
+      fence_after_sync();
+#pragma unroll
+      for (int c = 0; c < kGradN; c += 16) {
+        const int sub = c / kSub;
+        const uint32_t bits = I.live[sub] >> (c % kSub);
+        const int klo = I.lo[sub], khi = I.hi[sub];
+        const bool some = I.live[sub] != 0 && qlo <= qhi;
+        const bool above = (int64_t)klo - qhi >= reach, below = (int64_t)khi - qlo <= -reach;
+        const bool near = some && A.table && !above && !below, later = some && A.causal && khi > qlo;
+        uint32_t s[16], dp[16], wd[NS][8];
+        ld16(base + c, s);
+        ld16(base + S::kDp + c, dp);
+        tmem_wait_ld();
+        if (near || later) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const int4 kp = *reinterpret_cast<const int4*>(&I.pos[c + e]);
+            const int k4[4] = {kp.x, kp.y, kp.z, kp.w};
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+              const int d = k4[f] - qp;
+              int2 t = make_int2(0, -1);
+              if (A.table) t = lut[clamp_reach(d, reach) + reach];
+              float p = ex2(fmaf(__uint_as_float(s[e + f]), A.scale2, __int_as_float(t.x) - L));
+              if ((A.causal && d > 0) || !((bits >> (e + f)) & 1u)) p = 0.f;
+              const float x = __uint_as_float(dp[e + f]), px = p * x;
+              if (t.y >= 0) {
+                float2 v = mine[t.y];
+                v.x += px;
+                v.y += p;
+                mine[t.y] = v;
+              }
+              ta += px;
+              tb += p;
+              s[e + f] = __float_as_uint(p * (x - delta));
+            }
+          }
+        } else {
+          const float flat = (A.table && some ? __int_as_float(lut[above ? 2 * reach : 0].x) : 0.f) - L;
+          float sa = 0.f, sb = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float p = ex2(fmaf(__uint_as_float(s[e]), A.scale2, flat));
+            if (!((bits >> e) & 1u)) p = 0.f;
+            const float x = __uint_as_float(dp[e]);
+            sa = fmaf(p, x, sa);
+            sb += p;
+            s[e] = __float_as_uint(p * (x - delta));
+          }
+          if (above) {
+            ha += sa;
+            hb += sb;
+          } else {
+            la += sa;
+            lb += sb;
+          }
+          ta += sa;
+          tb += sb;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          uint32_t o[NS];
+          split2<NS>(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1]), o);
+#pragma unroll
+          for (int n = 0; n < NS; ++n) wd[n][e] = o[n];
+        }
+#pragma unroll
+        for (int n = 0; n < NS; ++n) st8(base + S::kDs + n * 32 + c / 2, wd[n]);
+      }
+      tmem_wait_st();
+      fence_before_sync();
+      arrive(&pfull);
+    }
+    if (tiles > 0) {
+      wait(&sfull, tiles & 1, &abort_flag, polls);
+      fence_after_sync();
+    }
+    const float broken = abort_flag ? NAN : 0.f;
+    if (w0 == 0)
+      store_row<T, DC>(base + S::kDq, static_cast<T*>(A.dq) + b * A.dqs[0] + h * A.dqs[1] + i * A.dqs[2], A.dqs[2], A.D,
+                       A.scale + broken, !live || tiles == 0, valid);
+    if (A.table) {
+      const int hi = lut[2 * reach].y, lo = lut[0].y;
+      if (hi >= 0) {
+        mine[hi].x += ha;
+        mine[hi].y += hb;
+      }
+      if (lo >= 0) {
+        mine[lo].x += la;
+        mine[lo].y += lb;
+      }
+      if (!windows) {
+        ta = tb = 0.f;
+        for (int c = 0; c < wn; ++c) {
+          ta += mine[c * 128].x;
+          tb += mine[c * 128].y;
+        }
+      }
+      const float mean = live && tb != 0.f ? ta / tb : 0.f;
+      for (int c = 0; c < wn; ++c) {
+        const float2 v = mine[c * 128];
+        mine[c * 128].x = live ? fmaf(-v.y, mean, v.x) + broken : 0.f;
+      }
+      named_barrier(2, 128);
+      float* part = A.dpart + (((int64_t)h * A.B + b) * nq + qb) * A.buckets.num_buckets + w0;
+      for (int c = warp; c < wn; c += 4) {
+        const float2* r = hist + c * 128 + lane;
+        const float v = lanes_sum((r[0].x + r[32].x) + (r[64].x + r[96].x), 32);
+        if (lane == 0) part[c] = v;
+      }
+    }
+  } else if (warp == 4) {
+    if (lane == 0 && tiles > 0) {
+      const uint32_t id_s = idesc_bf16(128, kGradN, false), id_o = idesc_bf16(128, (A.D + 15) / 16 * 16, true);
+      const uint32_t aQ = smem_u32(sQ), aO = smem_u32(sO);
+      for (int j = 0; j < tiles; ++j) {
+        const int st = j % ST;
+        const uint32_t aK = smem_u32(sK) + st * S::kTile, aV = smem_u32(sV) + st * S::kTile;
+        wait(&full[st], (j / ST) & 1, &abort_flag, polls);
+        scores<NS, 128, kGradN>(tmem, aQ, aK, A.D, DC, id_s);
+        scores<NS, 128, kGradN>(tmem + S::kDp, aO, aV, A.D, DC, id_s);
+        mma_commit(&sfull);
+        wait(&pfull, j & 1, &abort_flag, polls);
+        fence_after_sync();
+        values<NS, kGradN>(tmem + S::kDq, tmem + S::kDs, 32, aK, DC, id_o, j > 0, [](int k) { return k * 8; });
+        mma_commit(&empty[st]);
+      }
+      mma_commit(&sfull);
+      if (abort_flag) {  // nothing may be in flight when the TMEM is freed
+        mma_commit(&done);
+        mbar_wait(&done, 0, polls);
+      }
+    }
+  } else {
+    const int t = tid - 160, w = t >> 5;
+    const T* K = static_cast<const T*>(A.k) + b * A.ks[0] + hk * A.ks[1];
+    const T* V = static_cast<const T*>(A.v) + b * A.vs[0] + hk * A.vs[1];
+    for (int j = 0; j < tiles; ++j) {
+      const int st = j % ST;
+      const int64_t j0 = (int64_t)j * kGradN;
+      TileInfo<kGradN>& I = info[j % S::kInfo];
+      if (j >= ST) wait(&empty[st], (j / ST - 1) & 1, &abort_flag, polls);
+      if (w < kGradN / kSub)
+        fill_info<kGradN>(
+            I, w, [&](int e) { return j0 + e < A.Lk && (!mask || mask[j0 + e]); },
+            [&](int e) { return attn_k_pos(A, b, j0 + e); });
+      named_barrier(1, 96);
+      const auto live = [&](int r) { return (I.live[r >> 5] >> (r & 31)) & 1u; };
+      load_tile<T, NS, VEC, kGradN>(sK + st * S::kTile, K + j0 * A.ks[2], A.ks[2], A.D, DC, t, 96, live);
+      load_tile<T, NS, VEC, kGradN>(sV + st * S::kTile, V + j0 * A.vs[2], A.vs[2], A.D, DC, t, 96, live);
+      if constexpr (ASYNC) {
+        cp_commit();
+        if (j > 0) {
+          cp_wait<1>();
+          fence_proxy_async_smem();
+          arrive(&full[(j - 1) % ST]);
+        }
+        if (j + 1 < tiles) continue;
+        cp_wait<0>();
+      }
+      fence_proxy_async_smem();
+      arrive(&full[st]);
+    }
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  if (warp == 0) tmem_dealloc(tmem, S::kAlloc);
+}
+
+}  // namespace tc
+}  // namespace fx

@@ -78,7 +78,10 @@ bool aligned(const fx_attn_args* a, bool grad) {
   add(a->q, a->q_stride);
   add(a->k, a->k_stride);
   add(a->v, a->v_stride);
-  if (grad) add(a->dout, a->dout_stride);
+  if (grad) {
+    add(a->dout, a->dout_stride);
+    add(a->out, a->out_stride);
+  }
   return m % 16 == 0;
 }
 
@@ -166,6 +169,26 @@ int bwd(cudaStream_t s, const AttnArgs& A, int lanes, bool vec) {
   return FX_ERR_SHAPE;
 }
 
+// The tensor-core gradient holds both sides of a block in shared memory: float32's three parts
+// fit to a head dimension of 64.
+bool use_tc_grad(const fx_attn_args* a) { return a->dtype != FX_F32 || a->dim <= 64; }
+
+struct GradWorkspace {
+  size_t lut, dpart, total;  // offsets behind delta
+  int64_t parts;
+};
+
+GradWorkspace grad_workspace(const fx_attn_args* a) {
+  GradWorkspace w;
+  const size_t rows = (size_t)(a->batch * a->heads * a->q_len);
+  w.parts = a->batch * (use_tc_grad(a) ? (a->q_len + 127) / 128 : a->q_len);
+  const int reach = a->table ? make_buckets(a->buckets).reach : 0;
+  w.lut = align256(rows * 4);
+  w.dpart = w.lut + (a->table ? align256((size_t)a->heads * (2 * reach + 1) * 4) : 0);
+  w.total = w.dpart + (a->table ? (size_t)a->heads * w.parts * a->buckets.num_buckets * 4 : 0) + 256;
+  return w;
+}
+
 }  // namespace
 
 extern "C" {
@@ -200,8 +223,7 @@ int fermix_biased_attention(void* stream, const fx_attn_args* a, void* ws, size_
 
 size_t fermix_biased_attention_grad_workspace_bytes(const fx_attn_args* a) {
   if (check(a) || no_rows(a)) return 0;
-  const size_t rows = (size_t)(a->batch * a->heads * a->q_len);
-  return align256(rows * 4) + (a->table ? align256(rows * a->buckets.num_buckets * 4) : 0) + 256;
+  return grad_workspace(a).total;
 }
 
 int fermix_biased_attention_grad(void* stream, const fx_attn_args* a, void* ws, size_t wsb) {
@@ -223,19 +245,21 @@ int fermix_biased_attention_grad(void* stream, const fx_attn_args* a, void* ws, 
   const DevInfo* D = dev_info();
   if (!D) return FX_ERR_DEVICE;
   AttnArgs A = make(a);
-  const size_t rows = (size_t)(a->batch * a->heads * a->q_len);
-  const size_t need = fermix_biased_attention_grad_workspace_bytes(a);
-  if (need && (!ws || wsb < need)) return FX_ERR_WORKSPACE;
+  const GradWorkspace w = grad_workspace(a);
+  if (!no_rows(a) && (!ws || wsb < w.total)) return FX_ERR_WORKSPACE;
   unsigned char* p = reinterpret_cast<unsigned char*>(align256(reinterpret_cast<uintptr_t>(ws)));
   A.delta = reinterpret_cast<float*>(p);
-  A.dpart = reinterpret_cast<float*>(p + align256(rows * 4));
-  const bool vec = aligned(a, true);
-  const int st =
-      a->dtype == FX_F32 ? bwd<float>(s, A, lanes_of(a), vec) : bwd<bf16>(s, A, lanes_of(a), vec);
+  A.lut = reinterpret_cast<float*>(p + w.lut);
+  A.dpart = reinterpret_cast<float*>(p + w.dpart);
+  const bool vec = aligned(a, true), f32 = a->dtype == FX_F32;
+  // without queries dk and dv are zero: the rows kernels write them
+  const int st = use_tc_grad(a) && !no_rows(a) ? launch_attn_tc_bwd(s, A, f32, vec)
+                 : f32                         ? bwd<float>(s, A, lanes_of(a), vec)
+                                               : bwd<bf16>(s, A, lanes_of(a), vec);
   if (st || !a->table) return st;
   const int nb = a->buckets.num_buckets;
   const dim3 grid((nb + 31) / 32, A.H);
-  const int64_t parts = a->batch * a->q_len;
+  const int64_t parts = w.parts;
   if (a->dtype == FX_F32)
     bias_finish_kernel<float><<<grid, 1024, 0, s>>>(A.dpart, static_cast<float*>(a->dtable), parts, nb);
   else
