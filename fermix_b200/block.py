@@ -22,11 +22,39 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .api import _ptr, _stream_ptr
 
 _KIND = {torch.float32: _lib.FX_F32, torch.bfloat16: _lib.FX_BF16}
 _INTS = (torch.int32, torch.int64, torch.int16, torch.uint8)
 _GATE_NONE, _GATE_FULL, _GATE_ROW, _GATE_GROUP = range(4)
+
+
+# ------------------------------------------------------------------ calls
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call(fn, device, *args):
+    """fn(stream, *args) on the device's current stream. The common case, the device being current
+    already, takes no context: a small call is bound by the host."""
+    index = device.index
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return _lib.check(fn(torch._C._cuda_getCurrentRawStream(index), *args))
+    status = fn(torch._C._cuda_getCurrentRawStream(index), *args)
+    if status:
+        _lib.check(status)
+
+
+def _call_with_workspace(fn, size, device, args):
+    """As _call, with the workspace that size(args) asks for (kept alive until the launches are queued)."""
+    ref = ctypes.byref(args)
+    if device.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            nbytes = size(ref)
+    else:
+        nbytes = size(ref)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    _call(fn, device, ref, _ptr(ws), nbytes)
 
 
 # ------------------------------------------------------------------ checks
@@ -74,7 +102,7 @@ def _edges(num_buckets, max_distance, bidirectional):
 
 
 def _positions(pos, length, batch, device, name):
-    """An int32 (length) or (batch, length) tensor with contiguous rows, and its batch stride."""
+    """pos as an int32 (length) or (batch, length) tensor with contiguous rows."""
     if not isinstance(pos, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor, got {type(pos).__name__}")
     if pos.dtype not in _INTS:
@@ -87,7 +115,11 @@ def _positions(pos, length, batch, device, name):
         pos = pos.to(torch.int32)
     if pos.shape[-1] > 1 and pos.stride(-1) != 1:
         pos = pos.contiguous()
-    return pos, pos.stride(0) if pos.dim() == 2 else 0
+    return pos
+
+
+def _batch_stride(pos):
+    return pos.stride(0) if pos is not None and pos.dim() == 2 else 0
 
 
 def _buckets(num_buckets, max_distance, bidirectional, q_pos, k_pos, q_stride, k_stride):
@@ -96,23 +128,13 @@ def _buckets(num_buckets, max_distance, bidirectional, q_pos, k_pos, q_stride, k
                         _ptr(k_pos), q_stride, k_stride)
 
 
-def _workspace(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
 # ------------------------------------------------------------------ residual with its norms
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, f, post_weight, pre_weight, post_bias, pre_bias, gate, scale, form, kind, eps):
-        gate_shape, shape, gate_mode = form
         given = None if gate is None else gate.shape
-        if gate is not None:
-            gate = gate.expand(gate_shape).contiguous()
-        r, z = torch.empty_like(x), torch.empty_like(x)
-        a = _norm_args(x, f, post_weight, pre_weight, post_bias, pre_bias, gate, scale, shape, kind, gate_mode, eps)
-        a.r, a.z = _ptr(r), _ptr(z)
-        with torch.cuda.device(x.device):
-            _lib.check(_lib.lib().fermix_residual_norm(_stream_ptr(x.device), ctypes.byref(a)))
+        r, z, gate = _norm_forward(x, f, post_weight, pre_weight, post_bias, pre_bias, gate, scale, form, kind, eps)
+        _, shape, gate_mode = form
         ctx.save_for_backward(x, f, post_weight, pre_weight, post_bias, pre_bias, gate, scale)
         ctx.rest, ctx.given = (shape, kind, gate_mode, eps), given
         ctx.set_materialize_grads(False)
@@ -137,10 +159,7 @@ class _ResidualNorm(torch.autograd.Function):
         (a.dx, a.df, a.dpost_weight, a.dpre_weight, a.dpost_bias, a.dpre_bias, a.dgate,
          a.dscale) = (_ptr(g) for g in grads)
         L = _lib.lib()
-        with torch.cuda.device(x.device):
-            nb = L.fermix_residual_norm_grad_workspace_bytes(ctypes.byref(a))
-            ws = _workspace(nb, x.device)
-            _lib.check(L.fermix_residual_norm_grad(_stream_ptr(x.device), ctypes.byref(a), _ptr(ws), nb))
+        _call_with_workspace(L.fermix_residual_norm_grad, L.fermix_residual_norm_grad_workspace_bytes, x.device, a)
         if shared:
             grads[6] = grads[6].sum_to_size(ctx.given).to(x.dtype)
         return (*grads, None, None, None)
@@ -154,6 +173,22 @@ def _norm_args(x, f, post_weight, pre_weight, post_bias, pre_bias, gate, scale, 
     a.post_weight, a.post_bias, a.pre_weight, a.pre_bias = (_ptr(t) for t in
                                                             (post_weight, post_bias, pre_weight, pre_bias))
     return a
+
+
+def _norm_forward(x, f, post_weight, pre_weight, post_bias, pre_bias, gate, scale, form, kind, eps):
+    """(r, z, the gate as the kernel took it)."""
+    gate_shape, shape, gate_mode = form
+    if gate is not None:
+        gate = gate.expand(gate_shape).contiguous()
+    r, z = torch.empty_like(x), torch.empty_like(x)
+    a = _norm_args(x, f, post_weight, pre_weight, post_bias, pre_bias, gate, scale, shape, kind, gate_mode, eps)
+    a.r, a.z = r.data_ptr(), z.data_ptr()
+    _call(_lib.lib().fermix_residual_norm, x.device, ctypes.byref(a))
+    return r, z, gate
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _gate_form(gate, x):
@@ -214,41 +249,47 @@ def residual_norm(x, f, post_weight, pre_weight, *, post_bias=None, pre_bias=Non
         _tensor(gate, "gate", x)
     form = _gate_form(gate, x)
     post_weight, pre_weight, post_bias, pre_bias, scale = params
-    return _ResidualNorm.apply(x.contiguous(), f.contiguous(), post_weight, pre_weight, post_bias, pre_bias, gate,
-                               scale, form, int(kind == "layer"), float(eps))
+    args = (x.contiguous(), f.contiguous(), post_weight, pre_weight, post_bias, pre_bias, gate, scale)
+    rest = (form, int(kind == "layer"), float(eps))
+    if _wants_grad(*args):
+        return _ResidualNorm.apply(*args, *rest)
+    return _norm_forward(*args, *rest)[:2]
 
 
 # ------------------------------------------------------------------ position bias
 class _PositionBias(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, table, q_pos, k_pos, q_stride, k_stride, batch, q_len, k_len, max_distance, bidirectional):
-        a = _lib.BiasArgs()
-        a.dtype = _KIND[table.dtype]
-        a.batch, a.heads, a.q_len, a.k_len = batch, table.shape[0], q_len, k_len
-        a.buckets = _buckets(table.shape[1], max_distance, bidirectional, q_pos, k_pos, q_stride, k_stride)
-        out = torch.empty((batch, table.shape[0], q_len, k_len), dtype=table.dtype, device=table.device)
-        a.table, a.out = _ptr(table), _ptr(out)
-        with torch.cuda.device(table.device):
-            _lib.check(_lib.lib().fermix_position_bias(_stream_ptr(table.device), ctypes.byref(a)))
+    def forward(ctx, table, q_pos, k_pos, shape, max_distance, bidirectional):
+        out, ctx.args = _bias_forward(table, q_pos, k_pos, shape, max_distance, bidirectional)
         ctx.save_for_backward(q_pos, k_pos)
-        ctx.args, ctx.table = a, (table.shape, table.dtype)
+        ctx.table = table.shape, table.dtype
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         a = ctx.args
-        q_pos, k_pos = ctx.saved_tensors
+        q_pos, k_pos = ctx.saved_tensors  # alive until the launches are queued
         grad = grad.contiguous()
         dtable = torch.empty(ctx.table[0], dtype=ctx.table[1], device=grad.device)
-        a.grad, a.dtable = _ptr(grad), _ptr(dtable)
-        a.buckets.q_pos, a.buckets.k_pos = _ptr(q_pos), _ptr(k_pos)
+        a.grad, a.dtable = grad.data_ptr(), dtable.data_ptr()
+        a.buckets.q_pos, a.buckets.k_pos = q_pos.data_ptr(), k_pos.data_ptr()
         L = _lib.lib()
-        with torch.cuda.device(grad.device):
-            nb = L.fermix_position_bias_grad_workspace_bytes(ctypes.byref(a))
-            ws = _workspace(nb, grad.device)
-            _lib.check(L.fermix_position_bias_grad(_stream_ptr(grad.device), ctypes.byref(a), _ptr(ws), nb))
-        return dtable, None, None, None, None, None, None, None, None, None
+        _call_with_workspace(L.fermix_position_bias_grad, L.fermix_position_bias_grad_workspace_bytes, grad.device, a)
+        return dtable, None, None, None, None, None
+
+
+def _bias_forward(table, q_pos, k_pos, shape, max_distance, bidirectional):
+    a = _lib.BiasArgs()
+    a.dtype = _KIND[table.dtype]
+    a.heads, a.q_len, a.k_len = shape[-3:]
+    a.batch = shape[0] if len(shape) == 4 else 1
+    a.buckets = _buckets(table.shape[1], max_distance, bidirectional, q_pos, k_pos, _batch_stride(q_pos),
+                         _batch_stride(k_pos))
+    out = torch.empty(shape, dtype=table.dtype, device=table.device)
+    a.table, a.out = table.data_ptr(), out.data_ptr()
+    _call(_lib.lib().fermix_position_bias, table.device, ctypes.byref(a))
+    return out, a
 
 
 def position_bias(table, q_pos, k_pos=None, *, max_distance=128, bidirectional=True):
@@ -265,7 +306,7 @@ def position_bias(table, q_pos, k_pos=None, *, max_distance=128, bidirectional=T
         raise ValueError(f"table must have shape (heads, num_buckets), got {tuple(table.shape)}")
     if k_pos is None:
         k_pos = q_pos
-    batch = 1
+    batch = None
     for name, p in (("q_pos", q_pos), ("k_pos", k_pos)):
         if not isinstance(p, torch.Tensor):
             raise TypeError(f"{name} must be a torch tensor, got {type(p).__name__}")
@@ -273,11 +314,11 @@ def position_bias(table, q_pos, k_pos=None, *, max_distance=128, bidirectional=T
             raise ValueError(f"{name} must have shape (length,) or (batch, length), got {tuple(p.shape)}")
         if p.dim() == 2:
             batch = p.shape[0]
-    q, qs = _positions(q_pos, q_pos.shape[-1], batch, table.device, "q_pos")
-    k, ks = _positions(k_pos, k_pos.shape[-1], batch, table.device, "k_pos")
-    out = _PositionBias.apply(table.contiguous(), q, k, qs, ks, batch, q.shape[-1], k.shape[-1], max_distance,
-                              bool(bidirectional))
-    return out if q.dim() == 2 or k.dim() == 2 else out[0]
+    q = _positions(q_pos, q_pos.shape[-1], batch, table.device, "q_pos")
+    k = q if k_pos is q_pos else _positions(k_pos, k_pos.shape[-1], batch, table.device, "k_pos")
+    shape = (() if batch is None else (batch,)) + (table.shape[0], q.shape[-1], k.shape[-1])
+    args = (table.contiguous(), q, k, shape, max_distance, bool(bidirectional))
+    return _PositionBias.apply(*args) if _wants_grad(table) else _bias_forward(*args)[0]
 
 
 # ------------------------------------------------------------------ attention
@@ -291,8 +332,7 @@ def _attn_args(q, k, v, table, q_pos, k_pos, key_mask, out, lse, causal, scale, 
     a.batch, a.heads, a.q_len, a.dim = q.shape
     a.kv_heads, a.k_len = k.shape[1], k.shape[2]
     a.scale = scale
-    qs = q_pos.stride(0) if q_pos is not None and q_pos.dim() == 2 else 0
-    ks = k_pos.stride(0) if k_pos is not None and k_pos.dim() == 2 else 0
+    qs, ks = _batch_stride(q_pos), _batch_stride(k_pos)
     if table is not None:
         a.buckets = _buckets(table.shape[1], max_distance, bidirectional, q_pos, k_pos, qs, ks)
     else:
@@ -314,10 +354,7 @@ def _attn_forward(q, k, v, table, q_pos, k_pos, key_mask, with_lse, causal, scal
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if with_lse else None
     a = _attn_args(q, k, v, table, q_pos, k_pos, key_mask, out, lse, causal, scale, max_distance, bidirectional)
     L = _lib.lib()
-    with torch.cuda.device(q.device):
-        nb = L.fermix_biased_attention_workspace_bytes(ctypes.byref(a))
-        ws = _workspace(nb, q.device)
-        _lib.check(L.fermix_biased_attention(_stream_ptr(q.device), ctypes.byref(a), _ptr(ws), nb))
+    _call_with_workspace(L.fermix_biased_attention, L.fermix_biased_attention_workspace_bytes, q.device, a)
     return out, lse
 
 
@@ -341,10 +378,7 @@ class _BiasedAttention(torch.autograd.Function):
         a.dout_stride[:], a.dq_stride[:] = _strides(dout), _strides(dq)
         a.dk_stride[:], a.dv_stride[:] = _strides(dk), _strides(dv)
         L = _lib.lib()
-        with torch.cuda.device(q.device):
-            nb = L.fermix_biased_attention_grad_workspace_bytes(ctypes.byref(a))
-            ws = _workspace(nb, q.device)
-            _lib.check(L.fermix_biased_attention_grad(_stream_ptr(q.device), ctypes.byref(a), _ptr(ws), nb))
+        _call_with_workspace(L.fermix_biased_attention_grad, L.fermix_biased_attention_grad_workspace_bytes, q.device, a)
         return (dq, dk, dv, dtable) + (None,) * 8
 
 
@@ -388,9 +422,9 @@ def biased_attention(q, k, v, table=None, *, q_pos=None, k_pos=None, key_mask=No
             raise ValueError(f"table must have shape ({heads}, num_buckets), got {tuple(table.shape)}")
         table = table.contiguous()
     if q_pos is not None:
-        q_pos, _ = _positions(q_pos, q_len, batch, q.device, "q_pos")
+        q_pos = _positions(q_pos, q_len, batch, q.device, "q_pos")
     if k_pos is not None:
-        k_pos, _ = _positions(k_pos, k_len, batch, q.device, "k_pos")
+        k_pos = _positions(k_pos, k_len, batch, q.device, "k_pos")
     if key_mask is not None:
         if not isinstance(key_mask, torch.Tensor) or key_mask.dtype != torch.bool:
             raise TypeError("key_mask must be a bool tensor (True: the key takes part)")
@@ -401,7 +435,6 @@ def biased_attention(q, k, v, table=None, *, q_pos=None, k_pos=None, key_mask=No
             key_mask = key_mask.contiguous()
     rest = (bool(causal), float(dim**-0.5 if scale is None else scale), max_distance, bool(bidirectional))
     q, k, v = _rows(q), _rows(k), _rows(v)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
-                                    (table is not None and table.requires_grad)):
+    if _wants_grad(q, k, v, table):
         return _BiasedAttention.apply(q, k, v, table, q_pos, k_pos, key_mask, *rest)
     return _attn_forward(q, k, v, table, q_pos, k_pos, key_mask, False, *rest)[0]

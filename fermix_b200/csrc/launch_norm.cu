@@ -16,16 +16,17 @@ int check(const fx_norm_args* a) {
   return FX_OK;
 }
 
-// Threads of a row: 8 entries each up to a width of 4096 (registers of the backward: five
-// rows and six running sums of 8 entries), 16 above it.
+// Threads of a row: a 16-byte chunk each up to 512 threads (registers of the backward: five rows
+// and six running sums), two or four chunks above that.
 struct Shape {
-  int entries, tpr, threads, rpb;
+  int chunks, tpr, threads, rpb;
 };
 
-Shape shape_of(int64_t width) {
+Shape shape_of(const fx_norm_args* a) {
+  const int64_t entries = a->dtype == FX_F32 ? 4 : 8, all = (a->width + entries - 1) / entries;
   Shape s;
-  s.entries = width <= 4096 ? 8 : 16;
-  const int need = (int)((width + s.entries - 1) / s.entries);
+  s.chunks = all <= 512 ? 1 : all <= 1024 ? 2 : 4;
+  const int need = (int)((all + s.chunks - 1) / s.chunks);
   if (need <= 32) {
     s.tpr = 1;
     while (s.tpr < need) s.tpr *= 2;
@@ -38,18 +39,20 @@ Shape shape_of(int64_t width) {
   return s;
 }
 
-// Backward grid: two blocks of 256 threads an SM (or the same number of threads), the rows
-// in equal contiguous parts.
-void split(const fx_norm_args* a, const Shape& s, int sms, int& grid, int64_t& per) {
+// As many blocks as are resident at a time, the rows in equal contiguous parts.
+void split(const fx_norm_args* a, const Shape& s, int sms, bool grad, int& grid, int64_t& per) {
   const int64_t N = a->groups * a->rows, units = (N + s.rpb - 1) / s.rpb;
-  const int64_t cap = (int64_t)sms * (512 / s.threads);
+  const bool f32 = a->dtype == FX_F32, one = s.chunks == 1;
+  const int resident = grad ? (one ? (f32 ? kNormBwdResident<float, 1> : kNormBwdResident<bf16, 1>) : 512)
+                            : (one ? (f32 ? kNormFwdResident<float, 1> : kNormFwdResident<bf16, 1>) : 512);
+  const int64_t cap = (int64_t)sms * (resident / s.threads);
   const int64_t blocks = units < cap ? units : cap;
   per = (units + blocks - 1) / blocks * s.rpb;
   grid = (int)((N + per - 1) / per);
 }
 
 size_t part_bytes(const fx_norm_args* a, int grid) {
-  return align256((size_t)kNormParams * grid * a->width * sizeof(float));
+  return align256((size_t)kNormSums * grid * a->width * sizeof(float));
 }
 size_t gpart_bytes(const fx_norm_args* a, int grid) {
   return a->gate_mode == FX_GATE_GROUP ? align256((size_t)(grid + a->groups) * a->width * sizeof(float)) : 0;
@@ -97,20 +100,29 @@ bool aligned(const fx_norm_args* a) {
 
 template <typename T, int NV, bool ALIGNED>
 int launch(cudaStream_t s, const NormArgs& A, const Shape& h, int grid, bool grad) {
-  if (grad) {
-    const size_t smem = A.tpr > 32 ? 0 : (size_t)(kNormThreads / 32) * A.W * sizeof(float);
-    norm_bwd_kernel<T, NV, ALIGNED><<<grid, h.threads, smem, s>>>(A);
-  } else {
-    norm_fwd_kernel<T, NV, ALIGNED><<<grid, h.threads, 0, s>>>(A);
-  }
+  const size_t ring = (size_t)h.threads * (grad ? NormRing<T, NV, ALIGNED, 5>::kThreadBytes
+                                                : NormRing<T, NV, ALIGNED, 3>::kThreadBytes);
+  const size_t sums = grad && A.tpr <= 32 ? (size_t)(kNormThreads / 32) * A.W * sizeof(float) : 0;
+  auto kern = !grad ? norm_fwd_kernel<T, NV, ALIGNED>
+              : A.layer ? norm_bwd_kernel<T, NV, ALIGNED, true>
+                        : norm_bwd_kernel<T, NV, ALIGNED, false>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(ring + sums)) != cudaSuccess)
+    return FX_ERR_CUDA;
+  kern<<<grid, h.threads, ring + sums, s>>>(A);
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+}
+
+template <typename T, int NV>
+int by_alignment(cudaStream_t s, const NormArgs& A, const Shape& h, int grid, bool grad, bool al) {
+  return al ? launch<T, NV, true>(s, A, h, grid, grad) : launch<T, NV, false>(s, A, h, grid, grad);
 }
 
 template <typename T>
 int dispatch_type(cudaStream_t s, const NormArgs& A, const Shape& h, int grid, bool grad, bool al) {
-  constexpr int NV = sizeof(T) / 2;  // chunks of 8 entries
-  if (h.entries == 8) return al ? launch<T, NV, true>(s, A, h, grid, grad) : launch<T, NV, false>(s, A, h, grid, grad);
-  return al ? launch<T, 2 * NV, true>(s, A, h, grid, grad) : launch<T, 2 * NV, false>(s, A, h, grid, grad);
+  if (h.chunks == 1) return by_alignment<T, 1>(s, A, h, grid, grad, al);
+  if (h.chunks == 2) return by_alignment<T, 2>(s, A, h, grid, grad, al);
+  if constexpr (sizeof(T) == 4) return by_alignment<T, 4>(s, A, h, grid, grad, al);
+  return FX_ERR_SHAPE;
 }
 
 int dispatch(cudaStream_t s, const fx_norm_args* a, const NormArgs& A, const Shape& h, int grid, bool grad) {
@@ -132,18 +144,20 @@ int fermix_residual_norm(void* stream, const fx_norm_args* a) {
     return FX_ERR_NULL;
   const DevInfo* D = dev_info();
   if (!D) return FX_ERR_DEVICE;
-  const Shape h = shape_of(a->width);
-  const int64_t units = (N + h.rpb - 1) / h.rpb, cap = (int64_t)D->sms * (2048 / h.threads);
-  return dispatch(static_cast<cudaStream_t>(stream), a, make(a, h), h, (int)(units < cap ? units : cap), false);
+  const Shape h = shape_of(a);
+  NormArgs A = make(a, h);
+  int grid;
+  split(a, h, D->sms, false, grid, A.per);
+  return dispatch(static_cast<cudaStream_t>(stream), a, A, h, grid, false);
 }
 
 size_t fermix_residual_norm_grad_workspace_bytes(const fx_norm_args* a) {
   const DevInfo* D = dev_info();
   if (check(a) || !D || a->groups * a->rows == 0) return 0;
-  const Shape h = shape_of(a->width);
+  const Shape h = shape_of(a);
   int grid;
   int64_t per;
-  split(a, h, D->sms, grid, per);
+  split(a, h, D->sms, true, grid, per);
   return part_bytes(a, grid) + gpart_bytes(a, grid) + 256;
 }
 
@@ -156,8 +170,8 @@ int fermix_residual_norm_grad(void* stream, const fx_norm_args* a, void* ws, siz
     return FX_ERR_NULL;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const size_t size = a->dtype == FX_F32 ? 4 : 2;
-  void* outs[kNormParams] = {a->dpost_weight, a->post_bias ? a->dpost_bias : nullptr, a->dpre_weight,
-                             a->pre_bias ? a->dpre_bias : nullptr, a->scale ? a->dscale : nullptr};
+  void* outs[5] = {a->dpost_weight, a->post_bias ? a->dpost_bias : nullptr, a->dpre_weight,
+                   a->pre_bias ? a->dpre_bias : nullptr, a->scale ? a->dscale : nullptr};
   if (N == 0) {
     for (void* p : outs)
       if (p && cudaMemsetAsync(p, 0, (size_t)a->width * size, s) != cudaSuccess) return FX_ERR_CUDA;
@@ -171,10 +185,10 @@ int fermix_residual_norm_grad(void* stream, const fx_norm_args* a, void* ws, siz
     return FX_ERR_NULL;
   const DevInfo* D = dev_info();
   if (!D) return FX_ERR_DEVICE;
-  const Shape h = shape_of(a->width);
+  const Shape h = shape_of(a);
   int grid;
   int64_t per;
-  split(a, h, D->sms, grid, per);
+  split(a, h, D->sms, true, grid, per);
   if (!ws || wsb < part_bytes(a, grid) + gpart_bytes(a, grid) + 256) return FX_ERR_WORKSPACE;
   NormArgs A = make(a, h);
   A.per = per;
@@ -185,7 +199,14 @@ int fermix_residual_norm_grad(void* stream, const fx_norm_args* a, void* ws, siz
   NormFinish F{};
   F.part = A.part;
   F.gpart = A.gpart;
-  for (int p = 0; p < kNormParams; ++p) F.out[p] = outs[p];
+  F.pw = a->post_weight;
+  F.pb = a->post_bias;
+  F.scale = a->scale;
+  F.dpw = outs[0];
+  F.dpb = outs[1];
+  F.drw = outs[2];
+  F.drb = outs[3];
+  F.dscale = outs[4];
   F.dgate = a->dgate;
   F.groups = a->gate_mode == FX_GATE_GROUP ? a->groups : 0;
   F.R = a->rows;
@@ -194,10 +215,10 @@ int fermix_residual_norm_grad(void* stream, const fx_norm_args* a, void* ws, siz
   F.dgate_f32 = a->dgate_f32 != 0;
   F.W = (int)a->width;
   F.cols = (F.W + 31) / 32;
-  const int64_t blocks = (int64_t)kNormParams * F.cols + (F.groups * a->width + 255) / 256;
+  const int64_t blocks = (int64_t)2 * F.cols + (F.groups * a->width + 1023) / 1024;
   if (blocks > INT32_MAX) return FX_ERR_SHAPE;
-  if (a->dtype == FX_F32) norm_finish_kernel<float><<<(unsigned)blocks, 256, 0, s>>>(F);
-  else norm_finish_kernel<bf16><<<(unsigned)blocks, 256, 0, s>>>(F);
+  if (a->dtype == FX_F32) norm_finish_kernel<float><<<(unsigned)blocks, 1024, 0, s>>>(F);
+  else norm_finish_kernel<bf16><<<(unsigned)blocks, 1024, 0, s>>>(F);
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
