@@ -12,7 +12,7 @@ int check(const fx_norm_args* a) {
   if (a->groups < 0 || a->rows < 0 || a->width < 1 || a->width > FX_NORM_MAX_WIDTH || a->kind < 0 || a->kind > 1 ||
       a->gate_mode < FX_GATE_NONE || a->gate_mode > FX_GATE_GROUP)
     return FX_ERR_SHAPE;
-  if (a->groups > 0 && a->rows > (int64_t{1} << 46) / a->width / a->groups) return FX_ERR_SHAPE;
+  if (a->groups > 0 && a->rows > (int64_t{1} << 40) / a->groups) return FX_ERR_SHAPE;
   return FX_OK;
 }
 
@@ -49,7 +49,7 @@ void split(const fx_norm_args* a, const Shape& s, int sms, bool grad, int& grid,
   const int64_t blocks = units < cap ? units : cap;
   per = (units + blocks - 1) / blocks * s.rpb;
   grid = (int)((N + per - 1) / per);
-}
+}  // per < 2^31: N <= 2^40 rows over at least 2^9 blocks where N is that large
 
 size_t part_bytes(const fx_norm_args* a, int grid) {
   return align256((size_t)kNormSums * grid * a->width * sizeof(float));
@@ -98,30 +98,31 @@ bool aligned(const fx_norm_args* a) {
   return m % 16 == 0;
 }
 
-template <typename T, int NV, bool ALIGNED>
+template <typename T, int NV, bool ALIGNED, bool WIDE>
 int launch(cudaStream_t s, const NormArgs& A, const Shape& h, int grid, bool grad) {
-  const size_t ring = (size_t)h.threads * (grad ? NormRing<T, NV, ALIGNED, 5>::kThreadBytes
-                                                : NormRing<T, NV, ALIGNED, 3>::kThreadBytes);
-  const size_t sums = grad && A.tpr <= 32 ? (size_t)(kNormThreads / 32) * A.W * sizeof(float) : 0;
-  auto kern = !grad ? norm_fwd_kernel<T, NV, ALIGNED>
-              : A.layer ? norm_bwd_kernel<T, NV, ALIGNED, true>
-                        : norm_bwd_kernel<T, NV, ALIGNED, false>;
+  const size_t ring = (size_t)h.threads * (grad ? NormRing<T, NV, ALIGNED, WIDE, 5>::kThreadBytes
+                                                : NormRing<T, NV, ALIGNED, WIDE, 3>::kThreadBytes);
+  const size_t sums = grad && !WIDE ? (size_t)(kNormThreads / 32) * A.W * sizeof(float) : 0;
+  auto kern = !grad     ? norm_fwd_kernel<T, NV, ALIGNED, WIDE>
+              : A.layer ? norm_bwd_kernel<T, NV, ALIGNED, WIDE, true>
+                        : norm_bwd_kernel<T, NV, ALIGNED, WIDE, false>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(ring + sums)) != cudaSuccess)
     return FX_ERR_CUDA;
   kern<<<grid, h.threads, ring + sums, s>>>(A);
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
-template <typename T, int NV>
-int by_alignment(cudaStream_t s, const NormArgs& A, const Shape& h, int grid, bool grad, bool al) {
-  return al ? launch<T, NV, true>(s, A, h, grid, grad) : launch<T, NV, false>(s, A, h, grid, grad);
-}
-
+// Several chunks a thread only where more than 512 threads were needed, a block to a row.
 template <typename T>
 int dispatch_type(cudaStream_t s, const NormArgs& A, const Shape& h, int grid, bool grad, bool al) {
-  if (h.chunks == 1) return by_alignment<T, 1>(s, A, h, grid, grad, al);
-  if (h.chunks == 2) return by_alignment<T, 2>(s, A, h, grid, grad, al);
-  if constexpr (sizeof(T) == 4) return by_alignment<T, 4>(s, A, h, grid, grad, al);
+  if (h.chunks == 1 && h.tpr <= 32)
+    return al ? launch<T, 1, true, false>(s, A, h, grid, grad) : launch<T, 1, false, false>(s, A, h, grid, grad);
+  if (h.chunks == 1)
+    return al ? launch<T, 1, true, true>(s, A, h, grid, grad) : launch<T, 1, false, true>(s, A, h, grid, grad);
+  if (h.chunks == 2)
+    return al ? launch<T, 2, true, true>(s, A, h, grid, grad) : launch<T, 2, false, true>(s, A, h, grid, grad);
+  if constexpr (sizeof(T) == 4)
+    return al ? launch<T, 4, true, true>(s, A, h, grid, grad) : launch<T, 4, false, true>(s, A, h, grid, grad);
   return FX_ERR_SHAPE;
 }
 

@@ -45,6 +45,8 @@ constexpr int kNormSums = 4;
 
 // Sums over the TPR threads of a row. Blocks that hold one row go through shared memory,
 // alternating between two buffers so that one barrier a sum is enough.
+// WIDE: more than a warp a row.
+template <bool WIDE>
 struct RowSum {
   float* red;  // 2 x 32 x 4
   int tpr, flip;
@@ -56,19 +58,24 @@ struct RowSum {
     __syncthreads();
     return buf;
   }
+  __device__ __forceinline__ void lanes(float& a, float& b) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+      if (WIDE || o < tpr) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        b += __shfl_xor_sync(0xffffffffu, b, o);
+      }
+  }
   // the means of a and b
   __device__ __forceinline__ float2 mean2(float a, float b) {
-    const int width = tpr < 32 ? tpr : 32;
-    for (int o = width >> 1; o > 0; o >>= 1) {
-      a += __shfl_xor_sync(0xffffffffu, a, o);
-      b += __shfl_xor_sync(0xffffffffu, b, o);
-    }
-    if (tpr > 32) {
+    lanes(a, b);
+    if (WIDE) {
       const float4* buf = put(a, b, 0.f);
       const int nw = tpr >> 5;
       a = b = 0.f;
+#pragma unroll 4
       for (int i = 0; i < nw; ++i) {
-        const float4 v = buf[i];
+        const float2 v = *reinterpret_cast<const float2*>(&buf[i]);
         a += v.x;
         b += v.y;
       }
@@ -76,34 +83,30 @@ struct RowSum {
     return make_float2(a * inv_w, b * inv_w);
   }
   __device__ __forceinline__ float mean(float a) {
-    a = lanes_sum(a, tpr < 32 ? tpr : 32);
-    if (tpr > 32) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+      if (WIDE || o < tpr) a += __shfl_xor_sync(0xffffffffu, a, o);
+    if (WIDE) {
       const float4* buf = put(a, 0.f, 0.f);
       const int nw = tpr >> 5;
       a = 0.f;
+#pragma unroll 4
       for (int i = 0; i < nw; ++i) a += buf[i].x;
     }
     return a * inv_w;
   }
   // (mean, mean of the centred squares) from the sums a of v - c and b of (v - c)^2 over the
-  // `count` entries of the warp (or group): c is an entry, so nothing of a large mean cancels;
-  // the warps are joined about the common mean.
-  __device__ __forceinline__ float2 moments(float a, float b, float c, float count) {
-    const int width = tpr < 32 ? tpr : 32;
-    for (int o = width >> 1; o > 0; o >>= 1) {
-      a += __shfl_xor_sync(0xffffffffu, a, o);
-      b += __shfl_xor_sync(0xffffffffu, b, o);
-    }
-    if (tpr <= 32) {
-      const float m = a * inv_w;
-      return make_float2(c + m, fmaxf(fmaf(-m, a, b), 0.f) * inv_w);
-    }
-    const float m = count > 0.f ? __fdividef(a, count) : 0.f;
-    const float4* buf = put(c + m, fmaxf(fmaf(-m, a, b), 0.f), count);
+  // 1 / inv_count entries of the warp (or group): c is an entry, so nothing of a large mean
+  // cancels; the warps are joined about the first one's mean.
+  __device__ __forceinline__ float2 moments(float a, float b, float c, float count, float inv_count) {
+    lanes(a, b);
+    const float m = a * inv_count, sq = fmaxf(fmaf(-m, a, b), 0.f);
+    if (!WIDE) return make_float2(c + m, sq * inv_w);
+    const float4* buf = put(c + m, sq, count);
     const int nw = tpr >> 5;
-    // about the first warp's mean
     const float base = buf[0].x;
     float s = 0.f, q = 0.f, d2 = 0.f;
+#pragma unroll 4
     for (int i = 0; i < nw; ++i) {
       const float4 v = buf[i];
       const float d = v.x - base, nd = v.z * d;
@@ -129,12 +132,14 @@ __device__ __forceinline__ void cp_async16(uint4* dst, const void* src) {
 // either. ALIGNED: every row and parameter starts on a 16-byte boundary and the width is whole
 // chunks. Otherwise a chunk is cut out of the two aligned 16-byte pieces around it, and stored
 // as aligned pieces joined with the neighbour's entries.
-template <typename T, int NV, bool ALIGNED>
+template <typename T, int NV, bool ALIGNED, bool WIDE>
 struct NormRow {
   static constexpr int C = 16 / sizeof(T), E = C * NV;
   int t, tpr, W;
-  float count;  // entries of the row that this warp (or group) holds
+  float count, inv_count;  // entries of the row that this warp (or group) holds
+  float kept[ALIGNED ? NV : E];  // 1 within the row, 0 past its end
   __device__ __forceinline__ int at(int v) const { return (v * tpr + t) * C; }
+  __device__ __forceinline__ float keep(int e) const { return kept[ALIGNED ? e / C : e]; }
   __device__ __forceinline__ bool in(int e) const { return at(e / C) + (ALIGNED ? 0 : e % C) < W; }
   static constexpr int P = ALIGNED ? 1 : 2;  // aligned pieces that hold a chunk
   // Whether the aligned pieces around entries [c, c + C) of the row at p lie in [begin, end).
@@ -228,8 +233,8 @@ struct NormRow {
                                        bool there, float (&o)[E]) const {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
+      uint4 r = make_uint4(0u, 0u, 0u, 0u);
       if (there && at(v) < W) {
-        uint4 r;
         if constexpr (ALIGNED) {
           r = slot[v * stride];
         } else {
@@ -237,11 +242,10 @@ struct NormRow {
           r = slot[2 * v * stride];
           if (w.whole) r = shifted(r, w.two ? slot[(2 * v + 1) * stride] : make_uint4(0u, 0u, 0u, 0u), w.off);
         }
-        unpack(*reinterpret_cast<const Pack<T, C>*>(&r), v, o, 0.f);
-      } else {
-#pragma unroll
-        for (int e = 0; e < C; ++e) o[v * C + e] = 0.f;
       }
+      const Pack<T, C> k = *reinterpret_cast<const Pack<T, C>*>(&r);
+#pragma unroll
+      for (int e = 0; e < C; ++e) o[v * C + e] = ALIGNED || in(v * C + e) ? to_f(k.e[e]) : 0.f;
     }
   }
   // Every lane of the warp calls this; a row that is not there is not written.
@@ -300,7 +304,7 @@ struct NormRow {
     }
   }
   // v <- normalised v (entries outside the row are 0 and stay so), returns 1 / rms.
-  __device__ __forceinline__ float normalise(float (&v)[E], bool layer, float eps, RowSum& sum) const {
+  __device__ __forceinline__ float normalise(float (&v)[E], bool layer, float eps, RowSum<WIDE>& sum) const {
     if (!layer) {
       float q = 0.f;
 #pragma unroll
@@ -310,23 +314,22 @@ struct NormRow {
       for (int e = 0; e < E; ++e) v[e] *= inv;
       return inv;
     }
-    const int lanes = tpr < 32 ? tpr : 32;
-    const float c = __shfl_sync(0xffffffffu, v[0], threadIdx.x & 31 & ~(lanes - 1));
+    const float c = __shfl_sync(0xffffffffu, v[0], WIDE ? 0 : threadIdx.x & 31 & ~(tpr - 1));
     float a = 0.f, q = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const float d = in(e) ? v[e] - c : 0.f;
+      const float d = fmaf(-c, keep(e), v[e]);
       a += d;
       q = fmaf(d, d, q);
     }
-    const float2 m = sum.moments(a, q, c, count);
+    const float2 m = sum.moments(a, q, c, count, inv_count);
     const float inv = rsqrtf(m.y + eps);
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = in(e) ? (v[e] - m.x) * inv : 0.f;
+    for (int e = 0; e < E; ++e) v[e] = fmaf(-m.x, keep(e), v[e]) * inv;
     return inv;
   }
   // a <- the gradient through normalise(): inv (a - mean(a) [layer] - n mean(a n))
-  __device__ __forceinline__ void back(float (&a)[E], const float (&n)[E], float inv, bool layer, RowSum& sum) const {
+  __device__ __forceinline__ void back(float (&a)[E], const float (&n)[E], float inv, bool layer, RowSum<WIDE>& sum) const {
     float s = 0.f, d = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -335,29 +338,33 @@ struct NormRow {
     }
     const float2 m = layer ? sum.mean2(s, d) : make_float2(0.f, sum.mean(d));
 #pragma unroll
-    for (int e = 0; e < E; ++e) a[e] = inv * (fmaf(-n[e], m.y, a[e]) - m.x);
+    for (int e = 0; e < E; ++e) a[e] = inv * fmaf(-m.x, keep(e), fmaf(-n[e], m.y, a[e]));
   }
 };
 
 template <typename Row>
 __device__ __forceinline__ Row make_row(int t, int tpr, int W) {
-  Row row{t, tpr, W, 0.f};
+  Row row;
+  row.t = t;
+  row.tpr = tpr;
+  row.W = W;
   float n = 0.f;
 #pragma unroll
-  for (int v = 0; v < Row::E / Row::C; ++v) {
-    const int left = W - row.at(v);
-    n += (float)(left < 0 ? 0 : left < Row::C ? left : Row::C);
+  for (int e = 0; e < Row::E; ++e) {
+    n += row.in(e) ? 1.f : 0.f;
+    row.kept[sizeof(row.kept) / 4 == Row::E ? e : e / Row::C] = row.in(e) ? 1.f : 0.f;
   }
   row.count = lanes_sum(n, tpr < 32 ? tpr : 32);
+  row.inv_count = row.count > 0.f ? 1.f / row.count : 0.f;
   return row;
 }
 
 // The arrays of a row (nullptr: not there), and this thread's ring of their entries: three rows
 // deep, two where the pieces are twice as many. Rows of several chunks a thread that would not
 // fit are loaded when they are needed.
-template <typename T, int NV, bool ALIGNED, int K>
+template <typename T, int NV, bool ALIGNED, bool WIDE, int K>
 struct NormRing {
-  using Row = NormRow<T, NV, ALIGNED>;
+  using Row = NormRow<T, NV, ALIGNED, WIDE>;
   static constexpr int S = NV == 1 ? (ALIGNED ? 3 : 2) : NV == 2 && ALIGNED ? 2 : 0;
   static constexpr int kThreadBytes = S * K * NV * Row::P * 16;
   const T* array[K];
@@ -390,20 +397,21 @@ struct NormRing {
   }
 };
 
-// The rows of a block in steps of rpb, each step within one group of the gate (gate_mode 3).
+// The rows of a block in steps of rpb, each step within one group of the gate (gate_mode 3);
+// counted from the block's first row.
 struct NormWalk {
-  int64_t base, end, last, R;
-  int rpb;
+  int base, end, last, rpb;
   bool grouped;
-  __device__ __forceinline__ int64_t segment_end(int64_t i) const {
+  int64_t first, R;
+  __device__ __forceinline__ int segment_end(int i) const {
     if (!grouped) return last;
-    const int64_t e = (i / R + 1) * R;
-    return e < last ? e : last;
+    const int64_t e = ((first + i) / R + 1) * R - first;
+    return e < last ? (int)e : last;
   }
   __device__ __forceinline__ NormWalk(const NormArgs& A, int rpb_)
-      : base((int64_t)blockIdx.x * A.per), last(base + A.per < A.N ? base + A.per : A.N), R(A.R), rpb(rpb_),
-        grouped(A.gate_mode == FX_GATE_GROUP) {
-    end = segment_end(base);
+      : base(0), rpb(rpb_), grouped(A.gate_mode == FX_GATE_GROUP), first((int64_t)blockIdx.x * A.per), R(A.R) {
+    last = (int)(first + A.per < A.N ? A.per : A.N - first);
+    end = segment_end(0);
   }
   __device__ __forceinline__ void step() {
     base += rpb;
@@ -418,18 +426,18 @@ struct NormWalk {
 template <typename T, int NV>
 constexpr int kNormFwdResident = NV > 1 ? 512 : sizeof(T) == 4 ? 1024 : 768;
 
-template <typename T, int NV, bool ALIGNED>
+template <typename T, int NV, bool ALIGNED, bool WIDE>
 __global__ void __launch_bounds__(kNormFwdResident<T, NV>) norm_fwd_kernel(const __grid_constant__ NormArgs A) {
-  using Row = NormRow<T, NV, ALIGNED>;
+  using Row = NormRow<T, NV, ALIGNED, WIDE>;
   constexpr int E = Row::E;
   extern __shared__ uint4 ring_mem[];
   __shared__ __align__(16) float red[256];
-  const int tpr = A.tpr, W = A.W, rpb = tpr > 32 ? 1 : blockDim.x / tpr;
-  const int sub = tpr > 32 ? 0 : threadIdx.x / tpr;
+  const int tpr = A.tpr, W = A.W, rpb = WIDE ? 1 : blockDim.x / tpr;
+  const int sub = WIDE ? 0 : threadIdx.x / tpr;
   const Row row = make_row<Row>((int)threadIdx.x - sub * tpr, tpr, W);
-  RowSum sum{red, tpr, 0, 1.f / (float)W};
+  RowSum<WIDE> sum{red, tpr, 0, 1.f / (float)W};
   const T* gate = static_cast<const T*>(A.gate);
-  using Ring = NormRing<T, NV, ALIGNED, 3>;
+  using Ring = NormRing<T, NV, ALIGNED, WIDE, 3>;
   Ring ring;
   ring.array[0] = static_cast<const T*>(A.f);
   ring.array[1] = static_cast<const T*>(A.x);
@@ -452,17 +460,18 @@ __global__ void __launch_bounds__(kNormFwdResident<T, NV>) norm_fwd_kernel(const
     g[e] = 1.f;
   }
   NormWalk now(A, rpb), ahead = now;
-  int64_t seg = -1;
+  int seg = -1;
 #pragma unroll
   for (int n = 0; n < Ring::S - 1; ++n) {
-    ring.fetch(row, n, ahead.base + sub, ahead.base + sub < ahead.end);
+    ring.fetch(row, n, ahead.first + ahead.base + sub, ahead.base + sub < ahead.end);
     ahead.step();
   }
   int stage = 0;
   for (; now.base < now.last; now.step()) {
-    const int64_t i = now.base + sub;
-    const bool there = i < now.end;
-    ring.fetch(row, stage == 0 ? Ring::S - 1 : stage - 1, ahead.base + sub, ahead.base + sub < ahead.end);
+    const int64_t i = now.first + now.base + sub;
+    const bool there = now.base + sub < now.end;
+    ring.fetch(row, stage == 0 ? Ring::S - 1 : stage - 1, ahead.first + ahead.base + sub,
+               ahead.base + sub < ahead.end);
     ahead.step();
     ring.wait();
     float f[E], x[E];
@@ -476,7 +485,7 @@ __global__ void __launch_bounds__(kNormFwdResident<T, NV>) norm_fwd_kernel(const
       for (int e = 0; e < E; ++e) g[e] = g1;
     } else if (now.grouped && now.end != seg) {
       seg = now.end;
-      row.load(gate + now.base / A.R * W, g, 0.f);
+      row.load(gate + (now.first + now.base) / A.R * W, g, 0.f);
     }
     stage = ring.next(stage);
     row.normalise(f, A.layer, A.eps, sum);
@@ -521,18 +530,18 @@ __device__ __forceinline__ void norm_block_sum(float (&acc)[Row::E], const Row& 
 template <typename T, int NV>
 constexpr int kNormBwdResident = sizeof(T) == 4 && NV == 1 ? 768 : 512;
 
-template <typename T, int NV, bool ALIGNED, bool LAYER>
+template <typename T, int NV, bool ALIGNED, bool WIDE, bool LAYER>
 __global__ void __launch_bounds__(kNormBwdResident<T, NV>) norm_bwd_kernel(const __grid_constant__ NormArgs A) {
-  using Row = NormRow<T, NV, ALIGNED>;
+  using Row = NormRow<T, NV, ALIGNED, WIDE>;
   constexpr int E = Row::E;
   extern __shared__ uint4 ring_mem[];
   __shared__ __align__(16) float red[256];
-  const int tpr = A.tpr, W = A.W, rpb = tpr > 32 ? 1 : blockDim.x / tpr;
-  const int sub = tpr > 32 ? 0 : threadIdx.x / tpr;
+  const int tpr = A.tpr, W = A.W, rpb = WIDE ? 1 : blockDim.x / tpr;
+  const int sub = WIDE ? 0 : threadIdx.x / tpr;
   const Row row = make_row<Row>((int)threadIdx.x - sub * tpr, tpr, W);
-  RowSum sum{red, tpr, 0, 1.f / (float)W};
+  RowSum<WIDE> sum{red, tpr, 0, 1.f / (float)W};
   const T* gate = static_cast<const T*>(A.gate);
-  using Ring = NormRing<T, NV, ALIGNED, 5>;
+  using Ring = NormRing<T, NV, ALIGNED, WIDE, 5>;
   Ring ring;
   ring.array[0] = static_cast<const T*>(A.f);
   ring.array[1] = static_cast<const T*>(A.x);
@@ -561,23 +570,25 @@ __global__ void __launch_bounds__(kNormBwdResident<T, NV>) norm_bwd_kernel(const
   NormWalk now(A, rpb), ahead = now;
 #pragma unroll
   for (int n = 0; n < Ring::S - 1; ++n) {
-    ring.fetch(row, n, ahead.base + sub, ahead.base + sub < ahead.end);
+    ring.fetch(row, n, ahead.first + ahead.base + sub, ahead.base + sub < ahead.end);
     ahead.step();
   }
   int stage = 0;
   while (now.base < now.last) {
     float Pg[E], Qg[E];  // of a segment
-    const int64_t grp = now.grouped ? now.base / A.R : 0, end = now.end;
+    const int64_t grp = now.grouped ? (now.first + now.base) / A.R : 0;
+    const int end = now.end;
     if (now.grouped) {
       row.load(gate + grp * W, g, 0.f);
 #pragma unroll
       for (int e = 0; e < E; ++e) Pg[e] = P[e], Qg[e] = Q[e], P[e] = Q[e] = 0.f;
     }
     for (; now.base < end && now.end == end; now.step()) {
-      const int64_t i = now.base + sub;
-      const bool there = i < end;
+      const int64_t i = now.first + now.base + sub;
+      const bool there = now.base + sub < end;
       const int64_t o = there ? i * W : 0;
-      ring.fetch(row, stage == 0 ? Ring::S - 1 : stage - 1, ahead.base + sub, ahead.base + sub < ahead.end);
+      ring.fetch(row, stage == 0 ? Ring::S - 1 : stage - 1, ahead.first + ahead.base + sub,
+               ahead.base + sub < ahead.end);
       ahead.step();
       ring.wait();
       float f[E], x[E], t[E], a[E];
@@ -606,7 +617,7 @@ __global__ void __launch_bounds__(kNormBwdResident<T, NV>) norm_bwd_kernel(const
       ring.take(row, stage, 3, i, there, t);
       stage = ring.next(stage);
 #pragma unroll
-      for (int e = 0; e < E; ++e) t[e] = there && row.in(e) ? t[e] + a[e] : 0.f;
+      for (int e = 0; e < E; ++e) t[e] += a[e];  // 0 past the width and in rows that are not there
       row.store(static_cast<T*>(A.dx) + o, t, there);
       if (A.gate_mode == FX_GATE_FULL || A.gate_mode == FX_GATE_ROW) {
         float rowg = 0.f;
