@@ -16,9 +16,9 @@ int raise_smem(K kern, size_t smem) {
 }
 
 // ---- launch_attn_tc.cu: tcgen05 kernels
-int launch_attn_tc_fwd(cudaStream_t s, const AttnArgs& A, bool is_f32, bool vec);
+int launch_attn_tc_fwd(cudaStream_t s, const AttnArgs& A, bool is_f32, bool aligned);
 // Backward (float32: dim <= 64). A.delta, A.lut and A.dpart (batch x query blocks of 128 parts a
 // head) are workspace.
-int launch_attn_tc_bwd(cudaStream_t s, const AttnArgs& A, bool is_f32, bool vec);
+int launch_attn_tc_bwd(cudaStream_t s, const AttnArgs& A, bool is_f32, bool aligned);
 
 }  // namespace fxh

@@ -11,10 +11,13 @@
 // TF32 products cost the same and keep 22 bits). bfloat16 keeps float32's exponent range, so
 // neither the parts nor the score gradients need a scale.
 //
-// Loading is by threads (cp.async, or through registers where a type is split or an address
-// is not on 16 bytes), not by tensor maps: a masked key's row must be zero whatever it
-// holds, rows end anywhere, and strides are the caller's.
+// bfloat16 tiles on 16-byte boundaries come by tensor maps (one thread issues a tile's copies;
+// rows and entries past the ends are filled with zeros); two more warps then clear the rows
+// of masked keys, whatever those hold, before the tensor cores may read the tile. float32 is split
+// on the way and unaligned storage has no map: those tiles are loaded by the threads.
 #pragma once
+#include <cuda.h>
+
 #include "attn_rows.cuh"
 #include "umma.cuh"
 
@@ -25,11 +28,24 @@ using namespace umma;
 
 constexpr int kSub = 32;  // keys (or queries) whose positions are summarised together
 
-// K-major / MN-major operand in the 128-byte swizzle. lbo: bytes between chunks of 64 entries
-// (MN-major only), groups of 8 rows are 1024 bytes apart.
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lbo) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 | (uint64_t)(1024u >> 4) << 32 |
-         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+// A tile's layout: chunks of RB bytes a row (128, or 64 for float32's parts of up to 32 entries, which
+// halves what they take), DC of them. The 16-byte piece c of row r is at piece
+// c ^ (r & 7) (RB = 128) or c ^ (r / 2 & 3) (RB = 64) of its row.
+template <int RB_, int DC_>
+struct Rows {
+  static constexpr int RB = RB_, DC = DC_, kDim = RB / 2 * DC;  // bytes, chunks, entries
+  static __device__ __forceinline__ uint32_t at(int rows, int r, int c) {
+    constexpr int P = RB / 16;
+    return (uint32_t)(c / P) * (uint32_t)(rows * RB) + r * RB + (((c % P) ^ (RB == 128 ? r & 7 : (r >> 1) & 3)) << 4);
+  }
+};
+
+// K-major / MN-major operand. lbo: bytes between chunks (MN-major only); groups of 8 rows follow
+// each other.
+template <int RB>
+__device__ __forceinline__ uint64_t desc(uint32_t saddr, uint32_t lbo) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 | (uint64_t)(RB * 8 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)(RB == 128 ? 2 : 4) << 61;
 }
 // kind::f16, bfloat16 operands, float32 accumulator
 __device__ __forceinline__ uint32_t idesc_bf16(int M, int N, bool b_mn) {
@@ -125,95 +141,123 @@ __device__ __forceinline__ void wait(uint64_t* m, uint32_t parity, volatile int*
 __device__ __forceinline__ void named_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// How a tile is brought in: by the threads, entry by entry or in 16-byte pieces, or by a tensor map.
+enum { LOAD_ENTRIES, LOAD_PIECES, LOAD_TMA };
+
+// Tensor maps of q, k, v and dout: (entry, token, head, batch), boxes of one chunk by BN or 128
+// tokens. A dimension the tensor is expanded along has one entry in its map (mul 0).
+struct alignas(64) TmaMaps {
+  CUtensorMap m[4];
+  int head_mul[4], batch_mul[4];
+};
+enum { MAP_Q, MAP_K, MAP_V, MAP_DO };
+
+// One tile (DC chunks of `rows` rows from token i0) by one thread; the mbarrier was told the bytes.
+template <typename L>
+__device__ __forceinline__ void tma_tile(unsigned char* dst, const TmaMaps& M, int which, int rows, int64_t i0, int h, int b,
+                                         uint64_t* mbar) {
+#pragma unroll
+  for (int c = 0; c < L::DC; ++c)
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(smem_u32(dst) + (uint32_t)(c * rows * L::RB)),
+        "l"(&M.m[which]), "r"(c * 64), "r"((int)i0), "r"(h * M.head_mul[which]), "r"(b * M.batch_mul[which]),
+        "r"(smem_u32(mbar))
+        : "memory");
 }
 
-// Rows [0, R) of a tile from p (element strides `step` a row, dim entries a row, entries
-// beyond dim up to the next multiple of 16 zero), row r only if live(r), by `n` threads of index
-// t. Parts of a split type are R * chunks * 128 bytes apart. cp.async copies are left open.
-template <typename T, int NS, bool VEC, int R, typename Live>
-__device__ __forceinline__ void load_tile(unsigned char* dst, const T* p, int64_t step, int dim, int chunks, int t,
-                                          int n, Live live) {
-  const int pieces = (dim + 15) / 16 * 2;  // of 8 entries
-  const uint32_t part = (uint32_t)R * 128u * (uint32_t)chunks;
-  for (int i = t; i < R * pieces; i += n) {
-    const int r = i / pieces, c = i - r * pieces;
-    const bool ok = live(r);
-    unsigned char* d = dst + (uint32_t)(c >> 3) * (R * 128u) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-    if constexpr (NS == 1 && VEC && sizeof(T) == 2) {
-      const bool has = ok && c * 8 < dim;
-      cp16(smem_u32(d), has ? p + r * step + c * 8 : p, has ? 16 : 0);
-    } else {
-      float x[8];
+// Zeros in the rows of a tile that are not live, by `n` threads of index t.
+template <typename L, typename Live>
+__device__ __forceinline__ void clear_rows(unsigned char* dst, int rows, int t, int n, Live live) {
+  for (int i = t; i < rows * L::DC; i += n) {
+    const int r = i % rows, c = i / rows;
+    if (!live(r)) {
+      uint4* p = reinterpret_cast<uint4*>(dst + (uint32_t)(c * rows + r) * L::RB);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = 0.f;
-      if (ok) {
-        const T* s = p + r * step + c * 8;
-        if constexpr (VEC) {
-          constexpr int V = 16 / sizeof(T);
-#pragma unroll
-          for (int h = 0; h < 8; h += V) {
-            if (c * 8 + h < dim) {
-              const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(s + h);
-#pragma unroll
-              for (int e = 0; e < V; ++e) x[h + e] = to_f(k.e[e]);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (c * 8 + e < dim) x[e] = to_f(s[e]);
-        }
-      }
-      uint32_t w[4][NS];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) split2<NS>(x[2 * e], x[2 * e + 1], w[e]);
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-        *reinterpret_cast<uint4*>(d + s * part) = make_uint4(w[0][s], w[1][s], w[2][s], w[3][s]);
+      for (int e = 0; e < L::RB / 16; ++e) p[e] = make_uint4(0u, 0u, 0u, 0u);
     }
   }
 }
 
-// D (+)= A B^T over `steps` k-steps of 16 entries, both K-major tiles of RA / RB rows.
-template <int NS, int RA, int RB>
-__device__ __forceinline__ void scores(uint32_t d, uint32_t a, uint32_t b, int dim, int chunks, uint32_t idesc) {
+// Rows [0, R) of a tile from p (element strides `step` a row, dim entries a row, entries
+// beyond dim up to the next multiple of 16 zero), row r only if live(r), by `n` threads of index
+// t, through registers. Parts of a split type follow each other.
+template <typename T, int NS, bool PIECES, int R, typename L, typename Live>
+__device__ __forceinline__ void load_tile(unsigned char* dst, const T* p, int64_t step, int dim, int t, int n, Live live) {
+  const int pieces = (dim + 15) / 16 * 2;  // of 8 entries
+  const int dr = n / pieces, dc = n - dr * pieces;
+  int r = t / pieces, c = t - r * pieces;
+  while (r < R) {
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 0.f;
+    if (live(r)) {
+      const T* s = p + r * step + c * 8;
+      if constexpr (PIECES) {
+        constexpr int V = 16 / sizeof(T);
+#pragma unroll
+        for (int h = 0; h < 8; h += V) {
+          if (c * 8 + h < dim) {
+            const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(s + h);
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[h + e] = to_f(k.e[e]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c * 8 + e < dim) x[e] = to_f(s[e]);
+      }
+    }
+    uint32_t w[4][NS];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split2<NS>(x[2 * e], x[2 * e + 1], w[e]);
+    unsigned char* d = dst + L::at(R, r, c);
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+      *reinterpret_cast<uint4*>(d + s * (R * L::RB * L::DC)) = make_uint4(w[0][s], w[1][s], w[2][s], w[3][s]);
+    r += dr;
+    c += dc;
+    if (c >= pieces) {
+      c -= pieces;
+      ++r;
+    }
+  }
+}
+
+// D (+)= A B^T over the k-steps of 16 entries, both K-major tiles of RA / RB rows.
+template <int NS, int RA, int RB, typename L>
+__device__ __forceinline__ void scores(uint32_t d, uint32_t a, uint32_t b, int dim, uint32_t idesc) {
   const int steps = (dim + 15) / 16;
+  constexpr int K = L::RB / 32;  // steps of a chunk
   bool acc = false;
   // the smaller products first
 #pragma unroll
   for (int sum = NS - 1; sum >= 0; --sum) {
 #pragma unroll
     for (int i = 0; i <= sum; ++i) {
-      const uint32_t ap = a + i * (RA * 128u * chunks), bp = b + (sum - i) * (RB * 128u * chunks);
+      const uint32_t ap = a + i * (RA * L::RB * L::DC), bp = b + (sum - i) * (RB * L::RB * L::DC);
       for (int k = 0; k < steps; ++k) {
-        mma_ss(d, desc_sw128(ap + (k >> 2) * (RA * 128u) + (k & 3) * 32u, 16),
-               desc_sw128(bp + (k >> 2) * (RB * 128u) + (k & 3) * 32u, 16), idesc, acc);
+        mma_ss(d, desc<L::RB>(ap + (k / K) * (RA * L::RB) + (k % K) * 32u, 16),
+               desc<L::RB>(bp + (k / K) * (RB * L::RB) + (k % K) * 32u, 16), idesc, acc);
         acc = true;
       }
     }
   }
 }
 
-// D (+)= A B, A in TMEM (NS parts, `apart` columns apart; k-step kk at a + acol(kk)), B the
-// MN-major view of a tile of RB rows (the contraction's index).
-template <int NS, int RB, typename Col>
-__device__ __forceinline__ void values(uint32_t d, uint32_t a, uint32_t apart, uint32_t b, int chunks, uint32_t idesc,
-                                       bool acc, Col acol) {
+// D (+)= A B, A in TMEM (8 columns a part and k-step, from acol(part, k)), B the MN-major view
+// of a tile of RB rows (the contraction's index).
+template <int NS, int RB, typename L, typename Col>
+__device__ __forceinline__ void values(uint32_t d, uint32_t b, uint32_t idesc, bool acc, Col acol) {
 #pragma unroll
   for (int sum = NS - 1; sum >= 0; --sum) {
 #pragma unroll
     for (int i = 0; i <= sum; ++i) {
-      const uint32_t bp = b + (sum - i) * (RB * 128u * chunks);
+      const uint32_t bp = b + (sum - i) * (RB * L::RB * L::DC);
 #pragma unroll
       for (int k = 0; k < RB / 16; ++k) {
-        mma_ts(d, a + i * apart + acol(k), desc_sw128(bp + k * 2048u, RB * 128u), idesc, acc);
+        mma_ts(d, acol(i, k), desc<L::RB>(bp + k * 16u * L::RB, RB * L::RB), idesc, acc);
         acc = true;
       }
     }
@@ -253,40 +297,44 @@ __device__ __forceinline__ uint32_t fill_info(TileInfo<R>& I, int sub, Live live
 // exponentials run while the other's products do. The probabilities overwrite (QT = 2) or
 // follow the scores in TMEM and are the A operand of the second product. The output is
 // rescaled only when the maximum has grown by more than 2^8.
-template <typename T, int NS, int QT, int BN, int DC, int ST>
+template <int NS, int QT, int BN, typename L, int ST>
 struct FwdShape {
   static constexpr int kThreads = 128 * QT + 128;
-  static constexpr uint32_t kQ = NS * DC * 16384u, kKV = NS * DC * BN * 128u;
+  static constexpr uint32_t kRow = NS * L::DC * L::RB, kQ = 128 * kRow, kKV = BN * kRow;
   static constexpr int kInfo = ST + 1;
   static constexpr uint32_t kTileBytes = QT * kQ + 2 * ST * kKV;
   // TMEM columns of a tile: scores, then (NS > 1) the probabilities' parts, then the output
   static constexpr int kP = NS == 1 ? 0 : BN;
   static constexpr int kO = NS == 1 ? BN : BN + NS * BN / 2;
-  static constexpr int kCols = QT * (kO + 64 * DC);
+  static constexpr int kTile = kO + L::kDim;
+  static constexpr int kCols = QT * kTile;
   static constexpr int kAlloc = kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
+  // blocks an SM holds by TMEM and shared memory (float32's parts of 128 entries: one)
+  static constexpr int kBlocks = QT == 1 && kAlloc <= 256 && kTileBytes <= 104 * 1024 ? 2 : 1;
 };
 
-template <typename T, int NS, int QT, int BN, int DC, int ST, bool VEC>
-__global__ void __launch_bounds__(FwdShape<T, NS, QT, BN, DC, ST>::kThreads, QT == 1 && DC == 1 ? 2 : 1)
-    attn_fwd_kernel(const __grid_constant__ AttnArgs A) {
-  using S = FwdShape<T, NS, QT, BN, DC, ST>;
+template <typename T, int NS, int QT, int BN, typename L, int ST, int LOAD>
+__global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShape<NS, QT, BN, L, ST>::kBlocks)
+    attn_fwd_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TmaMaps M) {
+  using S = FwdShape<NS, QT, BN, L, ST>;
+  constexpr bool TMA = LOAD == LOAD_TMA, PIECES = LOAD == LOAD_PIECES;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   unsigned char *sQ = sm, *sK = sm + QT * S::kQ, *sV = sK + ST * S::kKV;
   float* lut = reinterpret_cast<float*>(sm + S::kTileBytes);
   __shared__ TileInfo<BN> info[S::kInfo];
-  __shared__ uint64_t kfull[ST], vfull[ST], kempty[ST], vempty[ST], sfull[QT], pfull[QT], done;
+  __shared__ uint64_t kfull[ST], vfull[ST], kempty[ST], vempty[ST], kraw[ST], vraw[ST], qraw, sfull[QT], pfull[QT], done;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   __shared__ int last_live;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  // block -> (batch, head, query block); late query blocks first (causal: the longest)
-  int64_t blk = blockIdx.x;
-  const int64_t nq = (A.Lq + 128 * QT - 1) / (128 * QT);
-  const int64_t qb = nq - 1 - blk % nq;
-  blk /= nq;
-  const int h = (int)(blk % A.H), b = (int)(blk / A.H), hk = h / (A.H / A.Hk);
+  // block -> (batch, head, query block); under a causal order the longest blocks first
+  const int64_t nq = (A.Lq + 128 * QT - 1) / (128 * QT), heads = (int64_t)A.B * A.H;
+  const bool ordered = A.causal && !A.q_pos && !A.k_pos;
+  const int64_t qb = ordered ? nq - 1 - blockIdx.x / heads : blockIdx.x % nq;
+  const int64_t bh = ordered ? blockIdx.x % heads : blockIdx.x / nq;
+  const int h = (int)(bh % A.H), b = (int)(bh / A.H), hk = h / (A.H / A.Hk);
   const int64_t i0 = qb * 128 * QT;
   const uint8_t* mask = A.mask ? A.mask + b * A.mask_stride : nullptr;
   const int reach = A.buckets.reach;
@@ -295,35 +343,42 @@ __global__ void __launch_bounds__(FwdShape<T, NS, QT, BN, DC, ST>::kThreads, QT 
     abort_flag = 0;
     last_live = mask ? 0 : (int)A.Lk;
     for (int i = 0; i < ST; ++i) {
-      mbar_init(&kfull[i], 96);
-      mbar_init(&vfull[i], 96);
+      mbar_init(&kfull[i], TMA ? 64 : 96);
+      mbar_init(&vfull[i], TMA ? 64 : 96);
       mbar_init(&kempty[i], 1);
       mbar_init(&vempty[i], 1);
+      mbar_init(&kraw[i], 2);  // the copies, and the positions
+      mbar_init(&vraw[i], 1);
     }
+    mbar_init(&qraw, 1);
     for (int t = 0; t < QT; ++t) {
       mbar_init(&sfull[t], 1);
       mbar_init(&pfull[t], 128);
     }
     mbar_init(&done, 1);
     fence_mbar_init();
+    if constexpr (TMA) {
+      mbar_arrive_expect_tx(&qraw, QT * S::kQ);
+      for (int t = 0; t < QT; ++t) tma_tile<L>(sQ + t * S::kQ, M, MAP_Q, 128, i0 + t * 128, h, b, &qraw);
+    }
   }
   if (warp == 0) {
     tmem_alloc(&tmem_slot, S::kAlloc);
     tmem_relinquish();
   }
-  const T* Q = static_cast<const T*>(A.q) + b * A.qs[0] + h * A.qs[1];
+  if constexpr (!TMA) {
+    const T* Q = static_cast<const T*>(A.q) + b * A.qs[0] + h * A.qs[1];
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int64_t first = i0 + t * 128;
-    load_tile<T, NS, VEC, 128>(sQ + t * S::kQ, Q + first * A.qs[2], A.qs[2], A.D, DC, tid, S::kThreads,
-                               [&](int r) { return first + r < A.Lq; });
+    for (int t = 0; t < QT; ++t) {
+      const int64_t first = i0 + t * 128;
+      load_tile<T, NS, PIECES, 128, L>(sQ + t * S::kQ, Q + first * A.qs[2], A.qs[2], A.D, tid, S::kThreads,
+                                       [&](int r) { return first + r < A.Lq; });
+    }
   }
   if (A.table) {
     const T* t = static_cast<const T*>(A.table) + (int64_t)h * A.buckets.num_buckets;
     for (int d = tid; d <= 2 * reach; d += S::kThreads) lut[d] = bias2(to_f(t[bucket_of(A.buckets, d - reach)]));
   }
-  cp_commit();
-  cp_wait<0>();
   fence_proxy_async_smem();
   fence_before_sync();
   __syncthreads();
@@ -336,7 +391,7 @@ __global__ void __launch_bounds__(FwdShape<T, NS, QT, BN, DC, ST>::kThreads, QT 
     __syncthreads();
   }
   int64_t keys = last_live;
-  if (A.causal && !A.q_pos && !A.k_pos) {
+  if (ordered) {
     const int64_t end = i0 + 128 * QT < A.Lq ? i0 + 128 * QT : A.Lq;
     const int64_t seen = A.Lk - A.Lq + end;
     keys = seen < keys ? (seen > 0 ? seen : 0) : keys;
@@ -353,7 +408,7 @@ __global__ void __launch_bounds__(FwdShape<T, NS, QT, BN, DC, ST>::kThreads, QT 
     const int qp = valid ? attn_q_pos(A, b, i) : 0;
     const int qlo = __reduce_min_sync(0xffffffffu, valid ? qp : INT32_MAX);
     const int qhi = __reduce_max_sync(0xffffffffu, valid ? qp : INT32_MIN);
-    const uint32_t base = tmem + ((uint32_t)(warp & 3) << 21) + t * (S::kO + 64 * DC);
+    const uint32_t base = tmem + ((uint32_t)(warp & 3) << 21) + t * S::kTile;
     float m = -INFINITY, l = 0.f;  // m: the reference the exponentials are taken to
     for (int j = 0; j < tiles; ++j) {
       const TileInfo<BN>& I = info[j % S::kInfo];
@@ -411,7 +466,7 @@ __global__ void __launch_bounds__(FwdShape<T, NS, QT, BN, DC, ST>::kThreads, QT 
         l *= f;
         if (j > 0) {
 #pragma unroll
-          for (int c = 0; c < 64 * DC; c += 16) {
+          for (int c = 0; c < L::kDim; c += 16) {
             if (c < A.D) {
               uint32_t o[16];
               ld16(base + S::kO + c, o);
@@ -455,7 +510,7 @@ __global__ void __launch_bounds__(FwdShape<T, NS, QT, BN, DC, ST>::kThreads, QT 
     const bool ovec =
         A.D % V == 0 && ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(A.os[2] * sizeof(T))) & 15) == 0;
 #pragma unroll
-    for (int c = 0; c < 64 * DC; c += 16) {
+    for (int c = 0; c < L::kDim; c += 16) {
       if (c < A.D) {
         uint32_t o[16];
         if (tiles > 0) {
@@ -485,10 +540,11 @@ __global__ void __launch_bounds__(FwdShape<T, NS, QT, BN, DC, ST>::kThreads, QT 
     if (lane == 0 && tiles > 0) {
       const uint32_t id_s = idesc_bf16(128, BN, false), id_o = idesc_bf16(128, (A.D + 15) / 16 * 16, true);
       const uint32_t aQ = smem_u32(sQ), aK = smem_u32(sK), aV = smem_u32(sV);
+      if constexpr (TMA) wait(&qraw, 0, &abort_flag, polls);
       wait(&kfull[0], 0, &abort_flag, polls);
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
-        scores<NS, 128, BN>(tmem + t * (S::kO + 64 * DC), aQ + t * S::kQ, aK, A.D, DC, id_s);
+        scores<NS, 128, BN, L>(tmem + t * S::kTile, aQ + t * S::kQ, aK, A.D, id_s);
         mma_commit(&sfull[t]);
       }
       mma_commit(&kempty[0]);
@@ -498,12 +554,13 @@ __global__ void __launch_bounds__(FwdShape<T, NS, QT, BN, DC, ST>::kThreads, QT 
         if (j + 1 < tiles) wait(&kfull[sn], ((j + 1) / ST) & 1, &abort_flag, polls);
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
-          const uint32_t d = tmem + t * (S::kO + 64 * DC);
+          const uint32_t d = tmem + t * S::kTile;
           wait(&pfull[t], j & 1, &abort_flag, polls);
           fence_after_sync();
-          values<NS, BN>(d + S::kO, d + S::kP, BN / 2, aV + st * S::kKV, DC, id_o, j > 0, [](int k) { return k * 8; });
+          values<NS, BN, L>(d + S::kO, aV + st * S::kKV, id_o, j > 0,
+                            [=](int part, int k) { return d + S::kP + part * (BN / 2) + k * 8; });
           if (t == QT - 1) mma_commit(&vempty[st]);
-          if (j + 1 < tiles) scores<NS, 128, BN>(d, aQ + t * S::kQ, aK + sn * S::kKV, A.D, DC, id_s);
+          if (j + 1 < tiles) scores<NS, 128, BN, L>(d, aQ + t * S::kQ, aK + sn * S::kKV, A.D, id_s);
           mma_commit(&sfull[t]);  // after the last keys: the output is whole
         }
         if (j + 1 < tiles) mma_commit(&kempty[sn]);
@@ -516,41 +573,66 @@ __global__ void __launch_bounds__(FwdShape<T, NS, QT, BN, DC, ST>::kThreads, QT 
   } else {
     // -------------------------------------------------------- loads
     const int t = tid - 128 * QT - 32, w = t >> 5;
-    const T* K = static_cast<const T*>(A.k) + b * A.ks[0] + hk * A.ks[1];
-    const T* V = static_cast<const T*>(A.v) + b * A.vs[0] + hk * A.vs[1];
-    constexpr bool ASYNC = NS == 1 && VEC && sizeof(T) == 2;
-    for (int j = 0; j < tiles; ++j) {
-      const int st = j % ST;
+    const auto fill = [&](int j, int sub) {
       const int64_t j0 = (int64_t)j * BN;
-      TileInfo<BN>& I = info[j % S::kInfo];
-      if (j >= ST) wait(&kempty[st], (j / ST - 1) & 1, &abort_flag, polls);
-      for (int sub = w; sub < BN / kSub; sub += 3)
-        fill_info<BN>(
-            I, sub, [&](int e) { return j0 + e < A.Lk && (!mask || mask[j0 + e]); },
-            [&](int e) { return attn_k_pos(A, b, j0 + e); });
-      named_barrier(1, 96);
-      const auto live = [&](int r) { return (I.live[r >> 5] >> (r & 31)) & 1u; };
-      load_tile<T, NS, VEC, BN>(sK + st * S::kKV, K + j0 * A.ks[2], A.ks[2], A.D, DC, t, 96, live);
-      if constexpr (ASYNC) {
-        cp_commit();
-        if (j > 0) {  // the values of the tile before have landed
-          cp_wait<1>();
-          fence_proxy_async_smem();
-          arrive(&vfull[(j - 1) % ST]);
+      fill_info<BN>(
+          info[j % S::kInfo], sub, [&](int e) { return j0 + e < A.Lk && (!mask || mask[j0 + e]); },
+          [&](int e) { return attn_k_pos(A, b, j0 + e); });
+    };
+    if constexpr (TMA) {
+      if (w == 0) {
+        for (int j = 0; j < tiles; ++j) {
+          const int st = j % ST;
+          if (j >= ST) wait(&kempty[st], (j / ST - 1) & 1, &abort_flag, polls);
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&kraw[st], S::kKV);
+            tma_tile<L>(sK + st * S::kKV, M, MAP_K, BN, (int64_t)j * BN, hk, b, &kraw[st]);
+          }
+          for (int sub = 0; sub < BN / kSub; ++sub) fill(j, sub);
+          __syncwarp();
+          if (lane == 0) arrive(&kraw[st]);
+          if (j >= ST) wait(&vempty[st], (j / ST - 1) & 1, &abort_flag, polls);
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&vraw[st], S::kKV);
+            tma_tile<L>(sV + st * S::kKV, M, MAP_V, BN, (int64_t)j * BN, hk, b, &vraw[st]);
+          }
         }
-        cp_wait<0>();
+      } else {
+        for (int j = 0; j < tiles; ++j) {
+          const int st = j % ST;
+          const TileInfo<BN>& I = info[j % S::kInfo];
+          const auto live = [&](int r) { return (I.live[r >> 5] >> (r & 31)) & 1u; };
+          if (mask) wait(&vraw[st], (j / ST) & 1, &abort_flag, polls);
+          wait(&kraw[st], (j / ST) & 1, &abort_flag, polls);
+          if (mask) {
+            clear_rows<L>(sK + st * S::kKV, BN, t - 32, 64, live);
+            clear_rows<L>(sV + st * S::kKV, BN, t - 32, 64, live);
+            fence_proxy_async_smem();
+          }
+          arrive(&kfull[st]);
+          if (!mask) wait(&vraw[st], (j / ST) & 1, &abort_flag, polls);
+          arrive(&vfull[st]);
+        }
       }
-      fence_proxy_async_smem();
-      arrive(&kfull[st]);
-      if (j >= ST) wait(&vempty[st], (j / ST - 1) & 1, &abort_flag, polls);
-      load_tile<T, NS, VEC, BN>(sV + st * S::kKV, V + j0 * A.vs[2], A.vs[2], A.D, DC, t, 96, live);
-      if constexpr (ASYNC) {
-        cp_commit();
-        if (j + 1 < tiles) continue;
-        cp_wait<0>();
+    } else {
+      const T* K = static_cast<const T*>(A.k) + b * A.ks[0] + hk * A.ks[1];
+      const T* V = static_cast<const T*>(A.v) + b * A.vs[0] + hk * A.vs[1];
+      for (int j = 0; j < tiles; ++j) {
+        const int st = j % ST;
+        const int64_t j0 = (int64_t)j * BN;
+        TileInfo<BN>& I = info[j % S::kInfo];
+        if (j >= ST) wait(&kempty[st], (j / ST - 1) & 1, &abort_flag, polls);
+        for (int sub = w; sub < BN / kSub; sub += 3) fill(j, sub);
+        named_barrier(1, 96);
+        const auto live = [&](int r) { return (I.live[r >> 5] >> (r & 31)) & 1u; };
+        load_tile<T, NS, PIECES, BN, L>(sK + st * S::kKV, K + j0 * A.ks[2], A.ks[2], A.D, t, 96, live);
+        fence_proxy_async_smem();
+        arrive(&kfull[st]);
+        if (j >= ST) wait(&vempty[st], (j / ST - 1) & 1, &abort_flag, polls);
+        load_tile<T, NS, PIECES, BN, L>(sV + st * S::kKV, V + j0 * A.vs[2], A.vs[2], A.D, t, 96, live);
+        fence_proxy_async_smem();
+        arrive(&vfull[st]);
       }
-      fence_proxy_async_smem();
-      arrive(&vfull[st]);
     }
   }
   fence_before_sync();

@@ -49,12 +49,12 @@ __global__ void __launch_bounds__(256) attn_prep_kernel(const __grid_constant__ 
 }
 
 // Row r of the block from TMEM (columns col ..), times f, to p (zero: 0).
-template <typename T, int DC>
+template <typename T, int DIM>
 __device__ __forceinline__ void store_row(uint32_t taddr, T* p, int64_t step, int dim, float f, bool zero, bool valid) {
   constexpr int V = 16 / sizeof(T);
   const bool vec = dim % V == 0 && ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(step * sizeof(T))) & 15) == 0;
 #pragma unroll
-  for (int c = 0; c < 64 * DC; c += 16) {
+  for (int c = 0; c < DIM; c += 16) {
     if (c < dim) {
       uint32_t o[16];
       ld16(taddr + c, o);
@@ -78,17 +78,18 @@ __device__ __forceinline__ void store_row(uint32_t taddr, T* p, int64_t step, in
 }
 
 // ---------------------------------------------------------------- dk, dv
-template <int NS, int DC, int ST>
+template <int NS, typename L, int ST>
 struct DkvShape {
   static constexpr int kThreads = 384;  // 8 warps on the scores, one issuing, three loading
-  static constexpr uint32_t kOwn = NS * DC * 16384u, kTile = NS * DC * kGradN * 128u;
+  static constexpr uint32_t kRow = NS * L::DC * L::RB, kOwn = 128 * kRow, kTile = kGradN * kRow;
   static constexpr uint32_t kTileBytes = 2 * kOwn + 2 * ST * kTile;
-  // TMEM: scores, do.v, [p, ds: NS parts of 32 columns], dv, dk. With one part p and ds take the
-  // place of the scores: each half of the columns in the place of its own half.
-  static constexpr int kDp = kGradN, kP = NS == 1 ? 0 : 2 * kGradN, kDs = NS == 1 ? kGradN : kP + NS * 32;
-  static constexpr int kDv = NS == 1 ? 2 * kGradN : kDs + NS * 32, kDk = kDv + 64 * DC;
-  static constexpr int kCols = kDk + 64 * DC, kAlloc = kCols <= 256 ? 256 : 512;
+  // TMEM: scores, do.v, [third parts of p and ds], dv, dk. p and ds of 16 columns take the place of
+  // those 16 once read: 8 columns a part, two parts; the third has 32 columns of its own.
+  static constexpr int kDp = kGradN, kP3 = 2 * kGradN, kDs3 = kP3 + 32;
+  static constexpr int kDv = NS == 1 ? 2 * kGradN : kDs3 + 32, kDk = kDv + L::kDim;
+  static constexpr int kCols = kDk + L::kDim, kAlloc = kCols <= 256 ? 256 : 512;
   static constexpr int kInfo = ST + 1;
+  static constexpr int kBlocks = kAlloc <= 256 && kTileBytes <= 104 * 1024 ? 2 : 1;  // an SM holds
 };
 
 struct alignas(16) QueryInfo {
@@ -96,18 +97,17 @@ struct alignas(16) QueryInfo {
   float lse[kGradN], delta[kGradN];  // lse +inf: a row without keys, or past the end
 };
 
-template <typename T, int NS, int DC, int ST, bool VEC>
-__global__ void __launch_bounds__(DkvShape<NS, DC, ST>::kThreads, NS == 1 && DC == 1 ? 2 : 1)
-    attn_dkv_kernel(const __grid_constant__ AttnArgs A) {
-  using S = DkvShape<NS, DC, ST>;
-  constexpr bool ASYNC = NS == 1 && VEC && sizeof(T) == 2;
-  static_assert(!ASYNC || ST >= 2, "a tile's arrival is told after the next one's issue");
+template <typename T, int NS, typename L, int ST, int LOAD>
+__global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L, ST>::kBlocks)
+    attn_dkv_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TmaMaps M) {
+  using S = DkvShape<NS, L, ST>;
+  constexpr bool TMA = LOAD == LOAD_TMA, PIECES = LOAD == LOAD_PIECES;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   unsigned char *sK = sm, *sV = sm + S::kOwn, *sQ = sV + S::kOwn, *sO = sQ + ST * S::kTile;
   float* lut = reinterpret_cast<float*>(sm + S::kTileBytes);
   __shared__ QueryInfo info[S::kInfo];
-  __shared__ uint64_t full[ST], empty[ST], sfull, pfull, done;
+  __shared__ uint64_t full[ST], empty[ST], loaded[ST], own, sfull, pfull, done;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = A.H / A.Hk;
@@ -125,9 +125,11 @@ __global__ void __launch_bounds__(DkvShape<NS, DC, ST>::kThreads, NS == 1 && DC 
   if (tid == 0) {
     abort_flag = 0;
     for (int i = 0; i < ST; ++i) {
-      mbar_init(&full[i], 96);
+      mbar_init(&full[i], TMA ? 64 : 96);
       mbar_init(&empty[i], 1);
+      mbar_init(&loaded[i], 2);  // the copies, and what goes with the rows
     }
+    mbar_init(&own, 1);
     mbar_init(&sfull, 1);
     mbar_init(&pfull, 256);
     mbar_init(&done, 1);
@@ -137,13 +139,25 @@ __global__ void __launch_bounds__(DkvShape<NS, DC, ST>::kThreads, NS == 1 && DC 
     tmem_alloc(&tmem_slot, S::kAlloc);
     tmem_relinquish();
   }
-  const T* K = static_cast<const T*>(A.k) + b * A.ks[0] + hk * A.ks[1] + j0 * A.ks[2];
-  const T* V = static_cast<const T*>(A.v) + b * A.vs[0] + hk * A.vs[1] + j0 * A.vs[2];
   const auto key_live = [&](int r) { return j0 + r < A.Lk && (!mask || mask[j0 + r]); };
-  load_tile<T, NS, VEC, 128>(sK, K, A.ks[2], A.D, DC, tid, S::kThreads, key_live);
-  load_tile<T, NS, VEC, 128>(sV, V, A.vs[2], A.D, DC, tid, S::kThreads, key_live);
-  cp_commit();
-  cp_wait<0>();
+  if constexpr (TMA) {
+    if (tid == 0) {
+      mbar_arrive_expect_tx(&own, 2 * S::kOwn);
+      tma_tile<L>(sK, M, MAP_K, 128, j0, hk, b, &own);
+      tma_tile<L>(sV, M, MAP_V, 128, j0, hk, b, &own);
+    }
+    __syncthreads();
+    wait(&own, 0, &abort_flag, A.polls);
+    if (mask) {
+      clear_rows<L>(sK, 128, tid, S::kThreads, key_live);
+      clear_rows<L>(sV, 128, tid, S::kThreads, key_live);
+    }
+  } else {
+    const T* K = static_cast<const T*>(A.k) + b * A.ks[0] + hk * A.ks[1] + j0 * A.ks[2];
+    const T* V = static_cast<const T*>(A.v) + b * A.vs[0] + hk * A.vs[1] + j0 * A.vs[2];
+    load_tile<T, NS, PIECES, 128, L>(sK, K, A.ks[2], A.D, tid, S::kThreads, key_live);
+    load_tile<T, NS, PIECES, 128, L>(sV, V, A.vs[2], A.D, tid, S::kThreads, key_live);
+  }
   fence_proxy_async_smem();
   fence_before_sync();
   __syncthreads();
@@ -222,11 +236,10 @@ __global__ void __launch_bounds__(DkvShape<NS, DC, ST>::kThreads, NS == 1 && DC 
             for (int i = 0; i < NS; ++i) wd[i][(e + f) / 2] = o[i];
           }
         }
-        const uint32_t at = NS == 1 ? col - c + c / 2 : col / 2;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-          st8(base + S::kP + i * 32 + at, wp[i]);
-          st8(base + S::kDs + i * 32 + at, wd[i]);
+          st8(base + (i < 2 ? col + i * 8 : S::kP3 + col / 2), wp[i]);
+          st8(base + (i < 2 ? S::kDp + col + i * 8 : S::kDs3 + col / 2), wd[i]);
         }
       }
       tmem_wait_st();
@@ -240,27 +253,30 @@ __global__ void __launch_bounds__(DkvShape<NS, DC, ST>::kThreads, NS == 1 && DC 
     const bool zero = !live || tiles == 0, valid = j < A.Lk;
     const float f = abort_flag ? NAN : 1.f;
     if (wg == 0)
-      store_row<T, DC>(base + S::kDv, static_cast<T*>(A.dv) + b * A.dvs[0] + hk * A.dvs[1] + j * A.dvs[2], A.dvs[2], A.D,
+      store_row<T, L::kDim>(base + S::kDv, static_cast<T*>(A.dv) + b * A.dvs[0] + hk * A.dvs[1] + j * A.dvs[2], A.dvs[2], A.D,
                        f, zero, valid);
     else
-      store_row<T, DC>(base + S::kDk, static_cast<T*>(A.dk) + b * A.dks[0] + hk * A.dks[1] + j * A.dks[2], A.dks[2], A.D,
+      store_row<T, L::kDim>(base + S::kDk, static_cast<T*>(A.dk) + b * A.dks[0] + hk * A.dks[1] + j * A.dks[2], A.dks[2], A.D,
                        f * A.scale, zero, valid);
   } else if (warp == 8) {
     if (lane == 0 && tiles > 0) {
       const uint32_t id_s = idesc_bf16(128, kGradN, false), id_o = idesc_bf16(128, (A.D + 15) / 16 * 16, true);
       const uint32_t aK = smem_u32(sK), aV = smem_u32(sV);
-      const auto acol = [](int k) { return NS == 1 ? (k >> 1) * 32 + (k & 1) * 8 : k * 8; };
+      const auto p_at = [=](int part, int k) { return tmem + (part < 2 ? k * 16 + part * 8 : S::kP3 + k * 8); };
+      const auto ds_at = [=](int part, int k) {
+        return tmem + (part < 2 ? S::kDp + k * 16 + part * 8 : S::kDs3 + k * 8);
+      };
       for (int64_t it = 0; it < tiles; ++it) {
         const int st = (int)(it % ST);
         const uint32_t aQ = smem_u32(sQ) + st * S::kTile, aO = smem_u32(sO) + st * S::kTile;
         wait(&full[st], (it / ST) & 1, &abort_flag, polls);
-        scores<NS, 128, kGradN>(tmem, aK, aQ, A.D, DC, id_s);
-        scores<NS, 128, kGradN>(tmem + S::kDp, aV, aO, A.D, DC, id_s);
+        scores<NS, 128, kGradN, L>(tmem, aK, aQ, A.D, id_s);
+        scores<NS, 128, kGradN, L>(tmem + S::kDp, aV, aO, A.D, id_s);
         mma_commit(&sfull);
         wait(&pfull, it & 1, &abort_flag, polls);
         fence_after_sync();
-        values<NS, kGradN>(tmem + S::kDv, tmem + S::kP, 32, aO, DC, id_o, it > 0, acol);
-        values<NS, kGradN>(tmem + S::kDk, tmem + S::kDs, 32, aQ, DC, id_o, it > 0, acol);
+        values<NS, kGradN, L>(tmem + S::kDv, aO, id_o, it > 0, p_at);
+        values<NS, kGradN, L>(tmem + S::kDk, aQ, id_o, it > 0, ds_at);
         mma_commit(&empty[st]);
       }
       mma_commit(&sfull);
@@ -271,42 +287,65 @@ __global__ void __launch_bounds__(DkvShape<NS, DC, ST>::kThreads, NS == 1 && DC 
     }
   } else {
     const int t = tid - 288, w = t >> 5;
-    for (int64_t it = 0; it < tiles; ++it) {
-      const int st = (int)(it % ST), h = (int)(hk * G + it / per);
-      const int64_t i0 = (q0 + it % per) * kGradN;
+    // lse, delta and positions of 32 rows of a tile, by a warp
+    const auto fill = [&](int64_t it, int sub) {
       QueryInfo& I = info[it % S::kInfo];
-      if (it >= ST) wait(&empty[st], (it / ST - 1) & 1, &abort_flag, polls);
-      const float* lse = A.lse + ((int64_t)b * A.H + h) * A.Lq;
-      const float* delta = A.delta + ((int64_t)b * A.H + h) * A.Lq;
-      if (w < kGradN / kSub) {
-        const uint32_t bits = fill_info<kGradN>(
-            I.t, w, [&](int e) { return i0 + e < A.Lq && lse[i0 + e] != -INFINITY; },
-            [&](int e) { return attn_q_pos(A, b, i0 + e); });
-        const int e = w * kSub + lane;
-        const bool ok = (bits >> lane) & 1u;
-        I.lse[e] = ok ? lse[i0 + e] : INFINITY;
-        I.delta[e] = ok ? delta[i0 + e] : 0.f;
-      }
-      named_barrier(1, 96);
-      const auto row_live = [&](int r) { return (I.t.live[r >> 5] >> (r & 31)) & 1u; };
-      load_tile<T, NS, VEC, kGradN>(
-          sQ + st * S::kTile, static_cast<const T*>(A.q) + b * A.qs[0] + h * A.qs[1] + i0 * A.qs[2], A.qs[2], A.D, DC, t,
-          96, row_live);
-      load_tile<T, NS, VEC, kGradN>(
-          sO + st * S::kTile, static_cast<const T*>(A.dout) + b * A.dos[0] + h * A.dos[1] + i0 * A.dos[2], A.dos[2], A.D,
-          DC, t, 96, row_live);
-      if constexpr (ASYNC) {
-        cp_commit();
-        if (it > 0) {
-          cp_wait<1>();
-          fence_proxy_async_smem();
-          arrive(&full[(it - 1) % ST]);
+      const int64_t i0 = (q0 + it % per) * kGradN, row = ((int64_t)b * A.H + hk * G + it / per) * A.Lq;
+      const int e = sub * kSub + lane;
+      const float ls = i0 + e < A.Lq ? A.lse[row + i0 + e] : -INFINITY;
+      const uint32_t bits = fill_info<kGradN>(
+          I.t, sub, [&](int) { return ls != -INFINITY; }, [&](int x) { return attn_q_pos(A, b, i0 + x); });
+      const bool ok = (bits >> lane) & 1u;
+      I.lse[e] = ok ? ls : INFINITY;
+      I.delta[e] = ok ? A.delta[row + i0 + e] : 0.f;
+    };
+    if constexpr (TMA) {
+      if (w == 0) {
+        for (int64_t it = 0; it < tiles; ++it) {
+          const int st = (int)(it % ST), h = (int)(hk * G + it / per);
+          const int64_t i0 = (q0 + it % per) * kGradN;
+          if (it >= ST) wait(&empty[st], (it / ST - 1) & 1, &abort_flag, polls);
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&loaded[st], 2 * S::kTile);
+            tma_tile<L>(sQ + st * S::kTile, M, MAP_Q, kGradN, i0, h, b, &loaded[st]);
+            tma_tile<L>(sO + st * S::kTile, M, MAP_DO, kGradN, i0, h, b, &loaded[st]);
+          }
+          for (int sub = 0; sub < kGradN / kSub; ++sub) fill(it, sub);
+          __syncwarp();
+          if (lane == 0) arrive(&loaded[st]);
         }
-        if (it + 1 < tiles) continue;
-        cp_wait<0>();
+      } else {
+        for (int64_t it = 0; it < tiles; ++it) {
+          const int st = (int)(it % ST);
+          const QueryInfo& I = info[it % S::kInfo];
+          wait(&loaded[st], (it / ST) & 1, &abort_flag, polls);
+          if ((I.t.live[0] & I.t.live[1]) != 0xffffffffu) {
+            const auto row_live = [&](int r) { return (I.t.live[r >> 5] >> (r & 31)) & 1u; };
+            clear_rows<L>(sQ + st * S::kTile, kGradN, t - 32, 64, row_live);
+            clear_rows<L>(sO + st * S::kTile, kGradN, t - 32, 64, row_live);
+            fence_proxy_async_smem();
+          }
+          arrive(&full[st]);
+        }
       }
-      fence_proxy_async_smem();
-      arrive(&full[st]);
+    } else {
+      for (int64_t it = 0; it < tiles; ++it) {
+        const int st = (int)(it % ST), h = (int)(hk * G + it / per);
+        const int64_t i0 = (q0 + it % per) * kGradN;
+        const QueryInfo& I = info[it % S::kInfo];
+        if (it >= ST) wait(&empty[st], (it / ST - 1) & 1, &abort_flag, polls);
+        if (w < kGradN / kSub) fill(it, w);
+        named_barrier(1, 96);
+        const auto row_live = [&](int r) { return (I.t.live[r >> 5] >> (r & 31)) & 1u; };
+        load_tile<T, NS, PIECES, kGradN, L>(
+            sQ + st * S::kTile, static_cast<const T*>(A.q) + b * A.qs[0] + h * A.qs[1] + i0 * A.qs[2], A.qs[2], A.D, t, 96,
+            row_live);
+        load_tile<T, NS, PIECES, kGradN, L>(
+            sO + st * S::kTile, static_cast<const T*>(A.dout) + b * A.dos[0] + h * A.dos[1] + i0 * A.dos[2], A.dos[2], A.D,
+            t, 96, row_live);
+        fence_proxy_async_smem();
+        arrive(&full[st]);
+      }
     }
   }
   fence_before_sync();
@@ -316,15 +355,17 @@ __global__ void __launch_bounds__(DkvShape<NS, DC, ST>::kThreads, NS == 1 && DC 
 }
 
 // ---------------------------------------------------------------- dq, dtable
-template <int NS, int DC, int ST>
+template <int NS, typename L, int ST>
 struct DqShape {
   static constexpr int kThreads = 256;  // 4 warps on the scores, one issuing, three loading
-  static constexpr uint32_t kOwn = NS * DC * 16384u, kTile = NS * DC * kGradN * 128u;
+  static constexpr uint32_t kRow = NS * L::DC * L::RB, kOwn = 128 * kRow, kTile = kGradN * kRow;
   static constexpr uint32_t kTileBytes = 2 * kOwn + 2 * ST * kTile;
-  // TMEM: scores, do.v, [ds: NS parts], dq. With one part ds follows the reads over the scores.
-  static constexpr int kDp = kGradN, kDs = NS == 1 ? 0 : 2 * kGradN, kDq = NS == 1 ? 2 * kGradN : kDs + NS * 32;
-  static constexpr int kCols = kDq + 64 * DC, kAlloc = kCols <= 256 ? 256 : 512;
+  // TMEM: scores, do.v, dq. ds of 16 columns takes the place of those once read: 8 columns a part,
+  // two parts over the scores, the third over do.v.
+  static constexpr int kDp = kGradN, kDq = 2 * kGradN;
+  static constexpr int kCols = kDq + L::kDim, kAlloc = kCols <= 256 ? 256 : 512;
   static constexpr int kInfo = ST + 1;
+  static constexpr int kBlocks = kAlloc <= 256 && kTileBytes <= 104 * 1024 ? 2 : 1;  // an SM holds
 };
 
 // The table's gradient: a row's ds sum to 0, and a bucket that holds all of a row's keys gets
@@ -334,19 +375,18 @@ struct DqShape {
 // of more than kWindow buckets take a launch for every kWindow of them.
 constexpr int kWindow = 64;
 
-template <typename T, int NS, int DC, int ST, bool VEC>
-__global__ void __launch_bounds__(DqShape<NS, DC, ST>::kThreads, NS == 1 && DC == 1 ? 2 : 1)
-    attn_dq_kernel(const __grid_constant__ AttnArgs A, int w0, int wn) {
-  using S = DqShape<NS, DC, ST>;
-  constexpr bool ASYNC = NS == 1 && VEC && sizeof(T) == 2;
-  static_assert(!ASYNC || ST >= 2, "a tile's arrival is told after the next one's issue");
+template <typename T, int NS, typename L, int ST, int LOAD>
+__global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, ST>::kBlocks)
+    attn_dq_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TmaMaps M, int w0, int wn) {
+  using S = DqShape<NS, L, ST>;
+  constexpr bool TMA = LOAD == LOAD_TMA, PIECES = LOAD == LOAD_PIECES;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   unsigned char *sQ = sm, *sO = sm + S::kOwn, *sK = sO + S::kOwn, *sV = sK + ST * S::kTile;
   float2* hist = reinterpret_cast<float2*>(sm + S::kTileBytes);  // wn x 128 (a, b)
   int2* lut = reinterpret_cast<int2*>(hist + wn * 128);           // (bias, column of its bucket or -1)
   __shared__ TileInfo<kGradN> info[S::kInfo];
-  __shared__ uint64_t full[ST], empty[ST], sfull, pfull, done;
+  __shared__ uint64_t full[ST], empty[ST], loaded[ST], own, sfull, pfull, done;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   __shared__ int last_live;
@@ -366,9 +406,11 @@ __global__ void __launch_bounds__(DqShape<NS, DC, ST>::kThreads, NS == 1 && DC =
     abort_flag = 0;
     last_live = mask ? 0 : (int)A.Lk;
     for (int i = 0; i < ST; ++i) {
-      mbar_init(&full[i], 96);
+      mbar_init(&full[i], TMA ? 64 : 96);
       mbar_init(&empty[i], 1);
+      mbar_init(&loaded[i], 2);  // the copies, and what goes with the rows
     }
+    mbar_init(&own, 1);
     mbar_init(&sfull, 1);
     mbar_init(&pfull, 128);
     mbar_init(&done, 1);
@@ -379,10 +421,18 @@ __global__ void __launch_bounds__(DqShape<NS, DC, ST>::kThreads, NS == 1 && DC =
     tmem_relinquish();
   }
   const auto row_live = [&](int r) { return i0 + r < A.Lq && lse[i0 + r] != -INFINITY; };
-  load_tile<T, NS, VEC, 128>(sQ, static_cast<const T*>(A.q) + b * A.qs[0] + h * A.qs[1] + i0 * A.qs[2], A.qs[2], A.D, DC,
-                             tid, S::kThreads, row_live);
-  load_tile<T, NS, VEC, 128>(sO, static_cast<const T*>(A.dout) + b * A.dos[0] + h * A.dos[1] + i0 * A.dos[2], A.dos[2],
-                             A.D, DC, tid, S::kThreads, row_live);
+  if constexpr (TMA) {
+    if (tid == 0) {
+      mbar_arrive_expect_tx(&own, 2 * S::kOwn);
+      tma_tile<L>(sQ, M, MAP_Q, 128, i0, h, b, &own);
+      tma_tile<L>(sO, M, MAP_DO, 128, i0, h, b, &own);
+    }
+  } else {
+    load_tile<T, NS, PIECES, 128, L>(sQ, static_cast<const T*>(A.q) + b * A.qs[0] + h * A.qs[1] + i0 * A.qs[2], A.qs[2],
+                                     A.D, tid, S::kThreads, row_live);
+    load_tile<T, NS, PIECES, 128, L>(sO, static_cast<const T*>(A.dout) + b * A.dos[0] + h * A.dos[1] + i0 * A.dos[2],
+                                     A.dos[2], A.D, tid, S::kThreads, row_live);
+  }
   if (A.table) {
     for (int d = tid; d < span; d += S::kThreads) {
       const int c = bucket_of(A.buckets, d - reach) - w0;
@@ -390,8 +440,12 @@ __global__ void __launch_bounds__(DqShape<NS, DC, ST>::kThreads, NS == 1 && DC =
     }
     for (int i = tid; i < wn * 128; i += S::kThreads) hist[i] = make_float2(0.f, 0.f);
   }
-  cp_commit();
-  cp_wait<0>();
+  if constexpr (TMA) {
+    __syncthreads();
+    wait(&own, 0, &abort_flag, A.polls);
+    clear_rows<L>(sQ, 128, tid, S::kThreads, row_live);
+    clear_rows<L>(sO, 128, tid, S::kThreads, row_live);
+  }
   fence_proxy_async_smem();
   fence_before_sync();
   __syncthreads();
@@ -415,7 +469,7 @@ __global__ void __launch_bounds__(DqShape<NS, DC, ST>::kThreads, NS == 1 && DC =
     const int64_t i = i0 + tid;
     const bool valid = i < A.Lq, live = row_live(tid);
     const int qp = live ? attn_q_pos(A, b, i) : 0;
-    const float L = live ? lse[i] : INFINITY, delta = live ? A.delta[bh * A.Lq + i] : 0.f;
+    const float lse_i = live ? lse[i] : INFINITY, delta = live ? A.delta[bh * A.Lq + i] : 0.f;
     const int qlo = __reduce_min_sync(0xffffffffu, live ? qp : INT32_MAX);
     const int qhi = __reduce_max_sync(0xffffffffu, live ? qp : INT32_MIN);
     const uint32_t base = tmem + ((uint32_t)(warp & 3) << 21);
@@ -449,7 +503,7 @@ __global__ void __launch_bounds__(DqShape<NS, DC, ST>::kThreads, NS == 1 && DC =
               const int d = k4[f] - qp;
               int2 t = make_int2(0, -1);
               if (A.table) t = lut[clamp_reach(d, reach) + reach];
-              float p = ex2(fmaf(__uint_as_float(s[e + f]), A.scale2, __int_as_float(t.x) - L));
+              float p = ex2(fmaf(__uint_as_float(s[e + f]), A.scale2, __int_as_float(t.x) - lse_i));
               if ((A.causal && d > 0) || !((bits >> (e + f)) & 1u)) p = 0.f;
               const float x = __uint_as_float(dp[e + f]), px = p * x;
               if (t.y >= 0) {
@@ -464,7 +518,7 @@ __global__ void __launch_bounds__(DqShape<NS, DC, ST>::kThreads, NS == 1 && DC =
             }
           }
         } else {
-          const float flat = (A.table && some ? __int_as_float(lut[above ? 2 * reach : 0].x) : 0.f) - L;
+          const float flat = (A.table && some ? __int_as_float(lut[above ? 2 * reach : 0].x) : 0.f) - lse_i;
           float sa = 0.f, sb = 0.f;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -493,7 +547,7 @@ __global__ void __launch_bounds__(DqShape<NS, DC, ST>::kThreads, NS == 1 && DC =
           for (int n = 0; n < NS; ++n) wd[n][e] = o[n];
         }
 #pragma unroll
-        for (int n = 0; n < NS; ++n) st8(base + S::kDs + n * 32 + c / 2, wd[n]);
+        for (int n = 0; n < NS; ++n) st8(base + c + (n < 2 ? n * 8 : S::kDp), wd[n]);
       }
       tmem_wait_st();
       fence_before_sync();
@@ -505,7 +559,7 @@ __global__ void __launch_bounds__(DqShape<NS, DC, ST>::kThreads, NS == 1 && DC =
     }
     const float broken = abort_flag ? NAN : 0.f;
     if (w0 == 0)
-      store_row<T, DC>(base + S::kDq, static_cast<T*>(A.dq) + b * A.dqs[0] + h * A.dqs[1] + i * A.dqs[2], A.dqs[2], A.D,
+      store_row<T, L::kDim>(base + S::kDq, static_cast<T*>(A.dq) + b * A.dqs[0] + h * A.dqs[1] + i * A.dqs[2], A.dqs[2], A.D,
                        A.scale + broken, !live || tiles == 0, valid);
     if (A.table) {
       const int hi = lut[2 * reach].y, lo = lut[0].y;
@@ -545,12 +599,13 @@ __global__ void __launch_bounds__(DqShape<NS, DC, ST>::kThreads, NS == 1 && DC =
         const int st = j % ST;
         const uint32_t aK = smem_u32(sK) + st * S::kTile, aV = smem_u32(sV) + st * S::kTile;
         wait(&full[st], (j / ST) & 1, &abort_flag, polls);
-        scores<NS, 128, kGradN>(tmem, aQ, aK, A.D, DC, id_s);
-        scores<NS, 128, kGradN>(tmem + S::kDp, aO, aV, A.D, DC, id_s);
+        scores<NS, 128, kGradN, L>(tmem, aQ, aK, A.D, id_s);
+        scores<NS, 128, kGradN, L>(tmem + S::kDp, aO, aV, A.D, id_s);
         mma_commit(&sfull);
         wait(&pfull, j & 1, &abort_flag, polls);
         fence_after_sync();
-        values<NS, kGradN>(tmem + S::kDq, tmem + S::kDs, 32, aK, DC, id_o, j > 0, [](int k) { return k * 8; });
+        values<NS, kGradN, L>(tmem + S::kDq, aK, id_o, j > 0,
+                              [=](int part, int k) { return tmem + k * 16 + (part < 2 ? part * 8 : S::kDp); });
         mma_commit(&empty[st]);
       }
       mma_commit(&sfull);
@@ -561,33 +616,56 @@ __global__ void __launch_bounds__(DqShape<NS, DC, ST>::kThreads, NS == 1 && DC =
     }
   } else {
     const int t = tid - 160, w = t >> 5;
-    const T* K = static_cast<const T*>(A.k) + b * A.ks[0] + hk * A.ks[1];
-    const T* V = static_cast<const T*>(A.v) + b * A.vs[0] + hk * A.vs[1];
-    for (int j = 0; j < tiles; ++j) {
-      const int st = j % ST;
+    const auto fill = [&](int j, int sub) {
       const int64_t j0 = (int64_t)j * kGradN;
-      TileInfo<kGradN>& I = info[j % S::kInfo];
-      if (j >= ST) wait(&empty[st], (j / ST - 1) & 1, &abort_flag, polls);
-      if (w < kGradN / kSub)
-        fill_info<kGradN>(
-            I, w, [&](int e) { return j0 + e < A.Lk && (!mask || mask[j0 + e]); },
-            [&](int e) { return attn_k_pos(A, b, j0 + e); });
-      named_barrier(1, 96);
-      const auto live = [&](int r) { return (I.live[r >> 5] >> (r & 31)) & 1u; };
-      load_tile<T, NS, VEC, kGradN>(sK + st * S::kTile, K + j0 * A.ks[2], A.ks[2], A.D, DC, t, 96, live);
-      load_tile<T, NS, VEC, kGradN>(sV + st * S::kTile, V + j0 * A.vs[2], A.vs[2], A.D, DC, t, 96, live);
-      if constexpr (ASYNC) {
-        cp_commit();
-        if (j > 0) {
-          cp_wait<1>();
-          fence_proxy_async_smem();
-          arrive(&full[(j - 1) % ST]);
+      fill_info<kGradN>(
+          info[j % S::kInfo], sub, [&](int e) { return j0 + e < A.Lk && (!mask || mask[j0 + e]); },
+          [&](int e) { return attn_k_pos(A, b, j0 + e); });
+    };
+    if constexpr (TMA) {
+      if (w == 0) {
+        for (int j = 0; j < tiles; ++j) {
+          const int st = j % ST;
+          if (j >= ST) wait(&empty[st], (j / ST - 1) & 1, &abort_flag, polls);
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&loaded[st], 2 * S::kTile);
+            tma_tile<L>(sK + st * S::kTile, M, MAP_K, kGradN, (int64_t)j * kGradN, hk, b, &loaded[st]);
+            tma_tile<L>(sV + st * S::kTile, M, MAP_V, kGradN, (int64_t)j * kGradN, hk, b, &loaded[st]);
+          }
+          for (int sub = 0; sub < kGradN / kSub; ++sub) fill(j, sub);
+          __syncwarp();
+          if (lane == 0) arrive(&loaded[st]);
         }
-        if (j + 1 < tiles) continue;
-        cp_wait<0>();
+      } else {
+        for (int j = 0; j < tiles; ++j) {
+          const int st = j % ST;
+          const TileInfo<kGradN>& I = info[j % S::kInfo];
+          wait(&loaded[st], (j / ST) & 1, &abort_flag, polls);
+          if (mask && (I.live[0] & I.live[1]) != 0xffffffffu) {
+            const auto live = [&](int r) { return (I.live[r >> 5] >> (r & 31)) & 1u; };
+            clear_rows<L>(sK + st * S::kTile, kGradN, t - 32, 64, live);
+            clear_rows<L>(sV + st * S::kTile, kGradN, t - 32, 64, live);
+            fence_proxy_async_smem();
+          }
+          arrive(&full[st]);
+        }
       }
-      fence_proxy_async_smem();
-      arrive(&full[st]);
+    } else {
+      const T* K = static_cast<const T*>(A.k) + b * A.ks[0] + hk * A.ks[1];
+      const T* V = static_cast<const T*>(A.v) + b * A.vs[0] + hk * A.vs[1];
+      for (int j = 0; j < tiles; ++j) {
+        const int st = j % ST;
+        const int64_t j0 = (int64_t)j * kGradN;
+        const TileInfo<kGradN>& I = info[j % S::kInfo];
+        if (j >= ST) wait(&empty[st], (j / ST - 1) & 1, &abort_flag, polls);
+        if (w < kGradN / kSub) fill(j, w);
+        named_barrier(1, 96);
+        const auto live = [&](int r) { return (I.live[r >> 5] >> (r & 31)) & 1u; };
+        load_tile<T, NS, PIECES, kGradN, L>(sK + st * S::kTile, K + j0 * A.ks[2], A.ks[2], A.D, t, 96, live);
+        load_tile<T, NS, PIECES, kGradN, L>(sV + st * S::kTile, V + j0 * A.vs[2], A.vs[2], A.D, t, 96, live);
+        fence_proxy_async_smem();
+        arrive(&full[st]);
+      }
     }
   }
   fence_before_sync();

@@ -71,16 +71,18 @@ AttnArgs make(const fx_attn_args* a) {
 bool aligned(const fx_attn_args* a, bool grad) {
   const int size = a->dtype == FX_F32 ? 4 : 2;
   uintptr_t m = (uintptr_t)a->dim * size;
-  auto add = [&](const void* p, const int64_t* s) {
+  auto add = [&](const void* p, const int64_t* s, int64_t heads, int64_t len) {
+    const int64_t n[3] = {a->batch, heads, len};
     m |= reinterpret_cast<uintptr_t>(p);
-    for (int i = 0; i < 3; ++i) m |= (uintptr_t)(s[i] * size);
+    for (int i = 0; i < 3; ++i)
+      if (n[i] > 1) m |= (uintptr_t)(s[i] * size);
   };
-  add(a->q, a->q_stride);
-  add(a->k, a->k_stride);
-  add(a->v, a->v_stride);
+  add(a->q, a->q_stride, a->heads, a->q_len);
+  add(a->k, a->k_stride, a->kv_heads, a->k_len);
+  add(a->v, a->v_stride, a->kv_heads, a->k_len);
   if (grad) {
-    add(a->dout, a->dout_stride);
-    add(a->out, a->out_stride);
+    add(a->dout, a->dout_stride, a->heads, a->q_len);
+    add(a->out, a->out_stride, a->heads, a->q_len);
   }
   return m % 16 == 0;
 }

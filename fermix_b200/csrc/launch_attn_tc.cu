@@ -7,23 +7,82 @@ namespace fxh {
 
 namespace {
 
-template <typename T, int NS, int QT, int BN, int DC, int ST, bool VEC>
+using tc::LOAD_ENTRIES;
+using tc::LOAD_PIECES;
+using tc::LOAD_TMA;
+using Narrow = tc::Rows<64, 1>;   // dim <= 32 (float32)
+using Half = tc::Rows<128, 1>;    // dim <= 64
+using Whole = tc::Rows<128, 2>;   // dim <= 128
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// The map of a bfloat16 tensor (batch, head, token) by element strides: boxes of 64 entries by
+// `rows` tokens. false: no such map (the caller loads by the threads).
+bool make_map(tc::TmaMaps& M, int which, const void* p, const int64_t* stride, int B, int H, int64_t L, int D, int rows) {
+  if (p == nullptr || L == 0) {  // no token is asked for
+    M.m[which] = M.m[tc::MAP_Q];
+    return true;
+  }
+  const int64_t n[3] = {L, H, B}, st[3] = {stride[2], stride[1], stride[0]};
+  cuuint64_t dims[4] = {(cuuint64_t)D, 1, 1, 1}, bytes[3];
+  for (int i = 0; i < 3; ++i) {
+    const bool one = n[i] == 1 || st[i] == 0;  // a dimension of one entry takes any stride
+    if (i == 0 && st[0] == 0 && L > 1) return false;
+    dims[i + 1] = one ? 1 : (cuuint64_t)n[i];
+    bytes[i] = one ? (cuuint64_t)((D * 2 + 15) / 16 * 16) : (cuuint64_t)st[i] * 2;
+    if (bytes[i] >= (cuuint64_t{1} << 40)) return false;
+  }
+  M.head_mul[which] = dims[2] > 1;
+  M.batch_mul[which] = dims[3] > 1;
+  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, ones[4] = {1, 1, 1, 1};
+  return encode_tiled()(&M.m[which], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(p), dims, bytes, box, ones,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int NS, int QT, int BN, typename L, int ST, int LOAD>
 int fwd(cudaStream_t s, const AttnArgs& A) {
-  using S = tc::FwdShape<T, NS, QT, BN, DC, ST>;
+  using S = tc::FwdShape<NS, QT, BN, L, ST>;
+  tc::TmaMaps M{};
+  if constexpr (LOAD == LOAD_TMA) {
+    if (!encode_tiled() || !make_map(M, tc::MAP_Q, A.q, A.qs, A.B, A.H, A.Lq, A.D, 128) ||
+        !make_map(M, tc::MAP_K, A.k, A.ks, A.B, A.Hk, A.Lk, A.D, BN) ||
+        !make_map(M, tc::MAP_V, A.v, A.vs, A.B, A.Hk, A.Lk, A.D, BN))
+      return fwd<T, NS, QT, BN, L, ST, LOAD_ENTRIES>(s, A);
+  }
   const size_t smem = S::kTileBytes + 1024 + (A.table ? (2 * A.buckets.reach + 1) * sizeof(float) : 0);
-  auto kern = tc::attn_fwd_kernel<T, NS, QT, BN, DC, ST, VEC>;
+  auto kern = tc::attn_fwd_kernel<T, NS, QT, BN, L, ST, LOAD>;
   if (raise_smem(kern, smem)) return FX_ERR_CUDA;
   const int64_t blocks = (A.Lq + 128 * QT - 1) / (128 * QT) * A.H * A.B;
   if (blocks > kMaxGrid) return FX_ERR_SHAPE;
-  kern<<<(unsigned)blocks, S::kThreads, smem, s>>>(A);
+  kern<<<(unsigned)blocks, S::kThreads, smem, s>>>(A, M);
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
-template <bool VEC>
-int fwd_shape(cudaStream_t s, const AttnArgs& A, bool is_f32) {
-  if (is_f32) return A.D <= 64 ? fwd<float, 3, 1, 64, 1, 1, VEC>(s, A) : fwd<float, 3, 1, 64, 2, 1, VEC>(s, A);
-  if (A.Lq <= 128) return A.D <= 64 ? fwd<bf16, 1, 1, 64, 1, 2, VEC>(s, A) : fwd<bf16, 1, 1, 64, 2, 2, VEC>(s, A);
-  return A.D <= 64 ? fwd<bf16, 1, 2, 128, 1, 2, VEC>(s, A) : fwd<bf16, 1, 2, 128, 2, 2, VEC>(s, A);
+template <int LOAD>
+int fwd_f32(cudaStream_t s, const AttnArgs& A) {
+  if (A.D <= 32) return fwd<float, 3, 1, 64, Narrow, 2, LOAD>(s, A);
+  return A.D <= 64 ? fwd<float, 3, 1, 64, Half, 1, LOAD>(s, A) : fwd<float, 3, 1, 64, Whole, 1, LOAD>(s, A);
+}
+
+template <int LOAD>
+int fwd_bf16(cudaStream_t s, const AttnArgs& A) {
+  if (A.Lq <= 128) return A.D <= 64 ? fwd<bf16, 1, 1, 64, Half, 2, LOAD>(s, A) : fwd<bf16, 1, 1, 64, Whole, 2, LOAD>(s, A);
+  return A.D <= 64 ? fwd<bf16, 1, 2, 128, Half, 2, LOAD>(s, A) : fwd<bf16, 1, 2, 128, Whole, 2, LOAD>(s, A);
 }
 
 template <typename T, int LPR, bool VEC>
@@ -36,8 +95,22 @@ int prep(cudaStream_t s, const AttnArgs& A) {
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
-template <typename T, int NS, int DC, int ST, bool VEC>
+template <typename T, int NS, typename L, int ST, int LOAD>
 int bwd(cudaStream_t s, const AttnArgs& A) {
+  tc::TmaMaps rows128{}, rows64{};  // of the blocks' own rows, of the streamed tiles
+  if constexpr (LOAD == LOAD_TMA) {
+    bool ok = encode_tiled() != nullptr;
+    for (int own = 0; own < 2 && ok; ++own) {
+      tc::TmaMaps& M = own ? rows128 : rows64;
+      const int n = own ? 128 : tc::kGradN;
+      ok = make_map(M, tc::MAP_Q, A.q, A.qs, A.B, A.H, A.Lq, A.D, n) &&
+           make_map(M, tc::MAP_K, A.k, A.ks, A.B, A.Hk, A.Lk, A.D, n) &&
+           make_map(M, tc::MAP_V, A.v, A.vs, A.B, A.Hk, A.Lk, A.D, n) &&
+           make_map(M, tc::MAP_DO, A.dout, A.dos, A.B, A.H, A.Lq, A.D, n);
+    }
+    if (!ok) return bwd<T, NS, L, ST, LOAD_ENTRIES>(s, A);
+  }
+  constexpr bool VEC = LOAD != LOAD_ENTRIES;
   const int lanes = (A.D * (int)sizeof(T) + 15) / 16;
   int st = lanes <= 8 ? prep<T, 8, VEC>(s, A) : lanes <= 16 ? prep<T, 16, VEC>(s, A) : prep<T, 32, VEC>(s, A);
   if (st) return st;
@@ -45,16 +118,22 @@ int bwd(cudaStream_t s, const AttnArgs& A) {
   const int64_t kblocks = (A.Lk + 127) / 128 * A.Hk * A.B, qblocks = (A.Lq + 127) / 128 * A.H * A.B;
   if (kblocks > kMaxGrid || qblocks > kMaxGrid) return FX_ERR_SHAPE;
   if (kblocks > 0) {
-    using S = tc::DkvShape<NS, DC, ST>;
-    auto kern = tc::attn_dkv_kernel<T, NS, DC, ST, VEC>;
+    using S = tc::DkvShape<NS, L, ST>;
+    auto kern = tc::attn_dkv_kernel<T, NS, L, ST, LOAD>;
     const size_t smem = S::kTileBytes + 1024 + span * sizeof(float);
     if (raise_smem(kern, smem)) return FX_ERR_CUDA;
-    kern<<<(unsigned)kblocks, S::kThreads, smem, s>>>(A);
+    tc::TmaMaps M = rows64;
+    M.m[tc::MAP_K] = rows128.m[tc::MAP_K];
+    M.m[tc::MAP_V] = rows128.m[tc::MAP_V];
+    kern<<<(unsigned)kblocks, S::kThreads, smem, s>>>(A, M);
     if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
   }
   if (qblocks > 0) {
-    using S = tc::DqShape<NS, DC, ST>;
-    auto kern = tc::attn_dq_kernel<T, NS, DC, ST, VEC>;
+    using S = tc::DqShape<NS, L, ST>;
+    auto kern = tc::attn_dq_kernel<T, NS, L, ST, LOAD>;
+    tc::TmaMaps M = rows64;
+    M.m[tc::MAP_Q] = rows128.m[tc::MAP_Q];
+    M.m[tc::MAP_DO] = rows128.m[tc::MAP_DO];
     const int nb = A.table ? A.buckets.num_buckets : 0;
     // buckets of a launch: up to kWindow, fewer where the tiles and the distances' table are large
     const DevInfo* D = dev_info();
@@ -66,7 +145,7 @@ int bwd(cudaStream_t s, const AttnArgs& A) {
       const int wn = nb - w0 < window ? nb - w0 : window;
       const size_t smem = S::kTileBytes + 1024 + (size_t)wn * 1024 + span * sizeof(int2);
       if (raise_smem(kern, smem)) return FX_ERR_CUDA;
-      kern<<<(unsigned)qblocks, S::kThreads, smem, s>>>(A, w0, wn);
+      kern<<<(unsigned)qblocks, S::kThreads, smem, s>>>(A, M, w0, wn);
       if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
       w0 += window;
     } while (w0 < nb);
@@ -74,16 +153,26 @@ int bwd(cudaStream_t s, const AttnArgs& A) {
   return FX_OK;
 }
 
-}  // namespace
-
-int launch_attn_tc_bwd(cudaStream_t s, const AttnArgs& A, bool is_f32, bool vec) {
-  if (is_f32) return vec ? bwd<float, 3, 1, 1, true>(s, A) : bwd<float, 3, 1, 1, false>(s, A);
-  if (A.D <= 64) return vec ? bwd<bf16, 1, 1, 2, true>(s, A) : bwd<bf16, 1, 1, 2, false>(s, A);
-  return vec ? bwd<bf16, 1, 2, 2, true>(s, A) : bwd<bf16, 1, 2, 2, false>(s, A);
+template <int LOAD>
+int bwd_f32(cudaStream_t s, const AttnArgs& A) {
+  return A.D <= 32 ? bwd<float, 3, Narrow, 1, LOAD>(s, A) : bwd<float, 3, Half, 1, LOAD>(s, A);
 }
 
-int launch_attn_tc_fwd(cudaStream_t s, const AttnArgs& A, bool is_f32, bool vec) {
-  return vec ? fwd_shape<true>(s, A, is_f32) : fwd_shape<false>(s, A, is_f32);
+template <int LOAD>
+int bwd_bf16(cudaStream_t s, const AttnArgs& A) {
+  return A.D <= 64 ? bwd<bf16, 1, Half, 2, LOAD>(s, A) : bwd<bf16, 1, Whole, 2, LOAD>(s, A);
+}
+
+}  // namespace
+
+int launch_attn_tc_bwd(cudaStream_t s, const AttnArgs& A, bool is_f32, bool aligned) {
+  if (is_f32) return aligned ? bwd_f32<LOAD_PIECES>(s, A) : bwd_f32<LOAD_ENTRIES>(s, A);
+  return aligned ? bwd_bf16<LOAD_TMA>(s, A) : bwd_bf16<LOAD_ENTRIES>(s, A);
+}
+
+int launch_attn_tc_fwd(cudaStream_t s, const AttnArgs& A, bool is_f32, bool aligned) {
+  if (is_f32) return aligned ? fwd_f32<LOAD_PIECES>(s, A) : fwd_f32<LOAD_ENTRIES>(s, A);
+  return aligned ? fwd_bf16<LOAD_TMA>(s, A) : fwd_bf16<LOAD_ENTRIES>(s, A);
 }
 
 int attn_tc_status(int clear) {
