@@ -292,20 +292,31 @@ __device__ __forceinline__ uint32_t fill_info(TileInfo<R>& I, int sub, Live live
 
 // ---------------------------------------------------------------- forward
 // A block takes QT tiles of 128 query rows of one head (thread = row = TMEM lane) and walks the
-// keys BN at a time. Warps 4 t .. 4 t + 3 hold the running maximum and sum of tile t; the next
+// keys BN at a time. Warps 4 t .. 4 t + 3 hold the reference and sum of tile t; the next
 // warp issues the tensor instructions, the last three load. With QT = 2 one tile's
-// exponentials run while the other's products do. The probabilities overwrite (QT = 2) or
-// follow the scores in TMEM and are the A operand of the second product. The output is
-// rescaled only when the maximum has grown by more than 2^8.
+// exponentials run while the other's products do.
+//
+// The exponentials are taken to a reference per row: the maximum of the first 32 keys that
+// are not all masked, and from then on kept until a score passes it by more than 2^64. float32
+// sums and bfloat16 probabilities have the exponent range for that, so the usual pass over the
+// scores for their maximum, and the rescaling of the output when it grows, are left to the
+// rare case. References are whole numbers, so that moving one scales the probabilities already
+// written exactly. The usual case takes the reference off within the multiplication by the scale;
+// a reference of 2^23 and more (a table of the type's lowest value) is taken off after it, so that
+// what such a bias absorbs stays absorbed. The scores are read 32 columns at a time, each written back as
+// probabilities, the A operand of the second product: over the scores where TMEM is full
+// (QT = 2, 128 entries), else in columns of their own, which lets the next scores be formed
+// before this tile's second product.
 template <int NS, int QT, int BN, typename L, int ST>
 struct FwdShape {
   static constexpr int kThreads = 128 * QT + 128;
   static constexpr uint32_t kRow = NS * L::DC * L::RB, kQ = 128 * kRow, kKV = BN * kRow;
   static constexpr int kInfo = ST + 1;
   static constexpr uint32_t kTileBytes = QT * kQ + 2 * ST * kKV;
-  // TMEM columns of a tile: scores, then (NS > 1) the probabilities' parts, then the output
-  static constexpr int kP = NS == 1 ? 0 : BN;
-  static constexpr int kO = NS == 1 ? BN : BN + NS * BN / 2;
+  // TMEM columns of a tile: scores, the probabilities' parts, the output
+  static constexpr bool kOver = QT * (BN + NS * BN / 2 + L::kDim) > 512;  // probabilities over the scores
+  static constexpr int kP = kOver ? 0 : BN;
+  static constexpr int kO = kOver ? BN : BN + NS * BN / 2;
   static constexpr int kTile = kO + L::kDim;
   static constexpr int kCols = QT * kTile;
   static constexpr int kAlloc = kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
@@ -323,7 +334,8 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
   unsigned char *sQ = sm, *sK = sm + QT * S::kQ, *sV = sK + ST * S::kKV;
   float* lut = reinterpret_cast<float*>(sm + S::kTileBytes);
   __shared__ TileInfo<BN> info[S::kInfo];
-  __shared__ uint64_t kfull[ST], vfull[ST], kempty[ST], vempty[ST], kraw[ST], vraw[ST], qraw, sfull[QT], pfull[QT], done;
+  __shared__ uint64_t kfull[ST], vfull[ST], kempty[ST], vempty[ST], kraw[ST], vraw[ST], qraw, sfull[QT], pfull[QT],
+      ofull[QT], done;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   __shared__ int last_live;
@@ -354,6 +366,7 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
     for (int t = 0; t < QT; ++t) {
       mbar_init(&sfull[t], 1);
       mbar_init(&pfull[t], 128);
+      mbar_init(&ofull[t], 1);
     }
     mbar_init(&done, 1);
     fence_mbar_init();
@@ -409,40 +422,45 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
     const int qlo = __reduce_min_sync(0xffffffffu, valid ? qp : INT32_MAX);
     const int qhi = __reduce_max_sync(0xffffffffu, valid ? qp : INT32_MIN);
     const uint32_t base = tmem + ((uint32_t)(warp & 3) << 21) + t * S::kTile;
-    float m = -INFINITY, l = 0.f;  // m: the reference the exponentials are taken to
+    float m = -INFINITY, l = 0.f;  // m: the reference; -inf before the first key
+    const int qoff = qp - reach;
     for (int j = 0; j < tiles; ++j) {
       const TileInfo<BN>& I = info[j % S::kInfo];
       wait(&sfull[t], j & 1, &abort_flag, polls);
       fence_after_sync();
-      uint32_t s[BN];
-#pragma unroll
-      for (int c = 0; c < BN; c += 32) ld32(base + c, s + c);
-      tmem_wait_ld();
-      float top = m;
-#pragma unroll
+      bool free_p = S::kOver || j == 0;  // the last tile's second product has read the probabilities
+      uint32_t x[32];
+      ld32(base, x);
+#pragma unroll 1
       for (int sub = 0; sub < BN / kSub; ++sub) {
-        uint32_t* x = s + sub * kSub;
         const uint32_t bits = I.live[sub];
         const int lo = I.lo[sub], hi = I.hi[sub];
-        const bool later = A.causal && hi > qlo;
-        if (bits != 0 && valid | (qlo <= qhi)) {
-          const bool near = A.table && !((int64_t)lo - qhi >= reach || (int64_t)hi - qlo <= -reach);
-          if (near || later) {
+        const bool none = bits == 0 || qlo > qhi, later = A.causal && hi > qlo;
+        const bool above = lo - (int64_t)qhi >= reach, below = hi - (int64_t)qlo <= -reach;
+        const bool near = A.table && !above && !below;
+        // scores less the reference; a second pass where it has to move: the scores, then less it
+        bool apart = __any_sync(0xffffffffu, m != -INFINITY && fabsf(m) >= 8388608.f);
+        for (;;) {
+          const float ref = apart || m == -INFINITY ? 0.f : m;
+          tmem_wait_ld();
+          if (none) {
+#pragma unroll
+            for (int c = 0; c < kSub; ++c) x[c] = 0xff800000u;
+          } else if (near || later) {
 #pragma unroll
             for (int c = 0; c < kSub; c += 4) {
               const int4 kp = *reinterpret_cast<const int4*>(&I.pos[sub * kSub + c]);
               const int k4[4] = {kp.x, kp.y, kp.z, kp.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const int d = k4[e] - qp;
-                const float bias = A.table ? lut[clamp_reach(d, reach) + reach] : 0.f;
-                float v = fmaf(__uint_as_float(x[c + e]), A.scale2, bias);
-                if (A.causal && d > 0) v = -INFINITY;
+                const float bias = A.table ? lut[min(max(k4[e] - qoff, 0), 2 * reach)] : 0.f;
+                float v = fmaf(__uint_as_float(x[c + e]), A.scale2, bias - ref);
+                if (A.causal && k4[e] > qp) v = -INFINITY;
                 x[c + e] = __float_as_uint(v);
               }
             }
           } else {
-            const float bias = !A.table ? 0.f : lut[(int64_t)lo - qhi >= reach ? 2 * reach : 0];
+            const float bias = (A.table ? lut[above ? 2 * reach : 0] : 0.f) - ref;
 #pragma unroll
             for (int c = 0; c < kSub; ++c) x[c] = __float_as_uint(fmaf(__uint_as_float(x[c]), A.scale2, bias));
           }
@@ -451,48 +469,79 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
             for (int c = 0; c < kSub; ++c)
               if (!((bits >> c) & 1u)) x[c] = 0xff800000u;
           }
-        } else {
+          float top = __uint_as_float(x[0]);
 #pragma unroll
-          for (int c = 0; c < kSub; ++c) x[c] = 0xff800000u;
-        }
+          for (int c = 1; c < kSub; ++c) top = fmaxf(top, __uint_as_float(x[c]));
+          if (!apart) {
+            if (!__any_sync(0xffffffffu, top > 64.f || (m == -INFINITY && top > -INFINITY))) break;
+            ld32(base + sub * kSub, x);
+            apart = true;
+            continue;
+          }
+          const bool move = m == -INFINITY ? top > -INFINITY : top - m > 64.f;
+          if (__any_sync(0xffffffffu, move)) {
+            if (!free_p) {  // the output is at rest
+              wait(&ofull[t], (j - 1) & 1, &abort_flag, polls);
+              fence_after_sync();
+              free_p = true;
+            }
+            float f = 1.f;
+            if (move) {
+              const float to = ceilf(top);
+              f = m == -INFINITY ? 0.f : ex2(m - to);
+              m = to;
+            }
+            l *= f;
+            if (j > 0) {
+#pragma unroll 1
+              for (int c = 0; c < L::kDim; c += 8) {
+                if (c < A.D) {
+                  uint32_t o[8];
+                  tmem_ld8(base + S::kO + c, o);
+                  tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < kSub; ++c) top = fmaxf(top, __uint_as_float(x[c]));
-      }
-      // the reference moves when it must: NaN and the first finite maximum included
-      const bool move = !(top - m <= 8.f) && top != -INFINITY;
-      if (__any_sync(0xffffffffu, move)) {
-        const float f = move ? ex2(m - top) : 1.f;
-        if (move) m = top;
-        l *= f;
-        if (j > 0) {
-#pragma unroll
-          for (int c = 0; c < L::kDim; c += 16) {
-            if (c < A.D) {
-              uint32_t o[16];
-              ld16(base + S::kO + c, o);
+                  for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                  tmem_st8(base + S::kO + c, o);
+                }
+              }
+            }
+#pragma unroll 1
+            for (int c = 0; c < NS * sub * (kSub / 2); c += 8) {  // the tile's probabilities so far
+              const int part = c / (sub * (kSub / 2)), col = c - part * (sub * (kSub / 2));
+              uint32_t o[8];
+              tmem_ld8(base + S::kP + part * (BN / 2) + col, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              st16(base + S::kO + c, o);
+              for (int e = 0; e < 8; ++e)
+                o[e] = pack2(__uint_as_float(o[e] << 16) * f, __uint_as_float(o[e] & 0xffff0000u) * f);
+              tmem_st8(base + S::kP + part * (BN / 2) + col, o);
             }
           }
-        }
-      }
-      const float ref = m == -INFINITY ? 0.f : m;
+          const float off = m == -INFINITY ? 0.f : m;
 #pragma unroll
-      for (int c = 0; c < BN; c += 32) {
+          for (int c = 0; c < kSub; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) - off);
+          break;
+        }
+        float s0 = 0.f, s1 = 0.f;
         uint32_t w[NS][16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float p0 = ex2(__uint_as_float(s[c + 2 * e]) - ref), p1 = ex2(__uint_as_float(s[c + 2 * e + 1]) - ref);
-          l += p0 + p1;
+          const float p0 = ex2(__uint_as_float(x[2 * e])), p1 = ex2(__uint_as_float(x[2 * e + 1]));
+          s0 += p0;
+          s1 += p1;
           uint32_t o[NS];
           split2<NS>(p0, p1, o);
 #pragma unroll
-          for (int i2 = 0; i2 < NS; ++i2) w[i2][e] = o[i2];
+          for (int n = 0; n < NS; ++n) w[n][e] = o[n];
+        }
+        l += s0 + s1;
+        if (sub + 1 < BN / kSub) ld32(base + (sub + 1) * kSub, x);
+        if (!free_p) {
+          wait(&ofull[t], (j - 1) & 1, &abort_flag, polls);
+          free_p = true;
         }
 #pragma unroll
-        for (int i2 = 0; i2 < NS; ++i2) st16(base + S::kP + i2 * (BN / 2) + c / 2, w[i2]);
+        for (int n = 0; n < NS; ++n) st16(base + S::kP + n * (BN / 2) + sub * (kSub / 2), w[n]);
       }
       tmem_wait_st();
       fence_before_sync();
@@ -500,7 +549,7 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
     }
     // -------------------------------------------------------- output
     if (tiles > 0) {
-      wait(&sfull[t], tiles & 1, &abort_flag, polls);
+      wait(&ofull[t], (tiles - 1) & 1, &abort_flag, polls);
       fence_after_sync();
     }
     const bool broken = abort_flag != 0;
@@ -550,20 +599,30 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
       mma_commit(&kempty[0]);
       for (int j = 0; j < tiles; ++j) {
         const int st = j % ST, sn = (j + 1) % ST;
-        wait(&vfull[st], (j / ST) & 1, &abort_flag, polls);
-        if (j + 1 < tiles) wait(&kfull[sn], ((j + 1) / ST) & 1, &abort_flag, polls);
+        const bool more = j + 1 < tiles;
+        if (more) wait(&kfull[sn], ((j + 1) / ST) & 1, &abort_flag, polls);
+        if (S::kOver) wait(&vfull[st], (j / ST) & 1, &abort_flag, polls);
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
           const uint32_t d = tmem + t * S::kTile;
           wait(&pfull[t], j & 1, &abort_flag, polls);
           fence_after_sync();
+          if (!S::kOver && more) {
+            scores<NS, 128, BN, L>(d, aQ + t * S::kQ, aK + sn * S::kKV, A.D, id_s);
+            mma_commit(&sfull[t]);
+            if (t == QT - 1) mma_commit(&kempty[sn]);
+          }
+          if (!S::kOver && t == 0) wait(&vfull[st], (j / ST) & 1, &abort_flag, polls);
           values<NS, BN, L>(d + S::kO, aV + st * S::kKV, id_o, j > 0,
                             [=](int part, int k) { return d + S::kP + part * (BN / 2) + k * 8; });
+          mma_commit(&ofull[t]);
           if (t == QT - 1) mma_commit(&vempty[st]);
-          if (j + 1 < tiles) scores<NS, 128, BN, L>(d, aQ + t * S::kQ, aK + sn * S::kKV, A.D, id_s);
-          mma_commit(&sfull[t]);  // after the last keys: the output is whole
+          if (S::kOver && more) {
+            scores<NS, 128, BN, L>(d, aQ + t * S::kQ, aK + sn * S::kKV, A.D, id_s);
+            mma_commit(&sfull[t]);
+            if (t == QT - 1) mma_commit(&kempty[sn]);
+          }
         }
-        if (j + 1 < tiles) mma_commit(&kempty[sn]);
       }
       if (abort_flag) {  // nothing may be in flight when the TMEM is freed
         mma_commit(&done);
