@@ -103,6 +103,26 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// two float32 operations in one instruction
+__device__ __forceinline__ uint64_t both(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void halves(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_both(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_both(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // (a, b) -> NS packed pairs whose sum is (a, b)
 template <int NS>
 __device__ __forceinline__ void split2(float a, float b, uint32_t (&o)[NS]) {
@@ -187,40 +207,46 @@ __device__ __forceinline__ void load_tile(unsigned char* dst, const T* p, int64_
   const int pieces = (dim + 15) / 16 * 2;  // of 8 entries
   const int dr = n / pieces, dc = n - dr * pieces;
   int r = t / pieces, c = t - r * pieces;
+  constexpr int U = 4;  // pieces on the way at a time
   while (r < R) {
-    float x[8];
+    float x[U][8];
+    unsigned char* d[U];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 0.f;
-    if (live(r)) {
-      const T* s = p + r * step + c * 8;
+    for (int u = 0; u < U; ++u) {
+      d[u] = r < R ? dst + L::at(R, r, c) : nullptr;
+      const bool ok = r < R && live(r);
+      const T* s = p + (ok ? r * step + c * 8 : 0);
       if constexpr (PIECES) {
         constexpr int V = 16 / sizeof(T);
 #pragma unroll
         for (int h = 0; h < 8; h += V) {
-          if (c * 8 + h < dim) {
-            const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(s + h);
+          Pack<T, V> k;
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[h + e] = to_f(k.e[e]);
-          }
+          for (int e = 0; e < V; ++e) k.e[e] = from_f<T>(0.f);
+          if (ok && c * 8 + h < dim) k = *reinterpret_cast<const Pack<T, V>*>(s + h);
+#pragma unroll
+          for (int e = 0; e < V; ++e) x[u][h + e] = to_f(k.e[e]);
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c * 8 + e < dim) x[e] = to_f(s[e]);
+        for (int e = 0; e < 8; ++e) x[u][e] = ok && c * 8 + e < dim ? to_f(s[e]) : 0.f;
+      }
+      r += dr;
+      c += dc;
+      if (c >= pieces) {
+        c -= pieces;
+        ++r;
       }
     }
-    uint32_t w[4][NS];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) split2<NS>(x[2 * e], x[2 * e + 1], w[e]);
-    unsigned char* d = dst + L::at(R, r, c);
+    for (int u = 0; u < U; ++u) {
+      if (d[u] == nullptr) continue;
+      uint32_t w[4][NS];
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
-      *reinterpret_cast<uint4*>(d + s * (R * L::RB * L::DC)) = make_uint4(w[0][s], w[1][s], w[2][s], w[3][s]);
-    r += dr;
-    c += dc;
-    if (c >= pieces) {
-      c -= pieces;
-      ++r;
+      for (int e = 0; e < 4; ++e) split2<NS>(x[u][2 * e], x[u][2 * e + 1], w[e]);
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+        *reinterpret_cast<uint4*>(d[u] + s * (R * L::RB * L::DC)) = make_uint4(w[0][s], w[1][s], w[2][s], w[3][s]);
     }
   }
 }
@@ -291,25 +317,124 @@ __device__ __forceinline__ uint32_t fill_info(TileInfo<R>& I, int sub, Live live
 }
 
 // ---------------------------------------------------------------- forward
-// A block takes QT tiles of 128 query rows of one head (thread = row = TMEM lane) and walks the
-// keys BN at a time. Warps 4 t .. 4 t + 3 hold the reference and sum of tile t; the next
-// warp issues the tensor instructions, the last three load. With QT = 2 one tile's
-// exponentials run while the other's products do.
+// A block takes QT tiles of 128 query rows of one head and walks the keys BN at a time. A row
+// (TMEM lane) of a tile belongs to two threads, each with half of the columns: a warp's
+// exponentials, lookups and conversions are chains that four warps a scheduler cover and two do
+// not (measured: 5.1 thousand cycles for 128 columns with one warp a scheduler, 3.2 with two).
+// Warps 8 t .. 8 t + 7 work on tile t, the next one issues the tensor instructions, the last three
+// load. With QT = 2 one tile's exponentials run while the other's products do.
 //
-// The exponentials are taken to a reference per row: the maximum of the first 32 keys that
-// are not all masked, and from then on kept until a score passes it by more than 2^64. float32
-// sums and bfloat16 probabilities have the exponent range for that, so the usual pass over the
-// scores for their maximum, and the rescaling of the output when it grows, are left to the
-// rare case. References are whole numbers, so that moving one scales the probabilities already
-// written exactly. The usual case takes the reference off within the multiplication by the scale;
-// a reference of 2^23 and more (a table of the type's lowest value) is taken off after it, so that
-// what such a bias absorbs stays absorbed. The scores are read 32 columns at a time, each written back as
-// probabilities, the A operand of the second product: over the scores where TMEM is full
-// (QT = 2, 128 entries), else in columns of their own, which lets the next scores be formed
-// before this tile's second product.
+// The exponentials are taken to a reference per row, set from the first tile that holds a live
+// key and kept until a score passes it by more than 2^64, which shows in the sums. float32 sums and
+// bfloat16 probabilities have the exponent range for that, so the usual pass over the scores
+// for their maximum, and the rescaling of the output when it grows, are left to the rare case. (Its
+// code is loops, not unrolled: it runs about once a block, and instructions fetched for one use
+// cost more than they do.) The reference is taken off after the bias is added, so that what a bias
+// of the type's lowest value absorbs stays absorbed. The probabilities go back to TMEM as the A
+// operand of the second product: over the scores where TMEM is full (QT = 2, 128 entries), else
+// to columns of their own, which lets the next scores be formed before this tile's second product.
+struct FwdLane {
+  uint32_t base;     // TMEM of the tile, this warp's lanes
+  int qp, qlo, qhi;  // this row's position, the warp's rows' least and greatest
+  bool valid;
+};
+
+// The greatest of the W scores from column c0 of a tile.
+template <int BN, int W>
+__device__ __forceinline__ float fwd_top(const AttnArgs& A, const TileInfo<BN>& I, const float* lut, const FwdLane& F,
+                                         int c0) {
+  const int reach = A.buckets.reach;
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = c0; c < c0 + W; c += 8) {
+    uint32_t x[8];
+    tmem_ld8(F.base + c, x);
+    tmem_wait_ld();
+    const uint32_t bits = I.live[c / kSub] >> (c % kSub);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int k = I.pos[c + e];
+      const float bias = A.table ? lut[clamp_reach(k - F.qp, reach) + reach] : 0.f;
+      const float v = fmaf(__uint_as_float(x[e]), A.scale2, bias);
+      if (((bits >> e) & 1u) && !(A.causal && k > F.qp)) top = fmaxf(top, v);
+    }
+  }
+  return top;
+}
+
+// NS parts of the probabilities of 32 columns into p, their sum back: x the raw scores, ref the
+// reference with its sign turned.
+template <int NS, int BN>
+__device__ __forceinline__ float fwd_columns(const AttnArgs& A, const TileInfo<BN>& I, const float* lut, const FwdLane& F,
+                                             int sub, float ref, uint32_t* x, uint32_t (*p)[16]) {
+  const int reach = A.buckets.reach, far = 2 * reach;
+  const uint32_t bits = I.live[sub];
+  const int lo = I.lo[sub], hi = I.hi[sub];
+  const bool above = lo - (int64_t)F.qhi >= reach, below = hi - (int64_t)F.qlo <= -reach;
+  if (bits == 0 || F.qlo > F.qhi) {
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) p[n][e] = 0u;
+    return 0.f;
+  }
+  if ((A.table && !above && !below) || (A.causal && hi > F.qlo)) {
+    const int qoff = F.qp - reach, qlim = A.causal ? F.qp : INT32_MAX;
+#pragma unroll
+    for (int c = 0; c < kSub; c += 16) {
+      int k[16];
+      float bias[16];
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        const int4 v = *reinterpret_cast<const int4*>(&I.pos[sub * kSub + c + e]);
+        k[e] = v.x;
+        k[e + 1] = v.y;
+        k[e + 2] = v.z;
+        k[e + 3] = v.w;
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) bias[e] = A.table ? lut[__vimin_s32_relu(k[e] - qoff, far)] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float v = fmaf(__uint_as_float(x[c + e]), A.scale2, bias[e]) + ref;
+        x[c + e] = k[e] > qlim ? 0xff800000u : __float_as_uint(v);
+      }
+    }
+  } else {
+    const float bias = A.table ? lut[above ? far : 0] : 0.f;
+    const uint64_t bb = both(bias, bias), ss = both(A.scale2, A.scale2), rr = both(ref, ref);
+#pragma unroll
+    for (int c = 0; c < kSub; c += 2) {
+      float v0, v1;
+      halves(add_both(fma_both(both(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), ss, bb), rr), v0, v1);
+      x[c] = __float_as_uint(v0);
+      x[c + 1] = __float_as_uint(v1);
+    }
+  }
+  if (bits != 0xffffffffu) {
+#pragma unroll
+    for (int c = 0; c < kSub; ++c)
+      if (!((bits >> c) & 1u)) x[c] = 0xff800000u;
+  }
+  uint64_t sum[2] = {0, 0};  // pairs of zeros
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const float p0 = ex2(__uint_as_float(x[2 * e])), p1 = ex2(__uint_as_float(x[2 * e + 1]));
+    sum[e & 1] = add_both(sum[e & 1], both(p0, p1));
+    uint32_t o[NS];
+    split2<NS>(p0, p1, o);
+#pragma unroll
+    for (int n = 0; n < NS; ++n) p[n][e] = o[n];
+  }
+  float a0, a1;
+  halves(add_both(sum[0], sum[1]), a0, a1);
+  return a0 + a1;
+}
+
 template <int NS, int QT, int BN, typename L, int ST>
 struct FwdShape {
-  static constexpr int kThreads = 128 * QT + 128;
+  static constexpr int kThreads = 256 * QT + 128;
+  static constexpr int kHalf = BN / 2;  // columns of a thread
   static constexpr uint32_t kRow = NS * L::DC * L::RB, kQ = 128 * kRow, kKV = BN * kRow;
   static constexpr int kInfo = ST + 1;
   static constexpr uint32_t kTileBytes = QT * kQ + 2 * ST * kKV;
@@ -338,7 +463,8 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
       ofull[QT], done;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
-  __shared__ int last_live;
+  __shared__ int last_live, moving[QT][2];
+  __shared__ float shared_row[QT][2][128];  // what the two threads of a row tell each other
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // block -> (batch, head, query block); under a causal order the longest blocks first
@@ -365,7 +491,7 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
     mbar_init(&qraw, 1);
     for (int t = 0; t < QT; ++t) {
       mbar_init(&sfull[t], 1);
-      mbar_init(&pfull[t], 128);
+      mbar_init(&pfull[t], 256);
       mbar_init(&ofull[t], 1);
     }
     mbar_init(&done, 1);
@@ -413,140 +539,88 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
   const uint32_t tmem = tmem_slot;
   const uint32_t polls = A.polls;
 
-  if (warp < 4 * QT) {
+  if (warp < 8 * QT) {
     // -------------------------------------------------------- softmax
-    const int t = warp >> 2;
-    const int64_t i = i0 + t * 128 + (tid & 127);
+    const int t = warp >> 3, half = (warp >> 2) & 1, r = tid & 127;
+    const int64_t i = i0 + t * 128 + r;
     const bool valid = i < A.Lq;
     const int qp = valid ? attn_q_pos(A, b, i) : 0;
-    const int qlo = __reduce_min_sync(0xffffffffu, valid ? qp : INT32_MAX);
-    const int qhi = __reduce_max_sync(0xffffffffu, valid ? qp : INT32_MIN);
-    const uint32_t base = tmem + ((uint32_t)(warp & 3) << 21) + t * S::kTile;
-    float m = -INFINITY, l = 0.f;  // m: the reference; -inf before the first key
-    const int qoff = qp - reach;
+    const FwdLane F{tmem + ((uint32_t)(warp & 3) << 21) + t * S::kTile, qp,
+                    __reduce_min_sync(0xffffffffu, valid ? qp : INT32_MAX),
+                    __reduce_max_sync(0xffffffffu, valid ? qp : INT32_MIN), valid};
+    const uint32_t base = F.base;
+    float m = -INFINITY, l = 0.f;  // the reference (-inf before the first key), the sum of this half
+    if ((tid & 255) < 2) moving[t][tid & 255] = 0;
+    named_barrier(2 + t, 256);
     for (int j = 0; j < tiles; ++j) {
       const TileInfo<BN>& I = info[j % S::kInfo];
       wait(&sfull[t], j & 1, &abort_flag, polls);
       fence_after_sync();
-      bool free_p = S::kOver || j == 0;  // the last tile's second product has read the probabilities
-      uint32_t x[32];
-      ld32(base, x);
-#pragma unroll 1
-      for (int sub = 0; sub < BN / kSub; ++sub) {
-        const uint32_t bits = I.live[sub];
-        const int lo = I.lo[sub], hi = I.hi[sub];
-        const bool none = bits == 0 || qlo > qhi, later = A.causal && hi > qlo;
-        const bool above = lo - (int64_t)qhi >= reach, below = hi - (int64_t)qlo <= -reach;
-        const bool near = A.table && !above && !below;
-        // scores less the reference; a second pass where it has to move: the scores, then less it
-        bool apart = __any_sync(0xffffffffu, m != -INFINITY && fabsf(m) >= 8388608.f);
-        for (;;) {
-          const float ref = apart || m == -INFINITY ? 0.f : m;
-          tmem_wait_ld();
-          if (none) {
+      uint32_t p[S::kHalf / kSub][NS][16];
+      float sum = 0.f;
+      bool moved = false;
+      for (;;) {
+        bool low = __any_sync(0xffffffffu, valid && m == -INFINITY);
+        if (!low || moved) {
+          const float ref = m == -INFINITY ? 0.f : -m;
+          sum = 0.f;
 #pragma unroll
-            for (int c = 0; c < kSub; ++c) x[c] = 0xff800000u;
-          } else if (near || later) {
-#pragma unroll
-            for (int c = 0; c < kSub; c += 4) {
-              const int4 kp = *reinterpret_cast<const int4*>(&I.pos[sub * kSub + c]);
-              const int k4[4] = {kp.x, kp.y, kp.z, kp.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float bias = A.table ? lut[min(max(k4[e] - qoff, 0), 2 * reach)] : 0.f;
-                float v = fmaf(__uint_as_float(x[c + e]), A.scale2, bias - ref);
-                if (A.causal && k4[e] > qp) v = -INFINITY;
-                x[c + e] = __float_as_uint(v);
-              }
-            }
-          } else {
-            const float bias = (A.table ? lut[above ? 2 * reach : 0] : 0.f) - ref;
-#pragma unroll
-            for (int c = 0; c < kSub; ++c) x[c] = __float_as_uint(fmaf(__uint_as_float(x[c]), A.scale2, bias));
-          }
-          if (bits != 0xffffffffu) {
-#pragma unroll
-            for (int c = 0; c < kSub; ++c)
-              if (!((bits >> c) & 1u)) x[c] = 0xff800000u;
-          }
-          float top = __uint_as_float(x[0]);
-#pragma unroll
-          for (int c = 1; c < kSub; ++c) top = fmaxf(top, __uint_as_float(x[c]));
-          if (!apart) {
-            if (!__any_sync(0xffffffffu, top > 64.f || (m == -INFINITY && top > -INFINITY))) break;
+          for (int c = 0; c < S::kHalf / kSub; ++c) {
+            const int sub = half * (S::kHalf / kSub) + c;
+            uint32_t x[kSub];
             ld32(base + sub * kSub, x);
-            apart = true;
-            continue;
+            tmem_wait_ld();
+            sum += fwd_columns<NS, BN>(A, I, lut, F, sub, ref, x, p[c]);
           }
-          const bool move = m == -INFINITY ? top > -INFINITY : top - m > 64.f;
-          if (__any_sync(0xffffffffu, move)) {
-            if (!free_p) {  // the output is at rest
-              wait(&ofull[t], (j - 1) & 1, &abort_flag, polls);
-              fence_after_sync();
-              free_p = true;
-            }
-            float f = 1.f;
-            if (move) {
-              const float to = ceilf(top);
-              f = m == -INFINITY ? 0.f : ex2(m - to);
-              m = to;
-            }
-            l *= f;
-            if (j > 0) {
-#pragma unroll 1
-              for (int c = 0; c < L::kDim; c += 8) {
-                if (c < A.D) {
-                  uint32_t o[8];
-                  tmem_ld8(base + S::kO + c, o);
-                  tmem_wait_ld();
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                  tmem_st8(base + S::kO + c, o);
-                }
-              }
-            }
-#pragma unroll 1
-            for (int c = 0; c < NS * sub * (kSub / 2); c += 8) {  // the tile's probabilities so far
-              const int part = c / (sub * (kSub / 2)), col = c - part * (sub * (kSub / 2));
-              uint32_t o[8];
-              tmem_ld8(base + S::kP + part * (BN / 2) + col, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                o[e] = pack2(__uint_as_float(o[e] << 16) * f, __uint_as_float(o[e] & 0xffff0000u) * f);
-              tmem_st8(base + S::kP + part * (BN / 2) + col, o);
-            }
-          }
-          const float off = m == -INFINITY ? 0.f : m;
-#pragma unroll
-          for (int c = 0; c < kSub; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) - off);
-          break;
+          low = __any_sync(0xffffffffu, valid && !(sum <= 1.8446744e19f));
         }
-        float s0 = 0.f, s1 = 0.f;
-        uint32_t w[NS][16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float p0 = ex2(__uint_as_float(x[2 * e])), p1 = ex2(__uint_as_float(x[2 * e + 1]));
-          s0 += p0;
-          s1 += p1;
-          uint32_t o[NS];
-          split2<NS>(p0, p1, o);
-#pragma unroll
-          for (int n = 0; n < NS; ++n) w[n][e] = o[n];
-        }
-        l += s0 + s1;
-        if (sub + 1 < BN / kSub) ld32(base + (sub + 1) * kSub, x);
-        if (!free_p) {
+        if (moved) break;
+        // both halves of all rows agree on whether references move (two flags in turn)
+        if (low && lane == 0) moving[t][j & 1] = 1;
+        named_barrier(2 + t, 256);
+        if (!moving[t][j & 1]) break;
+        shared_row[t][half][r] = fwd_top<BN, S::kHalf>(A, I, lut, F, half * S::kHalf);
+        if (!S::kOver && j > 0) {  // the output is at rest
           wait(&ofull[t], (j - 1) & 1, &abort_flag, polls);
-          free_p = true;
+          fence_after_sync();
         }
+        named_barrier(2 + t, 256);
+        if ((tid & 255) == 0) moving[t][j & 1] = 0;
+        const float top = fmaxf(shared_row[t][0][r], shared_row[t][1][r]);
+        float f = 1.f;
+        if (m == -INFINITY ? top > -INFINITY : top - m > 64.f) {
+          f = m == -INFINITY ? 0.f : ex2(m - top);
+          m = top;
+        }
+        l *= f;
+        if (j > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+#pragma unroll 1
+          for (int c = half * 8; c < A.D; c += 16) {
+            uint32_t o[8];
+            tmem_ld8(base + S::kO + c, o);
+            tmem_wait_ld();
 #pragma unroll
-        for (int n = 0; n < NS; ++n) st16(base + S::kP + n * (BN / 2) + sub * (kSub / 2), w[n]);
+            for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st8(base + S::kO + c, o);
+          }
+        }
+        moved = true;
       }
+      l += sum;
+      if (!S::kOver && j > 0) wait(&ofull[t], (j - 1) & 1, &abort_flag, polls);
+      if (S::kOver) named_barrier(2 + t, 256);  // both halves have read the scores
+#pragma unroll
+      for (int c = 0; c < S::kHalf / kSub; ++c)
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+          st16(base + S::kP + n * (BN / 2) + (half * S::kHalf + c * kSub) / 2, p[c][n]);
       tmem_wait_st();
       fence_before_sync();
       arrive(&pfull[t]);
     }
+    shared_row[t][half][r] = l;
+    named_barrier(2 + t, 256);
+    l = shared_row[t][0][r] + shared_row[t][1][r];
     // -------------------------------------------------------- output
     if (tiles > 0) {
       wait(&ofull[t], (tiles - 1) & 1, &abort_flag, polls);
@@ -559,7 +633,7 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
     const bool ovec =
         A.D % V == 0 && ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(A.os[2] * sizeof(T))) & 15) == 0;
 #pragma unroll
-    for (int c = 0; c < L::kDim; c += 16) {
+    for (int c = half * 16; c < L::kDim; c += 32) {
       if (c < A.D) {
         uint32_t o[16];
         if (tiles > 0) {
@@ -582,9 +656,9 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
         }
       }
     }
-    if (valid && A.lse)
+    if (valid && half == 0 && A.lse)
       A.lse[((int64_t)b * A.H + h) * A.Lq + i] = broken ? NAN : l == 0.f ? -INFINITY : m + log2f(l);
-  } else if (warp == 4 * QT) {
+  } else if (warp == 8 * QT) {
     // -------------------------------------------------------- tensor instructions
     if (lane == 0 && tiles > 0) {
       const uint32_t id_s = idesc_bf16(128, BN, false), id_o = idesc_bf16(128, (A.D + 15) / 16 * 16, true);
@@ -631,7 +705,7 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
     }
   } else {
     // -------------------------------------------------------- loads
-    const int t = tid - 128 * QT - 32, w = t >> 5;
+    const int t = tid - 256 * QT - 32, w = t >> 5;
     const auto fill = [&](int j, int sub) {
       const int64_t j0 = (int64_t)j * BN;
       fill_info<BN>(

@@ -47,12 +47,8 @@ struct BucketArgs {
 // the distance clamped to [-reach, reach], 2 reach + 1 entries.
 __device__ __forceinline__ int bucket_of(const BucketArgs& B, int d) {
   const int a = B.two_sided ? abs(d) : max(-d, 0);
-  int lo = 0, hi = B.num_edges;  // the number of edges <= a
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (B.edges[mid] <= a) lo = mid + 1;
-    else hi = mid;
-  }
+  int lo = 0;  // the number of edges <= a; the same edge for all threads of a step
+  for (int i = 0; i < B.num_edges; ++i) lo += B.edges[i] <= a;
   return lo + (B.two_sided && d > 0 ? B.num_buckets / 2 : 0);
 }
 

@@ -1,4 +1,5 @@
 // Attention with the position bias: checks, choice of kernel, launch shapes, workspace.
+#include "attn_decode.cuh"
 #include "attn_host.cuh"
 #include "attn_rows_grad.cuh"
 #include "position_bias.cuh"
@@ -99,14 +100,29 @@ int lanes_of(const fx_attn_args* a) {
   return need <= 8 ? 8 : need <= 16 ? 16 : 32;
 }
 
+// Whether the fragment kernel of a bfloat16 cache runs (attn_decode.cuh); float32 and tables whose
+// distances take more than 64 KB for a key head's query heads (it holds them all) take the rows
+// kernel.
+bool use_decode(const fx_attn_args* a) {
+  if (a->dtype != FX_BF16 || use_tc(a)) return false;
+  return !a->table || a->heads / a->kv_heads * (2 * make_buckets(a->buckets).reach + 1) <= 16384;
+}
+
+// Parts of the keys. Rows kernel: eight blocks an SM, parts of 128 keys at least. Fragment kernel:
+// parts of 512 keys at least (its eight warps take 128 a step), sixteen blocks an SM: the parts of a
+// ragged batch have different lengths, and short ones even that out.
 void split_keys(const fx_attn_args* a, int sms, AttnArgs& A) {
+  const bool dec = use_decode(a);
   const int64_t rows = a->heads / a->kv_heads * a->q_len;
-  const int64_t blocks = (rows + kRC - 1) / kRC * a->batch * a->kv_heads;
-  int64_t splits = (int64_t{8} * sms + blocks - 1) / blocks;
-  const int64_t most = (a->k_len + kMinSplit - 1) / kMinSplit;
+  const int64_t blocks = (dec ? 1 : (rows + kRC - 1) / kRC) * a->batch * a->kv_heads;
+  int64_t splits = (int64_t{dec ? 16 : 8} * sms + blocks - 1) / blocks;
+  const int64_t least = dec ? 512 : kMinSplit, most = (a->k_len + least - 1) / least;
   splits = splits < most ? splits : most;
+  if (dec && splits < (a->k_len + kDecodeMaxKeys - 1) / kDecodeMaxKeys)
+    splits = (a->k_len + kDecodeMaxKeys - 1) / kDecodeMaxKeys;
   if (splits < 1) splits = 1;
-  A.split_keys = ((a->k_len + splits - 1) / splits + 31) / 32 * 32;
+  const int64_t unit = dec ? 128 : 32;
+  A.split_keys = ((a->k_len + splits - 1) / splits + unit - 1) / unit * unit;
   A.splits = A.split_keys ? (int)((a->k_len + A.split_keys - 1) / A.split_keys) : 1;
   if (A.splits < 1) A.splits = 1;
 }
@@ -133,6 +149,23 @@ int launch_fwd(cudaStream_t s, const AttnArgs& A) {
     if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
   }
   return FX_OK;
+}
+
+template <int DB, bool VEC>
+int launch_decode(cudaStream_t s, const AttnArgs& A) {
+  const size_t rows = (size_t)(A.H / A.Hk * A.Lq);
+  const size_t lut = A.table ? (size_t)(A.H / A.Hk) * (2 * A.buckets.reach + 1) * 4 : 0;
+  const size_t join = (size_t)kDecodeWarps * (2 * kDecodeRows + rows * (64 * DB + 1)) * 4;
+  const size_t smem = lut > join ? lut : join;
+  auto kern = attn_decode_kernel<DB, VEC>;
+  if (raise_smem(kern, smem)) return FX_ERR_CUDA;
+  const int64_t blocks = (int64_t)A.B * A.Hk * A.splits;
+  if (blocks > kMaxGrid) return FX_ERR_SHAPE;
+  kern<<<(unsigned)blocks, kDecodeThreads, smem, s>>>(A);
+  if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
+  if (A.splits > 1)
+    attn_join_kernel<bf16><<<(unsigned)(((int64_t)A.B * A.H * A.Lq + 3) / 4), kRowsThreads, 0, s>>>(A);
+  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
 template <typename T, int LPK, bool VL>
@@ -219,6 +252,10 @@ int fermix_biased_attention(void* stream, const fx_attn_args* a, void* ws, size_
   if (need) {
     if (!ws || wsb < need) return FX_ERR_WORKSPACE;
     A.part = reinterpret_cast<float*>(align256(reinterpret_cast<uintptr_t>(ws)));
+  }
+  if (use_decode(a)) {
+    if (a->dim <= 64) return vec ? launch_decode<1, true>(s, A) : launch_decode<1, false>(s, A);
+    return vec ? launch_decode<2, true>(s, A) : launch_decode<2, false>(s, A);
   }
   return a->dtype == FX_F32 ? fwd<float>(s, A, lanes_of(a), vec) : fwd<bf16>(s, A, lanes_of(a), vec);
 }

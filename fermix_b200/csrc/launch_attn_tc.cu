@@ -1,4 +1,5 @@
 // The tcgen05 kernels of the biased attention (attn_tc.cuh): launch shapes.
+#include <cstdlib>
 #include "attn_host.cuh"
 #include "attn_tc.cuh"
 #include "attn_tc_grad.cuh"
@@ -81,6 +82,11 @@ int fwd_f32(cudaStream_t s, const AttnArgs& A) {
 
 template <int LOAD>
 int fwd_bf16(cudaStream_t s, const AttnArgs& A) {
+  if (getenv("FXV") && atoi(getenv("FXV"))==1 && A.D<=64) return fwd<bf16, 1, 1, 64, Half, 2, LOAD>(s, A);
+  if (getenv("FXV") && atoi(getenv("FXV"))==2 && A.D<=64) return fwd<bf16, 1, 1, 128, Half, 2, LOAD>(s, A);
+  if (getenv("FXV") && atoi(getenv("FXV"))==3 && A.D<=64) return fwd<bf16, 1, 1, 64, Half, 3, LOAD>(s, A);
+  if (getenv("FXV") && atoi(getenv("FXV"))==1) return fwd<bf16, 1, 1, 64, Whole, 2, LOAD>(s, A);
+  if (getenv("FXV") && atoi(getenv("FXV"))==2) return fwd<bf16, 1, 1, 128, Whole, 1, LOAD>(s, A);
   if (A.Lq <= 128) return A.D <= 64 ? fwd<bf16, 1, 1, 64, Half, 2, LOAD>(s, A) : fwd<bf16, 1, 1, 64, Whole, 2, LOAD>(s, A);
   return A.D <= 64 ? fwd<bf16, 1, 2, 128, Half, 2, LOAD>(s, A) : fwd<bf16, 1, 2, 128, Whole, 2, LOAD>(s, A);
 }
