@@ -10,6 +10,10 @@
 // columns is free, so a lane's 16-byte piece of a value row serves eight column tiles after two
 // byte permutations each. The scores' fragment is the probabilities' operand fragment. tcgen05
 // would need the cache staged through shared memory for 16 rows of 128.
+//
+// A lane copies the pieces it will use into a ring of its own in shared memory (cp.async), three
+// steps ahead: 96 KB a block on the way without registers (with the loads in registers, one step
+// at a time, 217 us for 64 key heads of 65536 keys, three quarters live; with the ring 186 us).
 #pragma once
 #include "attn_rows.cuh"
 
@@ -17,7 +21,7 @@ namespace fx {
 
 constexpr int kDecodeThreads = 256, kDecodeWarps = 8;
 constexpr int kDecodeRows = 16;       // query rows of a block
-constexpr int kDecodeMaxKeys = 8192;  // keys of a part, at most
+constexpr int kDecodeStages = 3;
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
@@ -26,37 +30,90 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Entries [c, c + 8) of a token, zero past D. VEC: tokens start on 16-byte boundaries and are
-// whole pieces; else entry by entry, in the same places, so that the results have the same bits.
+// Entries [c, c + 8) of a token, zero past D, into a slot of the ring. VEC: tokens start on 16-byte
+// boundaries and are whole pieces; else entry by entry, in the same places, so that the results
+// have the same bits.
 template <bool VEC>
-__device__ __forceinline__ uint4 piece8(const bf16* p, int c, int D) {
-  if (VEC) return c < D ? __ldg(reinterpret_cast<const uint4*>(p + c)) : make_uint4(0u, 0u, 0u, 0u);
+__device__ __forceinline__ void fetch8(uint4* slot, const bf16* p, int c, int D, bool ok) {
+  if (VEC) {
+    const int bytes = ok && c < D ? 16 : 0;  // 0: zeros, nothing is read
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                     static_cast<uint32_t>(__cvta_generic_to_shared(slot))),
+                 "l"(bytes ? p + c : p), "r"(bytes)
+                 : "memory");
+    return;
+  }
   Pack<bf16, 8> k;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) k.e[e] = c + e < D ? p[c + e] : from_f<bf16>(0.f);
-  return *reinterpret_cast<const uint4*>(&k);
+  for (int e = 0; e < 8; ++e) k.e[e] = ok && c + e < D ? p[c + e] : from_f<bf16>(0.f);
+  *slot = *reinterpret_cast<const uint4*>(&k);
 }
 
-// A block: one part of the keys of one (batch, key head). DB: 64-entry blocks of the head
+// A block: one part of the keys of one (batch, key head): of every `splits` runs of 128 keys one,
+// so that the parts of a cache whose end is masked have the same number of live keys. DB: 64-entry blocks of the head
 // dimension. Entries beyond D are zero.
 template <int DB, bool VEC>
 __global__ void __launch_bounds__(kDecodeThreads, DB == 1 ? 2 : 1) attn_decode_kernel(const __grid_constant__ AttnArgs A) {
-  extern __shared__ float sm[];  // table by distance of each head; after the keys, the warps' joins
-  __shared__ uint32_t live[kDecodeMaxKeys / 32];
+  constexpr int S = kDecodeStages, P = 8 * DB;  // pieces of a lane and step: keys 4 DB, values 4 DB
+  extern __shared__ uint4 ring_mem[];  // the ring (after the keys, the warps' joins), the table by distance
+  float* sm = reinterpret_cast<float*>(ring_mem + S * P * kDecodeThreads);
   const int G = A.H / A.Hk, reach = A.buckets.reach, span = A.table ? 2 * reach + 1 : 0;
   const int rows = G * (int)A.Lq;
   const int part = blockIdx.x % A.splits, z = blockIdx.x / A.splits, b = z / A.Hk, hk = z % A.Hk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int64_t j0 = part * A.split_keys;
-  const int count = (int)(j0 + A.split_keys < A.Lk ? A.split_keys : A.Lk - j0);
+  const int64_t j0 = part * (kDecodeWarps * 16), kStep = (int64_t)A.splits * (kDecodeWarps * 16);
+  const int64_t count = A.Lk - j0;
 
-  // live keys, one bit each
-  for (int w = warp; w * 32 < count; w += kDecodeWarps) {
-    const int e = w * 32 + lane;
-    const uint32_t bits =
-        __ballot_sync(0xffffffffu, e < count && (!A.mask || A.mask[b * A.mask_stride + j0 + e]));
-    if (lane == 0) live[w] = bits;
-  }
+  const bf16* K = static_cast<const bf16*>(A.k) + b * A.ks[0] + hk * A.ks[1] + j0 * A.ks[2];
+  const bf16* V = static_cast<const bf16*>(A.v) + b * A.vs[0] + hk * A.vs[1] + j0 * A.vs[2];
+  uint4* slots = ring_mem + (warp * S * P) * 32 + lane;  // slot (stage, piece) at (stage * P + piece) * 32
+  // Live keys of this warp's groups of 16: lane n holds group first + n, 32 groups at a time.
+  const auto group_bits = [&](int first) -> uint32_t {
+    const int64_t base = warp * 16 + (first + lane) * kStep;
+    if (base >= count) return 0u;
+    const int n = count - base < 16 ? (int)(count - base) : 16;
+    if (!A.mask) return (1u << n) - 1u;
+    const uint8_t* p = A.mask + b * A.mask_stride + j0 + base;
+    uint32_t bits = 0;
+    if (n == 16 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 16; ++e) bits |= ((w[e / 4] >> (e % 4 * 8)) & 0xffu ? 1u : 0u) << e;
+    } else {
+      for (int e = 0; e < n; ++e) bits |= (p[e] ? 1u : 0u) << e;
+    }
+    return bits;
+  };
+  uint32_t mine = group_bits(0), after = 0;  // of groups [first, first + 32) and the 32 after them
+  int first = 0;
+  const auto bits_of = [&](int n) { return __shfl_sync(0xffffffffu, n - first < 32 ? mine : after, n & 31); };
+  // keys base + g and base + 8 + g; values of keys base + {2t, 2t + 1, 2t + 8, 2t + 9}
+  const auto fetch = [&](int n_group, int stage) {
+    const uint32_t bits = bits_of(n_group);
+    const int64_t base = warp * 16 + n_group * kStep;
+    if (bits != 0) {
+      uint4* slot = slots + stage * P * 32;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int e = n * 8 + g;
+#pragma unroll
+        for (int c = 0; c < 2 * DB; ++c)
+          fetch8<VEC>(slot + (n * 2 * DB + c) * 32, K + (base + e) * A.ks[2], c * 32 + t * 8, A.D, (bits >> e) & 1u);
+      }
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const int e = 2 * t + (n & 1) + (n >> 1) * 8;
+#pragma unroll
+        for (int c = 0; c < DB; ++c)
+          fetch8<VEC>(slot + (4 * DB + n * DB + c) * 32, V + (base + e) * A.vs[2], c * 64 + g * 8, A.D,
+                      (bits >> e) & 1u);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int n = 0; n < S - 1; ++n) fetch(n, n);
   if (A.table) {
     const bf16* table = static_cast<const bf16*>(A.table) + (int64_t)hk * G * A.buckets.num_buckets;
     for (int i = threadIdx.x; i < G * span; i += kDecodeThreads)
@@ -75,31 +132,39 @@ __global__ void __launch_bounds__(kDecodeThreads, DB == 1 ? 2 : 1) attn_decode_k
     lut[r] = h * span;
     const bf16* p = static_cast<const bf16*>(A.q) + b * A.qs[0] + (hk * G + h) * A.qs[1] + i * A.qs[2];
 #pragma unroll
-    for (int c = 0; c < 2 * DB; ++c)
-      q[r][c] = row_ok[r] ? piece8<VEC>(p, c * 32 + t * 8, A.D) : make_uint4(0u, 0u, 0u, 0u);
+    for (int c = 0; c < 2 * DB; ++c) {
+      Pack<bf16, 8> x;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x.e[e] = row_ok[r] && c * 32 + t * 8 + e < A.D ? p[c * 32 + t * 8 + e] : from_f<bf16>(0.f);
+      q[r][c] = *reinterpret_cast<const uint4*>(&x);
+    }
   }
   const int rows_hi = rows > 8;
   __syncthreads();
 
-  const bf16* K = static_cast<const bf16*>(A.k) + b * A.ks[0] + hk * A.ks[1] + j0 * A.ks[2];
-  const bf16* V = static_cast<const bf16*>(A.v) + b * A.vs[0] + hk * A.vs[1] + j0 * A.vs[2];
   float o[8 * DB][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
   for (int e = 0; e < 8 * DB; ++e) o[e][0] = o[e][1] = o[e][2] = o[e][3] = 0.f;
 
-  for (int base = warp * 16; base < count; base += kDecodeWarps * 16) {
-    const uint32_t bits = (live[base >> 5] >> (base & 31)) & 0xffffu;
+  int stage = 0;
+  const int groups = (int)((count - warp * 16 + kStep - 1) / kStep);  // <= 0: none
+  for (int n_group = 0; n_group < groups; ++n_group, stage = stage == S - 1 ? 0 : stage + 1) {
+    const int64_t base = warp * 16 + n_group * kStep;
+    if ((n_group & 31) == 16) after = group_bits(n_group - 16 + 32);
+    if (n_group - first == 32) {
+      mine = after;
+      first = n_group;
+    }
+    fetch(n_group + S - 1, stage == 0 ? S - 1 : stage - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+    const uint32_t bits = bits_of(n_group);
     if (bits == 0) continue;
-    // keys base + g and base + 8 + g; values of keys base + {2t, 2t + 1, 2t + 8, 2t + 9}
+    const uint4* slot = slots + stage * P * 32;
     uint4 k[2][2 * DB], v[4][DB];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int e = n * 8 + g;
-      const bf16* p = K + (int64_t)(base + e) * A.ks[2];
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int c = 0; c < 2 * DB; ++c)
-        k[n][c] = (bits >> e) & 1u ? piece8<VEC>(p, c * 32 + t * 8, A.D) : make_uint4(0u, 0u, 0u, 0u);
-    }
+      for (int c = 0; c < 2 * DB; ++c) k[n][c] = slot[(n * 2 * DB + c) * 32];
     bool ok[4];
     int kp[4];
 #pragma unroll
@@ -107,10 +172,8 @@ __global__ void __launch_bounds__(kDecodeThreads, DB == 1 ? 2 : 1) attn_decode_k
       const int e = 2 * t + (n & 1) + (n >> 1) * 8;
       ok[n] = (bits >> e) & 1u;
       kp[n] = ok[n] ? attn_k_pos(A, b, j0 + base + e) : 0;
-      const bf16* p = V + (int64_t)(base + e) * A.vs[2];
 #pragma unroll
-      for (int c = 0; c < DB; ++c)
-        v[n][c] = ok[n] ? piece8<VEC>(p, c * 64 + g * 8, A.D) : make_uint4(0u, 0u, 0u, 0u);
+      for (int c = 0; c < DB; ++c) v[n][c] = slot[(4 * DB + n * DB + c) * 32];
     }
     float s[2][4] = {};  // s[n]: rows g, g + 8 of keys n * 8 + 2t, + 1
 #pragma unroll
@@ -189,8 +252,9 @@ __global__ void __launch_bounds__(kDecodeThreads, DB == 1 ? 2 : 1) attn_decode_k
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  float* wm = sm;                                  // warps x 16
+  float* wm = reinterpret_cast<float*>(ring_mem);                                  // warps x 16
   float* wl = wm + kDecodeWarps * kDecodeRows;     // warps x 16
   float* wo = wl + kDecodeWarps * kDecodeRows;     // warps x rows x (64 DB + 1)
   constexpr int W = 64 * DB + 1;

@@ -203,35 +203,54 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_kernel(const __grid_co
   }
 }
 
-// A warp a row: the parts' (m, l, o) into the output.
+// A block a row: the parts' (m, l, o) into the output. The parts' weights first, side by side,
+// then a thread an entry.
 template <typename T>
 __global__ void __launch_bounds__(kRowsThreads) attn_join_kernel(const __grid_constant__ AttnArgs A) {
-  const int G = A.H / A.Hk, lane = threadIdx.x & 31;
-  const int64_t rows = (int64_t)G * A.Lq;
-  const int64_t w = (int64_t)blockIdx.x * (kRowsThreads / 32) + (threadIdx.x >> 5);
-  if (w >= rows * A.B * A.Hk) return;
-  const int64_t z = w / rows, row = w % rows;
+  static_assert(FX_ATTN_MAX_DIM <= kRowsThreads);
+  __shared__ float red[kRowsThreads / 32], weight[kRowsThreads];
+  const int G = A.H / A.Hk, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t rows = (int64_t)G * A.Lq, w = blockIdx.x, z = w / rows, row = w % rows;
   const int b = (int)(z / A.Hk), h = (int)(z % A.Hk) * G + (int)(row / A.Lq);
   const int64_t i = row % A.Lq;
   const float* p = A.part + w * A.splits * (A.D + 2);
   float top = -INFINITY;
-  for (int s = lane; s < A.splits; s += 32) top = fmaxf(top, p[(int64_t)s * (A.D + 2)]);
+  for (int s = threadIdx.x; s < A.splits; s += kRowsThreads) top = fmaxf(top, p[(int64_t)s * (A.D + 2)]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) red[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kRowsThreads / 32; ++k) top = fmaxf(top, red[k]);
   const float ref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, acc[FX_ATTN_MAX_DIM / 32] = {};
-  for (int s = 0; s < A.splits; ++s, p += A.D + 2) {
-    const float f = exp2f(p[0] - ref);
-    sum = fmaf(p[1], f, sum);
-#pragma unroll
-    for (int e = 0; e < FX_ATTN_MAX_DIM / 32; ++e)
-      if (lane + 32 * e < A.D) acc[e] = fmaf(p[2 + lane + 32 * e], f, acc[e]);
+  float sum = 0.f, acc = 0.f;
+  for (int s0 = 0; s0 < A.splits; s0 += kRowsThreads) {
+    const int n = A.splits - s0 < kRowsThreads ? A.splits - s0 : kRowsThreads;
+    __syncthreads();
+    if (threadIdx.x < n) {
+      const float* q = p + (int64_t)(s0 + threadIdx.x) * (A.D + 2);
+      const float f = exp2f(q[0] - ref);
+      weight[threadIdx.x] = f;
+      sum = fmaf(q[1], f, sum);
+    }
+    __syncthreads();
+    if (threadIdx.x < A.D) {
+      const float* q = p + (int64_t)s0 * (A.D + 2) + 2 + threadIdx.x;
+#pragma unroll 8
+      for (int s = 0; s < n; ++s) acc = fmaf(q[(int64_t)s * (A.D + 2)], weight[s], acc);
+    }
   }
-  T* out = static_cast<T*>(A.out) + b * A.os[0] + h * A.os[1] + i * A.os[2];
+  sum = lanes_sum(sum, 32);
+  __syncthreads();
+  if (lane == 0) red[warp] = sum;
+  __syncthreads();
+  sum = 0.f;
 #pragma unroll
-  for (int e = 0; e < FX_ATTN_MAX_DIM / 32; ++e)
-    if (lane + 32 * e < A.D) out[lane + 32 * e] = from_f<T>(sum == 0.f ? 0.f : acc[e] / sum);
-  if (A.lse && lane == 0) A.lse[((int64_t)b * A.H + h) * A.Lq + i] = sum == 0.f ? -INFINITY : top + log2f(sum);
+  for (int k = 0; k < kRowsThreads / 32; ++k) sum += red[k];
+  if (threadIdx.x < A.D)
+    static_cast<T*>(A.out)[b * A.os[0] + h * A.os[1] + i * A.os[2] + threadIdx.x] =
+        from_f<T>(sum == 0.f ? 0.f : acc / sum);
+  if (A.lse && threadIdx.x == 0) A.lse[((int64_t)b * A.H + h) * A.Lq + i] = sum == 0.f ? -INFINITY : top + log2f(sum);
 }
 
 }  // namespace fx

@@ -101,28 +101,31 @@ int lanes_of(const fx_attn_args* a) {
 }
 
 // Whether the fragment kernel of a bfloat16 cache runs (attn_decode.cuh); float32 and tables whose
-// distances take more than 64 KB for a key head's query heads (it holds them all) take the rows
-// kernel.
+// distances take more than 16 KB (32 KB above 64 entries) for a key head's query heads, beside two
+// (one) rings of 96 KB (192 KB) an SM, take the rows kernel.
 bool use_decode(const fx_attn_args* a) {
   if (a->dtype != FX_BF16 || use_tc(a)) return false;
-  return !a->table || a->heads / a->kv_heads * (2 * make_buckets(a->buckets).reach + 1) <= 16384;
+  return !a->table || a->heads / a->kv_heads * (2 * make_buckets(a->buckets).reach + 1) <= (a->dim <= 64 ? 4096 : 8192);
 }
 
 // Parts of the keys. Rows kernel: eight blocks an SM, parts of 128 keys at least. Fragment kernel:
-// parts of 512 keys at least (its eight warps take 128 a step), sixteen blocks an SM: the parts of a
-// ragged batch have different lengths, and short ones even that out.
+// two rounds of the two blocks an SM holds (one above 64 entries), 512 keys a part at least; more
+// and shorter parts spend more time on a block's start (measured for 64 key heads of 65536 keys:
+// 37 parts 205 us, 9 parts 186 us).
 void split_keys(const fx_attn_args* a, int sms, AttnArgs& A) {
-  const bool dec = use_decode(a);
+  if (use_decode(a)) {
+    const int64_t blocks = a->batch * a->kv_heads, want = (int64_t{a->dim <= 64 ? 4 : 2} * sms) / blocks;
+    const int64_t most = (a->k_len + 511) / 512, splits = want < most ? want : most;
+    A.splits = splits < 1 ? 1 : (int)splits;
+    return;
+  }
   const int64_t rows = a->heads / a->kv_heads * a->q_len;
-  const int64_t blocks = (dec ? 1 : (rows + kRC - 1) / kRC) * a->batch * a->kv_heads;
-  int64_t splits = (int64_t{dec ? 16 : 8} * sms + blocks - 1) / blocks;
-  const int64_t least = dec ? 512 : kMinSplit, most = (a->k_len + least - 1) / least;
+  const int64_t blocks = (rows + kRC - 1) / kRC * a->batch * a->kv_heads;
+  int64_t splits = (int64_t{8} * sms + blocks - 1) / blocks;
+  const int64_t most = (a->k_len + kMinSplit - 1) / kMinSplit;
   splits = splits < most ? splits : most;
-  if (dec && splits < (a->k_len + kDecodeMaxKeys - 1) / kDecodeMaxKeys)
-    splits = (a->k_len + kDecodeMaxKeys - 1) / kDecodeMaxKeys;
   if (splits < 1) splits = 1;
-  const int64_t unit = dec ? 128 : 32;
-  A.split_keys = ((a->k_len + splits - 1) / splits + unit - 1) / unit * unit;
+  A.split_keys = ((a->k_len + splits - 1) / splits + 31) / 32 * 32;
   A.splits = A.split_keys ? (int)((a->k_len + A.split_keys - 1) / A.split_keys) : 1;
   if (A.splits < 1) A.splits = 1;
 }
@@ -145,7 +148,7 @@ int launch_fwd(cudaStream_t s, const AttnArgs& A) {
   kern<<<(unsigned)blocks, kRowsThreads, smem, s>>>(A);
   if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
   if (A.splits > 1) {
-    attn_join_kernel<T><<<(unsigned)(((int64_t)A.B * A.H * A.Lq + 3) / 4), kRowsThreads, 0, s>>>(A);
+    attn_join_kernel<T><<<(unsigned)((int64_t)A.B * A.H * A.Lq), kRowsThreads, 0, s>>>(A);
     if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
   }
   return FX_OK;
@@ -153,10 +156,11 @@ int launch_fwd(cudaStream_t s, const AttnArgs& A) {
 
 template <int DB, bool VEC>
 int launch_decode(cudaStream_t s, const AttnArgs& A) {
-  const size_t rows = (size_t)(A.H / A.Hk * A.Lq);
   const size_t lut = A.table ? (size_t)(A.H / A.Hk) * (2 * A.buckets.reach + 1) * 4 : 0;
-  const size_t join = (size_t)kDecodeWarps * (2 * kDecodeRows + rows * (64 * DB + 1)) * 4;
-  const size_t smem = lut > join ? lut : join;
+  const size_t ring = (size_t)kDecodeStages * 8 * DB * kDecodeThreads * 16;
+  static_assert(kDecodeWarps * (2 * kDecodeRows + kDecodeRows * (64 * DB + 1)) * 4 <=
+                kDecodeStages * 8 * DB * kDecodeThreads * 16);
+  const size_t smem = ring + lut;
   auto kern = attn_decode_kernel<DB, VEC>;
   if (raise_smem(kern, smem)) return FX_ERR_CUDA;
   const int64_t blocks = (int64_t)A.B * A.Hk * A.splits;
@@ -164,7 +168,7 @@ int launch_decode(cudaStream_t s, const AttnArgs& A) {
   kern<<<(unsigned)blocks, kDecodeThreads, smem, s>>>(A);
   if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
   if (A.splits > 1)
-    attn_join_kernel<bf16><<<(unsigned)(((int64_t)A.B * A.H * A.Lq + 3) / 4), kRowsThreads, 0, s>>>(A);
+    attn_join_kernel<bf16><<<(unsigned)((int64_t)A.B * A.H * A.Lq), kRowsThreads, 0, s>>>(A);
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
