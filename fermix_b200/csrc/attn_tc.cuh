@@ -123,6 +123,12 @@ __device__ __forceinline__ uint64_t add_both(uint64_t a, uint64_t b) {
   return r;
 }
 
+__device__ __forceinline__ uint64_t mul_both(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // (a, b) -> NS packed pairs whose sum is (a, b)
 template <int NS>
 __device__ __forceinline__ void split2(float a, float b, uint32_t (&o)[NS]) {

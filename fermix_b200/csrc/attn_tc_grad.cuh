@@ -134,6 +134,11 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
     mbar_init(&pfull, 256);
     mbar_init(&done, 1);
     fence_mbar_init();
+    if constexpr (TMA) {
+      mbar_arrive_expect_tx(&own, 2 * S::kOwn);
+      tma_tile<L>(sK, M, MAP_K, 128, j0, hk, b, &own);
+      tma_tile<L>(sV, M, MAP_V, 128, j0, hk, b, &own);
+    }
   }
   if (warp == 0) {
     tmem_alloc(&tmem_slot, S::kAlloc);
@@ -141,11 +146,6 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
   }
   const auto key_live = [&](int r) { return j0 + r < A.Lk && (!mask || mask[j0 + r]); };
   if constexpr (TMA) {
-    if (tid == 0) {
-      mbar_arrive_expect_tx(&own, 2 * S::kOwn);
-      tma_tile<L>(sK, M, MAP_K, 128, j0, hk, b, &own);
-      tma_tile<L>(sV, M, MAP_V, 128, j0, hk, b, &own);
-    }
     __syncthreads();
     wait(&own, 0, &abort_flag, A.polls);
     if (mask) {
@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
       const bool above = (int64_t)klo - qhi >= reach, below = (int64_t)khi - qlo <= -reach;
       const bool each = some && ((A.table && !above && !below) || (A.causal && khi > qlo));
       const float flat = A.table && some && !each ? lut[above ? 2 * reach : 0] : 0.f;
-#pragma unroll
+#pragma unroll 1  // one copy of the code: two no longer stay in the instruction cache
       for (int c = 0; c < 32; c += 16) {
         const int col = wg * 32 + c;
         uint32_t s[16], dp[16];
@@ -203,37 +203,64 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
         ld16(base + S::kDp + col, dp);
         tmem_wait_ld();
         uint32_t wp[NS][8], wd[NS][8];
+        float bias[16];  // less lse: +inf there leaves a row out
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
-          const float4 ls = *reinterpret_cast<const float4*>(&I.lse[col + e]);
-          const float4 de = *reinterpret_cast<const float4*>(&I.delta[col + e]);
-          const float l4[4] = {ls.x, ls.y, ls.z, ls.w}, d4[4] = {de.x, de.y, de.z, de.w};
-          float p[4], ds[4];
-          if (each) {
-            const int4 qp = *reinterpret_cast<const int4*>(&I.t.pos[col + e]);
-            const int q4[4] = {qp.x, qp.y, qp.z, qp.w};
+          const float4 v = *reinterpret_cast<const float4*>(&I.lse[col + e]);
+          bias[e] = -v.x;
+          bias[e + 1] = -v.y;
+          bias[e + 2] = -v.z;
+          bias[e + 3] = -v.w;
+        }
+        if (each) {
+          int q[16];
 #pragma unroll
-            for (int f = 0; f < 4; ++f) {
-              const int d = kp - q4[f];
-              const float bias = A.table ? lut[clamp_reach(d, reach) + reach] : 0.f;
-              p[f] = ex2(fmaf(__uint_as_float(s[e + f]), A.scale2, bias - l4[f]));
-              if (A.causal && d > 0) p[f] = 0.f;
-            }
-          } else {
-#pragma unroll
-            for (int f = 0; f < 4; ++f) p[f] = ex2(fmaf(__uint_as_float(s[e + f]), A.scale2, flat - l4[f]));
+          for (int e = 0; e < 16; e += 4) {
+            const int4 v = *reinterpret_cast<const int4*>(&I.t.pos[col + e]);
+            q[e] = v.x;
+            q[e + 1] = v.y;
+            q[e + 2] = v.z;
+            q[e + 3] = v.w;
           }
+          if (A.table) {
+            float t[16];
 #pragma unroll
-          for (int f = 0; f < 4; ++f) ds[f] = p[f] * (__uint_as_float(dp[e + f]) - d4[f]);
+            for (int e = 0; e < 16; ++e) t[e] = lut[__vimin_s32_relu(kp + reach - q[e], 2 * reach)];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) bias[e] += t[e];
+          }
+          if (A.causal) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (kp > q[e]) bias[e] = -INFINITY;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) bias[e] += flat;
+        }
+        const uint64_t ss = both(A.scale2, A.scale2);
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const float4 de = *reinterpret_cast<const float4*>(&I.delta[col + e]);
+          const uint64_t d2[2] = {both(-de.x, -de.y), both(-de.z, -de.w)};
 #pragma unroll
           for (int f = 0; f < 4; f += 2) {
+            const int i0 = e + f;
+            float v0, v1;
+            halves(fma_both(both(__uint_as_float(s[i0]), __uint_as_float(s[i0 + 1])), ss, both(bias[i0], bias[i0 + 1])), v0,
+                   v1);
+            const float p0 = ex2(v0), p1 = ex2(v1);
+            float d0, d1;
+            halves(mul_both(both(p0, p1),
+                            add_both(both(__uint_as_float(dp[i0]), __uint_as_float(dp[i0 + 1])), d2[f / 2])),
+                   d0, d1);
             uint32_t o[NS];
-            split2<NS>(p[f], p[f + 1], o);
+            split2<NS>(p0, p1, o);
 #pragma unroll
-            for (int i = 0; i < NS; ++i) wp[i][(e + f) / 2] = o[i];
-            split2<NS>(ds[f], ds[f + 1], o);
+            for (int i = 0; i < NS; ++i) wp[i][i0 / 2] = o[i];
+            split2<NS>(d0, d1, o);
 #pragma unroll
-            for (int i = 0; i < NS; ++i) wd[i][(e + f) / 2] = o[i];
+            for (int i = 0; i < NS; ++i) wd[i][i0 / 2] = o[i];
           }
         }
 #pragma unroll
@@ -415,19 +442,18 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
     mbar_init(&pfull, 128);
     mbar_init(&done, 1);
     fence_mbar_init();
+    if constexpr (TMA) {
+      mbar_arrive_expect_tx(&own, 2 * S::kOwn);
+      tma_tile<L>(sQ, M, MAP_Q, 128, i0, h, b, &own);
+      tma_tile<L>(sO, M, MAP_DO, 128, i0, h, b, &own);
+    }
   }
   if (warp == 0) {
     tmem_alloc(&tmem_slot, S::kAlloc);
     tmem_relinquish();
   }
   const auto row_live = [&](int r) { return i0 + r < A.Lq && lse[i0 + r] != -INFINITY; };
-  if constexpr (TMA) {
-    if (tid == 0) {
-      mbar_arrive_expect_tx(&own, 2 * S::kOwn);
-      tma_tile<L>(sQ, M, MAP_Q, 128, i0, h, b, &own);
-      tma_tile<L>(sO, M, MAP_DO, 128, i0, h, b, &own);
-    }
-  } else {
+  if constexpr (!TMA) {
     load_tile<T, NS, PIECES, 128, L>(sQ, static_cast<const T*>(A.q) + b * A.qs[0] + h * A.qs[1] + i0 * A.qs[2], A.qs[2],
                                      A.D, tid, S::kThreads, row_live);
     load_tile<T, NS, PIECES, 128, L>(sO, static_cast<const T*>(A.dout) + b * A.dos[0] + h * A.dos[1] + i0 * A.dos[2],
@@ -481,7 +507,7 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
       const TileInfo<kGradN>& I = info[j % S::kInfo];
       wait(&sfull, j & 1, &abort_flag, polls);
       fence_after_sync();
-#pragma unroll
+#pragma unroll 1  // one copy of the code: four no longer stay in the instruction cache
       for (int c = 0; c < kGradN; c += 16) {
         const int sub = c / kSub;
         const uint32_t bits = I.live[sub] >> (c % kSub);
@@ -493,51 +519,122 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
         ld16(base + c, s);
         ld16(base + S::kDp + c, dp);
         tmem_wait_ld();
+        const uint64_t ss = both(A.scale2, A.scale2), nd = both(-delta, -delta);
+        uint64_t sa = 0, sb = 0;  // pairs of zeros
         if (near || later) {
+          // everything that is read before the first histogram is written: the compiler may not
+          // move a lookup over a store
+          int k[16], at[16];
+          float bias[16];
 #pragma unroll
           for (int e = 0; e < 16; e += 4) {
-            const int4 kp = *reinterpret_cast<const int4*>(&I.pos[c + e]);
-            const int k4[4] = {kp.x, kp.y, kp.z, kp.w};
+            const int4 v = *reinterpret_cast<const int4*>(&I.pos[c + e]);
+            k[e] = v.x;
+            k[e + 1] = v.y;
+            k[e + 2] = v.z;
+            k[e + 3] = v.w;
+          }
 #pragma unroll
-            for (int f = 0; f < 4; ++f) {
-              const int d = k4[f] - qp;
-              int2 t = make_int2(0, -1);
-              if (A.table) t = lut[clamp_reach(d, reach) + reach];
-              float p = ex2(fmaf(__uint_as_float(s[e + f]), A.scale2, __int_as_float(t.x) - lse_i));
-              if ((A.causal && d > 0) || !((bits >> (e + f)) & 1u)) p = 0.f;
-              const float x = __uint_as_float(dp[e + f]), px = p * x;
-              if (t.y >= 0) {
-                float2 v = mine[t.y];
-                v.x += px;
-                v.y += p;
-                mine[t.y] = v;
+          for (int e = 0; e < 16; ++e) {
+            int2 t = make_int2(0, -1);
+            if (A.table) t = lut[__vimin_s32_relu(k[e] + reach - qp, 2 * reach)];
+            bias[e] = __int_as_float(t.x) - lse_i;
+            if ((A.causal && k[e] > qp) || !((bits >> e) & 1u)) bias[e] = -INFINITY;
+            at[e] = t.y;
+          }
+          float pr[16], px[16];
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            float v0, v1, x0, x1, y0, y1;
+            halves(fma_both(both(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), ss, both(bias[e], bias[e + 1])), v0, v1);
+            pr[e] = ex2(v0);
+            pr[e + 1] = ex2(v1);
+            const uint64_t pp = both(pr[e], pr[e + 1]), dd = both(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1]));
+            const uint64_t xx = mul_both(pp, dd);
+            halves(xx, x0, x1);
+            px[e] = x0;
+            px[e + 1] = x1;
+            halves(mul_both(pp, add_both(dd, nd)), y0, y1);
+            s[e] = __float_as_uint(y0);
+            s[e + 1] = __float_as_uint(y1);
+            sa = add_both(sa, xx);
+            sb = add_both(sb, pp);
+          }
+          if (A.table) {
+            // four columns at a time: runs of one bucket joined, the rest read together, unless a
+            // bucket comes back after another (positions in any order)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              const int o0 = at[e], o1 = at[e + 1], o2 = at[e + 2], o3 = at[e + 3];
+              const bool j1 = o1 == o0, j2 = o2 == o1, j3 = o3 == o2;
+              const bool back = (o2 == o0 && !j1) || (o3 == o1 && !j2) || (o3 == o0 && !(j1 && j2 && j3) && !(o2 == o0));
+              float a0 = px[e], a1 = px[e + 1], a2 = px[e + 2], a3 = px[e + 3];
+              float b0 = pr[e], b1 = pr[e + 1], b2 = pr[e + 2], b3 = pr[e + 3];
+              if (!__any_sync(0xffffffffu, back)) {
+                if (j1) a1 += a0, b1 += b0;
+                if (j2) a2 += a1, b2 += b1;
+                if (j3) a3 += a2, b3 += b2;
+                const bool w0 = !j1 && o0 >= 0, w1 = !j2 && o1 >= 0, w2 = !j3 && o2 >= 0, w3 = o3 >= 0;
+                float2 h0, h1, h2, h3;
+                if (w0) h0 = mine[o0];
+                if (w1) h1 = mine[o1];
+                if (w2) h2 = mine[o2];
+                if (w3) h3 = mine[o3];
+                if (w0) mine[o0] = make_float2(h0.x + a0, h0.y + b0);
+                if (w1) mine[o1] = make_float2(h1.x + a1, h1.y + b1);
+                if (w2) mine[o2] = make_float2(h2.x + a2, h2.y + b2);
+                if (w3) mine[o3] = make_float2(h3.x + a3, h3.y + b3);
+              } else {
+                const int o[4] = {o0, o1, o2, o3};
+                const float a[4] = {a0, a1, a2, a3}, bb[4] = {b0, b1, b2, b3};
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                  if (o[n] >= 0) {
+                    float2 v = mine[o[n]];
+                    v.x += a[n];
+                    v.y += bb[n];
+                    mine[o[n]] = v;
+                  }
               }
-              ta += px;
-              tb += p;
-              s[e + f] = __float_as_uint(p * (x - delta));
             }
           }
         } else {
           const float flat = (A.table && some ? __int_as_float(lut[above ? 2 * reach : 0].x) : 0.f) - lse_i;
-          float sa = 0.f, sb = 0.f;
+          const uint64_t bb = both(flat, flat);
+          const bool whole = (bits & 0xffffu) == 0xffffu;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float p = ex2(fmaf(__uint_as_float(s[e]), A.scale2, flat));
-            if (!((bits >> e) & 1u)) p = 0.f;
-            const float x = __uint_as_float(dp[e]);
-            sa = fmaf(p, x, sa);
-            sb += p;
-            s[e] = __float_as_uint(p * (x - delta));
+          for (int e = 0; e < 16; e += 2) {
+            float v0, v1, y0, y1;
+            halves(fma_both(both(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), ss, bb), v0, v1);
+            if (!whole) {
+              if (!((bits >> e) & 1u)) v0 = -INFINITY;
+              if (!((bits >> (e + 1)) & 1u)) v1 = -INFINITY;
+            }
+            const uint64_t pp = both(ex2(v0), ex2(v1)), dd = both(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1]));
+            sa = fma_both(pp, dd, sa);
+            sb = add_both(sb, pp);
+            halves(mul_both(pp, add_both(dd, nd)), y0, y1);
+            s[e] = __float_as_uint(y0);
+            s[e + 1] = __float_as_uint(y1);
           }
-          if (above) {
-            ha += sa;
-            hb += sb;
-          } else {
-            la += sa;
-            lb += sb;
+        }
+        {
+          float x0, x1, y0, y1;
+          halves(sa, x0, x1);
+          halves(sb, y0, y1);
+          x0 += x1;
+          y0 += y1;
+          if (!(near || later)) {
+            if (above) {
+              ha += x0;
+              hb += y0;
+            } else {
+              la += x0;
+              lb += y0;
+            }
           }
-          ta += sa;
-          tb += sb;
+          ta += x0;
+          tb += y0;
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -573,18 +670,26 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
       }
       if (!windows) {
         ta = tb = 0.f;
+#pragma unroll 8
         for (int c = 0; c < wn; ++c) {
-          ta += mine[c * 128].x;
-          tb += mine[c * 128].y;
+          const float2 v = mine[c * 128];
+          ta += v.x;
+          tb += v.y;
         }
       }
       const float mean = live && tb != 0.f ? ta / tb : 0.f;
-      for (int c = 0; c < wn; ++c) {
-        const float2 v = mine[c * 128];
-        mine[c * 128].x = live ? fmaf(-v.y, mean, v.x) + broken : 0.f;
+      for (int c = 0; c < wn; c += 8) {
+        float2 v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < wn) v[e] = mine[(c + e) * 128];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < wn) mine[(c + e) * 128].x = live ? fmaf(-v[e].y, mean, v[e].x) + broken : 0.f;
       }
       named_barrier(2, 128);
       float* part = A.dpart + (((int64_t)h * A.B + b) * nq + qb) * A.buckets.num_buckets + w0;
+#pragma unroll 4
       for (int c = warp; c < wn; c += 4) {
         const float2* r = hist + c * 128 + lane;
         const float v = lanes_sum((r[0].x + r[32].x) + (r[64].x + r[96].x), 32);
