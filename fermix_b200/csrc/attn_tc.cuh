@@ -90,6 +90,22 @@ __device__ __forceinline__ void st16(uint32_t a, const uint32_t* v) {
 __device__ __forceinline__ void st8(uint32_t a, const uint32_t* v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(a), FX_I8(v, 0));
 }
+__device__ __forceinline__ void st4(uint32_t a, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]));
+}
+template <int N>
+__device__ __forceinline__ void ld_cols(uint32_t a, uint32_t (&v)[N]) {
+  static_assert(N == 8 || N == 16);
+  if constexpr (N == 8) tmem_ld8(a, v);
+  else ld16(a, v);
+}
+template <int N>
+__device__ __forceinline__ void st_cols(uint32_t a, const uint32_t (&v)[N]) {
+  static_assert(N == 4 || N == 8);
+  if constexpr (N == 4) st4(a, v);
+  else st8(a, v);
+}
 #undef FX_R8
 #undef FX_I8
 
@@ -387,11 +403,11 @@ __device__ __forceinline__ float fwd_columns(const AttnArgs& A, const TileInfo<B
   if ((A.table && !above && !below) || (A.causal && hi > F.qlo)) {
     const int qoff = F.qp - reach, qlim = A.causal ? F.qp : INT32_MAX;
 #pragma unroll
-    for (int c = 0; c < kSub; c += 16) {
-      int k[16];
-      float bias[16];
+    for (int c = 0; c < kSub; c += 8) {
+      int k[8];
+      float bias[8];
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) {
+      for (int e = 0; e < 8; e += 4) {
         const int4 v = *reinterpret_cast<const int4*>(&I.pos[sub * kSub + c + e]);
         k[e] = v.x;
         k[e + 1] = v.y;
@@ -399,9 +415,9 @@ __device__ __forceinline__ float fwd_columns(const AttnArgs& A, const TileInfo<B
         k[e + 3] = v.w;
       }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) bias[e] = A.table ? lut[__vimin_s32_relu(k[e] - qoff, far)] : 0.f;
+      for (int e = 0; e < 8; ++e) bias[e] = A.table ? lut[__vimin_s32_relu(k[e] - qoff, far)] : 0.f;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
+      for (int e = 0; e < 8; ++e) {
         const float v = fmaf(__uint_as_float(x[c + e]), A.scale2, bias[e]) + ref;
         x[c + e] = k[e] > qlim ? 0xff800000u : __float_as_uint(v);
       }
@@ -448,6 +464,7 @@ struct FwdShape {
   static constexpr bool kOver = QT * (BN + NS * BN / 2 + L::kDim) > 512;  // probabilities over the scores
   static constexpr int kP = kOver ? 0 : BN;
   static constexpr int kO = kOver ? BN : BN + NS * BN / 2;
+  static_assert(!kOver || NS == 1);
   static constexpr int kTile = kO + L::kDim;
   static constexpr int kCols = QT * kTile;
   static constexpr int kAlloc = kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
@@ -562,7 +579,8 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
       const TileInfo<BN>& I = info[j % S::kInfo];
       wait(&sfull[t], j & 1, &abort_flag, polls);
       fence_after_sync();
-      uint32_t p[S::kHalf / kSub][NS][16];
+      uint32_t p[S::kOver ? S::kHalf / kSub : 1][NS][16];
+      bool free_p = S::kOver || j == 0;
       float sum = 0.f;
       bool moved = false;
       for (;;) {
@@ -570,13 +588,29 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
         if (!low || moved) {
           const float ref = m == -INFINITY ? 0.f : -m;
           sum = 0.f;
+          if constexpr (S::kOver) {  // held until both halves have read the scores
 #pragma unroll
-          for (int c = 0; c < S::kHalf / kSub; ++c) {
-            const int sub = half * (S::kHalf / kSub) + c;
-            uint32_t x[kSub];
-            ld32(base + sub * kSub, x);
-            tmem_wait_ld();
-            sum += fwd_columns<NS, BN>(A, I, lut, F, sub, ref, x, p[c]);
+            for (int c = 0; c < S::kHalf / kSub; ++c) {
+              const int sub = half * (S::kHalf / kSub) + c;
+              uint32_t x[kSub];
+              ld32(base + sub * kSub, x);
+              tmem_wait_ld();
+              sum += fwd_columns<NS, BN>(A, I, lut, F, sub, ref, x, p[c]);
+            }
+          } else {
+#pragma unroll 1  // one copy of the code: the score loops have to stay in the instruction cache
+            for (int sub = half * (S::kHalf / kSub); sub < (half + 1) * (S::kHalf / kSub); ++sub) {
+              uint32_t x[kSub];
+              ld32(base + sub * kSub, x);
+              tmem_wait_ld();
+              sum += fwd_columns<NS, BN>(A, I, lut, F, sub, ref, x, p[0]);
+              if (!free_p) {  // the last tile's second product has read the probabilities
+                wait(&ofull[t], (j - 1) & 1, &abort_flag, polls);
+                free_p = true;
+              }
+#pragma unroll
+              for (int n = 0; n < NS; ++n) st16(base + S::kP + n * (BN / 2) + sub * (kSub / 2), p[0][n]);
+            }
           }
           low = __any_sync(0xffffffffu, valid && !(sum <= 1.8446744e19f));
         }
@@ -586,10 +620,11 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
         named_barrier(2 + t, 256);
         if (!moving[t][j & 1]) break;
         shared_row[t][half][r] = fwd_top<BN, S::kHalf>(A, I, lut, F, half * S::kHalf);
-        if (!S::kOver && j > 0) {  // the output is at rest
+        if (!free_p) {  // the output is at rest
           wait(&ofull[t], (j - 1) & 1, &abort_flag, polls);
-          fence_after_sync();
+          free_p = true;
         }
+        fence_after_sync();
         named_barrier(2 + t, 256);
         if ((tid & 255) == 0) moving[t][j & 1] = 0;
         const float top = fmaxf(shared_row[t][0][r], shared_row[t][1][r]);
@@ -613,13 +648,12 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
         moved = true;
       }
       l += sum;
-      if (!S::kOver && j > 0) wait(&ofull[t], (j - 1) & 1, &abort_flag, polls);
-      if (S::kOver) named_barrier(2 + t, 256);  // both halves have read the scores
+      if constexpr (S::kOver) {
+        named_barrier(2 + t, 256);  // both halves have read the scores
 #pragma unroll
-      for (int c = 0; c < S::kHalf / kSub; ++c)
-#pragma unroll
-        for (int n = 0; n < NS; ++n)
-          st16(base + S::kP + n * (BN / 2) + (half * S::kHalf + c * kSub) / 2, p[c][n]);
+        for (int c = 0; c < S::kHalf / kSub; ++c)
+          st16(base + S::kP + (half * S::kHalf + c * kSub) / 2, p[c][0]);
+      }
       tmem_wait_st();
       fence_before_sync();
       arrive(&pfull[t]);

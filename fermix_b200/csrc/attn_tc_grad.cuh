@@ -90,6 +90,9 @@ struct DkvShape {
   static constexpr int kCols = kDk + L::kDim, kAlloc = kCols <= 256 ? 256 : 512;
   static constexpr int kInfo = ST + 1;
   static constexpr int kBlocks = kAlloc <= 256 && kTileBytes <= 104 * 1024 ? 2 : 1;  // an SM holds
+  // Columns of a step: 8 fit 80 registers without spills; the second part of 16 columns takes the
+  // place of their latter half, which has to be read by then.
+  static constexpr int kStepCols = NS == 1 ? 8 : 16;
 };
 
 struct alignas(16) QueryInfo {
@@ -195,17 +198,17 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
       const bool above = (int64_t)klo - qhi >= reach, below = (int64_t)khi - qlo <= -reach;
       const bool each = some && ((A.table && !above && !below) || (A.causal && khi > qlo));
       const float flat = A.table && some && !each ? lut[above ? 2 * reach : 0] : 0.f;
-#pragma unroll 1  // one copy of the code: two no longer stay in the instruction cache
-      for (int c = 0; c < 32; c += 16) {
+#pragma unroll 1  // one copy of the code, to stay in the instruction cache
+      for (int c = 0; c < 32; c += S::kStepCols) {
         const int col = wg * 32 + c;
-        uint32_t s[16], dp[16];
-        ld16(base + col, s);
-        ld16(base + S::kDp + col, dp);
+        uint32_t s[S::kStepCols], dp[S::kStepCols];
+        ld_cols<S::kStepCols>(base + col, s);
+        ld_cols<S::kStepCols>(base + S::kDp + col, dp);
         tmem_wait_ld();
-        uint32_t wp[NS][8], wd[NS][8];
-        float bias[16];  // less lse: +inf there leaves a row out
+        uint32_t wp[NS][S::kStepCols / 2], wd[NS][S::kStepCols / 2];
+        float bias[S::kStepCols];  // less lse: +inf there leaves a row out
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
+        for (int e = 0; e < S::kStepCols; e += 4) {
           const float4 v = *reinterpret_cast<const float4*>(&I.lse[col + e]);
           bias[e] = -v.x;
           bias[e + 1] = -v.y;
@@ -213,9 +216,9 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
           bias[e + 3] = -v.w;
         }
         if (each) {
-          int q[16];
+          int q[S::kStepCols];
 #pragma unroll
-          for (int e = 0; e < 16; e += 4) {
+          for (int e = 0; e < S::kStepCols; e += 4) {
             const int4 v = *reinterpret_cast<const int4*>(&I.t.pos[col + e]);
             q[e] = v.x;
             q[e + 1] = v.y;
@@ -223,24 +226,24 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
             q[e + 3] = v.w;
           }
           if (A.table) {
-            float t[16];
+            float t[S::kStepCols];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) t[e] = lut[__vimin_s32_relu(kp + reach - q[e], 2 * reach)];
+            for (int e = 0; e < S::kStepCols; ++e) t[e] = lut[__vimin_s32_relu(kp + reach - q[e], 2 * reach)];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) bias[e] += t[e];
+            for (int e = 0; e < S::kStepCols; ++e) bias[e] += t[e];
           }
           if (A.causal) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
+            for (int e = 0; e < S::kStepCols; ++e)
               if (kp > q[e]) bias[e] = -INFINITY;
           }
         } else {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) bias[e] += flat;
+          for (int e = 0; e < S::kStepCols; ++e) bias[e] += flat;
         }
         const uint64_t ss = both(A.scale2, A.scale2);
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
+        for (int e = 0; e < S::kStepCols; e += 4) {
           const float4 de = *reinterpret_cast<const float4*>(&I.delta[col + e]);
           const uint64_t d2[2] = {both(-de.x, -de.y), both(-de.z, -de.w)};
 #pragma unroll
@@ -265,8 +268,10 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
         }
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-          st8(base + (i < 2 ? col + i * 8 : S::kP3 + col / 2), wp[i]);
-          st8(base + (i < 2 ? S::kDp + col + i * 8 : S::kDs3 + col / 2), wd[i]);
+          // place within the 16 columns' 8 of a part
+          const int at = (col & ~15) + (col & 15) / 2;
+          st_cols<S::kStepCols / 2>(base + (i < 2 ? at + i * 8 : S::kP3 + col / 2), wp[i]);
+          st_cols<S::kStepCols / 2>(base + (i < 2 ? S::kDp + at + i * 8 : S::kDs3 + col / 2), wd[i]);
         }
       }
       tmem_wait_st();

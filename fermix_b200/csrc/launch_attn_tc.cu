@@ -1,5 +1,4 @@
 // The tcgen05 kernels of the biased attention (attn_tc.cuh): launch shapes.
-#include <cstdlib>
 #include "attn_host.cuh"
 #include "attn_tc.cuh"
 #include "attn_tc_grad.cuh"
@@ -80,15 +79,13 @@ int fwd_f32(cudaStream_t s, const AttnArgs& A) {
   return A.D <= 64 ? fwd<float, 3, 1, 64, Half, 1, LOAD>(s, A) : fwd<float, 3, 1, 64, Whole, 1, LOAD>(s, A);
 }
 
+// Up to 64 entries two blocks of one query tile an SM, above that one block of two tiles that share
+// the keys (one tile where there is only one). Measured, us: 64 x 8 heads x 512, dim 64: 152 and 161
+// with the other; 8 heads x 4095 causal: 78 and 89; 2 x 16 heads x 4096, dim 128: 478 and 420.
 template <int LOAD>
 int fwd_bf16(cudaStream_t s, const AttnArgs& A) {
-  if (getenv("FXV") && atoi(getenv("FXV"))==1 && A.D<=64) return fwd<bf16, 1, 1, 64, Half, 2, LOAD>(s, A);
-  if (getenv("FXV") && atoi(getenv("FXV"))==2 && A.D<=64) return fwd<bf16, 1, 1, 128, Half, 2, LOAD>(s, A);
-  if (getenv("FXV") && atoi(getenv("FXV"))==3 && A.D<=64) return fwd<bf16, 1, 1, 64, Half, 3, LOAD>(s, A);
-  if (getenv("FXV") && atoi(getenv("FXV"))==1) return fwd<bf16, 1, 1, 64, Whole, 2, LOAD>(s, A);
-  if (getenv("FXV") && atoi(getenv("FXV"))==2) return fwd<bf16, 1, 1, 128, Whole, 1, LOAD>(s, A);
-  if (A.Lq <= 128) return A.D <= 64 ? fwd<bf16, 1, 1, 64, Half, 2, LOAD>(s, A) : fwd<bf16, 1, 1, 64, Whole, 2, LOAD>(s, A);
-  return A.D <= 64 ? fwd<bf16, 1, 2, 128, Half, 2, LOAD>(s, A) : fwd<bf16, 1, 2, 128, Whole, 2, LOAD>(s, A);
+  if (A.D <= 64) return fwd<bf16, 1, 1, 128, Half, 2, LOAD>(s, A);
+  return A.Lq <= 128 ? fwd<bf16, 1, 1, 64, Whole, 2, LOAD>(s, A) : fwd<bf16, 1, 2, 128, Whole, 2, LOAD>(s, A);
 }
 
 template <typename T, int LPR, bool VEC>
