@@ -276,6 +276,9 @@ __device__ __forceinline__ void load_tile(unsigned char* dst, const T* p, int64_
 // D (+)= A B^T over the k-steps of 16 entries, both K-major tiles of RA / RB rows.
 template <int NS, int RA, int RB, typename L>
 __device__ __forceinline__ void scores(uint32_t d, uint32_t a, uint32_t b, int dim, uint32_t idesc) {
+  // One thread issues all of a block's tensor instructions, one after the other: building a
+  // descriptor for each took longer than the product, so they are stepped. Addresses are below
+  // 2^18 and stay in their field.
   const int steps = (dim + 15) / 16;
   constexpr int K = L::RB / 32;  // steps of a chunk
   bool acc = false;
@@ -284,11 +287,18 @@ __device__ __forceinline__ void scores(uint32_t d, uint32_t a, uint32_t b, int d
   for (int sum = NS - 1; sum >= 0; --sum) {
 #pragma unroll
     for (int i = 0; i <= sum; ++i) {
-      const uint32_t ap = a + i * (RA * L::RB * L::DC), bp = b + (sum - i) * (RB * L::RB * L::DC);
-      for (int k = 0; k < steps; ++k) {
-        mma_ss(d, desc<L::RB>(ap + (k / K) * (RA * L::RB) + (k % K) * 32u, 16),
-               desc<L::RB>(bp + (k / K) * (RB * L::RB) + (k % K) * 32u, 16), idesc, acc);
+      uint64_t da = desc<L::RB>(a + i * (RA * L::RB * L::DC), 16);
+      uint64_t db = desc<L::RB>(b + (sum - i) * (RB * L::RB * L::DC), 16);
+#pragma unroll 1
+      for (int k = 1; k <= steps; ++k) {
+        mma_ss(d, da, db, idesc, acc);
         acc = true;
+        da += 2;
+        db += 2;
+        if (L::DC > 1 && k % K == 0) {  // the next chunk
+          da += (RA * L::RB >> 4) - 2 * K;
+          db += (RB * L::RB >> 4) - 2 * K;
+        }
       }
     }
   }
