@@ -300,7 +300,7 @@ def position_bias(table, q_pos, k_pos=None, *, max_distance=128, bidirectional=T
     below half of its buckets, and the rest evenly spaced in the logarithm up to ``max_distance``
     (<= 2048; all longer distances share the last one); ``bidirectional`` gives half of the table to
     each sign, otherwise keys after the query share bucket 0. ``q_pos`` and ``k_pos`` (default:
-    q_pos) are integer tensors within +-2**30, in any order. Differentiable in ``table``."""
+    q_pos) are integer tensors within +-2**29, in any order. Differentiable in ``table``."""
     table = _tensor(table, "table")
     if table.dim() != 2:
         raise ValueError(f"table must have shape (heads, num_buckets), got {tuple(table.shape)}")
@@ -398,7 +398,7 @@ def biased_attention(q, k, v, table=None, *, q_pos=None, k_pos=None, key_mask=No
     (heads, num_buckets), of the same dtype, ``max_distance`` and ``bidirectional`` are those of
     :func:`position_bias`; None: no bias. ``k_pos`` defaults to 0, 1, ..., and ``q_pos`` to the last
     q_len of them (a new token attends from the end of the cache); integer tensors (length,) or
-    (batch, length), within +-2**30. ``key_mask`` (batch, k_len) bool: False leaves a key out,
+    (batch, length), within +-2**29. ``key_mask`` (batch, k_len) bool: False leaves a key out,
     whatever its k and v hold. ``causal`` leaves out keys with k_pos > q_pos. A query without any
     key gives 0 and has no gradient. ``scale`` defaults to dim ** -0.5.
 

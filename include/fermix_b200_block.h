@@ -58,7 +58,7 @@ size_t fermix_residual_norm_grad_workspace_bytes(const fx_norm_args* args);
  * With d = k_pos - q_pos: two-sided, bucket = #(edges <= |d|), plus num_buckets / 2 where
  * d > 0; one-sided, bucket = #(edges <= max(-d, 0)). edges is a HOST array, ascending,
  * edges[0] >= 1, num_edges < num_buckets (two-sided: < num_buckets / 2), and
- * edges[num_edges - 1] <= FX_BUCKET_MAX_EDGE. Positions are within +-2^30. */
+ * edges[num_edges - 1] <= FX_BUCKET_MAX_EDGE. Positions are within +-2^29. */
 #define FX_BUCKET_MAX 256
 #define FX_BUCKET_MAX_EDGE 2048
 
