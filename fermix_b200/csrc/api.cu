@@ -599,7 +599,7 @@ const char* fermix_strerror(int code) {
     case FX_ERR_DTYPE:
       return "unsupported dtype (float32, float64, complex64 and complex128 are supported)";
     case FX_ERR_SHAPE:
-      return "bad shape: batch and n must be >= 0 and n <= 46000";
+      return "bad shape: batch and n must be >= 0 and n <= 46000 (attention-block operators: the limits of fermix_b200_block.h)";
     case FX_ERR_PREC:
       return "prec must be 'tf32x3' or 'ieee'; 'tf32x3' applies to float32 / complex64 only";
     case FX_ERR_WORKSPACE:

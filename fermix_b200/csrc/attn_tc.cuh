@@ -183,6 +183,15 @@ __device__ __forceinline__ void wait(uint64_t* m, uint32_t parity, volatile int*
 __device__ __forceinline__ void named_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
+// After a wait that ran out no more copies are asked for, and those of the last ST of n tiles (and
+// the tensor instructions) are waited for, with a bound of their own, so that nothing is under way
+// when the block ends.
+constexpr uint32_t kDrainPolls = 1u << 20;
+template <int ST>
+__device__ __forceinline__ void drain(uint64_t (&bar)[ST], int64_t n) {
+  for (int64_t j = n > ST ? n - ST : 0; j < n; ++j) mbar_wait(&bar[j % ST], (uint32_t)(j / ST) & 1u, kDrainPolls);
+}
+
 // How a tile is brought in: by the threads, entry by entry or in 16-byte pieces, or by a tensor map.
 enum { LOAD_ENTRIES, LOAD_PIECES, LOAD_TMA };
 
@@ -710,10 +719,10 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
       A.lse[((int64_t)b * A.H + h) * A.Lq + i] = broken ? NAN : l == 0.f ? -INFINITY : m + log2f(l);
   } else if (warp == 8 * QT) {
     // -------------------------------------------------------- tensor instructions
+    if constexpr (TMA) wait(&qraw, 0, &abort_flag, polls);  // also where there are no keys: nothing is left under way
     if (lane == 0 && tiles > 0) {
       const uint32_t id_s = idesc_bf16(128, BN, false), id_o = idesc_bf16(128, (A.D + 15) / 16 * 16, true);
       const uint32_t aQ = smem_u32(sQ), aK = smem_u32(sK), aV = smem_u32(sV);
-      if constexpr (TMA) wait(&qraw, 0, &abort_flag, polls);
       wait(&kfull[0], 0, &abort_flag, polls);
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
@@ -750,7 +759,7 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
       }
       if (abort_flag) {  // nothing may be in flight when the TMEM is freed
         mma_commit(&done);
-        mbar_wait(&done, 0, polls);
+        mbar_wait(&done, 0, kDrainPolls);
       }
     }
   } else {
@@ -764,9 +773,12 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
     };
     if constexpr (TMA) {
       if (w == 0) {
+        int keys_asked = 0, values_asked = 0;
         for (int j = 0; j < tiles; ++j) {
           const int st = j % ST;
           if (j >= ST) wait(&kempty[st], (j / ST - 1) & 1, &abort_flag, polls);
+          if (__any_sync(0xffffffffu, abort_flag)) break;
+          ++keys_asked;
           if (lane == 0) {
             mbar_arrive_expect_tx(&kraw[st], S::kKV);
             tma_tile<L>(sK + st * S::kKV, M, MAP_K, BN, (int64_t)j * BN, hk, b, &kraw[st]);
@@ -775,10 +787,17 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
           __syncwarp();
           if (lane == 0) arrive(&kraw[st]);
           if (j >= ST) wait(&vempty[st], (j / ST - 1) & 1, &abort_flag, polls);
+          if (__any_sync(0xffffffffu, abort_flag)) break;
+          ++values_asked;
           if (lane == 0) {
             mbar_arrive_expect_tx(&vraw[st], S::kKV);
             tma_tile<L>(sV + st * S::kKV, M, MAP_V, BN, (int64_t)j * BN, hk, b, &vraw[st]);
           }
+        }
+        if (abort_flag) {
+          mbar_wait(&qraw, 0, kDrainPolls);
+          drain(kraw, keys_asked);
+          drain(vraw, values_asked);
         }
       } else {
         for (int j = 0; j < tiles; ++j) {

@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
       mma_commit(&sfull);
       if (abort_flag) {  // nothing may be in flight when the TMEM is freed
         mma_commit(&done);
-        mbar_wait(&done, 0, polls);
+        mbar_wait(&done, 0, kDrainPolls);
       }
     }
   } else {
@@ -333,10 +333,13 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
     };
     if constexpr (TMA) {
       if (w == 0) {
+        int64_t asked = 0;
         for (int64_t it = 0; it < tiles; ++it) {
           const int st = (int)(it % ST), h = (int)(hk * G + it / per);
           const int64_t i0 = (q0 + it % per) * kGradN;
           if (it >= ST) wait(&empty[st], (it / ST - 1) & 1, &abort_flag, polls);
+          if (__any_sync(0xffffffffu, abort_flag)) break;
+          ++asked;
           if (lane == 0) {
             mbar_arrive_expect_tx(&loaded[st], 2 * S::kTile);
             tma_tile<L>(sQ + st * S::kTile, M, MAP_Q, kGradN, i0, h, b, &loaded[st]);
@@ -345,6 +348,10 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
           for (int sub = 0; sub < kGradN / kSub; ++sub) fill(it, sub);
           __syncwarp();
           if (lane == 0) arrive(&loaded[st]);
+        }
+        if (abort_flag) {
+          mbar_wait(&own, 0, kDrainPolls);
+          drain(loaded, asked);
         }
       } else {
         for (int64_t it = 0; it < tiles; ++it) {
@@ -721,7 +728,7 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
       mma_commit(&sfull);
       if (abort_flag) {  // nothing may be in flight when the TMEM is freed
         mma_commit(&done);
-        mbar_wait(&done, 0, polls);
+        mbar_wait(&done, 0, kDrainPolls);
       }
     }
   } else {
@@ -734,9 +741,12 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
     };
     if constexpr (TMA) {
       if (w == 0) {
+        int64_t asked = 0;
         for (int j = 0; j < tiles; ++j) {
           const int st = j % ST;
           if (j >= ST) wait(&empty[st], (j / ST - 1) & 1, &abort_flag, polls);
+          if (__any_sync(0xffffffffu, abort_flag)) break;
+          ++asked;
           if (lane == 0) {
             mbar_arrive_expect_tx(&loaded[st], 2 * S::kTile);
             tma_tile<L>(sK + st * S::kTile, M, MAP_K, kGradN, (int64_t)j * kGradN, hk, b, &loaded[st]);
@@ -745,6 +755,10 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
           for (int sub = 0; sub < kGradN / kSub; ++sub) fill(j, sub);
           __syncwarp();
           if (lane == 0) arrive(&loaded[st]);
+        }
+        if (abort_flag) {
+          mbar_wait(&own, 0, kDrainPolls);
+          drain(loaded, asked);
         }
       } else {
         for (int j = 0; j < tiles; ++j) {
