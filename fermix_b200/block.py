@@ -326,7 +326,7 @@ def _strides(t):
     return t.stride()[:3]
 
 
-def _attn_args(q, k, v, table, q_pos, k_pos, key_mask, out, lse, causal, scale, max_distance, bidirectional):
+def _attn_args(q, k, v, table, out, lse, q_pos, k_pos, key_mask, causal, scale, max_distance, bidirectional):
     a = _lib.AttnArgs()
     a.dtype, a.causal = _KIND[q.dtype], int(causal)
     a.batch, a.heads, a.q_len, a.dim = q.shape
@@ -347,39 +347,48 @@ def _attn_args(q, k, v, table, q_pos, k_pos, key_mask, out, lse, causal, scale, 
     return a
 
 
-def _attn_forward(q, k, v, table, q_pos, k_pos, key_mask, with_lse, causal, scale, max_distance, bidirectional):
+def _attn_forward(q, k, v, table, rest, with_lse):
+    """(out, lse or None, the call's arguments)."""
     out = torch.empty_like(q)
     if out.stride(-1) != 1:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if with_lse else None
-    a = _attn_args(q, k, v, table, q_pos, k_pos, key_mask, out, lse, causal, scale, max_distance, bidirectional)
+    a = _attn_args(q, k, v, table, out, lse, *rest)
     L = _lib.lib()
     _call_with_workspace(L.fermix_biased_attention, L.fermix_biased_attention_workspace_bytes, q.device, a)
-    return out, lse
+    return out, lse, a
 
 
 class _BiasedAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, q_pos, k_pos, key_mask, *rest):
-        out, lse = _attn_forward(q, k, v, table, q_pos, k_pos, key_mask, True, *rest)
-        ctx.save_for_backward(q, k, v, table, q_pos, k_pos, key_mask, out, lse)
-        ctx.rest = rest
+    def forward(ctx, q, k, v, table, rest):
+        out, lse, ctx.args = _attn_forward(q, k, v, table, rest, True)
+        # the arguments hold addresses: everything they point to is saved
+        ctx.save_for_backward(q, k, v, table, out, lse, *rest[:3])
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, q_pos, k_pos, key_mask, out, lse = ctx.saved_tensors
+        q, k, v, table, out, lse, q_pos, k_pos, key_mask = ctx.saved_tensors
+        a = _lib.AttnArgs.from_buffer_copy(ctx.args)  # the graph may be run again, from another thread too
+        # a saved tensor may have been put elsewhere and back (saved-tensor hooks)
+        a.q, a.k, a.v, a.table, a.out, a.lse = (q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(table), out.data_ptr(),
+                                                lse.data_ptr())
+        a.q_stride[:], a.k_stride[:], a.v_stride[:], a.out_stride[:] = (_strides(q), _strides(k), _strides(v),
+                                                                        _strides(out))
+        a.buckets.q_pos, a.buckets.k_pos, a.key_mask = _ptr(q_pos), _ptr(k_pos), _ptr(key_mask)
+        a.buckets.q_pos_stride, a.buckets.k_pos_stride = _batch_stride(q_pos), _batch_stride(k_pos)
+        a.mask_stride = 0 if key_mask is None else key_mask.stride(0)
         dout = _rows(dout)
-        a = _attn_args(q, k, v, table, q_pos, k_pos, key_mask, out, lse, *ctx.rest)
-        dq, dk, dv = (_rows(torch.empty_like(t)) for t in (q, k, v))
+        dq, dk, dv = _rows(torch.empty_like(q)), _rows(torch.empty_like(k)), _rows(torch.empty_like(v))
         dtable = None if table is None else torch.empty_like(table)
-        a.dout, a.dq, a.dk, a.dv, a.dtable = _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dtable)
+        a.dout, a.dq, a.dk, a.dv, a.dtable = dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dtable)
         a.dout_stride[:], a.dq_stride[:] = _strides(dout), _strides(dq)
         a.dk_stride[:], a.dv_stride[:] = _strides(dk), _strides(dv)
         L = _lib.lib()
         _call_with_workspace(L.fermix_biased_attention_grad, L.fermix_biased_attention_grad_workspace_bytes, q.device, a)
-        return (dq, dk, dv, dtable) + (None,) * 8
+        return dq, dk, dv, dtable, None
 
 
 def _rows(t):
@@ -433,8 +442,9 @@ def biased_attention(q, k, v, table=None, *, q_pos=None, k_pos=None, key_mask=No
                              f"{tuple(key_mask.shape)} on {key_mask.device}")
         if k_len > 1 and key_mask.stride(1) != 1:
             key_mask = key_mask.contiguous()
-    rest = (bool(causal), float(dim**-0.5 if scale is None else scale), max_distance, bool(bidirectional))
+    rest = (q_pos, k_pos, key_mask, bool(causal), float(dim**-0.5 if scale is None else scale), max_distance,
+            bool(bidirectional))
     q, k, v = _rows(q), _rows(k), _rows(v)
     if _wants_grad(q, k, v, table):
-        return _BiasedAttention.apply(q, k, v, table, q_pos, k_pos, key_mask, *rest)
-    return _attn_forward(q, k, v, table, q_pos, k_pos, key_mask, False, *rest)[0]
+        return _BiasedAttention.apply(q, k, v, table, rest)
+    return _attn_forward(q, k, v, table, rest, False)[0]
