@@ -58,8 +58,11 @@ __global__ void __launch_bounds__(kDecodeThreads, DB == 1 ? 2 : 1) attn_decode_k
   extern __shared__ uint4 ring_mem[];  // the ring (after the keys, the warps' joins), the table by distance
   float* sm = reinterpret_cast<float*>(ring_mem + S * P * kDecodeThreads);
   const int G = A.H / A.Hk, reach = A.buckets.reach, span = A.table ? 2 * reach + 1 : 0;
-  const int rows = G * (int)A.Lq;
-  const int part = blockIdx.x % A.splits, z = blockIdx.x / A.splits, b = z / A.Hk, hk = z % A.Hk;
+  // this block's rows [row0, row0 + rows) of the key head's G Lq, of the query heads h0 and following
+  const int all = G * (int)A.Lq, chunks = (all + kDecodeRows - 1) / kDecodeRows;
+  const int part = blockIdx.x % A.splits, cz = blockIdx.x / A.splits, z = cz / chunks, b = z / A.Hk, hk = z % A.Hk;
+  const int row0 = cz % chunks * kDecodeRows, rows = all - row0 < kDecodeRows ? all - row0 : kDecodeRows;
+  const int h0 = row0 / (int)A.Lq, heads = (row0 + rows - 1) / (int)A.Lq - h0 + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int64_t j0 = part * (kDecodeWarps * 16), kStep = (int64_t)A.splits * (kDecodeWarps * 16);
   const int64_t count = A.Lk - j0;
@@ -115,8 +118,8 @@ __global__ void __launch_bounds__(kDecodeThreads, DB == 1 ? 2 : 1) attn_decode_k
 #pragma unroll
   for (int n = 0; n < S - 1; ++n) fetch(n, n);
   if (A.table) {
-    const bf16* table = static_cast<const bf16*>(A.table) + (int64_t)hk * G * A.buckets.num_buckets;
-    for (int i = threadIdx.x; i < G * span; i += kDecodeThreads)
+    const bf16* table = static_cast<const bf16*>(A.table) + ((int64_t)hk * G + h0) * A.buckets.num_buckets;
+    for (int i = threadIdx.x; i < heads * span; i += kDecodeThreads)
       sm[i] = bias2(to_f(table[i / span * A.buckets.num_buckets + bucket_of(A.buckets, i % span - reach)]));
   }
   // this lane's two rows, g and g + 8
@@ -127,9 +130,9 @@ __global__ void __launch_bounds__(kDecodeThreads, DB == 1 ? 2 : 1) attn_decode_k
   for (int r = 0; r < 2; ++r) {
     const int row = g + 8 * r;
     row_ok[r] = row < rows;
-    const int h = row_ok[r] ? row / (int)A.Lq : 0, i = row_ok[r] ? row % (int)A.Lq : 0;
+    const int h = row_ok[r] ? (row0 + row) / (int)A.Lq : h0, i = row_ok[r] ? (row0 + row) % (int)A.Lq : 0;
     qp[r] = attn_q_pos(A, b, i);
-    lut[r] = h * span;
+    lut[r] = (h - h0) * span;
     const bf16* p = static_cast<const bf16*>(A.q) + b * A.qs[0] + (hk * G + h) * A.qs[1] + i * A.qs[2];
 #pragma unroll
     for (int c = 0; c < 2 * DB; ++c) {
@@ -286,15 +289,15 @@ __global__ void __launch_bounds__(kDecodeThreads, DB == 1 ? 2 : 1) attn_decode_k
       acc = fmaf(wo[(w * rows + row) * W + c], f, acc);
     }
     if (A.splits > 1) {
-      float* p = A.part + (((int64_t)z * rows + row) * A.splits + part) * (A.D + 2);
+      float* p = A.part + (((int64_t)z * all + row0 + row) * A.splits + part) * (A.D + 2);
       p[2 + c] = acc;
       if (c == 0) {
         p[0] = top;
         p[1] = sum;
       }
     } else {
-      const int h = hk * G + row / (int)A.Lq;
-      const int64_t q_i = row % (int)A.Lq;
+      const int h = hk * G + (row0 + row) / (int)A.Lq;
+      const int64_t q_i = (row0 + row) % (int)A.Lq;
       static_cast<bf16*>(A.out)[b * A.os[0] + h * A.os[1] + q_i * A.os[2] + c] =
           from_f<bf16>(sum == 0.f ? 0.f : acc / sum);
       if (A.lse && c == 0) A.lse[((int64_t)b * A.H + h) * A.Lq + q_i] = sum == 0.f ? -INFINITY : top + log2f(sum);

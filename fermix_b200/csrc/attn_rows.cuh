@@ -253,4 +253,44 @@ __global__ void __launch_bounds__(kRowsThreads) attn_join_kernel(const __grid_co
   if (A.lse && threadIdx.x == 0) A.lse[((int64_t)b * A.H + h) * A.Lq + i] = sum == 0.f ? -INFINITY : top + log2f(sum);
 }
 
+// The same with a warp a row, for many rows of few parts. A lane weighs a part, 32 at a time, and adds
+// up to four entries of the row.
+template <typename T>
+__global__ void __launch_bounds__(kRowsThreads) attn_join_warp_kernel(const __grid_constant__ AttnArgs A) {
+  constexpr int NE = FX_ATTN_MAX_DIM / 32;
+  const int lane = threadIdx.x & 31, step = A.D + 2;
+  const int64_t w = (int64_t)blockIdx.x * (kRowsThreads / 32) + (threadIdx.x >> 5);
+  if (w >= (int64_t)A.B * A.H * A.Lq) return;
+  const int64_t i = w % A.Lq, bh = w / A.Lq, h = bh % A.H, b = bh / A.H;
+  const float* p = A.part + w * A.splits * step;
+  float top = -INFINITY;
+  for (int s = lane; s < A.splits; s += 32) top = fmaxf(top, p[(int64_t)s * step]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float ref = top == -INFINITY ? 0.f : top;
+  float sum = 0.f, acc[NE] = {};
+  for (int s0 = 0; s0 < A.splits; s0 += 32) {
+    const float* q = p + (int64_t)s0 * step;
+    const int n = A.splits - s0 < 32 ? A.splits - s0 : 32;
+    float f = 0.f;
+    if (lane < n) {
+      f = exp2f(q[lane * step] - ref);
+      sum = fmaf(q[lane * step + 1], f, sum);
+    }
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+      const float weight = __shfl_sync(0xffffffffu, f, s);
+#pragma unroll
+      for (int e = 0; e < NE; ++e)
+        if (lane + 32 * e < A.D) acc[e] = fmaf(q[s * step + 2 + lane + 32 * e], weight, acc[e]);
+    }
+  }
+  sum = lanes_sum(sum, 32);
+  T* out = static_cast<T*>(A.out) + b * A.os[0] + h * A.os[1] + i * A.os[2];
+#pragma unroll
+  for (int e = 0; e < NE; ++e)
+    if (lane + 32 * e < A.D) out[lane + 32 * e] = from_f<T>(sum == 0.f ? 0.f : acc[e] / sum);
+  if (A.lse && lane == 0) A.lse[w] = sum == 0.f ? -INFINITY : top + log2f(sum);
+}
+
 }  // namespace fx

@@ -509,11 +509,13 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
   __shared__ float shared_row[QT][2][128];  // what the two threads of a row tell each other
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  // block -> (batch, head, query block); under a causal order the longest blocks first
+  // block -> (batch, head, query block, part of the keys); under a causal order the longest blocks first
   const int64_t nq = (A.Lq + 128 * QT - 1) / (128 * QT), heads = (int64_t)A.B * A.H;
   const bool ordered = A.causal && !A.q_pos && !A.k_pos;
-  const int64_t qb = ordered ? nq - 1 - blockIdx.x / heads : blockIdx.x % nq;
-  const int64_t bh = ordered ? blockIdx.x % heads : blockIdx.x / nq;
+  const int part = blockIdx.x % A.splits;
+  const int64_t block = blockIdx.x / A.splits;
+  const int64_t qb = ordered ? nq - 1 - block / heads : block % nq;
+  const int64_t bh = ordered ? block % heads : block / nq;
   const int h = (int)(bh % A.H), b = (int)(bh / A.H), hk = h / (A.H / A.Hk);
   const int64_t i0 = qb * 128 * QT;
   const uint8_t* mask = A.mask ? A.mask + b * A.mask_stride : nullptr;
@@ -577,7 +579,9 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
     const int64_t seen = A.Lk - A.Lq + end;
     keys = seen < keys ? (seen > 0 ? seen : 0) : keys;
   }
-  const int tiles = (int)((keys + BN - 1) / BN);
+  // this part's tiles [first, first + tiles), numbered from 0 below
+  const int all = (int)((keys + BN - 1) / BN), per = (all + A.splits - 1) / A.splits;
+  const int first = part * per < all ? part * per : all, tiles = all - first < per ? all - first : per;
   const uint32_t tmem = tmem_slot;
   const uint32_t polls = A.polls;
 
@@ -686,6 +690,24 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
       fence_after_sync();
     }
     const bool broken = abort_flag != 0;
+    if (A.splits > 1) {  // (m, l, o) of this part for attn_join_kernel
+      float* p = A.part + ((((int64_t)b * A.H + h) * A.Lq + i) * A.splits + part) * (A.D + 2);
+#pragma unroll 1
+      for (int c = half * 8; c < A.D; c += 16) {
+        uint32_t o[8];
+        if (tiles > 0) {
+          tmem_ld8(base + S::kO + c, o);
+          tmem_wait_ld();
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (valid && c + e < A.D) p[2 + c + e] = l == 0.f ? 0.f : __uint_as_float(o[e]);
+      }
+      if (valid && half == 0) {
+        p[0] = m;
+        p[1] = broken ? NAN : l;
+      }
+    } else {
     const float inv = broken ? NAN : l == 0.f ? 0.f : 1.f / l;
     T* out = static_cast<T*>(A.out) + b * A.os[0] + h * A.os[1] + i * A.os[2];
     constexpr int V = 16 / sizeof(T);
@@ -717,6 +739,7 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
     }
     if (valid && half == 0 && A.lse)
       A.lse[((int64_t)b * A.H + h) * A.Lq + i] = broken ? NAN : l == 0.f ? -INFINITY : m + log2f(l);
+    }
   } else if (warp == 8 * QT) {
     // -------------------------------------------------------- tensor instructions
     if constexpr (TMA) wait(&qraw, 0, &abort_flag, polls);  // also where there are no keys: nothing is left under way
@@ -766,7 +789,7 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
     // -------------------------------------------------------- loads
     const int t = tid - 256 * QT - 32, w = t >> 5;
     const auto fill = [&](int j, int sub) {
-      const int64_t j0 = (int64_t)j * BN;
+      const int64_t j0 = (int64_t)(first + j) * BN;
       fill_info<BN>(
           info[j % S::kInfo], sub, [&](int e) { return j0 + e < A.Lk && (!mask || mask[j0 + e]); },
           [&](int e) { return attn_k_pos(A, b, j0 + e); });
@@ -781,7 +804,7 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
           ++keys_asked;
           if (lane == 0) {
             mbar_arrive_expect_tx(&kraw[st], S::kKV);
-            tma_tile<L>(sK + st * S::kKV, M, MAP_K, BN, (int64_t)j * BN, hk, b, &kraw[st]);
+            tma_tile<L>(sK + st * S::kKV, M, MAP_K, BN, (int64_t)(first + j) * BN, hk, b, &kraw[st]);
           }
           for (int sub = 0; sub < BN / kSub; ++sub) fill(j, sub);
           __syncwarp();
@@ -791,7 +814,7 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
           ++values_asked;
           if (lane == 0) {
             mbar_arrive_expect_tx(&vraw[st], S::kKV);
-            tma_tile<L>(sV + st * S::kKV, M, MAP_V, BN, (int64_t)j * BN, hk, b, &vraw[st]);
+            tma_tile<L>(sV + st * S::kKV, M, MAP_V, BN, (int64_t)(first + j) * BN, hk, b, &vraw[st]);
           }
         }
         if (abort_flag) {
@@ -821,7 +844,7 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
       const T* V = static_cast<const T*>(A.v) + b * A.vs[0] + hk * A.vs[1];
       for (int j = 0; j < tiles; ++j) {
         const int st = j % ST;
-        const int64_t j0 = (int64_t)j * BN;
+        const int64_t j0 = (int64_t)(first + j) * BN;
         TileInfo<BN>& I = info[j % S::kInfo];
         if (j >= ST) wait(&kempty[st], (j / ST - 1) & 1, &abort_flag, polls);
         for (int sub = w; sub < BN / kSub; sub += 3) fill(j, sub);

@@ -63,6 +63,7 @@ AttnArgs make(const fx_attn_args* a) {
   A.causal = a->causal != 0;
   A.scale = a->scale;
   A.scale2 = a->scale * kLog2e;
+  A.splits = 1;
   A.polls = wait_polls();
   if (a->table) A.buckets = make_buckets(a->buckets);
   return A;
@@ -88,33 +89,48 @@ bool aligned(const fx_attn_args* a, bool grad) {
   return m % 16 == 0;
 }
 
-// Rows of a key head (query heads that share it x queries) from which the tensor-core kernel
-// runs; below, the rows kernel splits the keys.
-constexpr int64_t kTcRows = 17;
-
-bool use_tc(const fx_attn_args* a) { return a->heads / a->kv_heads * a->q_len >= kTcRows; }
-
 // Lanes of a key: 16 bytes each, a power of two, eight at least.
 int lanes_of(const fx_attn_args* a) {
   const int need = (int)((a->dim * (a->dtype == FX_F32 ? 4 : 2) + 15) / 16);
   return need <= 8 ? 8 : need <= 16 ? 16 : 32;
 }
 
-// Whether the fragment kernel of a bfloat16 cache runs (attn_decode.cuh); float32 and tables whose
-// distances take more than 16 KB (32 KB above 64 entries) for a key head's query heads, beside two
-// (one) rings of 96 KB (192 KB) an SM, take the rows kernel.
-bool use_decode(const fx_attn_args* a) {
-  if (a->dtype != FX_BF16 || use_tc(a)) return false;
-  return !a->table || a->heads / a->kv_heads * (2 * make_buckets(a->buckets).reach + 1) <= (a->dim <= 64 ? 4096 : 8192);
+// Query heads whose distances a block of the fragment kernel holds: its rows are of that many at most.
+int decode_heads(int64_t shared) { return (int)(shared < kDecodeRows ? shared : kDecodeRows); }
+int64_t decode_chunks(const fx_attn_args* a) {
+  return (a->heads / a->kv_heads * a->q_len + kDecodeRows - 1) / kDecodeRows;
+}
+
+// Which kernel, by the queries of a head: few of them leave the tensor-core kernel's tile of 128 rows
+// empty, and the heads that share keys each read them again. Measured for 1, 2, 4, 8, 16, 32 queries
+// of 8 x 8 heads on 2 key heads of 4096 keys, us: bfloat16 dim 64 21, 24, 26, 28, 42, 60 by fragments
+// and 40 to 44 by tiles; dim 128 28, 28, 32, 46, 62, 93 and 48 to 54; float32 dim 32 30, 42, 60, 99, 165
+// by rows and 79 to 81 by tiles; dim 64 40, 62, 93, 175 and 136; dim 128 62, 101, 167, 332, 646 and
+// 369. The same places for 64 batches of 128 and 512 keys. The table by distance has to fit beside
+// two (one above 64 entries) of the fragment kernel's rings of 96 KB (192 KB) an SM: 16 (32) KB.
+// Where it does not, tiles are no slower than bfloat16 rows were, from one query on (48 us by rows).
+enum Kind { ROWS, DECODE, TC };
+
+Kind kind_of(const fx_attn_args* a) {
+  const bool wide = a->dim > 64;
+  if (a->dtype == FX_F32) return a->q_len <= (wide ? 8 : 4) ? ROWS : TC;
+  const bool fits = !a->table || decode_heads(a->heads / a->kv_heads) * (2 * make_buckets(a->buckets).reach + 1) <=
+                                     (wide ? 8192 : 4096);
+  return fits && a->q_len <= (wide ? 8 : 16) ? DECODE : TC;
 }
 
 // Parts of the keys. Rows kernel: eight blocks an SM, parts of 128 keys at least. Fragment kernel:
 // two rounds of the two blocks an SM holds (one above 64 entries), 512 keys a part at least; more
 // and shorter parts spend more time on a block's start (measured for 64 key heads of 65536 keys:
 // 37 parts 205 us, 9 parts 186 us).
-void split_keys(const fx_attn_args* a, int sms, AttnArgs& A) {
-  if (use_decode(a)) {
-    const int64_t blocks = a->batch * a->kv_heads, want = (int64_t{a->dim <= 64 ? 4 : 2} * sms) / blocks;
+void split_keys(const fx_attn_args* a, Kind kind, int sms, AttnArgs& A) {
+  if (kind == TC) {
+    A.splits = attn_tc_splits(A, a->dtype == FX_F32, sms);
+    return;
+  }
+  if (kind == DECODE) {
+    const int64_t blocks = decode_chunks(a) * a->batch * a->kv_heads;
+    const int64_t want = (int64_t{a->dim <= 64 ? 4 : 2} * sms) / blocks;
     const int64_t most = (a->k_len + 511) / 512, splits = want < most ? want : most;
     A.splits = splits < 1 ? 1 : (int)splits;
     return;
@@ -134,42 +150,50 @@ size_t part_bytes(const fx_attn_args* a, const AttnArgs& A) {
   return A.splits > 1 ? (size_t)(a->batch * a->heads * a->q_len) * A.splits * (a->dim + 2) * sizeof(float) + 256 : 0;
 }
 
-template <typename T, int LPK, bool VL>
+// A block a row joins the most parts at a time (256 rows of 9 parts: 5 us, 7 with a warp a row; 8 rows
+// of 128: 15 us less than with a warp); from 1024 rows on a warp each (8192 rows of 2 parts: 6 and 12 us).
+template <typename T>
+int join_parts(cudaStream_t s, const AttnArgs& A) {
+  const int64_t rows = (int64_t)A.B * A.H * A.Lq;
+  if (rows > kMaxGrid) return FX_ERR_SHAPE;
+  if (rows >= 1024)
+    attn_join_warp_kernel<T><<<(unsigned)((rows + kRowsThreads / 32 - 1) / (kRowsThreads / 32)), kRowsThreads, 0, s>>>(A);
+  else
+    attn_join_kernel<T><<<(unsigned)rows, kRowsThreads, 0, s>>>(A);
+  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+}
+
+template <int LPK, bool VL>
 int launch_fwd(cudaStream_t s, const AttnArgs& A) {
-  constexpr int NE = 16 / sizeof(T), GROUPS = kRowsThreads / LPK;
+  constexpr int NE = 4, GROUPS = kRowsThreads / LPK;
   const size_t lut = A.table ? (size_t)kRC * (2 * A.buckets.reach + 1) * 4 : 0;
   const size_t join = (size_t)GROUPS * kRC * (2 + LPK * NE) * 4;
   const size_t smem = lut > join ? lut : join;
-  auto kern = attn_rows_kernel<T, LPK, VL, kRC>;
+  auto kern = attn_rows_kernel<float, LPK, VL, kRC>;
   if (raise_smem(kern, smem)) return FX_ERR_CUDA;
   const int64_t rows = (int64_t)(A.H / A.Hk) * A.Lq;
   const int64_t blocks = (rows + kRC - 1) / kRC * A.B * A.Hk * A.splits;
   if (blocks > kMaxGrid) return FX_ERR_SHAPE;
   kern<<<(unsigned)blocks, kRowsThreads, smem, s>>>(A);
   if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
-  if (A.splits > 1) {
-    attn_join_kernel<T><<<(unsigned)((int64_t)A.B * A.H * A.Lq), kRowsThreads, 0, s>>>(A);
-    if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
-  }
-  return FX_OK;
+  return A.splits > 1 ? join_parts<float>(s, A) : FX_OK;
 }
 
 template <int DB, bool VEC>
 int launch_decode(cudaStream_t s, const AttnArgs& A) {
-  const size_t lut = A.table ? (size_t)(A.H / A.Hk) * (2 * A.buckets.reach + 1) * 4 : 0;
+  const size_t lut = A.table ? (size_t)decode_heads(A.H / A.Hk) * (2 * A.buckets.reach + 1) * 4 : 0;
   const size_t ring = (size_t)kDecodeStages * 8 * DB * kDecodeThreads * 16;
   static_assert(kDecodeWarps * (2 * kDecodeRows + kDecodeRows * (64 * DB + 1)) * 4 <=
                 kDecodeStages * 8 * DB * kDecodeThreads * 16);
   const size_t smem = ring + lut;
   auto kern = attn_decode_kernel<DB, VEC>;
   if (raise_smem(kern, smem)) return FX_ERR_CUDA;
-  const int64_t blocks = (int64_t)A.B * A.Hk * A.splits;
+  const int64_t chunks = ((int64_t)(A.H / A.Hk) * A.Lq + kDecodeRows - 1) / kDecodeRows;
+  const int64_t blocks = (int64_t)A.B * A.Hk * chunks * A.splits;
   if (blocks > kMaxGrid) return FX_ERR_SHAPE;
   kern<<<(unsigned)blocks, kDecodeThreads, smem, s>>>(A);
   if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
-  if (A.splits > 1)
-    attn_join_kernel<bf16><<<(unsigned)((int64_t)A.B * A.H * A.Lq), kRowsThreads, 0, s>>>(A);
-  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+  return A.splits > 1 ? join_parts<bf16>(s, A) : FX_OK;
 }
 
 template <typename T, int LPK, bool VL>
@@ -192,12 +216,10 @@ int launch_bwd(cudaStream_t s, const AttnArgs& A) {
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
-template <typename T>
 int fwd(cudaStream_t s, const AttnArgs& A, int lanes, bool vec) {
-  if (lanes == 8) return vec ? launch_fwd<T, 8, true>(s, A) : launch_fwd<T, 8, false>(s, A);
-  if (lanes == 16) return vec ? launch_fwd<T, 16, true>(s, A) : launch_fwd<T, 16, false>(s, A);
-  if constexpr (sizeof(T) == 4) return vec ? launch_fwd<T, 32, true>(s, A) : launch_fwd<T, 32, false>(s, A);
-  return FX_ERR_SHAPE;
+  if (lanes == 8) return vec ? launch_fwd<8, true>(s, A) : launch_fwd<8, false>(s, A);
+  if (lanes == 16) return vec ? launch_fwd<16, true>(s, A) : launch_fwd<16, false>(s, A);
+  return vec ? launch_fwd<32, true>(s, A) : launch_fwd<32, false>(s, A);
 }
 
 template <typename T>
@@ -234,9 +256,9 @@ extern "C" {
 
 size_t fermix_biased_attention_workspace_bytes(const fx_attn_args* a) {
   const DevInfo* D = dev_info();
-  if (check(a) || !D || no_rows(a) || use_tc(a)) return 0;
-  AttnArgs A{};
-  split_keys(a, D->sms, A);
+  if (check(a) || !D || no_rows(a)) return 0;
+  AttnArgs A = make(a);
+  split_keys(a, kind_of(a), D->sms, A);
   return part_bytes(a, A);
 }
 
@@ -250,18 +272,22 @@ int fermix_biased_attention(void* stream, const fx_attn_args* a, void* ws, size_
   AttnArgs A = make(a);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool vec = aligned(a, false);
-  if (use_tc(a)) return launch_attn_tc_fwd(s, A, a->dtype == FX_F32, vec);
-  split_keys(a, D->sms, A);
+  const Kind kind = kind_of(a);
+  split_keys(a, kind, D->sms, A);
   const size_t need = part_bytes(a, A);
   if (need) {
     if (!ws || wsb < need) return FX_ERR_WORKSPACE;
     A.part = reinterpret_cast<float*>(align256(reinterpret_cast<uintptr_t>(ws)));
   }
-  if (use_decode(a)) {
+  if (kind == TC) {
+    const int st = launch_attn_tc_fwd(s, A, a->dtype == FX_F32, vec);
+    return st || A.splits == 1 ? st : a->dtype == FX_F32 ? join_parts<float>(s, A) : join_parts<bf16>(s, A);
+  }
+  if (kind == DECODE) {
     if (a->dim <= 64) return vec ? launch_decode<1, true>(s, A) : launch_decode<1, false>(s, A);
     return vec ? launch_decode<2, true>(s, A) : launch_decode<2, false>(s, A);
   }
-  return a->dtype == FX_F32 ? fwd<float>(s, A, lanes_of(a), vec) : fwd<bf16>(s, A, lanes_of(a), vec);
+  return fwd(s, A, lanes_of(a), vec);
 }
 
 size_t fermix_biased_attention_grad_workspace_bytes(const fx_attn_args* a) {

@@ -7,6 +7,7 @@ namespace fxh {
 
 namespace {
 
+
 using tc::LOAD_ENTRIES;
 using tc::LOAD_PIECES;
 using tc::LOAD_TMA;
@@ -67,7 +68,7 @@ int fwd(cudaStream_t s, const AttnArgs& A) {
   const size_t smem = S::kTileBytes + 1024 + (A.table ? (2 * A.buckets.reach + 1) * sizeof(float) : 0);
   auto kern = tc::attn_fwd_kernel<T, NS, QT, BN, L, ST, LOAD>;
   if (raise_smem(kern, smem)) return FX_ERR_CUDA;
-  const int64_t blocks = (A.Lq + 128 * QT - 1) / (128 * QT) * A.H * A.B;
+  const int64_t blocks = (A.Lq + 128 * QT - 1) / (128 * QT) * A.H * A.B * A.splits;
   if (blocks > kMaxGrid) return FX_ERR_SHAPE;
   kern<<<(unsigned)blocks, S::kThreads, smem, s>>>(A, M);
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
@@ -176,6 +177,15 @@ int launch_attn_tc_bwd(cudaStream_t s, const AttnArgs& A, bool is_f32, bool alig
 int launch_attn_tc_fwd(cudaStream_t s, const AttnArgs& A, bool is_f32, bool aligned) {
   if (is_f32) return aligned ? fwd_f32<LOAD_PIECES>(s, A) : fwd_f32<LOAD_ENTRIES>(s, A);
   return aligned ? fwd_bf16<LOAD_TMA>(s, A) : fwd_bf16<LOAD_ENTRIES>(s, A);
+}
+
+int attn_tc_splits(const AttnArgs& A, bool is_f32, int sms) {
+  const int rows = !is_f32 && A.D > 64 && A.Lq > 128 ? 256 : 128;            // of a block
+  const int resident = (is_f32 ? A.D <= 64 : rows == 128) ? 2 : 1;           // blocks an SM holds
+  const int64_t blocks = (A.Lq + rows - 1) / rows * A.H * A.B, fill = (int64_t)sms * resident / blocks;
+  const int64_t most = is_f32 ? A.Lk / 128 : A.Lk < 2048 ? 1 : A.Lk / 512;
+  const int64_t splits = fill < most ? fill : most;
+  return splits < 1 ? 1 : (int)splits;
 }
 
 int attn_tc_status(int clear) {
