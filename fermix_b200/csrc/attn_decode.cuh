@@ -289,8 +289,8 @@ __global__ void __launch_bounds__(kDecodeThreads, DB == 1 ? 2 : 1) attn_decode_k
       acc = fmaf(wo[(w * rows + row) * W + c], f, acc);
     }
     if (A.splits > 1) {
-      float* p = A.part + (((int64_t)z * all + row0 + row) * A.splits + part) * (A.D + 2);
-      p[2 + c] = acc;
+      float* p = A.part + (((int64_t)z * all + row0 + row) * A.splits + part) * part_step(A.D);
+      p[4 + c] = acc;
       if (c == 0) {
         p[0] = top;
         p[1] = sum;

@@ -32,7 +32,7 @@ struct AttnArgs {
   float* delta;   // (batch, heads, q_len)
   float* dpart;   // partial table gradients (heads, parts, num_buckets)
   float* lut;     // table by distance, base 2 (heads, 2 reach + 1)
-  float* part;    // split parts: (rows, splits, dim + 2)
+  float* part;    // split parts: (rows, splits, part_step(dim)): m, l, -, -, o
   int64_t Lq, Lk;
   int64_t split_keys;
   int B, H, Hk, D, causal, splits;
@@ -41,6 +41,9 @@ struct AttnArgs {
   float scale;
   BucketArgs buckets;
 };
+
+// Floats of a split part, whole 16-byte pieces.
+__host__ __device__ constexpr int part_step(int dim) { return (dim + 3) / 4 * 4 + 4; }
 
 // The table's value in base 2; finite entries stay finite.
 __device__ __forceinline__ float bias2(float t) {
@@ -188,8 +191,8 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_kernel(const __grid_co
       acc = fmaf(so[(g * RC + r) * LPK * NE + c], f, acc);
     }
     if (A.splits > 1) {
-      float* p = A.part + ((z * rows + row) * A.splits + part) * (A.D + 2);
-      p[2 + c] = acc;
+      float* p = A.part + ((z * rows + row) * A.splits + part) * part_step(A.D);
+      p[4 + c] = acc;
       if (c == 0) {
         p[0] = top;
         p[1] = sum;
@@ -213,9 +216,10 @@ __global__ void __launch_bounds__(kRowsThreads) attn_join_kernel(const __grid_co
   const int64_t rows = (int64_t)G * A.Lq, w = blockIdx.x, z = w / rows, row = w % rows;
   const int b = (int)(z / A.Hk), h = (int)(z % A.Hk) * G + (int)(row / A.Lq);
   const int64_t i = row % A.Lq;
-  const float* p = A.part + w * A.splits * (A.D + 2);
+  const int step = part_step(A.D);
+  const float* p = A.part + w * A.splits * step;
   float top = -INFINITY;
-  for (int s = threadIdx.x; s < A.splits; s += kRowsThreads) top = fmaxf(top, p[(int64_t)s * (A.D + 2)]);
+  for (int s = threadIdx.x; s < A.splits; s += kRowsThreads) top = fmaxf(top, p[(int64_t)s * step]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) red[warp] = top;
@@ -228,16 +232,16 @@ __global__ void __launch_bounds__(kRowsThreads) attn_join_kernel(const __grid_co
     const int n = A.splits - s0 < kRowsThreads ? A.splits - s0 : kRowsThreads;
     __syncthreads();
     if (threadIdx.x < n) {
-      const float* q = p + (int64_t)(s0 + threadIdx.x) * (A.D + 2);
+      const float* q = p + (int64_t)(s0 + threadIdx.x) * step;
       const float f = exp2f(q[0] - ref);
       weight[threadIdx.x] = f;
       sum = fmaf(q[1], f, sum);
     }
     __syncthreads();
     if (threadIdx.x < A.D) {
-      const float* q = p + (int64_t)s0 * (A.D + 2) + 2 + threadIdx.x;
+      const float* q = p + (int64_t)s0 * step + 4 + threadIdx.x;
 #pragma unroll 8
-      for (int s = 0; s < n; ++s) acc = fmaf(q[(int64_t)s * (A.D + 2)], weight[s], acc);
+      for (int s = 0; s < n; ++s) acc = fmaf(q[(int64_t)s * step], weight[s], acc);
     }
   }
   sum = lanes_sum(sum, 32);
@@ -258,7 +262,7 @@ __global__ void __launch_bounds__(kRowsThreads) attn_join_kernel(const __grid_co
 template <typename T>
 __global__ void __launch_bounds__(kRowsThreads) attn_join_warp_kernel(const __grid_constant__ AttnArgs A) {
   constexpr int NE = FX_ATTN_MAX_DIM / 32;
-  const int lane = threadIdx.x & 31, step = A.D + 2;
+  const int lane = threadIdx.x & 31, step = part_step(A.D);
   const int64_t w = (int64_t)blockIdx.x * (kRowsThreads / 32) + (threadIdx.x >> 5);
   if (w >= (int64_t)A.B * A.H * A.Lq) return;
   const int64_t i = w % A.Lq, bh = w / A.Lq, h = bh % A.H, b = bh / A.H;
@@ -282,7 +286,7 @@ __global__ void __launch_bounds__(kRowsThreads) attn_join_warp_kernel(const __gr
       const float weight = __shfl_sync(0xffffffffu, f, s);
 #pragma unroll
       for (int e = 0; e < NE; ++e)
-        if (lane + 32 * e < A.D) acc[e] = fmaf(q[s * step + 2 + lane + 32 * e], weight, acc[e]);
+        if (lane + 32 * e < A.D) acc[e] = fmaf(q[s * step + 4 + lane + 32 * e], weight, acc[e]);
     }
   }
   sum = lanes_sum(sum, 32);

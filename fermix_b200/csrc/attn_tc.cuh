@@ -331,6 +331,37 @@ __device__ __forceinline__ void values(uint32_t d, uint32_t b, uint32_t idesc, b
   }
 }
 
+// The tensor cores cut off what they add to an accumulator below its last bit, always towards zero:
+// a float32 sum over 1165 keys (six products of 16 keys each) was off by 7e-6 of the result. So
+// float32 sums are moved on after kRest tiles of 64, added to the output in memory, which the thread
+// owns, with rounding; the accumulator starts anew.
+constexpr int kRest = 4;
+template <int NS>
+__device__ __forceinline__ bool starts(int64_t tile) {  // the tile starts a sum
+  return NS == 1 ? tile == 0 : tile % kRest == 0;
+}
+
+// Up to 8 entries of a sum (n of them are there) from the accumulator to p, added to what is there or
+// in its place.
+__device__ __forceinline__ void hold8(float* p, int n, bool vec, bool add, bool zero, const uint32_t (&o)[8]) {
+  if (vec) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+      if (e >= n) break;
+      float4 v = add ? *reinterpret_cast<const float4*>(p + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v.x += __uint_as_float(o[e]);
+      v.y += __uint_as_float(o[e + 1]);
+      v.z += __uint_as_float(o[e + 2]);
+      v.w += __uint_as_float(o[e + 3]);
+      *reinterpret_cast<float4*>(p + e) = zero ? make_float4(0.f, 0.f, 0.f, 0.f) : v;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = zero ? 0.f : (add ? p[e] : 0.f) + __uint_as_float(o[e]);
+  }
+}
+
 // Positions and liveness of up to R keys (or queries) of a tile.
 template <int R>
 struct alignas(16) TileInfo {  // positions are read four at a time
@@ -596,6 +627,12 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
                     __reduce_max_sync(0xffffffffu, valid ? qp : INT32_MIN), valid};
     const uint32_t base = F.base;
     float m = -INFINITY, l = 0.f;  // the reference (-inf before the first key), the sum of this half
+    // Where this row's sums are held (float32), entries [16 half, 16 half + 16) and every 32 on.
+    const auto held_row = [&]() -> float* {
+      if (A.splits > 1) return A.part + ((((int64_t)b * A.H + h) * A.Lq + i) * A.splits + part) * part_step(A.D) + 4;
+      return static_cast<float*>(A.out) + b * A.os[0] + h * A.os[1] + i * A.os[2];
+    };
+    const bool held = NS > 1 && tiles > kRest;
     if ((tid & 255) < 2) moving[t][tid & 255] = 0;
     named_barrier(2 + t, 256);
     for (int j = 0; j < tiles; ++j) {
@@ -605,6 +642,23 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
       uint32_t p[S::kOver ? S::kHalf / kSub : 1][NS][16];
       bool free_p = S::kOver || j == 0;
       float sum = 0.f;
+      if constexpr (NS > 1) {
+        if (j > 0 && starts<NS>(j)) {
+          wait(&ofull[t], (j - 1) & 1, &abort_flag, polls);
+          fence_after_sync();
+          free_p = true;
+          float* row = held_row();
+          const bool held_vec = A.splits > 1 || (A.D % 4 == 0 && (reinterpret_cast<uintptr_t>(row) & 15) == 0);
+          const int entries = A.splits > 1 ? (A.D + 3) / 4 * 4 : A.D;
+#pragma unroll 1
+          for (int c = half * 16; c < A.D; c += c & 8 ? 24 : 8) {
+            uint32_t o[8];
+            tmem_ld8(base + S::kO + c, o);
+            tmem_wait_ld();
+            if (valid) hold8(row + c, entries - c, held_vec, j > kRest, false, o);
+          }
+        }
+      }
       bool moved = false;
       for (;;) {
         bool low = __any_sync(0xffffffffu, valid && m == -INFINITY);
@@ -668,6 +722,13 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
             tmem_st8(base + S::kO + c, o);
           }
         }
+        if constexpr (NS > 1) {
+          if (j >= kRest && valid && f != 1.f) {
+            float* row = held_row();
+#pragma unroll 1
+            for (int c = half * 16; c < A.D; c += (c & 15) == 15 ? 17 : 1) row[c] *= f;
+          }
+        }
         moved = true;
       }
       l += sum;
@@ -691,17 +752,15 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
     }
     const bool broken = abort_flag != 0;
     if (A.splits > 1) {  // (m, l, o) of this part for attn_join_kernel
-      float* p = A.part + ((((int64_t)b * A.H + h) * A.Lq + i) * A.splits + part) * (A.D + 2);
+      float* p = A.part + ((((int64_t)b * A.H + h) * A.Lq + i) * A.splits + part) * part_step(A.D);
 #pragma unroll 1
-      for (int c = half * 8; c < A.D; c += 16) {
+      for (int c = half * 16; c < A.D; c += c & 8 ? 24 : 8) {
         uint32_t o[8];
         if (tiles > 0) {
           tmem_ld8(base + S::kO + c, o);
           tmem_wait_ld();
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (valid && c + e < A.D) p[2 + c + e] = l == 0.f ? 0.f : __uint_as_float(o[e]);
+        if (valid) hold8(p + 4 + c, (A.D + 3) / 4 * 4 - c, true, held, l == 0.f, o);
       }
       if (valid && half == 0) {
         p[0] = m;
@@ -720,6 +779,21 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
         if (tiles > 0) {
           ld16(base + S::kO + c, o);
           tmem_wait_ld();
+        }
+        if constexpr (NS > 1) {
+          if (held && valid) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              if (c + e >= A.D) break;
+              Pack<T, 4> v;
+              if (ovec) v = *reinterpret_cast<const Pack<T, 4>*>(out + c + e);
+              else
+#pragma unroll
+                for (int n = 0; n < 4; ++n) v.e[n] = c + e + n < A.D ? out[c + e + n] : 0.f;
+#pragma unroll
+              for (int n = 0; n < 4; ++n) o[e + n] = __float_as_uint(__uint_as_float(o[e + n]) + v.e[n]);
+            }
+          }
         }
         alignas(16) T r[16];
 #pragma unroll
@@ -769,7 +843,7 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
             if (t == QT - 1) mma_commit(&kempty[sn]);
           }
           if (!S::kOver && t == 0) wait(&vfull[st], (j / ST) & 1, &abort_flag, polls);
-          values<NS, BN, L>(d + S::kO, aV + st * S::kKV, id_o, j > 0,
+          values<NS, BN, L>(d + S::kO, aV + st * S::kKV, id_o, !starts<NS>(j),
                             [=](int part, int k) { return d + S::kP + part * (BN / 2) + k * 8; });
           mma_commit(&ofull[t]);
           if (t == QT - 1) mma_commit(&vempty[st]);

@@ -48,9 +48,10 @@ __global__ void __launch_bounds__(256) attn_prep_kernel(const __grid_constant__ 
   if (there && threadIdx.x % LPR == 0) A.delta[row] = s;
 }
 
-// Row r of the block from TMEM (columns col ..), times f, to p (zero: 0).
+// Row r of the block from TMEM (columns col ..), times f and added to p (held) or in its place, to p (zero: 0).
 template <typename T, int DIM>
-__device__ __forceinline__ void store_row(uint32_t taddr, T* p, int64_t step, int dim, float f, bool zero, bool valid) {
+__device__ __forceinline__ void store_row(uint32_t taddr, T* p, int64_t step, int dim, float f, bool held, bool zero,
+                                          bool valid) {
   constexpr int V = 16 / sizeof(T);
   const bool vec = dim % V == 0 && ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(step * sizeof(T))) & 15) == 0;
 #pragma unroll
@@ -62,6 +63,20 @@ __device__ __forceinline__ void store_row(uint32_t taddr, T* p, int64_t step, in
       alignas(16) T r[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) r[e] = from_f<T>(zero ? 0.f : __uint_as_float(o[e]) * f);
+      if (sizeof(T) == 4 && held && valid && !zero) {
+#pragma unroll
+        for (int e = 0; e < 16; e += V) {
+          if (vec && c + e < dim) {
+            const Pack<T, V> was = *reinterpret_cast<const Pack<T, V>*>(p + c + e);
+#pragma unroll
+            for (int n = 0; n < V; ++n) r[e + n] = from_f<T>(to_f(r[e + n]) + to_f(was.e[n]));
+          } else if (!vec) {
+#pragma unroll
+            for (int n = 0; n < V; ++n)
+              if (c + e + n < dim) r[e + n] = from_f<T>(to_f(r[e + n]) + to_f(p[c + e + n]));
+          }
+        }
+      }
       if (valid) {
         if (vec) {
 #pragma unroll
@@ -183,6 +198,13 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
     const int klo = __reduce_min_sync(0xffffffffu, live ? kp : INT32_MAX);
     const int khi = __reduce_max_sync(0xffffffffu, live ? kp : INT32_MIN);
     const uint32_t base = tmem + ((uint32_t)(warp & 3) << 21);
+    // the sums so far to dv (or dk)
+    const auto keep = [&](float f, bool held, bool zero) {
+      const bool dv = wg == 0;
+      const int64_t* st = dv ? A.dvs : A.dks;
+      T* p = static_cast<T*>(dv ? A.dv : A.dk) + b * st[0] + hk * st[1] + j * st[2];
+      store_row<T, L::kDim>(base + (dv ? S::kDv : S::kDk), p, st[2], A.D, dv ? f : f * A.scale, held, zero, j < A.Lk);
+    };
     for (int64_t it = 0; it < tiles; ++it) {
       if (A.table && it % per == 0) {  // the next head's table
         named_barrier(2, 256);
@@ -193,6 +215,7 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
       const QueryInfo& I = info[it % S::kInfo];
       wait(&sfull, it & 1, &abort_flag, polls);
       fence_after_sync();
+      if (NS > 1 && it > 0 && starts<NS>(it)) keep(1.f, it > kRest, false);
       const int qlo = I.t.lo[wg], qhi = I.t.hi[wg];
       const bool some = I.t.live[wg] != 0 && klo <= khi;
       const bool above = (int64_t)klo - qhi >= reach, below = (int64_t)khi - qlo <= -reach;
@@ -282,14 +305,7 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
       wait(&sfull, tiles & 1, &abort_flag, polls);
       fence_after_sync();
     }
-    const bool zero = !live || tiles == 0, valid = j < A.Lk;
-    const float f = abort_flag ? NAN : 1.f;
-    if (wg == 0)
-      store_row<T, L::kDim>(base + S::kDv, static_cast<T*>(A.dv) + b * A.dvs[0] + hk * A.dvs[1] + j * A.dvs[2], A.dvs[2], A.D,
-                       f, zero, valid);
-    else
-      store_row<T, L::kDim>(base + S::kDk, static_cast<T*>(A.dk) + b * A.dks[0] + hk * A.dks[1] + j * A.dks[2], A.dks[2], A.D,
-                       f * A.scale, zero, valid);
+    keep(abort_flag ? NAN : 1.f, NS > 1 && tiles > kRest, !live || tiles == 0);
   } else if (warp == 8) {
     if (lane == 0 && tiles > 0) {
       const uint32_t id_s = idesc_bf16(128, kGradN, false), id_o = idesc_bf16(128, (A.D + 15) / 16 * 16, true);
@@ -307,8 +323,8 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
         mma_commit(&sfull);
         wait(&pfull, it & 1, &abort_flag, polls);
         fence_after_sync();
-        values<NS, kGradN, L>(tmem + S::kDv, aO, id_o, it > 0, p_at);
-        values<NS, kGradN, L>(tmem + S::kDk, aQ, id_o, it > 0, ds_at);
+        values<NS, kGradN, L>(tmem + S::kDv, aO, id_o, !starts<NS>(it), p_at);
+        values<NS, kGradN, L>(tmem + S::kDk, aQ, id_o, !starts<NS>(it), ds_at);
         mma_commit(&empty[st]);
       }
       mma_commit(&sfull);
@@ -515,10 +531,16 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
     float ta = 0.f, tb = 0.f;                      // all of the row
     float ha = 0.f, hb = 0.f, la = 0.f, lb = 0.f;  // beyond the reach, above and below
     const bool windows = A.table && wn < A.buckets.num_buckets;
+    // the sums so far to dq
+    const auto keep = [&](float f, bool held, bool zero) {
+      store_row<T, L::kDim>(base + S::kDq, static_cast<T*>(A.dq) + b * A.dqs[0] + h * A.dqs[1] + i * A.dqs[2], A.dqs[2], A.D,
+                            f, held, zero, valid);
+    };
     for (int j = 0; j < tiles; ++j) {
       const TileInfo<kGradN>& I = info[j % S::kInfo];
       wait(&sfull, j & 1, &abort_flag, polls);
       fence_after_sync();
+      if (NS > 1 && w0 == 0 && j > 0 && starts<NS>(j)) keep(A.scale, j > kRest, false);
 #pragma unroll 1  // one copy of the code: four no longer stay in the instruction cache
       for (int c = 0; c < kGradN; c += 16) {
         const int sub = c / kSub;
@@ -667,9 +689,7 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
       fence_after_sync();
     }
     const float broken = abort_flag ? NAN : 0.f;
-    if (w0 == 0)
-      store_row<T, L::kDim>(base + S::kDq, static_cast<T*>(A.dq) + b * A.dqs[0] + h * A.dqs[1] + i * A.dqs[2], A.dqs[2], A.D,
-                       A.scale + broken, !live || tiles == 0, valid);
+    if (w0 == 0) keep(A.scale + broken, NS > 1 && tiles > kRest, !live || tiles == 0);
     if (A.table) {
       const int hi = lut[2 * reach].y, lo = lut[0].y;
       if (hi >= 0) {
@@ -721,7 +741,7 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
         mma_commit(&sfull);
         wait(&pfull, j & 1, &abort_flag, polls);
         fence_after_sync();
-        values<NS, kGradN, L>(tmem + S::kDq, aK, id_o, j > 0,
+        values<NS, kGradN, L>(tmem + S::kDq, aK, id_o, !starts<NS>(j),
                               [=](int part, int k) { return tmem + k * 16 + (part < 2 ? part * 8 : S::kDp); });
         mma_commit(&empty[st]);
       }

@@ -147,7 +147,7 @@ void split_keys(const fx_attn_args* a, Kind kind, int sms, AttnArgs& A) {
 }
 
 size_t part_bytes(const fx_attn_args* a, const AttnArgs& A) {
-  return A.splits > 1 ? (size_t)(a->batch * a->heads * a->q_len) * A.splits * (a->dim + 2) * sizeof(float) + 256 : 0;
+  return A.splits > 1 ? (size_t)(a->batch * a->heads * a->q_len) * A.splits * part_step((int)a->dim) * sizeof(float) + 256 : 0;
 }
 
 // A block a row joins the most parts at a time (256 rows of 9 parts: 5 us, 7 with a warp a row; 8 rows
