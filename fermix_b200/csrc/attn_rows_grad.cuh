@@ -8,6 +8,9 @@
 // delta from the rounded output would leave its rounding there, so the table's gradient keeps
 // a = sum p (do . v) and b = sum p of each row and bucket, and takes sum_i (a - b sum a / sum b).
 //
+// Bound: FMA instructions; this is the float32 path above 64 entries, whose three parts of both sides do
+// not fit shared memory, and the gradient where there are no queries.
+//
 // Nothing is added atomically: a block owns its rows of dq (or of dk and dv, over all the
 // query heads that share the key head), and its groups' partial sums are added in order.
 #pragma once

@@ -122,7 +122,7 @@ Kind kind_of(const fx_attn_args* a) {
 // Parts of the keys. Rows kernel: eight blocks an SM, parts of 128 keys at least. Fragment kernel:
 // two rounds of the two blocks an SM holds (one above 64 entries), 512 keys a part at least; more
 // and shorter parts spend more time on a block's start (measured for 64 key heads of 65536 keys:
-// 37 parts 205 us, 9 parts 186 us).
+// 37 parts 205 us, 9 parts 186 us). Tiles: attn_tc_splits.
 void split_keys(const fx_attn_args* a, Kind kind, int sms, AttnArgs& A) {
   if (kind == TC) {
     A.splits = attn_tc_splits(A, a->dtype == FX_F32, sms);

@@ -179,6 +179,9 @@ int launch_attn_tc_fwd(cudaStream_t s, const AttnArgs& A, bool is_f32, bool alig
   return aligned ? fwd_bf16<LOAD_TMA>(s, A) : fwd_bf16<LOAD_ENTRIES>(s, A);
 }
 
+// Parts that fill the device: of 128 keys at least in float32, of 512 in bfloat16 and none below 2048
+// keys. Measured, us, without and with: 8 heads of 512 x 512 float32 dim 64 67 and 32; 8 of 1024 x 1024 bfloat16
+// dim 64 30 and 36 in two parts; 8 heads of 128 queries on 2048 keys 44 and 28, of 64 on 16384 263 and 34.
 int attn_tc_splits(const AttnArgs& A, bool is_f32, int sms) {
   const int rows = !is_f32 && A.D > 64 && A.Lq > 128 ? 256 : 128;            // of a block
   const int resident = (is_f32 ? A.D <= 64 : rows == 128) ? 2 : 1;           // blocks an SM holds

