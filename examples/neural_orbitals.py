@@ -2,7 +2,7 @@
 tokens -> attention blocks -> orbitals -> log|psi| = log|det|, one training step of it, and the
 evaluation of one electron's token against the others.
 
-    python examples/neural_orbitals.py [--samples 64] [--electrons 32] [--sites 64] [--dtype float32]
+    python -m examples.neural_orbitals [--samples 64] [--electrons 32] [--sites 64] [--dtype float32]
 
 psi(occ) = det of the (electrons x electrons) matrix whose row i is a linear map of electron i's
 token after the blocks. The tokens of one sample attend to each other with a learned bias of

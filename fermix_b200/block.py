@@ -122,10 +122,11 @@ def _batch_stride(pos):
     return pos.stride(0) if pos is not None and pos.dim() == 2 else 0
 
 
-def _buckets(num_buckets, max_distance, bidirectional, q_pos, k_pos, q_stride, k_stride):
-    edges, count = _edges(num_buckets, max_distance, bool(bidirectional))
-    return _lib.Buckets(num_buckets, int(bool(bidirectional)), count, 0, ctypes.addressof(edges), _ptr(q_pos),
-                        _ptr(k_pos), q_stride, k_stride)
+def _set_buckets(a, num_buckets, max_distance, bidirectional, q_pos, k_pos, q_stride, k_stride):
+    """a.buckets; a keeps the edges it points to, which may leave the cache before a backward pass."""
+    a.edges, count = _edges(num_buckets, max_distance, bool(bidirectional))
+    a.buckets = _lib.Buckets(num_buckets, int(bool(bidirectional)), count, 0, ctypes.addressof(a.edges), _ptr(q_pos),
+                             _ptr(k_pos), q_stride, k_stride)
 
 
 # ------------------------------------------------------------------ residual with its norms
@@ -268,7 +269,7 @@ class _PositionBias(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        a = ctx.args
+        a = _lib.BiasArgs.from_buffer_copy(ctx.args)  # the graph may be run again, from another thread too
         q_pos, k_pos = ctx.saved_tensors  # alive until the launches are queued
         grad = grad.contiguous()
         dtable = torch.empty(ctx.table[0], dtype=ctx.table[1], device=grad.device)
@@ -284,8 +285,8 @@ def _bias_forward(table, q_pos, k_pos, shape, max_distance, bidirectional):
     a.dtype = _KIND[table.dtype]
     a.heads, a.q_len, a.k_len = shape[-3:]
     a.batch = shape[0] if len(shape) == 4 else 1
-    a.buckets = _buckets(table.shape[1], max_distance, bidirectional, q_pos, k_pos, _batch_stride(q_pos),
-                         _batch_stride(k_pos))
+    _set_buckets(a, table.shape[1], max_distance, bidirectional, q_pos, k_pos, _batch_stride(q_pos),
+                 _batch_stride(k_pos))
     out = torch.empty(shape, dtype=table.dtype, device=table.device)
     a.table, a.out = table.data_ptr(), out.data_ptr()
     _call(_lib.lib().fermix_position_bias, table.device, ctypes.byref(a))
@@ -334,7 +335,7 @@ def _attn_args(q, k, v, table, out, lse, q_pos, k_pos, key_mask, causal, scale, 
     a.scale = scale
     qs, ks = _batch_stride(q_pos), _batch_stride(k_pos)
     if table is not None:
-        a.buckets = _buckets(table.shape[1], max_distance, bidirectional, q_pos, k_pos, qs, ks)
+        _set_buckets(a, table.shape[1], max_distance, bidirectional, q_pos, k_pos, qs, ks)
     else:
         a.buckets.q_pos, a.buckets.k_pos, a.buckets.q_pos_stride, a.buckets.k_pos_stride = _ptr(q_pos), _ptr(
             k_pos), qs, ks

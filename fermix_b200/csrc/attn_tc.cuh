@@ -775,52 +775,52 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
         p[1] = broken ? NAN : l;
       }
     } else {
-    const float inv = broken ? NAN : l == 0.f ? 0.f : 1.f / l;
-    T* out = static_cast<T*>(A.out) + b * A.os[0] + h * A.os[1] + i * A.os[2];
-    constexpr int V = 16 / sizeof(T);
-    const bool ovec =
-        A.D % V == 0 && ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(A.os[2] * sizeof(T))) & 15) == 0;
+      const float inv = broken ? NAN : l == 0.f ? 0.f : 1.f / l;
+      T* out = static_cast<T*>(A.out) + b * A.os[0] + h * A.os[1] + i * A.os[2];
+      constexpr int V = 16 / sizeof(T);
+      const bool ovec =
+          A.D % V == 0 && ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(A.os[2] * sizeof(T))) & 15) == 0;
 #pragma unroll
-    for (int c = half * 16; c < L::kDim; c += 32) {
-      if (c < A.D) {
-        uint32_t o[16];
-        if (tiles > 0) {
-          ld16(base + S::kO + c, o);
-          tmem_wait_ld();
-        }
-        if constexpr (NS > 1) {
-          if (held && valid) {
+      for (int c = half * 16; c < L::kDim; c += 32) {
+        if (c < A.D) {
+          uint32_t o[16];
+          if (tiles > 0) {
+            ld16(base + S::kO + c, o);
+            tmem_wait_ld();
+          }
+          if constexpr (NS > 1) {
+            if (held && valid) {
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-              if (c + e >= A.D) break;
-              Pack<T, 4> v;
-              if (ovec) v = *reinterpret_cast<const Pack<T, 4>*>(out + c + e);
-              else
+              for (int e = 0; e < 16; e += 4) {
+                if (c + e >= A.D) break;
+                Pack<T, 4> v;
+                if (ovec) v = *reinterpret_cast<const Pack<T, 4>*>(out + c + e);
+                else
 #pragma unroll
-                for (int n = 0; n < 4; ++n) v.e[n] = c + e + n < A.D ? out[c + e + n] : 0.f;
+                  for (int n = 0; n < 4; ++n) v.e[n] = c + e + n < A.D ? out[c + e + n] : 0.f;
 #pragma unroll
-              for (int n = 0; n < 4; ++n) o[e + n] = __float_as_uint(__uint_as_float(o[e + n]) + v.e[n]);
+                for (int n = 0; n < 4; ++n) o[e + n] = __float_as_uint(__uint_as_float(o[e + n]) + v.e[n]);
+              }
+            }
+          }
+          alignas(16) T r[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) r[e] = from_f<T>(l == 0.f ? 0.f : __uint_as_float(o[e]) * inv);
+          if (valid) {
+            if (ovec) {
+#pragma unroll
+              for (int e = 0; e < 16; e += V)
+                if (c + e < A.D) *reinterpret_cast<Pack<T, V>*>(out + c + e) = *reinterpret_cast<Pack<T, V>*>(r + e);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (c + e < A.D) out[c + e] = r[e];
             }
           }
         }
-        alignas(16) T r[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) r[e] = from_f<T>(l == 0.f ? 0.f : __uint_as_float(o[e]) * inv);
-        if (valid) {
-          if (ovec) {
-#pragma unroll
-            for (int e = 0; e < 16; e += V)
-              if (c + e < A.D) *reinterpret_cast<Pack<T, V>*>(out + c + e) = *reinterpret_cast<Pack<T, V>*>(r + e);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (c + e < A.D) out[c + e] = r[e];
-          }
-        }
       }
-    }
-    if (valid && half == 0 && A.lse)
-      A.lse[((int64_t)b * A.H + h) * A.Lq + i] = broken ? NAN : l == 0.f ? -INFINITY : m + log2f(l);
+      if (valid && half == 0 && A.lse)
+        A.lse[((int64_t)b * A.H + h) * A.Lq + i] = broken ? NAN : l == 0.f ? -INFINITY : m + log2f(l);
     }
   } else if (warp == 8 * QT) {
     // -------------------------------------------------------- tensor instructions

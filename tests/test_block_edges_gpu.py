@@ -134,3 +134,25 @@ def test_long_float32_sums(dim):
     exp = torch.autograd.grad(want, list(b.values()), cot.double())
     for n, x, y in [("out", out, want), *zip(a, got, exp)]:
         assert ((x.double() - y).norm() / y.norm()).item() <= 6e-6, n
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_bucket_edges_outlive_their_cache(dtype):
+    """The buckets of a forward pass are those of its backward pass, whatever was asked for in between."""
+    import gc
+
+    from fermix_b200 import block
+
+    t, kw, cot = _attention_case((1, 2, 2, 40, 50, 16), dtype, 47)
+    a = {n: x.detach().requires_grad_(True) for n, x in t.items()}
+    pos = torch.arange(50, device="cuda")
+    want = torch.autograd.grad(fx.biased_attention(**a, **kw), list(a.values()), cot)
+    bias_want = torch.autograd.grad(fx.position_bias(a["table"], pos).sum(), a["table"])
+    out, bias = fx.biased_attention(**a, **kw), fx.position_bias(a["table"], pos)
+    block._edges.cache_clear()
+    gc.collect()
+    others = [block._edges(32, 200 + n, True) for n in range(40)]  # the freed arrays' sizes
+    got = torch.autograd.grad(out, list(a.values()), cot)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    assert torch.equal(torch.autograd.grad(bias.sum(), a["table"])[0], bias_want[0])
+    assert len(others) == 40
