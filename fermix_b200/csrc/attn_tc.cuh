@@ -20,7 +20,8 @@
 // entries), two threads a row, half the columns each; scores and probabilities live in TMEM. A row's
 // reference is its first tile's maximum and moves only when a score is 2^64 above it, which the sum of
 // the exponentials shows: no maximum is taken on the way. Few blocks of queries split the keys over
-// blocks. Bound: instructions of the softmax, about 40 issue slots a score and warp (64 x 8 heads of
+// blocks. Bound: the softmax's latency at two blocks an SM, what TMEM and registers allow: 0.44 of the
+// issue slots are used, warps wait for TMEM loads, fixed latencies and each other (64 x 8 heads of
 // 512 x 512, dim 64: 152 us, 229 TFLOP/s; 2 x 16 heads of 4096 x 4096, dim 128: 420 us, 654 TFLOP/s, 0.40
 // of the library's matrix rate). float32, 512 x 4 heads of 128 x 128, dim 32: 143 us.
 #pragma once
