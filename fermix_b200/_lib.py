@@ -109,7 +109,7 @@ class AttnArgs(ctypes.Structure):
                 _fields(_vp, "q k v table") + _fields(_i64x3, "q_stride k_stride v_stride") +
                 _fields(_vp, "key_mask") + _fields(_i64, "mask_stride") + _fields(_vp, "out") +
                 _fields(_i64x3, "out_stride") + _fields(_vp, "lse dout") + _fields(_i64x3, "dout_stride") +
-                _fields(_vp, "dq dk dv dtable") + _fields(_i64x3, "dq_stride dk_stride dv_stride"))
+                _fields(_vp, "dq dk dv dtable") + _fields(_i64x3, "dq_stride dk_stride dv_stride") + _fields(_vp, "lse_low"))
 
 
 _lib = None

@@ -343,7 +343,9 @@ def _attn_args(q, k, v, table, out, lse, q_pos, k_pos, key_mask, causal, scale, 
     a.q_stride[:], a.k_stride[:], a.v_stride[:] = _strides(q), _strides(k), _strides(v)
     if key_mask is not None:
         a.key_mask, a.mask_stride = _ptr(key_mask), key_mask.stride(0)
-    a.out, a.lse = _ptr(out), _ptr(lse)
+    a.out = _ptr(out)
+    if lse is not None:
+        a.lse, a.lse_low = lse.data_ptr(), lse[1].data_ptr()
     a.out_stride[:] = _strides(out)
     return a
 
@@ -353,7 +355,7 @@ def _attn_forward(q, k, v, table, rest, with_lse):
     out = torch.empty_like(q)
     if out.stride(-1) != 1:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if with_lse else None
+    lse = torch.empty((2, *q.shape[:3]), dtype=torch.float32, device=q.device) if with_lse else None  # and lse_low
     a = _attn_args(q, k, v, table, out, lse, *rest)
     L = _lib.lib()
     _call_with_workspace(L.fermix_biased_attention, L.fermix_biased_attention_workspace_bytes, q.device, a)
@@ -374,8 +376,8 @@ class _BiasedAttention(torch.autograd.Function):
         q, k, v, table, out, lse, q_pos, k_pos, key_mask = ctx.saved_tensors
         a = _lib.AttnArgs.from_buffer_copy(ctx.args)  # the graph may be run again, from another thread too
         # a saved tensor may have been put elsewhere and back (saved-tensor hooks)
-        a.q, a.k, a.v, a.table, a.out, a.lse = (q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(table), out.data_ptr(),
-                                                lse.data_ptr())
+        a.q, a.k, a.v, a.table, a.out, a.lse, a.lse_low = (q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(table),
+                                                           out.data_ptr(), lse.data_ptr(), lse[1].data_ptr())
         a.q_stride[:], a.k_stride[:], a.v_stride[:], a.out_stride[:] = (_strides(q), _strides(k), _strides(v),
                                                                         _strides(out))
         a.buckets.q_pos, a.buckets.k_pos, a.key_mask = _ptr(q_pos), _ptr(k_pos), _ptr(key_mask)

@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kDecodeThreads, DB == 1 ? 2 : 1) attn_decode_k
       const int64_t q_i = (row0 + row) % (int)A.Lq;
       static_cast<bf16*>(A.out)[b * A.os[0] + h * A.os[1] + q_i * A.os[2] + c] =
           from_f<bf16>(sum == 0.f ? 0.f : acc / sum);
-      if (A.lse && c == 0) A.lse[((int64_t)b * A.H + h) * A.Lq + q_i] = sum == 0.f ? -INFINITY : top + log2f(sum);
+      if (A.lse && c == 0) store_lse(A, ((int64_t)b * A.H + h) * A.Lq + q_i, top, sum);
     }
   }
 }

@@ -27,7 +27,7 @@ struct AttnArgs {
   int64_t q_pos_stride, k_pos_stride;
   void* out;
   int64_t os[3];
-  float* lse;
+  float *lse, *lse_low;  // (batch, heads, q_len) each
   const void* dout;
   int64_t dos[3];
   void *dq, *dk, *dv;
@@ -52,6 +52,14 @@ __host__ __device__ constexpr int part_step(int dim) { return (dim + 3) / 4 * 4 
 __device__ __forceinline__ float bias2(float t) {
   const float b = t * kLog2e;
   return isfinite(t) ? fminf(fmaxf(b, -3.4028234e38f), 3.4028234e38f) : b;
+}
+
+// The logarithm of a row's sum of exponentials, l to the reference m, as two floats: beside an m of 1e9
+// log2 l would be lost, and the gradient's probabilities with it. (Knuth's sum of two and its error.)
+__device__ __forceinline__ void store_lse(const AttnArgs& A, int64_t row, float m, float l, bool broken = false) {
+  const float g = log2f(l), hi = m + g, z = hi - m;
+  A.lse[row] = broken ? NAN : l == 0.f ? -INFINITY : hi;
+  if (A.lse_low) A.lse_low[row] = l == 0.f ? 0.f : (m - (hi - z)) + (g - z);
 }
 
 template <typename T, int NE, bool VECLOAD>
@@ -204,7 +212,7 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_kernel(const __grid_co
       const int h = hk * G + (int)(row / A.Lq);
       const int64_t i = row % A.Lq;
       static_cast<T*>(A.out)[b * A.os[0] + h * A.os[1] + i * A.os[2] + c] = from_f<T>(sum == 0.f ? 0.f : acc / sum);
-      if (A.lse && c == 0) A.lse[((int64_t)b * A.H + h) * A.Lq + i] = sum == 0.f ? -INFINITY : top + log2f(sum);
+      if (A.lse && c == 0) store_lse(A, ((int64_t)b * A.H + h) * A.Lq + i, top, sum);
     }
   }
 }
@@ -257,7 +265,7 @@ __global__ void __launch_bounds__(kRowsThreads) attn_join_kernel(const __grid_co
   if (threadIdx.x < A.D)
     static_cast<T*>(A.out)[b * A.os[0] + h * A.os[1] + i * A.os[2] + threadIdx.x] =
         from_f<T>(sum == 0.f ? 0.f : acc / sum);
-  if (A.lse && threadIdx.x == 0) A.lse[((int64_t)b * A.H + h) * A.Lq + i] = sum == 0.f ? -INFINITY : top + log2f(sum);
+  if (A.lse && threadIdx.x == 0) store_lse(A, ((int64_t)b * A.H + h) * A.Lq + i, top, sum);
 }
 
 // The same with a warp a row, for many rows of few parts. A lane weighs a part, 32 at a time, and adds
@@ -297,7 +305,7 @@ __global__ void __launch_bounds__(kRowsThreads) attn_join_warp_kernel(const __gr
 #pragma unroll
   for (int e = 0; e < NE; ++e)
     if (lane + 32 * e < A.D) out[lane + 32 * e] = from_f<T>(sum == 0.f ? 0.f : acc[e] / sum);
-  if (A.lse && lane == 0) A.lse[w] = sum == 0.f ? -INFINITY : top + log2f(sum);
+  if (A.lse && lane == 0) store_lse(A, w, top, sum);
 }
 
 }  // namespace fx

@@ -1,6 +1,6 @@
 // Gradient of the biased attention, a few rows (queries, then keys) at a time:
 //
-//   p_ij = 2^(s_ij - lse_i),  delta_i = sum_c o_ic do_ic,  ds_ij = p_ij (do_i . v_j - delta_i)
+//   p_ij = 2^((s_ij - lse_i) - lse_low_i),  delta_i = sum_c o_ic do_ic,  ds_ij = p_ij (do_i . v_j - delta_i)
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij do_i
 //   dtable[h, c] = sum of ds_ij over the pairs of bucket c
 //
@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_grad_kernel(const __gr
   const T* table = static_cast<const T*>(A.table) + (int64_t)hk * G * nb;
   const uint8_t* mask = A.mask ? A.mask + b * A.mask_stride : nullptr;
 
-  float x[RC][NE], y[RC][NE], ax[RC][NE], ay[RC][NE], lse[RC], del[RC];
+  float x[RC][NE], y[RC][NE], ax[RC][NE], ay[RC][NE], lse[RC], low[RC], del[RC];
   int pos[RC], head[RC];
   bool live[RC];
 #pragma unroll
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_grad_kernel(const __gr
     const int64_t row = r0 + r;
     live[r] = row < own && (!KEYS || !mask || mask[row]);
     pos[r] = head[r] = 0;
-    lse[r] = del[r] = 0.f;
+    lse[r] = low[r] = del[r] = 0.f;
 #pragma unroll
     for (int e = 0; e < NE; ++e) x[r][e] = y[r][e] = ax[r][e] = ay[r][e] = 0.f;
     if (!live[r]) continue;
@@ -74,6 +74,7 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_grad_kernel(const __gr
       const int64_t i = row % A.Lq, at = ((int64_t)b * A.H + hk * G + head[r]) * A.Lq + i;
       pos[r] = attn_q_pos(A, b, i);
       lse[r] = A.lse[at];
+      low[r] = A.lse_low ? A.lse_low[at] : 0.f;
       del[r] = A.delta[at];
       load_entries<T, NE, VECLOAD>(Q + head[r] * A.qs[1] + i * A.qs[2], c0, A.D, x[r]);
       load_entries<T, NE, VECLOAD>(DO + head[r] * A.dos[1] + i * A.dos[2], c0, A.D, y[r]);
@@ -82,7 +83,7 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_grad_kernel(const __gr
   __syncthreads();
   for (int64_t base = 0; base < other; base += GROUPS) {
     const int64_t j = base + group;
-    float u[NE], w[NE], lse_j = 0.f, del_j = 0.f;
+    float u[NE], w[NE], lse_j = 0.f, low_j = 0.f, del_j = 0.f;
     int pj = 0, hj = 0;
     bool there = j < other;
     if (!KEYS && there && mask) there = mask[j];
@@ -94,6 +95,7 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_grad_kernel(const __gr
         const int64_t i = j % A.Lq, at = ((int64_t)b * A.H + hk * G + hj) * A.Lq + i;
         pj = attn_q_pos(A, b, i);
         lse_j = A.lse[at];
+        low_j = A.lse_low ? A.lse_low[at] : 0.f;
         del_j = A.delta[at];
         load_entries<T, NE, VECLOAD>(Q + hj * A.qs[1] + i * A.qs[2], c0, A.D, u);
         load_entries<T, NE, VECLOAD>(DO + hj * A.dos[1] + i * A.dos[2], c0, A.D, w);
@@ -122,7 +124,7 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_grad_kernel(const __gr
           c = bucket_of(A.buckets, clamp_reach(d, A.buckets.reach));
           s += bias2(to_f(table[(KEYS ? hj : head[r]) * nb + c]));
         }
-        p = exp2f(s - L);
+        p = exp2f((s - L) - (KEYS ? low_j : low[r]));
         ds = p * (dp - de);
         if (!KEYS && A.table && gl == 0) {
           hist[((group * RC + r) * nb + c) * 2] += p * dp;

@@ -820,8 +820,7 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
           }
         }
       }
-      if (valid && half == 0 && A.lse)
-        A.lse[((int64_t)b * A.H + h) * A.Lq + i] = broken ? NAN : l == 0.f ? -INFINITY : m + log2f(l);
+      if (valid && half == 0 && A.lse) store_lse(A, ((int64_t)b * A.H + h) * A.Lq + i, m, l, broken);
     }
   } else if (warp == 8 * QT) {
     // -------------------------------------------------------- tensor instructions

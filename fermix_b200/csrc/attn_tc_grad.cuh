@@ -4,8 +4,11 @@
 // owns what it writes, so nothing is added atomically; the scores are formed twice for that
 // (seven products instead of five).
 //
-//   p = 2^(scale2 q.k + bias2 - lse),  ds = p (do.v - delta)
+//   p = 2^(((scale2 q.k + bias2) - lse) - lse_low),  ds = p (do.v - delta)
 //   dv = p^T do, dk = scale ds^T q, dq = scale ds k
+//
+// The bias is added first and the logarithm of the row's sum taken off as two floats, the forward's
+// order: what a huge bias absorbed there is absorbed here.
 //
 // In both, a thread holds one row of the 128-row block (TMEM lane), p and ds go back to TMEM as
 // the A operand of the second products, and the 64-row tiles of the other side stream through
@@ -118,7 +121,8 @@ struct DkvShape {
 
 struct alignas(16) QueryInfo {
   TileInfo<kGradN> t;
-  float lse[kGradN], delta[kGradN];  // lse +inf: a row without keys, or past the end
+  // the parts of -lse (-inf: a row without keys, or past the end) and -delta
+  float lse[kGradN], low[kGradN], delta[kGradN];
 };
 
 template <typename T, int NS, typename L, int ST, int LOAD>
@@ -235,15 +239,9 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
         ld_cols<S::kStepCols>(base + S::kDp + col, dp);
         tmem_wait_ld();
         uint32_t wp[NS][S::kStepCols / 2], wd[NS][S::kStepCols / 2];
-        float bias[S::kStepCols];  // less lse: +inf there leaves a row out
+        float bias[S::kStepCols];
 #pragma unroll
-        for (int e = 0; e < S::kStepCols; e += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(&I.lse[col + e]);
-          bias[e] = -v.x;
-          bias[e + 1] = -v.y;
-          bias[e + 2] = -v.z;
-          bias[e + 3] = -v.w;
-        }
+        for (int e = 0; e < S::kStepCols; ++e) bias[e] = flat;
         if (each) {
           int q[S::kStepCols];
 #pragma unroll
@@ -255,32 +253,30 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
             q[e + 3] = v.w;
           }
           if (A.table) {
-            float t[S::kStepCols];
 #pragma unroll
-            for (int e = 0; e < S::kStepCols; ++e) t[e] = lut[__vimin_s32_relu(kp + reach - q[e], 2 * reach)];
-#pragma unroll
-            for (int e = 0; e < S::kStepCols; ++e) bias[e] += t[e];
+            for (int e = 0; e < S::kStepCols; ++e) bias[e] = lut[__vimin_s32_relu(kp + reach - q[e], 2 * reach)];
           }
           if (A.causal) {
 #pragma unroll
             for (int e = 0; e < S::kStepCols; ++e)
               if (kp > q[e]) bias[e] = -INFINITY;
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < S::kStepCols; ++e) bias[e] += flat;
         }
         const uint64_t ss = both(A.scale2, A.scale2);
 #pragma unroll
         for (int e = 0; e < S::kStepCols; e += 4) {
           const float4 de = *reinterpret_cast<const float4*>(&I.delta[col + e]);
-          const uint64_t d2[2] = {both(-de.x, -de.y), both(-de.z, -de.w)};
+          const float4 hi = *reinterpret_cast<const float4*>(&I.lse[col + e]);
+          const float4 lo = *reinterpret_cast<const float4*>(&I.low[col + e]);
+          const uint64_t d2[2] = {both(de.x, de.y), both(de.z, de.w)};
+          const uint64_t h2[2] = {both(hi.x, hi.y), both(hi.z, hi.w)}, l2[2] = {both(lo.x, lo.y), both(lo.z, lo.w)};
 #pragma unroll
           for (int f = 0; f < 4; f += 2) {
             const int i0 = e + f;
             float v0, v1;
-            halves(fma_both(both(__uint_as_float(s[i0]), __uint_as_float(s[i0 + 1])), ss, both(bias[i0], bias[i0 + 1])), v0,
-                   v1);
+            const uint64_t sc =
+                fma_both(both(__uint_as_float(s[i0]), __uint_as_float(s[i0 + 1])), ss, both(bias[i0], bias[i0 + 1]));
+            halves(add_both(add_both(sc, h2[f / 2]), l2[f / 2]), v0, v1);
             const float p0 = ex2(v0), p1 = ex2(v1);
             float d0, d1;
             halves(mul_both(both(p0, p1),
@@ -350,8 +346,9 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
       const uint32_t bits = fill_info<kGradN>(
           I.t, sub, [&](int) { return ls != -INFINITY; }, [&](int x) { return attn_q_pos(A, b, i0 + x); });
       const bool ok = (bits >> lane) & 1u;
-      I.lse[e] = ok ? ls : INFINITY;
-      I.delta[e] = ok ? A.delta[row + i0 + e] : 0.f;
+      I.lse[e] = ok ? -ls : -INFINITY;
+      I.low[e] = ok && A.lse_low ? -A.lse_low[row + i0 + e] : 0.f;
+      I.delta[e] = ok ? -A.delta[row + i0 + e] : 0.f;
     };
     if constexpr (TMA) {
       if (w == 0) {
@@ -529,7 +526,7 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
     const int64_t i = i0 + tid;
     const bool valid = i < A.Lq, live = row_live(tid);
     const int qp = live ? attn_q_pos(A, b, i) : 0;
-    const float lse_i = live ? lse[i] : INFINITY, delta = live ? A.delta[bh * A.Lq + i] : 0.f;
+    const float lse_i = live ? lse[i] : INFINITY, low_i = live && A.lse_low ? A.lse_low[bh * A.Lq + i] : 0.f, delta = live ? A.delta[bh * A.Lq + i] : 0.f;
     const int qlo = __reduce_min_sync(0xffffffffu, live ? qp : INT32_MAX);
     const int qhi = __reduce_max_sync(0xffffffffu, live ? qp : INT32_MIN);
     const uint32_t base = tmem + ((uint32_t)(warp & 3) << 21);
@@ -560,6 +557,7 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
         ld16(base + S::kDp + c, dp);
         tmem_wait_ld();
         const uint64_t ss = both(A.scale2, A.scale2), nd = both(-delta, -delta);
+        const uint64_t nh = both(-lse_i, -lse_i), nl = both(-low_i, -low_i);
         uint64_t sa = 0, sb = 0;  // pairs of zeros
         if (near || later) {
           // everything that is read before the first histogram is written: the compiler may not
@@ -578,7 +576,7 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
           for (int e = 0; e < 16; ++e) {
             int2 t = make_int2(0, -1);
             if (A.table) t = lut[__vimin_s32_relu(k[e] + reach - qp, 2 * reach)];
-            bias[e] = __int_as_float(t.x) - lse_i;
+            bias[e] = __int_as_float(t.x);
             if ((A.causal && k[e] > qp) || !((bits >> e) & 1u)) bias[e] = -INFINITY;
             at[e] = t.y;
           }
@@ -586,7 +584,8 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
             float v0, v1, x0, x1, y0, y1;
-            halves(fma_both(both(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), ss, both(bias[e], bias[e + 1])), v0, v1);
+            const uint64_t sc = fma_both(both(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), ss, both(bias[e], bias[e + 1]));
+            halves(add_both(add_both(sc, nh), nl), v0, v1);
             pr[e] = ex2(v0);
             pr[e + 1] = ex2(v1);
             const uint64_t pp = both(pr[e], pr[e + 1]), dd = both(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1]));
@@ -639,13 +638,14 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
             }
           }
         } else {
-          const float flat = (A.table && some ? __int_as_float(lut[above ? 2 * reach : 0].x) : 0.f) - lse_i;
+          const float flat = A.table && some ? __int_as_float(lut[above ? 2 * reach : 0].x) : 0.f;
           const uint64_t bb = both(flat, flat);
           const bool whole = (bits & 0xffffu) == 0xffffu;
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
             float v0, v1, y0, y1;
-            halves(fma_both(both(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), ss, bb), v0, v1);
+            const uint64_t sc = fma_both(both(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), ss, bb);
+            halves(add_both(add_both(sc, nh), nl), v0, v1);
             if (!whole) {
               if (!((bits >> e) & 1u)) v0 = -INFINITY;
               if (!((bits >> (e + 1)) & 1u)) v1 = -INFINITY;

@@ -50,6 +50,7 @@ AttnArgs make(const fx_attn_args* a) {
   A.k_pos_stride = a->buckets.k_pos_stride;
   A.out = a->out;
   A.lse = a->lse;
+  A.lse_low = a->lse_low;
   A.dout = a->dout;
   A.dq = a->dq;
   A.dk = a->dk;

@@ -92,7 +92,10 @@ size_t fermix_position_bias_grad_workspace_bytes(const fx_bias_args* args);
  * key out whatever it holds; causal leaves out keys with k_pos > q_pos. A row with no key
  * gives 0, and no gradient. table NULL: no bias. lse (batch, heads, q_len) float32, the
  * logarithm (base 2) of each row's sum of exponentials: written by the forward when not
- * NULL, read by the backward. */
+ * NULL, read by the backward. lse_low, of the same shape: what lse's rounding left out of it,
+ * written (where lse is) and read alike; NULL: taken as zero, which is near enough unless a
+ * row's bias is huge beside its scores (log2 n of a row whose n keys all carry -1e9 is in
+ * lse_low alone). */
 #define FX_ATTN_MAX_DIM 128
 
 typedef struct {
@@ -113,6 +116,7 @@ typedef struct {
   int64_t dout_stride[3];
   void *dq, *dk, *dv, *dtable;
   int64_t dq_stride[3], dk_stride[3], dv_stride[3];
+  float* lse_low;
 } fx_attn_args;
 
 int fermix_biased_attention(void* stream, const fx_attn_args* args, void* workspace, size_t workspace_bytes);
