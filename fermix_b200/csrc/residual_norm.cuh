@@ -308,13 +308,14 @@ struct NormRow {
       }
     }
   }
-  // v <- normalised v (entries outside the row are 0 and stay so), returns 1 / rms.
-  __device__ __forceinline__ float normalise(float (&v)[E], bool layer, float eps, RowSum<WIDE>& sum) const {
+  // v <- normalised v (entries outside the row are 0 and stay so), returns 1 / rms; 0 of a row that is
+  // not there, whose own would be infinite without eps and make NaN of its zeros.
+  __device__ __forceinline__ float normalise(float (&v)[E], bool there, bool layer, float eps, RowSum<WIDE>& sum) const {
     if (!layer) {
       float q = 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) q = fmaf(v[e], v[e], q);
-      const float inv = rsqrtf(sum.mean(q) + eps);
+      const float rms = rsqrtf(sum.mean(q) + eps), inv = there ? rms : 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) v[e] *= inv;
       return inv;
@@ -328,7 +329,7 @@ struct NormRow {
       q = fmaf(d, d, q);
     }
     const float2 m = sum.moments(a, q, c, count, inv_count);
-    const float inv = rsqrtf(m.y + eps);
+    const float inv = there ? rsqrtf(m.y + eps) : 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = fmaf(-m.x, keep(e), v[e]) * inv;
     return inv;
@@ -493,11 +494,11 @@ __global__ void __launch_bounds__(kNormFwdResident<T, NV>) norm_fwd_kernel(const
       row.load(gate + (now.first + now.base) / A.R * W, g, 0.f);
     }
     stage = ring.next(stage);
-    row.normalise(f, A.layer, A.eps, sum);
+    row.normalise(f, there, A.layer, A.eps, sum);
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = fmaf(g[e], fmaf(f[e], s1[e], b1[e]), x[e]);
     row.store(static_cast<T*>(A.r) + (there ? i * W : 0), x, there);
-    row.normalise(x, A.layer, A.eps, sum);
+    row.normalise(x, there, A.layer, A.eps, sum);
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = fmaf(x[e], w2[e], b2[e]);
     row.store(static_cast<T*>(A.z) + (there ? i * W : 0), x, there);
@@ -607,10 +608,10 @@ __global__ void __launch_bounds__(kNormBwdResident<T, NV>) norm_bwd_kernel(const
         for (int e = 0; e < E; ++e) g[e] = g1;
       }
       // f becomes nf, x becomes nr
-      const float inv_f = row.normalise(f, LAYER, A.eps, sum);
+      const float inv_f = row.normalise(f, there, LAYER, A.eps, sum);
 #pragma unroll
       for (int e = 0; e < E; ++e) x[e] = fmaf(g[e], fmaf(f[e], s1[e], b1[e]), x[e]);
-      const float inv_r = row.normalise(x, LAYER, A.eps, sum);
+      const float inv_r = row.normalise(x, there, LAYER, A.eps, sum);
       ring.take(row, stage, 2, i, there, a);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
