@@ -10,7 +10,7 @@ the determinants turns the tokens of the occupied sites into the orbitals that `
 
 float32 and bfloat16; statistics, sums and softmax are float32, and every result is rounded
 once. Gradients go through torch autograd and are summed in a fixed order (two runs give the
-same bits). There is no CPU path and, as in the rest of the package, no fallback. None of this
+same bits); tangents (forward mode) and ``torch.func`` transforms are refused. There is no CPU path and, as in the rest of the package, no fallback. None of this
 has a counterpart in the reference, whose caller brings the network.
 """
 
@@ -19,6 +19,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -58,6 +59,22 @@ def _call_with_workspace(fn, size, device, args):
 
 
 # ------------------------------------------------------------------ checks
+def _refuse_transforms(**tensors):
+    """A tangent would be dropped without a word, and a transform's wrapper has no storage to read."""
+    level = forward_ad._current_level
+    if level < 0 and torch._C._functorch.peek_interpreter_stack() is None:
+        return
+    for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor):
+            continue
+        if torch._C._functorch.is_functorch_wrapped_tensor(t):
+            raise NotImplementedError(f"{name} is inside a torch.func transform (vmap, jvp, grad): the attention-block "
+                                      "operators support reverse-mode autograd only")
+        if level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} carries a tangent: the attention-block operators have no forward-mode "
+                                      "derivative")
+
+
 def _tensor(t, name, like=None):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor, got {type(t).__name__}")
@@ -229,6 +246,8 @@ def residual_norm(x, f, post_weight, pre_weight, *, post_bias=None, pre_bias=Non
     to ``x``: an entry each, one per row (..., 1), a vector per sample (batch, 1, width)) multiply
     the normed branch. All of one dtype; differentiable in every tensor. z is formed from the
     unrounded r."""
+    _refuse_transforms(x=x, f=f, post_weight=post_weight, pre_weight=pre_weight, post_bias=post_bias, pre_bias=pre_bias,
+                       gate=gate, scale=scale)
     x = _tensor(x, "x")
     if kind not in ("rms", "layer"):
         raise ValueError(f"kind must be 'rms' or 'layer', got {kind!r}")
@@ -302,6 +321,7 @@ def position_bias(table, q_pos, k_pos=None, *, max_distance=128, bidirectional=T
     (<= 2048; all longer distances share the last one); ``bidirectional`` gives half of the table to
     each sign, otherwise keys after the query share bucket 0. ``q_pos`` and ``k_pos`` (default:
     q_pos) are integer tensors within +-2**29, in any order. Differentiable in ``table``."""
+    _refuse_transforms(table=table, q_pos=q_pos, k_pos=k_pos)
     table = _tensor(table, "table")
     if table.dim() != 2:
         raise ValueError(f"table must have shape (heads, num_buckets), got {tuple(table.shape)}")
@@ -416,6 +436,7 @@ def biased_attention(q, k, v, table=None, *, q_pos=None, k_pos=None, key_mask=No
 
     Differentiable in q, k, v and table; under ``torch.no_grad()`` nothing is kept. Few queries
     (one new token) split the keys over the device and join the parts."""
+    _refuse_transforms(q=q, k=k, v=v, table=table, q_pos=q_pos, k_pos=k_pos, key_mask=key_mask)
     q = _tensor(q, "q")
     for name, t in (("k", k), ("v", v)):
         _tensor(t, name, q)
