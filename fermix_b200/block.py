@@ -128,11 +128,12 @@ def _positions(pos, length, batch, device, name):
         raise ValueError(f"{name} must be on {device}, got {pos.device}")
     if tuple(pos.shape) not in ((length,), (batch, length)):
         raise ValueError(f"{name} must have shape ({length},) or ({batch}, {length}), got {tuple(pos.shape)}")
-    if pos.dtype != torch.int32:
-        pos = pos.to(torch.int32)
-    if pos.shape[-1] > 1 and pos.stride(-1) != 1:
-        pos = pos.contiguous()
-    return pos
+    return _line(pos if pos.dtype == torch.int32 else pos.to(torch.int32))
+
+
+def _line(t):
+    """t (positions, a mask) with the entries of a row next to each other."""
+    return t if t is None or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
 def _batch_stride(pos):
@@ -161,9 +162,10 @@ class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_r, grad_z):
-        saved = ctx.saved_tensors
         if grad_r is None and grad_z is None:
             return (None,) * 11
+        # one that was put elsewhere and back (saved-tensor hooks) may have other strides
+        saved = tuple(None if t is None else t.contiguous() for t in ctx.saved_tensors)
         x = saved[0]
         a = _norm_args(*saved, *ctx.rest)
         grads = [None if t is None else torch.empty_like(t) for t in saved]
@@ -289,11 +291,14 @@ class _PositionBias(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         a = _lib.BiasArgs.from_buffer_copy(ctx.args)  # the graph may be run again, from another thread too
-        q_pos, k_pos = ctx.saved_tensors  # alive until the launches are queued
+        # alive until the launches are queued; one that was put elsewhere and back (saved-tensor hooks) may
+        # have other strides
+        q_pos, k_pos = (_line(t) for t in ctx.saved_tensors)
         grad = grad.contiguous()
         dtable = torch.empty(ctx.table[0], dtype=ctx.table[1], device=grad.device)
         a.grad, a.dtable = grad.data_ptr(), dtable.data_ptr()
         a.buckets.q_pos, a.buckets.k_pos = q_pos.data_ptr(), k_pos.data_ptr()
+        a.buckets.q_pos_stride, a.buckets.k_pos_stride = _batch_stride(q_pos), _batch_stride(k_pos)
         L = _lib.lib()
         _call_with_workspace(L.fermix_position_bias_grad, L.fermix_position_bias_grad_workspace_bytes, grad.device, a)
         return dtable, None, None, None, None, None
@@ -394,6 +399,9 @@ class _BiasedAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, table, out, lse, q_pos, k_pos, key_mask = ctx.saved_tensors
+        q, k, v, out, lse = _rows(q), _rows(k), _rows(v), _rows(out), lse.contiguous()
+        table = None if table is None else table.contiguous()
+        q_pos, k_pos, key_mask = _line(q_pos), _line(k_pos), _line(key_mask)
         a = _lib.AttnArgs.from_buffer_copy(ctx.args)  # the graph may be run again, from another thread too
         # a saved tensor may have been put elsewhere and back (saved-tensor hooks)
         a.q, a.k, a.v, a.table, a.out, a.lse, a.lse_low = (q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(table),
@@ -464,8 +472,7 @@ def biased_attention(q, k, v, table=None, *, q_pos=None, k_pos=None, key_mask=No
         if tuple(key_mask.shape) != (batch, k_len) or key_mask.device != q.device:
             raise ValueError(f"key_mask must have shape ({batch}, {k_len}) on {q.device}, got "
                              f"{tuple(key_mask.shape)} on {key_mask.device}")
-        if k_len > 1 and key_mask.stride(1) != 1:
-            key_mask = key_mask.contiguous()
+        key_mask = _line(key_mask)
     rest = (q_pos, k_pos, key_mask, bool(causal), float(dim**-0.5 if scale is None else scale), max_distance,
             bool(bidirectional))
     q, k, v = _rows(q), _rows(k), _rows(v)
