@@ -7,14 +7,6 @@ namespace fxh {
 
 constexpr int64_t kMaxGrid = INT32_MAX;
 
-template <typename K>
-int raise_smem(K kern, size_t smem) {
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return FX_ERR_CUDA;
-  return FX_OK;
-}
-
 // ---- launch_attn_tc.cu: tcgen05 kernels
 // A.splits parts of the keys, more than one: joined by attn_join_kernel.
 int launch_attn_tc_fwd(cudaStream_t s, const AttnArgs& A, bool is_f32, bool aligned);

@@ -26,4 +26,18 @@ inline BucketArgs make_buckets(const fx_buckets& b) {
   return B;
 }
 
+// The kernel's limit of shared memory for a launch of `smem` bytes: `most`, the same in every call,
+// so that a call of one thread does not lower it between another's and its launch. 48 KB, the kernel's own
+// shared memory (up to 4 KB) among them, need none.
+template <typename K>
+int raise_smem(K kern, size_t smem, size_t most) {
+  if (smem > most) return FX_ERR_SHAPE;
+  if (smem > 44 * 1024 &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess)
+    return FX_ERR_CUDA;
+  return FX_OK;
+}
+
+constexpr size_t kMaxSpan = 2 * FX_BUCKET_MAX_EDGE + 1;  // distances that a table by distance holds, at most
+
 }  // namespace fxh

@@ -97,6 +97,7 @@ int lanes_of(const fx_attn_args* a) {
 }
 
 // Query heads whose distances a block of the fragment kernel holds: its rows are of that many at most.
+constexpr int decode_lut_most(bool wide) { return wide ? 8192 : 4096; }  // their entries
 int decode_heads(int64_t shared) { return (int)(shared < kDecodeRows ? shared : kDecodeRows); }
 int64_t decode_chunks(const fx_attn_args* a) {
   return (a->heads / a->kv_heads * a->q_len + kDecodeRows - 1) / kDecodeRows;
@@ -116,7 +117,7 @@ Kind kind_of(const fx_attn_args* a) {
   const bool wide = a->dim > 64;
   if (a->dtype == FX_F32) return a->q_len <= (wide ? 8 : 4) ? ROWS : TC;
   const bool fits = !a->table || decode_heads(a->heads / a->kv_heads) * (2 * make_buckets(a->buckets).reach + 1) <=
-                                     (wide ? 8192 : 4096);
+                                     decode_lut_most(wide);
   return fits && a->q_len <= (wide ? 8 : 16) ? DECODE : TC;
 }
 
@@ -168,10 +169,11 @@ template <int LPK, bool VL>
 int launch_fwd(cudaStream_t s, const AttnArgs& A) {
   constexpr int NE = 4, GROUPS = kRowsThreads / LPK;
   const size_t lut = A.table ? (size_t)kRC * (2 * A.buckets.reach + 1) * 4 : 0;
-  const size_t join = (size_t)GROUPS * kRC * (2 + LPK * NE) * 4;
+  constexpr size_t join = (size_t)GROUPS * kRC * (2 + LPK * NE) * 4;
   const size_t smem = lut > join ? lut : join;
+  constexpr size_t lut_most = kRC * kMaxSpan * 4, most = lut_most > join ? lut_most : join;
   auto kern = attn_rows_kernel<float, LPK, VL, kRC>;
-  if (raise_smem(kern, smem)) return FX_ERR_CUDA;
+  if (raise_smem(kern, smem, most)) return FX_ERR_CUDA;
   const int64_t rows = (int64_t)(A.H / A.Hk) * A.Lq;
   const int64_t blocks = (rows + kRC - 1) / kRC * A.B * A.Hk * A.splits;
   if (blocks > kMaxGrid) return FX_ERR_SHAPE;
@@ -188,7 +190,7 @@ int launch_decode(cudaStream_t s, const AttnArgs& A) {
                 kDecodeStages * 8 * DB * kDecodeThreads * 16);
   const size_t smem = ring + lut;
   auto kern = attn_decode_kernel<DB, VEC>;
-  if (raise_smem(kern, smem)) return FX_ERR_CUDA;
+  if (raise_smem(kern, smem, ring + decode_lut_most(DB > 1) * 4)) return FX_ERR_CUDA;
   const int64_t chunks = ((int64_t)(A.H / A.Hk) * A.Lq + kDecodeRows - 1) / kDecodeRows;
   const int64_t blocks = (int64_t)A.B * A.Hk * chunks * A.splits;
   if (blocks > kMaxGrid) return FX_ERR_SHAPE;
@@ -200,13 +202,14 @@ int launch_decode(cudaStream_t s, const AttnArgs& A) {
 template <typename T, int LPK, bool VL>
 int launch_bwd(cudaStream_t s, const AttnArgs& A) {
   constexpr int NE = 16 / sizeof(T), GROUPS = kRowsThreads / LPK;
-  const size_t join = (size_t)GROUPS * kRC * LPK * NE * 4;
+  constexpr size_t join = (size_t)GROUPS * kRC * LPK * NE * 4;
   const size_t hist = A.table ? (size_t)GROUPS * kRC * A.buckets.num_buckets * 8 : 0;
   const size_t smem = hist > join ? hist : join;
+  constexpr size_t hist_most = (size_t)GROUPS * kRC * FX_BUCKET_MAX * 8, most = hist_most > join ? hist_most : join;
   const int64_t qrows = (int64_t)(A.H / A.Hk) * A.Lq;
   auto kq = attn_rows_grad_kernel<T, LPK, VL, kRC, false>;
   auto kk = attn_rows_grad_kernel<T, LPK, VL, kRC, true>;
-  if (raise_smem(kq, smem) || raise_smem(kk, join)) return FX_ERR_CUDA;
+  if (raise_smem(kq, smem, most) || raise_smem(kk, join, join)) return FX_ERR_CUDA;
   const int64_t qblocks = (qrows + kRC - 1) / kRC * A.B * A.Hk, kblocks = (A.Lk + kRC - 1) / kRC * A.B * A.Hk;
   if (qblocks > kMaxGrid || kblocks > kMaxGrid || (int64_t)A.B * A.H * A.Lq > kMaxGrid) return FX_ERR_SHAPE;
   if (A.Lq > 0) {

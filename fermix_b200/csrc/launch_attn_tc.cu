@@ -67,7 +67,7 @@ int fwd(cudaStream_t s, const AttnArgs& A) {
   }
   const size_t smem = S::kTileBytes + 1024 + (A.table ? (2 * A.buckets.reach + 1) * sizeof(float) : 0);
   auto kern = tc::attn_fwd_kernel<T, NS, QT, BN, L, ST, LOAD>;
-  if (raise_smem(kern, smem)) return FX_ERR_CUDA;
+  if (raise_smem(kern, smem, S::kTileBytes + 1024 + kMaxSpan * sizeof(float))) return FX_ERR_CUDA;
   const int64_t blocks = (A.Lq + 128 * QT - 1) / (128 * QT) * A.H * A.B * A.splits;
   if (blocks > kMaxGrid) return FX_ERR_SHAPE;
   kern<<<(unsigned)blocks, S::kThreads, smem, s>>>(A, M);
@@ -125,7 +125,7 @@ int bwd(cudaStream_t s, const AttnArgs& A) {
     using S = tc::DkvShape<NS, L, ST>;
     auto kern = tc::attn_dkv_kernel<T, NS, L, ST, LOAD>;
     const size_t smem = S::kTileBytes + 1024 + span * sizeof(float);
-    if (raise_smem(kern, smem)) return FX_ERR_CUDA;
+    if (raise_smem(kern, smem, S::kTileBytes + 1024 + kMaxSpan * sizeof(float))) return FX_ERR_CUDA;
     tc::TmaMaps M = rows64;
     M.m[tc::MAP_K] = rows128.m[tc::MAP_K];
     M.m[tc::MAP_V] = rows128.m[tc::MAP_V];
@@ -142,13 +142,14 @@ int bwd(cudaStream_t s, const AttnArgs& A) {
     // buckets of a launch: up to kWindow, fewer where the tiles and the distances' table are large
     const DevInfo* D = dev_info();
     if (!D) return FX_ERR_DEVICE;
-    const int64_t room = ((int64_t)D->smem_optin - 4096 - S::kTileBytes - span * (int64_t)sizeof(int2)) / 1024;
+    const int64_t most = (int64_t)D->smem_optin - 3072;  // beside the kernel's own shared memory
+    const int64_t room = (most - 1024 - S::kTileBytes - span * (int64_t)sizeof(int2)) / 1024;
     const int window = room < tc::kWindow ? (int)room : tc::kWindow;
     int w0 = 0;
     do {
       const int wn = nb - w0 < window ? nb - w0 : window;
       const size_t smem = S::kTileBytes + 1024 + (size_t)wn * 1024 + span * sizeof(int2);
-      if (raise_smem(kern, smem)) return FX_ERR_CUDA;
+      if (raise_smem(kern, smem, most)) return FX_ERR_CUDA;
       kern<<<(unsigned)qblocks, S::kThreads, smem, s>>>(A, M, w0, wn);
       if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
       w0 += window;

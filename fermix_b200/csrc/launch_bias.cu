@@ -50,14 +50,13 @@ BiasArgs make(const fx_bias_args* a) {
   return A;
 }
 
-size_t lut_bytes(const BiasArgs& A) { return (size_t)(2 * A.buckets.reach + 1 + 7) / 8 * 8 * 4; }
+constexpr size_t lut_size(int reach) { return (size_t)(2 * reach + 1 + 7) / 8 * 8 * 4; }
 
 template <typename T, int VEC>
 int launch(cudaStream_t s, const BiasArgs& A, int64_t blocks, bool grad) {
-  const size_t smem = lut_bytes(A) + (grad ? (size_t)A.buckets.num_buckets * kBiasThreads * 4 : 0);
+  const size_t smem = lut_size(A.buckets.reach) + (grad ? (size_t)A.buckets.num_buckets * kBiasThreads * 4 : 0);
   if (grad) {
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(bias_bwd_kernel<T, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)smem) != cudaSuccess)
+    if (raise_smem(bias_bwd_kernel<T, VEC>, smem, lut_size(FX_BUCKET_MAX_EDGE) + (size_t)FX_BUCKET_MAX * kBiasThreads * 4))
       return FX_ERR_CUDA;
     bias_bwd_kernel<T, VEC><<<(unsigned)blocks, kBiasThreads, smem, s>>>(A);
   } else {

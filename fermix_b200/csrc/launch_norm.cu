@@ -1,5 +1,5 @@
 // The gated residual with its norms (residual_norm.cuh): checks, launch shapes, workspace.
-#include "dispatch.cuh"
+#include "block_host.cuh"
 #include "residual_norm.cuh"
 
 namespace {
@@ -100,15 +100,16 @@ bool aligned(const fx_norm_args* a) {
 
 template <typename T, int NV, bool ALIGNED, bool WIDE>
 int launch(cudaStream_t s, const NormArgs& A, const Shape& h, int grid, bool grad) {
-  const size_t ring = (size_t)h.threads * (grad ? NormRing<T, NV, ALIGNED, WIDE, 5>::kThreadBytes
-                                                : NormRing<T, NV, ALIGNED, WIDE, 3>::kThreadBytes);
-  const size_t sums = grad && !WIDE ? (size_t)(kNormThreads / 32) * A.W * sizeof(float) : 0;
+  const size_t slots = grad ? NormRing<T, NV, ALIGNED, WIDE, 5>::kThreadBytes : NormRing<T, NV, ALIGNED, WIDE, 3>::kThreadBytes;
+  const size_t sums = grad && !WIDE ? (size_t)(kNormThreads / 32) * sizeof(float) : 0;  // an entry of the width
+  const size_t smem = h.threads * slots + A.W * sums;
+  // a row of up to 512 threads, or of up to a warp's chunks in a block of kNormThreads
+  const size_t most = WIDE ? 512 * slots : kNormThreads * slots + 32 * (16 / sizeof(T)) * sums;
   auto kern = !grad     ? norm_fwd_kernel<T, NV, ALIGNED, WIDE>
               : A.layer ? norm_bwd_kernel<T, NV, ALIGNED, WIDE, true>
                         : norm_bwd_kernel<T, NV, ALIGNED, WIDE, false>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(ring + sums)) != cudaSuccess)
-    return FX_ERR_CUDA;
-  kern<<<grid, h.threads, ring + sums, s>>>(A);
+  if (raise_smem(kern, smem, most)) return FX_ERR_CUDA;
+  kern<<<grid, h.threads, smem, s>>>(A);
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
