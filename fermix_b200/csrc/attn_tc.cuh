@@ -192,9 +192,10 @@ __device__ __forceinline__ void wait(uint64_t* m, uint32_t parity, volatile int*
 __device__ __forceinline__ void named_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
-// After a wait that ran out no more copies are asked for, and those of the last ST of n tiles (and
-// the tensor instructions) are waited for, with a bound of their own, so that nothing is under way
-// when the block ends.
+// After a wait that ran out no more copies are asked for. The threads that asked for the copies and the
+// tensor instructions wait for the last of them (of the last ST of n tiles) before they go, with a
+// bound of their own and whatever the flag says: another thread's wait may run out after they have
+// looked at it, and nothing may be under way when the block ends and its TMEM is freed.
 constexpr uint32_t kDrainPolls = 1u << 20;
 template <int ST>
 __device__ __forceinline__ void drain(uint64_t (&bar)[ST], int64_t n) {
@@ -862,10 +863,8 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
           }
         }
       }
-      if (abort_flag) {  // nothing may be in flight when the TMEM is freed
-        mma_commit(&done);
-        mbar_wait(&done, 0, kDrainPolls);
-      }
+      mma_commit(&done);
+      mbar_wait(&done, 0, kDrainPolls);
     }
   } else {
     // -------------------------------------------------------- loads
@@ -899,11 +898,9 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
             tma_tile<L>(sV + st * S::kKV, M, MAP_V, BN, (int64_t)(first + j) * BN, hk, b, &vraw[st]);
           }
         }
-        if (abort_flag) {
-          mbar_wait(&qraw, 0, kDrainPolls);
-          drain(kraw, keys_asked);
-          drain(vraw, values_asked);
-        }
+        mbar_wait(&qraw, 0, kDrainPolls);
+        drain(kraw, keys_asked);
+        drain(vraw, values_asked);
       } else {
         for (int j = 0; j < tiles; ++j) {
           const int st = j % ST;

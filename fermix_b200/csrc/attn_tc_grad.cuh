@@ -330,10 +330,8 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
         mma_commit(&empty[st]);
       }
       mma_commit(&sfull);
-      if (abort_flag) {  // nothing may be in flight when the TMEM is freed
-        mma_commit(&done);
-        mbar_wait(&done, 0, kDrainPolls);
-      }
+      mma_commit(&done);
+      mbar_wait(&done, 0, kDrainPolls);
     }
   } else {
     const int t = tid - 288, w = t >> 5;
@@ -368,10 +366,8 @@ __global__ void __launch_bounds__(DkvShape<NS, L, ST>::kThreads, DkvShape<NS, L,
           __syncwarp();
           if (lane == 0) arrive(&loaded[st]);
         }
-        if (abort_flag) {
-          mbar_wait(&own, 0, kDrainPolls);
-          drain(loaded, asked);
-        }
+        mbar_wait(&own, 0, kDrainPolls);
+        drain(loaded, asked);
       } else {
         for (int64_t it = 0; it < tiles; ++it) {
           const int st = (int)(it % ST);
@@ -752,10 +748,8 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
         mma_commit(&empty[st]);
       }
       mma_commit(&sfull);
-      if (abort_flag) {  // nothing may be in flight when the TMEM is freed
-        mma_commit(&done);
-        mbar_wait(&done, 0, kDrainPolls);
-      }
+      mma_commit(&done);
+      mbar_wait(&done, 0, kDrainPolls);
     }
   } else {
     const int t = tid - 160, w = t >> 5;
@@ -782,10 +776,8 @@ __global__ void __launch_bounds__(DqShape<NS, L, ST>::kThreads, DqShape<NS, L, S
           __syncwarp();
           if (lane == 0) arrive(&loaded[st]);
         }
-        if (abort_flag) {
-          mbar_wait(&own, 0, kDrainPolls);
-          drain(loaded, asked);
-        }
+        mbar_wait(&own, 0, kDrainPolls);
+        drain(loaded, asked);
       } else {
         for (int j = 0; j < tiles; ++j) {
           const int st = j % ST;
