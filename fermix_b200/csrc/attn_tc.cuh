@@ -777,7 +777,8 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
         p[1] = broken ? NAN : l;
       }
     } else {
-      const float inv = broken ? NAN : l == 0.f ? 0.f : 1.f / l;
+      const bool empty = l == 0.f && !broken;
+      const float inv = broken ? NAN : 1.f / l;
       T* out = static_cast<T*>(A.out) + b * A.os[0] + h * A.os[1] + i * A.os[2];
       constexpr int V = 16 / sizeof(T);
       const bool ovec =
@@ -807,7 +808,7 @@ __global__ void __launch_bounds__(FwdShape<NS, QT, BN, L, ST>::kThreads, FwdShap
           }
           alignas(16) T r[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) r[e] = from_f<T>(l == 0.f ? 0.f : __uint_as_float(o[e]) * inv);
+          for (int e = 0; e < 16; ++e) r[e] = from_f<T>(empty ? 0.f : __uint_as_float(o[e]) * inv);
           if (valid) {
             if (ovec) {
 #pragma unroll

@@ -64,3 +64,17 @@ def test_gradient(shape, mask, dtype):
     for x, y in zip(_grads(out, leaves, cot), want):
         assert torch.equal(x, y)
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_forward_of_rows_without_a_sum(shape, dtype):
+    """Scores that never came leave a row's sum at zero as a row without keys has it: NaN all the same."""
+    a, kw, _ = _case(shape, dtype, False)
+    a["table"] = torch.full_like(a["table"], -float("inf"))
+    with torch.no_grad(), _NoPolls():
+        out = fx.biased_attention(**a, **kw)
+        assert _lib.device_status(clear=True) == _lib.FX_ERR_TIMEOUT
+    assert torch.isnan(out).all()
+    with torch.no_grad():
+        assert (fx.biased_attention(**a, **kw) == 0).all()
