@@ -18,18 +18,26 @@
 
 namespace fx {
 
-template <typename T>
 __global__ void __launch_bounds__(kRowsThreads) attn_delta_kernel(const __grid_constant__ AttnArgs A) {
   const int lane = threadIdx.x & 31;
   const int64_t w = (int64_t)blockIdx.x * (kRowsThreads / 32) + (threadIdx.x >> 5);
   if (w >= (int64_t)A.B * A.H * A.Lq) return;
   const int64_t i = w % A.Lq, bh = w / A.Lq, h = bh % A.H, b = bh / A.H;
-  const T* o = static_cast<const T*>(A.out) + b * A.os[0] + h * A.os[1] + i * A.os[2];
-  const T* g = static_cast<const T*>(A.dout) + b * A.dos[0] + h * A.dos[1] + i * A.dos[2];
+  const float* o = static_cast<const float*>(A.out) + b * A.os[0] + h * A.os[1] + i * A.os[2];
+  const float* g = static_cast<const float*>(A.dout) + b * A.dos[0] + h * A.dos[1] + i * A.dos[2];
   float s = 0.f;
-  for (int c = lane; c < A.D; c += 32) s = fmaf(to_f(o[c]), to_f(g[c]), s);
+  for (int c = lane; c < A.D; c += 32) s = fmaf(o[c], g[c], s);
   s = lanes_sum(s, 32);
   if (lane == 0) A.delta[w] = s;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) attn_zero_kernel(const __grid_constant__ AttnArgs A) {
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x, token = n / A.D, c = n % A.D, j = token % A.Lk;
+  const int64_t bh = token / A.Lk, hk = bh % A.Hk, b = bh / A.Hk;
+  if (b >= A.B) return;
+  static_cast<T*>(A.dk)[b * A.dks[0] + hk * A.dks[1] + j * A.dks[2] + c] = from_f<T>(0.f);
+  static_cast<T*>(A.dv)[b * A.dvs[0] + hk * A.dvs[1] + j * A.dvs[2] + c] = from_f<T>(0.f);
 }
 
 // KEYS false: RC query rows against all keys, dq and the table; true: RC keys against all

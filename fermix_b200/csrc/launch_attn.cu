@@ -199,23 +199,22 @@ int launch_decode(cudaStream_t s, const AttnArgs& A) {
   return A.splits > 1 ? join_parts<bf16>(s, A) : FX_OK;
 }
 
-template <typename T, int LPK, bool VL>
+// float32 above 64 entries: 32 lanes a row.
+template <bool VL>
 int launch_bwd(cudaStream_t s, const AttnArgs& A) {
-  constexpr int NE = 16 / sizeof(T), GROUPS = kRowsThreads / LPK;
+  constexpr int LPK = 32, NE = 4, GROUPS = kRowsThreads / LPK;
   constexpr size_t join = (size_t)GROUPS * kRC * LPK * NE * 4;
   const size_t hist = A.table ? (size_t)GROUPS * kRC * A.buckets.num_buckets * 8 : 0;
   const size_t smem = hist > join ? hist : join;
   constexpr size_t hist_most = (size_t)GROUPS * kRC * FX_BUCKET_MAX * 8, most = hist_most > join ? hist_most : join;
   const int64_t qrows = (int64_t)(A.H / A.Hk) * A.Lq;
-  auto kq = attn_rows_grad_kernel<T, LPK, VL, kRC, false>;
-  auto kk = attn_rows_grad_kernel<T, LPK, VL, kRC, true>;
+  auto kq = attn_rows_grad_kernel<float, LPK, VL, kRC, false>;
+  auto kk = attn_rows_grad_kernel<float, LPK, VL, kRC, true>;
   if (raise_smem(kq, smem, most) || raise_smem(kk, join, join)) return FX_ERR_CUDA;
   const int64_t qblocks = (qrows + kRC - 1) / kRC * A.B * A.Hk, kblocks = (A.Lk + kRC - 1) / kRC * A.B * A.Hk;
   if (qblocks > kMaxGrid || kblocks > kMaxGrid || (int64_t)A.B * A.H * A.Lq > kMaxGrid) return FX_ERR_SHAPE;
-  if (A.Lq > 0) {
-    attn_delta_kernel<T><<<(unsigned)(((int64_t)A.B * A.H * A.Lq + 3) / 4), kRowsThreads, 0, s>>>(A);
-    kq<<<(unsigned)qblocks, kRowsThreads, smem, s>>>(A);
-  }
+  attn_delta_kernel<<<(unsigned)(((int64_t)A.B * A.H * A.Lq + 3) / 4), kRowsThreads, 0, s>>>(A);
+  kq<<<(unsigned)qblocks, kRowsThreads, smem, s>>>(A);
   if (A.Lk > 0) kk<<<(unsigned)kblocks, kRowsThreads, join, s>>>(A);
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
@@ -226,12 +225,13 @@ int fwd(cudaStream_t s, const AttnArgs& A, int lanes, bool vec) {
   return vec ? launch_fwd<32, true>(s, A) : launch_fwd<32, false>(s, A);
 }
 
+// Without queries dk and dv are zero.
 template <typename T>
-int bwd(cudaStream_t s, const AttnArgs& A, int lanes, bool vec) {
-  if (lanes == 8) return vec ? launch_bwd<T, 8, true>(s, A) : launch_bwd<T, 8, false>(s, A);
-  if (lanes == 16) return vec ? launch_bwd<T, 16, true>(s, A) : launch_bwd<T, 16, false>(s, A);
-  if constexpr (sizeof(T) == 4) return vec ? launch_bwd<T, 32, true>(s, A) : launch_bwd<T, 32, false>(s, A);
-  return FX_ERR_SHAPE;
+int no_queries(cudaStream_t s, const AttnArgs& A) {
+  const int64_t blocks = ((int64_t)A.B * A.Hk * A.Lk * A.D + 255) / 256;
+  if (blocks > kMaxGrid) return FX_ERR_SHAPE;
+  if (blocks > 0) attn_zero_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(A);
+  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
 // The tensor-core gradient holds both sides of a block in shared memory: float32's three parts
@@ -325,10 +325,10 @@ int fermix_biased_attention_grad(void* stream, const fx_attn_args* a, void* ws, 
   A.lut = reinterpret_cast<float*>(p + w.lut);
   A.dpart = reinterpret_cast<float*>(p + w.dpart);
   const bool vec = aligned(a, true), f32 = a->dtype == FX_F32;
-  // without queries dk and dv are zero: the rows kernels write them
-  const int st = use_tc_grad(a) && !no_rows(a) ? launch_attn_tc_bwd(s, A, f32, vec)
-                 : f32                         ? bwd<float>(s, A, lanes_of(a), vec)
-                                               : bwd<bf16>(s, A, lanes_of(a), vec);
+  const int st = no_rows(a)       ? (f32 ? no_queries<float>(s, A) : no_queries<bf16>(s, A))
+                 : use_tc_grad(a) ? launch_attn_tc_bwd(s, A, f32, vec)
+                 : vec            ? launch_bwd<true>(s, A)
+                                  : launch_bwd<false>(s, A);
   if (st || !a->table) return st;
   const int nb = a->buckets.num_buckets;
   const dim3 grid((nb + 31) / 32, A.H);

@@ -116,7 +116,7 @@ int bwd(cudaStream_t s, const AttnArgs& A) {
   }
   constexpr bool VEC = LOAD != LOAD_ENTRIES;
   const int lanes = (A.D * (int)sizeof(T) + 15) / 16;
-  int st = lanes <= 8 ? prep<T, 8, VEC>(s, A) : lanes <= 16 ? prep<T, 16, VEC>(s, A) : prep<T, 32, VEC>(s, A);
+  int st = lanes <= 8 ? prep<T, 8, VEC>(s, A) : prep<T, 16, VEC>(s, A);  // 16 at most
   if (st) return st;
   const int span = A.table ? 2 * A.buckets.reach + 1 : 0;
   const int64_t kblocks = (A.Lk + 127) / 128 * A.Hk * A.B, qblocks = (A.Lq + 127) / 128 * A.H * A.B;
