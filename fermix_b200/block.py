@@ -59,11 +59,14 @@ def _call_with_workspace(fn, size, device, args):
 
 
 # ------------------------------------------------------------------ checks
+def _transformed(peek=torch._C._functorch.peek_interpreter_stack):
+    """Whether a forward-mode level or a torch.func transform is open."""
+    return forward_ad._current_level >= 0 or peek() is not None
+
+
 def _refuse_transforms(**tensors):
     """A tangent would be dropped without a word, and a transform's wrapper has no storage to read."""
     level = forward_ad._current_level
-    if level < 0 and torch._C._functorch.peek_interpreter_stack() is None:
-        return
     for name, t in tensors.items():
         if not isinstance(t, torch.Tensor):
             continue
@@ -133,7 +136,7 @@ def _positions(pos, length, batch, device, name):
 
 def _line(t):
     """t (positions, a mask) with the entries of a row next to each other."""
-    return t if t is None or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
 def _batch_stride(pos):
@@ -165,7 +168,7 @@ class _ResidualNorm(torch.autograd.Function):
         if grad_r is None and grad_z is None:
             return (None,) * 11
         # one that was put elsewhere and back (saved-tensor hooks) may have other strides
-        saved = tuple(None if t is None else t.contiguous() for t in ctx.saved_tensors)
+        saved = [None if t is None else t.contiguous() for t in ctx.saved_tensors]
         x = saved[0]
         a = _norm_args(*saved, *ctx.rest)
         grads = [None if t is None else torch.empty_like(t) for t in saved]
@@ -248,8 +251,9 @@ def residual_norm(x, f, post_weight, pre_weight, *, post_bias=None, pre_bias=Non
     to ``x``: an entry each, one per row (..., 1), a vector per sample (batch, 1, width)) multiply
     the normed branch. All of one dtype; differentiable in every tensor. z is formed from the
     unrounded r."""
-    _refuse_transforms(x=x, f=f, post_weight=post_weight, pre_weight=pre_weight, post_bias=post_bias, pre_bias=pre_bias,
-                       gate=gate, scale=scale)
+    if _transformed():
+        _refuse_transforms(x=x, f=f, post_weight=post_weight, pre_weight=pre_weight, post_bias=post_bias,
+                           pre_bias=pre_bias, gate=gate, scale=scale)
     x = _tensor(x, "x")
     if kind not in ("rms", "layer"):
         raise ValueError(f"kind must be 'rms' or 'layer', got {kind!r}")
@@ -293,7 +297,8 @@ class _PositionBias(torch.autograd.Function):
         a = _lib.BiasArgs.from_buffer_copy(ctx.args)  # the graph may be run again, from another thread too
         # alive until the launches are queued; one that was put elsewhere and back (saved-tensor hooks) may
         # have other strides
-        q_pos, k_pos = (_line(t) for t in ctx.saved_tensors)
+        q_pos, k_pos = ctx.saved_tensors
+        q_pos, k_pos = _line(q_pos), _line(k_pos)
         grad = grad.contiguous()
         dtable = torch.empty(ctx.table[0], dtype=ctx.table[1], device=grad.device)
         a.grad, a.dtable = grad.data_ptr(), dtable.data_ptr()
@@ -326,7 +331,8 @@ def position_bias(table, q_pos, k_pos=None, *, max_distance=128, bidirectional=T
     (<= 2048; all longer distances share the last one); ``bidirectional`` gives half of the table to
     each sign, otherwise keys after the query share bucket 0. ``q_pos`` and ``k_pos`` (default:
     q_pos) are integer tensors within +-2**29, in any order. Differentiable in ``table``."""
-    _refuse_transforms(table=table, q_pos=q_pos, k_pos=k_pos)
+    if _transformed():
+        _refuse_transforms(table=table, q_pos=q_pos, k_pos=k_pos)
     table = _tensor(table, "table")
     if table.dim() != 2:
         raise ValueError(f"table must have shape (heads, num_buckets), got {tuple(table.shape)}")
@@ -352,6 +358,12 @@ def _strides(t):
     return t.stride()[:3]
 
 
+def _lse_parts(lse):
+    """The addresses of lse[0] and lse[1] (contiguous float32)."""
+    p = lse.data_ptr()
+    return p, p + 2 * lse.numel()
+
+
 def _attn_args(q, k, v, table, out, lse, q_pos, k_pos, key_mask, causal, scale, max_distance, bidirectional):
     a = _lib.AttnArgs()
     a.dtype, a.causal = _KIND[q.dtype], int(causal)
@@ -370,7 +382,7 @@ def _attn_args(q, k, v, table, out, lse, q_pos, k_pos, key_mask, causal, scale, 
         a.key_mask, a.mask_stride = _ptr(key_mask), key_mask.stride(0)
     a.out = _ptr(out)
     if lse is not None:
-        a.lse, a.lse_low = lse.data_ptr(), lse[1].data_ptr()
+        a.lse, a.lse_low = _lse_parts(lse)
     a.out_stride[:] = _strides(out)
     return a
 
@@ -399,13 +411,13 @@ class _BiasedAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, table, out, lse, q_pos, k_pos, key_mask = ctx.saved_tensors
+        # a saved tensor may have been put elsewhere and back (saved-tensor hooks), with other strides
         q, k, v, out, lse = _rows(q), _rows(k), _rows(v), _rows(out), lse.contiguous()
         table = None if table is None else table.contiguous()
         q_pos, k_pos, key_mask = _line(q_pos), _line(k_pos), _line(key_mask)
         a = _lib.AttnArgs.from_buffer_copy(ctx.args)  # the graph may be run again, from another thread too
-        # a saved tensor may have been put elsewhere and back (saved-tensor hooks)
-        a.q, a.k, a.v, a.table, a.out, a.lse, a.lse_low = (q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(table),
-                                                           out.data_ptr(), lse.data_ptr(), lse[1].data_ptr())
+        a.q, a.k, a.v, a.table, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(table), out.data_ptr()
+        a.lse, a.lse_low = _lse_parts(lse)
         a.q_stride[:], a.k_stride[:], a.v_stride[:], a.out_stride[:] = (_strides(q), _strides(k), _strides(v),
                                                                         _strides(out))
         a.buckets.q_pos, a.buckets.k_pos, a.key_mask = _ptr(q_pos), _ptr(k_pos), _ptr(key_mask)
@@ -444,7 +456,8 @@ def biased_attention(q, k, v, table=None, *, q_pos=None, k_pos=None, key_mask=No
 
     Differentiable in q, k, v and table; under ``torch.no_grad()`` nothing is kept. Few queries
     (one new token) split the keys over the device and join the parts."""
-    _refuse_transforms(q=q, k=k, v=v, table=table, q_pos=q_pos, k_pos=k_pos, key_mask=key_mask)
+    if _transformed():
+        _refuse_transforms(q=q, k=k, v=v, table=table, q_pos=q_pos, k_pos=k_pos, key_mask=key_mask)
     q = _tensor(q, "q")
     for name, t in (("k", k), ("v", v)):
         _tensor(t, name, q)
