@@ -451,8 +451,10 @@ def biased_attention(q, k, v, table=None, *, q_pos=None, k_pos=None, key_mask=No
     :func:`position_bias`; None: no bias. ``k_pos`` defaults to 0, 1, ..., and ``q_pos`` to the last
     q_len of them (a new token attends from the end of the cache); integer tensors (length,) or
     (batch, length), within +-2**29. ``key_mask`` (batch, k_len) bool: False leaves a key out,
-    whatever its k and v hold. ``causal`` leaves out keys with k_pos > q_pos. A query without any
-    key gives 0 and has no gradient. ``scale`` defaults to dim ** -0.5.
+    whatever its k and v hold. ``causal`` leaves out keys with k_pos > q_pos, as a table entry of -inf does
+    those of its bucket; what such keys hold has to be finite (0 times NaN). A query without any
+    key gives 0 and has no gradient. ``scale`` defaults to dim ** -0.5. A live infinity gives NaN in the
+    rows that read it.
 
     Differentiable in q, k, v and table; under ``torch.no_grad()`` nothing is kept. Few queries
     (one new token) split the keys over the device and join the parts."""

@@ -13,8 +13,16 @@
 //
 // A lane copies the pieces it will use into a ring of its own in shared memory (cp.async), three
 // steps ahead: 96 KB a block on the way without registers (with the loads in registers, one step
-// at a time, 217 us for 64 key heads of 65536 keys, three quarters live; with the ring 183 us,
-// 4.4 TB/s of the live keys' bytes, 0.67 of a copy's rate).
+// at a time, 217 us for 64 key heads of 65536 keys, three quarters live; with the ring 190 us,
+// 4.2 TB/s of the live keys' bytes, 0.65 of a copy's rate; all live 4.5 TB/s). What is left is not the
+// ring's depth, two blocks have 130 KB of an SM on the way: caches of different live lengths leave SMs idle
+// at the end (233 to 339 thousand cycles of work, 295 on average), and while they work 16 warps use
+// half of the issue slots and wait for fixed latencies (1.8 of 7 an instruction), shared memory (1.2) and
+// the positions' and mask's loads (0.6).
+//
+// The probabilities are rounded to bfloat16 for the second product, the tensor instruction's operand
+// type, and are summed unrounded: each entry of the output takes up to 2^-9 of the values' size, as much as the
+// rounding of the output itself.
 #pragma once
 #include "attn_rows.cuh"
 

@@ -8,8 +8,12 @@
 // delta from the rounded output would leave its rounding there, so the table's gradient keeps
 // a = sum p (do . v) and b = sum p of each row and bucket, and takes sum_i (a - b sum a / sum b).
 //
-// Bound: FMA instructions; this is the float32 path above 64 entries, whose three parts of both sides do
-// not fit shared memory, and the gradient where there are no queries.
+// This is the float32 path above 64 entries, whose three parts of both sides do not fit shared memory.
+// Bound: instructions, and few of them products: for every pair a warp walks the edges of the buckets
+// (15 comparisons for 32 buckets), reads the table from global memory and takes part in ten
+// shuffles beside 12 to 16 FMAs; 60 % of the issue slots are used. 8 x 4 heads of 512 x 512, dim 128: 2.6 ms for
+// dk and dv, 2.6 ms for dq and the table, trained 5.2 ms (dim 96 the same), where the plain form in
+// library calls takes 0.86 (0.94): the one form here that is slower than that.
 //
 // Nothing is added atomically: a block owns its rows of dq (or of dk and dv, over all the
 // query heads that share the key head), and its groups' partial sums are added in order.

@@ -22,8 +22,18 @@
 // the exponentials shows: no maximum is taken on the way. Few blocks of queries split the keys over
 // blocks. Bound: the softmax's latency at two blocks an SM, what TMEM and registers allow: 0.44 of the
 // issue slots are used, warps wait for TMEM loads, fixed latencies and each other (64 x 8 heads of
-// 512 x 512, dim 64: 152 us, 229 TFLOP/s; 2 x 16 heads of 4096 x 4096, dim 128: 420 us, 654 TFLOP/s, 0.40
-// of the library's matrix rate). float32, 512 x 4 heads of 128 x 128, dim 32: 143 us.
+// 512 x 512, dim 64, three quarters of the keys live: 154 us, 167 TFLOP/s of live pairs; 2 x 16 heads of
+// 4096 x 4096, dim 128: 406 us a call, 676 TFLOP/s, 0.42 of the library's matrix rate). float32, 512 x 4
+// heads of 128 x 128, dim 32: 142 us; its forward up to 64 entries spills 40 registers' worth (152 to
+// 160 bytes a thread) at the 80 that two blocks an SM leave.
+//
+// Fewer bits, and why: in bfloat16 the probabilities are rounded to the operand type of the second
+// product (their sum is not), 2^-9 of the values' size at most, as much as the output's own rounding.
+// Its sums stay in the accumulator over all keys, which cuts off towards zero below its last bit: 1.6e-8 of
+// the sum for every 16 keys by the figure at kRest, 1e-3, half of the output's rounding, after a
+// million keys in one part. In float32 the products of parts with index sum 5 and 6 are left out (2^-24
+// of a product), the exponential is the approximate instruction (2^-22 of its value), and an
+// infinite entry, whose parts are inf - inf, gives NaN in the rows that read it.
 #pragma once
 #include <cuda.h>
 

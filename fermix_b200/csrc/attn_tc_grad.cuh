@@ -16,9 +16,19 @@
 //
 // Bound: the latency of the threads' work between the matrix instructions (TMEM loads, exponentials,
 // operands back to TMEM, in dq the histogram) at two blocks an SM: 0.41 (dkv) and 0.37 (dq) of the issue
-// slots are used, 0.16 and 0.08 of the tensor pipe. Measured: 64 x 8 heads of 512 x 512, dim 64 in bfloat16:
-// dkv 192 us, dq 226 us; causal 8 heads of 4095: 140 and 148 us; float32 512 x 4 heads of 128 x 128, dim 32:
-// 210 and 220 us.
+// slots are used, 0.16 and 0.08 of the tensor pipe. Within a block the tensor work and the threads' work
+// take turns: the next tile's scores have to wait until p and ds, which lie over this tile's, are read.
+// Measured: 64 x 8 heads of 512 x 512, dim 64 in bfloat16, three quarters of the keys live: dkv 198 us, dq
+// 230 us; causal 8 heads of 4095: 141 and 148 us; float32 512 x 4 heads of 128 x 128, dim 32: 201 and
+// 219 us (spills of 56 and 72 bytes a thread).
+//
+// Fewer bits, and why: p and ds are rounded to bfloat16 for the second products, whose operands are of that
+// type (three parts each in float32, which keep 24 bits). delta = o . do is formed from the output as
+// stored, which spares a second pass over the values: its rounding adds up to 2^-9 |o| |do| to every dp of
+// a row, so dq and dk of a row whose ds cancel (a sharp softmax over nearly equal values) carry that
+// much beside their own; the table's gradient, which sums ds over whole rows, is mended for it below.
+// Measured, of dq's norm: ds 1.7e-3, as much as the rounding of the result itself; delta 0.4 to 0.9e-3
+// from the output and as much from the forward's p; in all 2.4 to 2.6e-3, float32 throughout 1.7e-3.
 #pragma once
 #include "attn_tc.cuh"
 

@@ -14,11 +14,15 @@
 // reach into one register; the block then adds the threads' columns in order, and
 // bias_finish_kernel the blocks' partial rows in order.
 //
-// Measured: 8 heads of 4096 x 4096 in bfloat16: forward 61 us (268 MB, 4.4 TB/s), backward 113 us
-// (2.4 TB/s); 128 x 8 heads of 255 x 255 sites in float32: forward 52 us (266 MB, 5.1 TB/s), backward
-// 128 us (2.1 TB/s). The backward is bound by its histogram, a read and a write of shared memory an entry
-// in order. Joining four entries of a bucket before the update (126 and 151 us) and reading the next
-// row's distances ahead (197 and 133 us) were slower.
+// Measured: 8 heads of 4096 x 4096 in bfloat16: forward 63 us (268 MB, 4.3 TB/s), backward 112 us
+// (2.4 TB/s); 128 x 8 heads of 255 x 255 sites in float32: forward 53 us (266 MB, 5.0 TB/s), backward
+// 125 us (2.1 TB/s). What binds the backward is latency, not a pipe: in the lattice, where a thread
+// reaches the histogram in about 6 % of its rows, 36 % of the issue slots of a working SM and 15 % of the
+// shared-memory pipe are used and two thirds of a warp's waits are for its loads; blocks on the diagonal
+// do all of the histogram, and SMs work for 133 to 219 thousand cycles, 178 on average. For the sites (rows
+// of 255, so 4-byte loads; 80 registers leave 19 warps an SM) it is 50 % and 28 %, the waits spread over
+// loads, fixed latencies and the histogram. Joining four entries of a bucket before the update (126 and
+// 151 us) and reading the next row's distances ahead (197 and 133 us) were slower.
 #pragma once
 #include "block_common.cuh"
 

@@ -14,8 +14,9 @@
 // dgate = scale (post_w sum t nf + post_b sum t).
 //
 // Bound: HBM. A row is read once and held in registers by a group of TPR threads (a part of a
-// warp for narrow rows, a block for wide ones), E entries a thread, so that the statistics
-// are two-pass (mean, then centred squares) without reading again. The backward recomputes
+// warp for narrow rows, a block for wide ones), E entries a thread. The mean and the centred squares
+// come from one reduction, of the sums of v - c and (v - c)^2 about an entry c of the row, so that
+// nothing of a large mean cancels. The backward recomputes
 // nf, r and nr from x, f and gate -- the same bytes that the saved statistics and r would
 // be, and r unrounded -- and keeps the sums over rows in registers while a block walks its
 // rows; each block writes one partial row per parameter and norm_finish_kernel adds those in
@@ -23,10 +24,15 @@
 // rows are under way: a thread copies its own entries of them into a ring in shared memory
 // (cp.async), which no other thread reads, so the ring needs no barrier.
 //
-// Measured: 524288 rows of 128 in float32, a gate for each entry: forward 247 us (1.34 GB, 5.4 TB/s,
-// 0.83 of a copy's rate), backward 395 us (2.15 GB with the inputs read again, 5.4 TB/s): HBM. 31293 rows
-// of 1000 in bfloat16, centred, a gate for each group: forward 86 us (250 MB, 2.9 TB/s), backward
-// 157 us (376 MB, 2.4 TB/s): instructions, of the two norms and their reductions over a block.
+// Measured: 524288 rows of 128 in float32, a gate for each entry: forward 232 us (1.34 GB, 5.8 TB/s,
+// 0.88 of a copy's rate), backward 370 us (2.15 GB with the inputs read again, 5.8 TB/s): HBM. 31293 rows
+// of 1000 in bfloat16, centred, a gate for each group: forward 89 us (250 MB, 2.8 TB/s), backward
+// 160 us (376 MB, 2.4 TB/s): instructions, of the two norms and their reductions over a block. Rows of 999,
+// off the 16-byte boundaries: 182 us a call forward, 484 us trained, where 1000 take 90 and 250. Rows of more
+// than 512 chunks give a thread two or four, which at 128 registers spill in the backward (1.0 to 1.6 KB a
+// thread in bfloat16 and from 4096 float32 entries on): 4096 rows of 8192, trained: float32 467 us (2.6
+// TB/s of what the inputs, results and gradients take), bfloat16 353 us (1.7 TB/s), unaligned bfloat16
+// 646 us; rows of 4096: 186 and 174 us.
 #pragma once
 #include "block_common.cuh"
 
