@@ -4,8 +4,8 @@ of ChenAo-Phys/fermix (src/fermix/__init__.py:1-10) on torch CUDA tensors, compu
 hand-written sm_100a kernels behind a C ABI (include/fermix_b200.h).
 
 Public functions: :func:`slogdet`, :func:`slogpf`, :func:`det`, :func:`pf`; and, for the
-network whose orbitals they take, :func:`biased_attention`, :func:`position_bias` and
-:func:`residual_norm`.
+network whose orbitals they take, :func:`token_embedding`, :func:`fused_linear`,
+:func:`biased_attention`, :func:`position_bias`, :func:`residual_norm` and :func:`token_logprobs`.
 """
 
 from .api import (
@@ -31,6 +31,7 @@ from .api import (
     pf_planar,
 )
 from .block import biased_attention, position_bias, residual_norm
+from .tokens import fused_linear, token_embedding, token_logprobs
 
 __version__ = "0.1.0"
 __all__ = [
@@ -56,6 +57,9 @@ __all__ = [
     "biased_attention",
     "position_bias",
     "residual_norm",
+    "token_embedding",
+    "fused_linear",
+    "token_logprobs",
     "FermixFallbackWarning",
     "__version__",
 ]

@@ -17,6 +17,7 @@ FX_PREC_DEFAULT, FX_PREC_TF32X3, FX_PREC_IEEE = 0, 1, 2
 FX_OP_SLOGDET, FX_OP_SLOGPF = 0, 1
 FX_ERR_TIMEOUT = 8
 FX_WAIT_POLLS_DEFAULT = 1 << 26
+FX_EMBED_MAX_WIDTH, FX_LOGPROBS_MAX, FX_TOP_MAX = 1 << 23, 1 << 30, 32
 FX_NORM_MAX_WIDTH, FX_ATTN_MAX_DIM, FX_BUCKET_MAX, FX_BUCKET_MAX_EDGE = 8192, 128, 256, 2048
 
 # every symbol include/fermix_b200.h declares, with its ctypes signature
@@ -65,6 +66,17 @@ SIGNATURES = {
     "fermix_biased_attention_workspace_bytes": (_sz, [_vp]),
     "fermix_biased_attention_grad": (_i, [_vp, _vp, _vp, _sz]),
     "fermix_biased_attention_grad_workspace_bytes": (_sz, [_vp]),
+    # include/fermix_b200_token.h
+    "fermix_token_embedding": (_i, [_vp, _vp]),
+    "fermix_token_embedding_grad": (_i, [_vp, _vp, _vp, _sz]),
+    "fermix_token_embedding_grad_workspace_bytes": (_sz, [_vp]),
+    "fermix_linear": (_i, [_vp, _vp, _vp, _sz]),
+    "fermix_linear_workspace_bytes": (_sz, [_vp]),
+    "fermix_linear_grad": (_i, [_vp, _vp, _vp, _sz]),
+    "fermix_linear_grad_workspace_bytes": (_sz, [_vp]),
+    "fermix_token_logprobs": (_i, [_vp, _vp, _vp, _sz]),
+    "fermix_token_logprobs_workspace_bytes": (_sz, [_vp]),
+    "fermix_token_logprobs_grad": (_i, [_vp, _vp]),
     # include/fermix_b200_xla.h
     "fermix_xla_custom_call": (None, [_vp, _vp, ctypes.c_char_p, _sz]),
     "fermix_xla_last_error": (_i, [_i]),
@@ -110,6 +122,30 @@ class AttnArgs(ctypes.Structure):
                 _fields(_vp, "key_mask") + _fields(_i64, "mask_stride") + _fields(_vp, "out") +
                 _fields(_i64x3, "out_stride") + _fields(_vp, "lse dout") + _fields(_i64x3, "dout_stride") +
                 _fields(_vp, "dq dk dv dtable") + _fields(_i64x3, "dq_stride dk_stride dv_stride") + _fields(_vp, "lse_low"))
+
+
+class EmbedArgs(ctypes.Structure):
+    """fx_embed_args (include/fermix_b200_token.h)."""
+
+    _fields_ = (_fields(_i32, "dtype token_bytes") + _fields(_i64, "count rows width padding") + _fields(_i32, "has_padding") +
+                _fields(_f32, "scale") + _fields(_vp, "tokens weight out grad dweight"))
+
+
+class LinearArgs(ctypes.Structure):
+    """fx_linear_args."""
+
+    _fields_ = (_fields(_i32, "dtype activation") + _fields(_i64, "rows inner outer") +
+                _fields(_vp, "x weight bias residual") + _fields(_i64, "x_stride weight_stride residual_stride") +
+                _fields(_vp, "y slope dy") + _fields(_i64, "dy_stride") + _fields(_vp, "dx dweight dbias"))
+
+
+class LogprobsArgs(ctypes.Structure):
+    """fx_logprobs_args."""
+
+    _fields_ = (_fields(_i32, "dtype token_bytes") + _fields(_i64, "rows entries padding") + _fields(_i32, "has_padding top") +
+                _fields(_f32, "scale") + _fields(_i32, "reserved") + _fields(_vp, "logits tokens mask") +
+                _fields(_i64, "logits_stride mask_stride") +
+                _fields(_vp, "logp entropy top_logp top_index stats grad_logp grad_entropy dlogits"))
 
 
 _lib = None

@@ -1,0 +1,195 @@
+// Embedding of tokens (token_embedding.cuh): checks, launch shapes, workspace.
+#include "block_host.cuh"
+#include "token_embedding.cuh"
+
+namespace {
+
+using namespace fxh;
+
+int check(const fx_embed_args* a) {
+  if (!a) return FX_ERR_NULL;
+  if (a->dtype != FX_F32 && a->dtype != FX_BF16) return FX_ERR_DTYPE;
+  if (a->token_bytes != 1 && a->token_bytes != 2 && a->token_bytes != 4 && a->token_bytes != 8) return FX_ERR_DTYPE;
+  if (a->count < 0 || a->count >= INT32_MAX || a->rows < 1 || a->rows >= INT32_MAX || a->width < 1 ||
+      a->width > FX_EMBED_MAX_WIDTH)
+    return FX_ERR_SHAPE;
+  if (a->rows > (int64_t{1} << 60) / a->width || a->count > (int64_t{1} << 60) / a->width) return FX_ERR_SHAPE;
+  return FX_OK;
+}
+
+Tokens tokens_of(const fx_embed_args* a) { return {a->tokens, a->token_bytes, a->has_padding != 0, a->padding}; }
+
+// Pieces of a row and the threads that share it. Rows that are not whole 16-byte pieces on
+// 16-byte boundaries go entry by entry.
+struct Shape {
+  bool vec;
+  int entries, chunks, tpr;
+};
+
+Shape shape_of(const fx_embed_args* a, const void* p, const void* q) {
+  const int size = a->dtype == FX_F32 ? 4 : 2;
+  Shape s;
+  s.vec = (a->width * size | reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q)) % 16 == 0;
+  s.entries = s.vec ? 16 / size : 1;
+  s.chunks = (int)(a->width / s.entries);
+  s.tpr = 1;
+  while (s.tpr < s.chunks && s.tpr < kEmbedThreads) s.tpr *= 2;
+  return s;
+}
+
+// Few tokens and rows are listed row by row in one launch: rows x count comparisons.
+// Otherwise the tokens are sorted.
+bool scans(const fx_embed_args* a) {
+  return a->count <= kScanTokens && a->rows <= 16384 && a->rows * a->count <= (int64_t{1} << 22);
+}
+
+// Tokens of a window: as many as leave every thread slot of the device a window's columns.
+int window_of(const fx_embed_args* a, const Shape& s, int sms) {
+  int w = 128;
+  while (w > 16 && a->count / w * s.chunks < (int64_t)sms * 1024) w /= 2;
+  return w;
+}
+
+struct SortPlan {
+  int passes, bits, blocks, window, windows;
+  size_t keys, hist, total, start, part, bytes;  // offsets
+};
+
+SortPlan plan_of(const fx_embed_args* a, const Shape& s, int sms) {
+  SortPlan P;
+  int bits = 1;
+  while (a->rows >> bits) ++bits;  // keys are 0 .. rows
+  P.passes = (bits + kSortBits - 1) / kSortBits;
+  P.bits = (bits + P.passes - 1) / P.passes;
+  P.blocks = (int)((a->count + kSortTile - 1) / kSortTile);
+  P.window = window_of(a, s, sms);
+  P.windows = (int)((a->count + P.window - 1) / P.window);
+  P.keys = 0;  // keys and places, two of each
+  P.hist = align256((size_t)(P.passes > 1 ? 4 : 2) * a->count * sizeof(int));
+  P.total = P.hist + align256(((size_t)P.blocks << P.bits) * sizeof(int));
+  P.start = P.total + align256((size_t{1} << P.bits) * sizeof(int));
+  P.part = P.start + align256((size_t)(a->rows + 1) * sizeof(int));
+  P.bytes = P.part + align256((size_t)P.windows * 2 * s.chunks * s.entries * sizeof(float));
+  return P;
+}
+
+template <typename T, int E>
+int run_fwd(cudaStream_t s, const EmbedFwd& A) {
+  const int64_t per = (int64_t)(kEmbedThreads / A.tpr) * kEmbedRows, blocks = (A.count + per - 1) / per;
+  embed_fwd_kernel<T, E><<<(unsigned)blocks, kEmbedThreads, 0, s>>>(A);
+  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+}
+
+template <typename T, int E>
+int run_scan(cudaStream_t s, const EmbedGrad& A, const Tokens& tok) {
+  embed_scan_kernel<T, E><<<(unsigned)A.rows, kEmbedThreads, 0, s>>>(A, tok);
+  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+}
+
+template <typename T, int E>
+int run_sums(cudaStream_t s, const EmbedGrad& A) {
+  const int groups = kEmbedThreads / A.tpr;
+  const unsigned cols = (unsigned)((A.chunks + A.tpr - 1) / A.tpr);
+  const dim3 windows((A.windows + groups - 1) / groups, cols), rows((unsigned)((A.rows + groups - 1) / groups), cols);
+  embed_window_kernel<T, E><<<windows, kEmbedThreads, 0, s>>>(A);
+  embed_join_kernel<T, E><<<rows, kEmbedThreads, 0, s>>>(A);
+  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+}
+
+int sort(cudaStream_t s, const fx_embed_args* a, const SortPlan& P, unsigned char* ws, EmbedGrad& A) {
+  int* lists = reinterpret_cast<int*>(ws + P.keys);
+  SortArgs S{};
+  S.tok = tokens_of(a);
+  S.rows = a->rows;
+  S.count = (int)a->count;
+  S.blocks = P.blocks;
+  S.bits = P.bits;
+  S.hist = reinterpret_cast<int*>(ws + P.hist);
+  S.total = reinterpret_cast<int*>(ws + P.total);
+  int* start = reinterpret_cast<int*>(ws + P.start);
+  const int digits = 1 << P.bits;
+  const size_t smem = (size_t)(kSortWarps + 1) * digits * sizeof(int);
+  if (raise_smem(sort_place_kernel, smem, (size_t)(kSortWarps + 1) * (sizeof(int) << kSortBits))) return FX_ERR_CUDA;
+  for (int p = 0; p < P.passes; ++p) {
+    S.keys_out = lists + (size_t)(p & 1) * 2 * a->count;
+    S.pos_out = S.keys_out + a->count;
+    S.shift = p * P.bits;
+    S.start = P.passes == 1 ? start : nullptr;
+    sort_count_kernel<<<P.blocks, kSortThreads, digits * sizeof(int), s>>>(S);
+    sort_scan_kernel<<<(digits + 7) / 8, 256, 0, s>>>(S);
+    sort_place_kernel<<<P.blocks, kSortThreads, smem, s>>>(S);
+    S.keys = S.keys_out;
+    S.pos = S.pos_out;
+  }
+  if (P.passes > 1)
+    sort_start_kernel<<<(unsigned)((a->rows + 256) / 256), 256, 0, s>>>(S.keys, S.count, start, a->rows);
+  A.keys = S.keys;
+  A.pos = S.pos;
+  A.start = start;
+  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fermix_token_embedding(void* stream, const fx_embed_args* a) {
+  const int e = check(a);
+  if (e) return e;
+  if (a->count == 0) return FX_OK;
+  if (!a->tokens || !a->weight || !a->out) return FX_ERR_NULL;
+  const Shape h = shape_of(a, a->weight, a->out);
+  EmbedFwd A{tokens_of(a), a->weight, a->out, a->count, a->rows, a->width, h.chunks, h.tpr, a->scale};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a->dtype == FX_F32) return h.vec ? run_fwd<float, 4>(s, A) : run_fwd<float, 1>(s, A);
+  return h.vec ? run_fwd<bf16, 8>(s, A) : run_fwd<bf16, 1>(s, A);
+}
+
+// Without the pointers the larger of the two forms counts: entry by entry, fewer windows never
+// need more.
+size_t fermix_token_embedding_grad_workspace_bytes(const fx_embed_args* a) {
+  const DevInfo* D = dev_info();
+  if (check(a) || !D || a->count == 0 || scans(a)) return 0;
+  return plan_of(a, shape_of(a, a->grad, a->dweight), D->sms).bytes + 256;
+}
+
+int fermix_token_embedding_grad(void* stream, const fx_embed_args* a, void* ws, size_t wsb) {
+  const int e = check(a);
+  if (e) return e;
+  if (!a->dweight) return FX_ERR_NULL;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a->count == 0)
+    return cudaMemsetAsync(a->dweight, 0, (size_t)(a->rows * a->width) * (a->dtype == FX_F32 ? 4 : 2), s) == cudaSuccess
+               ? FX_OK
+               : FX_ERR_CUDA;
+  if (!a->tokens || !a->grad) return FX_ERR_NULL;
+  const Shape h = shape_of(a, a->grad, a->dweight);
+  EmbedGrad A{};
+  A.grad = a->grad;
+  A.dweight = a->dweight;
+  A.rows = a->rows;
+  A.width = a->width;
+  A.count = (int)a->count;
+  A.chunks = h.chunks;
+  A.tpr = h.tpr;
+  A.scale = a->scale;
+  if (scans(a)) {
+    const Tokens t = tokens_of(a);
+    if (a->dtype == FX_F32) return h.vec ? run_scan<float, 4>(s, A, t) : run_scan<float, 1>(s, A, t);
+    return h.vec ? run_scan<bf16, 8>(s, A, t) : run_scan<bf16, 1>(s, A, t);
+  }
+  const DevInfo* D = dev_info();
+  if (!D) return FX_ERR_DEVICE;
+  const SortPlan P = plan_of(a, h, D->sms);
+  if (!ws || wsb < P.bytes + 256) return FX_ERR_WORKSPACE;
+  unsigned char* base = reinterpret_cast<unsigned char*>(align256(reinterpret_cast<uintptr_t>(ws)));
+  A.window = P.window;
+  A.windows = P.windows;
+  A.part = reinterpret_cast<float*>(base + P.part);
+  const int st = sort(s, a, P, base, A);
+  if (st) return st;
+  if (a->dtype == FX_F32) return h.vec ? run_sums<float, 4>(s, A) : run_sums<float, 1>(s, A);
+  return h.vec ? run_sums<bf16, 8>(s, A) : run_sums<bf16, 1>(s, A);
+}
+
+}  // extern "C"

@@ -1,0 +1,29 @@
+// Shared pieces of the operators on tokens.
+#pragma once
+#include "block_common.cuh"
+#include "fermix_b200_token.h"
+
+namespace fx {
+
+struct Tokens {
+  const void* p;
+  int bytes, has_padding;
+  int64_t padding;
+
+  __device__ __forceinline__ int64_t at(int64_t i) const {
+    switch (bytes) {
+      case 1: return static_cast<const uint8_t*>(p)[i];
+      case 2: return static_cast<const int16_t*>(p)[i];
+      case 4: return static_cast<const int32_t*>(p)[i];
+      default: return static_cast<const int64_t*>(p)[i];
+    }
+  }
+  __device__ __forceinline__ bool padded(int64_t t) const { return has_padding && t == padding; }
+  // The table's row of token i; `rows` where it has none.
+  __device__ __forceinline__ int key(int64_t i, int64_t rows) const {
+    const int64_t t = at(i);
+    return t < 0 || t >= rows || padded(t) ? (int)rows : (int)t;
+  }
+};
+
+}  // namespace fx
