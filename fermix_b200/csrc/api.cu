@@ -623,9 +623,10 @@ unsigned fermix_set_wait_polls(unsigned polls) { return g_wait_polls.exchange(po
 int fermix_device_status(int clear) {
   if (!dev_info()) return FX_ERR_DEVICE;
   if (cudaDeviceSynchronize() != cudaSuccess) return FX_ERR_CUDA;
-  const int a = tc_status(clear), b = update_status(clear), c = attn_tc_status(clear);
-  if (a < 0 || b < 0 || c < 0) return FX_ERR_CUDA;
-  return a ? a : b ? b : c;
+  const int a = tc_status(clear), b = update_status(clear), c = attn_tc_status(clear),
+            d = linear_status(clear);
+  if (a < 0 || b < 0 || c < 0 || d < 0) return FX_ERR_CUDA;
+  return a ? a : b ? b : c ? c : d;
 }
 
 int fermix_slogpf_ratio(void* stream, int dtype, int64_t batch, int64_t n, const void* g, const void* row,

@@ -2,6 +2,7 @@
 #include "attn_host.cuh"
 #include "attn_tc.cuh"
 #include "attn_tc_grad.cuh"
+#include "tensor_map.cuh"
 
 namespace fxh {
 
@@ -14,22 +15,6 @@ using tc::LOAD_TMA;
 using Narrow = tc::Rows<64, 1>;   // dim <= 32 (float32)
 using Half = tc::Rows<128, 1>;    // dim <= 64
 using Whole = tc::Rows<128, 2>;   // dim <= 128
-
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled encode_tiled() {
-  static const EncodeTiled fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult r;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess ||
-        r != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<EncodeTiled>(p);
-  }();
-  return fn;
-}
 
 // The map of a bfloat16 tensor (batch, head, token) by element strides: boxes of 64 entries by
 // `rows` tokens. false: no such map (the caller loads by the threads).

@@ -44,15 +44,24 @@ __device__ __forceinline__ ActOut activate(float h) {
   return o;
 }
 
-template <bool SLOPE>
-__device__ __forceinline__ ActOut activate(int act, float h) {
+template <int ACT, bool SLOPE, int N>
+__device__ __forceinline__ void activate_as(const float (&h)[N], float (&y)[N], float (&d)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const ActOut o = activate<ACT, SLOPE>(h[e]);
+    y[e] = o.y;
+    d[e] = o.d;
+  }
+}
+template <bool SLOPE, int N>
+__device__ __forceinline__ void activate_all(int act, const float (&h)[N], float (&y)[N], float (&d)[N]) {
   switch (act) {
-    case FX_ACT_RELU: return activate<FX_ACT_RELU, SLOPE>(h);
-    case FX_ACT_SILU: return activate<FX_ACT_SILU, SLOPE>(h);
-    case FX_ACT_GELU: return activate<FX_ACT_GELU, SLOPE>(h);
-    case FX_ACT_GELU_TANH: return activate<FX_ACT_GELU_TANH, SLOPE>(h);
-    case FX_ACT_TANH: return activate<FX_ACT_TANH, SLOPE>(h);
-    default: return activate<FX_ACT_NONE, SLOPE>(h);
+    case FX_ACT_RELU: return activate_as<FX_ACT_RELU, SLOPE>(h, y, d);
+    case FX_ACT_SILU: return activate_as<FX_ACT_SILU, SLOPE>(h, y, d);
+    case FX_ACT_GELU: return activate_as<FX_ACT_GELU, SLOPE>(h, y, d);
+    case FX_ACT_GELU_TANH: return activate_as<FX_ACT_GELU_TANH, SLOPE>(h, y, d);
+    case FX_ACT_TANH: return activate_as<FX_ACT_TANH, SLOPE>(h, y, d);
+    default: return activate_as<FX_ACT_NONE, SLOPE>(h, y, d);
   }
 }
 
@@ -79,14 +88,5 @@ struct Epilogue {
   int64_t rs;  // stride of a row of the residual
   void *y, *slope;  // (rows, cols) contiguous
 };
-
-template <typename T>
-__device__ __forceinline__ void epilogue_one(const Epilogue& E, int64_t i, int64_t j, int64_t cols, float h) {
-  if (E.bias) h += to_f(static_cast<const T*>(E.bias)[j]);
-  const ActOut o = E.slope ? activate<true>(E.act, h) : activate<false>(E.act, h);
-  if (E.slope) static_cast<typename SlopeOf<T>::type*>(E.slope)[i * cols + j] = from_f<typename SlopeOf<T>::type>(o.d);
-  const float y = E.residual ? to_f(static_cast<const T*>(E.residual)[i * E.rs + j]) + o.y : o.y;
-  static_cast<T*>(E.y)[i * cols + j] = from_f<T>(y);
-}
 
 }  // namespace fx

@@ -1,0 +1,550 @@
+// The linear map's products on the tensor cores: D(i, j) = sum over k of A(i, k) B(j, k), the
+// forward (x, W), dx (g, W) and dW (g, x) alike. Each operand is read as it is stored, along k
+// (K-major) or across it (MN-major).
+//
+// A pair of SMs holds a tile of 256 x 256: each brings 128 rows of A and 128 of B by tensor maps
+// (64 entries of k a stage) and keeps 128 x 256 of the sum in its TMEM, twice, so that one
+// tile's epilogue runs under the next tile's products. The grid is persistent.
+//
+// float32 runs on the same bfloat16 instructions: x = x1 + x2 + x3, each part the rest rounded to
+// bfloat16, holds 24 bits, and the six products with index sum <= 4 leave out terms of 2^-24. The
+// tensor cores cut off what they add to an accumulator below its last bit, always towards zero, so
+// float32 sums are moved on to registers, with rounding, every kChunk blocks of k. In bfloat16 the
+// whole sum stays in the accumulator: 1.6e-8 of it is lost for every 16 entries of k, which reaches
+// half of the output's rounding (2e-3) after a million.
+//
+// Few tiles split k over pairs of SMs; the parts are float32 sums in the workspace, added in
+// order by linear_join_kernel, which then does the epilogue.
+#pragma once
+#include <cuda.h>
+
+#include "linear_common.cuh"
+#include "umma.cuh"
+
+namespace fx {
+namespace lin {
+
+using namespace umma;
+
+constexpr int kTile = 256, kHalf = 128, kBlockK = 64;  // of a pair, of an SM, of a stage
+constexpr int kThreads = 320;                          // copies, products, 8 warps of epilogue
+constexpr uint32_t kOperand = kHalf * kBlockK * 2;     // bytes of one SM's rows in a stage
+
+template <int NP>
+struct Shape {
+  static constexpr int kStages = NP == 1 ? 6 : 2;
+  static constexpr uint32_t kStage = 2 * NP * kOperand;
+  static constexpr uint32_t kSmem = kStages * kStage + 8 * 4096 + 1024;
+  static constexpr int kChunk = 2;  // blocks of k in an accumulator (three parts)
+};
+
+struct alignas(64) Maps {
+  CUtensorMap a, b;
+};
+
+struct Args {
+  int64_t rows, cols;            // of the result
+  int blocks, tm, tn, splits, per;  // blocks of k, tiles, parts of k, blocks of a part
+  int a_mn, b_mn, vec;
+  uint32_t polls;
+  float* part;  // (splits, rows, part_ld)
+  int64_t part_ld;
+  Epilogue e;
+};
+
+// ---------------------------------------------------------------- instructions of a pair
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of the pair's first block's copy of a shared variable.
+__device__ __forceinline__ uint32_t first_block(const void* p) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+  return r;
+}
+__device__ __forceinline__ void arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+      "[%5];" ::"r"(dst),
+      "l"(m), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc ? 1u : 0u)
+      : "memory");
+}
+// Arrival at both blocks' copies of the barrier when the products issued so far are done.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ void alloc_pair(uint32_t* slot) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)));
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+}
+__device__ __forceinline__ void dealloc_pair(uint32_t t) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(t));
+}
+#define FX_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
+__device__ __forceinline__ void ld32(uint32_t a, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : FX_R8(v, 0), FX_R8(v, 8), FX_R8(v, 16), FX_R8(v, 24)
+      : "r"(a));
+}
+#undef FX_R8
+
+// 128-byte swizzled operand: rows of 64 entries of k, or, MN-major, rows of 64 entries across k, 64 of
+// them (of k) a chunk, chunks of 8 KB after each other.
+__device__ __forceinline__ uint64_t desc(uint32_t saddr, bool mn) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(mn ? 8192 >> 4 : 1) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// A bounded wait. One that runs out is recorded (the block's outputs become NaN) and waits once
+// more, with a limit of its own, so that nothing is under way that the block does not know of; if that
+// runs out too, the block's threads wait and issue no more.
+enum { RUNS = 0, LATE = 1, DEAD = 2 };
+constexpr uint32_t kLastPolls = 1u << 22;
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* state, uint32_t polls) {
+  if (mbar_wait(bar, parity, polls)) return true;
+  if (*state == DEAD) return false;
+  record_status(8);  // FX_ERR_TIMEOUT
+  if (*state == RUNS) *state = LATE;
+  if (mbar_wait(bar, parity, kLastPolls)) return true;
+  *state = DEAD;
+  return false;
+}
+
+// ---------------------------------------------------------------- epilogue
+// Four entries of a row from column j, `n` of them there.
+template <typename T>
+__device__ __forceinline__ void epilogue_four(const Epilogue& E, bool vec, int64_t i, int64_t j, int64_t cols, float (&h)[4],
+                                              const float (&bias)[4]) {
+  using TS = typename SlopeOf<T>::type;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) h[e] += bias[e];
+  float y[4], d[4];
+  if (E.slope) activate_all<true>(E.act, h, y, d);
+  else activate_all<false>(E.act, h, y, d);
+  T* out = static_cast<T*>(E.y) + i * cols + j;
+  const T* res = E.residual ? static_cast<const T*>(E.residual) + i * E.rs + j : nullptr;
+  TS* slope = E.slope ? static_cast<TS*>(E.slope) + i * cols + j : nullptr;
+  if (vec) {
+    if (slope) {
+      Pack<TS, 4> s;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s.e[e] = from_f<TS>(d[e]);
+      *reinterpret_cast<Pack<TS, 4>*>(slope) = s;
+    }
+    if (res) {
+      const Pack<T, 4> r = *reinterpret_cast<const Pack<T, 4>*>(res);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += to_f(r.e[e]);
+    }
+    Pack<T, 4> o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o.e[e] = from_f<T>(y[e]);
+    *reinterpret_cast<Pack<T, 4>*>(out) = o;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (j + e >= cols) break;
+      if (slope) slope[e] = from_f<TS>(d[e]);
+      out[e] = from_f<T>(res ? to_f(res[e]) + y[e] : y[e]);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_bias(const Epilogue& E, int64_t j, int64_t cols, float (&bias)[4]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) bias[e] = E.bias && j + e < cols ? to_f(static_cast<const T*>(E.bias)[j + e]) : 0.f;
+}
+
+// 32 x 32 entries of the sum, a row a lane, through shared memory to four entries of a row a
+// lane (eight lanes a row), so that stores cover whole sectors.
+template <typename T>
+__device__ __forceinline__ void store_block(const Args& G, unsigned char* stage, int64_t i0, int64_t j0, int split, bool late,
+                                            const uint32_t (&v)[32]) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+#pragma unroll
+  for (int p = 0; p < 8; ++p)
+    *reinterpret_cast<uint4*>(stage + lane * 128 + ((p ^ (lane & 7)) << 4)) =
+        make_uint4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
+  __syncwarp();
+  const int piece = lane & 7;
+  const int64_t j = j0 + piece * 4;
+  float bias[4];
+  if (!G.part) load_bias<T>(G.e, j, G.cols, bias);
+#pragma unroll 2
+  for (int s = 0; s < 8; ++s) {
+    const int r = s * 4 + (lane >> 3);
+    float4 x = *reinterpret_cast<const float4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
+    if (i0 + r >= G.rows || j >= G.cols) continue;
+    if (late) x.x = x.y = x.z = x.w = __int_as_float(0x7fc00000);
+    if (G.part) {
+      *reinterpret_cast<float4*>(G.part + (split * G.rows + i0 + r) * G.part_ld + j) = x;
+    } else {
+      float h[4] = {x.x, x.y, x.z, x.w};
+      epilogue_four<T>(G.e, G.vec, i0 + r, j, G.cols, h, bias);
+    }
+  }
+}
+
+struct Unit {
+  int m, n, split, first, last;  // tile, part of k, blocks of k
+};
+// Tiles in groups of 8 rows of tiles, down the columns of a group, so that what runs at a time shares
+// rows and columns; the parts of a tile next to each other.
+__device__ __forceinline__ Unit unit_of(const Args& G, int u) {
+  Unit U;
+  const int t = u / G.splits, group = t / (8 * G.tn), in = t - group * 8 * G.tn;
+  const int rows = min(8, G.tm - group * 8);
+  U.split = u - t * G.splits;
+  U.m = group * 8 + in % rows;
+  U.n = in / rows;
+  U.first = U.split * G.per;
+  U.last = min(U.first + G.per, G.blocks);
+  return U;
+}
+
+template <typename T, int NP>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    linear_tc_kernel(const __grid_constant__ Args G, const __grid_constant__ Maps M) {
+  using S = Shape<NP>;
+  constexpr int ST = S::kStages;
+  extern __shared__ unsigned char raw[];
+  unsigned char* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  __shared__ uint64_t full[ST], empty[ST], sum_full[2], sum_empty[2];
+  __shared__ uint32_t slot;
+  __shared__ volatile int state;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cta_rank();
+  if (tid == 0) {
+    state = RUNS;
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sum_full[i], 1);
+      mbar_init(&sum_empty[i], 16);  // the epilogue's warps of both blocks
+    }
+    fence_mbar_init();
+  }
+  if (warp == 2) alloc_pair(&slot);
+  fence_before_sync();
+  __syncthreads();
+  cluster_sync();
+  fence_after_sync();
+  const uint32_t tmem = slot;
+  const int units = G.tm * G.tn * G.splits, pairs = gridDim.x >> 1;
+  const int chunk = NP == 1 ? G.blocks : S::kChunk;
+
+  if (warp == 0) {
+    // -------------------------------------------------------- copies, one thread of each block
+    if (lane == 0) {
+      int it = 0;
+      for (int u = blockIdx.x >> 1; u < units && state != DEAD; u += pairs) {
+        const Unit U = unit_of(G, u);
+        const int i0 = U.m * kTile + rank * kHalf, j0 = U.n * kTile + rank * kHalf;
+        for (int kb = U.first; kb < U.last; ++kb, ++it) {
+          const int st = it % ST;
+          if (!wait(&empty[st], (it / ST & 1) ^ 1, &state, G.polls)) break;
+          const uint32_t bar = first_block(&full[st]), at = smem_u32(sm) + st * S::kStage;
+          if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * S::kStage);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+            const uint32_t a = at + p * kOperand, b = at + (NP + p) * kOperand;
+            if (G.a_mn) {
+              tma_box(a, &M.a, i0, kb * kBlockK, p, bar);
+              tma_box(a + 8192, &M.a, i0 + 64, kb * kBlockK, p, bar);
+            } else {
+              tma_box(a, &M.a, kb * kBlockK, i0, p, bar);
+            }
+            if (G.b_mn) {
+              tma_box(b, &M.b, j0, kb * kBlockK, p, bar);
+              tma_box(b + 8192, &M.b, j0 + 64, kb * kBlockK, p, bar);
+            } else {
+              tma_box(b, &M.b, kb * kBlockK, j0, p, bar);
+            }
+          }
+        }
+      }
+      // after a wait that ran out: the copies asked for, with a bound
+      if (state == DEAD)
+        for (int j = it > ST ? it - ST : 0; j < it; ++j) mbar_wait(&full[j % ST], j / ST & 1, 1u << 20);
+    }
+  } else if (warp == 1) {
+    // -------------------------------------------------------- products, one thread of the pair
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = 1u << 4 | 1u << 7 | 1u << 10 | (G.a_mn ? 1u << 15 : 0u) | (G.b_mn ? 1u << 16 : 0u) |
+                             (uint32_t)(kTile >> 3) << 17 | (uint32_t)(kTile >> 4) << 24;
+      const uint32_t sa = G.a_mn ? 128 : 2, sb = G.b_mn ? 128 : 2;  // 16 entries of k further, in 16 bytes
+      int it = 0, ch = 0;
+      for (int u = blockIdx.x >> 1; u < units && state != DEAD; u += pairs) {
+        const Unit U = unit_of(G, u);
+        for (int k0 = U.first; k0 < U.last; k0 += chunk, ++ch) {
+          const int buf = ch & 1;
+          if (!wait(&sum_empty[buf], (ch >> 1 & 1) ^ 1, &state, G.polls)) break;
+          fence_after_sync();
+          const uint32_t d = tmem + buf * kTile;
+          bool acc = false;
+          for (int kb = k0; kb < min(k0 + chunk, U.last); ++kb, ++it) {
+            const int st = it % ST;
+            if (!wait(&full[st], it / ST & 1, &state, G.polls)) break;
+            fence_after_sync();
+            const uint32_t at = smem_u32(sm) + st * S::kStage;
+#pragma unroll
+            for (int sum = NP - 1; sum >= 0; --sum) {  // the smaller products first
+#pragma unroll
+              for (int i = 0; i <= sum; ++i) {
+                uint64_t a = desc(at + i * kOperand, G.a_mn), b = desc(at + (NP + sum - i) * kOperand, G.b_mn);
+#pragma unroll
+                for (int k = 0; k < kBlockK / 16; ++k) {
+                  mma_pair(d, a, b, idesc, acc);
+                  acc = true;
+                  a += sa;
+                  b += sb;
+                }
+              }
+            }
+            commit_pair(&empty[st]);
+          }
+          commit_pair(&sum_full[buf]);
+        }
+      }
+      if (state == DEAD && ch > 0) mbar_wait(&sum_full[(ch - 1) & 1], (ch - 1) >> 1 & 1, 1u << 20);
+    }
+  } else {
+    // -------------------------------------------------------- epilogue
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    unsigned char* stage = sm + ST * S::kStage + (warp - 2) * 4096;
+    const uint32_t lanes = tmem + ((uint32_t)quarter << 21) + half * 128;
+    int ch = 0;
+    for (int u = blockIdx.x >> 1; u < units && state != DEAD; u += pairs) {
+      const Unit U = unit_of(G, u);
+      const int64_t i0 = (int64_t)U.m * kTile + rank * kHalf + quarter * 32, j0 = (int64_t)U.n * kTile + half * 128;
+      float acc[NP == 1 ? 1 : 4][32];
+      for (int k0 = U.first; k0 < U.last; k0 += chunk, ++ch) {
+        const int buf = ch & 1;
+        if (!wait(&sum_full[buf], ch >> 1 & 1, &state, G.polls)) break;
+        fence_after_sync();
+        if constexpr (NP == 1) {
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            if (j0 + c * 32 >= G.cols) break;
+            uint32_t v[32];
+            ld32(lanes + buf * kTile + c * 32, v);
+            tmem_wait_ld();
+            store_block<T>(G, stage, i0, j0 + c * 32, U.split, state != RUNS, v);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t v[32];
+            ld32(lanes + buf * kTile + c * 32, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) acc[c][e] = (k0 == U.first ? 0.f : acc[c][e]) + __uint_as_float(v[e]);
+          }
+        }
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) arrive_at(first_block(&sum_empty[buf]));
+      }
+      if constexpr (NP > 1) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (j0 + c * 32 >= G.cols) break;
+          uint32_t v[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(acc[c][e]);
+          store_block<T>(G, stage, i0, j0 + c * 32, U.split, state != RUNS, v);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  fence_before_sync();
+  cluster_sync();
+  fence_after_sync();
+  if (warp == 2) dealloc_pair(tmem);
+}
+
+// ---------------------------------------------------------------- around the products
+// The parts of a split sum in order, then the epilogue; four columns a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ Args G) {
+  const int64_t quads = G.part_ld / 4, n = G.rows * quads;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
+    const int64_t i = t / quads, j = (t - i * quads) * 4;
+    const float* p = G.part + i * G.part_ld + j;
+    float h[4] = {0.f, 0.f, 0.f, 0.f}, bias[4];
+#pragma unroll 4
+    for (int s = 0; s < G.splits; ++s) {
+      const float4 x = *reinterpret_cast<const float4*>(p + s * G.rows * G.part_ld);
+      h[0] += x.x;
+      h[1] += x.y;
+      h[2] += x.z;
+      h[3] += x.w;
+    }
+    load_bias<T>(G.e, j, G.cols, bias);
+    epilogue_four<T>(G.e, G.vec, i, j, G.cols, h, bias);
+  }
+}
+
+// (a, b) -> NP packed pairs of bfloat16 whose sum is (a, b). What rounds to infinity though it is
+// finite is cut off instead.
+template <int NP>
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&o)[NP]) {
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[i]) : "f"(b), "f"(a));
+    if (NP > 1 && i == 0) {
+      if ((o[0] & 0x7fffu) == 0x7f80u && fabsf(a) < INFINITY) o[0] = (o[0] & 0xffff0000u) | (o[0] & 0x8000u) | 0x7f7fu;
+      if ((o[0] & 0x7fff0000u) == 0x7f800000u && fabsf(b) < INFINITY) o[0] = (o[0] & 0x8000ffffu) | 0x7f7f0000u;
+    }
+    if (i + 1 < NP) {
+      a -= __uint_as_float(o[i] << 16);
+      b -= __uint_as_float(o[i] & 0xffff0000u);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_eight(const T* p, int64_t n, bool vec, float (&x)[8]) {
+  constexpr int V = 16 / sizeof(T);
+  if (vec) {
+#pragma unroll
+    for (int h = 0; h < 8; h += V) {
+      if (h < n) {
+        const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p + h);
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[h + e] = to_f(k.e[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[h + e] = 0.f;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = e < n ? to_f(p[e]) : 0.f;
+  }
+}
+
+template <int NP>
+__device__ __forceinline__ void store_parts(uint16_t* out, int64_t plane, const float (&x)[8]) {
+  uint32_t w[4][NP];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) split_pair<NP>(x[2 * e], x[2 * e + 1], w[e]);
+#pragma unroll
+  for (int p = 0; p < NP; ++p) *reinterpret_cast<uint4*>(out + p * plane) = make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]);
+}
+
+// An operand as the tensor maps take it: NP planes of bfloat16, (NP, rows, ld), ld a multiple of 8.
+struct PartsArgs {
+  const void* src;
+  int64_t stride, rows, cols, ld;
+  uint16_t* out;
+  int vec;
+};
+
+template <typename T, int NP>
+__global__ void __launch_bounds__(256) linear_parts_kernel(const __grid_constant__ PartsArgs A) {
+  const int64_t eights = A.ld / 8, n = A.rows * eights;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
+    const int64_t i = t / eights, j = (t - i * eights) * 8;
+    float x[8];
+    load_eight<T>(static_cast<const T*>(A.src) + i * A.stride + j, A.cols - j, A.vec, x);
+    store_parts<NP>(A.out + i * A.ld + j, A.rows * A.ld, x);
+  }
+}
+
+// g = dy act'(h) as parts (out not NULL), and each block's sums over its rows (sums not NULL):
+// `tpr` threads share a row, eight columns each.
+struct SlopeArgs {
+  const void *dy, *slope;
+  int64_t stride, rows, cols, ld, per;  // per: rows of a block
+  uint16_t* out;
+  float* sums;  // (gridDim.y, cols)
+  int tpr, vec;
+};
+
+template <typename T, int NP>
+__global__ void __launch_bounds__(256) linear_slope_kernel(const __grid_constant__ SlopeArgs A) {
+  using TS = typename SlopeOf<T>::type;
+  __shared__ float share[8][256];
+  const int groups = 256 / A.tpr, g = threadIdx.x / A.tpr, col = threadIdx.x & (A.tpr - 1);
+  const int64_t j = ((int64_t)blockIdx.x * A.tpr + col) * 8, r0 = blockIdx.y * A.per;
+  const int64_t end = r0 + A.per < A.rows ? r0 + A.per : A.rows;
+  float sum[8] = {};
+  if (j < A.cols) {
+#pragma unroll 2
+    for (int64_t i = r0 + g; i < end; i += groups) {
+      float x[8];
+      load_eight<T>(static_cast<const T*>(A.dy) + i * A.stride + j, A.cols - j, A.vec, x);
+      if (A.slope) {
+        float d[8];
+        load_eight<TS>(static_cast<const TS*>(A.slope) + i * A.cols + j, A.cols - j, A.vec, d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(x[e], d[e]);  // the same g whether it is stored or only summed
+      }
+      if (A.out) store_parts<NP>(A.out + i * A.ld + j, A.rows * A.ld, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[e] += x[e];
+    }
+  }
+  if (!A.sums) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) share[e][threadIdx.x] = sum[e];
+  __syncthreads();
+  // the groups' sums in order, a column a thread
+  for (int c = threadIdx.x; c < A.tpr * 8; c += 256) {
+    const int64_t jj = (int64_t)blockIdx.x * A.tpr * 8 + c;
+    if (jj >= A.cols) break;
+    float s = 0.f;
+    for (int k = 0; k < groups; ++k) s += share[c & 7][k * A.tpr + (c >> 3)];
+    A.sums[blockIdx.y * A.cols + jj] = s;
+  }
+}
+
+// The blocks' sums in order: 32 columns a block, eight warps that share the blocks.
+template <typename T>
+__global__ void __launch_bounds__(256) linear_bias_kernel(const float* sums, int blocks, int64_t cols, void* dbias) {
+  __shared__ float share[8][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t j = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (j < cols) {
+#pragma unroll 8
+    for (int b = w; b < blocks; b += 8) s += sums[b * cols + j];
+  }
+  share[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && j < cols) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += share[k][lane];
+    static_cast<T*>(dbias)[j] = from_f<T>(s);
+  }
+}
+
+}  // namespace lin
+}  // namespace fx

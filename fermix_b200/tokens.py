@@ -195,8 +195,8 @@ def fused_linear(x, weight, bias=None, *, activation=None, residual=None):
     outer, inner = weight.shape
     if x.dim() < 1 or x.shape[-1] != inner:
         raise ValueError(f"x must have shape (..., {inner}), got {tuple(x.shape)}")
-    if x.numel() >= (2**31 - 1) * inner or max(outer, inner) >= 2**31 - 1:
-        raise ValueError(f"fewer than 2**31 - 1 rows and columns, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if x.numel() >= 2**30 * inner or max(outer, inner) >= 2**30:
+        raise ValueError(f"fewer than 2**30 rows and columns, got {tuple(x.shape)} and {tuple(weight.shape)}")
     if bias is not None:
         if tuple(_tensor(bias, "bias", x).shape) != (outer,):
             raise ValueError(f"bias must have shape ({outer},), got {tuple(bias.shape)}")
