@@ -35,7 +35,7 @@ bool mappable(const void* p, int64_t stride, int64_t rows) {
          stride < (int64_t{1} << 38);
 }
 
-// How a product of rows x cols over `inner` is cut: tiles of 256 x 256 a pair of SMs; where they do
+// How a product of rows x cols over `inner` is cut: tiles of a pair of SMs; where they do
 // not fill the device, k is cut into parts of four blocks at least.
 struct Cut {
   int64_t rows, cols;
@@ -45,13 +45,13 @@ struct Cut {
   size_t part_bytes() const { return splits > 1 ? align256((size_t)splits * rows * part_ld() * sizeof(float)) : 0; }
 };
 
-Cut cut_of(int64_t rows, int64_t cols, int64_t inner, int sms) {
+Cut cut_of(int64_t rows, int64_t cols, int64_t inner, bool f32, int sms) {
   Cut C;
   C.rows = rows;
   C.cols = cols;
   C.blocks = (int)ceil_div(inner, lin::kBlockK);
-  C.tm = (int)ceil_div(rows, lin::kTile);
-  C.tn = (int)ceil_div(cols, lin::kTile);
+  C.tm = (int)ceil_div(rows, lin::kRows);
+  C.tn = (int)ceil_div(cols, f32 ? lin::Shape<3>::kCols : lin::Shape<1>::kCols);
   const int64_t tiles = (int64_t)C.tm * C.tn, fill = (sms / 2) / tiles, most = C.blocks / 4;
   int64_t splits = fill < most ? fill : most;
   if (splits < 1) splits = 1;
@@ -89,7 +89,7 @@ LinPlan plan_fwd(const fx_linear_args* a, int sms) {
   P.planes = P.f32 ? 3 : 1;
   P.new_x = P.f32 || !mappable(a->x, a->x_stride, a->rows);
   P.new_w = P.f32 || !mappable(a->weight, a->weight_stride, a->outer);
-  P.y = cut_of(a->rows, a->outer, a->inner, sms);
+  P.y = cut_of(a->rows, a->outer, a->inner, P.f32, sms);
   Space S;
   if (P.new_x) P.x = S.take(parts_bytes(a->rows, a->inner, P.planes));
   if (P.new_w) P.w = S.take(parts_bytes(a->outer, a->inner, P.planes));
@@ -115,8 +115,8 @@ LinPlan plan_bwd(const fx_linear_args* a, int sms) {
   if (blocks > ceil_div(a->rows, groups * 4)) blocks = ceil_div(a->rows, groups * 4);
   P.per = ceil_div(a->rows, blocks);
   P.blocks = (int)ceil_div(a->rows, P.per);
-  P.dx = cut_of(a->rows, a->inner, a->outer, sms);
-  P.dw = cut_of(a->outer, a->inner, a->rows, sms);
+  P.dx = cut_of(a->rows, a->inner, a->outer, P.f32, sms);
+  P.dw = cut_of(a->outer, a->inner, a->rows, P.f32, sms);
   Space S;
   if (P.new_x) P.x = S.take(parts_bytes(a->rows, a->inner, P.planes));
   if (P.new_w) P.w = S.take(parts_bytes(a->outer, a->inner, P.planes));
@@ -128,14 +128,14 @@ LinPlan plan_bwd(const fx_linear_args* a, int sms) {
   return P;
 }
 
-// The map of a matrix: boxes of 64 entries by 128 rows (K-major), 64 by 64 (MN-major).
-int make_map(CUtensorMap* m, const Operand& o, int planes, bool mn) {
+// The map of a matrix: boxes of 64 entries by `rows` (K-major) or 64 rows (MN-major).
+int make_map(CUtensorMap* m, const Operand& o, int planes, bool mn, int rows) {
   const EncodeTiled encode = encode_tiled();
   if (!encode) return FX_ERR_CUDA;
   const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)planes};
   const int64_t ld = o.rows > 1 ? o.ld : ld_of(o.cols);
   const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, planes > 1 ? (cuuint64_t)(o.rows * ld * 2) : (cuuint64_t)ld * 2};
-  const cuuint32_t box[3] = {64, mn ? 64u : 128u, 1}, ones[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, mn ? 64u : (cuuint32_t)rows, 1}, ones[3] = {1, 1, 1};
   return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.p), dims, strides, box, ones,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
@@ -151,12 +151,29 @@ bool fours(const Epilogue& e, int64_t rows, int64_t cols, int size) {
   return cols % 4 == 0 && m % piece == 0;
 }
 
+template <typename T, int NP, int ACT>
+int launch(cudaStream_t s, const lin::Args& G, const lin::Maps& M, int64_t pairs, int sms) {
+  constexpr size_t smem = lin::Shape<NP>::kSmem;
+  if (G.splits > 1) {
+    auto kern = lin::linear_tc_kernel<T, NP, lin::kPart>;
+    if (raise_smem(kern, smem, smem)) return FX_ERR_CUDA;
+    kern<<<(unsigned)(2 * pairs), lin::kThreads, smem, s>>>(G, M);
+    const int64_t blocks = ceil_div(G.rows * G.part_ld / 4, 256), most = (int64_t)sms * 8;
+    lin::linear_join_kernel<T, ACT><<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(G);
+  } else {
+    auto kern = lin::linear_tc_kernel<T, NP, ACT>;
+    if (raise_smem(kern, smem, smem)) return FX_ERR_CUDA;
+    kern<<<(unsigned)(2 * pairs), lin::kThreads, smem, s>>>(G, M);
+  }
+  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+}
+
 template <typename T, int NP>
 int product(cudaStream_t s, const Cut& C, const Operand& a, bool a_mn, const Operand& b, bool b_mn, const Epilogue& e,
             float* part, int sms) {
   lin::Maps M;
-  int st = make_map(&M.a, a, NP, a_mn);
-  if (!st) st = make_map(&M.b, b, NP, b_mn);
+  int st = make_map(&M.a, a, NP, a_mn, lin::kHalf);
+  if (!st) st = make_map(&M.b, b, NP, b_mn, lin::Shape<NP>::kCols / 2);
   if (st) return st;
   if (C.units() > INT32_MAX) return FX_ERR_SHAPE;
   lin::Args G{};
@@ -174,16 +191,15 @@ int product(cudaStream_t s, const Cut& C, const Operand& a, bool a_mn, const Ope
   G.part = C.splits > 1 ? part : nullptr;
   G.part_ld = C.part_ld();
   G.e = e;
-  auto kern = lin::linear_tc_kernel<T, NP>;
-  const size_t smem = lin::Shape<NP>::kSmem;
-  if (raise_smem(kern, smem, smem)) return FX_ERR_CUDA;
   const int64_t pairs = C.units() < sms / 2 ? C.units() : sms / 2;
-  kern<<<(unsigned)(2 * pairs), lin::kThreads, smem, s>>>(G, M);
-  if (C.splits > 1) {
-    const int64_t blocks = ceil_div(C.rows * C.part_ld() / 4, 256), most = (int64_t)sms * 8;
-    lin::linear_join_kernel<T><<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(G);
+  switch (e.act) {
+    case FX_ACT_RELU: return launch<T, NP, FX_ACT_RELU>(s, G, M, pairs, sms);
+    case FX_ACT_SILU: return launch<T, NP, FX_ACT_SILU>(s, G, M, pairs, sms);
+    case FX_ACT_GELU: return launch<T, NP, FX_ACT_GELU>(s, G, M, pairs, sms);
+    case FX_ACT_GELU_TANH: return launch<T, NP, FX_ACT_GELU_TANH>(s, G, M, pairs, sms);
+    case FX_ACT_TANH: return launch<T, NP, FX_ACT_TANH>(s, G, M, pairs, sms);
+    default: return launch<T, NP, FX_ACT_NONE>(s, G, M, pairs, sms);
   }
-  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
 template <typename T, int NP>

@@ -6,12 +6,14 @@
 
 namespace fx {
 
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(fminf(-x, 80.f))); }
+
 // h -> (act(h), act'(h))
 struct ActOut {
   float y, d;
 };
 
-template <int ACT, bool SLOPE>
+template <int ACT>
 __device__ __forceinline__ ActOut activate(float h) {
   ActOut o;
   o.d = 1.f;
@@ -23,46 +25,31 @@ __device__ __forceinline__ ActOut activate(float h) {
     if (h != h) o.d = h;
     if (h < 0.f) o.y = 0.f;
   } else if constexpr (ACT == FX_ACT_SILU) {
-    const float s = 1.f / (1.f + __expf(-h));
-    o.y = h < -88.f ? 0.f : h * s;
-    if (SLOPE) o.d = s * fmaf(fmaxf(h, -88.f), 1.f - s, 1.f);
+    const float s = sigmoid(h);
+    o.y = h < -80.f ? 0.f : h * s;
+    o.d = s * fmaf(fmaxf(h, -80.f), 1.f - s, 1.f);
   } else if constexpr (ACT == FX_ACT_GELU) {
-    // the normal distribution's integral up to h: half of erfc(-h / sqrt 2), which keeps its digits where h < 0
-    const float c = 0.5f * erfcf(-0.70710678118654752f * h);
+    // erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x), x >= 0: Abramowitz and Stegun 7.1.26, off by
+    // 1.5e-7 at most. With x = |h| / sqrt 2 the exponential is the normal density's.
+    const float x = fabsf(h) * 0.70710678118654752f, t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f)), e = __expf(-x * x);
+    const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float tail = 0.5f * q * e, c = h < 0.f ? tail : 1.f - tail;
     o.y = h < -14.f ? 0.f : h * c;
-    if (SLOPE) o.d = fmaf(fminf(fmaxf(h, -20.f), 20.f) * 0.3989422804014327f, __expf(-0.5f * h * h), c);
+    o.d = fmaf(fminf(fmaxf(h, -20.f), 20.f) * 0.3989422804014327f, e, c);
   } else if constexpr (ACT == FX_ACT_GELU_TANH) {
     // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u))
     const float k = 1.5957691216057308f, h2 = fminf(h * h, 1e6f);
-    const float s = 1.f / (1.f + __expf(-k * h * fmaf(0.044715f, h2, 1.f)));
+    const float s = sigmoid(k * h * fmaf(0.044715f, h2, 1.f));
     o.y = h < -10.f ? 0.f : h * s;
-    if (SLOPE) o.d = fabsf(h) > 12.f ? s : s * fmaf(h * (1.f - s), k * fmaf(0.134145f, h2, 1.f), 1.f);
+    o.d = fabsf(h) > 12.f ? s : s * fmaf(h * (1.f - s), k * fmaf(0.134145f, h2, 1.f), 1.f);
   } else {
-    o.y = tanhf(h);
-    if (SLOPE) o.d = fmaf(-o.y, o.y, 1.f);
+    // tanh u = 2 sigmoid(2 u) - 1; near 0, where that cancels, its series (the next term is 5e-8 of it)
+    const float h2 = h * h;
+    o.y = h2 < 0.09f ? h * fmaf(h2, fmaf(h2, fmaf(h2, fmaf(h2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f)
+                     : fmaf(2.f, sigmoid(2.f * h), -1.f);
+    o.d = fmaf(-o.y, o.y, 1.f);
   }
   return o;
-}
-
-template <int ACT, bool SLOPE, int N>
-__device__ __forceinline__ void activate_as(const float (&h)[N], float (&y)[N], float (&d)[N]) {
-#pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const ActOut o = activate<ACT, SLOPE>(h[e]);
-    y[e] = o.y;
-    d[e] = o.d;
-  }
-}
-template <bool SLOPE, int N>
-__device__ __forceinline__ void activate_all(int act, const float (&h)[N], float (&y)[N], float (&d)[N]) {
-  switch (act) {
-    case FX_ACT_RELU: return activate_as<FX_ACT_RELU, SLOPE>(h, y, d);
-    case FX_ACT_SILU: return activate_as<FX_ACT_SILU, SLOPE>(h, y, d);
-    case FX_ACT_GELU: return activate_as<FX_ACT_GELU, SLOPE>(h, y, d);
-    case FX_ACT_GELU_TANH: return activate_as<FX_ACT_GELU_TANH, SLOPE>(h, y, d);
-    case FX_ACT_TANH: return activate_as<FX_ACT_TANH, SLOPE>(h, y, d);
-    default: return activate_as<FX_ACT_NONE, SLOPE>(h, y, d);
-  }
 }
 
 // The type the derivative is kept in: IEEE half beside bfloat16 (within +-1.2, 2^-12 of its value

@@ -2,9 +2,9 @@
 // forward (x, W), dx (g, W) and dW (g, x) alike. Each operand is read as it is stored, along k
 // (K-major) or across it (MN-major).
 //
-// A pair of SMs holds a tile of 256 x 256: each brings 128 rows of A and 128 of B by tensor maps
-// (64 entries of k a stage) and keeps 128 x 256 of the sum in its TMEM, twice, so that one
-// tile's epilogue runs under the next tile's products. The grid is persistent.
+// A pair of SMs holds a tile of 256 x 256 (256 x 128 in float32): each brings 128 rows of A and half
+// of the columns of B by tensor maps (64 entries of k a stage) and keeps 128 rows of the sum in its TMEM,
+// twice or more, so that one tile's epilogue runs under the next tile's products. The grid is persistent.
 //
 // float32 runs on the same bfloat16 instructions: x = x1 + x2 + x3, each part the rest rounded to
 // bfloat16, holds 24 bits, and the six products with index sum <= 4 leave out terms of 2^-24. The
@@ -26,15 +26,22 @@ namespace lin {
 
 using namespace umma;
 
-constexpr int kTile = 256, kHalf = 128, kBlockK = 64;  // of a pair, of an SM, of a stage
-constexpr int kThreads = 320;                          // copies, products, 8 warps of epilogue
-constexpr uint32_t kOperand = kHalf * kBlockK * 2;     // bytes of one SM's rows in a stage
+constexpr int kRows = 256, kHalf = 128, kBlockK = 64;  // rows of a pair and of an SM, entries of k of a stage
+constexpr int kWarps = 16;                             // of the epilogue
+constexpr int kThreads = 64 + 32 * kWarps;             // and one warp for the copies, one for the products
 
+// A stage is one part of 64 entries of k: 128 rows of A and half of the tile's columns of B an SM. bfloat16
+// tiles have 256 columns. The three parts' have 128, which leaves the registers for their sums and is
+// enough to keep the loads below the products.
 template <int NP>
 struct Shape {
-  static constexpr int kStages = NP == 1 ? 6 : 2;
-  static constexpr uint32_t kStage = 2 * NP * kOperand;
-  static constexpr uint32_t kSmem = kStages * kStage + 8 * 4096 + 1024;
+  static constexpr int kCols = NP == 1 ? 256 : 128, kBuffers = 512 / kCols;
+  static constexpr int kStages = NP == 1 ? 5 : 8;
+  static constexpr uint32_t kA = kHalf * kBlockK * 2, kB = kCols / 2 * kBlockK * 2, kStage = kA + kB;
+  static constexpr int kStrip = kCols / 4;         // columns of a warp
+  static constexpr int kStore = NP == 1 ? 32 : 16;  // of them stored at a time
+  static constexpr uint32_t kBlock = 32 * kStore * 4;
+  static constexpr uint32_t kSmem = kStages * kStage + kWarps * kBlock + 1024;
   static constexpr int kChunk = 2;  // blocks of k in an accumulator (three parts)
 };
 
@@ -61,14 +68,22 @@ __device__ __forceinline__ uint32_t cta_rank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// True in one lane of the warp, which is converged: the same one every time.
+__device__ __forceinline__ bool elected() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+  return r != 0;
+}
 // The address of the pair's first block's copy of a shared variable.
 __device__ __forceinline__ uint32_t first_block(const void* p) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
   return r;
 }
+// An arrival that orders TMEM reads alone (with the fence before it): a release to the cluster would wait for the
+// epilogue's stores to memory too, which took most of its time.
 __device__ __forceinline__ void arrive_at(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint32_t bar) {
   asm volatile(
@@ -107,6 +122,12 @@ __device__ __forceinline__ void ld32(uint32_t a, uint32_t (&v)[32]) {
       : FX_R8(v, 0), FX_R8(v, 8), FX_R8(v, 16), FX_R8(v, 24)
       : "r"(a));
 }
+__device__ __forceinline__ void ld16(uint32_t a, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : FX_R8(v, 0), FX_R8(v, 8)
+      : "r"(a));
+}
 #undef FX_R8
 
 // 128-byte swizzled operand: rows of 64 entries of k, or, MN-major, rows of 64 entries across k, 64 of
@@ -122,8 +143,10 @@ __device__ __forceinline__ uint64_t desc(uint32_t saddr, bool mn) {
 enum { RUNS = 0, LATE = 1, DEAD = 2 };
 constexpr uint32_t kLastPolls = 1u << 22;
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* state, uint32_t polls) {
-  if (mbar_wait(bar, parity, polls)) return true;
+  const uint32_t few = polls < 32 ? polls : 32;
+  if (mbar_wait(bar, parity, few)) return true;
   if (*state == DEAD) return false;
+  if (mbar_wait(bar, parity, polls - few)) return true;
   record_status(8);  // FX_ERR_TIMEOUT
   if (*state == RUNS) *state = LATE;
   if (mbar_wait(bar, parity, kLastPolls)) return true;
@@ -132,80 +155,95 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
 }
 
 // ---------------------------------------------------------------- epilogue
-// Four entries of a row from column j, `n` of them there.
-template <typename T>
-__device__ __forceinline__ void epilogue_four(const Epilogue& E, bool vec, int64_t i, int64_t j, int64_t cols, float (&h)[4],
-                                              const float (&bias)[4]) {
+// NaN in the place of sums that a wait did not end for.
+template <int C>
+__device__ __forceinline__ void spoil(int state, uint32_t (&v)[C]) {
+  if (state != RUNS) {
+#pragma unroll
+    for (int e = 0; e < C; ++e) v[e] = 0x7fc00000u;
+  }
+}
+
+constexpr int kPart = -1;  // in the place of an activation: the sums themselves, of a part of k
+
+// N entries of a row: activation, residual, stores.
+template <typename T, int ACT, int N>
+__device__ __forceinline__ void finish(const float (&h)[N], const Pack<T, N>* residual, T* y, typename SlopeOf<T>::type* slope) {
   using TS = typename SlopeOf<T>::type;
+  Pack<T, N> o;
+  Pack<TS, N> d;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) h[e] += bias[e];
-  float y[4], d[4];
-  if (E.slope) activate_all<true>(E.act, h, y, d);
-  else activate_all<false>(E.act, h, y, d);
-  T* out = static_cast<T*>(E.y) + i * cols + j;
-  const T* res = E.residual ? static_cast<const T*>(E.residual) + i * E.rs + j : nullptr;
-  TS* slope = E.slope ? static_cast<TS*>(E.slope) + i * cols + j : nullptr;
-  if (vec) {
-    if (slope) {
-      Pack<TS, 4> s;
+  for (int e = 0; e < N; ++e) {
+    const ActOut a = activate<ACT>(h[e]);
+    o.e[e] = from_f<T>(residual ? a.y + to_f(residual->e[e]) : a.y);
+    d.e[e] = from_f<TS>(a.d);
+  }
+  *reinterpret_cast<Pack<T, N>*>(y) = o;
+  if (ACT != FX_ACT_NONE && slope) *reinterpret_cast<Pack<TS, N>*>(slope) = d;
+}
+
+// 32 x C entries of the sum, a row a lane, through shared memory to N = 4 entries of a row a lane (or, where
+// rows are not whole pieces of four, N = 1), so that stores cover whole sectors. G.rows and G.cols end the result.
+template <typename T, int ACT, int C, int N>
+__device__ __forceinline__ void store_rows(const Args& G, const unsigned char* stage, int64_t i0, int64_t j0, int split) {
+  using TS = typename SlopeOf<T>::type;
+  constexpr int L = C / N, R = 32 / L;         // lanes of a row, rows at a time
+  constexpr int U = N == 4 ? C / 8 : 8;        // and as many times before the next residuals are read
+  const int lane = threadIdx.x & 31, c = lane % L * N, r0 = lane / L;
+  const int64_t j = j0 + c, i = i0 + r0;
+  const int last = (int)(G.rows - i < 32 ? G.rows - i : 32);  // of the rows from r0 on
+  if (j >= G.cols) return;
+  const auto at = [&](int r) {
+    const int p = c / 4;
+    return stage + r * (C * 4) + (((C == 32 ? p ^ (r & 7) : p ^ (r >> 1 & 3)) << 4) + (c & 3) * 4);
+  };
+  if constexpr (ACT == kPart) {
+    float* out = G.part + (split * G.rows + i) * G.part_ld + j;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s.e[e] = from_f<TS>(d[e]);
-      *reinterpret_cast<Pack<TS, 4>*>(slope) = s;
-    }
-    if (res) {
-      const Pack<T, 4> r = *reinterpret_cast<const Pack<T, 4>*>(res);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] += to_f(r.e[e]);
-    }
-    Pack<T, 4> o;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o.e[e] = from_f<T>(y[e]);
-    *reinterpret_cast<Pack<T, 4>*>(out) = o;
+    for (int k = 0; k < 32; k += R, out += R * G.part_ld)
+      if (k < last) *reinterpret_cast<Pack<float, N>*>(out) = *reinterpret_cast<const Pack<float, N>*>(at(k + r0));
   } else {
+    float bias[N];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (j + e >= cols) break;
-      if (slope) slope[e] = from_f<TS>(d[e]);
-      out[e] = from_f<T>(res ? to_f(res[e]) + y[e] : y[e]);
+    for (int e = 0; e < N; ++e) bias[e] = G.e.bias ? to_f(static_cast<const T*>(G.e.bias)[j + e]) : 0.f;
+    T* y = static_cast<T*>(G.e.y) + i * G.cols + j;
+    TS* slope = G.e.slope ? static_cast<TS*>(G.e.slope) + i * G.cols + j : nullptr;
+    const T* residual = G.e.residual ? static_cast<const T*>(G.e.residual) + i * G.e.rs + j : nullptr;
+    const int64_t step = R * G.cols;
+#pragma unroll 1
+    for (int k0 = 0; k0 < 32; k0 += U * R) {
+      Pack<T, N> res[U];
+      if (residual) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (k0 + u * R < last) res[u] = *reinterpret_cast<const Pack<T, N>*>(residual + (k0 + u * R) * G.e.rs);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const Pack<float, N> x = *reinterpret_cast<const Pack<float, N>*>(at(k0 + u * R + r0));
+        float h[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) h[e] = x.e[e] + bias[e];
+        if (k0 + u * R < last) finish<T, ACT, N>(h, residual ? &res[u] : nullptr, y, slope);
+        y += step;
+        if (slope) slope += step;
+      }
     }
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void load_bias(const Epilogue& E, int64_t j, int64_t cols, float (&bias)[4]) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) bias[e] = E.bias && j + e < cols ? to_f(static_cast<const T*>(E.bias)[j + e]) : 0.f;
-}
-
-// 32 x 32 entries of the sum, a row a lane, through shared memory to four entries of a row a
-// lane (eight lanes a row), so that stores cover whole sectors.
-template <typename T>
-__device__ __forceinline__ void store_block(const Args& G, unsigned char* stage, int64_t i0, int64_t j0, int split, bool late,
-                                            const uint32_t (&v)[32]) {
+template <typename T, int ACT, int C>
+__device__ __forceinline__ void store_block(const Args& G, unsigned char* stage, int64_t i0, int64_t j0, int split,
+                                            const uint32_t (&v)[C]) {
   const int lane = threadIdx.x & 31;
   __syncwarp();
 #pragma unroll
-  for (int p = 0; p < 8; ++p)
-    *reinterpret_cast<uint4*>(stage + lane * 128 + ((p ^ (lane & 7)) << 4)) =
+  for (int p = 0; p < C / 4; ++p)
+    *reinterpret_cast<uint4*>(stage + lane * (C * 4) + ((C == 32 ? p ^ (lane & 7) : p ^ (lane >> 1 & 3)) << 4)) =
         make_uint4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
   __syncwarp();
-  const int piece = lane & 7;
-  const int64_t j = j0 + piece * 4;
-  float bias[4];
-  if (!G.part) load_bias<T>(G.e, j, G.cols, bias);
-#pragma unroll 2
-  for (int s = 0; s < 8; ++s) {
-    const int r = s * 4 + (lane >> 3);
-    float4 x = *reinterpret_cast<const float4*>(stage + r * 128 + ((piece ^ (r & 7)) << 4));
-    if (i0 + r >= G.rows || j >= G.cols) continue;
-    if (late) x.x = x.y = x.z = x.w = __int_as_float(0x7fc00000);
-    if (G.part) {
-      *reinterpret_cast<float4*>(G.part + (split * G.rows + i0 + r) * G.part_ld + j) = x;
-    } else {
-      float h[4] = {x.x, x.y, x.z, x.w};
-      epilogue_four<T>(G.e, G.vec, i0 + r, j, G.cols, h, bias);
-    }
-  }
+  if (ACT == kPart || G.vec) store_rows<T, ACT, C, 4>(G, stage, i0, j0, split);
+  else if constexpr (ACT != kPart) store_rows<T, ACT, C, 1>(G, stage, i0, j0, split);
 }
 
 struct Unit {
@@ -225,14 +263,14 @@ __device__ __forceinline__ Unit unit_of(const Args& G, int u) {
   return U;
 }
 
-template <typename T, int NP>
+template <typename T, int NP, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     linear_tc_kernel(const __grid_constant__ Args G, const __grid_constant__ Maps M) {
   using S = Shape<NP>;
   constexpr int ST = S::kStages;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
-  __shared__ uint64_t full[ST], empty[ST], sum_full[2], sum_empty[2];
+  __shared__ uint64_t full[ST], empty[ST], sum_full[S::kBuffers], sum_empty[S::kBuffers];
   __shared__ uint32_t slot;
   __shared__ volatile int state;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -243,9 +281,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < S::kBuffers; ++i) {
       mbar_init(&sum_full[i], 1);
-      mbar_init(&sum_empty[i], 16);  // the epilogue's warps of both blocks
+      mbar_init(&sum_empty[i], 2 * kWarps);  // the epilogue's warps of both blocks
     }
     fence_mbar_init();
   }
@@ -264,15 +302,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int it = 0;
       for (int u = blockIdx.x >> 1; u < units && state != DEAD; u += pairs) {
         const Unit U = unit_of(G, u);
-        const int i0 = U.m * kTile + rank * kHalf, j0 = U.n * kTile + rank * kHalf;
-        for (int kb = U.first; kb < U.last; ++kb, ++it) {
-          const int st = it % ST;
-          if (!wait(&empty[st], (it / ST & 1) ^ 1, &state, G.polls)) break;
-          const uint32_t bar = first_block(&full[st]), at = smem_u32(sm) + st * S::kStage;
-          if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * S::kStage);
-#pragma unroll
-          for (int p = 0; p < NP; ++p) {
-            const uint32_t a = at + p * kOperand, b = at + (NP + p) * kOperand;
+        const int i0 = U.m * kRows + rank * kHalf, j0 = U.n * S::kCols + rank * (S::kCols / 2);
+        for (int kb = U.first; kb < U.last; ++kb) {
+#pragma unroll 1
+          for (int p = 0; p < NP; ++p, ++it) {
+            const int st = it % ST;
+            if (!wait(&empty[st], (it / ST & 1) ^ 1, &state, G.polls)) break;
+            const uint32_t bar = first_block(&full[st]), a = smem_u32(sm) + st * S::kStage, b = a + S::kA;
+            if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * S::kStage);
             if (G.a_mn) {
               tma_box(a, &M.a, i0, kb * kBlockK, p, bar);
               tma_box(a + 8192, &M.a, i0 + 64, kb * kBlockK, p, bar);
@@ -281,7 +318,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
             if (G.b_mn) {
               tma_box(b, &M.b, j0, kb * kBlockK, p, bar);
-              tma_box(b + 8192, &M.b, j0 + 64, kb * kBlockK, p, bar);
+              if (S::kB > 8192) tma_box(b + 8192, &M.b, j0 + 64, kb * kBlockK, p, bar);
             } else {
               tma_box(b, &M.b, kb * kBlockK, j0, p, bar);
             }
@@ -293,77 +330,101 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (int j = it > ST ? it - ST : 0; j < it; ++j) mbar_wait(&full[j % ST], j / ST & 1, 1u << 20);
     }
   } else if (warp == 1) {
-    // -------------------------------------------------------- products, one thread of the pair
-    if (lane == 0 && rank == 0) {
+    // -------------------------------------------------------- products, one warp of the pair
+    // The whole warp runs the loops, so that descriptors stay in uniform registers, and one lane issues.
+    if (rank == 0) {
       const uint32_t idesc = 1u << 4 | 1u << 7 | 1u << 10 | (G.a_mn ? 1u << 15 : 0u) | (G.b_mn ? 1u << 16 : 0u) |
-                             (uint32_t)(kTile >> 3) << 17 | (uint32_t)(kTile >> 4) << 24;
+                             (uint32_t)(S::kCols >> 3) << 17 | (uint32_t)(kRows >> 4) << 24;
       const uint32_t sa = G.a_mn ? 128 : 2, sb = G.b_mn ? 128 : 2;  // 16 entries of k further, in 16 bytes
-      int it = 0, ch = 0;
+      const uint64_t a0 = desc(smem_u32(sm), G.a_mn), b0 = desc(smem_u32(sm) + S::kA, G.b_mn);
+      int st = 0, ch = 0;
+      uint32_t phase = 0;
       for (int u = blockIdx.x >> 1; u < units && state != DEAD; u += pairs) {
         const Unit U = unit_of(G, u);
         for (int k0 = U.first; k0 < U.last; k0 += chunk, ++ch) {
-          const int buf = ch & 1;
-          if (!wait(&sum_empty[buf], (ch >> 1 & 1) ^ 1, &state, G.polls)) break;
+          const int buf = ch % S::kBuffers;
+          if (!wait(&sum_empty[buf], (ch / S::kBuffers & 1) ^ 1, &state, G.polls)) break;
           fence_after_sync();
-          const uint32_t d = tmem + buf * kTile;
-          bool acc = false;
-          for (int kb = k0; kb < min(k0 + chunk, U.last); ++kb, ++it) {
-            const int st = it % ST;
-            if (!wait(&full[st], it / ST & 1, &state, G.polls)) break;
-            fence_after_sync();
-            const uint32_t at = smem_u32(sm) + st * S::kStage;
+          const uint32_t d = tmem + buf * S::kCols;
+          const int k1 = min(k0 + chunk, U.last);
+          for (int kb = k0; kb < k1; ++kb) {
+            int at[NP];  // the stages of the parts
 #pragma unroll
-            for (int sum = NP - 1; sum >= 0; --sum) {  // the smaller products first
+            for (int p = 0; p < NP; ++p) {
+              at[p] = st;
+              if (!wait(&full[st], phase, &state, G.polls)) break;
+              fence_after_sync();
+              if (elected()) {
+                // the products of this part with those before it, and what is left out of none: index sum <= 4
 #pragma unroll
-              for (int i = 0; i <= sum; ++i) {
-                uint64_t a = desc(at + i * kOperand, G.a_mn), b = desc(at + (NP + sum - i) * kOperand, G.b_mn);
+                for (int q = 0; q <= p; ++q) {
 #pragma unroll
-                for (int k = 0; k < kBlockK / 16; ++k) {
-                  mma_pair(d, a, b, idesc, acc);
-                  acc = true;
-                  a += sa;
-                  b += sb;
+                  for (int t = 0; t < (p == q ? 1 : 2); ++t) {
+                    const int i = t ? q : p, j = t ? p : q;
+                    if (i + j >= NP) continue;
+                    const uint64_t a1 = a0 + (uint32_t)(at[i] * (S::kStage >> 4)), b1 = b0 + (uint32_t)(at[j] * (S::kStage >> 4));
+#pragma unroll
+                    for (int k = 0; k < kBlockK / 16; ++k)
+                      mma_pair(d, a1 + k * sa, b1 + k * sb, idesc, kb > k0 || i > 0 || j > 0 || k > 0);
+                  }
+                }
+                if (p == NP - 1) {
+#pragma unroll
+                  for (int q = 0; q < NP; ++q) commit_pair(&empty[at[q]]);
+                  if (kb == k1 - 1) commit_pair(&sum_full[buf]);
                 }
               }
+              __syncwarp();
+              if (++st == ST) {
+                st = 0;
+                phase ^= 1;
+              }
             }
-            commit_pair(&empty[st]);
           }
-          commit_pair(&sum_full[buf]);
         }
       }
-      if (state == DEAD && ch > 0) mbar_wait(&sum_full[(ch - 1) & 1], (ch - 1) >> 1 & 1, 1u << 20);
+      if (state == DEAD && ch > 0) mbar_wait(&sum_full[(ch - 1) % S::kBuffers], (ch - 1) / S::kBuffers & 1, 1u << 20);
     }
   } else {
     // -------------------------------------------------------- epilogue
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    unsigned char* stage = sm + ST * S::kStage + (warp - 2) * 4096;
-    const uint32_t lanes = tmem + ((uint32_t)quarter << 21) + half * 128;
+    constexpr int C = S::kStore, B = S::kStrip / C;
+    const int quarter = warp & 3, strip = (warp - 2) >> 2;
+    unsigned char* stage = sm + ST * S::kStage + (warp - 2) * S::kBlock;
+    const uint32_t lanes = tmem + ((uint32_t)quarter << 21) + strip * S::kStrip;
     int ch = 0;
     for (int u = blockIdx.x >> 1; u < units && state != DEAD; u += pairs) {
       const Unit U = unit_of(G, u);
-      const int64_t i0 = (int64_t)U.m * kTile + rank * kHalf + quarter * 32, j0 = (int64_t)U.n * kTile + half * 128;
-      float acc[NP == 1 ? 1 : 4][32];
+      const int64_t i0 = (int64_t)U.m * kRows + rank * kHalf + quarter * 32, j0 = (int64_t)U.n * S::kCols + strip * S::kStrip;
+      float acc[NP == 1 ? 1 : B][C];
       for (int k0 = U.first; k0 < U.last; k0 += chunk, ++ch) {
-        const int buf = ch & 1;
-        if (!wait(&sum_full[buf], ch >> 1 & 1, &state, G.polls)) break;
+        const int buf = ch % S::kBuffers;
+        if (!wait(&sum_full[buf], ch / S::kBuffers & 1, &state, G.polls)) break;
         fence_after_sync();
+        const uint32_t from = lanes + buf * S::kCols;
         if constexpr (NP == 1) {
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            if (j0 + c * 32 >= G.cols) break;
-            uint32_t v[32];
-            ld32(lanes + buf * kTile + c * 32, v);
+          for (int c = 0; c < B; ++c) {
+            if (j0 + c * C >= G.cols) break;
+            uint32_t v[C];
+            ld32(from + c * C, v);
             tmem_wait_ld();
-            store_block<T>(G, stage, i0, j0 + c * 32, U.split, state != RUNS, v);
+            spoil(state, v);
+            store_block<T, ACT, C>(G, stage, i0, j0 + c * C, U.split, v);
           }
         } else {
+          const bool more = k0 > U.first;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
-            ld32(lanes + buf * kTile + c * 32, v);
+          for (int c = 0; c < B; ++c) {
+            uint32_t v[C];
+            ld16(from + c * C, v);
             tmem_wait_ld();
+            if (more) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) acc[c][e] = (k0 == U.first ? 0.f : acc[c][e]) + __uint_as_float(v[e]);
+              for (int e = 0; e < C; ++e) acc[c][e] += __uint_as_float(v[e]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < C; ++e) acc[c][e] = __uint_as_float(v[e]);
+            }
           }
         }
         fence_before_sync();
@@ -372,12 +433,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       if constexpr (NP > 1) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (j0 + c * 32 >= G.cols) break;
-          uint32_t v[32];
+        for (int c = 0; c < B; ++c) {
+          if (j0 + c * C >= G.cols) break;
+          uint32_t v[C];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(acc[c][e]);
-          store_block<T>(G, stage, i0, j0 + c * 32, U.split, state != RUNS, v);
+          for (int e = 0; e < C; ++e) v[e] = __float_as_uint(acc[c][e]);
+          spoil(state, v);
+          store_block<T, ACT, C>(G, stage, i0, j0 + c * C, U.split, v);
         }
       }
     }
@@ -391,13 +453,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // ---------------------------------------------------------------- around the products
 // The parts of a split sum in order, then the epilogue; four columns a thread.
-template <typename T>
+template <typename T, int ACT>
 __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ Args G) {
   const int64_t quads = G.part_ld / 4, n = G.rows * quads;
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
     const int64_t i = t / quads, j = (t - i * quads) * 4;
     const float* p = G.part + i * G.part_ld + j;
-    float h[4] = {0.f, 0.f, 0.f, 0.f}, bias[4];
+    float h[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int s = 0; s < G.splits; ++s) {
       const float4 x = *reinterpret_cast<const float4*>(p + s * G.rows * G.part_ld);
@@ -406,8 +468,27 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
       h[2] += x.z;
       h[3] += x.w;
     }
-    load_bias<T>(G.e, j, G.cols, bias);
-    epilogue_four<T>(G.e, G.vec, i, j, G.cols, h, bias);
+    using TS = typename SlopeOf<T>::type;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (G.e.bias && j + e < G.cols) h[e] += to_f(static_cast<const T*>(G.e.bias)[j + e]);
+    T* y = static_cast<T*>(G.e.y) + i * G.cols + j;
+    TS* slope = G.e.slope ? static_cast<TS*>(G.e.slope) + i * G.cols + j : nullptr;
+    const T* residual = G.e.residual ? static_cast<const T*>(G.e.residual) + i * G.e.rs + j : nullptr;
+    if (G.vec) {
+      Pack<T, 4> res;
+      if (residual) res = *reinterpret_cast<const Pack<T, 4>*>(residual);
+      finish<T, ACT, 4>(h, residual ? &res : nullptr, y, slope);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (j + e >= G.cols) break;
+        Pack<T, 1> res;
+        if (residual) res.e[0] = residual[e];
+        const float one[1] = {h[e]};
+        finish<T, ACT, 1>(one, residual ? &res : nullptr, y + e, slope ? slope + e : nullptr);
+      }
+    }
   }
 }
 
