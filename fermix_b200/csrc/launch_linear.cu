@@ -143,12 +143,12 @@ int make_map(CUtensorMap* m, const Operand& o, int planes, bool mn, int rows) {
              : FX_ERR_CUDA;
 }
 
-// Whether y, slope and the residual are rows of whole pieces of four entries.
-bool fours(const Epilogue& e, int64_t rows, int64_t cols, int size) {
-  const uintptr_t piece = 4 * size;
+// Whether y, slope and the residual are rows of whole 16-byte pieces.
+bool pieces(const Epilogue& e, int64_t rows, int64_t cols, int size) {
   const uintptr_t m = reinterpret_cast<uintptr_t>(e.y) | reinterpret_cast<uintptr_t>(e.slope) |
-                      reinterpret_cast<uintptr_t>(e.residual) | (uintptr_t)(e.residual && rows > 1 ? e.rs * size : 0);
-  return cols % 4 == 0 && m % piece == 0;
+                      reinterpret_cast<uintptr_t>(e.residual) | (uintptr_t)(e.residual && rows > 1 ? e.rs * size : 0) |
+                      (uintptr_t)(cols * size);
+  return m % 16 == 0;
 }
 
 template <typename T, int NP, int ACT>
@@ -158,8 +158,11 @@ int launch(cudaStream_t s, const lin::Args& G, const lin::Maps& M, int64_t pairs
     auto kern = lin::linear_tc_kernel<T, NP, lin::kPart>;
     if (raise_smem(kern, smem, smem)) return FX_ERR_CUDA;
     kern<<<(unsigned)(2 * pairs), lin::kThreads, smem, s>>>(G, M);
-    const int64_t blocks = ceil_div(G.rows * G.part_ld / 4, 256), most = (int64_t)sms * 8;
-    lin::linear_join_kernel<T, ACT><<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(G);
+    constexpr int N = 16 / sizeof(T);
+    const int64_t blocks = ceil_div(G.rows * G.cols / (G.vec ? N : 1), 256), most = (int64_t)sms * 8;
+    const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+    if (G.vec) lin::linear_join_kernel<T, ACT, N><<<grid, 256, 0, s>>>(G);
+    else lin::linear_join_kernel<T, ACT, 1><<<grid, 256, 0, s>>>(G);
   } else {
     auto kern = lin::linear_tc_kernel<T, NP, ACT>;
     if (raise_smem(kern, smem, smem)) return FX_ERR_CUDA;
@@ -186,7 +189,7 @@ int product(cudaStream_t s, const Cut& C, const Operand& a, bool a_mn, const Ope
   G.per = C.per;
   G.a_mn = a_mn;
   G.b_mn = b_mn;
-  G.vec = fours(e, C.rows, C.cols, sizeof(T));
+  G.vec = pieces(e, C.rows, C.cols, sizeof(T));
   G.polls = wait_polls();
   G.part = C.splits > 1 ? part : nullptr;
   G.part_ld = C.part_ld();

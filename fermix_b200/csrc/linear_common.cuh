@@ -6,9 +6,24 @@
 
 namespace fx {
 
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + __expf(fminf(-x, 80.f))); }
+// 2^x and 1 / x, to 2^-22 of the value.
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fast_inverse(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 1 / (1 + exp(-x)), of scale x where scale is given
+__device__ __forceinline__ float sigmoid(float x, float scale = 1.f) {
+  return fast_inverse(1.f + fast_exp2(x * (-1.4426950408889634f * scale)));
+}
 
-// h -> (act(h), act'(h))
+// h -> (act(h), act'(h)). Finite at every finite h: where an exponential overflows, its inverse is 0. The products
+// are rounded by themselves, so that act(h) has the same bits whatever is done with it.
 struct ActOut {
   float y, d;
 };
@@ -17,37 +32,37 @@ template <int ACT>
 __device__ __forceinline__ ActOut activate(float h) {
   ActOut o;
   o.d = 1.f;
-  if constexpr (ACT == FX_ACT_NONE) {
-    o.y = h;
-  } else if constexpr (ACT == FX_ACT_RELU) {
-    o.y = h > 0.f ? h : 0.f * h;  // a NaN stays
-    o.d = h > 0.f ? 1.f : 0.f;
-    if (h != h) o.d = h;
-    if (h < 0.f) o.y = 0.f;
+  if constexpr (ACT == FX_ACT_RELU) {
+    o.y = h < 0.f ? 0.f : h;  // a NaN stays
+    o.d = h > 0.f ? 1.f : h != h ? h : 0.f;
   } else if constexpr (ACT == FX_ACT_SILU) {
     const float s = sigmoid(h);
-    o.y = h < -80.f ? 0.f : h * s;
-    o.d = s * fmaf(fmaxf(h, -80.f), 1.f - s, 1.f);
+    o.y = __fmul_rn(h, s);
+    o.d = fmaf(o.y, 1.f - s, s);
   } else if constexpr (ACT == FX_ACT_GELU) {
     // erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + p x), x >= 0: Abramowitz and Stegun 7.1.26, off by
-    // 1.5e-7 at most. With x = |h| / sqrt 2 the exponential is the normal density's.
-    const float x = fabsf(h) * 0.70710678118654752f, t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f)), e = __expf(-x * x);
-    const float q = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-    const float tail = 0.5f * q * e, c = h < 0.f ? tail : 1.f - tail;
-    o.y = h < -14.f ? 0.f : h * c;
-    o.d = fmaf(fminf(fmaxf(h, -20.f), 20.f) * 0.3989422804014327f, e, c);
+    // 1.5e-7 at most. With x = |h| / sqrt 2 the exponential is the normal density's; the halves are in the a's.
+    const float t = fast_inverse(fmaf(0.3275911f * 0.70710678118654752f, fabsf(h), 1.f));
+    const float e = fast_exp2(h * h * (-0.5f * 1.4426950408889634f));
+    const float q = fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f), 0.5f * 1.421413741f),
+                                 0.5f * -0.284496736f), 0.5f * 0.254829592f);
+    const float tail = q * (t * e), c = h < 0.f ? tail : 1.f - tail;
+    o.y = __fmul_rn(h, c);
+    o.d = fmaf(h * 0.3989422804014327f, e, c);
   } else if constexpr (ACT == FX_ACT_GELU_TANH) {
-    // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u))
-    const float k = 1.5957691216057308f, h2 = fminf(h * h, 1e6f);
-    const float s = sigmoid(k * h * fmaf(0.044715f, h2, 1.f));
-    o.y = h < -10.f ? 0.f : h * s;
-    o.d = fabsf(h) > 12.f ? s : s * fmaf(h * (1.f - s), k * fmaf(0.134145f, h2, 1.f), 1.f);
-  } else {
+    // (1 + tanh u) / 2 is the sigmoid of 2 u
+    const float k = 1.5957691216057308f, h2 = h * h;
+    const float s = sigmoid(h * fmaf(0.044715f, h2, 1.f), k);
+    o.y = __fmul_rn(h, s);
+    o.d = fmaf(o.y * (1.f - s), k * fmaf(0.134145f, fminf(h2, 1e6f), 1.f), s);
+  } else if constexpr (ACT == FX_ACT_TANH) {
     // tanh u = 2 sigmoid(2 u) - 1; near 0, where that cancels, its series (the next term is 5e-8 of it)
     const float h2 = h * h;
-    o.y = h2 < 0.09f ? h * fmaf(h2, fmaf(h2, fmaf(h2, fmaf(h2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f)
-                     : fmaf(2.f, sigmoid(2.f * h), -1.f);
+    o.y = h2 < 0.09f ? __fmul_rn(h, fmaf(h2, fmaf(h2, fmaf(h2, fmaf(h2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f))
+                     : fmaf(2.f, sigmoid(h, 2.f), -1.f);
     o.d = fmaf(-o.y, o.y, 1.f);
+  } else {
+    o.y = h;
   }
   return o;
 }
@@ -66,6 +81,31 @@ __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
 template <>
 __device__ __forceinline__ __half from_f<__half>(float x) {
   return __float2half_rn(x);
+}
+
+// N entries rounded into a pack, two at a time where the type has it.
+template <int N>
+__device__ __forceinline__ void round_into(Pack<float, N>& o, const float (&x)[N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) o.e[e] = x[e];
+}
+template <int N>
+__device__ __forceinline__ void round_into(Pack<bf16, N>& o, const float (&x)[N]) {
+  if constexpr (N == 1) {
+    o.e[0] = __float2bfloat16_rn(x[0]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) *reinterpret_cast<__nv_bfloat162*>(&o.e[e]) = __floats2bfloat162_rn(x[e], x[e + 1]);
+  }
+}
+template <int N>
+__device__ __forceinline__ void round_into(Pack<__half, N>& o, const float (&x)[N]) {
+  if constexpr (N == 1) {
+    o.e[0] = __float2half_rn(x[0]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) *reinterpret_cast<__half2*>(&o.e[e]) = __floats2half2_rn(x[e], x[e + 1]);
+  }
 }
 
 // What is done with a sum h of the product: bias, activation, derivative, residual, store.

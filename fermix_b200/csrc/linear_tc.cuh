@@ -167,71 +167,106 @@ __device__ __forceinline__ void spoil(int state, uint32_t (&v)[C]) {
 constexpr int kPart = -1;  // in the place of an activation: the sums themselves, of a part of k
 
 // N entries of a row: activation, residual, stores.
-template <typename T, int ACT, int N>
-__device__ __forceinline__ void finish(const float (&h)[N], const Pack<T, N>* residual, T* y, typename SlopeOf<T>::type* slope) {
-  using TS = typename SlopeOf<T>::type;
-  Pack<T, N> o;
-  Pack<TS, N> d;
+template <typename T, int ACT, int N, bool RES, bool SLOPE>
+__device__ __forceinline__ void finish(const float (&h)[N], const Pack<T, N>& residual, T* y, typename SlopeOf<T>::type* slope) {
+  float v[N], d[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) {
     const ActOut a = activate<ACT>(h[e]);
-    o.e[e] = from_f<T>(residual ? a.y + to_f(residual->e[e]) : a.y);
-    d.e[e] = from_f<TS>(a.d);
+    v[e] = RES ? a.y + to_f(residual.e[e]) : a.y;
+    d[e] = a.d;
   }
+  Pack<T, N> o;
+  round_into<N>(o, v);
   *reinterpret_cast<Pack<T, N>*>(y) = o;
-  if (ACT != FX_ACT_NONE && slope) *reinterpret_cast<Pack<TS, N>*>(slope) = d;
+  if constexpr (SLOPE) {
+    Pack<typename SlopeOf<T>::type, N> s;
+    round_into<N>(s, d);
+    *reinterpret_cast<Pack<typename SlopeOf<T>::type, N>*>(slope) = s;
+  }
 }
 
-// 32 x C entries of the sum, a row a lane, through shared memory to N = 4 entries of a row a lane (or, where
-// rows are not whole pieces of four, N = 1), so that stores cover whole sectors. G.rows and G.cols end the result.
-template <typename T, int ACT, int C, int N>
-__device__ __forceinline__ void store_rows(const Args& G, const unsigned char* stage, int64_t i0, int64_t j0, int split) {
+// Where a staged entry is: rows of C, 16-byte pieces swizzled.
+template <int C>
+__device__ __forceinline__ uint32_t staged(int r, int piece) {
+  return r * (C * 4) + ((C == 32 ? piece ^ (r & 7) : piece ^ (r >> 1 & 3)) << 4);
+}
+
+// Of 32 x C staged entries of the sum, N entries of a row a lane (16 bytes of the result, or, where rows are
+// not whole pieces, one), so that stores cover whole sectors. G.rows and G.cols end the result.
+template <typename T, int ACT, int C, int N, bool RES, bool SLOPE>
+__device__ __forceinline__ void store_rows(const Args& G, const unsigned char* stage, int64_t i0, int64_t j0) {
   using TS = typename SlopeOf<T>::type;
-  constexpr int L = C / N, R = 32 / L;         // lanes of a row, rows at a time
-  constexpr int U = N == 4 ? C / 8 : 8;        // and as many times before the next residuals are read
+  constexpr int L = C / N, R = 32 / L;       // lanes of a row, rows at a time
+  constexpr int U = N == 1 ? 8 : 2;          // and as many times before the next residuals are read
   const int lane = threadIdx.x & 31, c = lane % L * N, r0 = lane / L;
   const int64_t j = j0 + c, i = i0 + r0;
   const int last = (int)(G.rows - i < 32 ? G.rows - i : 32);  // of the rows from r0 on
   if (j >= G.cols) return;
-  const auto at = [&](int r) {
-    const int p = c / 4;
-    return stage + r * (C * 4) + (((C == 32 ? p ^ (r & 7) : p ^ (r >> 1 & 3)) << 4) + (c & 3) * 4);
-  };
-  if constexpr (ACT == kPart) {
-    float* out = G.part + (split * G.rows + i) * G.part_ld + j;
+  float bias[N];
 #pragma unroll
-    for (int k = 0; k < 32; k += R, out += R * G.part_ld)
-      if (k < last) *reinterpret_cast<Pack<float, N>*>(out) = *reinterpret_cast<const Pack<float, N>*>(at(k + r0));
-  } else {
-    float bias[N];
-#pragma unroll
-    for (int e = 0; e < N; ++e) bias[e] = G.e.bias ? to_f(static_cast<const T*>(G.e.bias)[j + e]) : 0.f;
-    T* y = static_cast<T*>(G.e.y) + i * G.cols + j;
-    TS* slope = G.e.slope ? static_cast<TS*>(G.e.slope) + i * G.cols + j : nullptr;
-    const T* residual = G.e.residual ? static_cast<const T*>(G.e.residual) + i * G.e.rs + j : nullptr;
-    const int64_t step = R * G.cols;
+  for (int e = 0; e < N; ++e) bias[e] = G.e.bias ? to_f(static_cast<const T*>(G.e.bias)[j + e]) : 0.f;
+  T* y = static_cast<T*>(G.e.y) + i * G.cols + j;
+  TS* slope = SLOPE ? static_cast<TS*>(G.e.slope) + i * G.cols + j : nullptr;
+  const T* residual = RES ? static_cast<const T*>(G.e.residual) + i * G.e.rs + j : nullptr;
+  const int64_t step = R * G.cols, rstep = R * G.e.rs;
 #pragma unroll 1
-    for (int k0 = 0; k0 < 32; k0 += U * R) {
-      Pack<T, N> res[U];
-      if (residual) {
+  for (int k0 = 0; k0 < 32; k0 += U * R) {
+    Pack<T, N> res[U];
+    if constexpr (RES) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (k0 + u * R < last) res[u] = *reinterpret_cast<const Pack<T, N>*>(residual + (k0 + u * R) * G.e.rs);
+      for (int u = 0; u < U; ++u, residual += rstep)
+        if (k0 + u * R < last) res[u] = *reinterpret_cast<const Pack<T, N>*>(residual);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float h[N];
+      if constexpr (N == 1) {
+        h[0] = *reinterpret_cast<const float*>(stage + staged<C>(k0 + u * R + r0, c / 4) + (c & 3) * 4);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; e += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(stage + staged<C>(k0 + u * R + r0, (c + e) / 4));
+          h[e] = x.x;
+          h[e + 1] = x.y;
+          h[e + 2] = x.z;
+          h[e + 3] = x.w;
+        }
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const Pack<float, N> x = *reinterpret_cast<const Pack<float, N>*>(at(k0 + u * R + r0));
-        float h[N];
-#pragma unroll
-        for (int e = 0; e < N; ++e) h[e] = x.e[e] + bias[e];
-        if (k0 + u * R < last) finish<T, ACT, N>(h, residual ? &res[u] : nullptr, y, slope);
-        y += step;
-        if (slope) slope += step;
-      }
+      for (int e = 0; e < N; ++e) h[e] += bias[e];
+      if (k0 + u * R < last) finish<T, ACT, N, RES, SLOPE>(h, res[u], y, slope);
+      y += step;
+      if constexpr (SLOPE) slope += step;
     }
   }
 }
 
+template <typename T, int ACT, int C, int N>
+__device__ __forceinline__ void store_rows(const Args& G, const unsigned char* stage, int64_t i0, int64_t j0) {
+  if (ACT != FX_ACT_NONE && G.e.slope) {
+    if (G.e.residual) store_rows<T, ACT, C, N, true, true>(G, stage, i0, j0);
+    else store_rows<T, ACT, C, N, false, true>(G, stage, i0, j0);
+  } else {
+    if (G.e.residual) store_rows<T, ACT, C, N, true, false>(G, stage, i0, j0);
+    else store_rows<T, ACT, C, N, false, false>(G, stage, i0, j0);
+  }
+}
+
+// The sums themselves, four a lane; the parts' rows are whole pieces.
+template <int C>
+__device__ __forceinline__ void store_part(const Args& G, const unsigned char* stage, int64_t i0, int64_t j0, int split) {
+  constexpr int L = C / 4, R = 32 / L;
+  const int lane = threadIdx.x & 31, r0 = lane / L;
+  const int64_t j = j0 + lane % L * 4, i = i0 + r0;
+  if (j >= G.cols) return;
+  float* out = G.part + (split * G.rows + i) * G.part_ld + j;
+#pragma unroll
+  for (int k = 0; k < 32; k += R, out += R * G.part_ld)
+    if (i + k < G.rows) *reinterpret_cast<float4*>(out) = *reinterpret_cast<const float4*>(stage + staged<C>(k + r0, lane % L));
+}
+
+// 32 x C entries of the sum, a row a lane, through shared memory to memory.
 template <typename T, int ACT, int C>
 __device__ __forceinline__ void store_block(const Args& G, unsigned char* stage, int64_t i0, int64_t j0, int split,
                                             const uint32_t (&v)[C]) {
@@ -239,11 +274,14 @@ __device__ __forceinline__ void store_block(const Args& G, unsigned char* stage,
   __syncwarp();
 #pragma unroll
   for (int p = 0; p < C / 4; ++p)
-    *reinterpret_cast<uint4*>(stage + lane * (C * 4) + ((C == 32 ? p ^ (lane & 7) : p ^ (lane >> 1 & 3)) << 4)) =
-        make_uint4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
+    *reinterpret_cast<uint4*>(stage + staged<C>(lane, p)) = make_uint4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
   __syncwarp();
-  if (ACT == kPart || G.vec) store_rows<T, ACT, C, 4>(G, stage, i0, j0, split);
-  else if constexpr (ACT != kPart) store_rows<T, ACT, C, 1>(G, stage, i0, j0, split);
+  if constexpr (ACT == kPart) {
+    store_part<C>(G, stage, i0, j0, split);
+  } else {
+    if (G.vec) store_rows<T, ACT, C, 16 / sizeof(T)>(G, stage, i0, j0);
+    else store_rows<T, ACT, C, 1>(G, stage, i0, j0);
+  }
 }
 
 struct Unit {
@@ -253,11 +291,11 @@ struct Unit {
 // rows and columns; the parts of a tile next to each other.
 __device__ __forceinline__ Unit unit_of(const Args& G, int u) {
   Unit U;
-  const int t = u / G.splits, group = t / (8 * G.tn), in = t - group * 8 * G.tn;
+  const int t = G.splits == 1 ? u : u / G.splits, group = t / (8 * G.tn), in = t - group * 8 * G.tn;
   const int rows = min(8, G.tm - group * 8);
   U.split = u - t * G.splits;
-  U.m = group * 8 + in % rows;
-  U.n = in / rows;
+  U.n = rows == 8 ? in >> 3 : in / rows;
+  U.m = group * 8 + in - U.n * rows;
   U.first = U.split * G.per;
   U.last = min(U.first + G.per, G.blocks);
   return U;
@@ -452,42 +490,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------- around the products
-// The parts of a split sum in order, then the epilogue; four columns a thread.
-template <typename T, int ACT>
+// The parts of a split sum in order, then the epilogue; N columns a thread (of parts whose rows are whole
+// pieces of four).
+template <typename T, int ACT, int N>
 __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ Args G) {
-  const int64_t quads = G.part_ld / 4, n = G.rows * quads;
+  using TS = typename SlopeOf<T>::type;
+  const int64_t pieces = G.cols / N, n = G.rows * pieces;
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
-    const int64_t i = t / quads, j = (t - i * quads) * 4;
+    const int64_t i = t / pieces, j = (t - i * pieces) * N;
     const float* p = G.part + i * G.part_ld + j;
-    float h[4] = {0.f, 0.f, 0.f, 0.f};
+    float h[N] = {};
 #pragma unroll 4
-    for (int s = 0; s < G.splits; ++s) {
-      const float4 x = *reinterpret_cast<const float4*>(p + s * G.rows * G.part_ld);
-      h[0] += x.x;
-      h[1] += x.y;
-      h[2] += x.z;
-      h[3] += x.w;
-    }
-    using TS = typename SlopeOf<T>::type;
+    for (int s = 0; s < G.splits; ++s, p += G.rows * G.part_ld) {
+      if constexpr (N == 1) {
+        h[0] += *p;
+      } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (G.e.bias && j + e < G.cols) h[e] += to_f(static_cast<const T*>(G.e.bias)[j + e]);
+        for (int e = 0; e < N; e += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(p + e);
+          h[e] += x.x;
+          h[e + 1] += x.y;
+          h[e + 2] += x.z;
+          h[e + 3] += x.w;
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (G.e.bias) h[e] += to_f(static_cast<const T*>(G.e.bias)[j + e]);
     T* y = static_cast<T*>(G.e.y) + i * G.cols + j;
     TS* slope = G.e.slope ? static_cast<TS*>(G.e.slope) + i * G.cols + j : nullptr;
-    const T* residual = G.e.residual ? static_cast<const T*>(G.e.residual) + i * G.e.rs + j : nullptr;
-    if (G.vec) {
-      Pack<T, 4> res;
-      if (residual) res = *reinterpret_cast<const Pack<T, 4>*>(residual);
-      finish<T, ACT, 4>(h, residual ? &res : nullptr, y, slope);
+    Pack<T, N> res = {};
+    if (G.e.residual) {
+      res = *reinterpret_cast<const Pack<T, N>*>(static_cast<const T*>(G.e.residual) + i * G.e.rs + j);
+      if (ACT != FX_ACT_NONE && slope) finish<T, ACT, N, true, true>(h, res, y, slope);
+      else finish<T, ACT, N, true, false>(h, res, y, slope);
     } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (j + e >= G.cols) break;
-        Pack<T, 1> res;
-        if (residual) res.e[0] = residual[e];
-        const float one[1] = {h[e]};
-        finish<T, ACT, 1>(one, residual ? &res : nullptr, y + e, slope ? slope + e : nullptr);
-      }
+      if (ACT != FX_ACT_NONE && slope) finish<T, ACT, N, false, true>(h, res, y, slope);
+      else finish<T, ACT, N, false, false>(h, res, y, slope);
     }
   }
 }
