@@ -35,14 +35,16 @@ bool mappable(const void* p, int64_t stride, int64_t rows) {
          stride < (int64_t{1} << 38);
 }
 
-// How a product of rows x cols over `inner` is cut: tiles of a pair of SMs; where they do
-// not fill the device, k is cut into parts of four blocks at least.
+// How a product of rows x cols over `inner` is cut: tiles of a pair of SMs, as many whole rounds of them as there
+// are, and the rest split along k so that it fills the device once. A part has four blocks of k at least, and
+// after a whole round it has to save eight blocks' time (three in float32, whose blocks have six products),
+// about what the join costs.
 struct Cut {
   int64_t rows, cols;
-  int blocks, tm, tn, splits, per;
-  int64_t units() const { return (int64_t)tm * tn * splits; }
-  int64_t part_ld() const { return (cols + 3) / 4 * 4; }
-  size_t part_bytes() const { return splits > 1 ? align256((size_t)splits * rows * part_ld() * sizeof(float)) : 0; }
+  int blocks, tm, tn, whole, splits, per;
+  int64_t units() const { return whole + ((int64_t)tm * tn - whole) * splits; }
+  int64_t joined() const { return splits > 1 ? (int64_t)tm * tn - whole : 0; }
+  size_t part_bytes() const { return (size_t)joined() * splits * (lin::kTile * lin::kTile * sizeof(float)); }
 };
 
 Cut cut_of(int64_t rows, int64_t cols, int64_t inner, bool f32, int sms) {
@@ -50,13 +52,22 @@ Cut cut_of(int64_t rows, int64_t cols, int64_t inner, bool f32, int sms) {
   C.rows = rows;
   C.cols = cols;
   C.blocks = (int)ceil_div(inner, lin::kBlockK);
-  C.tm = (int)ceil_div(rows, lin::kRows);
-  C.tn = (int)ceil_div(cols, f32 ? lin::Shape<3>::kCols : lin::Shape<1>::kCols);
-  const int64_t tiles = (int64_t)C.tm * C.tn, fill = (sms / 2) / tiles, most = C.blocks / 4;
-  int64_t splits = fill < most ? fill : most;
-  if (splits < 1) splits = 1;
-  C.per = (int)ceil_div(C.blocks, splits);
-  C.splits = (int)ceil_div(C.blocks, C.per);
+  C.tm = (int)ceil_div(rows, lin::kTile);
+  C.tn = (int)ceil_div(cols, lin::kTile);
+  const int64_t tiles = (int64_t)C.tm * C.tn, pairs = sms / 2, rest = tiles % pairs;
+  C.whole = (int)tiles;
+  C.splits = 1;
+  C.per = C.blocks;
+  int64_t splits = rest ? pairs / rest : 1;
+  if (splits > C.blocks / 4) splits = C.blocks / 4;
+  if (splits > 1) {
+    const int64_t per = ceil_div(C.blocks, splits);
+    if (tiles < pairs || C.blocks - per >= (f32 ? 3 : 8)) {
+      C.whole = (int)(tiles - rest);
+      C.per = (int)per;
+      C.splits = (int)ceil_div(C.blocks, per);
+    }
+  }
   return C;
 }
 
@@ -128,14 +139,14 @@ LinPlan plan_bwd(const fx_linear_args* a, int sms) {
   return P;
 }
 
-// The map of a matrix: boxes of 64 entries by `rows` (K-major) or 64 rows (MN-major).
-int make_map(CUtensorMap* m, const Operand& o, int planes, bool mn, int rows) {
+// The map of a matrix: boxes of 64 entries by 128 rows (K-major), 64 by 64 (MN-major).
+int make_map(CUtensorMap* m, const Operand& o, int planes, bool mn) {
   const EncodeTiled encode = encode_tiled();
   if (!encode) return FX_ERR_CUDA;
   const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)planes};
   const int64_t ld = o.rows > 1 ? o.ld : ld_of(o.cols);
   const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, planes > 1 ? (cuuint64_t)(o.rows * ld * 2) : (cuuint64_t)ld * 2};
-  const cuuint32_t box[3] = {64, mn ? 64u : (cuuint32_t)rows, 1}, ones[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, mn ? 64u : 128u, 1}, ones[3] = {1, 1, 1};
   return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.p), dims, strides, box, ones,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
@@ -143,30 +154,24 @@ int make_map(CUtensorMap* m, const Operand& o, int planes, bool mn, int rows) {
              : FX_ERR_CUDA;
 }
 
-// Whether y, slope and the residual are rows of whole 16-byte pieces.
+// Whether y, slope, the residual and the bias are rows of whole 16-byte pieces.
 bool pieces(const Epilogue& e, int64_t rows, int64_t cols, int size) {
   const uintptr_t m = reinterpret_cast<uintptr_t>(e.y) | reinterpret_cast<uintptr_t>(e.slope) |
-                      reinterpret_cast<uintptr_t>(e.residual) | (uintptr_t)(e.residual && rows > 1 ? e.rs * size : 0) |
-                      (uintptr_t)(cols * size);
+                      reinterpret_cast<uintptr_t>(e.residual) | reinterpret_cast<uintptr_t>(e.bias) |
+                      (uintptr_t)(e.residual && rows > 1 ? e.rs * size : 0) | (uintptr_t)(cols * size);
   return m % 16 == 0;
 }
 
 template <typename T, int NP, int ACT>
-int launch(cudaStream_t s, const lin::Args& G, const lin::Maps& M, int64_t pairs, int sms) {
+int launch(cudaStream_t s, const lin::Args& G, const lin::Maps& M, int64_t pairs, int64_t joined) {
   constexpr size_t smem = lin::Shape<NP>::kSmem;
-  if (G.splits > 1) {
-    auto kern = lin::linear_tc_kernel<T, NP, lin::kPart>;
-    if (raise_smem(kern, smem, smem)) return FX_ERR_CUDA;
-    kern<<<(unsigned)(2 * pairs), lin::kThreads, smem, s>>>(G, M);
+  auto kern = lin::linear_tc_kernel<T, NP, ACT>;
+  if (raise_smem(kern, smem, smem)) return FX_ERR_CUDA;
+  kern<<<(unsigned)(2 * pairs), lin::kThreads, smem, s>>>(G, M);
+  if (joined) {  // 74 tiles at most, 256 blocks each
     constexpr int N = 16 / sizeof(T);
-    const int64_t blocks = ceil_div(G.rows * G.cols / (G.vec ? N : 1), 256), most = (int64_t)sms * 8;
-    const unsigned grid = (unsigned)(blocks < most ? blocks : most);
-    if (G.vec) lin::linear_join_kernel<T, ACT, N><<<grid, 256, 0, s>>>(G);
-    else lin::linear_join_kernel<T, ACT, 1><<<grid, 256, 0, s>>>(G);
-  } else {
-    auto kern = lin::linear_tc_kernel<T, NP, ACT>;
-    if (raise_smem(kern, smem, smem)) return FX_ERR_CUDA;
-    kern<<<(unsigned)(2 * pairs), lin::kThreads, smem, s>>>(G, M);
+    if (G.vec) lin::linear_join_kernel<T, ACT, N><<<(unsigned)(joined * (256 / N)), 256, 0, s>>>(G);
+    else lin::linear_join_kernel<T, ACT, 1><<<(unsigned)(joined * 256), 256, 0, s>>>(G);
   }
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
@@ -175,33 +180,33 @@ template <typename T, int NP>
 int product(cudaStream_t s, const Cut& C, const Operand& a, bool a_mn, const Operand& b, bool b_mn, const Epilogue& e,
             float* part, int sms) {
   lin::Maps M;
-  int st = make_map(&M.a, a, NP, a_mn, lin::kHalf);
-  if (!st) st = make_map(&M.b, b, NP, b_mn, lin::Shape<NP>::kCols / 2);
+  int st = make_map(&M.a, a, NP, a_mn);
+  if (!st) st = make_map(&M.b, b, NP, b_mn);
   if (st) return st;
-  if (C.units() > INT32_MAX) return FX_ERR_SHAPE;
+  if ((int64_t)C.tm * C.tn > INT32_MAX / 2) return FX_ERR_SHAPE;
   lin::Args G{};
   G.rows = C.rows;
   G.cols = C.cols;
   G.blocks = C.blocks;
   G.tm = C.tm;
   G.tn = C.tn;
+  G.whole = C.whole;
   G.splits = C.splits;
   G.per = C.per;
   G.a_mn = a_mn;
   G.b_mn = b_mn;
   G.vec = pieces(e, C.rows, C.cols, sizeof(T));
   G.polls = wait_polls();
-  G.part = C.splits > 1 ? part : nullptr;
-  G.part_ld = C.part_ld();
+  G.part = part;
   G.e = e;
   const int64_t pairs = C.units() < sms / 2 ? C.units() : sms / 2;
   switch (e.act) {
-    case FX_ACT_RELU: return launch<T, NP, FX_ACT_RELU>(s, G, M, pairs, sms);
-    case FX_ACT_SILU: return launch<T, NP, FX_ACT_SILU>(s, G, M, pairs, sms);
-    case FX_ACT_GELU: return launch<T, NP, FX_ACT_GELU>(s, G, M, pairs, sms);
-    case FX_ACT_GELU_TANH: return launch<T, NP, FX_ACT_GELU_TANH>(s, G, M, pairs, sms);
-    case FX_ACT_TANH: return launch<T, NP, FX_ACT_TANH>(s, G, M, pairs, sms);
-    default: return launch<T, NP, FX_ACT_NONE>(s, G, M, pairs, sms);
+    case FX_ACT_RELU: return launch<T, NP, FX_ACT_RELU>(s, G, M, pairs, C.joined());
+    case FX_ACT_SILU: return launch<T, NP, FX_ACT_SILU>(s, G, M, pairs, C.joined());
+    case FX_ACT_GELU: return launch<T, NP, FX_ACT_GELU>(s, G, M, pairs, C.joined());
+    case FX_ACT_GELU_TANH: return launch<T, NP, FX_ACT_GELU_TANH>(s, G, M, pairs, C.joined());
+    case FX_ACT_TANH: return launch<T, NP, FX_ACT_TANH>(s, G, M, pairs, C.joined());
+    default: return launch<T, NP, FX_ACT_NONE>(s, G, M, pairs, C.joined());
   }
 }
 

@@ -2,9 +2,9 @@
 // forward (x, W), dx (g, W) and dW (g, x) alike. Each operand is read as it is stored, along k
 // (K-major) or across it (MN-major).
 //
-// A pair of SMs holds a tile of 256 x 256 (256 x 128 in float32): each brings 128 rows of A and half
-// of the columns of B by tensor maps (64 entries of k a stage) and keeps 128 rows of the sum in its TMEM,
-// twice or more, so that one tile's epilogue runs under the next tile's products. The grid is persistent.
+// A pair of SMs holds a tile of 256 x 256: each brings 128 rows of A and 128 of B by tensor maps (64
+// entries of k a stage) and keeps 128 rows of the sum in its TMEM, twice, so that one tile's epilogue
+// runs under the next tile's products. The grid is persistent.
 //
 // float32 runs on the same bfloat16 instructions: x = x1 + x2 + x3, each part the rest rounded to
 // bfloat16, holds 24 bits, and the six products with index sum <= 4 leave out terms of 2^-24. The
@@ -13,8 +13,8 @@
 // whole sum stays in the accumulator: 1.6e-8 of it is lost for every 16 entries of k, which reaches
 // half of the output's rounding (2e-3) after a million.
 //
-// Few tiles split k over pairs of SMs; the parts are float32 sums in the workspace, added in
-// order by linear_join_kernel, which then does the epilogue.
+// Tiles that do not fill the device, or the last round of many, split k over pairs of SMs; the parts are
+// float32 sums in the workspace, added in order by linear_join_kernel, which then does the epilogue.
 #pragma once
 #include <cuda.h>
 
@@ -26,21 +26,17 @@ namespace lin {
 
 using namespace umma;
 
-constexpr int kRows = 256, kHalf = 128, kBlockK = 64;  // rows of a pair and of an SM, entries of k of a stage
-constexpr int kWarps = 16;                             // of the epilogue
+constexpr int kTile = 256, kHalf = 128, kBlockK = 64;  // of a pair, of an SM, of a stage
+constexpr int kWarps = 16;                             // of the epilogue: 32 rows, 64 columns each
 constexpr int kThreads = 64 + 32 * kWarps;             // and one warp for the copies, one for the products
+constexpr uint32_t kOperand = kHalf * kBlockK * 2;     // bytes of an SM's rows of an operand
 
-// A stage is one part of 64 entries of k: 128 rows of A and half of the tile's columns of B an SM. bfloat16
-// tiles have 256 columns. The three parts' have 128, which leaves the registers for their sums and is
-// enough to keep the loads below the products.
 template <int NP>
 struct Shape {
-  static constexpr int kCols = NP == 1 ? 256 : 128, kBuffers = 512 / kCols;
-  static constexpr int kStages = NP == 1 ? 5 : 8;
-  static constexpr uint32_t kA = kHalf * kBlockK * 2, kB = kCols / 2 * kBlockK * 2, kStage = kA + kB;
-  static constexpr int kStrip = kCols / 4;         // columns of a warp
-  static constexpr int kStore = NP == 1 ? 32 : 16;  // of them stored at a time
+  static constexpr int kStages = NP == 1 ? 5 : 2;
+  static constexpr int kStore = NP == 1 ? 32 : 16;  // columns that a warp stores at a time
   static constexpr uint32_t kBlock = 32 * kStore * 4;
+  static constexpr uint32_t kStage = 2 * NP * kOperand;  // the parts of A, the parts of B
   static constexpr uint32_t kSmem = kStages * kStage + kWarps * kBlock + 1024;
   static constexpr int kChunk = 2;  // blocks of k in an accumulator (three parts)
 };
@@ -50,13 +46,15 @@ struct alignas(64) Maps {
 };
 
 struct Args {
-  int64_t rows, cols;            // of the result
-  int blocks, tm, tn, splits, per;  // blocks of k, tiles, parts of k, blocks of a part
-  int a_mn, b_mn, vec;
+  int64_t rows, cols;  // of the result
+  int blocks, tm, tn;  // blocks of k, tiles
+  int whole, splits, per;  // tiles that a pair does alone; parts of the others, blocks of a part
+  int a_mn, b_mn, vec;  // vec: rows of y, slope, residual and bias are whole pieces of 16 bytes
   uint32_t polls;
-  float* part;  // (splits, rows, part_ld)
-  int64_t part_ld;
+  float* part;  // of the tiles from `whole` on: (tile, part, 256, 256)
   Epilogue e;
+
+  __host__ __device__ int units() const { return whole + (tm * tn - whole) * splits; }
 };
 
 // ---------------------------------------------------------------- instructions of a pair
@@ -128,6 +126,13 @@ __device__ __forceinline__ void ld16(uint32_t a, uint32_t (&v)[16]) {
       : FX_R8(v, 0), FX_R8(v, 8)
       : "r"(a));
 }
+#define FX_I8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
+__device__ __forceinline__ void st16(uint32_t a, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(a),
+      FX_I8(v, 0), FX_I8(v, 8));
+}
+#undef FX_I8
 #undef FX_R8
 
 // 128-byte swizzled operand: rows of 64 entries of k, or, MN-major, rows of 64 entries across k, 64 of
@@ -164,8 +169,6 @@ __device__ __forceinline__ void spoil(int state, uint32_t (&v)[C]) {
   }
 }
 
-constexpr int kPart = -1;  // in the place of an activation: the sums themselves, of a part of k
-
 // N entries of a row: activation, residual, stores.
 template <typename T, int ACT, int N, bool RES, bool SLOPE>
 __device__ __forceinline__ void finish(const float (&h)[N], const Pack<T, N>& residual, T* y, typename SlopeOf<T>::type* slope) {
@@ -186,33 +189,25 @@ __device__ __forceinline__ void finish(const float (&h)[N], const Pack<T, N>& re
   }
 }
 
-// Where a staged entry is: rows of C, 16-byte pieces swizzled.
+// A warp's staging block holds 32 rows of C entries; the 16-byte piece p of row r is at piece
+// p ^ (r & 7) of its row (C = 32) or p ^ (r >> 1 & 3) (C = 16).
 template <int C>
-__device__ __forceinline__ uint32_t staged(int r, int piece) {
-  return r * (C * 4) + ((C == 32 ? piece ^ (r & 7) : piece ^ (r >> 1 & 3)) << 4);
+__device__ __forceinline__ uint32_t staged(int r, int p) {
+  return r * (C * 4) + ((C == 32 ? p ^ (r & 7) : p ^ (r >> 1 & 3)) << 4);
 }
 
 // Of 32 x C staged entries of the sum, N entries of a row a lane (16 bytes of the result, or, where rows are
-// not whole pieces, one), so that stores cover whole sectors. G.rows and G.cols end the result.
+// not whole pieces, one), so that stores cover whole sectors; R rows at a time. y, slope and residual are this
+// lane's, `last` is the number of rows from its first on.
 template <typename T, int ACT, int C, int N, bool RES, bool SLOPE>
-__device__ __forceinline__ void store_rows(const Args& G, const unsigned char* stage, int64_t i0, int64_t j0) {
-  using TS = typename SlopeOf<T>::type;
-  constexpr int L = C / N, R = 32 / L;       // lanes of a row, rows at a time
-  constexpr int U = N == 1 ? 8 : 2;          // and as many times before the next residuals are read
+__device__ __forceinline__ void store_rows(const Args& G, const unsigned char* stage, T* y, typename SlopeOf<T>::type* slope,
+                                           const T* residual, const Pack<T, N>& bias, int last) {
+  constexpr int L = C / N, R = 32 / L, U = N == 1 ? 8 : 2;  // U: residuals read ahead
   const int lane = threadIdx.x & 31, c = lane % L * N, r0 = lane / L;
-  const int64_t j = j0 + c, i = i0 + r0;
-  const int last = (int)(G.rows - i < 32 ? G.rows - i : 32);  // of the rows from r0 on
-  if (j >= G.cols) return;
-  float bias[N];
-#pragma unroll
-  for (int e = 0; e < N; ++e) bias[e] = G.e.bias ? to_f(static_cast<const T*>(G.e.bias)[j + e]) : 0.f;
-  T* y = static_cast<T*>(G.e.y) + i * G.cols + j;
-  TS* slope = SLOPE ? static_cast<TS*>(G.e.slope) + i * G.cols + j : nullptr;
-  const T* residual = RES ? static_cast<const T*>(G.e.residual) + i * G.e.rs + j : nullptr;
   const int64_t step = R * G.cols, rstep = R * G.e.rs;
-#pragma unroll 1
+#pragma unroll (N == 1 ? 1 : 32)
   for (int k0 = 0; k0 < 32; k0 += U * R) {
-    Pack<T, N> res[U];
+    Pack<T, N> res[U] = {};
     if constexpr (RES) {
 #pragma unroll
       for (int u = 0; u < U; ++u, residual += rstep)
@@ -224,9 +219,10 @@ __device__ __forceinline__ void store_rows(const Args& G, const unsigned char* s
       if constexpr (N == 1) {
         h[0] = *reinterpret_cast<const float*>(stage + staged<C>(k0 + u * R + r0, c / 4) + (c & 3) * 4);
       } else {
+        static_assert(R % 8 == 0);  // the swizzle is the same every time
 #pragma unroll
         for (int e = 0; e < N; e += 4) {
-          const float4 x = *reinterpret_cast<const float4*>(stage + staged<C>(k0 + u * R + r0, (c + e) / 4));
+          const float4 x = *reinterpret_cast<const float4*>(stage + (k0 + u * R) * (C * 4) + staged<C>(r0, (c + e) / 4));
           h[e] = x.x;
           h[e + 1] = x.y;
           h[e + 2] = x.z;
@@ -234,7 +230,7 @@ __device__ __forceinline__ void store_rows(const Args& G, const unsigned char* s
         }
       }
 #pragma unroll
-      for (int e = 0; e < N; ++e) h[e] += bias[e];
+      for (int e = 0; e < N; ++e) h[e] += to_f(bias.e[e]);
       if (k0 + u * R < last) finish<T, ACT, N, RES, SLOPE>(h, res[u], y, slope);
       y += step;
       if constexpr (SLOPE) slope += step;
@@ -242,63 +238,128 @@ __device__ __forceinline__ void store_rows(const Args& G, const unsigned char* s
   }
 }
 
-template <typename T, int ACT, int C, int N>
-__device__ __forceinline__ void store_rows(const Args& G, const unsigned char* stage, int64_t i0, int64_t j0) {
-  if (ACT != FX_ACT_NONE && G.e.slope) {
-    if (G.e.residual) store_rows<T, ACT, C, N, true, true>(G, stage, i0, j0);
-    else store_rows<T, ACT, C, N, false, true>(G, stage, i0, j0);
-  } else {
-    if (G.e.residual) store_rows<T, ACT, C, N, true, false>(G, stage, i0, j0);
-    else store_rows<T, ACT, C, N, false, false>(G, stage, i0, j0);
-  }
-}
+// A warp's 32 rows and 64 columns of a tile: where its lanes' entries go.
+template <typename T, int C, int N>
+struct Lines {
+  using TS = typename SlopeOf<T>::type;
+  T* y;
+  TS* slope;
+  const T *residual, *bias;
+  int last;      // rows
+  int64_t left;  // columns from this lane's first on
 
-// The sums themselves, four a lane; the parts' rows are whole pieces.
+  __device__ __forceinline__ Lines(const Args& G, int64_t i0, int64_t j0) {
+    constexpr int L = C / N;
+    const int lane = threadIdx.x & 31;
+    const int64_t i = i0 + lane / L, j = j0 + lane % L * N;
+    last = (int)(G.rows - i < 32 ? G.rows - i : 32);
+    left = G.cols - j;
+    y = static_cast<T*>(G.e.y) + i * G.cols + j;
+    slope = G.e.slope ? static_cast<TS*>(G.e.slope) + i * G.cols + j : nullptr;
+    residual = G.e.residual ? static_cast<const T*>(G.e.residual) + i * G.e.rs + j : nullptr;
+    bias = G.e.bias ? static_cast<const T*>(G.e.bias) + j : nullptr;
+  }
+  template <int ACT>
+  __device__ __forceinline__ void store(const Args& G, const unsigned char* stage) {  // and on to the next C columns
+    if (left > 0) {
+      Pack<T, N> b = {};
+      if (bias) b = *reinterpret_cast<const Pack<T, N>*>(bias);
+      if (ACT != FX_ACT_NONE && slope) {
+        if (residual) store_rows<T, ACT, C, N, true, true>(G, stage, y, slope, residual, b, last);
+        else store_rows<T, ACT, C, N, false, true>(G, stage, y, slope, residual, b, last);
+      } else {
+        if (residual) store_rows<T, ACT, C, N, true, false>(G, stage, y, slope, residual, b, last);
+        else store_rows<T, ACT, C, N, false, false>(G, stage, y, slope, residual, b, last);
+      }
+    }
+    y += C;
+    if (slope) slope += C;
+    if (residual) residual += C;
+    if (bias) bias += C;
+    left -= C;
+  }
+};
+
+// The sums themselves, to a row-major tile of 256 columns.
 template <int C>
-__device__ __forceinline__ void store_part(const Args& G, const unsigned char* stage, int64_t i0, int64_t j0, int split) {
+__device__ __forceinline__ void store_part(float* out, const unsigned char* stage) {
   constexpr int L = C / 4, R = 32 / L;
   const int lane = threadIdx.x & 31, r0 = lane / L;
-  const int64_t j = j0 + lane % L * 4, i = i0 + r0;
-  if (j >= G.cols) return;
-  float* out = G.part + (split * G.rows + i) * G.part_ld + j;
+  out += r0 * kTile + lane % L * 4;
 #pragma unroll
-  for (int k = 0; k < 32; k += R, out += R * G.part_ld)
-    if (i + k < G.rows) *reinterpret_cast<float4*>(out) = *reinterpret_cast<const float4*>(stage + staged<C>(k + r0, lane % L));
-}
-
-// 32 x C entries of the sum, a row a lane, through shared memory to memory.
-template <typename T, int ACT, int C>
-__device__ __forceinline__ void store_block(const Args& G, unsigned char* stage, int64_t i0, int64_t j0, int split,
-                                            const uint32_t (&v)[C]) {
-  const int lane = threadIdx.x & 31;
-  __syncwarp();
-#pragma unroll
-  for (int p = 0; p < C / 4; ++p)
-    *reinterpret_cast<uint4*>(stage + staged<C>(lane, p)) = make_uint4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
-  __syncwarp();
-  if constexpr (ACT == kPart) {
-    store_part<C>(G, stage, i0, j0, split);
-  } else {
-    if (G.vec) store_rows<T, ACT, C, 16 / sizeof(T)>(G, stage, i0, j0);
-    else store_rows<T, ACT, C, 1>(G, stage, i0, j0);
-  }
+  for (int k = 0; k < 32; k += R)
+    *reinterpret_cast<float4*>(out + k * kTile) = *reinterpret_cast<const float4*>(stage + staged<C>(k + r0, lane % L));
 }
 
 struct Unit {
-  int m, n, split, first, last;  // tile, part of k, blocks of k
+  int m, n, part, first, last;  // tile, place among the parts (-1: whole), blocks of k
 };
 // Tiles in groups of 8 rows of tiles, down the columns of a group, so that what runs at a time shares
 // rows and columns; the parts of a tile next to each other.
 __device__ __forceinline__ Unit unit_of(const Args& G, int u) {
   Unit U;
-  const int t = G.splits == 1 ? u : u / G.splits, group = t / (8 * G.tn), in = t - group * 8 * G.tn;
+  int t = u;
+  U.part = -1;
+  U.first = 0;
+  U.last = G.blocks;
+  if (u >= G.whole) {
+    U.part = u - G.whole;
+    const int q = U.part / G.splits;
+    t = G.whole + q;
+    U.first = (U.part - q * G.splits) * G.per;
+    U.last = min(U.first + G.per, G.blocks);
+  }
+  const int group = t / (8 * G.tn), in = t - group * 8 * G.tn;
   const int rows = min(8, G.tm - group * 8);
-  U.split = u - t * G.splits;
   U.n = rows == 8 ? in >> 3 : in / rows;
   U.m = group * 8 + in - U.n * rows;
-  U.first = U.split * G.per;
-  U.last = min(U.first + G.per, G.blocks);
   return U;
+}
+
+// The epilogue of a warp's 32 rows and 64 columns of a tile, in TMEM from `from` on, C columns at a time through the
+// warp's staging block.
+template <typename T, int ACT, int C>
+__device__ __forceinline__ void epilogue(const Args& G, const Unit& U, unsigned char* stage, int row, int col, uint32_t from,
+                                         volatile int* state) {
+  constexpr int B = 64 / C, UNROLL = C == 32 ? B : 1;  // float32 needs the registers
+  const int lane = threadIdx.x & 31;
+  const int64_t i0 = (int64_t)U.m * kTile + row, j0 = (int64_t)U.n * kTile + col;
+  const auto bring = [&](int c) {
+    uint32_t v[C];
+    if constexpr (C == 32) ld32(from + c * C, v);
+    else ld16(from + c * C, v);
+    tmem_wait_ld();
+    spoil(*state, v);
+    __syncwarp();
+#pragma unroll
+    for (int p = 0; p < C / 4; ++p)
+      *reinterpret_cast<uint4*>(stage + staged<C>(lane, p)) = make_uint4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
+    __syncwarp();
+  };
+  if (U.part >= 0) {
+    float* out = G.part + ((int64_t)U.part * kTile + row) * kTile + col;
+#pragma unroll UNROLL
+    for (int c = 0; c < B; ++c, out += C) {
+      bring(c);
+      store_part<C>(out, stage);
+    }
+  } else if (G.vec) {
+    Lines<T, C, 16 / sizeof(T)> lines(G, i0, j0);
+#pragma unroll UNROLL
+    for (int c = 0; c < B; ++c) {
+      if (j0 + c * C >= G.cols) break;
+      bring(c);
+      lines.template store<ACT>(G, stage);
+    }
+  } else {
+    Lines<T, C, 1> lines(G, i0, j0);
+#pragma unroll 1
+    for (int c = 0; c < B; ++c) {
+      if (j0 + c * C >= G.cols) break;
+      bring(c);
+      lines.template store<ACT>(G, stage);
+    }
+  }
 }
 
 template <typename T, int NP, int ACT>
@@ -308,7 +369,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   constexpr int ST = S::kStages;
   extern __shared__ unsigned char raw[];
   unsigned char* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
-  __shared__ uint64_t full[ST], empty[ST], sum_full[S::kBuffers], sum_empty[S::kBuffers];
+  __shared__ uint64_t full[ST], empty[ST], sum_full[2], sum_empty[2];
   __shared__ uint32_t slot;
   __shared__ volatile int state;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -319,7 +380,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < S::kBuffers; ++i) {
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&sum_full[i], 1);
       mbar_init(&sum_empty[i], 2 * kWarps);  // the epilogue's warps of both blocks
     }
@@ -331,7 +392,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_sync();
   fence_after_sync();
   const uint32_t tmem = slot;
-  const int units = G.tm * G.tn * G.splits, pairs = gridDim.x >> 1;
+  const int units = G.units(), pairs = gridDim.x >> 1;
   const int chunk = NP == 1 ? G.blocks : S::kChunk;
 
   if (warp == 0) {
@@ -340,14 +401,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int it = 0;
       for (int u = blockIdx.x >> 1; u < units && state != DEAD; u += pairs) {
         const Unit U = unit_of(G, u);
-        const int i0 = U.m * kRows + rank * kHalf, j0 = U.n * S::kCols + rank * (S::kCols / 2);
-        for (int kb = U.first; kb < U.last; ++kb) {
-#pragma unroll 1
-          for (int p = 0; p < NP; ++p, ++it) {
-            const int st = it % ST;
-            if (!wait(&empty[st], (it / ST & 1) ^ 1, &state, G.polls)) break;
-            const uint32_t bar = first_block(&full[st]), a = smem_u32(sm) + st * S::kStage, b = a + S::kA;
-            if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * S::kStage);
+        const int i0 = U.m * kTile + rank * kHalf, j0 = U.n * kTile + rank * kHalf;
+        for (int kb = U.first; kb < U.last; ++kb, ++it) {
+          const int st = it % ST;
+          if (!wait(&empty[st], (it / ST & 1) ^ 1, &state, G.polls)) break;
+          const uint32_t bar = first_block(&full[st]), at = smem_u32(sm) + st * S::kStage;
+          if (rank == 0) mbar_arrive_expect_tx(&full[st], 2 * S::kStage);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+            const uint32_t a = at + p * kOperand, b = at + (NP + p) * kOperand;
             if (G.a_mn) {
               tma_box(a, &M.a, i0, kb * kBlockK, p, bar);
               tma_box(a + 8192, &M.a, i0 + 64, kb * kBlockK, p, bar);
@@ -356,7 +418,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
             if (G.b_mn) {
               tma_box(b, &M.b, j0, kb * kBlockK, p, bar);
-              if (S::kB > 8192) tma_box(b + 8192, &M.b, j0 + 64, kb * kBlockK, p, bar);
+              tma_box(b + 8192, &M.b, j0 + 64, kb * kBlockK, p, bar);
             } else {
               tma_box(b, &M.b, kb * kBlockK, j0, p, bar);
             }
@@ -372,113 +434,90 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // The whole warp runs the loops, so that descriptors stay in uniform registers, and one lane issues.
     if (rank == 0) {
       const uint32_t idesc = 1u << 4 | 1u << 7 | 1u << 10 | (G.a_mn ? 1u << 15 : 0u) | (G.b_mn ? 1u << 16 : 0u) |
-                             (uint32_t)(S::kCols >> 3) << 17 | (uint32_t)(kRows >> 4) << 24;
+                             (uint32_t)(kTile >> 3) << 17 | (uint32_t)(kTile >> 4) << 24;
       const uint32_t sa = G.a_mn ? 128 : 2, sb = G.b_mn ? 128 : 2;  // 16 entries of k further, in 16 bytes
-      const uint64_t a0 = desc(smem_u32(sm), G.a_mn), b0 = desc(smem_u32(sm) + S::kA, G.b_mn);
+      const uint64_t a0 = desc(smem_u32(sm), G.a_mn), b0 = desc(smem_u32(sm) + NP * kOperand, G.b_mn);
       int st = 0, ch = 0;
       uint32_t phase = 0;
       for (int u = blockIdx.x >> 1; u < units && state != DEAD; u += pairs) {
         const Unit U = unit_of(G, u);
         for (int k0 = U.first; k0 < U.last; k0 += chunk, ++ch) {
-          const int buf = ch % S::kBuffers;
-          if (!wait(&sum_empty[buf], (ch / S::kBuffers & 1) ^ 1, &state, G.polls)) break;
+          const int buf = ch % 2;
+          if (!wait(&sum_empty[buf], (ch / 2 & 1) ^ 1, &state, G.polls)) break;
           fence_after_sync();
-          const uint32_t d = tmem + buf * S::kCols;
+          const uint32_t d = tmem + buf * kTile;
           const int k1 = min(k0 + chunk, U.last);
           for (int kb = k0; kb < k1; ++kb) {
-            int at[NP];  // the stages of the parts
+            if (!wait(&full[st], phase, &state, G.polls)) break;
+            fence_after_sync();
+            if (elected()) {
+              const uint64_t a1 = a0 + (uint32_t)(st * (S::kStage >> 4)), b1 = b0 + (uint32_t)(st * (S::kStage >> 4));
 #pragma unroll
-            for (int p = 0; p < NP; ++p) {
-              at[p] = st;
-              if (!wait(&full[st], phase, &state, G.polls)) break;
-              fence_after_sync();
-              if (elected()) {
-                // the products of this part with those before it, and what is left out of none: index sum <= 4
+              for (int sum = NP - 1; sum >= 0; --sum) {  // the smaller products first
 #pragma unroll
-                for (int q = 0; q <= p; ++q) {
+                for (int i = 0; i <= sum; ++i) {
 #pragma unroll
-                  for (int t = 0; t < (p == q ? 1 : 2); ++t) {
-                    const int i = t ? q : p, j = t ? p : q;
-                    if (i + j >= NP) continue;
-                    const uint64_t a1 = a0 + (uint32_t)(at[i] * (S::kStage >> 4)), b1 = b0 + (uint32_t)(at[j] * (S::kStage >> 4));
-#pragma unroll
-                    for (int k = 0; k < kBlockK / 16; ++k)
-                      mma_pair(d, a1 + k * sa, b1 + k * sb, idesc, kb > k0 || i > 0 || j > 0 || k > 0);
-                  }
-                }
-                if (p == NP - 1) {
-#pragma unroll
-                  for (int q = 0; q < NP; ++q) commit_pair(&empty[at[q]]);
-                  if (kb == k1 - 1) commit_pair(&sum_full[buf]);
+                  for (int k = 0; k < kBlockK / 16; ++k)
+                    mma_pair(d, a1 + i * (kOperand >> 4) + k * sa, b1 + (sum - i) * (kOperand >> 4) + k * sb, idesc,
+                             kb > k0 || sum < NP - 1 || i > 0 || k > 0);
                 }
               }
-              __syncwarp();
-              if (++st == ST) {
-                st = 0;
-                phase ^= 1;
-              }
+              commit_pair(&empty[st]);
+              if (kb == k1 - 1) commit_pair(&sum_full[buf]);
+            }
+            __syncwarp();
+            if (++st == ST) {
+              st = 0;
+              phase ^= 1;
             }
           }
         }
       }
-      if (state == DEAD && ch > 0) mbar_wait(&sum_full[(ch - 1) % S::kBuffers], (ch - 1) / S::kBuffers & 1, 1u << 20);
+      if (state == DEAD && ch > 0) mbar_wait(&sum_full[(ch - 1) % 2], (ch - 1) / 2 & 1, 1u << 20);
     }
   } else {
     // -------------------------------------------------------- epilogue
-    constexpr int C = S::kStore, B = S::kStrip / C;
-    const int quarter = warp & 3, strip = (warp - 2) >> 2;
+    constexpr int C = 16, B = 64 / C;
+    const int quarter = warp & 3, strip = (warp - 2) >> 2, row = rank * kHalf + quarter * 32, col = strip * 64;
     unsigned char* stage = sm + ST * S::kStage + (warp - 2) * S::kBlock;
-    const uint32_t lanes = tmem + ((uint32_t)quarter << 21) + strip * S::kStrip;
+    const uint32_t lanes = tmem + ((uint32_t)quarter << 21) + col;
     int ch = 0;
     for (int u = blockIdx.x >> 1; u < units && state != DEAD; u += pairs) {
       const Unit U = unit_of(G, u);
-      const int64_t i0 = (int64_t)U.m * kRows + rank * kHalf + quarter * 32, j0 = (int64_t)U.n * S::kCols + strip * S::kStrip;
       float acc[NP == 1 ? 1 : B][C];
       for (int k0 = U.first; k0 < U.last; k0 += chunk, ++ch) {
-        const int buf = ch % S::kBuffers;
-        if (!wait(&sum_full[buf], ch / S::kBuffers & 1, &state, G.polls)) break;
+        const int buf = ch % 2;
+        if (!wait(&sum_full[buf], ch / 2 & 1, &state, G.polls)) break;
         fence_after_sync();
-        const uint32_t from = lanes + buf * S::kCols;
-        if constexpr (NP == 1) {
-#pragma unroll 1
-          for (int c = 0; c < B; ++c) {
-            if (j0 + c * C >= G.cols) break;
-            uint32_t v[C];
-            ld32(from + c * C, v);
-            tmem_wait_ld();
-            spoil(state, v);
-            store_block<T, ACT, C>(G, stage, i0, j0 + c * C, U.split, v);
-          }
-        } else {
+        const uint32_t from = lanes + buf * kTile;
+        const bool last = k0 + chunk >= U.last;
+        if constexpr (NP > 1) {
+          // The sums so far are in registers; with the last of them they go back to TMEM, from where they are stored.
           const bool more = k0 > U.first;
+          if (more || !last) {
 #pragma unroll
-          for (int c = 0; c < B; ++c) {
-            uint32_t v[C];
-            ld16(from + c * C, v);
-            tmem_wait_ld();
-            if (more) {
+            for (int c = 0; c < B; ++c) {
+              uint32_t v[C];
+              ld16(from + c * C, v);
+              tmem_wait_ld();
+              if (more) {
 #pragma unroll
-              for (int e = 0; e < C; ++e) acc[c][e] += __uint_as_float(v[e]);
-            } else {
+                for (int e = 0; e < C; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) + acc[c][e]);
+              }
+              if (last) {
+                st16(from + c * C, v);
+              } else {
 #pragma unroll
-              for (int e = 0; e < C; ++e) acc[c][e] = __uint_as_float(v[e]);
+                for (int e = 0; e < C; ++e) acc[c][e] = __uint_as_float(v[e]);
+              }
             }
+            if (last) tmem_wait_st();
           }
         }
+        if (last) epilogue<T, ACT, S::kStore>(G, U, stage, row, col, from, &state);
         fence_before_sync();
         __syncwarp();
         if (lane == 0) arrive_at(first_block(&sum_empty[buf]));
-      }
-      if constexpr (NP > 1) {
-#pragma unroll
-        for (int c = 0; c < B; ++c) {
-          if (j0 + c * C >= G.cols) break;
-          uint32_t v[C];
-#pragma unroll
-          for (int e = 0; e < C; ++e) v[e] = __float_as_uint(acc[c][e]);
-          spoil(state, v);
-          store_block<T, ACT, C>(G, stage, i0, j0 + c * C, U.split, v);
-        }
       }
     }
   }
@@ -490,45 +529,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------- around the products
-// The parts of a split sum in order, then the epilogue; N columns a thread (of parts whose rows are whole
-// pieces of four).
+// The parts of the split tiles in order, then the epilogue; N columns a thread.
 template <typename T, int ACT, int N>
 __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ Args G) {
-  using TS = typename SlopeOf<T>::type;
-  const int64_t pieces = G.cols / N, n = G.rows * pieces;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
-    const int64_t i = t / pieces, j = (t - i * pieces) * N;
-    const float* p = G.part + i * G.part_ld + j;
-    float h[N] = {};
+  constexpr int P = kTile / N;  // pieces of a row
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int q = (int)(t / (P * kTile)), row = (int)(t / P) % kTile, col = (int)(t % P) * N;
+  const Unit U = unit_of(G, G.whole + q * G.splits);
+  const int64_t i = (int64_t)U.m * kTile + row, j = (int64_t)U.n * kTile + col;
+  if (i >= G.rows || j >= G.cols) return;
+  const float* p = G.part + ((int64_t)q * G.splits * kTile + row) * kTile + col;
+  float h[N] = {};
 #pragma unroll 4
-    for (int s = 0; s < G.splits; ++s, p += G.rows * G.part_ld) {
-      if constexpr (N == 1) {
-        h[0] += *p;
-      } else {
+  for (int s = 0; s < G.splits; ++s, p += kTile * kTile) {
+    if constexpr (N == 1) {
+      h[0] += *p;
+    } else {
 #pragma unroll
-        for (int e = 0; e < N; e += 4) {
-          const float4 x = *reinterpret_cast<const float4*>(p + e);
-          h[e] += x.x;
-          h[e + 1] += x.y;
-          h[e + 2] += x.z;
-          h[e + 3] += x.w;
-        }
+      for (int e = 0; e < N; e += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(p + e);
+        h[e] += x.x;
+        h[e + 1] += x.y;
+        h[e + 2] += x.z;
+        h[e + 3] += x.w;
       }
     }
+  }
+  using TS = typename SlopeOf<T>::type;
 #pragma unroll
-    for (int e = 0; e < N; ++e)
-      if (G.e.bias) h[e] += to_f(static_cast<const T*>(G.e.bias)[j + e]);
-    T* y = static_cast<T*>(G.e.y) + i * G.cols + j;
-    TS* slope = G.e.slope ? static_cast<TS*>(G.e.slope) + i * G.cols + j : nullptr;
-    Pack<T, N> res = {};
-    if (G.e.residual) {
-      res = *reinterpret_cast<const Pack<T, N>*>(static_cast<const T*>(G.e.residual) + i * G.e.rs + j);
-      if (ACT != FX_ACT_NONE && slope) finish<T, ACT, N, true, true>(h, res, y, slope);
-      else finish<T, ACT, N, true, false>(h, res, y, slope);
-    } else {
-      if (ACT != FX_ACT_NONE && slope) finish<T, ACT, N, false, true>(h, res, y, slope);
-      else finish<T, ACT, N, false, false>(h, res, y, slope);
-    }
+  for (int e = 0; e < N; ++e)
+    if (G.e.bias) h[e] += to_f(static_cast<const T*>(G.e.bias)[j + e]);
+  T* y = static_cast<T*>(G.e.y) + i * G.cols + j;
+  TS* slope = G.e.slope ? static_cast<TS*>(G.e.slope) + i * G.cols + j : nullptr;
+  Pack<T, N> res = {};
+  if (G.e.residual) {
+    res = *reinterpret_cast<const Pack<T, N>*>(static_cast<const T*>(G.e.residual) + i * G.e.rs + j);
+    if (ACT != FX_ACT_NONE && slope) finish<T, ACT, N, true, true>(h, res, y, slope);
+    else finish<T, ACT, N, true, false>(h, res, y, slope);
+  } else {
+    if (ACT != FX_ACT_NONE && slope) finish<T, ACT, N, false, true>(h, res, y, slope);
+    else finish<T, ACT, N, false, false>(h, res, y, slope);
   }
 }
 
