@@ -14,7 +14,9 @@ int check(const fx_linear_args* a) {
       a->inner < 1 || a->inner >= 1 << 30 || a->outer < 1 || a->outer >= 1 << 30 || a->x_stride < 0 ||
       a->weight_stride < 0 || a->residual_stride < 0 || a->dy_stride < 0)
     return FX_ERR_SHAPE;
-  return FX_OK;
+  // the tiles of each product are counted in 32 bits
+  const int64_t m = a->rows / 256 + 1, k = a->inner / 256 + 1, n = a->outer / 256 + 1, most = int64_t{1} << 28;
+  return m * n > most || m * k > most || n * k > most ? FX_ERR_SHAPE : FX_OK;
 }
 
 // A matrix as the tensor maps take it: (planes, rows, ld) of bfloat16.
@@ -35,40 +37,91 @@ bool mappable(const void* p, int64_t stride, int64_t rows) {
          stride < (int64_t{1} << 38);
 }
 
-// How a product of rows x cols over `inner` is cut: tiles of a pair of SMs, as many whole rounds of them as there
-// are, and the rest split along k so that it fills the device once. A part has four blocks of k at least, and
-// after a whole round it has to save eight blocks' time (three in float32, whose blocks have six products),
-// about what the join costs.
+// How a product of rows x cols over `inner` is cut into a launch's units.
 struct Cut {
   int64_t rows, cols;
   int blocks, tm, tn, whole, splits, per;
-  int64_t units() const { return whole + ((int64_t)tm * tn - whole) * splits; }
-  int64_t joined() const { return splits > 1 ? (int64_t)tm * tn - whole : 0; }
+  int tiles() const { return tm * tn; }
+  int joined() const { return tiles() - whole; }
+  int units() const { return whole + joined() * splits; }
   size_t part_bytes() const { return (size_t)joined() * splits * (lin::kTile * lin::kTile * sizeof(float)); }
+  // the last n tiles in parts of `most` blocks of k at most
+  void split(int n, int most) {
+    whole = tiles() - n;
+    splits = (blocks + most - 1) / most;
+    per = (blocks + splits - 1) / splits;
+    splits = (blocks + per - 1) / per;
+    if (splits == 1) whole = tiles();
+  }
 };
 
-Cut cut_of(int64_t rows, int64_t cols, int64_t inner, bool f32, int sms) {
+Cut whole_of(int64_t rows, int64_t cols, int64_t inner) {
   Cut C;
   C.rows = rows;
   C.cols = cols;
   C.blocks = (int)ceil_div(inner, lin::kBlockK);
   C.tm = (int)ceil_div(rows, lin::kTile);
   C.tn = (int)ceil_div(cols, lin::kTile);
-  const int64_t tiles = (int64_t)C.tm * C.tn, pairs = sms / 2, rest = tiles % pairs;
-  C.whole = (int)tiles;
+  C.whole = C.tiles();
   C.splits = 1;
   C.per = C.blocks;
-  int64_t splits = rest ? pairs / rest : 1;
-  if (splits > C.blocks / 4) splits = C.blocks / 4;
-  if (splits > 1) {
-    const int64_t per = ceil_div(C.blocks, splits);
-    if (tiles < pairs || C.blocks - per >= (f32 ? 3 : 8)) {
-      C.whole = (int)(tiles - rest);
-      C.per = (int)per;
-      C.splits = (int)ceil_div(C.blocks, per);
+  return C;
+}
+
+// How a launch's n products are cut and ordered (c[0]'s units are the long ones); `ahead` as in lin::Group.
+// - Where the tiles do not fill the device once, k is split so that the parts do, four blocks at least each.
+// - Of one product, the tiles after the whole rounds are split alike, if that saves the time of eight blocks (three in
+//   float32, whose blocks have six products), about what the join costs.
+// - Of two products, the one with the longer tiles is split where a tile takes longer than a pair's share of the work.
+// Measured, us, without and with: 8192 x 8192 -> 2048 bfloat16 (256 tiles of 128 blocks on 74 pairs) 217 and 200.
+int cut(Cut* c, int n, bool f32, int sms) {
+  const int pairs = sms / 2, least = 4;
+  if (n == 2 && c[1].blocks > c[0].blocks) {
+    const Cut t = c[0];
+    c[0] = c[1];
+    c[1] = t;
+  }
+  int64_t tiles = 0, work = 0;
+  for (int i = 0; i < n; ++i) {
+    tiles += c[i].tiles();
+    work += (int64_t)c[i].tiles() * c[i].blocks;
+  }
+  // the shortest parts of the first m products with which their units fit one round
+  const auto fit = [&](int m, int64_t most) {
+    for (;; most += 1 + most / 32) {
+      int64_t units = 0;
+      for (int i = 0; i < m; ++i) units += c[i].tiles() * ceil_div(c[i].blocks, most);
+      if (units <= pairs) break;
+    }
+    for (int i = 0; i < m; ++i) c[i].split(c[i].tiles(), (int)(most < c[i].blocks ? most : c[i].blocks));
+  };
+  const int64_t share = work / pairs > least ? work / pairs : least;
+  if (tiles < pairs) {
+    fit(n, share);
+  } else if (n == 1) {
+    const int rest = (int)(tiles % pairs);
+    if (rest) {
+      const int most = (int)ceil_div(c[0].blocks, pairs / rest);
+      if (most >= least && c[0].blocks - most >= (f32 ? 3 : 8)) c[0].split(rest, most);
+    }
+  } else if (c[0].blocks > share && c[0].tiles() <= pairs) {
+    fit(1, share);
+  }
+  if (n == 1) return 0;
+  // the rounds of short units, beside the last of the long ones, that end the launch soonest
+  const int64_t longs = c[0].units(), shorts = c[1].units(), l = c[0].per, t = c[1].per, rounds = longs / pairs,
+                rest = longs % pairs;
+  int best = 0;
+  int64_t end = INT64_MAX;
+  for (int ahead = 0; ahead <= (rest ? l / t + 1 : 0); ++ahead) {
+    const int64_t left = shorts - ahead * (pairs - rest), more = left > 0 ? ceil_div(left, pairs) : 0;
+    const int64_t a = rest ? (rounds + 1) * l + more * t : 0, b = rounds * l + (ahead + more) * t;
+    if ((a > b ? a : b) < end) {
+      end = a > b ? a : b;
+      best = ahead;
     }
   }
-  return C;
+  return best;
 }
 
 // The plan of a call: which operands are laid out anew, and where.
@@ -88,10 +141,17 @@ struct LinPlan {
   int planes;
   bool new_x, new_w, new_g, slope;  // laid out anew
   size_t x = 0, w = 0, g = 0, sums = 0, part = 0, bytes = 0;
-  Cut y, dx, dw;
+  Cut c[2];
+  int products = 0, ahead = 0, dx = 0, dw = 0;  // where dx and dW are among them
   // the pass over dy: blocks of rows, rows of a block, threads of a row
   int64_t per = 0;
   int blocks = 0, tpr = 0;
+
+  size_t part_bytes() const {
+    size_t n = 0;
+    for (int i = 0; i < products; ++i) n += c[i].part_bytes();
+    return n;
+  }
 };
 
 LinPlan plan_fwd(const fx_linear_args* a, int sms) {
@@ -100,11 +160,12 @@ LinPlan plan_fwd(const fx_linear_args* a, int sms) {
   P.planes = P.f32 ? 3 : 1;
   P.new_x = P.f32 || !mappable(a->x, a->x_stride, a->rows);
   P.new_w = P.f32 || !mappable(a->weight, a->weight_stride, a->outer);
-  P.y = cut_of(a->rows, a->outer, a->inner, P.f32, sms);
+  P.c[P.products++] = whole_of(a->rows, a->outer, a->inner);
+  P.ahead = cut(P.c, 1, P.f32, sms);
   Space S;
   if (P.new_x) P.x = S.take(parts_bytes(a->rows, a->inner, P.planes));
   if (P.new_w) P.w = S.take(parts_bytes(a->outer, a->inner, P.planes));
-  P.part = S.take(P.y.part_bytes());
+  P.part = S.take(P.part_bytes());
   P.bytes = S.bytes ? S.bytes + 256 : 0;
   return P;
 }
@@ -114,10 +175,9 @@ LinPlan plan_bwd(const fx_linear_args* a, int sms) {
   P.f32 = a->dtype == FX_F32;
   P.planes = P.f32 ? 3 : 1;
   P.slope = a->activation != FX_ACT_NONE;
-  const bool products = a->dx || a->dweight;
   P.new_x = a->dweight && (P.f32 || !mappable(a->x, a->x_stride, a->rows));
   P.new_w = a->dx && (P.f32 || !mappable(a->weight, a->weight_stride, a->outer));
-  P.new_g = products && (P.f32 || P.slope || !mappable(a->dy, a->dy_stride, a->rows));
+  P.new_g = (a->dx || a->dweight) && (P.f32 || P.slope || !mappable(a->dy, a->dy_stride, a->rows));
   P.tpr = 1;
   while (P.tpr < 32 && P.tpr * 8 < a->outer) P.tpr *= 2;
   const int64_t groups = 256 / P.tpr, strips = ceil_div(a->outer, P.tpr * 8);
@@ -126,15 +186,16 @@ LinPlan plan_bwd(const fx_linear_args* a, int sms) {
   if (blocks > ceil_div(a->rows, groups * 4)) blocks = ceil_div(a->rows, groups * 4);
   P.per = ceil_div(a->rows, blocks);
   P.blocks = (int)ceil_div(a->rows, P.per);
-  P.dx = cut_of(a->rows, a->inner, a->outer, P.f32, sms);
-  P.dw = cut_of(a->outer, a->inner, a->rows, P.f32, sms);
+  if (a->dx) P.c[P.products++] = whole_of(a->rows, a->inner, a->outer);
+  if (a->dweight) P.c[P.products++] = whole_of(a->outer, a->inner, a->rows);
+  if (P.products) P.ahead = cut(P.c, P.products, P.f32, sms);
+  if (P.products == 2) (ceil_div(a->rows, lin::kBlockK) > ceil_div(a->outer, lin::kBlockK) ? P.dx : P.dw) = 1;
   Space S;
   if (P.new_x) P.x = S.take(parts_bytes(a->rows, a->inner, P.planes));
   if (P.new_w) P.w = S.take(parts_bytes(a->outer, a->inner, P.planes));
   if (P.new_g) P.g = S.take(parts_bytes(a->rows, a->outer, P.planes));
   if (a->dbias) P.sums = S.take((size_t)P.blocks * a->outer * sizeof(float));
-  const size_t p = a->dx ? P.dx.part_bytes() : 0, q = a->dweight ? P.dw.part_bytes() : 0;
-  P.part = S.take(p > q ? p : q);
+  P.part = S.take(P.part_bytes());
   P.bytes = S.bytes ? S.bytes + 256 : 0;
   return P;
 }
@@ -162,114 +223,152 @@ bool pieces(const Epilogue& e, int64_t rows, int64_t cols, int size) {
   return m % 16 == 0;
 }
 
-template <typename T, int NP, int ACT>
-int launch(cudaStream_t s, const lin::Args& G, const lin::Maps& M, int64_t pairs, int64_t joined) {
-  constexpr size_t smem = lin::Shape<NP>::kSmem;
-  auto kern = lin::linear_tc_kernel<T, NP, ACT>;
-  if (raise_smem(kern, smem, smem)) return FX_ERR_CUDA;
-  kern<<<(unsigned)(2 * pairs), lin::kThreads, smem, s>>>(G, M);
-  if (joined) {  // 74 tiles at most, 256 blocks each
-    constexpr int N = 16 / sizeof(T);
-    if (G.vec) lin::linear_join_kernel<T, ACT, N><<<(unsigned)(joined * (256 / N)), 256, 0, s>>>(G);
-    else lin::linear_join_kernel<T, ACT, 1><<<(unsigned)(joined * 256), 256, 0, s>>>(G);
-  }
-  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
-}
-
+// The products of a call, gathered for one launch.
 template <typename T, int NP>
-int product(cudaStream_t s, const Cut& C, const Operand& a, bool a_mn, const Operand& b, bool b_mn, const Epilogue& e,
-            float* part, int sms) {
+struct Products {
+  const LinPlan& P;
+  lin::Group G{};
   lin::Maps M;
-  int st = make_map(&M.a, a, NP, a_mn);
-  if (!st) st = make_map(&M.b, b, NP, b_mn);
-  if (st) return st;
-  if ((int64_t)C.tm * C.tn > INT32_MAX / 2) return FX_ERR_SHAPE;
-  lin::Args G{};
-  G.rows = C.rows;
-  G.cols = C.cols;
-  G.blocks = C.blocks;
-  G.tm = C.tm;
-  G.tn = C.tn;
-  G.whole = C.whole;
-  G.splits = C.splits;
-  G.per = C.per;
-  G.a_mn = a_mn;
-  G.b_mn = b_mn;
-  G.vec = pieces(e, C.rows, C.cols, sizeof(T));
-  G.polls = wait_polls();
-  G.part = part;
-  G.e = e;
-  const int64_t pairs = C.units() < sms / 2 ? C.units() : sms / 2;
-  switch (e.act) {
-    case FX_ACT_RELU: return launch<T, NP, FX_ACT_RELU>(s, G, M, pairs, C.joined());
-    case FX_ACT_SILU: return launch<T, NP, FX_ACT_SILU>(s, G, M, pairs, C.joined());
-    case FX_ACT_GELU: return launch<T, NP, FX_ACT_GELU>(s, G, M, pairs, C.joined());
-    case FX_ACT_GELU_TANH: return launch<T, NP, FX_ACT_GELU_TANH>(s, G, M, pairs, C.joined());
-    case FX_ACT_TANH: return launch<T, NP, FX_ACT_TANH>(s, G, M, pairs, C.joined());
-    default: return launch<T, NP, FX_ACT_NONE>(s, G, M, pairs, C.joined());
+  float* parts;
+
+  Products(const LinPlan& P, unsigned char* ws) : P(P), parts(reinterpret_cast<float*>(ws + P.part)) {}
+  int set(int n, const Operand& a, bool a_mn, const Operand& b, bool b_mn, const Epilogue& e) {
+    const Cut& C = P.c[n];
+    lin::Args& A = G.p[n];
+    A.rows = C.rows;
+    A.cols = C.cols;
+    A.blocks = C.blocks;
+    A.tm = C.tm;
+    A.tn = C.tn;
+    A.whole = C.whole;
+    A.splits = C.splits;
+    A.per = C.per;
+    A.a_mn = a_mn;
+    A.b_mn = b_mn;
+    A.vec = pieces(e, C.rows, C.cols, sizeof(T));
+    A.part = parts + (n ? P.c[0].part_bytes() / sizeof(float) : 0);
+    A.e = e;
+    int st = make_map(&M.m[2 * n], a, NP, a_mn);
+    if (!st) st = make_map(&M.m[2 * n + 1], b, NP, b_mn);
+    return st;
   }
-}
+  template <int ACT>
+  int launch(cudaStream_t s, int sms) {
+    constexpr size_t smem = lin::Shape<NP>::kSmem;
+    auto kern = lin::linear_tc_kernel<T, NP, ACT>;
+    if (raise_smem(kern, smem, smem)) return FX_ERR_CUDA;
+    G.polls = wait_polls();
+    const int units = G.p[0].units() + G.p[1].units(), pairs = units < sms / 2 ? units : sms / 2;
+    G.longs = P.products == 2 ? G.p[0].units() : G.p[0].whole;
+    G.shorts = units - G.longs;
+    G.ahead = P.ahead;
+    kern<<<2 * pairs, lin::kThreads, smem, s>>>(G, M);
+    const int joined = G.p[0].joined() + G.p[1].joined();
+    if (joined) {  // fewer tiles than pairs
+      constexpr int N = 16 / sizeof(T);
+      if (G.p[0].vec && (P.products == 1 || G.p[1].vec)) lin::linear_join_kernel<T, ACT, N><<<joined * (lin::kTile / N), 256, 0, s>>>(G);
+      else lin::linear_join_kernel<T, ACT, 1><<<joined * lin::kTile, 256, 0, s>>>(G);
+    }
+    return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+  }
+  int launch(cudaStream_t s, int act, int sms) {
+    switch (act) {
+      case FX_ACT_RELU: return launch<FX_ACT_RELU>(s, sms);
+      case FX_ACT_SILU: return launch<FX_ACT_SILU>(s, sms);
+      case FX_ACT_GELU: return launch<FX_ACT_GELU>(s, sms);
+      case FX_ACT_GELU_TANH: return launch<FX_ACT_GELU_TANH>(s, sms);
+      case FX_ACT_TANH: return launch<FX_ACT_TANH>(s, sms);
+      default: return launch<FX_ACT_NONE>(s, sms);
+    }
+  }
+};
 
 template <typename T, int NP>
-int layout(cudaStream_t s, const void* src, int64_t stride, int64_t rows, int64_t cols, void* out, int sms) {
-  lin::PartsArgs A{src, stride, rows, cols, ld_of(cols), static_cast<uint16_t*>(out),
-                   aligned(src, stride, rows, cols, sizeof(T))};
-  const int64_t blocks = ceil_div(rows * (A.ld / 8), 256), most = (int64_t)sms * 8;
-  lin::linear_parts_kernel<T, NP><<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(A);
-  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
-}
+struct Prep {
+  lin::PrepArgs A{};
+  int n = 0, sms;
 
-// The operand in place, or laid out anew at `out`.
+  explicit Prep(int sms) : sms(sms) {}
+  // The operand in place, or laid out anew at `out`.
+  Operand operand(bool anew, const void* p, int64_t stride, int64_t rows, int64_t cols, void* out) {
+    if (!anew) return {p, rows, cols, stride};
+    const int64_t ld = ld_of(cols), blocks = ceil_div(rows * (ld / 8), 256), most = (int64_t)sms * 8;
+    A.o[n++] = {p, stride, rows, cols, ld, static_cast<uint16_t*>(out), aligned(p, stride, rows, cols, sizeof(T)),
+                (int)(blocks < most ? blocks : most)};
+    return {out, rows, cols, ld};
+  }
+  int launch(cudaStream_t s) {
+    const int blocks = A.g.blocks + A.o[0].blocks + A.o[1].blocks;
+    if (!blocks) return FX_OK;
+    lin::linear_prep_kernel<T, NP><<<blocks, 256, 0, s>>>(A);
+    return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+  }
+};
+
+// A thread that has made no call yet (autograd's, on its first backward pass) has no current context, which the encoding
+// of tensor maps, a driver call, needs; this runtime call brings it.
 template <typename T, int NP>
-int operand(cudaStream_t s, bool anew, const void* p, int64_t stride, int64_t rows, int64_t cols, void* out, int sms,
-            Operand& o) {
-  o = {anew ? out : p, rows, cols, anew ? ld_of(cols) : stride};
-  return anew ? layout<T, NP>(s, p, stride, rows, cols, out, sms) : FX_OK;
+int ready() {
+  return raise_smem(lin::linear_tc_kernel<T, NP, FX_ACT_NONE>, lin::Shape<NP>::kSmem, lin::Shape<NP>::kSmem);
 }
 
 template <typename T, int NP>
 int forward(cudaStream_t s, const fx_linear_args* a, const LinPlan& P, unsigned char* ws, int sms) {
-  Operand x, w;
-  int st = operand<T, NP>(s, P.new_x, a->x, a->x_stride, a->rows, a->inner, ws + P.x, sms, x);
-  if (!st) st = operand<T, NP>(s, P.new_w, a->weight, a->weight_stride, a->outer, a->inner, ws + P.w, sms, w);
-  if (st) return st;
-  const Epilogue e{a->activation, a->bias, a->residual, a->residual_stride, a->y, a->slope};
-  return product<T, NP>(s, P.y, x, false, w, false, e, reinterpret_cast<float*>(ws + P.part), sms);
+  if (ready<T, NP>()) return FX_ERR_CUDA;
+  Prep<T, NP> prep(sms);
+  const Operand x = prep.operand(P.new_x, a->x, a->x_stride, a->rows, a->inner, ws + P.x);
+  const Operand w = prep.operand(P.new_w, a->weight, a->weight_stride, a->outer, a->inner, ws + P.w);
+  Products<T, NP> products(P, ws);
+  int st = products.set(0, x, false, w, false, {a->activation, a->bias, a->residual, a->residual_stride, a->y, a->slope});
+  if (!st) st = prep.launch(s);
+  return st ? st : products.launch(s, a->activation, sms);
 }
 
 template <typename T, int NP>
 int backward(cudaStream_t s, const fx_linear_args* a, const LinPlan& P, unsigned char* ws, int sms) {
+  if (ready<T, NP>()) return FX_ERR_CUDA;
+  Prep<T, NP> prep(sms);
   Operand g{a->dy, a->rows, a->outer, a->dy_stride};
   if (P.new_g || a->dbias) {
-    const void* slope = P.slope ? a->slope : nullptr;
-    const int64_t ld = ld_of(a->outer);
-    lin::SlopeArgs A{a->dy, slope, a->dy_stride, a->rows, a->outer, ld, P.per,
-                     P.new_g ? reinterpret_cast<uint16_t*>(ws + P.g) : nullptr,
-                     a->dbias ? reinterpret_cast<float*>(ws + P.sums) : nullptr, P.tpr,
-                     aligned(a->dy, a->dy_stride, a->rows, a->outer, sizeof(T)) &&
-                         reinterpret_cast<uintptr_t>(slope) % 16 == 0};
-    const dim3 grid((unsigned)ceil_div(a->outer, P.tpr * 8), (unsigned)P.blocks);
-    lin::linear_slope_kernel<T, NP><<<grid, 256, 0, s>>>(A);
-    if (a->dbias) lin::linear_bias_kernel<T><<<(unsigned)ceil_div(a->outer, 32), 256, 0, s>>>(A.sums, P.blocks, a->outer, a->dbias);
-    if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
-    if (P.new_g) g = {A.out, a->rows, a->outer, ld};
+    lin::PrepArgs& A = prep.A;
+    A.slope = P.slope ? a->slope : nullptr;
+    A.sums = a->dbias ? reinterpret_cast<float*>(ws + P.sums) : nullptr;
+    A.per = P.per;
+    A.tpr = P.tpr;
+    const int64_t strips = ceil_div(a->outer, P.tpr * 8);
+    if (strips * P.blocks > INT32_MAX / 2) return FX_ERR_SHAPE;
+    A.strips = (int)strips;
+    A.g = {a->dy, a->dy_stride, a->rows, a->outer, ld_of(a->outer), P.new_g ? reinterpret_cast<uint16_t*>(ws + P.g) : nullptr,
+           aligned(a->dy, a->dy_stride, a->rows, a->outer, sizeof(T)) && reinterpret_cast<uintptr_t>(A.slope) % 16 == 0,
+           A.strips * P.blocks};
+    if (P.new_g) g = {A.g.out, a->rows, a->outer, A.g.ld};
   }
-  float* part = reinterpret_cast<float*>(ws + P.part);
+  const Epilogue none{FX_ACT_NONE, nullptr, nullptr, 0, nullptr, nullptr};
+  Products<T, NP> products(P, ws);
+  int st = FX_OK;
   if (a->dx) {
-    Operand w;
-    int st = operand<T, NP>(s, P.new_w, a->weight, a->weight_stride, a->outer, a->inner, ws + P.w, sms, w);
-    const Epilogue e{FX_ACT_NONE, nullptr, nullptr, 0, a->dx, nullptr};
-    if (!st) st = product<T, NP>(s, P.dx, g, false, w, true, e, part, sms);
-    if (st) return st;
+    const Operand w = prep.operand(P.new_w, a->weight, a->weight_stride, a->outer, a->inner, ws + P.w);
+    Epilogue e = none;
+    e.y = a->dx;
+    st = products.set(P.dx, g, false, w, true, e);
   }
-  if (a->dweight) {
-    Operand x;
-    int st = operand<T, NP>(s, P.new_x, a->x, a->x_stride, a->rows, a->inner, ws + P.x, sms, x);
-    const Epilogue e{FX_ACT_NONE, nullptr, nullptr, 0, a->dweight, nullptr};
-    if (!st) st = product<T, NP>(s, P.dw, g, true, x, true, e, part, sms);
-    if (st) return st;
+  if (!st && a->dweight) {
+    const Operand x = prep.operand(P.new_x, a->x, a->x_stride, a->rows, a->inner, ws + P.x);
+    Epilogue e = none;
+    e.y = a->dweight;
+    st = products.set(P.dw, g, true, x, true, e);
   }
-  return FX_OK;
+  if (!st) st = prep.launch(s);
+  if (st) return st;
+  if (P.products) {
+    products.G.sums = prep.A.sums;
+    products.G.dbias = a->dbias;
+    products.G.sum_blocks = P.blocks;
+    products.G.sum_cols = a->outer;
+    return products.launch(s, FX_ACT_NONE, sms);
+  }
+  if (a->dbias) lin::linear_bias_kernel<T><<<(unsigned)ceil_div(a->outer, 256), 256, 0, s>>>(prep.A.sums, P.blocks, a->outer, a->dbias);
+  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
 unsigned char* base_of(void* ws) { return reinterpret_cast<unsigned char*>(align256(reinterpret_cast<uintptr_t>(ws))); }

@@ -41,20 +41,35 @@ struct Shape {
   static constexpr int kChunk = 2;  // blocks of k in an accumulator (three parts)
 };
 
-struct alignas(64) Maps {
-  CUtensorMap a, b;
-};
-
+// One product, cut into units: tiles that a pair does alone, then parts of the others.
 struct Args {
-  int64_t rows, cols;  // of the result
-  int blocks, tm, tn;  // blocks of k, tiles
-  int whole, splits, per;  // tiles that a pair does alone; parts of the others, blocks of a part
-  int a_mn, b_mn, vec;  // vec: rows of y, slope, residual and bias are whole pieces of 16 bytes
-  uint32_t polls;
-  float* part;  // of the tiles from `whole` on: (tile, part, 256, 256)
+  int64_t rows, cols;      // of the result
+  int blocks, tm, tn;      // blocks of k, tiles
+  int whole, splits, per;  // tiles done alone; parts of each other tile, blocks of k of a part
+  int a_mn, b_mn, vec;     // vec: rows of y, slope, residual and bias are whole pieces of 16 bytes
+  float* part;             // of the tiles from `whole` on: (tile, part, 256, 256)
   Epilogue e;
 
-  __host__ __device__ int units() const { return whole + (tm * tn - whole) * splits; }
+  __host__ __device__ int joined() const { return tm * tn - whole; }
+  __host__ __device__ int units() const { return whole + joined() * splits; }
+};
+
+// The products of a launch: one, or a backward pass' two, whose tiles fill the device together. Its units are of two
+// lengths, `longs` long ones (of one product its whole tiles, of two the first product's units) and then `shorts` short
+// ones. The pairs of SMs take the long ones in turn; those left without one in the last round do `ahead` rounds of
+// short ones meanwhile, then all pairs take the other short ones in turn.
+struct Group {
+  Args p[2];
+  int longs, shorts, ahead;
+  uint32_t polls;
+  // a backward pass' sums of g over blocks of rows, (sum_blocks, sum_cols), and where their sums go
+  const float* sums;
+  void* dbias;
+  int sum_blocks;
+  int64_t sum_cols;
+};
+struct alignas(64) Maps {
+  CUtensorMap m[4];  // A and B of each product
 };
 
 // ---------------------------------------------------------------- instructions of a pair
@@ -292,21 +307,22 @@ __device__ __forceinline__ void store_part(float* out, const unsigned char* stag
 }
 
 struct Unit {
-  int m, n, part, first, last;  // tile, place among the parts (-1: whole), blocks of k
+  int q, m, n, part, first, last;  // product, tile, place among the parts (-1: whole), blocks of k
 };
 // Tiles in groups of 8 rows of tiles, down the columns of a group, so that what runs at a time shares
 // rows and columns; the parts of a tile next to each other.
 __device__ __forceinline__ Unit unit_of(const Args& G, int u) {
   Unit U;
   int t = u;
+  U.q = 0;
   U.part = -1;
   U.first = 0;
   U.last = G.blocks;
   if (u >= G.whole) {
     U.part = u - G.whole;
-    const int q = U.part / G.splits;
-    t = G.whole + q;
-    U.first = (U.part - q * G.splits) * G.per;
+    const int v = U.part / G.splits;
+    t = G.whole + v;
+    U.first = (U.part - v * G.splits) * G.per;
     U.last = min(U.first + G.per, G.blocks);
   }
   const int group = t / (8 * G.tn), in = t - group * 8 * G.tn;
@@ -314,6 +330,25 @@ __device__ __forceinline__ Unit unit_of(const Args& G, int u) {
   U.n = rows == 8 ? in >> 3 : in / rows;
   U.m = group * 8 + in - U.n * rows;
   return U;
+}
+// Pair `pair`'s i-th unit of a launch by `pairs`; false behind its last.
+__device__ __forceinline__ bool unit_of(const Group& G, int pair, int pairs, int i, Unit& U) {
+  const int rounds = G.longs / pairs, rest = G.longs - rounds * pairs;
+  int u;
+  if (i < rounds + (pair < rest)) {
+    u = i * pairs + pair;
+  } else {
+    i -= rounds;
+    int v;
+    if (pair >= rest && i < G.ahead) v = i * (pairs - rest) + pair - rest;
+    else v = G.ahead * (pairs - rest) + (i - (pair < rest ? 1 : G.ahead)) * pairs + pair;
+    if (v >= G.shorts) return false;
+    u = G.longs + v;
+  }
+  const int first = G.p[0].units(), q = u >= first;
+  U = unit_of(G.p[q], u - (q ? first : 0));
+  U.q = q;
+  return true;
 }
 
 // The epilogue of a warp's 32 rows and 64 columns of a tile, in TMEM from `from` on, C columns at a time through the
@@ -362,9 +397,20 @@ __device__ __forceinline__ void epilogue(const Args& G, const Unit& U, unsigned 
   }
 }
 
+// The sums of g over the rows from those of blocks of rows, in order: 32 columns a warp.
+template <typename T>
+__device__ __forceinline__ void bias_sums(const float* sums, int blocks, int64_t cols, void* dbias, int64_t warp, int64_t warps) {
+  for (int64_t j = warp * 32 + (threadIdx.x & 31); j < cols; j += warps * 32) {
+    float s = 0.f;
+#pragma unroll 16
+    for (int b = 0; b < blocks; ++b) s += sums[b * cols + j];
+    static_cast<T*>(dbias)[j] = from_f<T>(s);
+  }
+}
+
 template <typename T, int NP, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    linear_tc_kernel(const __grid_constant__ Args G, const __grid_constant__ Maps M) {
+    linear_tc_kernel(const __grid_constant__ Group G, const __grid_constant__ Maps M) {
   using S = Shape<NP>;
   constexpr int ST = S::kStages;
   extern __shared__ unsigned char raw[];
@@ -392,15 +438,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_sync();
   fence_after_sync();
   const uint32_t tmem = slot;
-  const int units = G.units(), pairs = gridDim.x >> 1;
-  const int chunk = NP == 1 ? G.blocks : S::kChunk;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  Unit U;
+  constexpr int kAll = 1 << 30;
+  constexpr int chunk = NP == 1 ? kAll : S::kChunk;  // blocks of k in an accumulator
 
   if (warp == 0) {
     // -------------------------------------------------------- copies, one thread of each block
     if (lane == 0) {
       int it = 0;
-      for (int u = blockIdx.x >> 1; u < units && state != DEAD; u += pairs) {
-        const Unit U = unit_of(G, u);
+      for (int n = 0; state != DEAD && unit_of(G, pair, pairs, n, U); ++n) {
+        const CUtensorMap *ma = &M.m[2 * U.q], *mb = ma + 1;
+        const bool a_mn = G.p[U.q].a_mn, b_mn = G.p[U.q].b_mn;
         const int i0 = U.m * kTile + rank * kHalf, j0 = U.n * kTile + rank * kHalf;
         for (int kb = U.first; kb < U.last; ++kb, ++it) {
           const int st = it % ST;
@@ -410,17 +459,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int p = 0; p < NP; ++p) {
             const uint32_t a = at + p * kOperand, b = at + (NP + p) * kOperand;
-            if (G.a_mn) {
-              tma_box(a, &M.a, i0, kb * kBlockK, p, bar);
-              tma_box(a + 8192, &M.a, i0 + 64, kb * kBlockK, p, bar);
+            if (a_mn) {
+              tma_box(a, ma, i0, kb * kBlockK, p, bar);
+              tma_box(a + 8192, ma, i0 + 64, kb * kBlockK, p, bar);
             } else {
-              tma_box(a, &M.a, kb * kBlockK, i0, p, bar);
+              tma_box(a, ma, kb * kBlockK, i0, p, bar);
             }
-            if (G.b_mn) {
-              tma_box(b, &M.b, j0, kb * kBlockK, p, bar);
-              tma_box(b + 8192, &M.b, j0 + 64, kb * kBlockK, p, bar);
+            if (b_mn) {
+              tma_box(b, mb, j0, kb * kBlockK, p, bar);
+              tma_box(b + 8192, mb, j0 + 64, kb * kBlockK, p, bar);
             } else {
-              tma_box(b, &M.b, kb * kBlockK, j0, p, bar);
+              tma_box(b, mb, kb * kBlockK, j0, p, bar);
             }
           }
         }
@@ -433,14 +482,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // -------------------------------------------------------- products, one warp of the pair
     // The whole warp runs the loops, so that descriptors stay in uniform registers, and one lane issues.
     if (rank == 0) {
-      const uint32_t idesc = 1u << 4 | 1u << 7 | 1u << 10 | (G.a_mn ? 1u << 15 : 0u) | (G.b_mn ? 1u << 16 : 0u) |
-                             (uint32_t)(kTile >> 3) << 17 | (uint32_t)(kTile >> 4) << 24;
-      const uint32_t sa = G.a_mn ? 128 : 2, sb = G.b_mn ? 128 : 2;  // 16 entries of k further, in 16 bytes
-      const uint64_t a0 = desc(smem_u32(sm), G.a_mn), b0 = desc(smem_u32(sm) + NP * kOperand, G.b_mn);
       int st = 0, ch = 0;
       uint32_t phase = 0;
-      for (int u = blockIdx.x >> 1; u < units && state != DEAD; u += pairs) {
-        const Unit U = unit_of(G, u);
+      for (int n = 0; state != DEAD && unit_of(G, pair, pairs, n, U); ++n) {
+        const bool a_mn = G.p[U.q].a_mn, b_mn = G.p[U.q].b_mn;
+        const uint32_t idesc = 1u << 4 | 1u << 7 | 1u << 10 | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
+                               (uint32_t)(kTile >> 3) << 17 | (uint32_t)(kTile >> 4) << 24;
+        const uint32_t sa = a_mn ? 128 : 2, sb = b_mn ? 128 : 2;  // 16 entries of k further, in 16 bytes
+        const uint64_t a0 = desc(smem_u32(sm), a_mn), b0 = desc(smem_u32(sm) + NP * kOperand, b_mn);
         for (int k0 = U.first; k0 < U.last; k0 += chunk, ++ch) {
           const int buf = ch % 2;
           if (!wait(&sum_empty[buf], (ch / 2 & 1) ^ 1, &state, G.polls)) break;
@@ -477,20 +526,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
   } else {
     // -------------------------------------------------------- epilogue
+    if (G.dbias)  // while the first tile's products run
+      bias_sums<T>(G.sums, G.sum_blocks, G.sum_cols, G.dbias, blockIdx.x * kWarps + warp - 2, gridDim.x * kWarps);
     constexpr int C = 16, B = 64 / C;
     const int quarter = warp & 3, strip = (warp - 2) >> 2, row = rank * kHalf + quarter * 32, col = strip * 64;
     unsigned char* stage = sm + ST * S::kStage + (warp - 2) * S::kBlock;
     const uint32_t lanes = tmem + ((uint32_t)quarter << 21) + col;
     int ch = 0;
-    for (int u = blockIdx.x >> 1; u < units && state != DEAD; u += pairs) {
-      const Unit U = unit_of(G, u);
+    for (int n = 0; state != DEAD && unit_of(G, pair, pairs, n, U); ++n) {
       float acc[NP == 1 ? 1 : B][C];
       for (int k0 = U.first; k0 < U.last; k0 += chunk, ++ch) {
         const int buf = ch % 2;
         if (!wait(&sum_full[buf], ch / 2 & 1, &state, G.polls)) break;
         fence_after_sync();
         const uint32_t from = lanes + buf * kTile;
-        const bool last = k0 + chunk >= U.last;
+        const bool last = NP == 1 || k0 + chunk >= U.last;
         if constexpr (NP > 1) {
           // The sums so far are in registers; with the last of them they go back to TMEM, from where they are stored.
           const bool more = k0 > U.first;
@@ -514,7 +564,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (last) tmem_wait_st();
           }
         }
-        if (last) epilogue<T, ACT, S::kStore>(G, U, stage, row, col, from, &state);
+        if (last) epilogue<T, ACT, S::kStore>(G.p[U.q], U, stage, row, col, from, &state);
         fence_before_sync();
         __syncwarp();
         if (lane == 0) arrive_at(first_block(&sum_empty[buf]));
@@ -529,16 +579,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------- around the products
-// The parts of the split tiles in order, then the epilogue; N columns a thread.
+// The parts of the split tiles in order, then the epilogue; N columns a thread, P * 256 threads a tile. Both
+// products' tiles, one after the other.
 template <typename T, int ACT, int N>
-__global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ Args G) {
+__global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ Group H) {
   constexpr int P = kTile / N;  // pieces of a row
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int q = (int)(t / (P * kTile)), row = (int)(t / P) % kTile, col = (int)(t % P) * N;
-  const Unit U = unit_of(G, G.whole + q * G.splits);
+  int v = (int)(t / (P * kTile));
+  const int second = v >= H.p[0].joined();
+  const Args& G = H.p[second];
+  if (second) v -= H.p[0].joined();
+  const int row = (int)(t / P) % kTile, col = (int)(t % P) * N;
+  const Unit U = unit_of(G, G.whole + v * G.splits);
   const int64_t i = (int64_t)U.m * kTile + row, j = (int64_t)U.n * kTile + col;
   if (i >= G.rows || j >= G.cols) return;
-  const float* p = G.part + ((int64_t)q * G.splits * kTile + row) * kTile + col;
+  const float* p = G.part + ((int64_t)v * G.splits * kTile + row) * kTile + col;
   float h[N] = {};
 #pragma unroll 4
   for (int s = 0; s < G.splits; ++s, p += kTile * kTile) {
@@ -620,18 +675,27 @@ __device__ __forceinline__ void store_parts(uint16_t* out, int64_t plane, const 
   for (int p = 0; p < NP; ++p) *reinterpret_cast<uint4*>(out + p * plane) = make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]);
 }
 
-// An operand as the tensor maps take it: NP planes of bfloat16, (NP, rows, ld), ld a multiple of 8.
-struct PartsArgs {
+// What is laid out anew for the products: up to two operands as NP planes of bfloat16, (NP, rows, ld), ld a multiple
+// of 8, and g = dy act'(h) likewise (out not NULL) with each block's sums over its rows (sums not NULL): `tpr` threads
+// share a row of g, eight columns each, `per` rows a block.
+struct Layout {
   const void* src;
   int64_t stride, rows, cols, ld;
   uint16_t* out;
-  int vec;
+  int vec, blocks;  // blocks of the launch that work on it
+};
+struct PrepArgs {
+  Layout g, o[2];
+  const void* slope;
+  float* sums;  // (blocks of rows, cols)
+  int64_t per;
+  int tpr, strips;
 };
 
 template <typename T, int NP>
-__global__ void __launch_bounds__(256) linear_parts_kernel(const __grid_constant__ PartsArgs A) {
+__device__ __forceinline__ void lay_out(const Layout& A, int block) {
   const int64_t eights = A.ld / 8, n = A.rows * eights;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
+  for (int64_t t = (int64_t)block * 256 + threadIdx.x; t < n; t += (int64_t)A.blocks * 256) {
     const int64_t i = t / eights, j = (t - i * eights) * 8;
     float x[8];
     load_eight<T>(static_cast<const T*>(A.src) + i * A.stride + j, A.cols - j, A.vec, x);
@@ -639,32 +703,31 @@ __global__ void __launch_bounds__(256) linear_parts_kernel(const __grid_constant
   }
 }
 
-// g = dy act'(h) as parts (out not NULL), and each block's sums over its rows (sums not NULL):
-// `tpr` threads share a row, eight columns each.
-struct SlopeArgs {
-  const void *dy, *slope;
-  int64_t stride, rows, cols, ld, per;  // per: rows of a block
-  uint16_t* out;
-  float* sums;  // (gridDim.y, cols)
-  int tpr, vec;
-};
-
 template <typename T, int NP>
-__global__ void __launch_bounds__(256) linear_slope_kernel(const __grid_constant__ SlopeArgs A) {
+__global__ void __launch_bounds__(256) linear_prep_kernel(const __grid_constant__ PrepArgs P) {
   using TS = typename SlopeOf<T>::type;
   __shared__ float share[8][256];
-  const int groups = 256 / A.tpr, g = threadIdx.x / A.tpr, col = threadIdx.x & (A.tpr - 1);
-  const int64_t j = ((int64_t)blockIdx.x * A.tpr + col) * 8, r0 = blockIdx.y * A.per;
-  const int64_t end = r0 + A.per < A.rows ? r0 + A.per : A.rows;
+  int block = blockIdx.x;
+  if (block >= P.g.blocks) {
+    block -= P.g.blocks;
+    if (block < P.o[0].blocks) lay_out<T, NP>(P.o[0], block);
+    else lay_out<T, NP>(P.o[1], block - P.o[0].blocks);
+    return;
+  }
+  const Layout& A = P.g;
+  const int strip = block % P.strips, rows = block / P.strips;
+  const int groups = 256 / P.tpr, g = threadIdx.x / P.tpr, col = threadIdx.x & (P.tpr - 1);
+  const int64_t j = ((int64_t)strip * P.tpr + col) * 8, r0 = rows * P.per;
+  const int64_t end = r0 + P.per < A.rows ? r0 + P.per : A.rows;
   float sum[8] = {};
   if (j < A.cols) {
 #pragma unroll 2
     for (int64_t i = r0 + g; i < end; i += groups) {
       float x[8];
-      load_eight<T>(static_cast<const T*>(A.dy) + i * A.stride + j, A.cols - j, A.vec, x);
-      if (A.slope) {
+      load_eight<T>(static_cast<const T*>(A.src) + i * A.stride + j, A.cols - j, A.vec, x);
+      if (P.slope) {
         float d[8];
-        load_eight<TS>(static_cast<const TS*>(A.slope) + i * A.cols + j, A.cols - j, A.vec, d);
+        load_eight<TS>(static_cast<const TS*>(P.slope) + i * A.cols + j, A.cols - j, A.vec, d);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = __fmul_rn(x[e], d[e]);  // the same g whether it is stored or only summed
       }
@@ -673,38 +736,24 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(const __grid_constant
       for (int e = 0; e < 8; ++e) sum[e] += x[e];
     }
   }
-  if (!A.sums) return;
+  if (!P.sums) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) share[e][threadIdx.x] = sum[e];
   __syncthreads();
   // the groups' sums in order, a column a thread
-  for (int c = threadIdx.x; c < A.tpr * 8; c += 256) {
-    const int64_t jj = (int64_t)blockIdx.x * A.tpr * 8 + c;
+  for (int c = threadIdx.x; c < P.tpr * 8; c += 256) {
+    const int64_t jj = (int64_t)strip * P.tpr * 8 + c;
     if (jj >= A.cols) break;
     float s = 0.f;
-    for (int k = 0; k < groups; ++k) s += share[c & 7][k * A.tpr + (c >> 3)];
-    A.sums[blockIdx.y * A.cols + jj] = s;
+    for (int k = 0; k < groups; ++k) s += share[c & 7][k * P.tpr + (c >> 3)];
+    P.sums[rows * A.cols + jj] = s;
   }
 }
 
-// The blocks' sums in order: 32 columns a block, eight warps that share the blocks.
+// The sums alone, where no product follows.
 template <typename T>
 __global__ void __launch_bounds__(256) linear_bias_kernel(const float* sums, int blocks, int64_t cols, void* dbias) {
-  __shared__ float share[8][32];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t j = (int64_t)blockIdx.x * 32 + lane;
-  float s = 0.f;
-  if (j < cols) {
-#pragma unroll 8
-    for (int b = w; b < blocks; b += 8) s += sums[b * cols + j];
-  }
-  share[w][lane] = s;
-  __syncthreads();
-  if (w == 0 && j < cols) {
-#pragma unroll
-    for (int k = 1; k < 8; ++k) s += share[k][lane];
-    static_cast<T*>(dbias)[j] = from_f<T>(s);
-  }
+  bias_sums<T>(sums, blocks, cols, dbias, blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8);
 }
 
 }  // namespace lin
