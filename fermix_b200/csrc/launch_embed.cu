@@ -74,9 +74,9 @@ SortPlan plan_of(const fx_embed_args* a, const Shape& s, int sms) {
 }
 
 template <typename T, int E>
-int run_fwd(cudaStream_t s, const EmbedFwd& A) {
-  const int64_t per = (int64_t)(kEmbedThreads / A.tpr) * kEmbedRows, blocks = (A.count + per - 1) / per;
-  embed_fwd_kernel<T, E><<<(unsigned)blocks, kEmbedThreads, 0, s>>>(A);
+int run_fwd(cudaStream_t s, const EmbedFwd& A, int sms) {
+  const int64_t per = (int64_t)(kEmbedThreads / A.tpr) * kEmbedRows, blocks = (A.count + per - 1) / per, most = (int64_t)sms * 8;
+  embed_fwd_kernel<T, E><<<(unsigned)(blocks < most ? blocks : most), kEmbedThreads, 0, s>>>(A);
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
@@ -87,10 +87,11 @@ int run_scan(cudaStream_t s, const EmbedGrad& A, const Tokens& tok) {
 }
 
 template <typename T, int E>
-int run_sums(cudaStream_t s, const EmbedGrad& A) {
+int run_sums(cudaStream_t s, const EmbedGrad& A, int sms) {
   const int groups = kEmbedThreads / A.tpr;
   const unsigned cols = (unsigned)((A.chunks + A.tpr - 1) / A.tpr);
-  const dim3 windows((A.windows + groups - 1) / groups, cols), rows((unsigned)((A.rows + groups - 1) / groups), cols);
+  const int64_t blocks = (A.rows + A.rpb - 1) / A.rpb, most = ((int64_t)sms * 8 + cols - 1) / cols;
+  const dim3 windows((A.windows + groups - 1) / groups, cols), rows((unsigned)(blocks < most ? blocks : most), cols);
   embed_window_kernel<T, E><<<windows, kEmbedThreads, 0, s>>>(A);
   embed_join_kernel<T, E><<<rows, kEmbedThreads, 0, s>>>(A);
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
@@ -138,11 +139,13 @@ int fermix_token_embedding(void* stream, const fx_embed_args* a) {
   if (e) return e;
   if (a->count == 0) return FX_OK;
   if (!a->tokens || !a->weight || !a->out) return FX_ERR_NULL;
+  const DevInfo* D = dev_info();
+  if (!D) return FX_ERR_DEVICE;
   const Shape h = shape_of(a, a->weight, a->out);
   EmbedFwd A{tokens_of(a), a->weight, a->out, a->count, a->rows, a->width, h.chunks, h.tpr, a->scale};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a->dtype == FX_F32) return h.vec ? run_fwd<float, 4>(s, A) : run_fwd<float, 1>(s, A);
-  return h.vec ? run_fwd<bf16, 8>(s, A) : run_fwd<bf16, 1>(s, A);
+  if (a->dtype == FX_F32) return h.vec ? run_fwd<float, 4>(s, A, D->sms) : run_fwd<float, 1>(s, A, D->sms);
+  return h.vec ? run_fwd<bf16, 8>(s, A, D->sms) : run_fwd<bf16, 1>(s, A, D->sms);
 }
 
 // Without the pointers the larger of the two forms counts: entry by entry, fewer windows never
@@ -185,11 +188,12 @@ int fermix_token_embedding_grad(void* stream, const fx_embed_args* a, void* ws, 
   unsigned char* base = reinterpret_cast<unsigned char*>(align256(reinterpret_cast<uintptr_t>(ws)));
   A.window = P.window;
   A.windows = P.windows;
+  A.rpb = a->count / a->rows >= 2 * P.window ? 1 : kEmbedThreads / h.tpr;
   A.part = reinterpret_cast<float*>(base + P.part);
   const int st = sort(s, a, P, base, A);
   if (st) return st;
-  if (a->dtype == FX_F32) return h.vec ? run_sums<float, 4>(s, A) : run_sums<float, 1>(s, A);
-  return h.vec ? run_sums<bf16, 8>(s, A) : run_sums<bf16, 1>(s, A);
+  if (a->dtype == FX_F32) return h.vec ? run_sums<float, 4>(s, A, D->sms) : run_sums<float, 1>(s, A, D->sms);
+  return h.vec ? run_sums<bf16, 8>(s, A, D->sms) : run_sums<bf16, 1>(s, A, D->sms);
 }
 
 }  // extern "C"

@@ -33,44 +33,47 @@ struct EmbedFwd {
 
 constexpr int kEmbedRows = 4;  // rows a thread has on the way
 
+// A persistent grid: the next rows' tokens are read before this round's rows are.
 template <typename T, int E>
 __global__ void __launch_bounds__(kEmbedThreads) embed_fwd_kernel(EmbedFwd A) {
   using P = Pack<T, E>;
   const int rpb = kEmbedThreads / A.tpr, lane = threadIdx.x & (A.tpr - 1);
-  const int64_t r0 = (int64_t)blockIdx.x * (rpb * kEmbedRows) + threadIdx.x / A.tpr;
-  const P* src[kEmbedRows];
-  float other[kEmbedRows];  // what a row without a source holds
+  const int64_t step = (int64_t)gridDim.x * rpb * kEmbedRows;
+  int64_t r0 = (int64_t)blockIdx.x * (rpb * kEmbedRows) + threadIdx.x / A.tpr;
+  int64_t next[kEmbedRows];
 #pragma unroll
-  for (int u = 0; u < kEmbedRows; ++u) {
-    const int64_t r = r0 + (int64_t)u * rpb;
-    src[u] = nullptr;
-    other[u] = 0.f;
-    if (r < A.count) {
-      const int64_t t = A.tok.at(r);
-      if (A.tok.padded(t)) continue;
-      if (t >= 0 && t < A.rows) src[u] = reinterpret_cast<const P*>(static_cast<const T*>(A.weight) + t * A.width);
-      else other[u] = __int_as_float(0x7fc00000);
-    }
-  }
-  for (int c = lane; c < A.chunks; c += A.tpr) {
-    P v[kEmbedRows];
-#pragma unroll
-    for (int u = 0; u < kEmbedRows; ++u)
-      if (src[u]) v[u] = src[u][c];
+  for (int u = 0; u < kEmbedRows; ++u) next[u] = r0 + u * rpb < A.count ? A.tok.at(r0 + u * rpb) : 0;
+  for (; r0 < A.count; r0 += step) {
+    const P* src[kEmbedRows];
+    float other[kEmbedRows];  // what a row without a source holds
 #pragma unroll
     for (int u = 0; u < kEmbedRows; ++u) {
-      const int64_t r = r0 + (int64_t)u * rpb;
-      if (r >= A.count) break;
-      P o;
+      const int64_t t = next[u], r = r0 + step + u * rpb;
+      const bool ok = t >= 0 && t < A.rows && !A.tok.padded(t);
+      src[u] = ok ? reinterpret_cast<const P*>(static_cast<const T*>(A.weight) + t * A.width) : nullptr;
+      other[u] = A.tok.padded(t) ? 0.f : __int_as_float(0x7fc00000);
+      next[u] = r < A.count ? A.tok.at(r) : 0;
+    }
+    for (int c = lane; c < A.chunks; c += A.tpr) {
+      P v[kEmbedRows];
 #pragma unroll
-      for (int e = 0; e < E; ++e) o.e[e] = from_f<T>(src[u] ? to_f(v[u].e[e]) * A.scale : other[u]);
-      reinterpret_cast<P*>(static_cast<T*>(A.out) + r * A.width)[c] = o;
+      for (int u = 0; u < kEmbedRows; ++u)
+        if (src[u]) v[u] = src[u][c];
+#pragma unroll
+      for (int u = 0; u < kEmbedRows; ++u) {
+        const int64_t r = r0 + u * rpb;
+        if (r >= A.count) break;
+        P o;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o.e[e] = from_f<T>(src[u] ? to_f(v[u].e[e]) * A.scale : other[u]);
+        reinterpret_cast<P*>(static_cast<T*>(A.out) + r * A.width)[c] = o;
+      }
     }
   }
 }
 
 // ---------------------------------------------------------------- sort by token
-constexpr int kSortThreads = 256, kSortWarps = kSortThreads / 32, kSortRounds = 16;
+constexpr int kSortThreads = 256, kSortWarps = kSortThreads / 32, kSortRounds = 4;
 constexpr int kSortTile = kSortThreads * kSortRounds;  // tokens of a block
 constexpr int kSortBits = 11;
 
@@ -215,11 +218,11 @@ struct EmbedGrad {
   void* dweight;
   float* part;  // (windows, 2, chunks * E)
   int64_t rows, width;
-  int count, window, windows, chunks, tpr;
+  int count, window, windows, chunks, tpr, rpb;
   float scale;
 };
 
-constexpr int kEmbedAhead = 8;  // rows a thread has on the way
+constexpr int kEmbedAhead = 4;  // rows a thread has on the way
 
 template <typename T, int E>
 __device__ __forceinline__ void embed_write(const EmbedGrad& A, int64_t v, int c, const float (&acc)[E]) {
@@ -231,7 +234,7 @@ __device__ __forceinline__ void embed_write(const EmbedGrad& A, int64_t v, int c
 
 // A group of tpr threads sums the runs of one window, a piece of the columns a thread.
 template <typename T, int E>
-__global__ void __launch_bounds__(kEmbedThreads) embed_window_kernel(EmbedGrad A) {
+__global__ void __launch_bounds__(kEmbedThreads, 4) embed_window_kernel(EmbedGrad A) {
   using P = Pack<T, E>;
   const int w = blockIdx.x * (kEmbedThreads / A.tpr) + threadIdx.x / A.tpr;
   const int c = blockIdx.y * A.tpr + (threadIdx.x & (A.tpr - 1));
@@ -254,26 +257,36 @@ __global__ void __launch_bounds__(kEmbedThreads) embed_window_kernel(EmbedGrad A
       for (int e = 0; e < E; ++e) p[e] = acc[e];
     }
   };
-  for (int i = begin; i < end; i += kEmbedAhead) {
-    int key[kEmbedAhead];
-    P x[kEmbedAhead];
+  int key[kEmbedAhead], pos[kEmbedAhead];  // of the rows to come
+  const auto look = [&](int i) {
 #pragma unroll
     for (int u = 0; u < kEmbedAhead; ++u) {
       key[u] = i + u < end ? A.keys[i + u] : (int)A.rows;
-      if (key[u] < A.rows)
-        x[u] = reinterpret_cast<const P*>(static_cast<const T*>(A.grad) + (int64_t)A.pos[i + u] * A.width)[c];
+      pos[u] = i + u < end ? A.pos[i + u] : 0;
     }
+  };
+  look(begin);
+  const P* grad = reinterpret_cast<const P*>(A.grad) + c;
+  for (int i = begin; i < end; i += kEmbedAhead) {
+    P x[kEmbedAhead];
+    int now[kEmbedAhead];
+#pragma unroll
+    for (int u = 0; u < kEmbedAhead; ++u) {
+      now[u] = key[u];
+      if (now[u] < A.rows) x[u] = grad[(int64_t)pos[u] * A.chunks];
+    }
+    look(i + kEmbedAhead);
 #pragma unroll
     for (int u = 0; u < kEmbedAhead; ++u) {
       if (i + u >= end) break;
-      if (key[u] != cur) {
+      if (now[u] != cur) {
         leave(false);
-        cur = key[u];
+        cur = now[u];
         head = i + u == begin && cur == before;
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = 0.f;
       }
-      if (key[u] < A.rows) {
+      if (now[u] < A.rows) {
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] += to_f(x[u].e[e]);
       }
@@ -282,57 +295,61 @@ __global__ void __launch_bounds__(kEmbedThreads) embed_window_kernel(EmbedGrad A
   leave(cur == after);
 }
 
-// Rows without a token, and rows whose run crosses windows.
+// Rows without a token, and rows whose run crosses windows, whose parts are added in order: by a group of tpr
+// threads a row, or, where a row has `kFew` parts or more, by all groups of the block, each a run of them.
+// `rpb` rows a block at a time: as many as it has groups, or one, where the rows have many tokens.
 template <typename T, int E>
 __global__ void __launch_bounds__(kEmbedThreads) embed_join_kernel(EmbedGrad A) {
-  constexpr int kFew = 16;  // parts that one group adds
+  constexpr int kFew = 4;
   __shared__ float share[kEmbedThreads * E];
   const int groups = kEmbedThreads / A.tpr, g = threadIdx.x / A.tpr, lane = threadIdx.x & (A.tpr - 1);
-  const int64_t v0 = (int64_t)blockIdx.x * groups;
   const int c = blockIdx.y * A.tpr + lane;
   const int64_t line = (int64_t)A.chunks * E;
-  auto add = [&](float (&acc)[E], int first, int last, int step, int w0) {
-    for (int w = first; w <= last; w += step) {
-      const float* p = A.part + ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * line + (int64_t)c * E;
+  auto add = [&](float (&acc)[E], int first, int last, int w0) {
+#pragma unroll 4
+    for (int w = first; w <= last; ++w) {
+      const Pack<float, E> p = *reinterpret_cast<const Pack<float, E>*>(A.part + ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * line + (int64_t)c * E);
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += p[e];
+      for (int e = 0; e < E; ++e) acc[e] += p.e[e];
     }
   };
-  bool many = false;
-  if (v0 + g < A.rows) {
+  for (int64_t v0 = (int64_t)blockIdx.x * A.rpb; v0 < A.rows; v0 += (int64_t)gridDim.x * A.rpb) {
+    bool many = false;
     const int64_t v = v0 + g;
-    const int s = A.start[v], e = A.start[v + 1], w0 = s / A.window, w1 = (e - 1) / A.window;
-    float acc[E];
+    if (g < A.rpb && v < A.rows) {
+      const int s = A.start[v], e = A.start[v + 1], w0 = s / A.window, w1 = (e - 1) / A.window;
+      float acc[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) acc[i] = 0.f;
-    if (s == e) {
-      if (c < A.chunks) embed_write<T, E>(A, v, c, acc);
-    } else if (w1 > w0) {
-      many = w1 - w0 >= kFew;
-      if (!many && c < A.chunks) {
-        add(acc, w0, w1, 1, w0);
-        embed_write<T, E>(A, v, c, acc);
+      for (int i = 0; i < E; ++i) acc[i] = 0.f;
+      if (s == e) {
+        if (c < A.chunks) embed_write<T, E>(A, v, c, acc);
+      } else if (w1 > w0) {
+        many = groups > 1 && w1 - w0 >= kFew;
+        if (!many && c < A.chunks) {
+          add(acc, w0, w1, w0);
+          embed_write<T, E>(A, v, c, acc);
+        }
       }
     }
-  }
-  if (!__syncthreads_or(many)) return;
-  for (int k = 0; k < groups && v0 + k < A.rows; ++k) {  // the whole block on one row
-    const int64_t v = v0 + k;
-    const int s = A.start[v], e = A.start[v + 1], w0 = s / A.window, w1 = (e - 1) / A.window;
-    if (s == e || w1 - w0 < kFew) continue;
-    float acc[E];
+    if (groups == 1 || !__syncthreads_or(many)) continue;
+    for (int k = 0; k < A.rpb && v0 + k < A.rows; ++k) {  // the whole block on one row
+      const int s = A.start[v0 + k], e = A.start[v0 + k + 1], w0 = s / A.window, w1 = (e - 1) / A.window;
+      if (s == e || w1 - w0 < kFew) continue;
+      float acc[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) acc[i] = 0.f;
-    if (c < A.chunks) add(acc, w0 + g, w1, groups, w0);
-    __syncthreads();
+      for (int i = 0; i < E; ++i) acc[i] = 0.f;
+      const int per = (w1 - w0 + groups) / groups, first = w0 + g * per;
+      if (c < A.chunks) add(acc, first, min(first + per - 1, w1), w0);
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < E; ++i) share[i * kEmbedThreads + threadIdx.x] = acc[i];
-    __syncthreads();
-    if (g == 0 && c < A.chunks) {
-      for (int j = 1; j < groups; ++j)
+      for (int i = 0; i < E; ++i) share[i * kEmbedThreads + threadIdx.x] = acc[i];
+      __syncthreads();
+      if (g == 0 && c < A.chunks) {
+        for (int j = 1; j < groups; ++j)
 #pragma unroll
-        for (int i = 0; i < E; ++i) acc[i] += share[i * kEmbedThreads + j * A.tpr + lane];
-      embed_write<T, E>(A, v, c, acc);
+          for (int i = 0; i < E; ++i) acc[i] += share[i * kEmbedThreads + j * A.tpr + lane];
+        embed_write<T, E>(A, v0 + k, c, acc);
+      }
     }
   }
 }

@@ -26,6 +26,17 @@ _TOKEN_BYTES = {torch.int32: 4, torch.int64: 8, torch.int16: 2, torch.uint8: 1}
 _ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "tanh": 5}
 
 
+def _once(fn):
+    """As ``once_differentiable``, whose wrapping costs more than a small call's launches, only where a graph of the
+    gradients is asked for."""
+    guarded = once_differentiable(fn)
+
+    def backward(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+
+    return staticmethod(backward)
+
+
 # ------------------------------------------------------------------ checks
 def _tokens(tokens, like, name="tokens"):
     if not isinstance(tokens, torch.Tensor):
@@ -79,8 +90,7 @@ class _TokenEmbedding(torch.autograd.Function):
         ctx.table, ctx.rest = (weight.shape, weight.dtype), (scale, padding)
         return _embed_forward(tokens, weight, scale, padding)
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         tokens = ctx.saved_tensors[0].contiguous()
         grad = grad.contiguous()
@@ -150,8 +160,7 @@ class _FusedLinear(torch.autograd.Function):
         ctx.activation, ctx.bias = activation, bias is not None
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         x, weight, slope = ctx.saved_tensors
         wants_x, wants_weight, wants_bias, wants_residual, _ = ctx.needs_input_grad
@@ -262,8 +271,7 @@ class _TokenLogprobs(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return out
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_logp, grad_entropy, *_):
         if grad_logp is None and grad_entropy is None:
             return (None,) * 6

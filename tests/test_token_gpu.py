@@ -492,3 +492,14 @@ def test_a_model_of_all_three(dtype):
     assert abs(loss.item() - want.item()) <= tol * abs(want.item())
     for g, w in zip(grads, wgrads):
         assert (g.double() - w).norm() <= tol * w.norm()
+
+
+def test_second_derivatives_are_refused():
+    w = torch.randn(9, 8, device="cuda", requires_grad=True)
+    t = torch.randint(0, 9, (5,), device="cuda")
+    x = torch.randn(5, 8, device="cuda", requires_grad=True)
+    for out, leaf in ((fx.token_embedding(t, w), w), (fx.fused_linear(x, w, activation="silu"), x),
+                      (fx.token_logprobs(x, t.clamp(max=7))[0], x)):
+        (g,) = torch.autograd.grad((out * out).sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
