@@ -43,15 +43,15 @@ bool scans(const fx_embed_args* a) {
   return a->count <= kScanTokens && a->rows <= 16384 && a->rows * a->count <= (int64_t{1} << 22);
 }
 
-// Tokens of a window: as many as leave every thread slot of the device a window's columns.
-int window_of(const fx_embed_args* a, const Shape& s, int sms) {
-  int w = 128;
-  while (w > 16 && a->count / w * s.chunks < (int64_t)sms * 1024) w /= 2;
+// Tokens of a window (a power of two): as many as leave every thread slot of the device a window's columns.
+int shift_of(const fx_embed_args* a, const Shape& s, int sms) {
+  int w = 7;
+  while (w > 4 && (a->count >> w) * s.chunks < (int64_t)sms * 1024) --w;
   return w;
 }
 
 struct SortPlan {
-  int passes, bits, blocks, window, windows;
+  int passes, bits, blocks, shift, windows;
   size_t keys, hist, total, start, part, bytes;  // offsets
 };
 
@@ -62,8 +62,8 @@ SortPlan plan_of(const fx_embed_args* a, const Shape& s, int sms) {
   P.passes = (bits + kSortBits - 1) / kSortBits;
   P.bits = (bits + P.passes - 1) / P.passes;
   P.blocks = (int)((a->count + kSortTile - 1) / kSortTile);
-  P.window = window_of(a, s, sms);
-  P.windows = (int)((a->count + P.window - 1) / P.window);
+  P.shift = shift_of(a, s, sms);
+  P.windows = (int)((a->count + (1 << P.shift) - 1) >> P.shift);
   P.keys = 0;  // keys and places, two of each
   P.hist = align256((size_t)(P.passes > 1 ? 4 : 2) * a->count * sizeof(int));
   P.total = P.hist + align256(((size_t)P.blocks << P.bits) * sizeof(int));
@@ -74,9 +74,9 @@ SortPlan plan_of(const fx_embed_args* a, const Shape& s, int sms) {
 }
 
 template <typename T, int E>
-int run_fwd(cudaStream_t s, const EmbedFwd& A, int sms) {
-  const int64_t per = (int64_t)(kEmbedThreads / A.tpr) * kEmbedRows, blocks = (A.count + per - 1) / per, most = (int64_t)sms * 8;
-  embed_fwd_kernel<T, E><<<(unsigned)(blocks < most ? blocks : most), kEmbedThreads, 0, s>>>(A);
+int run_fwd(cudaStream_t s, const EmbedFwd& A) {
+  const int64_t per = 32 * (kEmbedThreads / 32) / (A.tpr > 32 ? A.tpr / 32 : 1);  // rows of a block
+  embed_fwd_kernel<T, E><<<(unsigned)((A.count + per - 1) / per), kEmbedThreads, 0, s>>>(A);
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
@@ -89,11 +89,12 @@ int run_scan(cudaStream_t s, const EmbedGrad& A, const Tokens& tok) {
 template <typename T, int E>
 int run_sums(cudaStream_t s, const EmbedGrad& A, int sms) {
   const int groups = kEmbedThreads / A.tpr;
-  const unsigned cols = (unsigned)((A.chunks + A.tpr - 1) / A.tpr);
-  const int64_t blocks = (A.rows + A.rpb - 1) / A.rpb, most = ((int64_t)sms * 8 + cols - 1) / cols;
-  const dim3 windows((A.windows + groups - 1) / groups, cols), rows((unsigned)(blocks < most ? blocks : most), cols);
+  const dim3 windows((A.windows + groups - 1) / groups, (unsigned)((A.chunks + A.tpr - 1) / A.tpr));
   embed_window_kernel<T, E><<<windows, kEmbedThreads, 0, s>>>(A);
-  embed_join_kernel<T, E><<<rows, kEmbedThreads, 0, s>>>(A);
+  // the join: a warp for every row of the table, a block for every window that a long run may begin in, as far as the
+  // device holds them
+  const int64_t blocks = (A.rows + 7) / 8, want = blocks > A.windows ? blocks : A.windows, most = (int64_t)sms * 4;
+  embed_join_kernel<T, E><<<(unsigned)(want < most ? want : most), kEmbedThreads, 0, s>>>(A);
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
@@ -104,26 +105,27 @@ int sort(cudaStream_t s, const fx_embed_args* a, const SortPlan& P, unsigned cha
   S.rows = a->rows;
   S.count = (int)a->count;
   S.blocks = P.blocks;
-  S.bits = P.bits;
   S.hist = reinterpret_cast<int*>(ws + P.hist);
   S.total = reinterpret_cast<int*>(ws + P.total);
   int* start = reinterpret_cast<int*>(ws + P.start);
-  const int digits = 1 << P.bits;
-  const size_t smem = (size_t)(kSortWarps + 1) * digits * sizeof(int);
-  if (raise_smem(sort_place_kernel, smem, (size_t)(kSortWarps + 1) * (sizeof(int) << kSortBits))) return FX_ERR_CUDA;
+  S.mask = (1 << P.bits) - 1;
+  S.digits = P.passes == 1 ? (int)a->rows + 1 : 1 << P.bits;
+  constexpr size_t each = sizeof(int) + kSortWarps * sizeof(uint16_t);  // a digit's
+  const size_t smem = (size_t)(S.digits + 1) * each;
+  if (raise_smem(sort_place_kernel, smem, each << (kSortBits + 1))) return FX_ERR_CUDA;
   for (int p = 0; p < P.passes; ++p) {
     S.keys_out = lists + (size_t)(p & 1) * 2 * a->count;
     S.pos_out = S.keys_out + a->count;
     S.shift = p * P.bits;
     S.start = P.passes == 1 ? start : nullptr;
-    sort_count_kernel<<<P.blocks, kSortThreads, digits * sizeof(int), s>>>(S);
-    sort_scan_kernel<<<(digits + 7) / 8, 256, 0, s>>>(S);
+    sort_count_kernel<<<P.blocks, kSortThreads, S.digits * sizeof(int), s>>>(S);
+    sort_scan_kernel<<<(S.digits + 7) / 8, 256, 0, s>>>(S);
     sort_place_kernel<<<P.blocks, kSortThreads, smem, s>>>(S);
     S.keys = S.keys_out;
     S.pos = S.pos_out;
   }
   if (P.passes > 1)
-    sort_start_kernel<<<(unsigned)((a->rows + 256) / 256), 256, 0, s>>>(S.keys, S.count, start, a->rows);
+    sort_start_kernel<<<(unsigned)((a->count + 256) / 256), 256, 0, s>>>(S.keys, S.count, start, (int)a->rows);
   A.keys = S.keys;
   A.pos = S.pos;
   A.start = start;
@@ -139,13 +141,11 @@ int fermix_token_embedding(void* stream, const fx_embed_args* a) {
   if (e) return e;
   if (a->count == 0) return FX_OK;
   if (!a->tokens || !a->weight || !a->out) return FX_ERR_NULL;
-  const DevInfo* D = dev_info();
-  if (!D) return FX_ERR_DEVICE;
   const Shape h = shape_of(a, a->weight, a->out);
   EmbedFwd A{tokens_of(a), a->weight, a->out, a->count, a->rows, a->width, h.chunks, h.tpr, a->scale};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a->dtype == FX_F32) return h.vec ? run_fwd<float, 4>(s, A, D->sms) : run_fwd<float, 1>(s, A, D->sms);
-  return h.vec ? run_fwd<bf16, 8>(s, A, D->sms) : run_fwd<bf16, 1>(s, A, D->sms);
+  if (a->dtype == FX_F32) return h.vec ? run_fwd<float, 4>(s, A) : run_fwd<float, 1>(s, A);
+  return h.vec ? run_fwd<bf16, 8>(s, A) : run_fwd<bf16, 1>(s, A);
 }
 
 // Without the pointers the larger of the two forms counts: entry by entry, fewer windows never
@@ -186,9 +186,8 @@ int fermix_token_embedding_grad(void* stream, const fx_embed_args* a, void* ws, 
   const SortPlan P = plan_of(a, h, D->sms);
   if (!ws || wsb < P.bytes + 256) return FX_ERR_WORKSPACE;
   unsigned char* base = reinterpret_cast<unsigned char*>(align256(reinterpret_cast<uintptr_t>(ws)));
-  A.window = P.window;
+  A.shift = P.shift;
   A.windows = P.windows;
-  A.rpb = a->count / a->rows >= 2 * P.window ? 1 : kEmbedThreads / h.tpr;
   A.part = reinterpret_cast<float*>(base + P.part);
   const int st = sort(s, a, P, base, A);
   if (st) return st;

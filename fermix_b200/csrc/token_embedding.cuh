@@ -31,64 +31,68 @@ struct EmbedFwd {
   float scale;
 };
 
-constexpr int kEmbedRows = 4;  // rows a thread has on the way
+// A warp takes 32 rows at a time, whose tokens its lanes look up, one each (a token's row for every lane of a row
+// took as many instructions as the rest). tpr <= 32: 32 / tpr rows at a time; above that tpr / 32 warps share the rows.
+constexpr int kEmbedAhead = 4;  // rows a thread has on the way
 
-// A persistent grid: the next rows' tokens are read before this round's rows are.
 template <typename T, int E>
 __global__ void __launch_bounds__(kEmbedThreads) embed_fwd_kernel(EmbedFwd A) {
   using P = Pack<T, E>;
-  const int rpb = kEmbedThreads / A.tpr, lane = threadIdx.x & (A.tpr - 1);
-  const int64_t step = (int64_t)gridDim.x * rpb * kEmbedRows;
-  int64_t r0 = (int64_t)blockIdx.x * (rpb * kEmbedRows) + threadIdx.x / A.tpr;
-  int64_t next[kEmbedRows];
+  const int lane = threadIdx.x & 31, wpr = A.tpr > 32 ? A.tpr / 32 : 1, lpr = A.tpr < 32 ? A.tpr : 32;
+  const int warp = threadIdx.x >> 5, c0 = (warp % wpr) * 32 + lane % lpr, rows = 32 / lpr, sub = lane / lpr;
+  const int64_t per = kEmbedThreads / 32 / wpr, r0 = ((int64_t)blockIdx.x * per + warp / wpr) * 32;
+  int mine = -1;  // the row of token r0 + lane; -1: zeros, -2: none
+  if (r0 + lane < A.count) {
+    const int64_t t = A.tok.at(r0 + lane);
+    mine = A.tok.padded(t) ? -1 : t >= 0 && t < A.rows ? (int)t : -2;
+  }
+  const int n = (int)(A.count - r0 < 32 ? A.count - r0 : 32);
+  for (int c = c0; c - lane % lpr < A.chunks; c += A.tpr) {
+    const P* in = static_cast<const P*>(A.weight) + c;
+    P* out = static_cast<P*>(A.out) + (r0 + sub) * A.chunks + c;
+    const int64_t step = (int64_t)rows * A.chunks;
+    for (int k = 0; k < 32; k += kEmbedAhead * rows) {
+      P v[kEmbedAhead];
+      int row[kEmbedAhead];
 #pragma unroll
-  for (int u = 0; u < kEmbedRows; ++u) next[u] = r0 + u * rpb < A.count ? A.tok.at(r0 + u * rpb) : 0;
-  for (; r0 < A.count; r0 += step) {
-    const P* src[kEmbedRows];
-    float other[kEmbedRows];  // what a row without a source holds
+      for (int u = 0; u < kEmbedAhead; ++u) {
+        row[u] = __shfl_sync(0xffffffffu, mine, (k + u * rows + sub) & 31);
+        if (row[u] >= 0 && k + u * rows + sub < n && c < A.chunks) v[u] = in[(int64_t)row[u] * A.chunks];
+      }
 #pragma unroll
-    for (int u = 0; u < kEmbedRows; ++u) {
-      const int64_t t = next[u], r = r0 + step + u * rpb;
-      const bool ok = t >= 0 && t < A.rows && !A.tok.padded(t);
-      src[u] = ok ? reinterpret_cast<const P*>(static_cast<const T*>(A.weight) + t * A.width) : nullptr;
-      other[u] = A.tok.padded(t) ? 0.f : __int_as_float(0x7fc00000);
-      next[u] = r < A.count ? A.tok.at(r) : 0;
-    }
-    for (int c = lane; c < A.chunks; c += A.tpr) {
-      P v[kEmbedRows];
-#pragma unroll
-      for (int u = 0; u < kEmbedRows; ++u)
-        if (src[u]) v[u] = src[u][c];
-#pragma unroll
-      for (int u = 0; u < kEmbedRows; ++u) {
-        const int64_t r = r0 + u * rpb;
-        if (r >= A.count) break;
+      for (int u = 0; u < kEmbedAhead; ++u, out += step) {
+        if (k + u * rows + sub >= n || c >= A.chunks) continue;
         P o;
+        if (row[u] >= 0) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) o.e[e] = from_f<T>(src[u] ? to_f(v[u].e[e]) * A.scale : other[u]);
-        reinterpret_cast<P*>(static_cast<T*>(A.out) + r * A.width)[c] = o;
+          for (int e = 0; e < E; ++e) o.e[e] = from_f<T>(to_f(v[u].e[e]) * A.scale);
+        } else {
+#pragma unroll
+          for (int e = 0; e < E; ++e) o.e[e] = from_f<T>(row[u] == -1 ? 0.f : __int_as_float(0x7fc00000));
+        }
+        *out = o;
       }
     }
   }
 }
 
 // ---------------------------------------------------------------- sort by token
-constexpr int kSortThreads = 256, kSortWarps = kSortThreads / 32, kSortRounds = 4;
+constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32, kSortRounds = 4;
 constexpr int kSortTile = kSortThreads * kSortRounds;  // tokens of a block
 constexpr int kSortBits = 11;
 
 struct SortArgs {
-  Tokens tok;           // first pass
+  Tokens tok;             // first pass
   const int *keys, *pos;  // later passes
   int *keys_out, *pos_out;
   int* hist;    // (digits, blocks)
   int* total;   // (digits)
   int* start;   // one pass only: first place of each token, (rows + 1)
   int64_t rows;
-  int count, blocks, shift, bits;
+  int count, blocks, shift, digits;  // digits: that occur
+  int mask;
 };
 
-// Token (or key) e = warp's first + 32 round + lane, and its digit; -1 behind the last.
 __device__ __forceinline__ void sort_load(const SortArgs& A, int (&key)[kSortRounds], int base) {
 #pragma unroll
   for (int i = 0; i < kSortRounds; ++i) {
@@ -96,28 +100,29 @@ __device__ __forceinline__ void sort_load(const SortArgs& A, int (&key)[kSortRou
     key[i] = e >= A.count ? -1 : A.keys ? A.keys[e] : A.tok.key(e, A.rows);
   }
 }
+__device__ __forceinline__ int sort_digit(const SortArgs& A, int key) { return key < 0 ? -1 : (key >> A.shift) & A.mask; }
 
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortArgs A) {
   extern __shared__ int hist[];
-  const int digits = 1 << A.bits, lane = threadIdx.x & 31;
-  for (int d = threadIdx.x; d < digits; d += kSortThreads) hist[d] = 0;
-  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  for (int d = threadIdx.x; d < A.digits; d += kSortThreads) hist[d] = 0;
   int key[kSortRounds];
   sort_load(A, key, blockIdx.x * kSortTile + (threadIdx.x >> 5) * (32 * kSortRounds) + lane);
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < kSortRounds; ++i) {
-    const int d = key[i] < 0 ? -1 : (key[i] >> A.shift) & (digits - 1);
+    const int d = sort_digit(A, key[i]);
     const unsigned same = __match_any_sync(0xffffffffu, d);  // one addition for equal digits
     if (d >= 0 && lane == __ffs(same) - 1) atomicAdd(&hist[d], __popc(same));
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < digits; d += kSortThreads) A.hist[(int64_t)d * A.blocks + blockIdx.x] = hist[d];
+  for (int d = threadIdx.x; d < A.digits; d += kSortThreads) A.hist[(int64_t)d * A.blocks + blockIdx.x] = hist[d];
 }
 
 // Counts of a digit -> first place within the digit for each block; a warp a digit.
 __global__ void __launch_bounds__(256) sort_scan_kernel(SortArgs A) {
   const int d = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (d >= 1 << A.bits) return;
+  if (d >= A.digits) return;
   int* h = A.hist + (int64_t)d * A.blocks;
   int sum = 0;
   for (int b = 0; b < A.blocks; b += 32) {
@@ -134,16 +139,21 @@ __global__ void __launch_bounds__(256) sort_scan_kernel(SortArgs A) {
   if (lane == 0) A.total[d] = sum;
 }
 
+// Every token to its place: the digit's first, those of earlier blocks, of the block's earlier warps, of the warp's
+// earlier rounds and lanes.
 __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortArgs A) {
-  extern __shared__ int at[];  // (warps, digits), then the digits' first places
+  extern __shared__ int first[];  // (digits), then 16-bit counts (warps, digits)
   __shared__ int sums[kSortWarps];
-  const int digits = 1 << A.bits, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int* first = at + kSortWarps * digits;
-  for (int i = threadIdx.x; i < kSortWarps * digits; i += kSortThreads) at[i] = 0;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, wide = (A.digits + 1) / 2 * 2;
+  uint16_t* at = reinterpret_cast<uint16_t*>(first + wide);
+  for (int i = threadIdx.x; i < kSortWarps * wide / 2; i += kSortThreads) reinterpret_cast<int*>(at)[i] = 0;
+  int key[kSortRounds];
+  const int base = blockIdx.x * kSortTile + w * (32 * kSortRounds) + lane;
+  sort_load(A, key, base);
   // first places of the digits: a thread sums a run of them
-  const int per = (digits + kSortThreads - 1) / kSortThreads, d0 = threadIdx.x * per;
+  const int per = (A.digits + kSortThreads - 1) / kSortThreads, d0 = threadIdx.x * per;
   int own = 0;
-  for (int d = d0; d < d0 + per && d < digits; ++d) own += A.total[d];
+  for (int d = d0; d < d0 + per && d < A.digits; ++d) own += A.total[d];
   int s = own;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -154,41 +164,38 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortArgs A) {
   __syncthreads();
   int run = s - own;
   for (int i = 0; i < w; ++i) run += sums[i];
-  for (int d = d0; d < d0 + per && d < digits; ++d) {
-    first[d] = run;
+  for (int d = d0; d < d0 + per && d < A.digits; ++d) {
+    first[d] = run + A.hist[(int64_t)d * A.blocks + blockIdx.x];
     if (A.start && blockIdx.x == 0 && d <= A.rows) A.start[d] = run;
     run += A.total[d];
   }
   // each warp counts its own tokens
-  int key[kSortRounds];
-  const int base = blockIdx.x * kSortTile + w * (32 * kSortRounds) + lane;
-  sort_load(A, key, base);
-  int* mine = at + w * digits;
+  uint16_t* mine = at + w * wide;
 #pragma unroll
   for (int i = 0; i < kSortRounds; ++i) {
-    const int d = key[i] < 0 ? -1 : (key[i] >> A.shift) & (digits - 1);
+    const int d = sort_digit(A, key[i]);
     const unsigned same = __match_any_sync(0xffffffffu, d);
-    if (d >= 0 && lane == __ffs(same) - 1) mine[d] += __popc(same);
+    if (d >= 0 && lane == __ffs(same) - 1) mine[d] += (uint16_t)__popc(same);
     __syncwarp();
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < digits; d += kSortThreads) {
-    int p = first[d] + A.hist[(int64_t)d * A.blocks + blockIdx.x];
+  for (int d = threadIdx.x; d < A.digits; d += kSortThreads) {
+    int p = 0;
     for (int i = 0; i < kSortWarps; ++i) {
-      const int n = at[i * digits + d];
-      at[i * digits + d] = p;
+      const int n = at[i * wide + d];
+      at[i * wide + d] = (uint16_t)p;
       p += n;
     }
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kSortRounds; ++i) {
-    const int d = key[i] < 0 ? -1 : (key[i] >> A.shift) & (digits - 1);
+    const int d = sort_digit(A, key[i]);
     const unsigned same = __match_any_sync(0xffffffffu, d);
     int p = 0;
-    if (d >= 0) p = mine[d] + __popc(same & ((1u << lane) - 1));
+    if (d >= 0) p = first[d] + mine[d] + __popc(same & ((1u << lane) - 1));
     __syncwarp();
-    if (d >= 0 && lane == __ffs(same) - 1) mine[d] += __popc(same);
+    if (d >= 0 && lane == __ffs(same) - 1) mine[d] += (uint16_t)__popc(same);
     __syncwarp();
     if (d >= 0) {
       const int e = base + 32 * i;
@@ -198,17 +205,19 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortArgs A) {
   }
 }
 
-// start[v]: the first place of a token >= v in the sorted list.
-__global__ void sort_start_kernel(const int* keys, int count, int* start, int64_t rows) {
-  const int64_t v = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (v > rows) return;
-  int lo = 0, hi = count;
-  while (lo < hi) {
-    const int mid = lo + ((hi - lo) >> 1);
-    if (keys[mid] < v) lo = mid + 1;
-    else hi = mid;
+// start[v]: the first place of a token >= v in the sorted list; a warp 32 places, each fills the tokens
+// between its own and the one before.
+__global__ void __launch_bounds__(256) sort_start_kernel(const int* keys, int count, int* start, int rows) {
+  const int lane = threadIdx.x & 31;
+  const int64_t base = ((int64_t)blockIdx.x * 256 + threadIdx.x) - lane, i = base + lane;
+  const int to = i < count ? keys[i] : rows, from = i == 0 ? -1 : i <= count ? keys[i - 1] : rows;
+  unsigned steps = __ballot_sync(0xffffffffu, i <= count && to > from);
+  while (steps) {
+    const int src = __ffs(steps) - 1;
+    steps &= steps - 1;
+    const int a = __shfl_sync(0xffffffffu, from, src), b = __shfl_sync(0xffffffffu, to, src);
+    for (int64_t v = (int64_t)a + 1 + lane; v <= b; v += 32) start[v] = (int)(base + src);
   }
-  start[v] = lo;
 }
 
 // ---------------------------------------------------------------- gradient
@@ -218,11 +227,9 @@ struct EmbedGrad {
   void* dweight;
   float* part;  // (windows, 2, chunks * E)
   int64_t rows, width;
-  int count, window, windows, chunks, tpr, rpb;
+  int count, shift, windows, chunks, tpr;  // windows of 1 << shift tokens
   float scale;
 };
-
-constexpr int kEmbedAhead = 4;  // rows a thread has on the way
 
 template <typename T, int E>
 __device__ __forceinline__ void embed_write(const EmbedGrad& A, int64_t v, int c, const float (&acc)[E]) {
@@ -234,12 +241,12 @@ __device__ __forceinline__ void embed_write(const EmbedGrad& A, int64_t v, int c
 
 // A group of tpr threads sums the runs of one window, a piece of the columns a thread.
 template <typename T, int E>
-__global__ void __launch_bounds__(kEmbedThreads, 4) embed_window_kernel(EmbedGrad A) {
+__global__ void __launch_bounds__(kEmbedThreads, E > 4 ? 3 : 4) embed_window_kernel(EmbedGrad A) {
   using P = Pack<T, E>;
   const int w = blockIdx.x * (kEmbedThreads / A.tpr) + threadIdx.x / A.tpr;
   const int c = blockIdx.y * A.tpr + (threadIdx.x & (A.tpr - 1));
   if (w >= A.windows || c >= A.chunks) return;
-  const int begin = w * A.window, end = min(begin + A.window, A.count);
+  const int begin = w << A.shift, end = min(begin + (1 << A.shift), A.count);
   const int before = begin > 0 ? A.keys[begin - 1] : -1;
   const int after = end < A.count ? A.keys[end] : -1;
   float acc[E];
@@ -295,60 +302,84 @@ __global__ void __launch_bounds__(kEmbedThreads, 4) embed_window_kernel(EmbedGra
   leave(cur == after);
 }
 
-// Rows without a token, and rows whose run crosses windows, whose parts are added in order: by a group of tpr
-// threads a row, or, where a row has `kFew` parts or more, by all groups of the block, each a run of them.
-// `rpb` rows a block at a time: as many as it has groups, or one, where the rows have many tokens.
+// Rows without a token, and rows whose run crosses windows, whose parts are added in order: up to kFew of them by a
+// warp a row, which looks 32 rows up at a time; longer runs by a block, whose groups of tpr threads have a stretch of
+// the windows each.
 template <typename T, int E>
 __global__ void __launch_bounds__(kEmbedThreads) embed_join_kernel(EmbedGrad A) {
   constexpr int kFew = 4;
   __shared__ float share[kEmbedThreads * E];
-  const int groups = kEmbedThreads / A.tpr, g = threadIdx.x / A.tpr, lane = threadIdx.x & (A.tpr - 1);
-  const int c = blockIdx.y * A.tpr + lane;
+  const int lane = threadIdx.x & 31, last_token = (int)A.rows;
   const int64_t line = (int64_t)A.chunks * E;
-  auto add = [&](float (&acc)[E], int first, int last, int w0) {
-#pragma unroll 4
-    for (int w = first; w <= last; ++w) {
-      const Pack<float, E> p = *reinterpret_cast<const Pack<float, E>*>(A.part + ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * line + (int64_t)c * E);
+  float acc[E];
+  // acc = the parts of the run that begins in window w0, those of windows [first, last], of piece c
+  auto add = [&](int c, int first, int last, int w0) {
+    constexpr int kAhead = E > 4 ? 4 : 8;
+    const float* part = A.part + (int64_t)c * E;
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += p.e[e];
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int w = first; w <= last; w += kAhead) {
+      Pack<float, E> p[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (w + u <= last) p[u] = *reinterpret_cast<const Pack<float, E>*>(part + ((int64_t)(w + u) * 2 + (w + u == w0 ? 1 : 0)) * line);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (w + u <= last) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] += p[u].e[e];
+        }
     }
   };
-  for (int64_t v0 = (int64_t)blockIdx.x * A.rpb; v0 < A.rows; v0 += (int64_t)gridDim.x * A.rpb) {
-    bool many = false;
-    const int64_t v = v0 + g;
-    if (g < A.rpb && v < A.rows) {
-      const int s = A.start[v], e = A.start[v + 1], w0 = s / A.window, w1 = (e - 1) / A.window;
-      float acc[E];
+  // The runs of more windows: a lane looks at one window each, whether the run that goes on behind it began in it.
+  for (int64_t base = blockIdx.x; base < A.windows; base += (int64_t)32 * gridDim.x) {
+    const int64_t mine = base + (int64_t)lane * gridDim.x, place = (mine + 1) << A.shift;
+    int row = mine < A.windows && place < A.count ? A.keys[place] : last_token, end = 0;
+    if (row < A.rows) {
+      end = (A.start[row + 1] - 1) >> A.shift;
+      if (A.start[row] >> A.shift != mine || end - mine < kFew) row = last_token;
+    }
+    unsigned found = __ballot_sync(0xffffffffu, row < A.rows);  // the same in every warp
+    while (found) {
+      const int src = __ffs(found) - 1, groups = kEmbedThreads / A.tpr, g = threadIdx.x / A.tpr;
+      found &= found - 1;
+      const int w = (int)(base + (int64_t)src * gridDim.x), w1 = __shfl_sync(0xffffffffu, end, src);
+      const int v = __shfl_sync(0xffffffffu, row, src);
+      const int per = (w1 - w + groups) / groups, first = w + g * per;
+      for (int c0 = 0; c0 < A.chunks; c0 += A.tpr) {
+        const int c = c0 + (threadIdx.x & (A.tpr - 1));
+        if (c < A.chunks) add(c, first, min(first + per - 1, w1), w);
+        __syncthreads();
 #pragma unroll
-      for (int i = 0; i < E; ++i) acc[i] = 0.f;
-      if (s == e) {
-        if (c < A.chunks) embed_write<T, E>(A, v, c, acc);
-      } else if (w1 > w0) {
-        many = groups > 1 && w1 - w0 >= kFew;
-        if (!many && c < A.chunks) {
-          add(acc, w0, w1, w0);
+        for (int i = 0; i < E; ++i) share[i * kEmbedThreads + threadIdx.x] = acc[i];
+        __syncthreads();
+        if (g == 0 && c < A.chunks) {
+          for (int j = 1; j < groups; ++j)
+#pragma unroll
+            for (int i = 0; i < E; ++i) acc[i] += share[i * kEmbedThreads + j * A.tpr + threadIdx.x];
           embed_write<T, E>(A, v, c, acc);
         }
       }
     }
-    if (groups == 1 || !__syncthreads_or(many)) continue;
-    for (int k = 0; k < A.rpb && v0 + k < A.rows; ++k) {  // the whole block on one row
-      const int s = A.start[v0 + k], e = A.start[v0 + k + 1], w0 = s / A.window, w1 = (e - 1) / A.window;
-      if (s == e || w1 - w0 < kFew) continue;
-      float acc[E];
+  }
+  // a warp's rows are far from each other: the frequent tokens, whose rows cross, often are not
+  const int64_t warps = (int64_t)gridDim.x * (kEmbedThreads / 32);
+  for (int64_t base = (int64_t)blockIdx.x * (kEmbedThreads / 32) + (threadIdx.x >> 5); base < A.rows; base += warps * 32) {
+    const int64_t mine = base + lane * warps;
+    const bool in = mine < A.rows;
+    const int s = in ? A.start[mine] : 0, e = in ? A.start[mine + 1] : 0;
+    const int w0 = s >> A.shift, w1 = (e - 1) >> A.shift;
+    unsigned empty = __ballot_sync(0xffffffffu, in && s == e);
+    unsigned cross = __ballot_sync(0xffffffffu, in && s < e && w1 > w0 && w1 - w0 < kFew);
 #pragma unroll
-      for (int i = 0; i < E; ++i) acc[i] = 0.f;
-      const int per = (w1 - w0 + groups) / groups, first = w0 + g * per;
-      if (c < A.chunks) add(acc, first, min(first + per - 1, w1), w0);
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < E; ++i) share[i * kEmbedThreads + threadIdx.x] = acc[i];
-      __syncthreads();
-      if (g == 0 && c < A.chunks) {
-        for (int j = 1; j < groups; ++j)
-#pragma unroll
-          for (int i = 0; i < E; ++i) acc[i] += share[i * kEmbedThreads + j * A.tpr + lane];
-        embed_write<T, E>(A, v0 + k, c, acc);
+    for (int i = 0; i < E; ++i) acc[i] = 0.f;
+    for (; empty; empty &= empty - 1)
+      for (int c = lane; c < A.chunks; c += 32) embed_write<T, E>(A, base + (__ffs(empty) - 1) * warps, c, acc);
+    for (; cross; cross &= cross - 1) {
+      const int src = __ffs(cross) - 1, a = __shfl_sync(0xffffffffu, w0, src), b = __shfl_sync(0xffffffffu, w1, src);
+      for (int c = lane; c < A.chunks; c += 32) {
+        add(c, a, b, a);
+        embed_write<T, E>(A, base + src * warps, c, acc);
       }
     }
   }
