@@ -16,23 +16,14 @@ int check(const fx_logprobs_args* a) {
   return FX_OK;
 }
 
-// Rows of whole 16-byte pieces on 16-byte boundaries (the mask's as many entries).
-int entries_of(const fx_logprobs_args* a) {
-  const int64_t size = a->dtype == FX_F32 ? 4 : 2, E = 16 / size;
-  const uintptr_t m = (uintptr_t)(a->entries * size) | (uintptr_t)(a->rows > 1 ? a->logits_stride * size : 0) |
-                      reinterpret_cast<uintptr_t>(a->logits) | reinterpret_cast<uintptr_t>(a->dlogits);
-  if (m % 16) return 1;
-  if (a->mask && ((uintptr_t)(a->rows > 1 ? a->mask_stride : 0) | reinterpret_cast<uintptr_t>(a->mask)) % E) return 1;
-  return (int)E;
-}
+constexpr int64_t kWarpRow = 1024;  // entries of a row that a warp takes
 
-// Parts of a row: enough to give every SM six blocks, of 8192 entries at least.
+// Parts of a row, in 16-byte pieces: enough to give every SM eight blocks, of 4096 entries at least.
 void split(const fx_logprobs_args* a, int sms, int& parts, int& per) {
-  const int64_t step = kProbThreads * 8, want = (6 * (int64_t)sms + a->rows - 1) / a->rows;
-  int64_t most = (a->entries + 8191) / 8192;
-  parts = (int)(want < most ? want : most);
-  per = (int)(((a->entries + parts - 1) / parts + step - 1) / step * step);
-  parts = (int)((a->entries + per - 1) / per);
+  const int64_t E = a->dtype == FX_F32 ? 4 : 8, pieces = a->entries / E + 2, want = (8 * (int64_t)sms + a->rows - 1) / a->rows;
+  const int64_t most = (a->entries + 4095) / 4096, n = a->entries <= kWarpRow ? 1 : want < most ? want : most;
+  per = (int)(((pieces + n - 1) / n + kProbThreads - 1) / kProbThreads * kProbThreads);
+  parts = (int)((pieces + per - 1) / per);
 }
 
 ProbArgs make(const fx_logprobs_args* a) {
@@ -57,21 +48,28 @@ ProbArgs make(const fx_logprobs_args* a) {
   return A;
 }
 
-template <typename T, int E>
+template <typename T, bool TOP>
 int run(cudaStream_t s, const ProbArgs& A) {
-  const int64_t blocks = A.rows * A.parts;
-  if (blocks > INT32_MAX) return FX_ERR_SHAPE;
-  if (A.top) prob_kernel<T, E, true><<<(unsigned)blocks, kProbThreads, 0, s>>>(A);
-  else prob_kernel<T, E, false><<<(unsigned)blocks, kProbThreads, 0, s>>>(A);
-  if (A.parts > 1) prob_join_kernel<T><<<(unsigned)((A.rows + 3) / 4), 128, 0, s>>>(A);
+  if (A.entries <= kWarpRow) {
+    prob_kernel<T, TOP, 1><<<(unsigned)((A.rows + kProbWarps - 1) / kProbWarps), kProbThreads, 0, s>>>(A);
+  } else {
+    const int64_t blocks = A.rows * A.parts;
+    if (blocks > INT32_MAX) return FX_ERR_SHAPE;
+    prob_kernel<T, TOP, kProbWarps><<<(unsigned)blocks, kProbThreads, 0, s>>>(A);
+    if (A.parts > 1) prob_join_kernel<T, TOP><<<(unsigned)A.rows, kProbThreads, 0, s>>>(A);
+  }
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
-template <typename T, int E>
+template <typename T>
 int run_grad(cudaStream_t s, const ProbArgs& A) {
-  const int64_t blocks = A.rows * A.parts;
-  if (blocks > INT32_MAX) return FX_ERR_SHAPE;
-  prob_grad_kernel<T, E><<<(unsigned)blocks, kProbThreads, 0, s>>>(A);
+  if (A.entries <= kWarpRow) {
+    prob_grad_kernel<T, 1><<<(unsigned)((A.rows + kProbWarps - 1) / kProbWarps), kProbThreads, 0, s>>>(A);
+  } else {
+    const int64_t blocks = A.rows * A.parts;
+    if (blocks > INT32_MAX) return FX_ERR_SHAPE;
+    prob_grad_kernel<T, kProbWarps><<<(unsigned)blocks, kProbThreads, 0, s>>>(A);
+  }
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
@@ -110,9 +108,8 @@ int fermix_token_logprobs(void* stream, const fx_logprobs_args* a, void* ws, siz
                                          align256((size_t)a->rows * A.parts * sizeof(float4)));
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int E = entries_of(a);
-  if (a->dtype == FX_F32) return E > 1 ? run<float, 4>(s, A) : run<float, 1>(s, A);
-  return E > 1 ? run<bf16, 8>(s, A) : run<bf16, 1>(s, A);
+  if (a->dtype == FX_F32) return a->top ? run<float, true>(s, A) : run<float, false>(s, A);
+  return a->top ? run<bf16, true>(s, A) : run<bf16, false>(s, A);
 }
 
 int fermix_token_logprobs_grad(void* stream, const fx_logprobs_args* a) {
@@ -125,9 +122,7 @@ int fermix_token_logprobs_grad(void* stream, const fx_logprobs_args* a) {
   ProbArgs A = make(a);
   split(a, D->sms, A.parts, A.per);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int E = entries_of(a);
-  if (a->dtype == FX_F32) return E > 1 ? run_grad<float, 4>(s, A) : run_grad<float, 1>(s, A);
-  return E > 1 ? run_grad<bf16, 8>(s, A) : run_grad<bf16, 1>(s, A);
+  return a->dtype == FX_F32 ? run_grad<float>(s, A) : run_grad<bf16>(s, A);
 }
 
 }  // extern "C"

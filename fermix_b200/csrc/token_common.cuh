@@ -5,6 +5,27 @@
 
 namespace fx {
 
+// The entries of a pack as float32; bfloat16 by words, an instruction an entry.
+template <int N>
+__device__ __forceinline__ void unpack(const Pack<float, N>& p, float* x) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) x[e] = p.e[e];
+}
+template <int N>
+__device__ __forceinline__ void unpack(const Pack<bf16, N>& p, float* x) {
+  if constexpr (N % 2) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = to_f(p.e[e]);
+  } else {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&p);
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      x[e] = __uint_as_float(w[e / 2] << 16);
+      x[e + 1] = __uint_as_float(w[e / 2] & 0xffff0000u);
+    }
+  }
+}
+
 struct Tokens {
   const void* p;
   int bytes, has_padding;

@@ -1,20 +1,26 @@
 // Log probabilities of given tokens under softmax(scale logits), with entropy and the likeliest
 // entries, and their gradient.
 //
-// One pass over a row keeps the running maximum m, S = sum of exp(scale (x - m)) and
-// W = sum of exp(scale (x - m)) (x - m); then with L = log S
-//   log p_t = scale (x_t - m) - L,   entropy = L - scale W / S.
-// The likeliest entries are kept by each warp, one a lane in descending order; an entry that
-// passes the last of them is inserted, which becomes rare after the first few hundred.
-// Bound by HBM where rows are many or long. A block takes a row, or a part of one where the
-// rows do not fill the device; parts are joined in order by a second kernel.
+// One pass over a row keeps a reference m near its maximum, S = sum of exp(scale (x - m)) and
+// W = sum of exp(scale (x - m)) log2(the same); then with L = log S
+//   log p_t = scale (x_t - m) - L,   entropy = L - W / (S log2 e).
+// A lane's reference moves when an entry is 2^kRise above it, not with every new maximum: in a row of 16 pieces a lane some
+// lane of a warp has one at every piece.
+// A lane takes a 16-byte piece at a time, on its boundary wherever the row begins, through a ring of asynchronous copies
+// of its own, four pieces deep: bytes on the way cost no registers (with two pieces ahead in registers, which halved the
+// threads, 8191 x 32000 bfloat16 took 197 us, with one and no ring 154). The likeliest entries are kept by each
+// warp, one a lane in descending order: of the pieces at hand the largest entries are taken one by one (a warp-wide
+// maximum each) while they pass the last of the list, which few do after the first; lists are joined by sorting networks.
+// Bound by HBM where rows are many or long, close to the rate of the exponentials (16 a cycle and SM). A warp takes a row
+// of up to 1024 entries, a block a longer one, or a part of it where the rows do not fill the device; parts are joined in
+// order by a second kernel.
 #pragma once
 #include "token_common.cuh"
 
 namespace fx {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kProbThreads = 256, kProbWarps = kProbThreads / 32;
+constexpr int kProbThreads = 128, kProbWarps = kProbThreads / 32;
 
 struct ProbArgs {
   Tokens tok;
@@ -28,7 +34,7 @@ struct ProbArgs {
   float4* part;
   int2* part_top;
   int64_t rows;
-  int entries, top, parts, per;  // per: entries of a part, a multiple of kProbThreads * 8
+  int entries, top, parts, per;  // per: 16-byte pieces of a part
   float scale;
   // backward
   const float *glogp, *gentropy;
@@ -42,35 +48,43 @@ __device__ __forceinline__ float exp2_of(float x) {
 }
 
 constexpr float kNone = -INFINITY;
+constexpr float kRise = 8.f;
+constexpr float kFar = -1e30f;  // in the place of log2(0), whose product with 0 it leaves 0
 
+// c = scale log2 e.
 struct Sums {
   float m = kNone, s = 0.f, w = 0.f;
 
   // Everything so far to the reference `to` >= m.
   __device__ __forceinline__ void move(float to, float c) {
     if (m != kNone) {
-      const float d = m - to, f = exp2_of(d * c);
-      w = f * (w + fmaxf(d, -1e30f) * s);
+      const float t = fmaxf((m - to) * c, kFar), f = exp2_of((m - to) * c);
+      w = f * (w + t * s);
       s *= f;
     }
     m = to;
   }
-  __device__ __forceinline__ void join(float m2, float s2, float w2, float c) {
-    const float to = fmaxf(m, m2);
-    Sums o;
-    o.m = m2;
-    o.s = s2;
-    o.w = w2;
-    if (to != kNone) {
-      move(to, c);
-      o.move(to, c);
+  // The lanes' sums, in every lane.
+  __device__ __forceinline__ void join_lanes(float c) {
+    float to = m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, o));
+    if (to != kNone) move(to, c);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      w += __shfl_xor_sync(0xffffffffu, w, o);
     }
-    s += o.s;
-    w += o.w;
   }
 };
 
-// Of a warp: entry `lane` of the list in descending order, ties to the lower index.
+// Order of floats as unsigned numbers; NaN is not asked for.
+__device__ __forceinline__ unsigned ordered(float x) {
+  const unsigned u = __float_as_uint(x);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// Of a warp: entry `lane` of the list in descending order, ties to the lower index; index -1: none.
 struct Best {
   float v = kNone;
   int i = -1;
@@ -89,19 +103,50 @@ struct Best {
       i = pi;
     }
   }
+  // The 32 first of this list and another, whose entries come in ascending order: lane k has entry 31 - k. Of each pair the
+  // better one is among them, and the result rises to its maximum and falls again: five steps sort it.
+  __device__ __forceinline__ void merge(float x, int j) {
+    if (!before(x, j)) {
+      v = x;
+      i = j;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float ov = __shfl_xor_sync(0xffffffffu, v, o);
+      const int oi = __shfl_xor_sync(0xffffffffu, i, o);
+      const bool low = (threadIdx.x & o) == 0;  // keeps the better one
+      if (before(ov, oi) != low) {
+        v = ov;
+        i = oi;
+      }
+    }
+  }
 };
 
-// Lists of `top` entries in src (lists after each other), joined by one warp.
-template <typename Get>
-__device__ __forceinline__ void best_join(Best& best, int top, int lists, Get get) {
-  for (int l = 0; l < lists; ++l) {
-    for (int k = 0; k < top; ++k) {
-      const int2 e = get(l, k);  // descending: the first that is behind the last ends the list
-      const float x = __int_as_float(e.x);
-      const float lv = __shfl_sync(0xffffffffu, best.v, top - 1);
-      const int li = __shfl_sync(0xffffffffu, best.i, top - 1);
-      if (e.y < 0 || lv > x || (lv == x && (unsigned)li < (unsigned)e.y)) break;
-      best.insert(x, e.y);
+// N entries of each lane, entry e of index at(e), which rises with e and (for the same e) with the lane: those that belong in the first
+// `top` of the list. `last` is entry top - 1.
+template <int N, typename At>
+__device__ __forceinline__ void take_best(Best& best, float& last, int top, float (&x)[N], At at) {
+  for (;;) {
+    float m = x[0];
+    int e = 0;
+#pragma unroll
+    for (int k = 1; k < N; ++k)
+      if (x[k] > m) {  // the first of equal ones
+        m = x[k];
+        e = k;
+      }
+    if (!(m > last)) m = kNone;  // NaN and what the list has no room for
+    const unsigned key = __reduce_max_sync(0xffffffffu, ordered(m));
+    if (key == ordered(kNone)) return;
+    const unsigned mine = ordered(m) == key ? (unsigned)at(e) : 0xffffffffu, j = __reduce_min_sync(0xffffffffu, mine);
+    const int src = __ffs(__ballot_sync(0xffffffffu, mine == j)) - 1;
+    best.insert(__shfl_sync(0xffffffffu, m, src), (int)j);
+    last = __shfl_sync(0xffffffffu, best.v, top - 1);
+    if ((threadIdx.x & 31) == src) {
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (k == e) x[k] = kNone;
     }
   }
 }
@@ -123,7 +168,7 @@ __device__ __forceinline__ void prob_finish(const ProbArgs& A, int64_t r, const 
       lp = none || out ? (S.s != S.s ? S.s : kNone) : (x - S.m) * A.scale - L;
     }
     A.logp[r] = lp;
-    A.entropy[r] = none ? 0.f : fmaxf(L - A.scale * (S.w / S.s), 0.f) + 0.f * S.s;
+    A.entropy[r] = none ? 0.f : fmaxf(L - 0.6931471805599453f * (S.w / S.s), 0.f) + 0.f * S.s;
     if (A.stats) {
       A.stats[r] = none ? 0.f : S.m;
       A.stats[A.rows + r] = none ? INFINITY : log2f(S.s);
@@ -136,90 +181,219 @@ __device__ __forceinline__ void prob_finish(const ProbArgs& A, int64_t r, const 
   }
 }
 
-template <typename T, int E, bool TOP>
-__global__ void __launch_bounds__(kProbThreads) prob_kernel(ProbArgs A) {
+// The sums and lists of a block's warps, in warp 0. Called by the whole block.
+template <bool TOP>
+__device__ __forceinline__ void prob_join_warps(Sums& S, Best& best, float c) {
   __shared__ float4 sums[kProbWarps];
   __shared__ int2 lists[kProbWarps][32];
-  const int64_t r = blockIdx.x / A.parts;
-  const int part = blockIdx.x % A.parts;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  if (A.tok.padded(A.tok.at(r))) {
+  if (lane == 0) sums[w] = make_float4(S.m, S.s, S.w, 0.f);
+  if (TOP) lists[w][lane] = make_int2(__float_as_int(best.v), best.i);
+  __syncthreads();
+  if (w) return;
+  const float4 q = lane < kProbWarps ? sums[lane] : make_float4(kNone, 0.f, 0.f, 0.f);
+  S.m = q.x;
+  S.s = q.y;
+  S.w = q.z;
+  S.join_lanes(c);
+  if (TOP)
+    for (int k = 1; k < kProbWarps; ++k) {
+      const int2 e = lists[k][31 - lane];
+      best.merge(__int_as_float(e.x), e.y);
+    }
+}
+
+// A row as pieces of E entries on 16-byte boundaries; piece 0 may begin before the row, the last end behind it.
+template <typename T>
+struct PieceRow {
+  static constexpr int E = 16 / sizeof(T);
+  const T* base;  // of piece 0
+  int off, entries;  // entries of piece 0 before the row
+  int whole, end;    // pieces [whole, end) lie in the row
+
+  __device__ __forceinline__ PieceRow(const T* x, int V) {
+    off = (int)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T));
+    base = x - off;
+    entries = V;
+    whole = off > 0;
+    end = (int)(((int64_t)V + off) / E);
+  }
+  __device__ __forceinline__ int pieces() const { return end + (((int64_t)entries + off) % E != 0); }
+  __device__ __forceinline__ int first(int k) const { return k * E - off; }  // entry of the row
+  __device__ __forceinline__ bool has(int e) const { return e >= 0 && e < entries; }
+
+  // Piece k to a slot of this thread's; entries outside the row -inf.
+  __device__ __forceinline__ void bring(Pack<T, E>* slot, int k) const {
+    if (k >= whole && k < end) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(slot)),
+                   "l"(base + (int64_t)k * E)
+                   : "memory");
+    } else {
+      Pack<T, E> p;
+#pragma unroll
+      for (int e = 0; e < E; ++e) p.e[e] = has(first(k) + e) ? base[(int64_t)k * E + e] : from_f<T>(kNone);
+      *slot = p;
+    }
+  }
+  // Bit e: entry e of piece k is in the row and its byte of the mask is not 0.
+  __device__ __forceinline__ unsigned kept(const uint8_t* mask, bool aligned, int k) const {
+    unsigned keep = 0;
+    const int e0 = first(k);
+    if (aligned && k >= whole && k < end) {
+      const Pack<uint8_t, E> b = *reinterpret_cast<const Pack<uint8_t, E>*>(mask + e0);
+#pragma unroll
+      for (int e = 0; e < E; ++e) keep |= (b.e[e] ? 1u : 0u) << e;
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (has(e0 + e) && mask[e0 + e]) keep |= 1u << e;
+    }
+    return keep;
+  }
+};
+
+constexpr int kRing = 4;
+template <int N>
+__device__ __forceinline__ void ring_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ring_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+// A row (or one of its parts) by WARPS warps.
+template <typename T, bool TOP, int WARPS>
+__global__ void __launch_bounds__(kProbThreads, TOP ? 8 : 12) prob_kernel(ProbArgs A) {
+  using Row = PieceRow<T>;
+  constexpr int E = Row::E, STEP = WARPS * 32;
+  __shared__ Pack<T, E> ring[kRing][kProbThreads];
+  const int lane = threadIdx.x & 31;
+  const int64_t r = WARPS == 1 ? (int64_t)blockIdx.x * kProbWarps + (threadIdx.x >> 5) : blockIdx.x / A.parts;
+  const int part = WARPS == 1 ? 0 : (int)(blockIdx.x % A.parts), t = WARPS == 1 ? lane : threadIdx.x;
+  if (r >= A.rows) return;
+  if (A.tok.has_padding && A.tok.padded(A.tok.at(r))) {
     if (part == 0) {
-      if (threadIdx.x == 0) {
+      if (t == 0) {
         A.logp[r] = A.entropy[r] = 0.f;
         if (A.stats) {
           A.stats[r] = 0.f;
           A.stats[A.rows + r] = INFINITY;
         }
       }
-      if (TOP && threadIdx.x < A.top) {
-        A.top_logp[r * A.top + threadIdx.x] = kNone;
-        A.top_index[r * A.top + threadIdx.x] = -1;
+      if (TOP && t < A.top) {
+        A.top_logp[r * A.top + t] = kNone;
+        A.top_index[r * A.top + t] = -1;
       }
     }
     return;
   }
-  const T* x = static_cast<const T*>(A.logits) + r * A.ls;
+  const Row row(static_cast<const T*>(A.logits) + r * A.ls, A.entries);
   const uint8_t* mask = A.mask ? A.mask + r * A.ms : nullptr;
-  const float c = A.scale * kLog2e;
-  const int begin = part * A.per, end = min(begin + A.per, A.entries);
+  const bool mask_aligned = (reinterpret_cast<uintptr_t>(mask) - row.off) % E == 0;
+  const float c = A.scale * kLog2e, rise = fminf(kRise / c, 3e38f);
+  const int begin = part * A.per, end = min(begin + A.per, row.pieces());
   Sums S;
+  float s2[2] = {}, w2[2] = {};  // two sums each
   Best best;
   float last = kNone;  // of the list
-  for (int i0 = begin; i0 < end; i0 += kProbThreads * E) {  // the whole warp stays for the list
-    const int i = i0 + threadIdx.x * E;
-    float v[E];
-    if (i < end) {
-      const Pack<T, E> p = *reinterpret_cast<const Pack<T, E>*>(x + i);  // E > 1: entries are a multiple of E
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = to_f(p.e[e]);
-      if (mask) {
-        Pack<uint8_t, E> k = *reinterpret_cast<const Pack<uint8_t, E>*>(mask + i);
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (!k.e[e]) v[e] = kNone;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = kNone;
+  float m = 0.f;  // the reference, 0 before the first entry
+  // The entries of piece k (its first is the row's entry `from`), -inf where there are none; by whole warps. (Two entries an
+  // instruction, f32x2, took twice the instructions: the pairs have to be moved together.)
+  const auto take = [&](float (&v)[E], float top, int from) {
+    if (top > S.m + rise) {
+      S.s = s2[0] + s2[1];
+      S.w = w2[0] + w2[1];
+      S.move(top, c);
+      s2[0] = S.s;
+      w2[0] = S.w;
+      s2[1] = w2[1] = 0.f;
+      m = top;
     }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float a = (v[e] - m) * c, p = exp2_of(a);
+      s2[e & 1] += p;
+      w2[e & 1] = fmaf(p, fmaxf(a, kFar), w2[e & 1]);
+    }
+    if constexpr (TOP) {
+      if (__any_sync(0xffffffffu, top > last)) take_best(best, last, A.top, v, [&](int e) { return from + e; });
+    }
+  };
+  const auto greatest = [](const float (&v)[E]) {
     float top = v[0];
 #pragma unroll
     for (int e = 1; e < E; ++e) top = fmaxf(top, v[e]);
-    if (top > S.m) S.move(top, c);
-    const float m = S.m == kNone ? 0.f : S.m;
+    return top;
+  };
+  // piece k by lane 0, the others without entries; where it is not whole, or masked
+  const auto take_checked = [&](int k, bool has) {
+    float v[E];
+    const unsigned keep = !has ? 0u : mask ? row.kept(mask, mask_aligned, k) : 0xffffffffu;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float d = v[e] - m, p = exp2_of(d * c);
-      S.s += p;
-      S.w = fmaf(p, fmaxf(d, -1e30f), S.w);
-    }
-    if constexpr (TOP) {
-      unsigned who = __ballot_sync(0xffffffffu, top > last);
-      while (who) {
-        const int src = __ffs(who) - 1;
-        who &= who - 1;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float y = __shfl_sync(0xffffffffu, v[e], src);
-          if (y > last) {
-            best.insert(y, i0 + (w * 32 + src) * E + e);
-            last = __shfl_sync(0xffffffffu, best.v, A.top - 1);
-          }
-        }
+    for (int e = 0; e < E; ++e)
+      v[e] = (keep >> e & 1u) && row.has(row.first(k) + e) ? to_f(row.base[(int64_t)k * E + e]) : kNone;
+    take(v, greatest(v), row.first(k));
+  };
+  if (mask) {
+#pragma unroll 1
+    for (int i = begin; i < end; i += STEP) take_checked(i + t, i + t < end);
+  } else {
+    // pieces [b0, e0) are whole, a round of them every lane's but for the last; the one before and the one behind are the
+    // row's ends
+    const int b0 = max(begin, row.whole), e0 = min(end, row.end), rounds = max(e0 - b0, 0) / STEP;
+    const bool more = b0 + rounds * STEP + t < e0;
+    const T* from = row.base + (int64_t)(b0 + t) * E;
+    const uint32_t mine = (uint32_t)__cvta_generic_to_shared(&ring[0][threadIdx.x]);
+    const auto fetch = [&](int slot, int j) {
+      if (j < rounds || (j == rounds && more))
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + slot * (kProbThreads * 16)),
+                     "l"(from + (int64_t)j * (STEP * E))
+                     : "memory");
+      ring_commit();
+    };
+    const auto piece = [&](float (&v)[E], int slot) {  // its greatest
+      const Pack<T, E> p = ring[slot][threadIdx.x];
+      unpack<E>(p, v);
+      if constexpr (sizeof(T) == 2) {
+        const __nv_bfloat162* q = reinterpret_cast<const __nv_bfloat162*>(&p);
+        const float2 m = __bfloat1622float2(__hmax2(__hmax2(q[0], q[1]), __hmax2(q[2], q[3])));
+        return fmaxf(m.x, m.y);
+      } else {
+        return greatest(v);
       }
-    }
-  }
+    };
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    S.join(__shfl_xor_sync(0xffffffffu, S.m, o), __shfl_xor_sync(0xffffffffu, S.s, o), __shfl_xor_sync(0xffffffffu, S.w, o), c);
-  if (lane == 0) sums[w] = make_float4(S.m, S.s, S.w, 0.f);
-  if constexpr (TOP) lists[w][lane] = make_int2(__float_as_int(best.v), best.i);
-  __syncthreads();
-  if (w) return;
-  for (int k = 1; k < kProbWarps; ++k) S.join(sums[k].x, sums[k].y, sums[k].z, c);
-  if constexpr (TOP) best_join(best, A.top, kProbWarps - 1, [&](int l, int k) { return lists[l + 1][k]; });
-  if (A.parts == 1) {
+    for (int d = 0; d < kRing; ++d) fetch(d, d);
+    if (begin < b0) take_checked(begin, t == 0);
+    int slot = 0;
+#pragma unroll 1
+    for (int j = 0; j < rounds; ++j) {
+      float v[E];
+      ring_wait<kRing - 1>();
+      const float top = piece(v, slot);
+      fetch(slot, j + kRing);
+      slot = (slot + 1) % kRing;
+      take(v, top, row.first(b0 + t + j * STEP));
+    }
+    if (b0 + rounds * STEP < e0) {
+      float v[E], top = kNone;
+      ring_wait<0>();
+      if (more) {
+        top = piece(v, slot);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = kNone;
+      }
+      take(v, top, row.first(b0 + t + rounds * STEP));
+    }
+    if (e0 < end && e0 >= b0) take_checked(e0, t == 0);  // not the piece before, where that is the only one
+  }
+  S.s = s2[0] + s2[1];
+  S.w = w2[0] + w2[1];
+  S.join_lanes(c);
+  if constexpr (WARPS > 1) {
+    prob_join_warps<TOP>(S, best, c);
+    if (threadIdx.x >= 32) return;
+  }
+  if (WARPS == 1 || A.parts == 1) {
     prob_finish<T>(A, r, S, best);
   } else {
     if (lane == 0) A.part[blockIdx.x] = make_float4(S.m, S.s, S.w, 0.f);
@@ -227,67 +401,129 @@ __global__ void __launch_bounds__(kProbThreads) prob_kernel(ProbArgs A) {
   }
 }
 
-// A warp a row.
-template <typename T>
-__global__ void __launch_bounds__(128) prob_join_kernel(ProbArgs A) {
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (r >= A.rows || A.tok.padded(A.tok.at(r))) return;
+// A block a row: its parts in order by stretches of them a warp.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kProbThreads) prob_join_kernel(ProbArgs A) {
+  const int64_t r = blockIdx.x;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  if (A.tok.padded(A.tok.at(r))) return;
   const float c = A.scale * kLog2e;
+  const int per = (A.parts + kProbWarps - 1) / kProbWarps, first = w * per, end = min(first + per, A.parts);
   Sums S;
-  for (int p = lane; p < A.parts; p += 32) {
-    const float4 q = A.part[r * A.parts + p];
-    S.join(q.x, q.y, q.z, c);
+  for (int p = first + lane; p - lane < end; p += 32) {  // what is there so far counts as lane 0's
+    const float4 q = p < end ? A.part[r * A.parts + p] : make_float4(kNone, 0.f, 0.f, 0.f);
+    Sums one;
+    one.m = q.x;
+    one.s = q.y;
+    one.w = q.z;
+    one.join_lanes(c);
+    Sums both = lane ? one : S;
+    if (lane > 1) both = Sums{};
+    both.join_lanes(c);
+    S = both;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    S.join(__shfl_xor_sync(0xffffffffu, S.m, o), __shfl_xor_sync(0xffffffffu, S.s, o), __shfl_xor_sync(0xffffffffu, S.w, o), c);
   Best best;
-  if (A.top) {
+  if constexpr (TOP) {
     const int2* p = A.part_top + r * A.parts * A.top;
-    if (lane < A.top) {
-      const int2 q = p[lane];
-      best.v = __int_as_float(q.x);
-      best.i = q.y;
+    constexpr int kAhead = 4;
+    for (int l = first; l < end; l += kAhead) {
+      int2 q[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        q[u] = l + u < end && 31 - lane < A.top ? p[(l + u) * A.top + 31 - lane] : make_int2(__float_as_int(kNone), -1);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (l + u < end) best.merge(__int_as_float(q[u].x), q[u].y);
     }
-    best_join(best, A.top, A.parts - 1, [&](int l, int k) { return p[(l + 1) * A.top + k]; });
   }
-  prob_finish<T>(A, r, S, best);
+  prob_join_warps<TOP>(S, best, c);
+  if (w == 0) prob_finish<T>(A, r, S, best);
 }
 
 // ---------------------------------------------------------------- gradient
 // d = scale (g (hit - p) - e p (log p + H)), entry by entry: HBM.
 template <typename T, int E>
-__global__ void __launch_bounds__(kProbThreads) prob_grad_kernel(ProbArgs A) {
-  const int64_t r = blockIdx.x / A.parts;
-  const int begin = (int)(blockIdx.x % A.parts) * A.per, end = min(begin + A.per, A.entries);
-  const int64_t t = A.tok.at(r);
-  const bool padded = A.tok.padded(t);
-  const T* x = static_cast<const T*>(A.logits) + r * A.ls;
+__device__ __forceinline__ Pack<T, E> prob_round(const float (&d)[E]) {
+  Pack<T, E> o;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) o.e[e] = d[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; e += 2) *reinterpret_cast<__nv_bfloat162*>(&o.e[e]) = __floats2bfloat162_rn(d[e], d[e + 1]);
+  }
+  return o;
+}
+
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(kProbThreads, 12) prob_grad_kernel(ProbArgs A) {
+  using Row = PieceRow<T>;
+  constexpr int E = Row::E, STEP = WARPS * 32;
+  __shared__ Pack<T, E> ring[kRing][kProbThreads];
+  const int64_t r = WARPS == 1 ? (int64_t)blockIdx.x * kProbWarps + (threadIdx.x >> 5) : blockIdx.x / A.parts;
+  const int part = WARPS == 1 ? 0 : (int)(blockIdx.x % A.parts), lane = WARPS == 1 ? threadIdx.x & 31 : threadIdx.x;
+  if (r >= A.rows) return;
+  const Row row(static_cast<const T*>(A.logits) + r * A.ls, A.entries);
   const uint8_t* mask = A.mask ? A.mask + r * A.ms : nullptr;
-  T* out = static_cast<T*>(A.dlogits) + r * A.entries;
-  const float g = A.glogp && t >= 0 && t < A.entries ? A.glogp[r] : 0.f, e = A.gentropy ? A.gentropy[r] : 0.f;
-  const float m = A.stats[r], l2 = A.stats[A.rows + r], c = A.scale * kLog2e, H = A.entropy[r];
-  constexpr float kLn2 = 0.6931471805599453f;
-  for (int i = begin + threadIdx.x * E; i < end; i += kProbThreads * E) {
-    Pack<T, E> o;
-    if (padded) {
-#pragma unroll
-      for (int k = 0; k < E; ++k) o.e[k] = from_f<T>(0.f);
+  const bool mask_aligned = (reinterpret_cast<uintptr_t>(mask) - row.off) % E == 0;
+  T* out = static_cast<T*>(A.dlogits) + r * A.entries - row.off;  // of piece 0
+  const bool out_aligned = reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  const int begin = part * A.per + lane, end = min(part * A.per + A.per, row.pieces());
+  const auto store = [&](int k, const Pack<T, E>& o) {
+    if (out_aligned && k >= row.whole && k < row.end) {
+      *reinterpret_cast<Pack<T, E>*>(out + (int64_t)k * E) = o;
     } else {
-      const Pack<T, E> p = *reinterpret_cast<const Pack<T, E>*>(x + i);
-      Pack<uint8_t, E> keep;
-      if (mask) keep = *reinterpret_cast<const Pack<uint8_t, E>*>(mask + i);
 #pragma unroll
-      for (int k = 0; k < E; ++k) {
-        const float q = (to_f(p.e[k]) - m) * c - l2, pr = exp2_of(q);
-        // q of an entry without probability is -inf: 0 all the same
-        float d = -pr * (g + e * (fmaxf(q, -300.f) * kLn2 + H));
-        if (i + k == t) d += g;
-        o.e[k] = from_f<T>(mask && !keep.e[k] ? 0.f : d * A.scale);
-      }
+      for (int e = 0; e < E; ++e)
+        if (row.has(row.first(k) + e)) out[(int64_t)k * E + e] = o.e[e];
     }
-    *reinterpret_cast<Pack<T, E>*>(out + i) = o;
+  };
+  const int64_t t = A.tok.at(r);
+  if (A.tok.padded(t)) {
+    const float zero[E] = {};
+    for (int k = begin; k < end; k += STEP) store(k, prob_round<T, E>(zero));
+    return;
+  }
+#pragma unroll
+  for (int d = 0; d < kRing; ++d) {
+    if (begin + d * STEP < end) row.bring(&ring[d][threadIdx.x], begin + d * STEP);
+    ring_commit();
+  }
+  const bool given = t >= 0 && t < A.entries;
+  const float g = A.glogp && given ? A.glogp[r] : 0.f, ent = A.gentropy ? A.gentropy[r] : 0.f;
+  const float m = A.stats[r], l2 = A.stats[A.rows + r], c = A.scale * kLog2e;
+  // - scale p (g + e (log p + H)), log p = ln2 q
+  const float gs = -A.scale * (g + ent * A.entropy[r]), es = -A.scale * ent * 0.6931471805599453f, hit = A.scale * g;
+  const int at = given ? (int)t : -E;  // the token's entry
+  int slot = 0;
+#pragma unroll 1
+  for (int k = begin; k < end; k += STEP) {
+    ring_wait<kRing - 1>();
+    const Pack<T, E> v = ring[slot][threadIdx.x];
+    if (k + kRing * STEP < end) row.bring(&ring[slot][threadIdx.x], k + kRing * STEP);
+    ring_commit();
+    slot = slot + 1 == kRing ? 0 : slot + 1;
+    float d[E];
+    unpack<E>(v, d);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float q = fmaf(d[e] - m, c, -l2);
+      // an entry without probability has log2 p = -inf: 0 all the same
+      d[e] = exp2_of(q) * fmaf(es, fmaxf(q, -300.f), gs);
+    }
+    const unsigned here = (unsigned)(at - row.first(k));
+    if (here < (unsigned)E) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if ((unsigned)e == here) d[e] += hit;
+    }
+    if (mask) {
+      const unsigned keep = row.kept(mask, mask_aligned, k);
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (!(keep >> e & 1u)) d[e] = 0.f;
+    }
+    store(k, prob_round<T, E>(d));
   }
 }
 
