@@ -83,6 +83,21 @@ __device__ __forceinline__ __half from_f<__half>(float x) {
   return __float2half_rn(x);
 }
 
+template <int N>
+__device__ __forceinline__ void unpack(const Pack<__half, N>& p, float* x) {
+  if constexpr (N % 2) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = to_f(p.e[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p.e[e]));
+      x[e] = f.x;
+      x[e + 1] = f.y;
+    }
+  }
+}
+
 // N entries rounded into a pack, two at a time where the type has it.
 template <int N>
 __device__ __forceinline__ void round_into(Pack<float, N>& o, const float (&x)[N]) {

@@ -187,11 +187,12 @@ __device__ __forceinline__ void spoil(int state, uint32_t (&v)[C]) {
 // N entries of a row: activation, residual, stores.
 template <typename T, int ACT, int N, bool RES, bool SLOPE>
 __device__ __forceinline__ void finish(const float (&h)[N], const Pack<T, N>& residual, T* y, typename SlopeOf<T>::type* slope) {
-  float v[N], d[N];
+  float v[N], d[N], res[N];
+  unpack<N>(residual, res);
 #pragma unroll
   for (int e = 0; e < N; ++e) {
     const ActOut a = activate<ACT>(h[e]);
-    v[e] = RES ? a.y + to_f(residual.e[e]) : a.y;
+    v[e] = RES ? a.y + res[e] : a.y;
     d[e] = a.d;
   }
   Pack<T, N> o;
@@ -220,6 +221,8 @@ __device__ __forceinline__ void store_rows(const Args& G, const unsigned char* s
   constexpr int L = C / N, R = 32 / L, U = N == 1 ? 8 : 2;  // U: residuals read ahead
   const int lane = threadIdx.x & 31, c = lane % L * N, r0 = lane / L;
   const int64_t step = R * G.cols, rstep = R * G.e.rs;
+  float b[N];
+  unpack<N>(bias, b);
 #pragma unroll (N == 1 ? 1 : 32)
   for (int k0 = 0; k0 < 32; k0 += U * R) {
     Pack<T, N> res[U] = {};
@@ -245,7 +248,7 @@ __device__ __forceinline__ void store_rows(const Args& G, const unsigned char* s
         }
       }
 #pragma unroll
-      for (int e = 0; e < N; ++e) h[e] += to_f(bias.e[e]);
+      for (int e = 0; e < N; ++e) h[e] += b[e];
       if (k0 + u * R < last) finish<T, ACT, N, RES, SLOPE>(h, res[u], y, slope);
       y += step;
       if constexpr (SLOPE) slope += step;
@@ -652,9 +655,7 @@ __device__ __forceinline__ void load_eight(const T* p, int64_t n, bool vec, floa
 #pragma unroll
     for (int h = 0; h < 8; h += V) {
       if (h < n) {
-        const Pack<T, V> k = *reinterpret_cast<const Pack<T, V>*>(p + h);
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[h + e] = to_f(k.e[e]);
+        unpack<V>(*reinterpret_cast<const Pack<T, V>*>(p + h), x + h);
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e) x[h + e] = 0.f;
@@ -721,7 +722,7 @@ __global__ void __launch_bounds__(256) linear_prep_kernel(const __grid_constant_
   const int64_t end = r0 + P.per < A.rows ? r0 + P.per : A.rows;
   float sum[8] = {};
   if (j < A.cols) {
-#pragma unroll 2
+#pragma unroll 4
     for (int64_t i = r0 + g; i < end; i += groups) {
       float x[8];
       load_eight<T>(static_cast<const T*>(A.src) + i * A.stride + j, A.cols - j, A.vec, x);

@@ -64,8 +64,10 @@ __global__ void __launch_bounds__(kEmbedThreads) embed_fwd_kernel(EmbedFwd A) {
         if (k + u * rows + sub >= n || c >= A.chunks) continue;
         P o;
         if (row[u] >= 0) {
+          float x[E];
+          unpack<E>(v[u], x);
 #pragma unroll
-          for (int e = 0; e < E; ++e) o.e[e] = from_f<T>(to_f(v[u].e[e]) * A.scale);
+          for (int e = 0; e < E; ++e) o.e[e] = from_f<T>(x[e] * A.scale);
         } else {
 #pragma unroll
           for (int e = 0; e < E; ++e) o.e[e] = from_f<T>(row[u] == -1 ? 0.f : __int_as_float(0x7fc00000));
@@ -294,8 +296,10 @@ __global__ void __launch_bounds__(kEmbedThreads, E > 4 ? 3 : 4) embed_window_ker
         for (int e = 0; e < E; ++e) acc[e] = 0.f;
       }
       if (now[u] < A.rows) {
+        float y[E];
+        unpack<E>(x[u], y);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += to_f(x[u].e[e]);
+        for (int e = 0; e < E; ++e) acc[e] += y[e];
       }
     }
   }
