@@ -1,5 +1,6 @@
 // The linear map with its epilogue (linear_tc.cuh): checks, launch shapes, workspace.
 #include "block_host.cuh"
+#include "linear_rows.cuh"
 #include "linear_tc.cuh"
 #include "tensor_map.cuh"
 
@@ -153,6 +154,35 @@ struct LinPlan {
     return n;
   }
 };
+
+// Few rows are bound by the weights' bytes and need no layout (linear_rows.cuh). Measured, us, against the tiles of the
+// tensor cores at 8192 -> 4096: 32 rows bfloat16 24 and 27, float32 99 and 138; 64 rows bfloat16 52 and 26.
+bool few_rows(const fx_linear_args* a) { return a->rows <= 32; }
+
+template <typename T, int NP, int MT, int NT>
+int rows_launch(cudaStream_t s, const lin::RowArgs& A, bool al) {
+  const unsigned blocks = (unsigned)ceil_div(A.outer, 16 * MT);
+  constexpr size_t smem = lin::RowRing<T, MT, NT>::kSmem;
+  if (al) {
+    auto kern = lin::linear_rows_kernel<T, NP, MT, NT, true>;
+    if (raise_smem(kern, smem, smem)) return FX_ERR_CUDA;
+    kern<<<blocks, lin::kRowWarps * 32, smem, s>>>(A);
+  } else {
+    lin::linear_rows_kernel<T, NP, MT, NT, false><<<blocks, lin::kRowWarps * 32, 0, s>>>(A);
+  }
+  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+}
+
+template <typename T, int NP>
+int rows_forward(cudaStream_t s, const fx_linear_args* a) {
+  const lin::RowArgs A{a->x, a->weight, a->x_stride, a->weight_stride, (int)a->rows, (int)a->inner, (int)a->outer,
+                       {a->activation, a->bias, a->residual, a->residual_stride, a->y, a->slope}};
+  const bool al = aligned(a->x, a->x_stride, a->rows, a->inner, sizeof(T)) &&
+                  aligned(a->weight, a->weight_stride, a->outer, a->inner, sizeof(T));
+  if (A.rows <= 8) return rows_launch<T, NP, 1, 1>(s, A, al);
+  if (A.rows <= 16) return rows_launch<T, NP, 1, 2>(s, A, al);
+  return rows_launch<T, NP, NP == 1 ? 2 : 1, 4>(s, A, al);
+}
 
 LinPlan plan_fwd(const fx_linear_args* a, int sms) {
   LinPlan P{};
@@ -393,7 +423,7 @@ extern "C" {
 
 size_t fermix_linear_workspace_bytes(const fx_linear_args* a) {
   const DevInfo* D = dev_info();
-  return check(a) || !D || a->rows == 0 ? 0 : plan_fwd(a, D->sms).bytes;
+  return check(a) || !D || few_rows(a) ? 0 : plan_fwd(a, D->sms).bytes;
 }
 
 int fermix_linear(void* stream, const fx_linear_args* a, void* ws, size_t wsb) {
@@ -401,11 +431,12 @@ int fermix_linear(void* stream, const fx_linear_args* a, void* ws, size_t wsb) {
   if (e) return e;
   if (a->rows == 0) return FX_OK;
   if (!a->x || !a->weight || !a->y) return FX_ERR_NULL;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (few_rows(a)) return a->dtype == FX_F32 ? rows_forward<float, 3>(s, a) : rows_forward<bf16, 1>(s, a);
   const DevInfo* D = dev_info();
   if (!D) return FX_ERR_DEVICE;
   const LinPlan P = plan_fwd(a, D->sms);
   if (P.bytes && (!ws || wsb < P.bytes)) return FX_ERR_WORKSPACE;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   return P.f32 ? forward<float, 3>(s, a, P, base_of(ws), D->sms) : forward<bf16, 1>(s, a, P, base_of(ws), D->sms);
 }
 

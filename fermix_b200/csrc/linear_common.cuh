@@ -131,4 +131,41 @@ struct Epilogue {
   void *y, *slope;  // (rows, cols) contiguous
 };
 
+__device__ __forceinline__ ActOut activate_as(int act, float h) {
+  switch (act) {
+    case FX_ACT_RELU: return activate<FX_ACT_RELU>(h);
+    case FX_ACT_SILU: return activate<FX_ACT_SILU>(h);
+    case FX_ACT_GELU: return activate<FX_ACT_GELU>(h);
+    case FX_ACT_GELU_TANH: return activate<FX_ACT_GELU_TANH>(h);
+    case FX_ACT_TANH: return activate<FX_ACT_TANH>(h);
+    default: return activate<FX_ACT_NONE>(h);
+  }
+}
+
+// One entry of the sum: bias, activation, residual, stores.
+template <typename T>
+__device__ __forceinline__ void store_entry(const Epilogue& E, int64_t i, int64_t j, int64_t cols, float h) {
+  using TS = typename SlopeOf<T>::type;
+  if (E.bias) h += to_f(static_cast<const T*>(E.bias)[j]);
+  ActOut a = activate_as(E.act, h);
+  if (E.act != FX_ACT_NONE && E.slope) static_cast<TS*>(E.slope)[i * cols + j] = from_f<TS>(a.d);
+  if (E.residual) a.y += to_f(static_cast<const T*>(E.residual)[i * E.rs + j]);
+  static_cast<T*>(E.y)[i * cols + j] = from_f<T>(a.y);
+}
+
+// (a, b) -> NP packed pairs of bfloat16 whose sum is (a, b). The first is rounded to a finite number where its value is,
+// which leaves the rest to the second.
+template <int NP>
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&o)[NP]) {
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    if (NP > 1 && i == 0) asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(o[i]) : "f"(b), "f"(a));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[i]) : "f"(b), "f"(a));
+    if (i + 1 < NP) {
+      a -= __uint_as_float(o[i] << 16);
+      b -= __uint_as_float(o[i] & 0xffff0000u);
+    }
+  }
+}
+
 }  // namespace fx

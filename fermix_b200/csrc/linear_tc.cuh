@@ -630,24 +630,6 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
   }
 }
 
-// (a, b) -> NP packed pairs of bfloat16 whose sum is (a, b). What rounds to infinity though it is
-// finite is cut off instead.
-template <int NP>
-__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&o)[NP]) {
-#pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[i]) : "f"(b), "f"(a));
-    if (NP > 1 && i == 0) {
-      if ((o[0] & 0x7fffu) == 0x7f80u && fabsf(a) < INFINITY) o[0] = (o[0] & 0xffff0000u) | (o[0] & 0x8000u) | 0x7f7fu;
-      if ((o[0] & 0x7fff0000u) == 0x7f800000u && fabsf(b) < INFINITY) o[0] = (o[0] & 0x8000ffffu) | 0x7f7f0000u;
-    }
-    if (i + 1 < NP) {
-      a -= __uint_as_float(o[i] << 16);
-      b -= __uint_as_float(o[i] & 0xffff0000u);
-    }
-  }
-}
-
 template <typename T>
 __device__ __forceinline__ void load_eight(const T* p, int64_t n, bool vec, float (&x)[8]) {
   constexpr int V = 16 / sizeof(T);
