@@ -177,6 +177,32 @@ def lib():
     return _lib
 
 
+_binding = None
+
+
+def binding():
+    """The Python module that binds the operators on tokens to torch (csrc/torch_binding.cpp); raises if
+    it has not been built."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    lib()
+    with _lock:
+        if _binding is None:
+            import importlib.util
+
+            path = os.path.join(LIB_DIR, "fermix_torch.so")
+            if not os.path.exists(path):
+                raise FermixError(f"{path} is missing: build it with `python -m fermix_b200.build` "
+                                  "(fermix_b200 has no CPU fallback)")
+            spec = importlib.util.spec_from_file_location("fermix_torch", path)
+            m = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(m)
+            m.raise_as(FermixError)
+            _binding = m
+    return _binding
+
+
 def device_status(clear=False):
     """The kernels' status on the current CUDA device (synchronises it): 0, or
     FX_ERR_TIMEOUT when a kernel gave up a bounded wait since the last clear (its members'

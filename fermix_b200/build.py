@@ -1,7 +1,8 @@
 """Build libfermix_b200.so in-tree for sm_100a (nvcc cross-compiles without a GPU).
 
 Each csrc/*.cu is compiled to an object of its own, in parallel, then linked into one
-shared library:
+shared library; csrc/torch_binding.cpp becomes the Python module that binds the operators on
+tokens to torch (fermix_torch.so, against the installed torch):
 
     python -m fermix_b200.build [--force] [-j N]
 """
@@ -18,6 +19,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 OBJ_DIR = os.path.join(OUT_DIR, "obj")
 OUT = os.path.join(OUT_DIR, "libfermix_b200.so")
+BINDING = os.path.join(CSRC, "torch_binding.cpp")
+BINDING_OUT = os.path.join(OUT_DIR, "fermix_torch.so")
 INCLUDE = os.path.join(ROOT, "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -55,20 +58,52 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _binding_deps():
+    return [BINDING, os.path.abspath(__file__)] + glob.glob(os.path.join(INCLUDE, "*.h"))
+
+
 def up_to_date():
-    return not _stale(OUT, sources() + [os.path.abspath(__file__)])
+    return not _stale(OUT, sources() + [os.path.abspath(__file__)]) and not _stale(BINDING_OUT, _binding_deps())
 
 
-def _compile(cu, verbose):
-    obj = _obj(cu)
-    cmd = [_nvcc(), *NVCC_FLAGS, "-I", INCLUDE, "-c", "-o", obj + ".tmp", cu]
+def _run(cmd, name, verbose):
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"nvcc failed on {os.path.basename(cu)}:\n{r.stdout}\n{r.stderr}")
+        raise RuntimeError(f"{cmd[0]} failed on {name}:\n{r.stdout}\n{r.stderr}")
     if verbose and (r.stdout.strip() or r.stderr.strip()):
         print(r.stdout + r.stderr, flush=True)
+
+
+def _compile_binding(verbose):
+    import sysconfig
+
+    import torch
+
+    root = os.path.join(os.path.dirname(torch.__file__), "include")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())) if os.path.sep in _nvcc() else "/usr/local/cuda", "include")
+    obj = os.path.join(OBJ_DIR, "torch_binding.o")
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-c", "-DTORCH_EXTENSION_NAME=fermix_torch",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-I", INCLUDE, "-isystem", root, "-isystem",
+          os.path.join(root, "torch", "csrc", "api", "include"), "-isystem", cuda, "-isystem",
+          sysconfig.get_paths()["include"], "-o", obj + ".tmp", BINDING], os.path.basename(BINDING), verbose)
+    os.replace(obj + ".tmp", obj)
+
+
+def _link_binding(verbose):
+    import torch
+
+    _run(["g++", "-shared", "-o", BINDING_OUT + ".tmp", os.path.join(OBJ_DIR, "torch_binding.o"),
+          "-L", os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+          "-lc10_cuda", "-ltorch_cuda", "-L", OUT_DIR, "-l:libfermix_b200.so", "-Wl,-rpath,$ORIGIN"],
+         os.path.basename(BINDING_OUT), verbose)
+    os.replace(BINDING_OUT + ".tmp", BINDING_OUT)
+
+
+def _compile(cu, verbose):
+    obj = _obj(cu)
+    _run([_nvcc(), *NVCC_FLAGS, "-I", INCLUDE, "-c", "-o", obj + ".tmp", cu], os.path.basename(cu), verbose)
     os.replace(obj + ".tmp", obj)
     return obj
 
@@ -79,17 +114,21 @@ def build(force=False, verbose=False, jobs=None):
     os.makedirs(OBJ_DIR, exist_ok=True)
     hdr = headers() + [os.path.abspath(__file__)]
     todo = [cu for cu in units() if force or _stale(_obj(cu), [cu] + hdr)]
-    jobs = jobs or max(1, min(len(todo), os.cpu_count() or 1))
-    if todo:
-        with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as ex:
-            for f in [ex.submit(_compile, cu, verbose) for cu in todo]:
-                f.result()
-    objs = [_obj(cu) for cu in units()]
-    cmd = [_nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", OUT + ".tmp", *objs]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
-    os.replace(OUT + ".tmp", OUT)
+    bind = force or _stale(os.path.join(OBJ_DIR, "torch_binding.o"), _binding_deps())
+    jobs = jobs or max(1, min(len(todo) + bind, os.cpu_count() or 1))
+    with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as ex:
+        work = [ex.submit(_compile_binding, verbose)] if bind else []
+        work += [ex.submit(_compile, cu, verbose) for cu in todo]
+        for f in work:
+            f.result()
+    if force or todo or _stale(OUT, sources()):
+        objs = [_obj(cu) for cu in units()]
+        _run([_nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", OUT + ".tmp", *objs], os.path.basename(OUT), verbose)
+        os.replace(OUT + ".tmp", OUT)
+    if force or bind or not os.path.exists(BINDING_OUT):
+        _link_binding(verbose)
+    for path in (OUT, BINDING_OUT):  # both at least as new as what they come from
+        os.utime(path)
     return OUT
 
 
