@@ -19,22 +19,35 @@ int check(const fx_embed_args* a) {
 
 Tokens tokens_of(const fx_embed_args* a) { return {a->tokens, a->token_bytes, a->has_padding != 0, a->padding}; }
 
-// Pieces of a row and the threads that share it. Rows that are not whole 16-byte pieces on
-// 16-byte boundaries go entry by entry.
+// Pieces of a row, the largest up to 16 bytes that rows are whole pieces of, on boundaries of theirs, and the threads
+// that share a row.
 struct Shape {
-  bool vec;
   int entries, chunks, tpr;
 };
 
 Shape shape_of(const fx_embed_args* a, const void* p, const void* q) {
   const int size = a->dtype == FX_F32 ? 4 : 2;
+  const uintptr_t m = (uintptr_t)(a->width * size) | reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q);
+  int piece = 16;
+  while (piece > size && m % piece) piece /= 2;
   Shape s;
-  s.vec = (a->width * size | reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q)) % 16 == 0;
-  s.entries = s.vec ? 16 / size : 1;
+  s.entries = piece / size;
   s.chunks = (int)(a->width / s.entries);
   s.tpr = 1;
   while (s.tpr < s.chunks && s.tpr < kEmbedThreads) s.tpr *= 2;
   return s;
+}
+
+// f.template operator()<T, E>() for the type and the entries of a piece.
+template <typename F>
+int by_piece(int dtype, int entries, F f) {
+  if (dtype == FX_F32) {
+    if (entries == 4) return f.template operator()<float, 4>();
+    return entries == 2 ? f.template operator()<float, 2>() : f.template operator()<float, 1>();
+  }
+  if (entries == 8) return f.template operator()<bf16, 8>();
+  if (entries == 4) return f.template operator()<bf16, 4>();
+  return entries == 2 ? f.template operator()<bf16, 2>() : f.template operator()<bf16, 1>();
 }
 
 // Few tokens and rows are listed row by row in one launch: rows x count comparisons.
@@ -73,30 +86,44 @@ SortPlan plan_of(const fx_embed_args* a, const Shape& s, int sms) {
   return P;
 }
 
-template <typename T, int E>
-int run_fwd(cudaStream_t s, const EmbedFwd& A) {
-  const int64_t per = 32 * (kEmbedThreads / 32) / (A.tpr > 32 ? A.tpr / 32 : 1);  // rows of a block
-  embed_fwd_kernel<T, E><<<(unsigned)((A.count + per - 1) / per), kEmbedThreads, 0, s>>>(A);
-  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
-}
+struct Fwd {
+  cudaStream_t s;
+  const EmbedFwd& A;
+  template <typename T, int E>
+  int operator()() const {
+    const int64_t per = 32 * (kEmbedThreads / 32) / (A.tpr > 32 ? A.tpr / 32 : 1);  // rows of a block
+    embed_fwd_kernel<T, E><<<(unsigned)((A.count + per - 1) / per), kEmbedThreads, 0, s>>>(A);
+    return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+  }
+};
 
-template <typename T, int E>
-int run_scan(cudaStream_t s, const EmbedGrad& A, const Tokens& tok) {
-  embed_scan_kernel<T, E><<<(unsigned)A.rows, kEmbedThreads, 0, s>>>(A, tok);
-  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
-}
+struct Scan {
+  cudaStream_t s;
+  const EmbedGrad& A;
+  const Tokens& tok;
+  template <typename T, int E>
+  int operator()() const {
+    embed_scan_kernel<T, E><<<(unsigned)A.rows, kEmbedThreads, 0, s>>>(A, tok);
+    return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+  }
+};
 
-template <typename T, int E>
-int run_sums(cudaStream_t s, const EmbedGrad& A, int sms) {
-  const int groups = kEmbedThreads / A.tpr;
-  const dim3 windows((A.windows + groups - 1) / groups, (unsigned)((A.chunks + A.tpr - 1) / A.tpr));
-  embed_window_kernel<T, E><<<windows, kEmbedThreads, 0, s>>>(A);
-  // the join: a warp for every row of the table, a block for every window that a long run may begin in, as far as the
-  // device holds them
-  const int64_t blocks = (A.rows + 7) / 8, want = blocks > A.windows ? blocks : A.windows, most = (int64_t)sms * 4;
-  embed_join_kernel<T, E><<<(unsigned)(want < most ? want : most), kEmbedThreads, 0, s>>>(A);
-  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
-}
+struct SumRuns {
+  cudaStream_t s;
+  const EmbedGrad& A;
+  int sms;
+  template <typename T, int E>
+  int operator()() const {
+    const int groups = kEmbedThreads / A.tpr;
+    const dim3 windows((A.windows + groups - 1) / groups, (unsigned)((A.chunks + A.tpr - 1) / A.tpr));
+    embed_window_kernel<T, E><<<windows, kEmbedThreads, 0, s>>>(A);
+    // the join: a warp for every row of the table, a block for every window that a long run may begin in, as far as the
+    // device holds them
+    const int64_t blocks = (A.rows + 7) / 8, want = blocks > A.windows ? blocks : A.windows, most = (int64_t)sms * 4;
+    embed_join_kernel<T, E><<<(unsigned)(want < most ? want : most), kEmbedThreads, 0, s>>>(A);
+    return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+  }
+};
 
 int sort(cudaStream_t s, const fx_embed_args* a, const SortPlan& P, unsigned char* ws, EmbedGrad& A) {
   int* lists = reinterpret_cast<int*>(ws + P.keys);
@@ -144,8 +171,7 @@ int fermix_token_embedding(void* stream, const fx_embed_args* a) {
   const Shape h = shape_of(a, a->weight, a->out);
   EmbedFwd A{tokens_of(a), a->weight, a->out, a->count, a->rows, a->width, h.chunks, h.tpr, a->scale};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a->dtype == FX_F32) return h.vec ? run_fwd<float, 4>(s, A) : run_fwd<float, 1>(s, A);
-  return h.vec ? run_fwd<bf16, 8>(s, A) : run_fwd<bf16, 1>(s, A);
+  return by_piece(a->dtype, h.entries, Fwd{s, A});
 }
 
 // Without the pointers the larger of the two forms counts: entry by entry, fewer windows never
@@ -178,8 +204,7 @@ int fermix_token_embedding_grad(void* stream, const fx_embed_args* a, void* ws, 
   A.scale = a->scale;
   if (scans(a)) {
     const Tokens t = tokens_of(a);
-    if (a->dtype == FX_F32) return h.vec ? run_scan<float, 4>(s, A, t) : run_scan<float, 1>(s, A, t);
-    return h.vec ? run_scan<bf16, 8>(s, A, t) : run_scan<bf16, 1>(s, A, t);
+    return by_piece(a->dtype, h.entries, Scan{s, A, t});
   }
   const DevInfo* D = dev_info();
   if (!D) return FX_ERR_DEVICE;
@@ -191,8 +216,7 @@ int fermix_token_embedding_grad(void* stream, const fx_embed_args* a, void* ws, 
   A.part = reinterpret_cast<float*>(base + P.part);
   const int st = sort(s, a, P, base, A);
   if (st) return st;
-  if (a->dtype == FX_F32) return h.vec ? run_sums<float, 4>(s, A, D->sms) : run_sums<float, 1>(s, A, D->sms);
-  return h.vec ? run_sums<bf16, 8>(s, A, D->sms) : run_sums<bf16, 1>(s, A, D->sms);
+  return by_piece(a->dtype, h.entries, SumRuns{s, A, D->sms});
 }
 
 }  // extern "C"

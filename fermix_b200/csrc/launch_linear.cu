@@ -158,30 +158,36 @@ struct LinPlan {
 // Few rows are bound by the weights' bytes and need no layout (linear_rows.cuh). Measured, us, against the tiles of the
 // tensor cores at 8192 -> 4096: 32 rows bfloat16 24 and 27, float32 99 and 138; 64 rows bfloat16 52 and 26.
 bool few_rows(const fx_linear_args* a) { return a->rows <= 32; }
+// So are few outputs by the rows' bytes, in float32, where the tiles' layout would read and write four times as much.
+bool few_outputs(const fx_linear_args* a) { return a->dtype == FX_F32 && a->outer <= 32; }
 
-template <typename T, int NP, int MT, int NT>
+template <typename T, int NP, int MT, int NT, int WARPS>
 int rows_launch(cudaStream_t s, const lin::RowArgs& A, bool al) {
   const unsigned blocks = (unsigned)ceil_div(A.outer, 16 * MT);
-  constexpr size_t smem = lin::RowRing<T, MT, NT>::kSmem;
-  if (al) {
-    auto kern = lin::linear_rows_kernel<T, NP, MT, NT, true>;
-    if (raise_smem(kern, smem, smem)) return FX_ERR_CUDA;
-    kern<<<blocks, lin::kRowWarps * 32, smem, s>>>(A);
-  } else {
-    lin::linear_rows_kernel<T, NP, MT, NT, false><<<blocks, lin::kRowWarps * 32, 0, s>>>(A);
-  }
+  constexpr size_t smem = lin::RowRing<T, MT, NT, WARPS>::kSmem;
+  auto kern = al ? lin::linear_rows_kernel<T, NP, MT, NT, WARPS, true> : lin::linear_rows_kernel<T, NP, MT, NT, WARPS, false>;
+  if (raise_smem(kern, smem, smem)) return FX_ERR_CUDA;
+  kern<<<blocks, WARPS * 32, smem, s>>>(A);
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }
 
 template <typename T, int NP>
 int rows_forward(cudaStream_t s, const fx_linear_args* a) {
-  const lin::RowArgs A{a->x, a->weight, a->x_stride, a->weight_stride, (int)a->rows, (int)a->inner, (int)a->outer,
-                       {a->activation, a->bias, a->residual, a->residual_stride, a->y, a->slope}};
-  const bool al = aligned(a->x, a->x_stride, a->rows, a->inner, sizeof(T)) &&
-                  aligned(a->weight, a->weight_stride, a->outer, a->inner, sizeof(T));
-  if (A.rows <= 8) return rows_launch<T, NP, 1, 1>(s, A, al);
-  if (A.rows <= 16) return rows_launch<T, NP, 1, 2>(s, A, al);
-  return rows_launch<T, NP, NP == 1 ? 2 : 1, 4>(s, A, al);
+  lin::RowArgs A{a->x, a->weight, a->x_stride, a->weight_stride, (int)a->rows, (int)a->inner, (int)a->outer, false,
+                 {a->activation, a->bias, a->residual, a->residual_stride, a->y, a->slope}};
+  if (!few_rows(a)) {
+    A.x = a->weight;
+    A.w = a->x;
+    A.xs = a->weight_stride;
+    A.ws = a->x_stride;
+    A.rows = (int)a->outer;
+    A.outer = (int)a->rows;
+    A.swapped = true;
+  }
+  const bool al = aligned(A.x, A.xs, A.rows, A.inner, sizeof(T)) && aligned(A.w, A.ws, A.outer, A.inner, sizeof(T));
+  if (A.rows <= 8) return rows_launch<T, NP, 1, 1, 8>(s, A, al);
+  if (A.rows <= 16) return rows_launch<T, NP, 1, 2, 8>(s, A, al);
+  return rows_launch<T, NP, NP == 1 ? 2 : 1, 4, NP == 1 ? 16 : 8>(s, A, al);
 }
 
 LinPlan plan_fwd(const fx_linear_args* a, int sms) {
@@ -211,8 +217,9 @@ LinPlan plan_bwd(const fx_linear_args* a, int sms) {
   P.tpr = 1;
   while (P.tpr < 32 && P.tpr * 8 < a->outer) P.tpr *= 2;
   const int64_t groups = 256 / P.tpr, strips = ceil_div(a->outer, P.tpr * 8);
-  // eight blocks an SM, of four rows a thread at least
-  int64_t blocks = ceil_div((int64_t)sms * 8, strips);
+  // as many blocks as an SM holds, of four rows a thread at least
+  int64_t blocks = (int64_t)sms * (P.f32 ? 4 : 5) / strips;
+  if (blocks < 1) blocks = 1;
   if (blocks > ceil_div(a->rows, groups * 4)) blocks = ceil_div(a->rows, groups * 4);
   P.per = ceil_div(a->rows, blocks);
   P.blocks = (int)ceil_div(a->rows, P.per);
@@ -423,7 +430,7 @@ extern "C" {
 
 size_t fermix_linear_workspace_bytes(const fx_linear_args* a) {
   const DevInfo* D = dev_info();
-  return check(a) || !D || few_rows(a) ? 0 : plan_fwd(a, D->sms).bytes;
+  return check(a) || !D || few_rows(a) || few_outputs(a) ? 0 : plan_fwd(a, D->sms).bytes;
 }
 
 int fermix_linear(void* stream, const fx_linear_args* a, void* ws, size_t wsb) {
@@ -432,7 +439,7 @@ int fermix_linear(void* stream, const fx_linear_args* a, void* ws, size_t wsb) {
   if (a->rows == 0) return FX_OK;
   if (!a->x || !a->weight || !a->y) return FX_ERR_NULL;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (few_rows(a)) return a->dtype == FX_F32 ? rows_forward<float, 3>(s, a) : rows_forward<bf16, 1>(s, a);
+  if (few_rows(a) || few_outputs(a)) return a->dtype == FX_F32 ? rows_forward<float, 3>(s, a) : rows_forward<bf16, 1>(s, a);
   const DevInfo* D = dev_info();
   if (!D) return FX_ERR_DEVICE;
   const LinPlan P = plan_fwd(a, D->sms);

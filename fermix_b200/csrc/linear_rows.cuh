@@ -1,7 +1,8 @@
 // The linear map of few rows (a token a walker): bound by the weights' bytes, which are read once, straight into
-// the operand registers of the warps' tensor instructions (m16n8k16: 16 outputs by 8 rows of x).
+// the operand registers of the warps' tensor instructions (m16n8k16: 16 outputs by 8 rows of x). Of few outputs likewise
+// (float32, where the tiles of linear_tc.cuh would read and write x's parts besides): x and the weights change places.
 //
-// A block has 16 MT outputs and all rows; its eight warps share k in steps of 32, and their sums are added in order
+// A block has 16 MT outputs and all rows; its WARPS warps share k in steps of 32, and their sums are added in order
 // through shared memory. The order of k within a step is free as long as both operands have it: lane t of a
 // group of four takes entries 8 t .. 8 t + 7 of its row (float32: 4 t .. and 16 + 4 t .., four each), pieces of 16
 // bytes next to its neighbours', which are two instructions' worth of a fragment. Each lane's pieces come through a ring of asynchronous copies of its own: held in registers, the
@@ -16,12 +17,13 @@
 namespace fx {
 namespace lin {
 
-constexpr int kRowWarps = 8, kRowStep = 32;
+constexpr int kRowStep = 32;
 
 struct RowArgs {
   const void *x, *w;
   int64_t xs, ws;  // strides of a row
-  int rows, inner, outer;
+  int rows, inner, outer;  // of x; of both; of w
+  bool swapped;            // w is the map's x and x its weights
   Epilogue e;
 };
 
@@ -78,20 +80,23 @@ __device__ __forceinline__ void parts_of(const Eight<float>& v, uint32_t (&o)[NP
   }
 }
 
-// A lane's ring: the 16-byte pieces of a step, and as many steps as a block of about 100 KB holds.
-template <typename T, int MT, int NT>
+// A lane's ring: the 16-byte pieces of a step, and as many steps as a block of about 100 KB (of sixteen warps, which
+// has an SM to itself, 200) holds. The sums take its place.
+template <typename T, int MT, int NT, int WARPS>
 struct RowRing {
   static constexpr int kEach = sizeof(T) / 2, kPieces = (2 * MT + NT) * kEach;
-  static constexpr int kStep = kPieces * kRowWarps * 32 * 16, kFit = 100 * 1024 / kStep;
+  static constexpr int kStep = kPieces * WARPS * 32 * 16, kFit = (WARPS > 8 ? 200 : 100) * 1024 / kStep;
   static constexpr int kDepth = kFit < 2 ? 2 : kFit > 8 ? 8 : kFit;
-  static constexpr size_t kSmem = (size_t)kDepth * kStep;
+  static constexpr size_t kSums = (size_t)WARPS * 8 * NT * (16 * MT + 1) * sizeof(float);
+  static constexpr size_t kRing = (size_t)kDepth * kStep, kSmem = kRing > kSums ? kRing : kSums;
 };
 
 // MT tiles of 16 outputs, NT of 8 rows.
-template <typename T, int NP, int MT, int NT, bool ALIGNED>
-__global__ void __launch_bounds__(kRowWarps * 32) linear_rows_kernel(const __grid_constant__ RowArgs A) {
+template <typename T, int NP, int MT, int NT, int WARPS, bool ALIGNED>
+__global__ void __launch_bounds__(WARPS * 32) linear_rows_kernel(const __grid_constant__ RowArgs A) {
   constexpr int kOut = 16 * MT, kIn = 8 * NT, LD = kOut + 1;
-  __shared__ float sums[kRowWarps][kIn * LD];
+  extern __shared__ uint4 ring[];  // (steps, pieces, threads), then the warps' sums
+  float* sums = reinterpret_cast<float*>(ring);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int j0 = blockIdx.x * kOut;
   // Outputs that are not there read the last one's: what comes of them is not stored.
@@ -135,15 +140,14 @@ __global__ void __launch_bounds__(kRowWarps * 32) linear_rows_kernel(const __gri
   const int whole = ALIGNED ? A.inner / kRowStep : 0, steps = (A.inner + kRowStep - 1) / kRowStep;
   int s = warp;
   if constexpr (ALIGNED) {
-    using R = RowRing<T, MT, NT>;
-    extern __shared__ uint4 ring[];  // (steps, pieces, threads)
+    using R = RowRing<T, MT, NT, WARPS>;
     const auto fetch = [&](int slot, int step) {
       if (step < whole) {
-        const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring + slot * (R::kPieces * kRowWarps * 32) + threadIdx.x);
+        const uint32_t to = (uint32_t)__cvta_generic_to_shared(ring + slot * (R::kPieces * WARPS * 32) + threadIdx.x);
         const auto piece = [&](int p, const T* from) {
 #pragma unroll
           for (int h = 0; h < R::kEach; ++h)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (p * R::kEach + h) * (kRowWarps * 32 * 16)),
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (p * R::kEach + h) * (WARPS * 32 * 16)),
                          "l"(reinterpret_cast<const uint4*>(from + step * kRowStep) + h * 4 + t)
                          : "memory");
         };
@@ -155,17 +159,17 @@ __global__ void __launch_bounds__(kRowWarps * 32) linear_rows_kernel(const __gri
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    for (int d = 0; d < R::kDepth; ++d) fetch(d, s + d * kRowWarps);
+    for (int d = 0; d < R::kDepth; ++d) fetch(d, s + d * WARPS);
     int slot = 0;
 #pragma unroll 1
-    for (; s < whole; s += kRowWarps) {
+    for (; s < whole; s += WARPS) {
       asm volatile("cp.async.wait_group %0;" ::"n"(R::kDepth - 1) : "memory");
       Eight<T> a[2 * MT], b[NT];
-      const uint4* from = ring + slot * (R::kPieces * kRowWarps * 32) + threadIdx.x;
+      const uint4* from = ring + slot * (R::kPieces * WARPS * 32) + threadIdx.x;
       const auto piece = [&](int p, Eight<T>& v) {
 #pragma unroll
         for (int h = 0; h < R::kEach; ++h) {
-          const uint4 q = from[(p * R::kEach + h) * (kRowWarps * 32)];
+          const uint4 q = from[(p * R::kEach + h) * (WARPS * 32)];
           v.w[4 * h] = q.x;
           v.w[4 * h + 1] = q.y;
           v.w[4 * h + 2] = q.z;
@@ -179,13 +183,13 @@ __global__ void __launch_bounds__(kRowWarps * 32) linear_rows_kernel(const __gri
         b[n] = {};
         if (n * 8 + g < A.rows) piece(2 * MT + n, b[n]);
       }
-      fetch(slot, s + R::kDepth * kRowWarps);
+      fetch(slot, s + R::kDepth * WARPS);
       slot = slot + 1 == R::kDepth ? 0 : slot + 1;
       multiply(a, b);
     }
   }
 #pragma unroll 1
-  for (; s < steps; s += kRowWarps) {  // what is left, and rows off the 16-byte boundaries
+  for (; s < steps; s += WARPS) {  // what is left, and rows off the 16-byte boundaries
     Eight<T> a[2 * MT], b[NT];
     const int k = s * kRowStep, left = A.inner - k;
 #pragma unroll
@@ -194,20 +198,23 @@ __global__ void __launch_bounds__(kRowWarps * 32) linear_rows_kernel(const __gri
     for (int n = 0; n < NT; ++n) b[n] = load_row(x[n] + k, t, left);
     multiply(a, b);
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sums[warp][(n * 8 + t * 2 + (e & 1)) * LD + m * 16 + g + (e >> 1) * 8] = acc[m][n][e];
+      for (int e = 0; e < 4; ++e) sums[warp * (kIn * LD) + (n * 8 + t * 2 + (e & 1)) * LD + m * 16 + g + (e >> 1) * 8] = acc[m][n][e];
   __syncthreads();
-  for (int v = threadIdx.x; v < kOut * kIn; v += kRowWarps * 32) {
+  for (int v = threadIdx.x; v < kOut * kIn; v += WARPS * 32) {
     const int i = v / kOut, o = v % kOut, j = j0 + o;
     if (i >= A.rows || j >= A.outer) continue;
-    float h[1] = {sums[0][i * LD + o]};
+    float h = sums[i * LD + o];
 #pragma unroll
-    for (int k = 1; k < kRowWarps; ++k) h[0] += sums[k][i * LD + o];
-    store_entry<T>(A.e, i, j, A.outer, h[0]);
+    for (int k = 1; k < WARPS; ++k) h += sums[k * (kIn * LD) + i * LD + o];
+    if (A.swapped) store_entry<T>(A.e, j, i, A.rows, h);
+    else store_entry<T>(A.e, i, j, A.outer, h);
   }
 }
 
