@@ -139,6 +139,19 @@ int sort(cudaStream_t s, const fx_embed_args* a, const SortPlan& P, unsigned cha
   S.digits = P.passes == 1 ? (int)a->rows + 1 : 1 << P.bits;
   constexpr size_t each = sizeof(int) + kSortWarps * sizeof(uint16_t);  // a digit's
   const size_t smem = (size_t)(S.digits + 1) * each;
+  if (a->count <= kSortSmall) {
+    int bits = 1;
+    while (a->rows >> bits) ++bits;
+    S.keys_out = lists;
+    S.pos_out = lists + a->count;
+    if (raise_smem(sort_small_kernel, kSmallSmem, kSmallSmem)) return FX_ERR_CUDA;
+    sort_small_kernel<<<1, kSmallThreads, kSmallSmem, s>>>(S, (bits + 7) / 8);
+    sort_start_kernel<<<(unsigned)((a->count + 256) / 256), 256, 0, s>>>(S.keys_out, S.count, start, (int)a->rows);
+    A.keys = S.keys_out;
+    A.pos = S.pos_out;
+    A.start = start;
+    return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+  }
   if (raise_smem(sort_place_kernel, smem, each << (kSortBits + 1))) return FX_ERR_CUDA;
   for (int p = 0; p < P.passes; ++p) {
     S.keys_out = lists + (size_t)(p & 1) * 2 * a->count;

@@ -70,13 +70,14 @@ Cut whole_of(int64_t rows, int64_t cols, int64_t inner) {
 }
 
 // How a launch's n products are cut and ordered (c[0]'s units are the long ones); `ahead` as in lin::Group.
-// - Where the tiles do not fill the device once, k is split so that the parts do, four blocks at least each.
+// - Where the tiles do not fill the device once, k is split so that the parts do, four blocks at least each (two in
+//   float32).
 // - Of one product, the tiles after the whole rounds are split alike, if that saves the time of eight blocks (three in
 //   float32, whose blocks have six products), about what the join costs.
 // - Of two products, the one with the longer tiles is split where a tile takes longer than a pair's share of the work.
 // Measured, us, without and with: 8192 x 8192 -> 2048 bfloat16 (256 tiles of 128 blocks on 74 pairs) 217 and 200.
 int cut(Cut* c, int n, bool f32, int sms) {
-  const int pairs = sms / 2, least = 4;
+  const int pairs = sms / 2, least = f32 ? 2 : 4;
   if (n == 2 && c[1].blocks > c[0].blocks) {
     const Cut t = c[0];
     c[0] = c[1];

@@ -207,6 +207,88 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortArgs A) {
   }
 }
 
+// Up to kSortSmall tokens in one launch: one block, all passes (of 8 bits) in shared memory.
+constexpr int kSmallThreads = 1024, kSmallWarps = kSmallThreads / 32, kSmallRounds = 8, kSmallDigits = 256;
+constexpr int kSortSmall = kSmallThreads * kSmallRounds;
+constexpr size_t kSmallSmem = 2 * kSortSmall * sizeof(int) + kSmallDigits * (sizeof(int) + kSmallWarps * sizeof(uint16_t));
+
+__global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SortArgs A, int passes) {
+  extern __shared__ int keys[];  // and places, the digits' first places, 16-bit counts (warps, digits)
+  __shared__ int sums[kSmallDigits / 32];
+  int *pos = keys + kSortSmall, *first = pos + kSortSmall;
+  uint16_t* at = reinterpret_cast<uint16_t*>(first + kSmallDigits);
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, base = w * (32 * kSmallRounds) + lane;
+  int key[kSmallRounds], from[kSmallRounds];
+#pragma unroll
+  for (int i = 0; i < kSmallRounds; ++i) {
+    from[i] = base + 32 * i;
+    key[i] = from[i] < A.count ? A.tok.key(from[i], A.rows) : -1;
+  }
+  for (int p = 0; p < passes; ++p) {
+    for (int i = threadIdx.x; i < kSmallDigits * kSmallWarps / 2; i += kSmallThreads) reinterpret_cast<int*>(at)[i] = 0;
+    __syncthreads();
+    uint16_t* mine = at + w * kSmallDigits;
+#pragma unroll
+    for (int i = 0; i < kSmallRounds; ++i) {
+      const int d = key[i] < 0 ? -1 : key[i] >> (8 * p) & (kSmallDigits - 1);
+      const unsigned same = __match_any_sync(0xffffffffu, d);
+      if (d >= 0 && lane == __ffs(same) - 1) mine[d] += (uint16_t)__popc(same);
+      __syncwarp();
+    }
+    __syncthreads();
+    int total = 0, s = 0;
+    if (threadIdx.x < kSmallDigits) {
+      for (int i = 0; i < kSmallWarps; ++i) {
+        const int n = at[i * kSmallDigits + threadIdx.x];
+        at[i * kSmallDigits + threadIdx.x] = (uint16_t)total;
+        total += n;
+      }
+      s = total;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += t;
+      }
+      if (lane == 31) sums[w] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x < kSmallDigits) {
+      int run = s - total;
+      for (int i = 0; i < w; ++i) run += sums[i];
+      first[threadIdx.x] = run;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSmallRounds; ++i) {
+      const int d = key[i] < 0 ? -1 : key[i] >> (8 * p) & (kSmallDigits - 1);
+      const unsigned same = __match_any_sync(0xffffffffu, d);
+      int to = 0;
+      if (d >= 0) to = first[d] + mine[d] + __popc(same & ((1u << lane) - 1));
+      __syncwarp();
+      if (d >= 0 && lane == __ffs(same) - 1) mine[d] += (uint16_t)__popc(same);
+      __syncwarp();
+      if (d >= 0) {
+        keys[to] = key[i];
+        pos[to] = from[i];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSmallRounds; ++i)
+      if (base + 32 * i < A.count) {
+        key[i] = keys[base + 32 * i];
+        from[i] = pos[base + 32 * i];
+      }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < kSmallRounds; ++i)
+    if (base + 32 * i < A.count) {
+      A.keys_out[base + 32 * i] = key[i];
+      A.pos_out[base + 32 * i] = from[i];
+    }
+}
+
 // start[v]: the first place of a token >= v in the sorted list; a warp 32 places, each fills the tokens
 // between its own and the one before.
 __global__ void __launch_bounds__(256) sort_start_kernel(const int* keys, int count, int* start, int rows) {
