@@ -158,9 +158,9 @@ struct LinPlan {
 
 // Few rows are bound by the weights' bytes and need no layout (linear_rows.cuh). Measured, us, against the tiles of the
 // tensor cores at 8192 -> 4096: 32 rows bfloat16 24 and 27, float32 99 and 138; 64 rows bfloat16 52 and 26.
-bool few_rows(const fx_linear_args* a) { return a->rows <= 32; }
+bool few_rows(const fx_linear_args* a) { return a->rows <= (a->dtype == FX_F32 ? 64 : 32); }
 // So are few outputs by the rows' bytes, in float32, where the tiles' layout would read and write four times as much.
-bool few_outputs(const fx_linear_args* a) { return a->dtype == FX_F32 && a->outer <= 32; }
+bool few_outputs(const fx_linear_args* a) { return a->dtype == FX_F32 && a->outer <= 64; }
 
 template <typename T, int NP, int MT, int NT, int WARPS>
 int rows_launch(cudaStream_t s, const lin::RowArgs& A, bool al) {
@@ -188,7 +188,9 @@ int rows_forward(cudaStream_t s, const fx_linear_args* a) {
   const bool al = aligned(A.x, A.xs, A.rows, A.inner, sizeof(T)) && aligned(A.w, A.ws, A.outer, A.inner, sizeof(T));
   if (A.rows <= 8) return rows_launch<T, NP, 1, 1, 8>(s, A, al);
   if (A.rows <= 16) return rows_launch<T, NP, 1, 2, 8>(s, A, al);
-  return rows_launch<T, NP, NP == 1 ? 2 : 1, 4, NP == 1 ? 16 : 8>(s, A, al);
+  if (NP == 1 || A.rows <= 32) return rows_launch<T, NP, NP == 1 ? 2 : 1, 4, NP == 1 ? 16 : 8>(s, A, al);
+  if constexpr (NP > 1) return rows_launch<T, NP, 1, 8, 8>(s, A, al);
+  return FX_ERR_SHAPE;
 }
 
 LinPlan plan_fwd(const fx_linear_args* a, int sms) {
