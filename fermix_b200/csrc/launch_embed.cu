@@ -1,6 +1,6 @@
 // Embedding of tokens (token_embedding.cuh): checks, launch shapes, workspace.
-#include "block_host.cuh"
 #include "token_embedding.cuh"
+#include "token_host.cuh"
 
 namespace {
 
@@ -116,12 +116,12 @@ struct SumRuns {
   int operator()() const {
     const int groups = kEmbedThreads / A.tpr;
     const dim3 windows((A.windows + groups - 1) / groups, (unsigned)((A.chunks + A.tpr - 1) / A.tpr));
-    embed_window_kernel<T, E><<<windows, kEmbedThreads, 0, s>>>(A);
+    const int st = launch_next(embed_window_kernel<T, E>, windows, kEmbedThreads, 0, s, A);
+    if (st) return st;
     // the join: a warp for every row of the table, a block for every window that a long run may begin in, as far as the
     // device holds them
     const int64_t blocks = (A.rows + 7) / 8, want = blocks > A.windows ? blocks : A.windows, most = (int64_t)sms * 4;
-    embed_join_kernel<T, E><<<(unsigned)(want < most ? want : most), kEmbedThreads, 0, s>>>(A);
-    return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+    return launch_next(embed_join_kernel<T, E>, (unsigned)(want < most ? want : most), kEmbedThreads, 0, s, A);
   }
 };
 
@@ -146,11 +146,11 @@ int sort(cudaStream_t s, const fx_embed_args* a, const SortPlan& P, unsigned cha
     S.pos_out = lists + a->count;
     if (raise_smem(sort_small_kernel, kSmallSmem, kSmallSmem)) return FX_ERR_CUDA;
     sort_small_kernel<<<1, kSmallThreads, kSmallSmem, s>>>(S, (bits + 7) / 8);
-    sort_start_kernel<<<(unsigned)((a->count + 256) / 256), 256, 0, s>>>(S.keys_out, S.count, start, (int)a->rows);
+    if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
     A.keys = S.keys_out;
     A.pos = S.pos_out;
     A.start = start;
-    return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+    return launch_next(sort_start_kernel, (unsigned)((a->count + 256) / 256), 256, 0, s, S.keys_out, S.count, start, (int)a->rows);
   }
   if (raise_smem(sort_place_kernel, smem, each << (kSortBits + 1))) return FX_ERR_CUDA;
   for (int p = 0; p < P.passes; ++p) {
@@ -158,18 +158,24 @@ int sort(cudaStream_t s, const fx_embed_args* a, const SortPlan& P, unsigned cha
     S.pos_out = S.keys_out + a->count;
     S.shift = p * P.bits;
     S.start = P.passes == 1 ? start : nullptr;
-    sort_count_kernel<<<P.blocks, kSortThreads, S.digits * sizeof(int), s>>>(S);
-    sort_scan_kernel<<<(S.digits + 7) / 8, 256, 0, s>>>(S);
-    sort_place_kernel<<<P.blocks, kSortThreads, smem, s>>>(S);
+    int st = FX_OK;
+    if (p) {
+      st = launch_next(sort_count_kernel, P.blocks, kSortThreads, S.digits * sizeof(int), s, S);
+    } else {  // the call's first: behind everything before it
+      sort_count_kernel<<<P.blocks, kSortThreads, S.digits * sizeof(int), s>>>(S);
+      if (cudaGetLastError() != cudaSuccess) st = FX_ERR_CUDA;
+    }
+    if (!st) st = launch_next(sort_scan_kernel, (S.digits + 7) / 8, 256, 0, s, S);
+    if (!st) st = launch_next(sort_place_kernel, P.blocks, kSortThreads, smem, s, S);
+    if (st) return st;
     S.keys = S.keys_out;
     S.pos = S.pos_out;
   }
-  if (P.passes > 1)
-    sort_start_kernel<<<(unsigned)((a->count + 256) / 256), 256, 0, s>>>(S.keys, S.count, start, (int)a->rows);
   A.keys = S.keys;
   A.pos = S.pos;
   A.start = start;
-  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+  if (P.passes == 1) return FX_OK;
+  return launch_next(sort_start_kernel, (unsigned)((a->count + 256) / 256), 256, 0, s, S.keys, S.count, start, (int)a->rows);
 }
 
 }  // namespace

@@ -1,8 +1,8 @@
 // The linear map with its epilogue (linear_tc.cuh): checks, launch shapes, workspace.
-#include "block_host.cuh"
 #include "linear_rows.cuh"
 #include "linear_tc.cuh"
 #include "tensor_map.cuh"
+#include "token_host.cuh"
 
 namespace {
 
@@ -293,7 +293,7 @@ struct Products {
     return st;
   }
   template <int ACT>
-  int launch(cudaStream_t s, int sms) {
+  int launch(cudaStream_t s, int sms, bool first) {
     constexpr size_t smem = lin::Shape<NP>::kSmem;
     auto kern = lin::linear_tc_kernel<T, NP, ACT>;
     if (raise_smem(kern, smem, smem)) return FX_ERR_CUDA;
@@ -302,23 +302,32 @@ struct Products {
     G.longs = P.products == 2 ? G.p[0].units() : G.p[0].whole;
     G.shorts = units - G.longs;
     G.ahead = P.ahead;
-    kern<<<2 * pairs, lin::kThreads, smem, s>>>(G, M);
+    int st = FX_OK;
+    if (!first) {
+      st = launch_next(kern, 2 * pairs, lin::kThreads, smem, s, G, M);
+    } else {
+      kern<<<2 * pairs, lin::kThreads, smem, s>>>(G, M);
+      if (cudaGetLastError() != cudaSuccess) st = FX_ERR_CUDA;
+    }
+    if (st) return st;
     const int joined = G.p[0].joined() + G.p[1].joined();
     if (joined) {  // fewer tiles than pairs
       constexpr int N = 16 / sizeof(T);
-      if (G.p[0].vec && (P.products == 1 || G.p[1].vec)) lin::linear_join_kernel<T, ACT, N><<<joined * (lin::kTile / N), 256, 0, s>>>(G);
-      else lin::linear_join_kernel<T, ACT, 1><<<joined * lin::kTile, 256, 0, s>>>(G);
+      if (G.p[0].vec && (P.products == 1 || G.p[1].vec))
+        return launch_next(lin::linear_join_kernel<T, ACT, N>, joined * (lin::kTile / N), 256, 0, s, G);
+      return launch_next(lin::linear_join_kernel<T, ACT, 1>, joined * lin::kTile, 256, 0, s, G);
     }
-    return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+    return FX_OK;
   }
-  int launch(cudaStream_t s, int act, int sms) {
+  // `first`: nothing of this call was launched before
+  int launch(cudaStream_t s, int act, int sms, bool first) {
     switch (act) {
-      case FX_ACT_RELU: return launch<FX_ACT_RELU>(s, sms);
-      case FX_ACT_SILU: return launch<FX_ACT_SILU>(s, sms);
-      case FX_ACT_GELU: return launch<FX_ACT_GELU>(s, sms);
-      case FX_ACT_GELU_TANH: return launch<FX_ACT_GELU_TANH>(s, sms);
-      case FX_ACT_TANH: return launch<FX_ACT_TANH>(s, sms);
-      default: return launch<FX_ACT_NONE>(s, sms);
+      case FX_ACT_RELU: return launch<FX_ACT_RELU>(s, sms, first);
+      case FX_ACT_SILU: return launch<FX_ACT_SILU>(s, sms, first);
+      case FX_ACT_GELU: return launch<FX_ACT_GELU>(s, sms, first);
+      case FX_ACT_GELU_TANH: return launch<FX_ACT_GELU_TANH>(s, sms, first);
+      case FX_ACT_TANH: return launch<FX_ACT_TANH>(s, sms, first);
+      default: return launch<FX_ACT_NONE>(s, sms, first);
     }
   }
 };
@@ -337,9 +346,10 @@ struct Prep {
                 (int)(blocks < most ? blocks : most)};
     return {out, rows, cols, ld};
   }
+  bool nothing() const { return A.g.blocks + A.o[0].blocks + A.o[1].blocks == 0; }
   int launch(cudaStream_t s) {
+    if (nothing()) return FX_OK;
     const int blocks = A.g.blocks + A.o[0].blocks + A.o[1].blocks;
-    if (!blocks) return FX_OK;
     lin::linear_prep_kernel<T, NP><<<blocks, 256, 0, s>>>(A);
     return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
   }
@@ -361,7 +371,7 @@ int forward(cudaStream_t s, const fx_linear_args* a, const LinPlan& P, unsigned 
   Products<T, NP> products(P, ws);
   int st = products.set(0, x, false, w, false, {a->activation, a->bias, a->residual, a->residual_stride, a->y, a->slope});
   if (!st) st = prep.launch(s);
-  return st ? st : products.launch(s, a->activation, sms);
+  return st ? st : products.launch(s, a->activation, sms, prep.nothing());
 }
 
 template <typename T, int NP>
@@ -405,10 +415,10 @@ int backward(cudaStream_t s, const fx_linear_args* a, const LinPlan& P, unsigned
     products.G.dbias = a->dbias;
     products.G.sum_blocks = P.blocks;
     products.G.sum_cols = a->outer;
-    return products.launch(s, FX_ACT_NONE, sms);
+    return products.launch(s, FX_ACT_NONE, sms, prep.nothing());
   }
-  if (a->dbias) lin::linear_bias_kernel<T><<<(unsigned)ceil_div(a->outer, 256), 256, 0, s>>>(prep.A.sums, P.blocks, a->outer, a->dbias);
-  return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
+  if (!a->dbias) return FX_OK;
+  return launch_next(lin::linear_bias_kernel<T>, (unsigned)ceil_div(a->outer, 256), 256, 0, s, prep.A.sums, P.blocks, a->outer, a->dbias);
 }
 
 unsigned char* base_of(void* ws) { return reinterpret_cast<unsigned char*>(align256(reinterpret_cast<uintptr_t>(ws))); }

@@ -1,5 +1,5 @@
 // Log probabilities of tokens (token_logprobs.cuh): checks, launch shapes, workspace.
-#include "block_host.cuh"
+#include "token_host.cuh"
 #include "token_logprobs.cuh"
 
 namespace {
@@ -56,7 +56,8 @@ int run(cudaStream_t s, const ProbArgs& A) {
     const int64_t blocks = A.rows * A.parts;
     if (blocks > INT32_MAX) return FX_ERR_SHAPE;
     prob_kernel<T, TOP, kProbWarps><<<(unsigned)blocks, kProbThreads, 0, s>>>(A);
-    if (A.parts > 1) prob_join_kernel<T, TOP><<<(unsigned)A.rows, kProbThreads, 0, s>>>(A);
+    if (cudaGetLastError() != cudaSuccess) return FX_ERR_CUDA;
+    if (A.parts > 1) return launch_next(prob_join_kernel<T, TOP>, (unsigned)A.rows, kProbThreads, 0, s, A);
   }
   return cudaGetLastError() == cudaSuccess ? FX_OK : FX_ERR_CUDA;
 }

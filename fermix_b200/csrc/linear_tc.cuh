@@ -440,6 +440,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   __syncthreads();
   cluster_sync();
   fence_after_sync();
+  wait_for_last();
   const uint32_t tmem = slot;
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   Unit U;
@@ -586,6 +587,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // products' tiles, one after the other.
 template <typename T, int ACT, int N>
 __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ Group H) {
+  wait_for_last();
   constexpr int P = kTile / N;  // pieces of a row
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
   int v = (int)(t / (P * kTile));
@@ -736,6 +738,7 @@ __global__ void __launch_bounds__(256) linear_prep_kernel(const __grid_constant_
 // The sums alone, where no product follows.
 template <typename T>
 __global__ void __launch_bounds__(256) linear_bias_kernel(const float* sums, int blocks, int64_t cols, void* dbias) {
+  wait_for_last();
   bias_sums<T>(sums, blocks, cols, dbias, blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8);
 }
 

@@ -26,6 +26,10 @@ __device__ __forceinline__ void unpack(const Pack<bf16, N>& p, float* x) {
   }
 }
 
+// A launch of the host's launch_next waits here, before it reads or writes anything in memory, until everything before it
+// is done.
+__device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 struct Tokens {
   const void* p;
   int bytes, has_padding;

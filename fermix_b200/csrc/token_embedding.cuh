@@ -105,6 +105,7 @@ __device__ __forceinline__ void sort_load(const SortArgs& A, int (&key)[kSortRou
 __device__ __forceinline__ int sort_digit(const SortArgs& A, int key) { return key < 0 ? -1 : (key >> A.shift) & A.mask; }
 
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortArgs A) {
+  wait_for_last();
   extern __shared__ int hist[];
   const int lane = threadIdx.x & 31;
   for (int d = threadIdx.x; d < A.digits; d += kSortThreads) hist[d] = 0;
@@ -123,6 +124,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortArgs A) {
 
 // Counts of a digit -> first place within the digit for each block; a warp a digit.
 __global__ void __launch_bounds__(256) sort_scan_kernel(SortArgs A) {
+  wait_for_last();
   const int d = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (d >= A.digits) return;
   int* h = A.hist + (int64_t)d * A.blocks;
@@ -144,6 +146,7 @@ __global__ void __launch_bounds__(256) sort_scan_kernel(SortArgs A) {
 // Every token to its place: the digit's first, those of earlier blocks, of the block's earlier warps, of the warp's
 // earlier rounds and lanes.
 __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortArgs A) {
+  wait_for_last();
   extern __shared__ int first[];  // (digits), then 16-bit counts (warps, digits)
   __shared__ int sums[kSortWarps];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, wide = (A.digits + 1) / 2 * 2;
@@ -292,6 +295,7 @@ __global__ void __launch_bounds__(kSmallThreads) sort_small_kernel(SortArgs A, i
 // start[v]: the first place of a token >= v in the sorted list; a warp 32 places, each fills the tokens
 // between its own and the one before.
 __global__ void __launch_bounds__(256) sort_start_kernel(const int* keys, int count, int* start, int rows) {
+  wait_for_last();
   const int lane = threadIdx.x & 31;
   const int64_t base = ((int64_t)blockIdx.x * 256 + threadIdx.x) - lane, i = base + lane;
   const int to = i < count ? keys[i] : rows, from = i == 0 ? -1 : i <= count ? keys[i - 1] : rows;
@@ -326,6 +330,7 @@ __device__ __forceinline__ void embed_write(const EmbedGrad& A, int64_t v, int c
 // A group of tpr threads sums the runs of one window, a piece of the columns a thread.
 template <typename T, int E>
 __global__ void __launch_bounds__(kEmbedThreads, E > 4 ? 3 : 4) embed_window_kernel(EmbedGrad A) {
+  wait_for_last();
   using P = Pack<T, E>;
   const int w = blockIdx.x * (kEmbedThreads / A.tpr) + threadIdx.x / A.tpr;
   const int c = blockIdx.y * A.tpr + (threadIdx.x & (A.tpr - 1));
@@ -393,6 +398,7 @@ __global__ void __launch_bounds__(kEmbedThreads, E > 4 ? 3 : 4) embed_window_ker
 // the windows each.
 template <typename T, int E>
 __global__ void __launch_bounds__(kEmbedThreads) embed_join_kernel(EmbedGrad A) {
+  wait_for_last();
   constexpr int kFew = 4;
   __shared__ float share[kEmbedThreads * E];
   const int lane = threadIdx.x & 31, last_token = (int)A.rows;

@@ -404,6 +404,7 @@ __global__ void __launch_bounds__(kProbThreads, TOP ? 8 : 12) prob_kernel(ProbAr
 // A block a row: its parts in order by stretches of them a warp.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kProbThreads) prob_join_kernel(ProbArgs A) {
+  wait_for_last();
   const int64_t r = blockIdx.x;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   if (A.tok.padded(A.tok.at(r))) return;
