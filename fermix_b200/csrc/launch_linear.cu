@@ -156,15 +156,34 @@ struct LinPlan {
   }
 };
 
-// Few rows are bound by the weights' bytes and need no layout (linear_rows.cuh). Measured, us, against the tiles of the
-// tensor cores at 8192 -> 4096: 32 rows bfloat16 24 and 27, float32 99 and 138; 64 rows bfloat16 52 and 26.
-bool few_rows(const fx_linear_args* a) { return a->rows <= (a->dtype == FX_F32 ? 64 : 32); }
-// So are few outputs by the rows' bytes, in float32, where the tiles' layout would read and write four times as much.
-bool few_outputs(const fx_linear_args* a) { return a->dtype == FX_F32 && a->outer <= 64; }
+// Blocks of 16 outputs and eight warps while there is at most one an SM, of 32 and four warps above (float32; us: 1000 x
+// 4096 x 32 23 and 41, 100000 x 264 x 32 150 and 80).
+bool few_blocks(int64_t narrow, int64_t wide, int sms) { return ceil_div(wide, 16) * ceil_div(narrow, 32) <= sms; }
+
+// Whether the rows' kernel (linear_rows.cuh), which needs no layout, takes the call. In bfloat16 few rows, which are bound
+// by the weights' bytes; measured, us, against the tiles of the tensor cores at 8192 -> 4096: 32 rows 24 and 27, 64 rows
+// 52 and 26.
+// In float32 the tiles' launches cost about 20 us, and their layout reads and writes an operand four times as much; the
+// rows' kernel costs the products of its slower instructions. Both are estimated, us, from times between 100 and 100000
+// of `wide`, 4 and 512 of `narrow` and 32 and 4096 of `inner`. Measured, us, rows and tiles, wide x inner x narrow: 300 x
+// 64 x 100 8 and 16, 300 x 4096 x 32 23 and 27, 129 x 5847 x 30 55 and 27, 4700 x 264 x 64 14 and 27, 4700 x 4096 x 64 61
+// and 98, 10000 x 264 x 100 35 and 31, 1000 x 1024 x 256 23 and 25, 1000 x 1024 x 512 37 and 27, 100000 x 1024 x 16 96 and
+// 354.
+bool by_rows(const fx_linear_args* a, int sms) {
+  if (a->dtype != FX_F32) return a->rows <= 32;
+  const int64_t narrow = a->rows < a->outer ? a->rows : a->outer, wide = a->rows < a->outer ? a->outer : a->rows;
+  const double part = narrow <= 16 ? 0.6 : 1, tiles = (a->inner < 128 ? 17 : 21) + 4.4e-6 * (double)a->inner * (double)(wide + narrow);
+  // rows off the 16-byte boundaries are loaded entry by entry, and not ahead: 79 x 3158 x 1468 53 and 41
+  const double k = (double)a->inner * (a->x_stride % 4 || a->weight_stride % 4 ? 1.6 : 1);
+  if (few_blocks(narrow, wide, sms)) return 7 + part * 0.004 * k < tiles;
+  const double waves = (double)ceil_div(ceil_div(wide, 32) * ceil_div(narrow, 32), sms);
+  const double one = 2.3 + 0.0085 * k, more = waves * (2.3 + 0.0055 * k);
+  return 7 + part * (one > more ? one : more) < tiles;
+}
 
 template <typename T, int NP, int MT, int NT, int WARPS>
 int rows_launch(cudaStream_t s, const lin::RowArgs& A, bool al) {
-  const unsigned blocks = (unsigned)ceil_div(A.outer, 16 * MT);
+  const dim3 blocks((unsigned)ceil_div(A.outer, 16 * MT), (unsigned)ceil_div(A.rows, 8 * NT));
   constexpr size_t smem = lin::RowRing<T, MT, NT, WARPS>::kSmem;
   auto kern = al ? lin::linear_rows_kernel<T, NP, MT, NT, WARPS, true> : lin::linear_rows_kernel<T, NP, MT, NT, WARPS, false>;
   if (raise_smem(kern, smem, smem)) return FX_ERR_CUDA;
@@ -173,10 +192,10 @@ int rows_launch(cudaStream_t s, const lin::RowArgs& A, bool al) {
 }
 
 template <typename T, int NP>
-int rows_forward(cudaStream_t s, const fx_linear_args* a) {
+int rows_forward(cudaStream_t s, const fx_linear_args* a, int sms) {
   lin::RowArgs A{a->x, a->weight, a->x_stride, a->weight_stride, (int)a->rows, (int)a->inner, (int)a->outer, false,
                  {a->activation, a->bias, a->residual, a->residual_stride, a->y, a->slope}};
-  if (!few_rows(a)) {
+  if (NP > 1 && a->outer < a->rows) {
     A.x = a->weight;
     A.w = a->x;
     A.xs = a->weight_stride;
@@ -186,11 +205,20 @@ int rows_forward(cudaStream_t s, const fx_linear_args* a) {
     A.swapped = true;
   }
   const bool al = aligned(A.x, A.xs, A.rows, A.inner, sizeof(T)) && aligned(A.w, A.ws, A.outer, A.inner, sizeof(T));
-  if (A.rows <= 8) return rows_launch<T, NP, 1, 1, 8>(s, A, al);
-  if (A.rows <= 16) return rows_launch<T, NP, 1, 2, 8>(s, A, al);
-  if (NP == 1 || A.rows <= 32) return rows_launch<T, NP, NP == 1 ? 2 : 1, 4, NP == 1 ? 16 : 8>(s, A, al);
-  if constexpr (NP > 1) return rows_launch<T, NP, 1, 8, 8>(s, A, al);
-  return FX_ERR_SHAPE;
+  if constexpr (NP == 1) {
+    if (A.rows <= 8) return rows_launch<T, NP, 1, 1, 8>(s, A, al);
+    if (A.rows <= 16) return rows_launch<T, NP, 1, 2, 8>(s, A, al);
+    return rows_launch<T, NP, 2, 4, 16>(s, A, al);
+  } else if (few_blocks(A.rows, A.outer, sms)) {
+    if (A.rows <= 8) return rows_launch<T, NP, 1, 1, 8>(s, A, al);
+    if (A.rows <= 16) return rows_launch<T, NP, 1, 2, 8>(s, A, al);
+    return rows_launch<T, NP, 1, 4, 8>(s, A, al);
+  } else {
+    if (A.rows <= 8) return rows_launch<T, NP, 2, 1, 4>(s, A, al);
+    // off the boundaries 32 outputs by 16 rows are slow (100000 x 263 x 16 117 us, of 16 outputs 74)
+    if (A.rows <= 16) return al ? rows_launch<T, NP, 2, 2, 4>(s, A, al) : rows_launch<T, NP, 1, 2, 8>(s, A, al);
+    return rows_launch<T, NP, 2, 4, 4>(s, A, al);
+  }
 }
 
 LinPlan plan_fwd(const fx_linear_args* a, int sms) {
@@ -443,7 +471,7 @@ extern "C" {
 
 size_t fermix_linear_workspace_bytes(const fx_linear_args* a) {
   const DevInfo* D = dev_info();
-  return check(a) || !D || few_rows(a) || few_outputs(a) ? 0 : plan_fwd(a, D->sms).bytes;
+  return check(a) || !D || by_rows(a, D->sms) ? 0 : plan_fwd(a, D->sms).bytes;
 }
 
 int fermix_linear(void* stream, const fx_linear_args* a, void* ws, size_t wsb) {
@@ -452,9 +480,9 @@ int fermix_linear(void* stream, const fx_linear_args* a, void* ws, size_t wsb) {
   if (a->rows == 0) return FX_OK;
   if (!a->x || !a->weight || !a->y) return FX_ERR_NULL;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (few_rows(a) || few_outputs(a)) return a->dtype == FX_F32 ? rows_forward<float, 3>(s, a) : rows_forward<bf16, 1>(s, a);
   const DevInfo* D = dev_info();
   if (!D) return FX_ERR_DEVICE;
+  if (by_rows(a, D->sms)) return a->dtype == FX_F32 ? rows_forward<float, 3>(s, a, D->sms) : rows_forward<bf16, 1>(s, a, D->sms);
   const LinPlan P = plan_fwd(a, D->sms);
   if (P.bytes && (!ws || wsb < P.bytes)) return FX_ERR_WORKSPACE;
   return P.f32 ? forward<float, 3>(s, a, P, base_of(ws), D->sms) : forward<bf16, 1>(s, a, P, base_of(ws), D->sms);

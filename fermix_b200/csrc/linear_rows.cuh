@@ -1,12 +1,14 @@
 // The linear map of few rows (a token a walker): bound by the weights' bytes, which are read once, straight into
-// the operand registers of the warps' tensor instructions (m16n8k16: 16 outputs by 8 rows of x). Of few outputs likewise
-// (float32, where the tiles of linear_tc.cuh would read and write x's parts besides): x and the weights change places.
+// the operand registers of the warps' tensor instructions (m16n8k16: 16 outputs by 8 rows of x). Of few outputs, and of
+// small maps, likewise in float32, where the tiles of linear_tc.cuh would read and write both operands' parts besides:
+// where the outputs are fewer than the rows, x and the weights change places.
 //
-// A block has 16 MT outputs and all rows; its WARPS warps share k in steps of 32, and their sums are added in order
-// through shared memory. The order of k within a step is free as long as both operands have it: lane t of a
-// group of four takes entries 8 t .. 8 t + 7 of its row (float32: 4 t .. and 16 + 4 t .., four each), pieces of 16
-// bytes next to its neighbours', which are two instructions' worth of a fragment. Each lane's pieces come through a ring of asynchronous copies of its own: held in registers, the
-// loads of a few steps were not all asked for before the first product, and the weights came at 2 TB/s.
+// A block has 16 MT outputs and 8 NT rows (all of them, up to 32); its WARPS warps share k in steps of 32, and their sums
+// are added in order through shared memory. The order of k within a step is free as long as both operands have it: lane t
+// of a group of four takes entries 8 t .. 8 t + 7 of its row (float32: 4 t .. and 16 + 4 t .., four each), pieces of 16
+// bytes next to its neighbours', which are two instructions' worth of a fragment. Each lane's pieces come through a ring of
+// asynchronous copies of its own: held in registers, the loads of a few steps were not all asked for before the first
+// product, and the weights came at 2 TB/s.
 //
 // float32 is split into three bfloat16 parts in registers, six products as in linear_tc.cuh; the instructions cut
 // off what they add to an accumulator below its last bit, so each step's sum starts from zero and is added with
@@ -81,30 +83,31 @@ __device__ __forceinline__ void parts_of(const Eight<float>& v, uint32_t (&o)[NP
 }
 
 // A lane's ring: the 16-byte pieces of a step, and as many steps as a block of about 100 KB (of sixteen warps, which
-// has an SM to itself, 200) holds. The sums take its place.
+// has an SM to itself, 200; of four, three of which share an SM, 72) holds. The sums take its place.
 template <typename T, int MT, int NT, int WARPS>
 struct RowRing {
   static constexpr int kEach = sizeof(T) / 2, kPieces = (2 * MT + NT) * kEach;
-  static constexpr int kStep = kPieces * WARPS * 32 * 16, kFit = (WARPS > 8 ? 200 : 100) * 1024 / kStep;
+  static constexpr int kStep = kPieces * WARPS * 32 * 16, kFit = (WARPS > 8 ? 200 : WARPS > 4 ? 100 : 72) * 1024 / kStep;
   static constexpr int kDepth = kFit < 2 ? 2 : kFit > 8 ? 8 : kFit;
   static constexpr size_t kSums = (size_t)WARPS * 8 * NT * (16 * MT + 1) * sizeof(float);
   static constexpr size_t kRing = (size_t)kDepth * kStep, kSmem = kRing > kSums ? kRing : kSums;
 };
 
-// MT tiles of 16 outputs, NT of 8 rows.
+// MT tiles of 16 outputs, NT of 8 rows. (16 outputs by 64 rows, whose weights' entries are split twice as often:
+// 4700 x 264 x 64 21 us, so 14.)
 template <typename T, int NP, int MT, int NT, int WARPS, bool ALIGNED>
-__global__ void __launch_bounds__(WARPS * 32) linear_rows_kernel(const __grid_constant__ RowArgs A) {
+__global__ void __launch_bounds__(WARPS * 32, WARPS > 4 ? 1 : 3) linear_rows_kernel(const __grid_constant__ RowArgs A) {
   constexpr int kOut = 16 * MT, kIn = 8 * NT, LD = kOut + 1;
   extern __shared__ uint4 ring[];  // (steps, pieces, threads), then the warps' sums
   float* sums = reinterpret_cast<float*>(ring);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int j0 = blockIdx.x * kOut;
+  const int j0 = blockIdx.x * kOut, i0 = blockIdx.y * kIn, here = min(A.rows - i0, kIn);
   // Outputs that are not there read the last one's: what comes of them is not stored.
   const T *w[2 * MT], *x[NT];
 #pragma unroll
   for (int m = 0; m < 2 * MT; ++m) w[m] = static_cast<const T*>(A.w) + (int64_t)min(j0 + m * 8 + g, A.outer - 1) * A.ws;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) x[n] = static_cast<const T*>(A.x) + (int64_t)min(n * 8 + g, A.rows - 1) * A.xs;
+  for (int n = 0; n < NT; ++n) x[n] = static_cast<const T*>(A.x) + (int64_t)(i0 + min(n * 8 + g, here - 1)) * A.xs;
   float acc[MT][NT][4] = {};
   const auto multiply = [&](const Eight<T> (&a)[2 * MT], const Eight<T> (&b)[NT]) {
     uint32_t ap[2 * MT][NP][4];
@@ -155,7 +158,7 @@ __global__ void __launch_bounds__(WARPS * 32) linear_rows_kernel(const __grid_co
         for (int m = 0; m < 2 * MT; ++m) piece(m, w[m]);
 #pragma unroll
         for (int n = 0; n < NT; ++n)  // (several lanes' copies of one address are slow)
-          if (n * 8 + g < A.rows) piece(2 * MT + n, x[n]);
+          if (n * 8 + g < here) piece(2 * MT + n, x[n]);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -181,7 +184,7 @@ __global__ void __launch_bounds__(WARPS * 32) linear_rows_kernel(const __grid_co
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         b[n] = {};
-        if (n * 8 + g < A.rows) piece(2 * MT + n, b[n]);
+        if (n * 8 + g < here) piece(2 * MT + n, b[n]);
       }
       fetch(slot, s + R::kDepth * WARPS);
       slot = slot + 1 == R::kDepth ? 0 : slot + 1;
@@ -209,12 +212,12 @@ __global__ void __launch_bounds__(WARPS * 32) linear_rows_kernel(const __grid_co
   __syncthreads();
   for (int v = threadIdx.x; v < kOut * kIn; v += WARPS * 32) {
     const int i = v / kOut, o = v % kOut, j = j0 + o;
-    if (i >= A.rows || j >= A.outer) continue;
+    if (i >= here || j >= A.outer) continue;
     float h = sums[i * LD + o];
 #pragma unroll
     for (int k = 1; k < WARPS; ++k) h += sums[k * (kIn * LD) + i * LD + o];
-    if (A.swapped) store_entry<T>(A.e, j, i, A.rows, h);
-    else store_entry<T>(A.e, i, j, A.outer, h);
+    if (A.swapped) store_entry<T>(A.e, j, i0 + i, A.rows, h);
+    else store_entry<T>(A.e, i0 + i, j, A.outer, h);
   }
 }
 

@@ -215,6 +215,30 @@ def test_linear(rows, inner, outer, dtype):
             _within(g, w, e, f"d_{n}, {act}")
 
 
+# float32 on both sides of the sizes where its kernels take turns: groups of 64 of the lesser side, either side the
+# longer one, rows off the 16-byte boundaries; long sums; and tiles cut along them
+@pytest.mark.parametrize("rows,inner,outer", [
+    (65, 40, 65), (130, 263, 300), (300, 264, 129), (1000, 64, 150), (97, 700, 770), (200, 1600, 66), (66, 2049, 70),
+    (70, 2100, 90), (4000, 64, 65), (33, 4097, 2050), (2050, 100, 40), (5000, 60, 33), (4801, 24, 257), (16500, 100, 20)])
+def test_linear_float32_between_kernels(rows, inner, outer):
+    gen = _gen(rows)
+    for act, withbias in ((None, True), ("gelu", False), ("silu", True)):
+        x = _randn(gen, rows, inner).requires_grad_()
+        weight = _randn(gen, outer, inner, scale=1.5 * inner**-0.5).requires_grad_()
+        bias = _randn(gen, outer).requires_grad_() if withbias else None
+        residual = _randn(gen, rows, outer).requires_grad_() if act else None
+        cot = _randn(gen, rows, outer)
+        want, wgrads, err, errs = _bounds(x, weight, bias, act, residual, cot, torch.float32)
+        out = fx.fused_linear(x, weight, bias, activation=act, residual=residual)
+        _within(out, want, err, f"out, {act}")
+        leaves = [t for t in (x, weight, bias, residual) if t is not None]
+        for g, w, e in zip(torch.autograd.grad(out, leaves, cot), wgrads, errs):
+            _within(g, w, e, f"gradient, {act}")
+        wide = _randn(gen, rows, inner + 5)[:, 3:inner + 3]  # another stride, off the boundaries
+        with torch.no_grad():
+            assert torch.equal(fx.fused_linear(wide, weight, bias), fx.fused_linear(wide.contiguous(), weight, bias))
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("rows", [3, 70, 400])
 def test_linear_strided_rows_and_leading_dimensions(rows, dtype):
