@@ -174,7 +174,7 @@ bool by_rows(const fx_linear_args* a, int sms) {
   const int64_t narrow = a->rows < a->outer ? a->rows : a->outer, wide = a->rows < a->outer ? a->outer : a->rows;
   const double part = narrow <= 16 ? 0.6 : 1, tiles = (a->inner < 128 ? 17 : 21) + 4.4e-6 * (double)a->inner * (double)(wide + narrow);
   // rows off the 16-byte boundaries are loaded entry by entry, and not ahead: 79 x 3158 x 1468 53 and 41
-  const double k = (double)a->inner * (a->x_stride % 4 || a->weight_stride % 4 ? 1.6 : 1);
+  const double k = (double)a->inner * ((a->x_stride | a->weight_stride | a->inner) % 4 ? 1.6 : 1);
   if (few_blocks(narrow, wide, sms)) return 7 + part * 0.004 * k < tiles;
   const double waves = (double)ceil_div(ceil_div(wide, 32) * ceil_div(narrow, 32), sms);
   const double one = 2.3 + 0.0085 * k, more = waves * (2.3 + 0.0055 * k);
@@ -249,7 +249,7 @@ LinPlan plan_bwd(const fx_linear_args* a, int sms) {
   while (P.tpr < 32 && P.tpr * 8 < a->outer) P.tpr *= 2;
   const int64_t groups = 256 / P.tpr, strips = ceil_div(a->outer, P.tpr * 8);
   // as many blocks as an SM holds, of four rows a thread at least
-  int64_t blocks = (int64_t)sms * (P.f32 ? 4 : 5) / strips;
+  int64_t blocks = (int64_t)sms * lin::kPrepBlocks / strips;
   if (blocks < 1) blocks = 1;
   if (blocks > ceil_div(a->rows, groups * 4)) blocks = ceil_div(a->rows, groups * 4);
   P.per = ceil_div(a->rows, blocks);

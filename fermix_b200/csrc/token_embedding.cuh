@@ -17,11 +17,6 @@ namespace fx {
 
 constexpr int kEmbedThreads = 256;
 
-template <typename T, int E>
-struct EmbedVec {
-  using P = Pack<T, E>;
-};
-
 struct EmbedFwd {
   Tokens tok;
   const void* weight;

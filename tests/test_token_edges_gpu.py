@@ -160,9 +160,15 @@ def test_a_wait_that_runs_out_is_reported_and_leaves_nan():
     assert _lib.device_status() == 0
     old = L.fermix_set_wait_polls(0)
     try:
-        for dtype in (torch.float32, torch.bfloat16):
-            got = fx.fused_linear(x.to(dtype), w.to(dtype), activation="relu")
+        # a float32 map of this size has no wait that could run out: its kernel keeps its sums in registers
+        assert torch.equal(fx.fused_linear(x, w, activation="relu"), want)
+        assert _lib.device_status() == 0
+        for a, b in ((x.bfloat16(), w.bfloat16()), (x.repeat(8, 1), w.repeat(4, 1))):
+            got = fx.fused_linear(a, b, activation="relu")
             assert torch.isnan(got).any()
+            assert _lib.device_status() == _lib.FX_ERR_TIMEOUT
+            _lib.device_status(clear=True)
+        fx.fused_linear(x.bfloat16(), w.bfloat16())
         assert _lib.device_status(clear=True) == _lib.FX_ERR_TIMEOUT
     finally:
         L.fermix_set_wait_polls(old)
@@ -197,9 +203,14 @@ def test_workspace_too_small_is_an_error():
     a = _lib.LinearArgs()
     a.dtype, a.rows, a.inner, a.outer, a.x_stride, a.weight_stride = _lib.FX_F32, 300, 64, 300, 64, 64
     a.x, a.weight, a.y = x.data_ptr(), w.data_ptr(), y.data_ptr()
+    stream = torch.cuda.current_stream().cuda_stream
+    # a small map needs none
+    assert L.fermix_linear_workspace_bytes(ctypes.byref(a)) == 0
+    assert L.fermix_linear(stream, ctypes.byref(a), None, 0) == 0
+    x, w, y = torch.zeros(2400, 64, device="cuda"), torch.zeros(1200, 64, device="cuda"), torch.zeros(2400, 1200, device="cuda")
+    a.rows, a.outer, a.x, a.weight, a.y = 2400, 1200, x.data_ptr(), w.data_ptr(), y.data_ptr()
     need = L.fermix_linear_workspace_bytes(ctypes.byref(a))
     ws = torch.empty(need, dtype=torch.uint8, device="cuda")
-    stream = torch.cuda.current_stream().cuda_stream
     assert need > 0
     assert L.fermix_linear(stream, ctypes.byref(a), ws.data_ptr(), need - 1) == 4
     assert L.fermix_linear(stream, ctypes.byref(a), None, 0) == 4
