@@ -7,6 +7,7 @@
 //   launch_tc.cu      tensor-memory (tcgen05) kernels, float32 tf32x3
 //   launch_large_*.cu blocked LU / Parlett-Reid engines for n > 256
 //   launch_update.cu  rank-k determinant and one-index Pfaffian moves
+//   launch_embed.cu, launch_linear.cu, launch_logprobs.cu  the operators on tokens
 // Each launcher below is a template defined in one of those files and explicitly
 // instantiated there for the four dtypes; the kernel templates themselves are only
 // instantiated in the file that launches them.

@@ -67,7 +67,7 @@ __device__ __forceinline__ ActOut activate(float h) {
   return o;
 }
 
-// The type the derivative is kept in: IEEE half beside bfloat16 (within +-1.2, 2^-12 of its value
+// The type the derivative is kept in: IEEE half beside bfloat16 (within +-1.2, 2^-11 of its value
 // or 2^-25 where it is small, an eighth of what bfloat16's rounding would leave), float32 beside float32.
 template <typename T>
 struct SlopeOf {
