@@ -494,8 +494,9 @@ __global__ void __launch_bounds__(kProbThreads, 12) prob_grad_kernel(ProbArgs A)
   const bool given = t >= 0 && t < A.entries;
   const float g = A.glogp && given ? A.glogp[r] : 0.f, ent = A.gentropy ? A.gentropy[r] : 0.f;
   const float m = A.stats[r], l2 = A.stats[A.rows + r], c = A.scale * kLog2e;
-  // - scale p (g + e (log p + H)), log p = ln2 q
-  const float gs = -A.scale * (g + ent * A.entropy[r]), es = -A.scale * ent * 0.6931471805599453f, hit = A.scale * g;
+  // - scale p (g + e (log p + H)), log p = ln2 q; a row without an entry of any probability has no hit either
+  const float gs = -A.scale * (g + ent * A.entropy[r]), es = -A.scale * ent * 0.6931471805599453f;
+  const float hit = l2 == INFINITY ? 0.f : A.scale * g;
   const int at = given ? (int)t : -E;  // the token's entry
   int slot = 0;
 #pragma unroll 1

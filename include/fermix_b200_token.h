@@ -82,7 +82,8 @@ size_t fermix_linear_grad_workspace_bytes(const fx_linear_args* args);
  * logits and mask (rows, entries) by the element stride of a row (mask: bytes, 0 leaves the entry
  * out, stride 0: one for all rows; NULL: none). Per row: logp of its token, entropy (in nats),
  * and the `top` <= FX_TOP_MAX likeliest entries, ties to the lowest index, with -inf and index -1
- * behind the last entry of any probability. A row without such an entry has entropy 0; a token
+ * behind the last entry of any probability. A row without such an entry has entropy 0 and
+ * dlogits 0, whether the mask or logits of -inf leave none; a token
  * that is masked or whose logit is -inf has logp -inf. A live NaN or +inf makes the row's numbers
  * NaN and its indices -1. A token equal to `padding` (where has_padding) leaves its row out: logp
  * and entropy 0, top -inf and -1, dlogits 0, whatever the logits hold; any other token outside

@@ -1,0 +1,40 @@
+"""token_logprobs on rows that leave nothing without a mask."""
+
+import math
+
+import pytest
+import torch
+
+import fermix_b200 as fx
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16]
+IDS = ["f32", "bf16"]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("entries", [1, 5, 70, 1024, 1500, 30000])
+@pytest.mark.parametrize("masked", [False, True])
+def test_a_row_without_entries_has_no_gradient(entries, masked, dtype):
+    """Rows of -inf, and rows whose mask leaves only entries of -inf: the same as rows that the mask leaves nothing of."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    logits = torch.randn(6, entries, generator=gen, device="cuda").to(dtype)
+    tokens = torch.randint(0, entries, (6,), generator=gen, device="cuda")
+    empty = [0, 3, 5]
+    logits[empty] = -math.inf
+    mask = None
+    if masked:
+        mask = torch.ones(6, entries, dtype=torch.bool, device="cuda")
+        logits[5, ::2] = 1.0
+        mask[5, ::2] = False  # what is left is -inf, or nothing
+        tokens[5] = entries - 1
+    logits.requires_grad_()
+    lp, ent = fx.token_logprobs(logits, tokens, scale=1.3, mask=mask)
+    assert (lp[empty] == -math.inf).all() and (ent[empty] == 0).all()
+    for cots in ((torch.ones(6, device="cuda"), None), (torch.full((6,), -2.5, device="cuda"), torch.ones(6, device="cuda"))):
+        outs, given = ((lp,), cots[:1]) if cots[1] is None else ((lp, ent), cots)
+        (grad,) = torch.autograd.grad(outs, logits, given, retain_graph=True)
+        assert (grad[empty] == 0).all()
+        if entries > 1:
+            assert all((grad[r] != 0).any() for r in (1, 2, 4))
