@@ -138,9 +138,9 @@ __device__ __forceinline__ void take_best(Best& best, float& last, int top, floa
         e = k;
       }
     if (!(m > last)) m = kNone;  // NaN and what the list has no room for
-    const unsigned key = __reduce_max_sync(0xffffffffu, ordered(m));
+    const unsigned own = ordered(m + 0.f), key = __reduce_max_sync(0xffffffffu, own);  // -0 + 0 is +0: the zeros are equal
     if (key == ordered(kNone)) return;
-    const unsigned mine = ordered(m) == key ? (unsigned)at(e) : 0xffffffffu, j = __reduce_min_sync(0xffffffffu, mine);
+    const unsigned mine = own == key ? (unsigned)at(e) : 0xffffffffu, j = __reduce_min_sync(0xffffffffu, mine);
     const int src = __ffs(__ballot_sync(0xffffffffu, mine == j)) - 1;
     best.insert(__shfl_sync(0xffffffffu, m, src), (int)j);
     last = __shfl_sync(0xffffffffu, best.v, top - 1);

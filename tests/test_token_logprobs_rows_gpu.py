@@ -1,4 +1,4 @@
-"""token_logprobs on rows that leave nothing without a mask."""
+"""token_logprobs on rows that leave nothing without a mask, and ties of signed zeros."""
 
 import math
 
@@ -38,3 +38,24 @@ def test_a_row_without_entries_has_no_gradient(entries, masked, dtype):
         assert (grad[empty] == 0).all()
         if entries > 1:
             assert all((grad[r] != 0).any() for r in (1, 2, 4))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("entries", [9, 40, 700, 1030, 9000, 70001])
+def test_ties_of_signed_zeros_go_to_the_lowest_index(entries, masked, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.full((4, entries), -1.0, device="cuda")
+    x[0, 0], x[0, 8] = -0.0, 0.0  # the later one is the positive zero, in another lane
+    x[1, entries - 1], x[1, entries // 2] = 0.0, -0.0
+    zeros = torch.rand(2, entries, generator=gen, device="cuda")
+    x[2:] = torch.where(zeros < 0.5, -0.0, 0.0)
+    x[3, ::3] = -1.0
+    x = x.to(dtype)
+    mask = torch.rand(4, entries, generator=gen, device="cuda") < 0.9 if masked else None
+    live = x if mask is None else x.masked_fill(~mask, -math.inf)
+    tokens = torch.zeros(4, dtype=torch.int64, device="cuda")
+    for top in (1, 2, 9, 32):
+        got = fx.token_logprobs(x, tokens, mask=mask, top=top)[3][:, :entries]
+        want = torch.sort(live + 0.0, dim=-1, descending=True, stable=True)  # -0 + 0 is +0
+        assert torch.equal(got, want.indices.masked_fill(want.values == -math.inf, -1)[:, :top])
