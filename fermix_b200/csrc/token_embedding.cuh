@@ -92,11 +92,12 @@ struct SortArgs {
   int mask;
 };
 
-__device__ __forceinline__ void sort_load(const SortArgs& A, int (&key)[kSortRounds], int base) {
+// Places behind the last token may pass 2^31 - 1, where the count itself does not: they are unsigned.
+__device__ __forceinline__ void sort_load(const SortArgs& A, int (&key)[kSortRounds], unsigned base) {
 #pragma unroll
   for (int i = 0; i < kSortRounds; ++i) {
-    const int e = base + 32 * i;
-    key[i] = e >= A.count ? -1 : A.keys ? A.keys[e] : A.tok.key(e, A.rows);
+    const unsigned e = base + 32 * i;
+    key[i] = e >= (unsigned)A.count ? -1 : A.keys ? A.keys[e] : A.tok.key(e, A.rows);
   }
 }
 __device__ __forceinline__ int sort_digit(const SortArgs& A, int key) { return key < 0 ? -1 : (key >> A.shift) & A.mask; }
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortArgs A) {
   uint16_t* at = reinterpret_cast<uint16_t*>(first + wide);
   for (int i = threadIdx.x; i < kSortWarps * wide / 2; i += kSortThreads) reinterpret_cast<int*>(at)[i] = 0;
   int key[kSortRounds];
-  const int base = blockIdx.x * kSortTile + w * (32 * kSortRounds) + lane;
+  const unsigned base = blockIdx.x * kSortTile + w * (32 * kSortRounds) + lane;
   sort_load(A, key, base);
   // first places of the digits: a thread sums a run of them
   const int per = (A.digits + kSortThreads - 1) / kSortThreads, d0 = threadIdx.x * per;
@@ -200,9 +201,9 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortArgs A) {
     if (d >= 0 && lane == __ffs(same) - 1) mine[d] += (uint16_t)__popc(same);
     __syncwarp();
     if (d >= 0) {
-      const int e = base + 32 * i;
+      const unsigned e = base + 32 * i;
       A.keys_out[p] = key[i];
-      A.pos_out[p] = A.pos ? A.pos[e] : e;
+      A.pos_out[p] = A.pos ? A.pos[e] : (int)e;
     }
   }
 }
@@ -332,9 +333,10 @@ __global__ void __launch_bounds__(kEmbedThreads, E > 4 ? 3 : 4) embed_window_ker
   const int w = blockIdx.x * (kEmbedThreads / A.tpr) + threadIdx.x / A.tpr;
   const int c = blockIdx.y * A.tpr + (threadIdx.x & (A.tpr - 1));
   if (w >= A.windows || c >= A.chunks) return;
-  const int begin = w << A.shift, end = min(begin + (1 << A.shift), A.count);
+  // unsigned: of the last window the look ahead, and the end of a whole one, may pass 2^31 - 1
+  const unsigned begin = (unsigned)w << A.shift, count = A.count, end = min(begin + (1u << A.shift), count);
   const int before = begin > 0 ? A.keys[begin - 1] : -1;
-  const int after = end < A.count ? A.keys[end] : -1;
+  const int after = end < count ? A.keys[end] : -1;
   float acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
@@ -351,7 +353,7 @@ __global__ void __launch_bounds__(kEmbedThreads, E > 4 ? 3 : 4) embed_window_ker
     }
   };
   int key[kEmbedAhead], pos[kEmbedAhead];  // of the rows to come
-  const auto look = [&](int i) {
+  const auto look = [&](unsigned i) {
 #pragma unroll
     for (int u = 0; u < kEmbedAhead; ++u) {
       key[u] = i + u < end ? A.keys[i + u] : (int)A.rows;
@@ -360,7 +362,7 @@ __global__ void __launch_bounds__(kEmbedThreads, E > 4 ? 3 : 4) embed_window_ker
   };
   look(begin);
   const P* grad = reinterpret_cast<const P*>(A.grad) + c;
-  for (int i = begin; i < end; i += kEmbedAhead) {
+  for (unsigned i = begin; i < end; i += kEmbedAhead) {
     P x[kEmbedAhead];
     int now[kEmbedAhead];
 #pragma unroll
