@@ -32,9 +32,10 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 bool aligned(const void* p, int64_t stride, int64_t rows, int64_t cols, int size) {
   return (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(cols * size) | (uintptr_t)(rows > 1 ? stride * size : 0)) % 16 == 0;
 }
-// bfloat16 rows that a tensor map can read in place (a row of zero stride is one row to it).
-bool mappable(const void* p, int64_t stride, int64_t rows) {
-  return (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(rows > 1 ? stride * 2 : 0)) % 16 == 0 && (rows == 1 || stride > 0) &&
+// bfloat16 rows that a tensor map can read in place. Its rows do not share entries: those of a broadcast (stride 0) or of
+// overlapping windows are laid out anew.
+bool mappable(const void* p, int64_t stride, int64_t rows, int64_t cols) {
+  return (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(rows > 1 ? stride * 2 : 0)) % 16 == 0 && (rows == 1 || stride >= cols) &&
          stride < (int64_t{1} << 38);
 }
 
@@ -225,8 +226,8 @@ LinPlan plan_fwd(const fx_linear_args* a, int sms) {
   LinPlan P{};
   P.f32 = a->dtype == FX_F32;
   P.planes = P.f32 ? 3 : 1;
-  P.new_x = P.f32 || !mappable(a->x, a->x_stride, a->rows);
-  P.new_w = P.f32 || !mappable(a->weight, a->weight_stride, a->outer);
+  P.new_x = P.f32 || !mappable(a->x, a->x_stride, a->rows, a->inner);
+  P.new_w = P.f32 || !mappable(a->weight, a->weight_stride, a->outer, a->inner);
   P.c[P.products++] = whole_of(a->rows, a->outer, a->inner);
   P.ahead = cut(P.c, 1, P.f32, sms);
   Space S;
@@ -242,9 +243,9 @@ LinPlan plan_bwd(const fx_linear_args* a, int sms) {
   P.f32 = a->dtype == FX_F32;
   P.planes = P.f32 ? 3 : 1;
   P.slope = a->activation != FX_ACT_NONE;
-  P.new_x = a->dweight && (P.f32 || !mappable(a->x, a->x_stride, a->rows));
-  P.new_w = a->dx && (P.f32 || !mappable(a->weight, a->weight_stride, a->outer));
-  P.new_g = (a->dx || a->dweight) && (P.f32 || P.slope || !mappable(a->dy, a->dy_stride, a->rows));
+  P.new_x = a->dweight && (P.f32 || !mappable(a->x, a->x_stride, a->rows, a->inner));
+  P.new_w = a->dx && (P.f32 || !mappable(a->weight, a->weight_stride, a->outer, a->inner));
+  P.new_g = (a->dx || a->dweight) && (P.f32 || P.slope || !mappable(a->dy, a->dy_stride, a->rows, a->outer));
   P.tpr = 1;
   while (P.tpr < 32 && P.tpr * 8 < a->outer) P.tpr *= 2;
   const int64_t groups = 256 / P.tpr, strips = ceil_div(a->outer, P.tpr * 8);
@@ -274,7 +275,7 @@ int make_map(CUtensorMap* m, const Operand& o, int planes, bool mn) {
   if (!encode) return FX_ERR_CUDA;
   const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)planes};
   const int64_t ld = o.rows > 1 ? o.ld : ld_of(o.cols);
-  const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, planes > 1 ? (cuuint64_t)(o.rows * ld * 2) : (cuuint64_t)ld * 2};
+  const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)(o.rows * ld * 2)};
   const cuuint32_t box[3] = {64, mn ? 64u : 128u, 1}, ones[3] = {1, 1, 1};
   return encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.p), dims, strides, box, ones,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

@@ -29,3 +29,22 @@ def test_embedding_gradient_of_the_most_tokens(kind, rows):
     assert int((grad != 0).sum()) == 3
     del out, cot, tokens
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows", [7, 70, 400, 2100])
+def test_linear_of_overlapping_windows(rows, dtype):
+    """Rows that share entries (windows of a sequence, 8 and 3 entries apart): the numbers of their copies."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    line = torch.randn(8 * rows + 1200, generator=gen, device="cuda").to(dtype)
+    for hop in (8, 3):
+        x, w = line.unfold(0, 72, hop)[:rows], line[5:].unfold(0, 72, hop)[:130]
+        dy = line[16:].unfold(0, 130, hop)[:rows]
+        assert x.stride() == (hop, 1) and dy.stride() == (hop, 1)
+        results = []
+        for copy in (lambda t: t, lambda t: t.contiguous()):
+            leaves = [copy(t).detach().requires_grad_() for t in (x, w)]
+            y = fx.fused_linear(*leaves, activation="silu")
+            plain = fx.fused_linear(*leaves)
+            results.append((y, plain, *torch.autograd.grad(y, leaves, copy(dy)), *torch.autograd.grad(plain, leaves, copy(dy))))
+        assert all(torch.equal(a, b) for a, b in zip(*results))
