@@ -178,6 +178,12 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
   *state = DEAD;
   return false;
 }
+// The same for a whole warp, whose lanes poll for themselves: instructions that need all of them follow, so they take one
+// way, on where the wait ended for every lane.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* state, uint32_t polls) {
+  return __all_sync(0xffffffffu, wait(bar, parity, state, polls));
+}
+__device__ __forceinline__ bool warp_runs(volatile int* state) { return __all_sync(0xffffffffu, *state != DEAD); }
 
 // ---------------------------------------------------------------- epilogue
 // NaN in the place of sums that a wait did not end for.
@@ -493,7 +499,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (rank == 0) {
       int st = 0, ch = 0;
       uint32_t phase = 0;
-      for (int n = 0; state != DEAD && unit_of(G, pair, pairs, n, U); ++n) {
+      for (int n = 0; warp_runs(&state) && unit_of(G, pair, pairs, n, U); ++n) {
         const bool a_mn = G.p[U.q].a_mn, b_mn = G.p[U.q].b_mn;
         const uint32_t idesc = 1u << 4 | 1u << 7 | 1u << 10 | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
                                (uint32_t)(kTile >> 3) << 17 | (uint32_t)(kTile >> 4) << 24;
@@ -501,12 +507,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const uint64_t a0 = desc(smem_u32(sm), a_mn), b0 = desc(smem_u32(sm) + NP * kOperand, b_mn);
         for (int k0 = U.first; k0 < U.last; k0 += chunk, ++ch) {
           const int buf = ch % 2;
-          if (!wait(&sum_empty[buf], (ch / 2 & 1) ^ 1, &state, G.polls)) break;
+          if (!wait_warp(&sum_empty[buf], (ch / 2 & 1) ^ 1, &state, G.polls)) break;
           fence_after_sync();
           const uint32_t d = tmem + buf * kTile;
           const int k1 = min(k0 + chunk, U.last);
           for (int kb = k0; kb < k1; ++kb) {
-            if (!wait(&full[st], phase, &state, G.polls)) break;
+            if (!wait_warp(&full[st], phase, &state, G.polls)) break;
             fence_after_sync();
             if (elected()) {
               const uint64_t a1 = a0 + (uint32_t)(st * (S::kStage >> 4)), b1 = b0 + (uint32_t)(st * (S::kStage >> 4));
@@ -542,11 +548,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     unsigned char* stage = sm + ST * S::kStage + (warp - 2) * S::kBlock;
     const uint32_t lanes = tmem + ((uint32_t)quarter << 21) + col;
     int ch = 0;
-    for (int n = 0; state != DEAD && unit_of(G, pair, pairs, n, U); ++n) {
+    for (int n = 0; warp_runs(&state) && unit_of(G, pair, pairs, n, U); ++n) {
       float acc[NP == 1 ? 1 : B][C];
       for (int k0 = U.first; k0 < U.last; k0 += chunk, ++ch) {
         const int buf = ch % 2;
-        if (!wait(&sum_full[buf], ch / 2 & 1, &state, G.polls)) break;
+        if (!wait_warp(&sum_full[buf], ch / 2 & 1, &state, G.polls)) break;
         fence_after_sync();
         const uint32_t from = lanes + buf * kTile;
         const bool last = NP == 1 || k0 + chunk >= U.last;
