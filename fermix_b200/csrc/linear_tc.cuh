@@ -164,7 +164,7 @@ __device__ __forceinline__ uint64_t desc(uint32_t saddr, bool mn) {
 
 // A bounded wait. One that runs out is recorded (the block's outputs become NaN) and waits once
 // more, with a limit of its own, so that nothing is under way that the block does not know of; if that
-// runs out too, the block's threads wait and issue no more.
+// runs out too, the block's threads wait and issue no more, and its tiles are filled with NaN.
 enum { RUNS = 0, LATE = 1, DEAD = 2 };
 constexpr uint32_t kLastPolls = 1u << 22;
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* state, uint32_t polls) {
@@ -422,6 +422,27 @@ __device__ __forceinline__ void bias_sums(const float* sums, int blocks, int64_t
   }
 }
 
+// NaN for a block's 128 rows of its units, by the epilogue's warps. (Not inlined: its registers would be the epilogue's.)
+template <typename T>
+__device__ __noinline__ void fill_nan(const Group& G, int first_row) {
+  using TS = typename SlopeOf<T>::type;
+  const float nan = __int_as_float(0x7fc00000);
+  Unit U;
+  for (int n = 0; unit_of(G, blockIdx.x >> 1, gridDim.x >> 1, n, U); ++n) {
+    const Args& A = G.p[U.q];
+    for (int e = threadIdx.x - 64; e < kHalf * kTile; e += 32 * kWarps) {
+      const int r = first_row + e / kTile, c = e % kTile;
+      const int64_t i = (int64_t)U.m * kTile + r, j = (int64_t)U.n * kTile + c;
+      if (U.part >= 0) {
+        A.part[((int64_t)U.part * kTile + r) * kTile + c] = nan;
+      } else if (i < A.rows && j < A.cols) {
+        static_cast<T*>(A.e.y)[i * A.cols + j] = from_f<T>(nan);
+        if (A.e.slope) static_cast<TS*>(A.e.slope)[i * A.cols + j] = from_f<TS>(nan);
+      }
+    }
+  }
+}
+
 template <typename T, int NP, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     linear_tc_kernel(const __grid_constant__ Group G, const __grid_constant__ Maps M) {
@@ -591,6 +612,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   cluster_sync();
   fence_after_sync();
   if (warp == 2) dealloc_pair(tmem);
+  if (warp >= 2 && state == DEAD) fill_nan<T>(G, rank * kHalf);
 }
 
 // ---------------------------------------------------------------- around the products
