@@ -510,7 +510,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
       }
-      // after a wait that ran out: the copies asked for, with a bound
+      // after a wait that ran out: the copies asked for, with a bound (the second block's are counted by the first's
+      // barriers: it waits its limit)
       if (state == DEAD)
         for (int j = it > ST ? it - ST : 0; j < it; ++j) mbar_wait(&full[j % ST], j / ST & 1, 1u << 20);
     }
@@ -518,7 +519,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // -------------------------------------------------------- products, one warp of the pair
     // The whole warp runs the loops, so that descriptors stay in uniform registers, and one lane issues.
     if (rank == 0) {
-      int st = 0, ch = 0;
+      int st = 0, ch = 0, issued = 0;  // blocks of k
       uint32_t phase = 0;
       for (int n = 0; warp_runs(&state) && unit_of(G, pair, pairs, n, U); ++n) {
         const bool a_mn = G.p[U.q].a_mn, b_mn = G.p[U.q].b_mn;
@@ -551,6 +552,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               if (kb == k1 - 1) commit_pair(&sum_full[buf]);
             }
             __syncwarp();
+            ++issued;
             if (++st == ST) {
               st = 0;
               phase ^= 1;
@@ -558,7 +560,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
       }
-      if (state == DEAD && ch > 0) mbar_wait(&sum_full[(ch - 1) % 2], (ch - 1) / 2 & 1, 1u << 20);
+      // after a wait that ran out: the products issued, which read shared memory and write TMEM, with a bound
+      if (!warp_runs(&state))
+        for (int j = issued > ST ? issued - ST : 0; j < issued; ++j) mbar_wait(&empty[j % ST], j / ST & 1, 1u << 20);
     }
   } else {
     // -------------------------------------------------------- epilogue
