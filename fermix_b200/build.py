@@ -20,6 +20,7 @@ OUT_DIR = os.path.join(HERE, "_lib")
 OBJ_DIR = os.path.join(OUT_DIR, "obj")
 OUT = os.path.join(OUT_DIR, "libfermix_b200.so")
 BINDING = os.path.join(CSRC, "torch_binding.cpp")
+BINDING_OBJ = os.path.join(OBJ_DIR, "torch_binding.o")
 BINDING_OUT = os.path.join(OUT_DIR, "fermix_torch.so")
 INCLUDE = os.path.join(ROOT, "include")
 
@@ -83,7 +84,7 @@ def _compile_binding(verbose):
 
     root = os.path.join(os.path.dirname(torch.__file__), "include")
     cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())) if os.path.sep in _nvcc() else "/usr/local/cuda", "include")
-    obj = os.path.join(OBJ_DIR, "torch_binding.o")
+    obj = BINDING_OBJ
     _run(["g++", "-O2", "-std=c++17", "-fPIC", "-c", "-DTORCH_EXTENSION_NAME=fermix_torch",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-I", INCLUDE, "-isystem", root, "-isystem",
           os.path.join(root, "torch", "csrc", "api", "include"), "-isystem", cuda, "-isystem",
@@ -94,7 +95,7 @@ def _compile_binding(verbose):
 def _link_binding(verbose):
     import torch
 
-    _run(["g++", "-shared", "-o", BINDING_OUT + ".tmp", os.path.join(OBJ_DIR, "torch_binding.o"),
+    _run(["g++", "-shared", "-o", BINDING_OUT + ".tmp", BINDING_OBJ,
           "-L", os.path.join(os.path.dirname(torch.__file__), "lib"), "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python",
           "-lc10_cuda", "-ltorch_cuda", "-L", OUT_DIR, "-l:libfermix_b200.so", "-Wl,-rpath,$ORIGIN"],
          os.path.basename(BINDING_OUT), verbose)
@@ -114,21 +115,20 @@ def build(force=False, verbose=False, jobs=None):
     os.makedirs(OBJ_DIR, exist_ok=True)
     hdr = headers() + [os.path.abspath(__file__)]
     todo = [cu for cu in units() if force or _stale(_obj(cu), [cu] + hdr)]
-    bind = force or _stale(os.path.join(OBJ_DIR, "torch_binding.o"), _binding_deps())
+    bind = force or _stale(BINDING_OBJ, _binding_deps())
     jobs = jobs or max(1, min(len(todo) + bind, os.cpu_count() or 1))
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as ex:
         work = [ex.submit(_compile_binding, verbose)] if bind else []
         work += [ex.submit(_compile, cu, verbose) for cu in todo]
         for f in work:
             f.result()
-    if force or todo or _stale(OUT, sources()):
-        objs = [_obj(cu) for cu in units()]
+    # what a call that failed half way has left is linked by the next: by the objects' times, not by what this call compiled
+    objs = [_obj(cu) for cu in units()]
+    if force or _stale(OUT, objs + sources()):
         _run([_nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", OUT + ".tmp", *objs], os.path.basename(OUT), verbose)
         os.replace(OUT + ".tmp", OUT)
-    if force or bind or not os.path.exists(BINDING_OUT):
+    if force or _stale(BINDING_OUT, [BINDING_OBJ] + _binding_deps()):
         _link_binding(verbose)
-    for path in (OUT, BINDING_OUT):  # both at least as new as what they come from
-        os.utime(path)
     return OUT
 
 
