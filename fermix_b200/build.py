@@ -22,6 +22,7 @@ OUT = os.path.join(OUT_DIR, "libfermix_b200.so")
 BINDING = os.path.join(CSRC, "torch_binding.cpp")
 BINDING_OBJ = os.path.join(OBJ_DIR, "torch_binding.o")
 BINDING_OUT = os.path.join(OUT_DIR, "fermix_torch.so")
+BINDING_FOR = BINDING_OUT + ".for"  # the torch and the Python that it was built for
 INCLUDE = os.path.join(ROOT, "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -63,8 +64,23 @@ def _binding_deps():
     return [BINDING, os.path.abspath(__file__)] + glob.glob(os.path.join(INCLUDE, "*.h"))
 
 
+def _installed():
+    import torch
+
+    return f"torch {torch.__version__}, C++11 ABI {int(torch.compiled_with_cxx11_abi())}, {sys.implementation.cache_tag}"
+
+
+def _binding_for():
+    try:
+        with open(BINDING_FOR) as f:
+            return f.read()
+    except OSError:
+        return None
+
+
 def up_to_date():
-    return not _stale(OUT, sources() + [os.path.abspath(__file__)]) and not _stale(BINDING_OUT, _binding_deps())
+    return (not _stale(OUT, sources() + [os.path.abspath(__file__)]) and not _stale(BINDING_OUT, _binding_deps()) and
+            _binding_for() == _installed())
 
 
 def _run(cmd, name, verbose):
@@ -115,7 +131,8 @@ def build(force=False, verbose=False, jobs=None):
     os.makedirs(OBJ_DIR, exist_ok=True)
     hdr = headers() + [os.path.abspath(__file__)]
     todo = [cu for cu in units() if force or _stale(_obj(cu), [cu] + hdr)]
-    bind = force or _stale(BINDING_OBJ, _binding_deps())
+    other = _binding_for() != _installed()  # until a module of the installed torch is linked
+    bind = force or other or _stale(BINDING_OBJ, _binding_deps())
     jobs = jobs or max(1, min(len(todo) + bind, os.cpu_count() or 1))
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as ex:
         work = [ex.submit(_compile_binding, verbose)] if bind else []
@@ -127,8 +144,10 @@ def build(force=False, verbose=False, jobs=None):
     if force or _stale(OUT, objs + sources()):
         _run([_nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", "-o", OUT + ".tmp", *objs], os.path.basename(OUT), verbose)
         os.replace(OUT + ".tmp", OUT)
-    if force or _stale(BINDING_OUT, [BINDING_OBJ] + _binding_deps()):
+    if force or other or _stale(BINDING_OUT, [BINDING_OBJ] + _binding_deps()):
         _link_binding(verbose)
+        with open(BINDING_FOR, "w") as f:
+            f.write(_installed())
     return OUT
 
 

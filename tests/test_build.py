@@ -21,7 +21,7 @@ class Tree:
         out, obj = path / "lib", path / "lib" / "obj"
         for name, value in dict(CSRC=path / "csrc", INCLUDE=path / "include", OUT_DIR=out, OBJ_DIR=obj, OUT=out / "library.so",
                                 BINDING=path / "csrc" / "torch_binding.cpp", BINDING_OBJ=obj / "torch_binding.o",
-                                BINDING_OUT=out / "binding.so", __file__=path / "csrc" / "all.cuh").items():
+                                BINDING_OUT=out / "binding.so", BINDING_FOR=out / "binding.for", __file__=path / "csrc" / "all.cuh").items():
             monkeypatch.setattr(build, name, str(value), raising=False)
         monkeypatch.setattr(build, "_run", self.run)
         for f in self.files:
@@ -85,3 +85,18 @@ def test_a_build_after_one_that_failed_links_all_that_was_compiled(tree, changed
     assert build.up_to_date()
     for out in (build.OUT, build.BINDING_OUT):  # written after the change, not marked as new
         assert int(open(out).read()) > since
+
+
+def test_another_torch_needs_another_binding(tree, monkeypatch):
+    tree.build()
+    monkeypatch.setattr(build, "_installed", lambda: "another torch")
+    assert not build.up_to_date()
+    tree.failing = {"binding.so"}
+    with pytest.raises(RuntimeError):
+        tree.build()
+    assert not build.up_to_date()  # the module of the torch before is still there
+    tree.failing = set()
+    assert tree.build() == {"torch_binding.cpp", "binding.so"}
+    assert build.up_to_date() and tree.build() == set()
+    os.remove(build.BINDING_FOR)
+    assert not build.up_to_date() and tree.build() == {"torch_binding.cpp", "binding.so"}
