@@ -33,9 +33,9 @@ bool aligned(const void* p, int64_t stride, int64_t rows, int64_t cols, int size
   return (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(cols * size) | (uintptr_t)(rows > 1 ? stride * size : 0)) % 16 == 0;
 }
 // bfloat16 rows that a tensor map can read in place. Its rows do not share entries: those of a broadcast (stride 0) or of
-// overlapping windows are laid out anew.
+// overlapping windows are laid out anew. A query of the workspace may leave the pointer out: the form that needs more.
 bool mappable(const void* p, int64_t stride, int64_t rows, int64_t cols) {
-  return (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(rows > 1 ? stride * 2 : 0)) % 16 == 0 && (rows == 1 || stride >= cols) &&
+  return p && (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(rows > 1 ? stride * 2 : 0)) % 16 == 0 && (rows == 1 || stride >= cols) &&
          stride < (int64_t{1} << 38);
 }
 

@@ -53,7 +53,9 @@ size_t fermix_token_embedding_grad_workspace_bytes(const fx_embed_args* args);
  * for FX_BF16 (a derivative lies within +-1.2 and needs more bits, not more range), float32
  * for FX_F32. The backward computes the gradients whose pointers are given: with
  * g = dy act'(h), dx = g W, dweight = g^T x, dbias = the sum of g over the rows. rows, inner and
- * outer < 2^30. */
+ * outer < 2^30. The workspace depends on sizes, types, strides, the alignment of x, weight and dy, and on
+ * which gradients are asked for (dx, dweight, dbias not NULL): the queries read all of these from the call's
+ * own arguments. x, weight and dy that are NULL in a query count as off every alignment, which is enough for any. */
 #define FX_ACT_NONE 0
 #define FX_ACT_RELU 1
 #define FX_ACT_SILU 2

@@ -1,9 +1,12 @@
 """The operators on tokens at the ends of what they accept."""
 
+import ctypes
+
 import pytest
 import torch
 
 import fermix_b200 as fx
+from fermix_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +51,35 @@ def test_linear_of_overlapping_windows(rows, dtype):
             plain = fx.fused_linear(*leaves)
             results.append((y, plain, *torch.autograd.grad(y, leaves, copy(dy)), *torch.autograd.grad(plain, leaves, copy(dy))))
         assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("kind", [_lib.FX_F32, _lib.FX_BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,inner,outer", [(700, 136, 264), (2400, 136, 1208)])
+def test_linear_workspace_asked_for_without_pointers(rows, inner, outer, kind):
+    """A query without operands covers operands anywhere: what the call itself needs is never more, and it runs."""
+    L, dtype = _lib.lib(), {_lib.FX_F32: torch.float32, _lib.FX_BF16: torch.bfloat16}[kind]
+    stream = torch.cuda.current_stream().cuda_stream
+    made = [torch.randn(n + 1, device="cuda").to(dtype) for n in (rows * inner, outer * inner, rows * outer)]
+    outs = [torch.empty(n, dtype=dtype, device="cuda") for n in (rows * outer, rows * inner, outer * inner, outer)]
+    a = _lib.LinearArgs()
+    a.dtype, a.rows, a.inner, a.outer = kind, rows, inner, outer
+    a.x_stride, a.weight_stride, a.dy_stride = inner, inner, outer
+    asked = L.fermix_linear_workspace_bytes(ctypes.byref(a))
+    a.dx, a.dweight, a.dbias = (t.data_ptr() for t in outs[1:])
+    asked_grad = L.fermix_linear_grad_workspace_bytes(ctypes.byref(a))
+    assert asked_grad > 0
+    assert asked > 0 or (kind == _lib.FX_F32 and rows == 700)  # a small float32 map needs none
+    for off in (0, 1):
+        a.x, a.weight, a.dy = (t[off:].data_ptr() for t in made)
+        a.y = outs[0].data_ptr()
+        assert L.fermix_linear_workspace_bytes(ctypes.byref(a)) <= asked
+        assert L.fermix_linear_grad_workspace_bytes(ctypes.byref(a)) <= asked_grad
+        ws = torch.empty(max(asked, asked_grad), dtype=torch.uint8, device="cuda")
+        assert L.fermix_linear(stream, ctypes.byref(a), ws.data_ptr(), asked) == 0
+        assert L.fermix_linear_grad(stream, ctypes.byref(a), ws.data_ptr(), asked_grad) == 0
+        x, w, dy = (t[off:off + n].view(-1, c) for t, n, c in zip(made, (rows * inner, outer * inner, rows * outer),
+                                                                   (inner, inner, outer)))
+        leaves = [t.clone().requires_grad_() for t in (x, w)]
+        y = fx.fused_linear(*leaves, bias := torch.zeros(outer, dtype=dtype, device="cuda", requires_grad=True))
+        want = (y, *torch.autograd.grad(y, (*leaves, bias), dy.clone()))
+        assert all(torch.equal(got, w.reshape(-1)) for got, w in zip(outs, want))
