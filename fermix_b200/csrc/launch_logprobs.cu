@@ -6,12 +6,15 @@ namespace {
 
 using namespace fxh;
 
+// Below it a difference of two logits may pass float32's range and still count, and the scale itself would be lost.
+constexpr float kLeastScale = 1e-30f;
+
 int check(const fx_logprobs_args* a) {
   if (!a) return FX_ERR_NULL;
   if (a->dtype != FX_F32 && a->dtype != FX_BF16) return FX_ERR_DTYPE;
   if (a->token_bytes != 1 && a->token_bytes != 2 && a->token_bytes != 4 && a->token_bytes != 8) return FX_ERR_DTYPE;
   if (a->rows < 0 || a->rows >= INT32_MAX || a->entries < 1 || a->entries > FX_LOGPROBS_MAX || a->top < 0 ||
-      a->top > FX_TOP_MAX || !(a->scale > 0.f) || a->scale > 1e30f || a->logits_stride < 0 || a->mask_stride < 0)
+      a->top > FX_TOP_MAX || !(a->scale >= kLeastScale) || a->scale > 1e30f || a->logits_stride < 0 || a->mask_stride < 0)
     return FX_ERR_SHAPE;
   return FX_OK;
 }

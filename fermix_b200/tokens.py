@@ -13,8 +13,6 @@ is no CPU path and no fallback. None of this has a counterpart in the reference,
 brings the network.
 """
 
-import math
-
 import torch
 
 from . import _lib
@@ -107,7 +105,7 @@ def token_logprobs(logits, tokens, *, scale=1.0, mask=None, top=0, padding=None)
     such an entry has entropy 0 and no gradient; a token that is masked, or whose logit is -inf, has
     logp -inf. A live NaN or +inf gives NaN (and indices -1) in its row. A token equal to ``padding``
     leaves its row out: logp and entropy 0, no alternatives, no gradient; any other token outside
-    [0, entries) has logp NaN and no gradient through it. ``scale`` (an inverse temperature) is positive.
+    [0, entries) has logp NaN and no gradient through it. ``scale`` (an inverse temperature) is from 1e-30 to 1e30.
 
     Differentiable in ``logits`` through logp and entropy."""
     if _transformed():
@@ -130,6 +128,6 @@ def token_logprobs(logits, tokens, *, scale=1.0, mask=None, top=0, padding=None)
     if not isinstance(top, int) or isinstance(top, bool) or not 0 <= top <= _lib.FX_TOP_MAX:
         raise ValueError(f"top must be a whole number from 0 to {_lib.FX_TOP_MAX}, got {top!r}")
     scale = float(scale)
-    if not 0 < scale <= 1e30 or not math.isfinite(scale):
-        raise ValueError(f"scale must be positive and at most 1e30, got {scale}")
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"scale must be from 1e-30 to 1e30, got {scale}")
     return tuple(_lib.binding().token_logprobs(logits, tokens, mask, scale, *_padding(padding), top))

@@ -89,7 +89,7 @@ size_t fermix_linear_grad_workspace_bytes(const fx_linear_args* args);
  * that is masked or whose logit is -inf has logp -inf. A live NaN or +inf makes the row's numbers
  * NaN and its indices -1. A token equal to `padding` (where has_padding) leaves its row out: logp
  * and entropy 0, top -inf and -1, dlogits 0, whatever the logits hold; any other token outside
- * [0, entries) has logp NaN and no gradient through it. scale > 0. stats (2, rows): written where
+ * [0, entries) has logp NaN and no gradient through it. 1e-30 <= scale <= 1e30. stats (2, rows): written where
  * not NULL, read by the backward with entropy: dlogits = scale (grad_logp (hit - p) -
  * grad_entropy p (log p + entropy)), 0 where masked; grad_logp and grad_entropy may be NULL. */
 #define FX_TOP_MAX 32

@@ -59,3 +59,20 @@ def test_ties_of_signed_zeros_go_to_the_lowest_index(entries, masked, dtype):
         got = fx.token_logprobs(x, tokens, mask=mask, top=top)[3][:, :entries]
         want = torch.sort(live + 0.0, dim=-1, descending=True, stable=True)  # -0 + 0 is +0
         assert torch.equal(got, want.indices.masked_fill(want.values == -math.inf, -1)[:, :top])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_scales_at_their_ends(dtype):
+    """Logits over the whole range of the type at the least and the largest scale; scales outside are refused by name."""
+    x = torch.tensor([[-3e38, 3e38, 0.0, 1e30, -math.inf], [1.0, 1.0 + 2.0**-7, 0.0, -1.0, 1.0]], device="cuda").to(dtype)
+    t = torch.tensor([1, 1], device="cuda")
+    for scale in (1e-30, 1e30):
+        lp, ent, best, index = fx.token_logprobs(x, t, scale=scale, top=2)
+        assert lp[0] == 0 and ent[0] == 0 and best[0].tolist()[0] == 0 and index[0].tolist() == [1, 3]
+        if scale > 1:
+            assert lp[1] == 0 and ent[1] == 0 and index[1].tolist() == [1, 0]
+        else:  # even odds
+            assert (lp[1] + math.log(5)).abs() <= 2.0**-20 and (ent[1] - math.log(5)).abs() <= 2.0**-20
+    for scale in (9e-31, 1e-44, 1e-60, 1.1e30):
+        with pytest.raises(ValueError, match="scale"):
+            fx.token_logprobs(x, t, scale=scale)
