@@ -71,11 +71,11 @@ def _refuse_transforms(**tensors):
         if not isinstance(t, torch.Tensor):
             continue
         if torch._C._functorch.is_functorch_wrapped_tensor(t):
-            raise NotImplementedError(f"{name} is inside a torch.func transform (vmap, jvp, grad): the attention-block "
-                                      "operators support reverse-mode autograd only")
+            raise NotImplementedError(f"{name} is inside a torch.func transform (vmap, jvp, grad): the operators of "
+                                      "fermix_b200's networks support reverse-mode autograd only")
         if level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
-            raise NotImplementedError(f"{name} carries a tangent: the attention-block operators have no forward-mode "
-                                      "derivative")
+            raise NotImplementedError(f"{name} carries a tangent: the operators of fermix_b200's networks have no "
+                                      "forward-mode derivative")
 
 
 def _tensor(t, name, like=None):
