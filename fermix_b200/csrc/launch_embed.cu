@@ -188,7 +188,7 @@ int fermix_token_embedding(void* stream, const fx_embed_args* a) {
   if (a->count == 0) return FX_OK;
   if (!a->tokens || !a->weight || !a->out) return FX_ERR_NULL;
   const Shape h = shape_of(a, a->weight, a->out);
-  EmbedFwd A{tokens_of(a), a->weight, a->out, a->count, a->rows, a->width, h.chunks, h.tpr, a->scale};
+  EmbedFwd A{tokens_of(a), a->weight, a->out, a->count, a->rows, h.chunks, h.tpr, a->scale};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return by_piece(a->dtype, h.entries, Fwd{s, A});
 }

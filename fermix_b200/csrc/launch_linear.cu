@@ -340,7 +340,7 @@ struct Products {
     }
     if (st) return st;
     const int joined = G.p[0].joined() + G.p[1].joined();
-    if (joined) {  // fewer tiles than pairs
+    if (joined) {  // tiles that are cut along k
       constexpr int N = 16 / sizeof(T);
       if (G.p[0].vec && (P.products == 1 || G.p[1].vec))
         return launch_next(lin::linear_join_kernel<T, ACT, N>, joined * (lin::kTile / N), 256, 0, s, G);

@@ -6,12 +6,7 @@
 
 namespace fx {
 
-// 2^x and 1 / x, to 2^-22 of the value.
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+// 1 / x, to 2^-22 of the value.
 __device__ __forceinline__ float fast_inverse(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -26,6 +26,13 @@ __device__ __forceinline__ void unpack(const Pack<bf16, N>& p, float* x) {
   }
 }
 
+// 2^x, to 2^-22 of the value.
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // A launch of the host's launch_next waits here, before it reads or writes anything in memory, until everything before it
 // is done.
 __device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

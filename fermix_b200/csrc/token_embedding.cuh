@@ -23,7 +23,7 @@ struct EmbedFwd {
   Tokens tok;
   const void* weight;
   void* out;
-  int64_t count, rows, width;
+  int64_t count, rows;
   int chunks, tpr;  // pieces of a row; threads of a row (a power of two)
   float scale;
 };

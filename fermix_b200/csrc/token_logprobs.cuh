@@ -42,12 +42,6 @@ struct ProbArgs {
   void* dlogits;
 };
 
-__device__ __forceinline__ float exp2_of(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 constexpr float kNone = -INFINITY;
 constexpr float kRise = 8.f;
 constexpr float kFar = -1e30f;  // in the place of log2(0), whose product with 0 it leaves 0
@@ -59,7 +53,7 @@ struct Sums {
   // Everything so far to the reference `to` >= m.
   __device__ __forceinline__ void move(float to, float c) {
     if (m != kNone) {
-      const float t = fmaxf((m - to) * c, kFar), f = exp2_of((m - to) * c);
+      const float t = fmaxf((m - to) * c, kFar), f = fast_exp2((m - to) * c);
       w = f * (w + t * s);
       s *= f;
     }
@@ -310,7 +304,7 @@ __global__ void __launch_bounds__(kProbThreads, TOP ? 8 : 12) prob_kernel(ProbAr
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const float a = (v[e] - m) * c, p = exp2_of(a);
+      const float a = (v[e] - m) * c, p = fast_exp2(a);
       s2[e & 1] += p;
       w2[e & 1] = fmaf(p, fmaxf(a, kFar), w2[e & 1]);
     }
@@ -512,7 +506,7 @@ __global__ void __launch_bounds__(kProbThreads, 12) prob_grad_kernel(ProbArgs A)
     for (int e = 0; e < E; ++e) {
       const float q = fmaf(d[e] - m, c, -l2);
       // an entry without probability has log2 p = -inf: 0 all the same
-      d[e] = exp2_of(q) * fmaf(es, fmaxf(q, -300.f), gs);
+      d[e] = fast_exp2(q) * fmaf(es, fmaxf(q, -300.f), gs);
     }
     const unsigned here = (unsigned)(at - row.first(k));
     if (here < (unsigned)E) {

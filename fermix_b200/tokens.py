@@ -7,7 +7,7 @@ way into the network, its position-wise maps, and the way out to probabilities o
   the likeliest alternatives.
 
 float32 and bfloat16, with the conventions of :mod:`fermix_b200.block`: sums are float32, every
-result is rounded once, gradients go through torch autograd and are summed in a fixed order (two
+result is rounded once (what else is rounded stands at the operator), gradients go through torch autograd and are summed in a fixed order (two
 runs give the same bits), tangents (forward mode) and ``torch.func`` transforms are refused, and there
 is no CPU path and no fallback. None of this has a counterpart in the reference, whose caller
 brings the network.
@@ -49,7 +49,7 @@ def token_embedding(tokens, weight, *, scale=1.0, padding=None):
     ``tokens`` (...) is an integer tensor, ``weight`` (rows, width), float32 or bfloat16. A token equal
     to ``padding`` (any whole number, a row of the table or not) gives zeros and has no gradient; any
     other token outside [0, rows) gives NaN and has no gradient. Differentiable in ``weight``: the rows of
-    the output's gradient are summed in float32 in the tokens' order and rounded once."""
+    the output's gradient are summed in float32 in a fixed order (by groups of a token's places) and rounded once."""
     if _transformed():
         _refuse_transforms(tokens=tokens, weight=weight)
     weight = _tensor(weight, "weight")
@@ -69,10 +69,11 @@ def fused_linear(x, weight, bias=None, *, activation=None, residual=None):
     ``x`` is (..., inner), ``weight`` (outer, inner), ``bias`` (outer,), ``residual`` (..., outer), float32 or
     bfloat16, all of one type; rows may be strided (a slice of a wider projection is read in place).
     ``activation`` is None, "relu", "silu", "gelu" (with the error function), "gelu_tanh" or "tanh". The
-    sum, the activation and the residual are float32, rounded once. float32 has the accuracy of float32
-    products; an infinity or a NaN gives NaN in the entries it reaches. Differentiable in all four; with an
-    activation the derivative at each entry is kept for the backward pass (float32, or half beside
-    bfloat16), under ``torch.no_grad()`` nothing is."""
+    sum, the activation and the residual are float32, rounded once. float32 products have float32's accuracy,
+    activations and their derivatives are good to 2^-20 of 1 + |h|; an infinity or a NaN gives NaN in the float32
+    entries it reaches. Differentiable in all four; with an activation the derivative at each entry is kept for the
+    backward pass (float32, or half beside bfloat16), under ``torch.no_grad()`` nothing is. In bfloat16 its product with
+    the output's gradient is rounded to bfloat16 before the products of the gradients in ``x`` and ``weight``."""
     if _transformed():
         _refuse_transforms(x=x, weight=weight, bias=bias, residual=residual)
     x = _tensor(x, "x")
