@@ -51,7 +51,8 @@ int by_piece(int dtype, int entries, F f) {
 }
 
 // Few tokens and rows are listed row by row in one launch: rows x count comparisons.
-// Otherwise the tokens are sorted.
+// Otherwise the tokens are sorted. (The rule does not see how few blocks a small table starts: trained, 4096 tokens over 64 x
+// 64 float32 16 us, over 2 x 4096 3.0 ms; 16384 tokens, which are sorted, over 2 x 4096 184 us.)
 bool scans(const fx_embed_args* a) {
   return a->count <= kScanTokens && a->rows <= 16384 && a->rows * a->count <= (int64_t{1} << 22);
 }

@@ -158,12 +158,12 @@ struct LinPlan {
 };
 
 // Blocks of 16 outputs and eight warps while there is at most one an SM, of 32 and four warps above (float32; us: 1000 x
-// 4096 x 32 23 and 41, 100000 x 264 x 32 150 and 80).
+// 4096 x 32 23 and 41, 100000 x 264 x 32 150 and 80). Between, blocks of 32 leave SMs idle: 4096 x 8192 x 32 76.
 bool few_blocks(int64_t narrow, int64_t wide, int sms) { return ceil_div(wide, 16) * ceil_div(narrow, 32) <= sms; }
 
 // Whether the rows' kernel (linear_rows.cuh), which needs no layout, takes the call. In bfloat16 few rows, which are bound
 // by the weights' bytes; measured, us, against the tiles of the tensor cores at 8192 -> 4096: 32 rows 24 and 27, 64 rows
-// 52 and 26.
+// 52 and 26. (Rows off the 16-byte boundaries come without the ring of copies: 32 x 8191 -> 4096 76 us.)
 // In float32 the tiles' launches cost about 20 us, and their layout reads and writes an operand four times as much; the
 // rows' kernel costs the products of its slower instructions. Both are estimated, us, from times between 100 and 100000
 // of `wide`, 4 and 512 of `narrow` and 32 and 4096 of `inner`. Measured, us, rows and tiles, wide x inner x narrow: 300 x
